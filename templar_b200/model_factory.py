@@ -174,10 +174,10 @@ def create_meta_model(hparams: SimpleNamespace, role: Literal["miner", "validato
         model = LlamaModel(args)
     model.parallel_dims, model.job_config = pdims, job
     # torchtitan.activation_checkpoint of the hparams: {"mode": "none" | "full" | "selective", "option": "op" | "<N>"}
-    # (reference src/tplr/model_factory.py:195-204)
+    # (reference src/tplr/model_factory.py:195-204), and "int8" of this package: saved activations in 8 bits
     mode = str(job.activation_checkpoint_mode or "none").lower()
-    if mode not in ("none", "full", "selective"):
-        raise ValueError(f"activation_checkpoint.mode must be none, full or selective, got {mode!r}")
+    if mode not in ("none", "full", "selective", "int8"):
+        raise ValueError(f"activation_checkpoint.mode must be none, full, selective or int8, got {mode!r}")
     model.activation_checkpointing = mode
     model.ac_option = str(job.selective_ac_option)
     return model

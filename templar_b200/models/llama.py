@@ -22,6 +22,7 @@ import torch
 import torch.nn as nn
 
 from ..ops import functional as OF
+from ..ops import quantized as OQ
 
 
 @dataclass
@@ -164,8 +165,17 @@ class TransformerBlock(nn.Module):
 
         With ``recompute_ops`` (per-op selective activation checkpointing) the normalised activations and the
         SwiGLU output are not stored: each is recomputed in the backward pass for the weight gradient of the
-        GEMM that consumed it, while every GEMM and attention output is kept."""
+        GEMM that consumed it, while every GEMM and attention output is kept.  With ``saved8`` the normalised rows and
+        the packed gate / up projection are stored in 8 bits and the SwiGLU output is not stored (ops/quantized.py)."""
         att, ff = self.attention, self.feed_forward
+        if getattr(self, "saved8", False):
+            n1, n2 = self.attention_norm, self.ffn_norm
+            wqkv, mg_qkv = att.packed or (torch.cat((att.wq.weight, att.wk.weight, att.wv.weight)), None)
+            w13, mg13 = ff.packed or (torch.cat((ff.w1.weight, ff.w3.weight)), None)
+            res, y, rows = OQ.add_rmsnorm_saved8(res, delta, n1.weight, n1.eps)
+            a = OQ.attention_block_saved8(y, wqkv, att.wo.weight, cos, sin, att.n_heads, att.n_kv, att.hd, rows, n1.weight, mg_qkv)
+            res, y, rows = OQ.add_rmsnorm_saved8(res, a, n2.weight, n2.eps)
+            return res, OQ.feed_forward_saved8(y, w13, ff.w2.weight, rows, n2.weight, mg13)
         if getattr(self, "recompute_ops", False) and att.packed is not None and ff.packed is not None:
             nw, eps = self.attention_norm, self.attention_norm.eps
             if delta is None:
@@ -210,7 +220,8 @@ class LlamaModel(nn.Module):
         self._rope_cache: dict = {}
         # False / True (every block recomputed), or the reference's modes (hparams torchtitan.activation_checkpoint):
         # "none", "full", "selective" with ``ac_option`` = "op" (per-op policy: GEMM and attention outputs kept,
-        # norms and activations recomputed) or an integer N (every N-th block recomputed whole)
+        # norms and activations recomputed) or an integer N (every N-th block recomputed whole); "int8": nothing is
+        # recomputed but the SwiGLU output, what the norms and the feed-forward part keep is held in 8 bits
         self.activation_checkpointing = False
         self.ac_option = "op"
 
@@ -281,6 +292,7 @@ class LlamaModel(nn.Module):
         every = int(self.ac_option) if mode == "selective" and str(self.ac_option).isdigit() else (1 if mode == "full" else 0)
         for count, (key, layer) in enumerate(self.layers.items(), start=1):
             layer.recompute_ops = per_op and torch.is_grad_enabled()
+            layer.saved8 = mode == "int8" and torch.is_grad_enabled()
             fn = layer.forward_fused
             if pg is not None:
                 fn = self._gated_block(pg, f"layers.{key}", layer)

@@ -1,0 +1,369 @@
+// Rows in 8 bits (sm_100a): what an 8-bit product takes as its operand and what a backward pass reads again.
+//
+// A group of a row (the whole row for products, 64 columns for saved activations) with the largest magnitude a is held as
+//   q = rint(x * (127 / a)) in [-127, 127],   scale = a / 127,   value = q * scale
+// with IEEE division, in fp32.  A group below 2^-100 (127 / a would overflow not far below) is zero with scale zero; a group with a
+// member that is not finite has scale NaN and q zero, so that all that is made of it is NaN and nothing is hidden.  Magnitudes are
+// compared by their bits, where NaN is above infinity and both above every number.
+#include "common.cuh"
+
+namespace {
+typedef __nv_bfloat16 bf16;
+typedef long long ll;
+
+struct Codes { float inv, scale; };
+__device__ __forceinline__ Codes codes_of(uint32_t top) {
+  const float a = __uint_as_float(top);
+  if (top >= 0x7f800000u) return {0.f, __uint_as_float(0x7fc00000u)};
+  if (a < 0x1p-100f) return {0.f, 0.f};
+  return {127.f / a, a / 127.f};
+}
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// x * inv is at most 127 (1 + 2^-23): it never rounds to 128; what is not finite converts to 0
+__device__ __forceinline__ int code(float x, float inv) { return __float2int_rn(x * inv); }
+
+// ------------------------------------------------------------------------------------------ rows -> 8 bits
+enum Mode {
+  ROWS = 0,          // a: bf16 rows of D, one scale a row
+  GROUPS = 1,        // a: bf16 rows of D, a scale for every 64 columns
+  NORM_ROWS = 2,     // h = a + b, rows h * rstd * w, one scale a row
+  NORM_SAVED = 3,    // h = a + b, y = h * rstd * w in bf16, rows h * rstd with a scale for every 64 columns, rstd
+  SWIGLU_ROWS = 4,   // a: bf16 [gate | up] rows of 2 D, rows silu(gate) * up, one scale a row
+};
+constexpr int GROUP = 64;
+
+struct RowsArgs {
+  const bf16 *a, *b, *w;
+  ll lda, ldb;
+  bf16 *h, *y;
+  int8_t* q;
+  ll ldq;            // bytes; columns from D on are written as zeros
+  float* scale;
+  ll scale_row, scale_group;
+  float* rstd;
+  ll T;
+  int D;
+  float eps;
+};
+
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + __expf(-g)) * u; }
+
+// One CTA a row, element by element: every width and alignment.
+template <int MODE>
+__global__ void __launch_bounds__(256) rows_q8_any_kernel(const RowsArgs p) {
+  __shared__ float red[32];
+  __shared__ uint32_t s_top[8];
+  grid_wait();
+  grid_release();
+  const ll row = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = p.D;
+  constexpr bool NORM = MODE == NORM_ROWS || MODE == NORM_SAVED;
+  const bf16 *a = p.a + row * p.lda, *b = p.b ? p.b + row * p.ldb : nullptr;
+  auto in = [&](int i) -> float {
+    if (MODE == SWIGLU_ROWS) return silu_mul(__bfloat162float(a[i]), __bfloat162float(a[D + i]));
+    if (!NORM || !b) return __bfloat162float(a[i]);
+    return __bfloat162float(__float2bfloat16(__bfloat162float(a[i]) + __bfloat162float(b[i])));   // as the residual stream stores it
+  };
+  float r = 1.f;
+  if (NORM) {
+    float ss = 0.f;
+    for (int i = threadIdx.x; i < D; i += 256) {
+      const float x = in(i);
+      if (p.h) p.h[row * D + i] = __float2bfloat16(x);
+      ss = fmaf(x, x, ss);
+    }
+    r = rsqrtf(block_sum(ss, red) / (float)D + p.eps);
+    if (MODE == NORM_SAVED && threadIdx.x == 0) p.rstd[row] = r;
+  }
+  int8_t* q = p.q + row * p.ldq;
+  auto value = [&](int i) -> float {
+    const float x = NORM ? in(i) * r : in(i);
+    return MODE == NORM_ROWS ? x * __bfloat162float(p.w[i]) : x;
+  };
+  if (MODE == GROUPS || MODE == NORM_SAVED) {
+    for (int g = warp; g * GROUP < D; g += 8) {
+      const int i0 = g * GROUP + lane, i1 = i0 + 32;
+      const float x0 = i0 < D ? value(i0) : 0.f, x1 = i1 < D ? value(i1) : 0.f;
+      const Codes c = codes_of(__reduce_max_sync(0xffffffffu, max(magnitude(x0), magnitude(x1))));
+      if (lane == 0) p.scale[row * p.scale_row + g * p.scale_group] = c.scale;
+      if (i0 < p.ldq) q[i0] = (int8_t)code(x0, c.inv);
+      if (i1 < p.ldq) q[i1] = (int8_t)code(x1, c.inv);
+      if (MODE == NORM_SAVED) {
+        if (i0 < D) p.y[row * D + i0] = __float2bfloat16(x0 * __bfloat162float(p.w[i0]));
+        if (i1 < D) p.y[row * D + i1] = __float2bfloat16(x1 * __bfloat162float(p.w[i1]));
+      }
+    }
+    return;
+  }
+  uint32_t top = 0;
+  for (int i = threadIdx.x; i < D; i += 256) top = max(top, magnitude(value(i)));
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) s_top[warp] = top;
+  __syncthreads();
+  for (int k = 0; k < 8; ++k) top = max(top, s_top[k]);
+  const Codes c = codes_of(top);
+  if (threadIdx.x == 0) p.scale[row * p.scale_row] = c.scale;
+  for (int i = threadIdx.x; i < p.ldq; i += 256) q[i] = i < D ? (int8_t)code(value(i), c.inv) : 0;
+}
+
+// ------------------------------------------------------------------------------------------ 8 bits -> rows
+// y = q * scale (* w of the column), rows of D; a scale for every `group` columns.
+__global__ void __launch_bounds__(256) dequantize_any_kernel(const int8_t* q, ll ldq, const float* scale, ll scale_row, ll scale_group, int group,
+                                                             const bf16* w, bf16* y, ll T, int D) {
+  grid_wait();
+  grid_release();
+  const ll total = T * D;
+  for (ll i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+    const ll row = i / D;
+    const int c = (int)(i - row * D);
+    float v = (float)q[row * ldq + c] * scale[row * scale_row + c / group * scale_group];
+    if (w) v *= __bfloat162float(w[c]);
+    y[i] = __float2bfloat16(v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ norm, backward from 8 bits
+// xn = q * scale; g = dy * w; dx = dres + rstd * (g - xn * mean(g * xn)); the CTA's sum of dy * xn goes to part[blockIdx.x].
+__global__ void __launch_bounds__(256) rmsnorm_saved8_bwd_any_kernel(const bf16* dy, const int8_t* q, ll ldq, const float* scale, ll scale_row,
+                                                                     ll scale_group, const float* rstd, const bf16* w, const bf16* dres,
+                                                                     bf16* dx, float* part, ll T, int D) {
+  __shared__ float red[32];
+  grid_wait();
+  grid_release();
+  float* mine = part + (ll)blockIdx.x * D;
+  for (int i = threadIdx.x; i < D; i += 256) mine[i] = 0.f;
+  for (ll row = blockIdx.x; row < T; row += gridDim.x) {
+    auto xn = [&](int i) { return (float)q[row * ldq + i] * scale[row * scale_row + i / GROUP * scale_group]; };
+    float dot = 0.f;
+    for (int i = threadIdx.x; i < D; i += 256) {
+      const float d = __bfloat162float(dy[row * D + i]), x = xn(i);
+      mine[i] += d * x;                                                  // this thread's own columns
+      dot = fmaf(d * __bfloat162float(w[i]), x, dot);
+    }
+    dot = block_sum(dot, red) / (float)D;
+    const float r = rstd[row];
+    for (int i = threadIdx.x; i < D; i += 256) {
+      float o = r * (__bfloat162float(dy[row * D + i]) * __bfloat162float(w[i]) - xn(i) * dot);
+      if (dres) o += __bfloat162float(dres[row * D + i]);
+      dx[row * D + i] = __float2bfloat16(o);
+    }
+    __syncthreads();
+  }
+}
+
+// Sum of the CTAs' parts in their order, the same on every run: added into an fp32 buffer or stored in bf16.
+__global__ void __launch_bounds__(256) sum_parts_kernel(const float* part, int n, int D, float* add, bf16* out) {
+  __shared__ float s[8][33];
+  grid_wait();
+  grid_release();
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float v = 0.f;
+  if (c < D)
+    for (int k = slice; k < n; k += 8) v += part[(ll)k * D + c];
+  s[slice][lane] = v;
+  __syncthreads();
+  if (slice == 0 && c < D) {
+    for (int k = 1; k < 8; ++k) v += s[k][lane];
+    if (add) add[c] += v;
+    else out[c] = __float2bfloat16(v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ SwiGLU around a saved projection
+// gu: fp32 [gate | up] rows of 2 F; act = silu(gate) * up in bf16; gate and up in 8 bits, a scale for every 64 columns of each
+// half.  One warp a group of both halves.
+__global__ void __launch_bounds__(256) swiglu_saved8_kernel(const float* gu, bf16* act, int8_t* q, ll ldq, float* scale, ll scale_row,
+                                                            ll scale_group, ll T, int F) {
+  grid_wait();
+  grid_release();
+  const int lane = threadIdx.x & 31, groups = (F + GROUP - 1) / GROUP;
+  for (ll at = blockIdx.x * 8LL + (threadIdx.x >> 5); at < T * groups; at += gridDim.x * 8LL) {
+    const ll row = at / groups;
+    const int g = (int)(at - row * groups);
+    float v[2][2];
+    for (int h = 0; h < 2; ++h) {
+      const int i0 = g * GROUP + lane, i1 = i0 + 32;
+      const float* src = gu + row * 2 * F + (ll)h * F;
+      v[h][0] = i0 < F ? src[i0] : 0.f;
+      v[h][1] = i1 < F ? src[i1] : 0.f;
+      const Codes c = codes_of(__reduce_max_sync(0xffffffffu, max(magnitude(v[h][0]), magnitude(v[h][1]))));
+      if (lane == 0) scale[row * scale_row + (h * groups + g) * scale_group] = c.scale;
+      if (i0 < F) q[row * ldq + (ll)h * F + i0] = (int8_t)code(v[h][0], c.inv);
+      if (i1 < F) q[row * ldq + (ll)h * F + i1] = (int8_t)code(v[h][1], c.inv);
+    }
+    for (int k = 0; k < 2; ++k) {
+      const int i = g * GROUP + lane + 32 * k;
+      if (i < F) act[row * F + i] = __float2bfloat16(silu_mul(v[0][k], v[1][k]));
+    }
+  }
+}
+
+// dact: fp32 [T, F]; the kept gate and up -> dgu = [dgate | dup] and the activation again, bf16.
+__global__ void __launch_bounds__(256) swiglu_saved8_bwd_kernel(const float* dact, const int8_t* q, ll ldq, const float* scale, ll scale_row,
+                                                                ll scale_group, bf16* dgu, bf16* act, ll T, int F) {
+  grid_wait();
+  grid_release();
+  const int groups = (F + GROUP - 1) / GROUP;
+  const ll total = T * F;
+  for (ll i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+    const ll row = i / F;
+    const int c = (int)(i - row * F);
+    const float* s = scale + row * scale_row;
+    const float g = (float)q[row * ldq + c] * s[c / GROUP * scale_group];
+    const float u = (float)q[row * ldq + F + c] * s[(groups + c / GROUP) * scale_group];
+    const float sg = 1.f / (1.f + __expf(-g)), sl = g * sg, d = dact[i];
+    dgu[row * 2 * F + c] = __float2bfloat16(d * u * (sg + sl * (1.f - sg)));
+    dgu[row * 2 * F + F + c] = __float2bfloat16(d * sl);
+    act[i] = __float2bfloat16(sl * u);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ product
+// y[t, n] = sx[t] * sw[n] * sum_k x[t, k] w[n, k]; 64 x 64 tiles, 64 bytes of k at a time, four products an instruction.
+template <class Out>
+__global__ void __launch_bounds__(256) gemm_q8_dot_kernel(const int8_t* x, const int8_t* w, const float* sx, const float* sw, Out* y, int T,
+                                                          int N, int K, ll ldx, ll ldw, ll ldy) {
+  __shared__ int s_x[64][17], s_w[64][17];
+  grid_wait();
+  grid_release();
+  const int t0 = blockIdx.y * 64, n0 = blockIdx.x * 64, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  int acc[4][4] = {};
+  for (int k0 = 0; k0 < K; k0 += 64) {
+    for (int i = threadIdx.x; i < 1024; i += 256) {                      // 64 rows of 16 words
+      const int r = i >> 4, k = k0 + (i & 15) * 4;
+      s_x[r][i & 15] = t0 + r < T && k < K ? *reinterpret_cast<const int*>(x + (ll)(t0 + r) * ldx + k) : 0;
+      s_w[r][i & 15] = n0 + r < N && k < K ? *reinterpret_cast<const int*>(w + (ll)(n0 + r) * ldw + k) : 0;
+    }
+    __syncthreads();
+    for (int k = 0; k < 16; ++k) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(s_x[ty + 16 * i][k], s_w[tx + 16 * j][k], acc[i][j]);
+    }
+    __syncthreads();
+  }
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 4; ++j) {
+      const int t = t0 + ty + 16 * i, n = n0 + tx + 16 * j;
+      if (t < T && n < N) y[(ll)t * ldy + n] = (Out)((float)acc[i][j] * (sx[t] * sw[n]));
+    }
+}
+
+template <int MODE>
+int rows_q8(const RowsArgs& p, void* stream) {
+  if (p.T <= 0) return 0;
+  if (p.T > 0x7fffffffLL || p.D <= 0 || p.ldq < p.D) return (int)cudaErrorInvalidValue;
+  return (int)launch_pdl(rows_q8_any_kernel<MODE>, (unsigned)p.T, 256, 0, (cudaStream_t)stream, p);
+}
+unsigned waves(ll ctas, int resident) {
+  const ll most = (ll)tplr_sm_count() * resident;
+  return (unsigned)(ctas < most ? ctas : most);
+}
+}  // namespace
+
+// bf16 rows (T of D, row stride ldx) in 8 bits: one scale a row (group 0) or for every 64 columns (group 64).  q: rows of ldq >= D bytes,
+// zeros behind column D; scale[row * scale_row + group * scale_group].
+TPLR_API int tplr_quantize_rows(const void* x, ll ldx, void* q, ll ldq, float* scale, ll scale_row, ll scale_group, ll T, int D, int group,
+                                void* stream) {
+  TPLR_ENTER();
+  RowsArgs p = {};
+  p.a = (const bf16*)x; p.lda = ldx; p.q = (int8_t*)q; p.ldq = ldq; p.scale = scale; p.scale_row = scale_row; p.scale_group = scale_group;
+  p.T = T; p.D = D;
+  if (group != 0 && group != GROUP) return (int)cudaErrorInvalidValue;
+  return group ? rows_q8<GROUPS>(p, stream) : rows_q8<ROWS>(p, stream);
+}
+
+// h = res + delta (delta null: h = res, h_out unused) and the rows h * rstd * w in 8 bits, one scale a row.  Dense rows of D.
+TPLR_API int tplr_add_rmsnorm_q8(const void* res, const void* delta, const void* w, void* h_out, void* q, ll ldq, float* scale, ll T, int D,
+                                 float eps, void* stream) {
+  TPLR_ENTER();
+  RowsArgs p = {};
+  p.a = (const bf16*)res; p.b = (const bf16*)delta; p.w = (const bf16*)w; p.lda = p.ldb = D; p.h = delta ? (bf16*)h_out : nullptr;
+  p.q = (int8_t*)q; p.ldq = ldq; p.scale = scale; p.scale_row = 1; p.T = T; p.D = D; p.eps = eps;
+  return rows_q8<NORM_ROWS>(p, stream);
+}
+
+// The training step's form: y = h * rstd * w in bf16, and for the backward pass rstd [T] and the rows h * rstd in 8 bits by 64 columns.
+TPLR_API int tplr_add_rmsnorm_saved8(const void* res, const void* delta, const void* w, void* h_out, void* y, void* q, ll ldq, float* scale,
+                                     ll scale_row, ll scale_group, float* rstd, ll T, int D, float eps, void* stream) {
+  TPLR_ENTER();
+  RowsArgs p = {};
+  p.a = (const bf16*)res; p.b = (const bf16*)delta; p.w = (const bf16*)w; p.lda = p.ldb = D; p.h = delta ? (bf16*)h_out : nullptr;
+  p.y = (bf16*)y; p.q = (int8_t*)q; p.ldq = ldq; p.scale = scale; p.scale_row = scale_row; p.scale_group = scale_group; p.rstd = rstd;
+  p.T = T; p.D = D; p.eps = eps;
+  return rows_q8<NORM_SAVED>(p, stream);
+}
+
+// silu(gate) * up of bf16 [gate | up] rows of 2 F (row stride ldgu) in 8 bits, one scale a row.
+TPLR_API int tplr_swiglu_q8(const void* gu, ll ldgu, void* q, ll ldq, float* scale, ll T, int F, void* stream) {
+  TPLR_ENTER();
+  RowsArgs p = {};
+  p.a = (const bf16*)gu; p.lda = ldgu; p.q = (int8_t*)q; p.ldq = ldq; p.scale = scale; p.scale_row = 1; p.T = T; p.D = F;
+  return rows_q8<SWIGLU_ROWS>(p, stream);
+}
+
+// y[T, D] (dense bf16) = q * scale, times w[column] where w is given; a scale for every `group` columns.
+TPLR_API int tplr_dequantize_rows(const void* q, ll ldq, const float* scale, ll scale_row, ll scale_group, int group, const void* w, void* y,
+                                  ll T, int D, void* stream) {
+  TPLR_ENTER();
+  if (T <= 0) return 0;
+  if (D <= 0 || group <= 0) return (int)cudaErrorInvalidValue;
+  return (int)launch_pdl(dequantize_any_kernel, waves((T * D + 255) / 256, 16), 256, 0, (cudaStream_t)stream, (const int8_t*)q, ldq, scale,
+                         scale_row, scale_group, group, (const bf16*)w, (bf16*)y, T, D);
+}
+
+// CTAs of the norm's backward: rows of the fp32 workspace that tplr_rmsnorm_saved8_bwd takes (each of D elements).
+TPLR_API int tplr_rmsnorm_saved8_parts(ll T, int D) { return (int)waves(T, 4); }
+
+// dx of the norm from its rows in 8 bits (dres null: 0), and its weight's gradient: added into dw_add (fp32) or stored in dw_out (bf16); both
+// null: not formed.
+TPLR_API int tplr_rmsnorm_saved8_bwd(const void* dy, const void* q, ll ldq, const float* scale, ll scale_row, ll scale_group,
+                                     const float* rstd, const void* w, const void* dres, void* dx, float* part, float* dw_add, void* dw_out,
+                                     ll T, int D, void* stream) {
+  TPLR_ENTER();
+  if (T <= 0) return 0;
+  if (D <= 0) return (int)cudaErrorInvalidValue;
+  const int n = tplr_rmsnorm_saved8_parts(T, D);
+  if (const cudaError_t e = launch_pdl(rmsnorm_saved8_bwd_any_kernel, n, 256, 0, (cudaStream_t)stream, (const bf16*)dy, (const int8_t*)q, ldq,
+                                       scale, scale_row, scale_group, rstd, (const bf16*)w, (const bf16*)dres, (bf16*)dx, part, T, D))
+    return (int)e;
+  if (!dw_add && !dw_out) return 0;
+  return (int)launch_pdl(sum_parts_kernel, (D + 31) / 32, 256, 0, (cudaStream_t)stream, part, n, D, dw_add, (bf16*)dw_out);
+}
+
+// The activation of a dense fp32 [gate | up] projection, and the projection in 8 bits (rows of ldq >= 2 F bytes) by 64 columns of each half.
+TPLR_API int tplr_swiglu_saved8(const float* gu, void* act, void* q, ll ldq, float* scale, ll scale_row, ll scale_group, ll T, int F,
+                                void* stream) {
+  TPLR_ENTER();
+  if (T <= 0) return 0;
+  if (F <= 0 || ldq < 2LL * F) return (int)cudaErrorInvalidValue;
+  const ll groups = T * ((F + GROUP - 1) / GROUP);
+  return (int)launch_pdl(swiglu_saved8_kernel, waves((groups + 7) / 8, 16), 256, 0, (cudaStream_t)stream, gu, (bf16*)act, (int8_t*)q, ldq,
+                         scale, scale_row, scale_group, T, F);
+}
+
+// Its backward: dact dense fp32 [T, F] -> dgu = [dgate | dup] (dense bf16) and the activation again.
+TPLR_API int tplr_swiglu_saved8_bwd(const float* dact, const void* q, ll ldq, const float* scale, ll scale_row, ll scale_group, void* dgu,
+                                    void* act, ll T, int F, void* stream) {
+  TPLR_ENTER();
+  if (T <= 0) return 0;
+  if (F <= 0) return (int)cudaErrorInvalidValue;
+  return (int)launch_pdl(swiglu_saved8_bwd_kernel, waves((T * F + 255) / 256, 16), 256, 0, (cudaStream_t)stream, dact, (const int8_t*)q, ldq,
+                         scale, scale_row, scale_group, (bf16*)dgu, (bf16*)act, T, F);
+}
+
+// y[T, N] = sx[t] * sw[n] * (x w^T) for int8 rows x [T, K] and w [N, K] (row strides multiples of 16 bytes, zeros or any codes behind
+// column K of x multiplied by zeros of w: w's rows are zero from K to its stride), y bf16 or fp32 with row stride ldy.
+TPLR_API int tplr_gemm_q8(const void* x, const void* w, const float* sx, const float* sw, void* y, int T, int N, int K, ll ldx, ll ldw,
+                          ll ldy, int out_fp32, unsigned int* status, void* stream) {
+  TPLR_ENTER();
+  if (T <= 0 || N <= 0) return 0;
+  if (K <= 0 || K > 131072 || (ldx | ldw) % 16 || (((uintptr_t)x | (uintptr_t)w) & 15)) return (int)cudaErrorInvalidValue;
+  const dim3 grid((N + 63) / 64, (T + 63) / 64);
+  if (out_fp32)
+    return (int)launch_pdl(gemm_q8_dot_kernel<float>, grid, 256, 0, (cudaStream_t)stream, (const int8_t*)x, (const int8_t*)w, sx, sw, (float*)y, T,
+                           N, K, ldx, ldw, ldy);
+  return (int)launch_pdl(gemm_q8_dot_kernel<bf16>, grid, 256, 0, (cudaStream_t)stream, (const int8_t*)x, (const int8_t*)w, sx, sw, (bf16*)y, T, N, K,
+                         ldx, ldw, ldy);
+}

@@ -976,6 +976,16 @@ def _rope_tables_ok(cos, sin, S: int, hd: int) -> bool:
                and t.shape[1] == hd // 2 and t.data_ptr() % 16 == 0 for t in (cos, sin))
 
 
+def _attention_block_fused(x, wqkv, wo, cos, sin, n_heads: int, n_kv: int, hd: int) -> bool:
+    """Whether the whole block runs as one node on the own kernels."""
+    B, S, K = x.shape
+    return (FUSED_PROJECTIONS and _ATTN_BACKEND == "tcgen05" and _GEMM_BACKEND == "tcgen05_2sm" and _native_ok(x, wqkv, wo)
+            and x.dtype == torch.bfloat16 and _own_heads(wqkv.shape[0], n_heads, n_kv, hd) and x.is_contiguous()
+            and wqkv.stride(1) == 1 and wo.stride(1) == 1 and wqkv.stride(0) % 8 == 0 and wo.stride(0) % 8 == 0 and K % 8 == 0
+            and wqkv.shape[1] == K and wo.shape[0] % 8 == 0 and wo.shape[1] == n_heads * hd and _aligned(x, wqkv, wo)
+            and _rope_tables_ok(cos, sin, S, hd) and _own_attention_faster(B, S, n_heads, n_kv, hd, torch.is_grad_enabled(), True))
+
+
 def attention_block(x, wqkv, wo, cos, sin, n_heads: int, n_kv: int, hd: int, main_grad_qkv=None, main_grad_wo=None):
     """Causal attention block without its norm and residual: ``attention(rope(x @ wqkv.T)) @ wo.T`` for the packed
     ``wqkv = [wq; wk; wv]``.  One autograd node on the own kernels, three elsewhere."""
@@ -983,12 +993,7 @@ def attention_block(x, wqkv, wo, cos, sin, n_heads: int, n_kv: int, hd: int, mai
         main_grad_qkv = getattr(wqkv, "main_grad", None)
     if main_grad_wo is None:
         main_grad_wo = getattr(wo, "main_grad", None)
-    B, S, K = x.shape
-    if (FUSED_PROJECTIONS and _ATTN_BACKEND == "tcgen05" and _GEMM_BACKEND == "tcgen05_2sm" and _native_ok(x, wqkv, wo)
-            and x.dtype == torch.bfloat16 and _own_heads(wqkv.shape[0], n_heads, n_kv, hd) and x.is_contiguous()
-            and wqkv.stride(1) == 1 and wo.stride(1) == 1 and wqkv.stride(0) % 8 == 0 and wo.stride(0) % 8 == 0 and K % 8 == 0
-            and wqkv.shape[1] == K and wo.shape[0] % 8 == 0 and wo.shape[1] == n_heads * hd and _aligned(x, wqkv, wo)
-            and _rope_tables_ok(cos, sin, S, hd) and _own_attention_faster(B, S, n_heads, n_kv, hd, torch.is_grad_enabled(), True)):
+    if _attention_block_fused(x, wqkv, wo, cos, sin, n_heads, n_kv, hd):
         if _buffers_ok((main_grad_qkv, wqkv), (main_grad_wo, wo)) and (host := native.host()):
             return host.attention_block(x, wqkv, wo, main_grad_qkv, main_grad_wo, cos, sin, n_heads, n_kv, hd,
                                         status_word(x.device))

@@ -108,6 +108,16 @@ def _declare(L: ctypes.CDLL) -> None:
         "tplr_add_rmsnorm_fwd": [vp, vp, vp, vp, vp, vp, ll, i, f, vp],
         "tplr_add_rmsnorm_bwd": [vp, vp, vp, vp, vp, vp, vp, ll, i, vp],
         "tplr_add_rmsnorm_bwd_v2": [vp, vp, vp, vp, vp, vp, vp, ll, i, vp, vp],
+        "tplr_quantize_rows": [vp, ll, vp, ll, vp, ll, ll, ll, i, i, vp],
+        "tplr_dequantize_rows": [vp, ll, vp, ll, ll, i, vp, vp, ll, i, vp],
+        "tplr_add_rmsnorm_q8": [vp, vp, vp, vp, vp, ll, vp, ll, i, f, vp],
+        "tplr_swiglu_q8": [vp, ll, vp, ll, vp, ll, i, vp],
+        "tplr_gemm_q8": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, i, vp, vp],
+        "tplr_add_rmsnorm_saved8": [vp, vp, vp, vp, vp, vp, ll, vp, ll, ll, vp, ll, i, f, vp],
+        "tplr_rmsnorm_saved8_parts": [ll, i],
+        "tplr_rmsnorm_saved8_bwd": [vp, vp, ll, vp, ll, ll, vp, vp, vp, vp, vp, vp, vp, ll, i, vp],
+        "tplr_swiglu_saved8": [vp, vp, vp, ll, vp, ll, ll, ll, i, vp],
+        "tplr_swiglu_saved8_bwd": [vp, vp, ll, vp, ll, ll, vp, vp, ll, i, vp],
         "tplr_rope": [vp, vp, vp, ll, i, i, i, ll, i, vp],
         "tplr_swiglu_fwd": [vp, vp, ll, i, vp],
         "tplr_swiglu_bwd": [vp, vp, vp, ll, i, vp],
