@@ -83,6 +83,9 @@ struct Gemm2Params {
   const float* rope_cos;
   const float* rope_sin;
   int rope_s, rope_cols, rope_dh;
+  // 8-bit operands (EPI 7 bf16, EPI 8 fp32 result): C[m, n] = acc * (q8_row[m] * q8_col[n]) of the int32 accumulator
+  const float* q8_row;
+  const float* q8_col;
   int world, rank;
   unsigned int epoch;
   // gather
@@ -135,6 +138,17 @@ __device__ __forceinline__ void umma_bf16_pair_lohi(uint32_t tmem_d, uint32_t a_
       "mov.b64 da, {%1, %2};\n\t"
       "mov.b64 db, {%3, %4};\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n\t}"
+      ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate) : "memory");
+}
+// 8-bit integers: K = 32 an instruction, the same 32 bytes of a row
+__device__ __forceinline__ void umma_i8_pair_lohi(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                                  uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 da, {%1, %2};\n\t"
+      "mov.b64 db, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %5, p;\n\t}"
       ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -632,13 +646,91 @@ __device__ __forceinline__ void epilogue_attn_dout(const Gemm2Params& p, uint32_
   }
 }
 
+// Epilogue of a product of 8-bit rows (EPI 7 stores bf16, EPI 8 fp32): the int32 accumulator times the scales of its row (one a
+// lane) and its column (the same for all lanes: 16-byte loads that the L1 answers).  Columns from N on are not stored; where C takes
+// no TMA store (a row stride that is not a multiple of 16 bytes) a warp writes its staged box row by row, 32 columns of one row at a
+// time, since a lane that stores its own row touches 32 lines an instruction.
+template <bool F32>
+__device__ __forceinline__ void epilogue_q8(const Gemm2Params& p, uint32_t tmem_acc, int quad, int lane, int m0, int n0,
+                                            uint32_t stage_base, uint32_t& n_boxes) {
+  constexpr int COLS = F32 ? 32 : 64;
+  const int row0 = m0 + quad * 32;
+  if (row0 >= p.M) return;                           // warp-uniform
+  const uint32_t lane_sel = (uint32_t)(quad * 32) << 16;
+  const float sr = p.q8_row[min(row0 + lane, p.M - 1)];
+#pragma unroll 1
+  for (int c = 0; c < p.tile_n / COLS; ++c) {
+    const int col0 = n0 + c * COLS;
+    if (col0 >= p.N) break;                          // warp-uniform
+    const uint32_t buf = box_begin(lane, stage_base, n_boxes);
+#pragma unroll
+    for (int hh = 0; hh < COLS / 32; ++hh) {
+      const int col = col0 + hh * 32;
+      uint32_t r[32];
+      float v[32];
+      tmem_ld32(tmem_acc + c * COLS + hh * 32 + lane_sel, r);
+      if (col + 32 <= p.N) {
+        const float4* sc = reinterpret_cast<const float4*>(p.q8_col + col);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float4 q = sc[e];
+          v[4 * e] = (float)(int)r[4 * e] * (sr * q.x); v[4 * e + 1] = (float)(int)r[4 * e + 1] * (sr * q.y);
+          v[4 * e + 2] = (float)(int)r[4 * e + 2] * (sr * q.z); v[4 * e + 3] = (float)(int)r[4 * e + 3] * (sr * q.w);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = col + e < p.N ? (float)(int)r[e] * (sr * p.q8_col[col + e]) : 0.f;
+      }
+      if (F32) {
+        const uint32_t rowaddr = buf + (uint32_t)lane * 128u, sw = (uint32_t)(lane & 7);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + (((uint32_t)j ^ sw) << 4)), "f"(v[4 * j]), "f"(v[4 * j + 1]),
+                       "f"(v[4 * j + 2]), "f"(v[4 * j + 3]) : "memory");
+      } else {
+        box_half(buf, lane, hh, v);
+      }
+    }
+    if (p.c_tma) {
+      box_store(&p.tmC, buf, lane, n_boxes, col0, row0);
+    } else {
+      __syncwarp();
+      const int rows = min(32, p.M - row0);
+#pragma unroll 1
+      for (int r = 0; r < rows; ++r) {
+        const uint32_t rowaddr = buf + (uint32_t)r * 128u, sw = (uint32_t)(r & 7);
+#pragma unroll
+        for (int hh = 0; hh < COLS / 32; ++hh) {
+          const int e = hh * 32 + lane;              // this lane's column of the box
+          if (col0 + e < p.N) {
+            if (F32) {
+              float o;
+              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(o) : "r"(rowaddr + ((((uint32_t)e >> 2) ^ sw) << 4) + (uint32_t)(e & 3) * 4u) : "memory");
+              reinterpret_cast<float*>(p.C)[(long long)(row0 + r) * p.ldc + col0 + e] = o;
+            } else {
+              uint16_t o;
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(o) : "r"(rowaddr + ((((uint32_t)e >> 3) ^ sw) << 4) + (uint32_t)(e & 7) * 2u) : "memory");
+              reinterpret_cast<uint16_t*>(p.C)[(long long)(row0 + r) * p.ldc + col0 + e] = o;
+            }
+          }
+        }
+      }
+      __syncwarp();                                  // the box is read out before its buffer is written again
+      ++n_boxes;
+    }
+  }
+}
+
 // EPI: 0 store bf16, 1 fp32 accumulate (C += acc), 2 store fp32, 3 fused SwiGLU of a packed [w1; w3] projection,
 // 4 store bf16 with the rotary embedding applied to the leading columns, 5 backward of the SwiGLU on the data gradient
-// of the down projection, 6 data gradient of the attention output projection with the attention backward's delta term
+// of the down projection, 6 data gradient of the attention output projection with the attention backward's delta term,
+// 7 / 8 product of 8-bit rows stored as bf16 / fp32
 template <bool A_MN, bool B_MN, int EPI>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 gemm2_kernel(const __grid_constant__ Gemm2Params p) {
   constexpr int RING_BYTES = (EPI == 5 ? EPI5_STAGES : STAGES) * STAGE_BYTES;
+  constexpr bool I8 = EPI == 7 || EPI == 8;
+  constexpr int KB = I8 ? 2 * BK : BK;               // elements of a k block: 128 bytes of a row
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t bar_full[MAX_STAGES], bar_empty[MAX_STAGES], bar_tfull[2], bar_tempty[2];
@@ -655,7 +747,7 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
   const uint32_t b_stage = B_MN ? (uint32_t)((cta_n + 63) / 64) * (BK * 128) : (uint32_t)cta_n * 128u;
   const int n_stages = min(MAX_STAGES, (int)(RING_BYTES / (A_STAGE + b_stage)));
   const int tiles_m = (p.M + TILE_M - 1) / TILE_M, tiles_n = (p.N + tile_n - 1) / tile_n;
-  const int k_blocks_all = (p.K + BK - 1) / BK;
+  const int k_blocks_all = (p.K + KB - 1) / KB;
   const int k_per = (k_blocks_all + p.k_splits - 1) / p.k_splits;   // k blocks per work unit (static mode)
   const int num_tiles = p.tri ? tiles_m * (tiles_m + 1) / 2 : tiles_m * tiles_n;
   volatile int* abort_flag = &s_abort;
@@ -735,7 +827,7 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
               if (cr == 0) mbar_expect_tx(full0 + 8u * s, 2 * (A_STAGE + b_stage));
               const uint32_t fb = fullp0 + 8u * s;
               const uint32_t a_dst = sA + s * A_STAGE, b_dst = sB + s * b_stage;
-              const int k0 = kbr * BK;
+              const int k0 = kbr * KB;
               if (!A_MN) {
                 tma_load_2d_pair(a_dst, &p.tmA, fb, k0, m0);
               } else {
@@ -764,7 +856,8 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
       // ----------------------------- MMA issuer (even CTA only) ----------------------
       if (cr == 0) {
         const bool leader = elect_one();
-        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((A_MN ? 1u : 0u) << 15) |
+        // accumulator fp32 (1) or int32 (2); operands bf16, or signed bytes under the same number
+        const uint32_t idesc = ((I8 ? 2u : 1u) << 4) | (1u << 7) | (1u << 10) | ((A_MN ? 1u : 0u) << 15) |
                                ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(tile_n >> 3) << 17) | ((uint32_t)(TILE_M >> 4) << 24);
         uint32_t tile_i = 0;
         bool ok = true;
@@ -789,9 +882,11 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
             const uint32_t a_lo = dA0.lo + s * (A_STAGE >> 4), b_lo = dB0.lo + s * (b_stage >> 4);
             if (leader) {
 #pragma unroll
-              for (int kk = 0; kk < BK / UMMA_K; ++kk)
-                umma_bf16_pair_lohi(d_tmem, a_lo + kk * A_KSTEP, dA0.hi, b_lo + kk * B_KSTEP, dB0.hi, idesc,
-                                    (kb > 0 || kk > 0) ? 1u : 0u);
+              for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+                if (I8) umma_i8_pair_lohi(d_tmem, a_lo + kk * A_KSTEP, dA0.hi, b_lo + kk * B_KSTEP, dB0.hi, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+                else    umma_bf16_pair_lohi(d_tmem, a_lo + kk * A_KSTEP, dA0.hi, b_lo + kk * B_KSTEP, dB0.hi, idesc,
+                                            (kb > 0 || kk > 0) ? 1u : 0u);
+              }
               umma_commit_pair(empty0 + 8u * s);
             }
             if (++s == (uint32_t)n_stages) { s = 0; ph ^= 1u; }
@@ -826,6 +921,7 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
           epilogue_rope<128>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
         else if (EPI == 4 && p.rope_dh == 64 && p.rope_cols % 64 == 0)
           epilogue_rope<64>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
+        else if (I8)       epilogue_q8<EPI == 8>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
         else if (p.c_tma)  epilogue_tma<EPI>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes, w.t % p.k_splits);
         else               epilogue_direct<EPI>(p, tmem_acc, quad, lane, m0, n0);
         tcgen05_fence_before();
@@ -924,7 +1020,7 @@ int launch2(Gemm2Params& p, int n_comm_pairs, int max_pairs, cudaStream_t st) {
   attr[1] = pdl_attr(p.world == 1);
   cfg.attrs = attr; cfg.numAttrs = 2;
   // all CTAs must be resident at once: compute CTAs wait for comm CTAs of the same launch
-  static int max_clusters[2][2][7] = {};
+  static int max_clusters[2][2][9] = {};
   int& mc = max_clusters[A_MN][B_MN][EPI];
   if (mc == 0) {
     cfg.gridDim = dim3(2 * (tplr_sm_count() / 2));
@@ -954,6 +1050,7 @@ int dispatch2(Gemm2Params& p, int a_mn, int b_mn, int epi, int n_comm_pairs, int
   TPLR_GEMM2_CASE(1, 1, 0) TPLR_GEMM2_CASE(1, 1, 1) TPLR_GEMM2_CASE(1, 1, 2)
   TPLR_GEMM2_CASE(1, 0, 0) TPLR_GEMM2_CASE(1, 0, 1) TPLR_GEMM2_CASE(1, 0, 2)
   TPLR_GEMM2_CASE(0, 0, 3) TPLR_GEMM2_CASE(0, 0, 4) TPLR_GEMM2_CASE(0, 1, 5) TPLR_GEMM2_CASE(0, 1, 6)
+  TPLR_GEMM2_CASE(0, 0, 7) TPLR_GEMM2_CASE(0, 0, 8)
 #undef TPLR_GEMM2_CASE
   return -104;
 }
@@ -1098,18 +1195,22 @@ __global__ void __launch_bounds__(256) round_rows_kernel(const float* __restrict
   }
 }
 
-// Fills the operand maps and the plain fields; returns 0 or a negative argument error.
-int fill_common(Gemm2Params& p, const void* A, const void* B, void* C, int M, int N, int K, long long lda,
-                long long ldb, long long ldc, int a_mn, int b_mn, int epi, unsigned int* status, int tile_n = TILE_N) {
-  if ((lda % 8) || (ldb % 8) || ((uintptr_t)A & 15) || ((uintptr_t)B & 15)) return -101;
-  if (!(a_mn ? make_map(&p.tmA, A, M, K, lda, 64, BK) : make_map(&p.tmA, A, K, M, lda, BK, CTA_M))) return -102;
-  if (!(b_mn ? make_map(&p.tmB, B, N, K, ldb, 64, BK) : make_map(&p.tmB, B, K, N, ldb, BK, tile_n / 2))) return -103;
+// Everything that is neither a map nor of one epilogue: sizes, tile order, one rank, K whole.
+void plain_fields(Gemm2Params& p, void* C, int M, int N, int K, long long ldc, unsigned int* status, int tile_n) {
   p.tile_n = tile_n;
   p.C = C; p.ldc = ldc; p.M = M; p.N = N; p.K = K; p.status = status;
   static const int group_m = [] { const char* e = getenv("TPLR_GEMM_GROUP_M"); const int v = e ? atoi(e) : 0; return v > 0 ? v : 8; }();
   p.world = 1; p.rank = 0; p.epoch = 0; p.group_m = group_m; p.m_rot = 0; p.n_rot = 0; p.m_inter = 1; p.k_splits = 1;
   p.tri = 0;
   p.ag_operand = 0; p.rs_on = 0;
+}
+// Fills the operand maps and the plain fields; returns 0 or a negative argument error.
+int fill_common(Gemm2Params& p, const void* A, const void* B, void* C, int M, int N, int K, long long lda,
+                long long ldb, long long ldc, int a_mn, int b_mn, int epi, unsigned int* status, int tile_n = TILE_N) {
+  if ((lda % 8) || (ldb % 8) || ((uintptr_t)A & 15) || ((uintptr_t)B & 15)) return -101;
+  if (!(a_mn ? make_map(&p.tmA, A, M, K, lda, 64, BK) : make_map(&p.tmA, A, K, M, lda, BK, CTA_M))) return -102;
+  if (!(b_mn ? make_map(&p.tmB, B, N, K, ldb, 64, BK) : make_map(&p.tmB, B, K, N, ldb, BK, tile_n / 2))) return -103;
+  plain_fields(p, C, M, N, K, ldc, status, tile_n);
   const bool f32 = epi != 0;
   p.c_tma = !((uintptr_t)C & 15) && (ldc * (f32 ? 4 : 2)) % 16 == 0;
   if (p.c_tma && C && !make_map(&p.tmC, C, N, M, ldc, f32 ? 32 : 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, f32)) return -110;
@@ -1281,6 +1382,25 @@ TPLR_API int tplr_gemm2_rope(const void* X, const void* W, void* QKV, int M, int
   if (!p.c_tma) return -111;
   p.rope_cos = cosb; p.rope_sin = sinb; p.rope_s = S; p.rope_cols = rope_cols; p.rope_dh = head_dim;
   return dispatch2(p, 0, 0, 4, 0, 0, (cudaStream_t)stream);
+}
+
+// C[M, N] = sx[m] * sw[n] * (X W^T) for 8-bit rows X [M, K] and W [N, K] (bases and row strides multiples of 16 bytes), C bf16 or fp32
+// with any row stride and alignment.  The sums are exact for K up to 131072.  A k block holds 128 values where a bf16 one holds 64,
+// at the same bytes and the same 500 cycles, so the tile rule is asked for half the K.
+TPLR_API int tplr_gemm2_q8(const void* X, const void* W, const float* sx, const float* sw, void* C, int M, int N, int K, long long ldx,
+                           long long ldw, long long ldc, int out_fp32, unsigned int* status, void* stream) {
+  TPLR_ENTER();
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (K > 131072 || (ldx % 16) || (ldw % 16) || (((uintptr_t)X | (uintptr_t)W | (uintptr_t)sw) & 15)) return -101;
+  Gemm2Params p = {};
+  const int tile_n = pick_tile(M, N, (K + 1) / 2, false, false, out_fp32 ? 2 : 0);
+  if (!make_map_u8(&p.tmA, X, K, M, ldx, 2 * BK, CTA_M)) return -102;
+  if (!make_map_u8(&p.tmB, W, K, N, ldw, 2 * BK, tile_n / 2)) return -103;
+  plain_fields(p, C, M, N, K, ldc, status, tile_n);
+  p.q8_row = sx; p.q8_col = sw;
+  p.c_tma = !((uintptr_t)C & 15) && (ldc * (out_fp32 ? 4 : 2)) % 16 == 0;
+  if (p.c_tma && !make_map(&p.tmC, C, N, M, ldc, out_fp32 ? 32 : 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, out_fp32 != 0)) return -110;
+  return dispatch2(p, 0, 0, out_fp32 ? 8 : 7, 0, 0, (cudaStream_t)stream);
 }
 
 // All-gather fused into the GEMM.  Operand `ag_operand` (1 = A, 2 = B) is the local FULL buffer

@@ -218,36 +218,93 @@ __global__ void __launch_bounds__(256) swiglu_saved8_bwd_kernel(const float* dac
   }
 }
 
-// ------------------------------------------------------------------------------------------ product
-// y[t, n] = sx[t] * sw[n] * sum_k x[t, k] w[n, k]; 64 x 64 tiles, 64 bytes of k at a time, four products an instruction.
-template <class Out>
-__global__ void __launch_bounds__(256) gemm_q8_dot_kernel(const int8_t* x, const int8_t* w, const float* sx, const float* sw, Out* y, int T,
+// ------------------------------------------------------------------------------------------ product, few tokens
+// y[t, n] = sx[t] * sw[n] * sum_k x[t, k] w[n, k] where the weight's bytes are all that counts: they are read once, 16 bytes a lane,
+// straight into the operands of mma.m16n8k32 (a tile of 128 rows by tcgen05 would stage them in shared memory first and use 8 to 32 of
+// its 256 columns).  The sum over k may be taken in any order, so a lane's 16 bytes of a row are its words of two instructions
+// as they lie: word j of a weight row and word j of a token are multiplied wherever the instruction thinks they are.  A CTA's
+// eight warps take 64-byte pieces of 16 * RT rows in turn, 512 bytes of a row together, and add their sums in shared memory.
+__device__ __forceinline__ uint4 ld_once(const int8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <int NT, int RT, int UNROLL, class Out>
+__global__ void __launch_bounds__(256) gemm_q8_few_kernel(const int8_t* x, const int8_t* w, const float* sx, const float* sw, Out* y, int T,
                                                           int N, int K, ll ldx, ll ldw, ll ldy) {
-  __shared__ int s_x[64][17], s_w[64][17];
+  __shared__ int s_sum[8][NT * 8][16 * RT + 1];
   grid_wait();
   grid_release();
-  const int t0 = blockIdx.y * 64, n0 = blockIdx.x * 64, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < K; k0 += 64) {
-    for (int i = threadIdx.x; i < 1024; i += 256) {                      // 64 rows of 16 words
-      const int r = i >> 4, k = k0 + (i & 15) * 4;
-      s_x[r][i & 15] = t0 + r < T && k < K ? *reinterpret_cast<const int*>(x + (ll)(t0 + r) * ldx + k) : 0;
-      s_w[r][i & 15] = n0 + r < N && k < K ? *reinterpret_cast<const int*>(w + (ll)(n0 + r) * ldw + k) : 0;
-    }
-    __syncthreads();
-    for (int k = 0; k < 16; ++k) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n0 = blockIdx.x * 16 * RT, kp = (K + 15) / 16 * 16;
+  int acc[RT][NT][4] = {};
+  const int8_t* wr[RT][2];
+  bool wok[RT][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+  for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(s_x[ty + 16 * i][k], s_w[tx + 16 * j][k], acc[i][j]);
+    for (int h = 0; h < 2; ++h) {
+      const int n = n0 + r * 16 + h * 8 + (lane >> 2);
+      wok[r][h] = n < N;
+      wr[r][h] = w + (ll)(n < N ? n : N - 1) * ldw;
     }
-    __syncthreads();
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  for (int k0 = warp * 64; k0 < kp; k0 += 512 * UNROLL) {
+    uint4 a[UNROLL][RT][2], b[UNROLL][NT];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int k = k0 + u * 512 + (lane & 3) * 16;
+      const bool in = k < kp;
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) a[u][r][h] = in && wok[r][h] ? ld_once(wr[r][h] + k) : zero;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int tok = t * 8 + (lane >> 2);
+        b[u][t] = in && tok < T ? *reinterpret_cast<const uint4*>(x + tok * ldx + k) : zero;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          mma_s8(acc[r][t], a[u][r][0].x, a[u][r][1].x, a[u][r][0].y, a[u][r][1].y, b[u][t].x, b[u][t].y);
+          mma_s8(acc[r][t], a[u][r][0].z, a[u][r][1].z, a[u][r][0].w, a[u][r][1].w, b[u][t].z, b[u][t].w);
+        }
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int t = t0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (t < T && n < N) y[(ll)t * ldy + n] = (Out)((float)acc[i][j] * (sx[t] * sw[n]));
-    }
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s_sum[warp][t * 8 + (lane & 3) * 2 + (e & 1)][r * 16 + (lane >> 2) + (e >> 1) * 8] = acc[r][t][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < NT * 8 * 16 * RT; i += 256) {
+    const int t = i / (16 * RT), c = i % (16 * RT), n = n0 + c;
+    if (t >= T || n >= N) continue;
+    int sum = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += s_sum[k][t][c];
+    y[t * ldy + n] = (Out)((float)sum * (sx[t] * sw[n]));
+  }
+}
+
+constexpr int FEW = 32;        // tokens that gemm_q8_few_kernel takes
+template <class Out>
+int gemm_q8_few(const int8_t* x, const int8_t* w, const float* sx, const float* sw, Out* y, int T, int N, int K, ll ldx, ll ldw, ll ldy,
+                cudaStream_t st) {
+#define TPLR_FEW(NT, RT, U) launch_pdl(gemm_q8_few_kernel<NT, RT, U, Out>, (N + 16 * RT - 1) / (16 * RT), 256, 0, st, x, w, sx, sw, y, T, N, K, ldx, ldw, ldy)
+  if (T <= 8) return (int)TPLR_FEW(1, 1, 4);
+  if (T <= 16) return (int)TPLR_FEW(2, 1, 4);
+  if (T <= 24) return (int)TPLR_FEW(3, 1, 2);
+  return (int)TPLR_FEW(4, 1, 2);
+#undef TPLR_FEW
 }
 
 template <int MODE>
@@ -353,17 +410,18 @@ TPLR_API int tplr_swiglu_saved8_bwd(const float* dact, const void* q, ll ldq, co
                          scale, scale_row, scale_group, (bf16*)dgu, (bf16*)act, T, F);
 }
 
-// y[T, N] = sx[t] * sw[n] * (x w^T) for int8 rows x [T, K] and w [N, K] (row strides multiples of 16 bytes, zeros or any codes behind
-// column K of x multiplied by zeros of w: w's rows are zero from K to its stride), y bf16 or fp32 with row stride ldy.
+extern "C" int tplr_gemm2_q8(const void* X, const void* W, const float* sx, const float* sw, void* C, int M, int N, int K, ll ldx, ll ldw,
+                             ll ldc, int out_fp32, unsigned int* status, void* stream);
+
+// y[T, N] = sx[t] * sw[n] * (x w^T) for int8 rows x [T, K] and w [N, K] on 16-byte boundaries, y bf16 or fp32 with row stride ldy.  The
+// bytes of a row from K to the next 16-byte boundary are read: zeros in x, anything in w.
 TPLR_API int tplr_gemm_q8(const void* x, const void* w, const float* sx, const float* sw, void* y, int T, int N, int K, ll ldx, ll ldw,
                           ll ldy, int out_fp32, unsigned int* status, void* stream) {
   TPLR_ENTER();
   if (T <= 0 || N <= 0) return 0;
   if (K <= 0 || K > 131072 || (ldx | ldw) % 16 || (((uintptr_t)x | (uintptr_t)w) & 15)) return (int)cudaErrorInvalidValue;
-  const dim3 grid((N + 63) / 64, (T + 63) / 64);
-  if (out_fp32)
-    return (int)launch_pdl(gemm_q8_dot_kernel<float>, grid, 256, 0, (cudaStream_t)stream, (const int8_t*)x, (const int8_t*)w, sx, sw, (float*)y, T,
-                           N, K, ldx, ldw, ldy);
-  return (int)launch_pdl(gemm_q8_dot_kernel<bf16>, grid, 256, 0, (cudaStream_t)stream, (const int8_t*)x, (const int8_t*)w, sx, sw, (bf16*)y, T, N, K,
-                         ldx, ldw, ldy);
+  if (T > FEW) return tplr_gemm2_q8(x, w, sx, sw, y, T, N, K, ldx, ldw, ldy, out_fp32, status, stream);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (out_fp32) return gemm_q8_few((const int8_t*)x, (const int8_t*)w, sx, sw, (float*)y, T, N, K, ldx, ldw, ldy, st);
+  return gemm_q8_few((const int8_t*)x, (const int8_t*)w, sx, sw, (bf16*)y, T, N, K, ldx, ldw, ldy, st);
 }

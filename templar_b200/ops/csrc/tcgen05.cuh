@@ -168,15 +168,13 @@ inline PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
   return fn;
 }
 
-// 2-D bf16 (or fp32) tensor map: `inner` contiguous elements, `outer` rows of `ld` elements, 128B swizzle.
-inline bool make_map(CUtensorMap* map, const void* ptr, long long inner, long long outer, long long ld,
-              int box_inner, int box_outer, CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B,
-              bool fp32 = false) {
+// 2-D tensor map: `inner` contiguous elements of `size` bytes, `outer` rows of `ld` elements.
+inline bool make_map_of(CUtensorMap* map, CUtensorMapDataType dt, int size, const void* ptr, long long inner, long long outer, long long ld,
+                        int box_inner, int box_outer, CUtensorMapSwizzle swz) {
   auto enc = get_encode();
   if (!enc) return false;
   cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
-  cuuint64_t strides[1] = {(cuuint64_t)ld * (fp32 ? 4 : 2)};
-  const CUtensorMapDataType dt = fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  cuuint64_t strides[1] = {(cuuint64_t)ld * size};
   cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = enc(map, dt, 2, const_cast<void*>(ptr), dims, strides, box, estr,
@@ -194,6 +192,18 @@ inline bool make_map(CUtensorMap* map, const void* ptr, long long inner, long lo
     fprintf(stderr, "[tplr] cuTensorMapEncodeTiled failed (%d): ptr=%p inner=%lld outer=%lld ld=%lld box=%dx%d\n",
             (int)r, ptr, inner, outer, ld, box_inner, box_outer);
   return r == CUDA_SUCCESS;
+}
+// bf16 (or fp32), 128B swizzle unless another one is asked for
+inline bool make_map(CUtensorMap* map, const void* ptr, long long inner, long long outer, long long ld,
+              int box_inner, int box_outer, CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B,
+              bool fp32 = false) {
+  return make_map_of(map, fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, fp32 ? 4 : 2, ptr, inner, outer, ld,
+                     box_inner, box_outer, swz);
+}
+// bytes
+inline bool make_map_u8(CUtensorMap* map, const void* ptr, long long inner, long long outer, long long ld, int box_inner, int box_outer,
+                        CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B) {
+  return make_map_of(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, ptr, inner, outer, ld, box_inner, box_outer, swz);
 }
 
 }  // namespace tplr_tc
