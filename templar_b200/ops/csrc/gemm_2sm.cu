@@ -697,21 +697,23 @@ __device__ __forceinline__ void epilogue_q8(const Gemm2Params& p, uint32_t tmem_
       __syncwarp();
       const int rows = min(32, p.M - row0);
 #pragma unroll 1
-      for (int r = 0; r < rows; ++r) {
-        const uint32_t rowaddr = buf + (uint32_t)r * 128u, sw = (uint32_t)(r & 7);
+      for (int r0 = 0; r0 < rows; r0 += 8) {         // eight rows on their way at a time
 #pragma unroll
         for (int hh = 0; hh < COLS / 32; ++hh) {
           const int e = hh * 32 + lane;              // this lane's column of the box
-          if (col0 + e < p.N) {
-            if (F32) {
-              float o;
-              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(o) : "r"(rowaddr + ((((uint32_t)e >> 2) ^ sw) << 4) + (uint32_t)(e & 3) * 4u) : "memory");
-              reinterpret_cast<float*>(p.C)[(long long)(row0 + r) * p.ldc + col0 + e] = o;
-            } else {
-              uint16_t o;
-              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(o) : "r"(rowaddr + ((((uint32_t)e >> 3) ^ sw) << 4) + (uint32_t)(e & 7) * 2u) : "memory");
-              reinterpret_cast<uint16_t*>(p.C)[(long long)(row0 + r) * p.ldc + col0 + e] = o;
-            }
+          uint32_t o[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t rowaddr = buf + (uint32_t)(r0 + i) * 128u;
+            if (F32) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(o[i]) : "r"(rowaddr + ((((uint32_t)e >> 2) ^ i) << 4) + (uint32_t)(e & 3) * 4u) : "memory");
+            else     asm volatile("ld.shared.u16 %0, [%1];" : "=r"(o[i]) : "r"(rowaddr + ((((uint32_t)e >> 3) ^ i) << 4) + (uint32_t)(e & 7) * 2u) : "memory");
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (r0 + i >= rows || col0 + e >= p.N) continue;
+            const long long at = (long long)(row0 + r0 + i) * p.ldc + col0 + e;
+            if (F32) reinterpret_cast<uint32_t*>(p.C)[at] = o[i];
+            else     reinterpret_cast<uint16_t*>(p.C)[at] = (uint16_t)o[i];
           }
         }
       }

@@ -106,6 +106,152 @@ __global__ void __launch_bounds__(256) rows_q8_any_kernel(const RowsArgs p) {
   for (int i = threadIdx.x; i < p.ldq; i += 256) q[i] = i < D ? (int8_t)code(value(i), c.inv) : 0;
 }
 
+struct alignas(16) bf16x8 { __nv_bfloat162 v[4]; };
+__device__ __forceinline__ void unpack8(const bf16x8& p, float* f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { const float2 t = __bfloat1622float2(p.v[i]); f[2 * i] = t.x; f[2 * i + 1] = t.y; }
+}
+__device__ __forceinline__ bf16x8 pack8(const float* f) {
+  bf16x8 p;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p.v[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+  return p;
+}
+__device__ __forceinline__ uint2 codes8(const float* x, float inv) {
+  uint2 r = make_uint2(0, 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r.x |= (uint32_t)(code(x[i], inv) & 255) << (8 * i);
+    r.y |= (uint32_t)(code(x[4 + i], inv) & 255) << (8 * i);
+  }
+  return r;
+}
+__device__ __forceinline__ void values8(const uint2& q, float scale, float* f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[i] = (float)(int8_t)(q.x >> (8 * i)) * scale;
+    f[4 + i] = (float)(int8_t)(q.y >> (8 * i)) * scale;
+  }
+}
+
+// The same from registers, for rows of whole 16-byte pieces: `tpr` threads (a power of two) share a row, VPL pieces each, so a row is
+// read once and its two reductions (the squares, the largest magnitude) run on values that are already there.  Several rows a CTA
+// share its barriers.  Memory bounds it: a thread asks for all its pieces before it waits for the first.
+template <int MODE, int VPL, int BLOCK>
+__global__ void __launch_bounds__(BLOCK) rows_q8_kernel(const RowsArgs p, const int tpr) {
+  constexpr bool NORM = MODE == NORM_ROWS || MODE == NORM_SAVED, BY_GROUP = MODE == GROUPS || MODE == NORM_SAVED;
+  __shared__ float s_sum[32];
+  __shared__ uint32_t s_top[32];
+  grid_wait();
+  grid_release();
+  const int t = threadIdx.x & (tpr - 1), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.D, nv = D / 8, warps = tpr >> 5;
+  const int row_warp = threadIdx.x / tpr * warps;                        // first warp of this thread's row
+  const ll row = (ll)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
+  const bool live = row < p.T;
+  const bf16x8* a = reinterpret_cast<const bf16x8*>(p.a + (live ? row : 0) * p.lda);
+  const bf16x8* b = MODE == SWIGLU_ROWS ? a + nv : p.b ? reinterpret_cast<const bf16x8*>(p.b + (live ? row : 0) * p.ldb) : nullptr;
+  const bool two = MODE == SWIGLU_ROWS || (NORM && p.b);
+  float v[VPL][8];
+  {
+    bf16x8 ra[VPL], rb[VPL];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j)
+      if (live && t + tpr * j < nv) {
+        ra[j] = a[t + tpr * j];
+        if (two) rb[j] = b[t + tpr * j];
+      }
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      const int i = t + tpr * j;
+      if (!live || i >= nv) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
+        continue;
+      }
+      unpack8(ra[j], v[j]);
+      if (two) {
+        float o[8];
+        unpack8(rb[j], o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[j][e] = MODE == SWIGLU_ROWS ? silu_mul(v[j][e], o[e]) : v[j][e] + o[e];
+        if (NORM) {                                                      // the norm sees the sum as the residual stream stores it
+          const bf16x8 h = pack8(v[j]);
+          reinterpret_cast<bf16x8*>(p.h + row * D)[i] = h;
+          unpack8(h, v[j]);
+        }
+      }
+    }
+  }
+  if (NORM) {
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(v[j][e], v[j][e], ss);
+    ss = warp_sum(ss);
+    if (warps > 1) {
+      if (lane == 0) s_sum[warp] = ss;
+      __syncthreads();
+      ss = 0.f;
+      for (int k = 0; k < warps; ++k) ss += s_sum[row_warp + k];
+    }
+    const float r = rsqrtf(ss / (float)D + p.eps);
+    if (MODE == NORM_SAVED && live && t == 0) p.rstd[row] = r;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      const int i = t + tpr * j;
+      if (i >= nv) continue;
+      float w[8];
+      unpack8(reinterpret_cast<const bf16x8*>(p.w)[i], w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[j][e] *= r;
+        w[e] *= v[j][e];
+      }
+      if (MODE == NORM_ROWS) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[j][e] = w[e];
+      } else if (live) {
+        reinterpret_cast<bf16x8*>(p.y + row * D)[i] = pack8(w);
+      }
+    }
+  }
+  uint32_t tops[VPL];
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) {
+    tops[j] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) tops[j] = max(tops[j], magnitude(v[j][e]));
+  }
+  Codes all = {};
+  if (!BY_GROUP) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) top = max(top, tops[j]);
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (warps > 1) {
+      if (lane == 0) s_top[warp] = top;
+      __syncthreads();
+      for (int k = 0; k < warps; ++k) top = max(top, s_top[row_warp + k]);
+    }
+    all = codes_of(top);
+    if (live && t == 0) p.scale[row * p.scale_row] = all.scale;
+  }
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) {
+    const int i = t + tpr * j;
+    Codes c = all;
+    if (BY_GROUP) {                                                      // eight lanes hold a group's 64 columns
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) tops[j] = max(tops[j], __shfl_xor_sync(0xffffffffu, tops[j], o));
+      c = codes_of(tops[j]);
+      if (live && (i & 7) == 0 && i < nv) p.scale[row * p.scale_row + (i >> 3) * p.scale_group] = c.scale;
+    }
+    if (live && (ll)i * 8 < p.ldq)                                       // zeros behind the row: v is 0 there
+      reinterpret_cast<uint2*>(p.q + row * p.ldq)[i] = codes8(v[j], i < nv ? c.inv : 0.f);
+  }
+}
+
 // ------------------------------------------------------------------------------------------ 8 bits -> rows
 // y = q * scale (* w of the column), rows of D; a scale for every `group` columns.
 __global__ void __launch_bounds__(256) dequantize_any_kernel(const int8_t* q, ll ldq, const float* scale, ll scale_row, ll scale_group, int group,
@@ -119,6 +265,30 @@ __global__ void __launch_bounds__(256) dequantize_any_kernel(const int8_t* q, ll
     float v = (float)q[row * ldq + c] * scale[row * scale_row + c / group * scale_group];
     if (w) v *= __bfloat162float(w[c]);
     y[i] = __float2bfloat16(v);
+  }
+}
+
+// The same for whole 16-byte pieces of y and groups of whole pieces: eight columns a thread, `lanes` threads (a power of two) on a row.
+__global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* q, ll ldq, const float* scale, ll scale_row, ll scale_group, int group,
+                                                         const bf16* w, bf16* y, ll T, int D, int lanes) {
+  grid_wait();
+  grid_release();
+  const int nv = D / 8, rows = 256 / lanes;
+  for (ll row = (ll)blockIdx.x * rows + threadIdx.x / lanes; row < T; row += (ll)gridDim.x * rows) {
+    const uint2* src = reinterpret_cast<const uint2*>(q + row * ldq);
+    const float* s = scale + row * scale_row;
+#pragma unroll 4
+    for (int i = threadIdx.x & (lanes - 1); i < nv; i += lanes) {
+      float f[8];
+      values8(src[i], s[i * 8 / group * scale_group], f);
+      if (w) {
+        float m[8];
+        unpack8(reinterpret_cast<const bf16x8*>(w)[i], m);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= m[e];
+      }
+      reinterpret_cast<bf16x8*>(y + row * D)[i] = pack8(f);
+    }
   }
 }
 
@@ -148,6 +318,102 @@ __global__ void __launch_bounds__(256) rmsnorm_saved8_bwd_any_kernel(const bf16*
       dx[row * D + i] = __float2bfloat16(o);
     }
     __syncthreads();
+  }
+}
+
+// The same for whole 16-byte pieces: `tpr` threads on a row, VPL pieces each, the row in registers between its sum and its output, the weight
+// gradient's sums of a thread's columns in registers over all rows of the CTA.
+template <int VPL>
+__global__ void __launch_bounds__(256, VPL == 2 ? 3 : 2)
+rmsnorm_saved8_bwd_kernel(const bf16* dy, const int8_t* q, ll ldq, const float* scale, ll scale_row, ll scale_group, const float* rstd, const bf16* w,
+                          const bf16* dres, bf16* dx, float* part, ll T, int D, int tpr) {
+  __shared__ float s_dot[2][32];
+  __shared__ float s_dw[256 * 8];
+  grid_wait();
+  grid_release();
+  const int t = threadIdx.x & (tpr - 1), slot = threadIdx.x / tpr, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nv = D / 8;
+  const int warps = tpr >> 5, rows = 256 / tpr;
+  bf16x8 wp[VPL];
+  float dw[VPL][8];
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[j][e] = 0.f;
+    if (t + tpr * j < nv) wp[j] = reinterpret_cast<const bf16x8*>(w)[t + tpr * j];
+  }
+  int turn = 0;
+  for (ll first = (ll)blockIdx.x * rows; first < T; first += (ll)gridDim.x * rows, turn ^= 1) {
+    const ll row = first + slot;
+    const bool live = row < T;
+    bf16x8 g[VPL], a[VPL];
+    uint2 c[VPL];
+    float sc[VPL];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      const int i = t + tpr * j;
+      if (live && i < nv) {
+        g[j] = reinterpret_cast<const bf16x8*>(dy + row * D)[i];
+        c[j] = reinterpret_cast<const uint2*>(q + row * ldq)[i];
+        sc[j] = scale[row * scale_row + (i >> 3) * scale_group];
+        if (dres) a[j] = reinterpret_cast<const bf16x8*>(dres + row * D)[i];
+      }
+    }
+    const float r = live ? rstd[row] : 0.f;
+    float dot = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j)
+      if (live && t + tpr * j < nv) {
+        float d[8], x[8], m[8];
+        unpack8(g[j], d); unpack8(wp[j], m); values8(c[j], sc[j], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          dw[j][e] = fmaf(d[e], x[e], dw[j][e]);
+          dot = fmaf(d[e] * m[e], x[e], dot);
+        }
+      }
+    dot = warp_sum(dot);
+    if (warps > 1) {                                                     // two buffers: one barrier a row
+      if (lane == 0) s_dot[turn][warp] = dot;
+      __syncthreads();
+      dot = 0.f;
+      for (int k = 0; k < warps; ++k) dot += s_dot[turn][slot * warps + k];
+    }
+    dot /= (float)D;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      const int i = t + tpr * j;
+      if (live && i < nv) {
+        float d[8], x[8], m[8], o[8];
+        unpack8(g[j], d); unpack8(wp[j], m); values8(c[j], sc[j], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = r * (d[e] * m[e] - x[e] * dot);
+        if (dres) {
+          unpack8(a[j], d);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] += d[e];
+        }
+        reinterpret_cast<bf16x8*>(dx + row * D)[i] = pack8(o);
+      }
+    }
+  }
+  float* mine = part + (ll)blockIdx.x * D;
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) {
+    const int i = t + tpr * j;
+    if (rows > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s_dw[e * 256 + threadIdx.x] = dw[j][e];
+      __syncthreads();
+      if (slot == 0)
+        for (int k = 1; k < rows; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dw[j][e] += s_dw[e * 256 + k * tpr + t];
+    }
+    if (slot == 0 && i < nv) {
+      reinterpret_cast<float4*>(mine + i * 8)[0] = make_float4(dw[j][0], dw[j][1], dw[j][2], dw[j][3]);
+      reinterpret_cast<float4*>(mine + i * 8)[1] = make_float4(dw[j][4], dw[j][5], dw[j][6], dw[j][7]);
+    }
   }
 }
 
@@ -220,10 +486,10 @@ __global__ void __launch_bounds__(256) swiglu_saved8_bwd_kernel(const float* dac
 
 // ------------------------------------------------------------------------------------------ product, few tokens
 // y[t, n] = sx[t] * sw[n] * sum_k x[t, k] w[n, k] where the weight's bytes are all that counts: they are read once, 16 bytes a lane,
-// straight into the operands of mma.m16n8k32 (a tile of 128 rows by tcgen05 would stage them in shared memory first and use 8 to 32 of
-// its 256 columns).  The sum over k may be taken in any order, so a lane's 16 bytes of a row are its words of two instructions
-// as they lie: word j of a weight row and word j of a token are multiplied wherever the instruction thinks they are.  A CTA's
-// eight warps take 64-byte pieces of 16 * RT rows in turn, 512 bytes of a row together, and add their sums in shared memory.
+// straight into the operands of mma.m16n8k32: nothing is set up before the first load, which for 2048 x 2048 is a third of
+// the time.  The sum over k may be taken in any order, so a lane's 16 bytes of a row are its words of two instructions as they lie:
+// word j of a weight row and word j of a token are multiplied wherever the instruction thinks they are.  A CTA's eight warps take
+// 64-byte pieces of 16 rows in turn, 512 bytes of a row together, and add their sums in shared memory.
 __device__ __forceinline__ uint4 ld_once(const int8_t* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
@@ -233,85 +499,83 @@ __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <int NT, int RT, int UNROLL, class Out>
+template <class Out>
 __global__ void __launch_bounds__(256) gemm_q8_few_kernel(const int8_t* x, const int8_t* w, const float* sx, const float* sw, Out* y, int T,
                                                           int N, int K, ll ldx, ll ldw, ll ldy) {
-  __shared__ int s_sum[8][NT * 8][16 * RT + 1];
+  constexpr int UNROLL = 4;
+  __shared__ int s_sum[8][8][17];
   grid_wait();
   grid_release();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n0 = blockIdx.x * 16 * RT, kp = (K + 15) / 16 * 16;
-  int acc[RT][NT][4] = {};
-  const int8_t* wr[RT][2];
-  bool wok[RT][2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n0 = blockIdx.x * 16, kp = (K + 15) / 16 * 16, tok = lane >> 2;
+  int acc[4] = {};
+  const int8_t* wr[2];
+  bool wok[2];
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int n = n0 + r * 16 + h * 8 + (lane >> 2);
-      wok[r][h] = n < N;
-      wr[r][h] = w + (ll)(n < N ? n : N - 1) * ldw;
-    }
+  for (int h = 0; h < 2; ++h) {
+    const int n = n0 + h * 8 + (lane >> 2);
+    wok[h] = n < N;
+    wr[h] = w + (ll)(n < N ? n : N - 1) * ldw;
+  }
   const uint4 zero = make_uint4(0, 0, 0, 0);
   for (int k0 = warp * 64; k0 < kp; k0 += 512 * UNROLL) {
-    uint4 a[UNROLL][RT][2], b[UNROLL][NT];
+    uint4 a[UNROLL][2], b[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       const int k = k0 + u * 512 + (lane & 3) * 16;
       const bool in = k < kp;
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) a[u][r][h] = in && wok[r][h] ? ld_once(wr[r][h] + k) : zero;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int tok = t * 8 + (lane >> 2);
-        b[u][t] = in && tok < T ? *reinterpret_cast<const uint4*>(x + tok * ldx + k) : zero;
-      }
+      for (int h = 0; h < 2; ++h) a[u][h] = in && wok[h] ? ld_once(wr[h] + k) : zero;
+      b[u] = in && tok < T ? *reinterpret_cast<const uint4*>(x + tok * ldx + k) : zero;
     }
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          mma_s8(acc[r][t], a[u][r][0].x, a[u][r][1].x, a[u][r][0].y, a[u][r][1].y, b[u][t].x, b[u][t].y);
-          mma_s8(acc[r][t], a[u][r][0].z, a[u][r][1].z, a[u][r][0].w, a[u][r][1].w, b[u][t].z, b[u][t].w);
-        }
+    for (int u = 0; u < UNROLL; ++u) {
+      mma_s8(acc, a[u][0].x, a[u][1].x, a[u][0].y, a[u][1].y, b[u].x, b[u].y);
+      mma_s8(acc, a[u][0].z, a[u][1].z, a[u][0].w, a[u][1].w, b[u].z, b[u].w);
+    }
   }
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s_sum[warp][t * 8 + (lane & 3) * 2 + (e & 1)][r * 16 + (lane >> 2) + (e >> 1) * 8] = acc[r][t][e];
+  for (int e = 0; e < 4; ++e) s_sum[warp][(lane & 3) * 2 + (e & 1)][(lane >> 2) + (e >> 1) * 8] = acc[e];
   __syncthreads();
-  for (int i = threadIdx.x; i < NT * 8 * 16 * RT; i += 256) {
-    const int t = i / (16 * RT), c = i % (16 * RT), n = n0 + c;
-    if (t >= T || n >= N) continue;
-    int sum = 0;
+  const int t = threadIdx.x >> 4, c = threadIdx.x & 15, n = n0 + c;
+  if (t >= T || n >= N) return;                                          // 16 threads a token: those from 8 on have none
+  int sum = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum += s_sum[k][t][c];
-    y[t * ldy + n] = (Out)((float)sum * (sx[t] * sw[n]));
-  }
+  for (int k = 0; k < 8; ++k) sum += s_sum[k][t][c];
+  y[t * ldy + n] = (Out)((float)sum * (sx[t] * sw[n]));
 }
 
-constexpr int FEW = 32;        // tokens that gemm_q8_few_kernel takes
+constexpr int FEW = 8;         // tokens of one instruction
 template <class Out>
 int gemm_q8_few(const int8_t* x, const int8_t* w, const float* sx, const float* sw, Out* y, int T, int N, int K, ll ldx, ll ldw, ll ldy,
                 cudaStream_t st) {
-#define TPLR_FEW(NT, RT, U) launch_pdl(gemm_q8_few_kernel<NT, RT, U, Out>, (N + 16 * RT - 1) / (16 * RT), 256, 0, st, x, w, sx, sw, y, T, N, K, ldx, ldw, ldy)
-  if (T <= 8) return (int)TPLR_FEW(1, 1, 4);
-  if (T <= 16) return (int)TPLR_FEW(2, 1, 4);
-  if (T <= 24) return (int)TPLR_FEW(3, 1, 2);
-  return (int)TPLR_FEW(4, 1, 2);
-#undef TPLR_FEW
+  return (int)launch_pdl(gemm_q8_few_kernel<Out>, (N + 15) / 16, 256, 0, st, x, w, sx, sw, y, T, N, K, ldx, ldw, ldy);
+}
+
+template <class... P>
+bool whole_pieces(P... ptrs) { return ((reinterpret_cast<uintptr_t>(ptrs) | ...) & 15) == 0; }
+// Threads of a row of `pieces` 16-byte pieces at `vpl` each.
+int row_threads(int pieces, int vpl) {
+  int n = 32;
+  while (n * vpl < pieces) n *= 2;
+  return n;
 }
 
 template <int MODE>
 int rows_q8(const RowsArgs& p, void* stream) {
   if (p.T <= 0) return 0;
   if (p.T > 0x7fffffffLL || p.D <= 0 || p.ldq < p.D) return (int)cudaErrorInvalidValue;
-  return (int)launch_pdl(rows_q8_any_kernel<MODE>, (unsigned)p.T, 256, 0, (cudaStream_t)stream, p);
+  cudaStream_t st = (cudaStream_t)stream;
+  const int pieces = (int)((p.ldq + 7) / 8);
+  if (p.D % 8 || p.ldq % 8 || p.lda % 8 || (p.b && p.ldb % 8) || p.D > 32760 || !whole_pieces(p.a, p.b, p.w, p.h, p.y, p.q))
+    return (int)launch_pdl(rows_q8_any_kernel<MODE>, (unsigned)p.T, 256, 0, st, p);
+  // one piece a thread while that leaves threads to spare on the chip, four where rows are many
+  const int vpl = p.T * pieces <= 2048LL * tplr_sm_count() && pieces <= 1024 ? 1 : 4;
+  const int tpr = row_threads(pieces, vpl), block = tpr > 256 ? 1024 : 256;
+  const unsigned grid = (unsigned)((p.T + block / tpr - 1) / (block / tpr));
+  if (block == 1024) return (int)(vpl == 1 ? launch_pdl(rows_q8_kernel<MODE, 1, 1024>, grid, block, 0, st, p, tpr)
+                                           : launch_pdl(rows_q8_kernel<MODE, 4, 1024>, grid, block, 0, st, p, tpr));
+  return (int)(vpl == 1 ? launch_pdl(rows_q8_kernel<MODE, 1, 256>, grid, block, 0, st, p, tpr)
+                        : launch_pdl(rows_q8_kernel<MODE, 4, 256>, grid, block, 0, st, p, tpr));
 }
 unsigned waves(ll ctas, int resident) {
   const ll most = (ll)tplr_sm_count() * resident;
@@ -366,11 +630,17 @@ TPLR_API int tplr_dequantize_rows(const void* q, ll ldq, const float* scale, ll 
   TPLR_ENTER();
   if (T <= 0) return 0;
   if (D <= 0 || group <= 0) return (int)cudaErrorInvalidValue;
+  if (D % 8 == 0 && ldq % 8 == 0 && (group % 8 == 0 || group >= D) && whole_pieces(q, w, y)) {
+    int lanes = 32;
+    while (lanes < 256 && lanes * 8 < D) lanes *= 2;
+    return (int)launch_pdl(dequantize_kernel, waves((T + 256 / lanes - 1) / (256 / lanes), 32), 256, 0, (cudaStream_t)stream, (const int8_t*)q,
+                           ldq, scale, scale_row, scale_group, group, (const bf16*)w, (bf16*)y, T, D, lanes);
+  }
   return (int)launch_pdl(dequantize_any_kernel, waves((T * D + 255) / 256, 16), 256, 0, (cudaStream_t)stream, (const int8_t*)q, ldq, scale,
                          scale_row, scale_group, group, (const bf16*)w, (bf16*)y, T, D);
 }
 
-// CTAs of the norm's backward: rows of the fp32 workspace that tplr_rmsnorm_saved8_bwd takes (each of D elements).
+// Rows (each of D elements) of the fp32 workspace that tplr_rmsnorm_saved8_bwd takes: its CTAs at most.
 TPLR_API int tplr_rmsnorm_saved8_parts(ll T, int D) { return (int)waves(T, 4); }
 
 // dx of the norm from its rows in 8 bits (dres null: 0), and its weight's gradient: added into dw_add (fp32) or stored in dw_out (bf16); both
@@ -381,12 +651,22 @@ TPLR_API int tplr_rmsnorm_saved8_bwd(const void* dy, const void* q, ll ldq, cons
   TPLR_ENTER();
   if (T <= 0) return 0;
   if (D <= 0) return (int)cudaErrorInvalidValue;
-  const int n = tplr_rmsnorm_saved8_parts(T, D);
-  if (const cudaError_t e = launch_pdl(rmsnorm_saved8_bwd_any_kernel, n, 256, 0, (cudaStream_t)stream, (const bf16*)dy, (const int8_t*)q, ldq,
-                                       scale, scale_row, scale_group, rstd, (const bf16*)w, (const bf16*)dres, (bf16*)dx, part, T, D))
-    return (int)e;
-  if (!dw_add && !dw_out) return 0;
-  return (int)launch_pdl(sum_parts_kernel, (D + 31) / 32, 256, 0, (cudaStream_t)stream, part, n, D, dw_add, (bf16*)dw_out);
+  cudaStream_t st = (cudaStream_t)stream;
+  const bf16 *g = (const bf16*)dy, *wp = (const bf16*)w, *a = (const bf16*)dres;
+  const int8_t* c = (const int8_t*)q;
+  int n;
+  cudaError_t e;
+  if (D % 8 || D > 8192 || ldq % 8 || !whole_pieces(dy, q, w, dres, dx, part)) {
+    n = (int)waves(T, 4);
+    e = launch_pdl(rmsnorm_saved8_bwd_any_kernel, n, 256, 0, st, g, c, ldq, scale, scale_row, scale_group, rstd, wp, a, (bf16*)dx, part, T, D);
+  } else {
+    const int vpl = D <= 4096 ? 2 : 4, tpr = row_threads(D / 8, vpl), rows = 256 / tpr;
+    n = (int)waves((T + rows - 1) / rows, vpl == 2 ? 3 : 2);
+    e = launch_pdl(vpl == 2 ? rmsnorm_saved8_bwd_kernel<2> : rmsnorm_saved8_bwd_kernel<4>, n, 256, 0, st, g, c, ldq, scale, scale_row, scale_group,
+                   rstd, wp, a, (bf16*)dx, part, T, D, tpr);
+  }
+  if (e != cudaSuccess || (!dw_add && !dw_out)) return (int)e;
+  return (int)launch_pdl(sum_parts_kernel, (D + 31) / 32, 256, 0, st, part, n, D, dw_add, (bf16*)dw_out);
 }
 
 // The activation of a dense fp32 [gate | up] projection, and the projection in 8 bits (rows of ldq >= 2 F bytes) by 64 columns of each half.
@@ -412,15 +692,24 @@ TPLR_API int tplr_swiglu_saved8_bwd(const float* dact, const void* q, ll ldq, co
 
 extern "C" int tplr_gemm2_q8(const void* X, const void* W, const float* sx, const float* sw, void* C, int M, int N, int K, ll ldx, ll ldw,
                              ll ldc, int out_fp32, unsigned int* status, void* stream);
+extern "C" int tplr_gemm_q8_stream(const void* X, const void* W, const float* sx, const float* sw, void* C, int T, int N, int K, ll ldx, ll ldw,
+                                   ll ldc, int out_fp32, unsigned int* status, void* stream);
 
 // y[T, N] = sx[t] * sw[n] * (x w^T) for int8 rows x [T, K] and w [N, K] on 16-byte boundaries, y bf16 or fp32 with row stride ldy.  The
 // bytes of a row from K to the next 16-byte boundary are read: zeros in x, anything in w.
+//
+// Which kernel: up to 8 tokens the one that loads the weight into registers, up to 64 the weight's rows as the tensor core's long side
+// with K cut over clusters, more on CTA pairs; up to 128 tokens the cut still wins where K is long.  Microseconds, the
+// three in that order, inner dimension x channels at 8 | 32 | 64 | 128 tokens: 2048 x 2048 2.8, 3.9, 7.5 | 7.4, 4.9, 7.5 | -, 6.7, 7.5 |
+// -, 10.4, 8.0; 4096 x 6144 6.5, 8.8, 14.5 | 15.6, 9.6, 11.5 | -, 11.7, 11.5 | -, 18.5, 12.1; 2048 x 16384 8.9, 9.2, 14.8 | 17.3, 9.9, 14.4 |
+// -, 12.0, 13.9 | -, 16.0, 14.5; 14336 x 4096 13.7, 13.4, 34.1 | 42.5, 13.8, 24.4 | -, 15.2, 24.6 | -, 19.0, 25.2; 8192 x 2048 at 128: 13.7, 16.1.
 TPLR_API int tplr_gemm_q8(const void* x, const void* w, const float* sx, const float* sw, void* y, int T, int N, int K, ll ldx, ll ldw,
                           ll ldy, int out_fp32, unsigned int* status, void* stream) {
   TPLR_ENTER();
   if (T <= 0 || N <= 0) return 0;
   if (K <= 0 || K > 131072 || (ldx | ldw) % 16 || (((uintptr_t)x | (uintptr_t)w) & 15)) return (int)cudaErrorInvalidValue;
-  if (T > FEW) return tplr_gemm2_q8(x, w, sx, sw, y, T, N, K, ldx, ldw, ldy, out_fp32, status, stream);
+  if (T > FEW) return (T <= (K >= 8192 ? 128 : 64) ? tplr_gemm_q8_stream : tplr_gemm2_q8)(x, w, sx, sw, y, T, N, K, ldx, ldw, ldy, out_fp32,
+                                                                                          status, stream);
   cudaStream_t st = (cudaStream_t)stream;
   if (out_fp32) return gemm_q8_few((const int8_t*)x, (const int8_t*)w, sx, sw, (float*)y, T, N, K, ldx, ldw, ldy, st);
   return gemm_q8_few((const int8_t*)x, (const int8_t*)w, sx, sw, (bf16*)y, T, N, K, ldx, ldw, ldy, st);

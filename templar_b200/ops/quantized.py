@@ -58,6 +58,12 @@ class QuantRows:
     __slots__ = ("q", "scale", "group", "shape")
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor, group: int, shape):
+        D = shape[-1]
+        if q.dtype != torch.int8 or q.dim() != 2 or q.shape[1] != _padded(D) or q.stride() != (q.shape[1], 1):
+            raise ValueError(f"QuantRows: dense int8 codes [T, {_padded(D)}] expected, got {q.dtype} {tuple(q.shape)}, strides {q.stride()}")
+        if scale.dtype != torch.float32 or scale.shape != (q.shape[0], -(-D // group) if group else 1) or scale.device != q.device:
+            raise ValueError(f"QuantRows: fp32 scales [{q.shape[0]}, {-(-D // group) if group else 1}] on {q.device} expected, got "
+                             f"{scale.dtype} {tuple(scale.shape)} on {scale.device}")
         self.q, self.scale, self.group, self.shape = q, scale, int(group), torch.Size(shape)
 
     @property
@@ -98,22 +104,25 @@ def quantize_rows(x: torch.Tensor, group: int = 0) -> QuantRows:
 
 def dequantize_rows(rows: QuantRows, dtype: torch.dtype = torch.bfloat16, weight: torch.Tensor | None = None) -> torch.Tensor:
     """The values ``q * scale``, times ``weight`` [columns] where one is given."""
-    q, scale, D = rows.q, rows.scale, rows.width
-    T = q.shape[0]
-    if weight is not None and weight.numel() != D:
-        raise ValueError(f"dequantize_rows: {weight.numel()} weights for {D} columns")
+    if weight is not None and weight.numel() != rows.width:
+        raise ValueError(f"dequantize_rows: {weight.numel()} weights for {rows.width} columns")
+    return _values(rows.q, rows.scale, rows.group, rows.shape, dtype, weight)
+
+
+def _values(q, scale, group: int, shape, dtype, weight=None):
+    T, D = q.shape[0], shape[-1]
     if q.is_cuda and dtype == torch.bfloat16 and _native_rows(weight):
-        y = torch.empty(rows.shape, dtype=dtype, device=q.device)
+        y = torch.empty(shape, dtype=dtype, device=q.device)
         w = None if weight is None else weight.detach().contiguous()
         native.check(native.lib().tplr_dequantize_rows(q.data_ptr(), q.stride(0), scale.data_ptr(), scale.stride(0),
-                                                       scale.stride(1) if rows.group else 0, rows.group or D, native.ptr(w),
+                                                       scale.stride(1) if group else 0, group or D, native.ptr(w),
                                                        y.data_ptr(), T, D, native.stream_ptr()), "dequantize_rows")
         return y
-    wide = scale if not rows.group else scale.repeat_interleave(rows.group, dim=1)[:, :D]
+    wide = scale if not group else scale.repeat_interleave(group, dim=1)[:, :D]
     v = q[:, :D].float() * wide
     if weight is not None:
         v = v * weight.detach().float()
-    return v.to(dtype).view(rows.shape)
+    return v.to(dtype).view(shape)
 
 
 # --------------------------------------------------------------------------- #
@@ -229,7 +238,8 @@ def linear_q8(x: torch.Tensor | QuantRows, w: QuantWeight, out_dtype: torch.dtyp
     T, N, K = x.q.shape[0], w.shape[0], w.shape[1]
     if x.q.is_cuda and out_dtype in (torch.bfloat16, torch.float32):
         y = torch.empty(*x.shape[:-1], N, dtype=out_dtype, device=x.q.device)
-        native.check(native.lib().tplr_gemm_q8(x.q.data_ptr(), w.q.data_ptr(), x.scale.data_ptr(), w.scale.data_ptr(), y.data_ptr(), T, N, K,
+        sx = x.scale.contiguous()
+        native.check(native.lib().tplr_gemm_q8(x.q.data_ptr(), w.q.data_ptr(), sx.data_ptr(), w.scale.data_ptr(), y.data_ptr(), T, N, K,
                                                x.q.stride(0), w.q.stride(0), N, int(out_dtype == torch.float32),
                                                OF.status_word(y.device).data_ptr(), native.stream_ptr()), "gemm_q8")
         return y
@@ -301,7 +311,7 @@ class _AddRMSNormSaved8(torch.autograd.Function):
             if add is not None and add is not mg:
                 mg.add_(add.view(mg.shape).to(mg.dtype))
             return dx, dx if ctx.needs_input_grad[1] else None, out, None, None
-        xn = dequantize_rows(QuantRows(q, scale, GROUP, (q.shape[0], D)), torch.float32)
+        xn = _values(q, scale, GROUP, (q.shape[0], D), torch.float32)
         d = dy.float().reshape(-1, D)
         g = d * w.float()
         dx = (rstd[:, None] * (g - xn * (g * xn).mean(-1, keepdim=True))).view(shape)
@@ -343,7 +353,7 @@ def _kept_input(x, rows: QuantRows | None, weight):
 
 def _input_again(q, scale, weight, shape, dtype):
     """The rows that a projection multiplied, from what was kept of them: [T, K]."""
-    return dequantize_rows(QuantRows(q, scale, GROUP, (q.shape[0], shape[-1])), dtype, weight)
+    return _values(q, scale, GROUP, (q.shape[0], shape[-1]), dtype, weight)
 
 
 class _LinearSaved8(torch.autograd.Function):
@@ -419,8 +429,7 @@ class _FeedForwardSaved8(torch.autograd.Function):
                          "swiglu_saved8_bwd")
         else:
             G = scale.shape[1] // 2
-            g, u = (dequantize_rows(QuantRows(q[:, i * Fd:(i + 1) * Fd], scale[:, i * G:(i + 1) * G], GROUP, (T, Fd)), torch.float32)
-                    for i in (0, 1))
+            g, u = (_values(q[:, i * Fd:(i + 1) * Fd], scale[:, i * G:(i + 1) * G], GROUP, (T, Fd), torch.float32) for i in (0, 1))
             sg = torch.sigmoid(g)
             silu = g * sg
             dgu = torch.cat((dact * u * (sg + silu * (1 - sg)), dact * silu), dim=1).to(ctx.dtype)

@@ -197,6 +197,10 @@ def test_refusals():
         ops.QuantWeight(torch.zeros(3, 4, dtype=torch.int8), torch.zeros(4))
     with pytest.raises(ValueError, match="leave 32 bits"):
         ops.QuantWeight(torch.zeros(1, 131088, dtype=torch.int8), torch.zeros(1))
+    with pytest.raises(ValueError, match="dense int8 codes"):
+        ops.QuantRows(torch.zeros(3, 20, dtype=torch.int8), torch.zeros(3, 1), 0, (3, 20))
+    with pytest.raises(ValueError, match="fp32 scales"):
+        ops.QuantRows(torch.zeros(3, 80, dtype=torch.int8), torch.zeros(3, 1), 64, (3, 80))
     with pytest.raises(ValueError, match="do not fit"):
         ops.feed_forward_saved8(x, rand(16, 32), rand(32, 9))
     with pytest.raises(ValueError, match="by 64 columns"):
