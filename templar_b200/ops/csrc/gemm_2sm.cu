@@ -25,6 +25,7 @@
 //
 // Replaces cuBLAS + NCCL behind the reference's tensor-parallel plan: colwise q/k/v/w1/w3,
 // rowwise wo/w2 with sequence-sharded activations (torchtitan models/llama3/infra/parallelize.py:151-219).
+#include "quant.cuh"
 #include "tcgen05.cuh"
 #include <stdlib.h>
 
@@ -86,6 +87,10 @@ struct Gemm2Params {
   // 8-bit operands (EPI 7 bf16, EPI 8 fp32 result): C[m, n] = acc * (q8_row[m] * q8_col[n]) of the int32 accumulator
   const float* q8_row;
   const float* q8_col;
+  // projection kept in 8 bits (EPI 9 writes it, EPI 10 reads it): the scale of row m and group g of 64 columns is
+  // q8_scale[g * q8_ld + m], gate groups first
+  float* q8_scale;
+  long long q8_ld;
   int world, rank;
   unsigned int epoch;
   // gather
@@ -723,14 +728,166 @@ __device__ __forceinline__ void epilogue_q8(const Gemm2Params& p, uint32_t tmem_
   }
 }
 
+// Epilogue of the fused [w1; w3] projection whose gate and up values are kept in 8 bits for the backward pass (EPI 9): as
+// epilogue_swiglu, but a row's 64 values of either half, a group, leave as codes with one scale instead of as bf16: half the
+// bytes of its two larger outputs.  The codes are made from the fp32 accumulators.  A lane has a row, so a group's largest
+// magnitude needs no exchange, and 32 rows' scales of a group lie side by side.
+// 16384 x 2048 -> 8192: XX us, where the bf16 form takes XX.
+__device__ __forceinline__ uint32_t box64_row(uint32_t buf, int row) { return buf + (uint32_t)row * 64u; }      // box of 64 bytes a row,
+__device__ __forceinline__ uint32_t box64_at(int row, int j) { return (uint32_t)(j ^ ((row >> 1) & 3)) << 4; }  // 64-byte swizzle
+__device__ __forceinline__ void epilogue_swiglu_q8(const Gemm2Params& p, uint32_t tmem_acc, int quad, int lane, int m0, int tn,
+                                                   uint32_t stage_base, uint32_t& n_boxes) {
+  const int row0 = m0 + quad * 32;
+  if (row0 >= p.M) return;                           // warp-uniform
+  const uint32_t lane_sel = (uint32_t)(quad * 32) << 16;
+  const int half = p.tile_n / 2;                     // features of a tile
+#pragma unroll 1
+  for (int c = 0; c < half / 64; ++c) {
+    const int f0 = tn * half + c * 64;               // first feature of this box
+    if (f0 >= p.swiglu_f) break;
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {           // 0: gate codes, 1: up codes
+      float v[64];
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        uint32_t r[32];
+        tmem_ld32(tmem_acc + part * half + c * 64 + hh * 32 + lane_sel, r);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[hh * 32 + e] = __uint_as_float(r[e]);
+      }
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 64; ++e) top = max(top, magnitude(v[e]));
+      const Codes q = codes_of(top);
+      if (row0 + lane < p.M) p.q8_scale[(long long)((part * p.swiglu_f + f0) / QUANT_GROUP) * p.q8_ld + row0 + lane] = q.scale;
+      const uint32_t buf = box_begin(lane, stage_base, n_boxes), rowaddr = box64_row(buf, lane);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + box64_at(lane, j)), "r"(codes4(v + 16 * j, q.inv)),
+                     "r"(codes4(v + 16 * j + 4, q.inv)), "r"(codes4(v + 16 * j + 8, q.inv)), "r"(codes4(v + 16 * j + 12, q.inv)) : "memory");
+      box_store(&p.tmC, buf, lane, n_boxes, part * p.swiglu_f + f0, row0);
+    }
+    const uint32_t buf = box_begin(lane, stage_base, n_boxes);
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      uint32_t rg[32], ru[32];
+      float v[32];
+      tmem_ld32(tmem_acc + c * 64 + hh * 32 + lane_sel, rg);
+      tmem_ld32(tmem_acc + half + c * 64 + hh * 32 + lane_sel, ru);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const float g = __uint_as_float(rg[e]);
+        v[e] = __fdividef(g, 1.f + __expf(-g)) * __uint_as_float(ru[e]);
+      }
+      box_half(buf, lane, hh, v);
+    }
+    box_store(&p.tmCr[0], buf, lane, n_boxes, f0, row0);
+  }
+}
+
+// Backward of the SwiGLU on the down projection's data gradient from the projection kept in 8 bits (EPI 10): as
+// epilogue_swiglu_bwd, with g and u as boxes of 32 rows x 64 codes (a quarter of that epilogue's loads), and the activation
+// s * g * u formed again as a third output for the down projection's weight gradient, which no pass stored.  The 64 columns' three outputs wait
+// packed in registers for the two buffers of the warp: the codes are read, and each exponential taken, once.
+// 16384 x 2048 -> 8192: XX us, where the bf16 form takes XX and forms no activation.
+struct CodeLoads {
+  uint32_t bar;                      // two mbarriers of this warp
+  uint32_t base;                     // two pairs of 2 KB buffers
+  uint32_t issued, used;             // box pairs asked for and consumed so far
+  float sg, su;                      // scales of this lane's row in the pair asked for last
+};
+__device__ __forceinline__ void codes_issue(const Gemm2Params& p, CodeLoads& L, int lane, int f0, int row0) {
+  const long long row = min(row0 + lane, p.M - 1);
+  L.sg = p.q8_scale[(long long)(f0 / QUANT_GROUP) * p.q8_ld + row];
+  L.su = p.q8_scale[(long long)((p.swiglu_f + f0) / QUANT_GROUP) * p.q8_ld + row];
+  if (lane == 0) {
+    const uint32_t s = L.issued & 1u, bar = L.bar + 8u * s, buf = L.base + s * 4096u;
+    mbar_expect_tx(bar, 4096);
+    tma_load_2d(buf, &p.tmGU, bar, f0, row0);
+    tma_load_2d(buf + 2048u, &p.tmGU, bar, p.swiglu_f + f0, row0);
+  }
+  ++L.issued;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void box_words(uint32_t buf, int lane, const uint32_t* w) {
+  const uint32_t rowaddr = buf + (uint32_t)lane * 128u, sw = (uint32_t)(lane & 7);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + (((uint32_t)j ^ sw) << 4)), "r"(w[4 * j]), "r"(w[4 * j + 1]),
+                 "r"(w[4 * j + 2]), "r"(w[4 * j + 3]) : "memory");
+}
+__device__ __forceinline__ bool epilogue_swiglu_bwd_q8(const Gemm2Params& p, uint32_t tmem_acc, int quad, int lane, int m0, int n0,
+                                                       CodeLoads& L, uint32_t stage_base, uint32_t& n_boxes, volatile int* abort_flag) {
+  const int row0 = m0 + quad * 32;
+  if (row0 >= p.M || n0 >= p.swiglu_f) return true;  // warp-uniform; nothing was asked for
+  const uint32_t lane_sel = (uint32_t)(quad * 32) << 16;
+#pragma unroll 1
+  for (int c = 0; c < p.tile_n / 64; ++c) {
+    const int f0 = n0 + c * 64;
+    if (f0 >= p.swiglu_f) break;                     // warp-uniform (swiglu_f is a multiple of 64)
+    const float sg = L.sg, su = L.su;
+    if (c + 1 < p.tile_n / 64 && f0 + 64 < p.swiglu_f) codes_issue(p, L, lane, f0 + 64, row0);
+    const uint32_t s = L.used & 1u;
+    const bool ok = mbar_wait(L.bar + 8u * s, (L.used >> 1) & 1u, abort_flag);
+    if (!__all_sync(0xffffffffu, ok)) return false;
+    ++L.used;
+    const uint32_t grow = box64_row(L.base + s * 4096u, lane), urow = grow + 2048u;
+    uint32_t dg[32], du[32], act[32];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      uint32_t r[32];
+      tmem_ld32(tmem_acc + c * 64 + hh * 32 + lane_sel, r);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int j = hh * 2 + q;                    // 16 columns
+        uint32_t gw[4], uw[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(gw[0]), "=r"(gw[1]), "=r"(gw[2]), "=r"(gw[3]) : "r"(grow + box64_at(lane, j)) : "memory");
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(uw[0]), "=r"(uw[1]), "=r"(uw[2]), "=r"(uw[3]) : "r"(urow + box64_at(lane, j)) : "memory");
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          float g[4], u[4], a[4];
+          numbers4(gw[w], g); numbers4(uw[w], u);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float dh = __uint_as_float(r[q * 16 + w * 4 + e]);
+            const float gv = g[e] * sg, uv = u[e] * su;
+            const float sig = __fdividef(1.f, 1.f + __expf(-gv)), silu = gv * sig;
+            a[e] = silu * uv;
+            g[e] = dh * uv * (sig + silu * (1.f - sig));
+            u[e] = dh * silu;
+          }
+          const int at = j * 8 + w * 2;
+          dg[at] = pack2(g[0], g[1]); dg[at + 1] = pack2(g[2], g[3]);
+          du[at] = pack2(u[0], u[1]); du[at + 1] = pack2(u[2], u[3]);
+          act[at] = pack2(a[0], a[1]); act[at + 1] = pack2(a[2], a[3]);
+        }
+      }
+    }
+    __syncwarp();                                    // every lane has read its codes: their buffer may be asked for again
+    uint32_t buf = box_begin(lane, stage_base, n_boxes);
+    box_words(buf, lane, dg);
+    box_store(&p.tmC, buf, lane, n_boxes, f0, row0);
+    buf = box_begin(lane, stage_base, n_boxes);
+    box_words(buf, lane, du);
+    box_store(&p.tmC, buf, lane, n_boxes, p.swiglu_f + f0, row0);
+    buf = box_begin(lane, stage_base, n_boxes);
+    box_words(buf, lane, act);
+    box_store(&p.tmCr[0], buf, lane, n_boxes, f0, row0);
+  }
+  return true;
+}
+
 // EPI: 0 store bf16, 1 fp32 accumulate (C += acc), 2 store fp32, 3 fused SwiGLU of a packed [w1; w3] projection,
 // 4 store bf16 with the rotary embedding applied to the leading columns, 5 backward of the SwiGLU on the data gradient
 // of the down projection, 6 data gradient of the attention output projection with the attention backward's delta term,
-// 7 / 8 product of 8-bit rows stored as bf16 / fp32
+// 7 / 8 product of 8-bit rows stored as bf16 / fp32, 9 as 3 with the projection kept in 8 bits, 10 as 5 from it
 template <bool A_MN, bool B_MN, int EPI>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 gemm2_kernel(const __grid_constant__ Gemm2Params p) {
-  constexpr int RING_BYTES = (EPI == 5 ? EPI5_STAGES : STAGES) * STAGE_BYTES;
+  constexpr int RING_BYTES = (EPI == 5 || EPI == 10 ? EPI5_STAGES : STAGES) * STAGE_BYTES;
   constexpr bool I8 = EPI == 7 || EPI == 8;
   constexpr int KB = I8 ? 2 * BK : BK;               // elements of a k block: 128 bytes of a row
   extern __shared__ uint8_t smem_raw[];
@@ -738,7 +895,7 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
   __shared__ __align__(8) uint64_t bar_full[MAX_STAGES], bar_empty[MAX_STAGES], bar_tfull[2], bar_tempty[2];
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
-  __shared__ __align__(8) uint64_t bar_gu[EPI == 5 ? 8 : 1];      // EPI 5: two per epilogue warp
+  __shared__ __align__(8) uint64_t bar_gu[EPI == 5 || EPI == 10 ? 8 : 1];      // EPI 5 and 10: two per epilogue warp
   __shared__ uint32_t s_ready[32];   // gather: bit c set once chunk c was seen ready (1024 chunks)
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
@@ -761,7 +918,7 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
       mbar_init(smem_u32(&bar_empty[s]), 1);
     }
     for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&bar_tfull[s]), 1); mbar_init(smem_u32(&bar_tempty[s]), 8); }
-    if (EPI == 5)
+    if (EPI == 5 || EPI == 10)
       for (int s = 0; s < 8; ++s) mbar_init(smem_u32(&bar_gu[s]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -813,7 +970,7 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
           const int kb0 = w.kb0;
           const int k_blocks = w.nkb;
           const int m0 = tm * TILE_M + (int)cr * CTA_M;
-          const int n0 = EPI == 3 ? tn * cta_n + (int)cr * p.swiglu_f : tn * tile_n + (int)cr * cta_n;
+          const int n0 = EPI == 3 || EPI == 9 ? tn * cta_n + (int)cr * p.swiglu_f : tn * tile_n + (int)cr * cta_n;
           if (p.ag_operand == 1 && !A_MN) ok = rows_ready_warp(m0, CTA_M);
           if (p.ag_operand == 2 && !B_MN) ok = ok && rows_ready_warp(n0, cta_n);
           for (int kb = 0; kb < k_blocks && ok; ++kb, ++it) {
@@ -902,6 +1059,8 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
       uint32_t tile_i = 0, n_boxes = 0;
       GuLoads gl = {};
       if (EPI == 5) gl = {smem_u32(&bar_gu[EPI == 5 ? 2 * quad : 0]), sEpi + (uint32_t)quad * 16384u, 0u, 0u};
+      CodeLoads cl = {};
+      if (EPI == 10) cl = {smem_u32(&bar_gu[EPI == 10 ? 2 * quad : 0]), sEpi + (uint32_t)quad * 16384u, 0u, 0u, 0.f, 0.f};
       bool ok = true;
       Work w;
       work_init(p, w, pair);
@@ -911,6 +1070,7 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
         const int m0 = tm * TILE_M + (int)cr * CTA_M, n0 = tn * tile_n;
         const uint32_t acc = tile_i & 1, acc_ph = (tile_i >> 1) & 1;
         if (EPI == 5 && m0 + quad * 32 < p.M && n0 < p.swiglu_f) gu_issue(p, gl, lane, n0, m0 + quad * 32);   // while the main loop runs
+        if (EPI == 10 && m0 + quad * 32 < p.M && n0 < p.swiglu_f) codes_issue(p, cl, lane, n0, m0 + quad * 32);
         ok = mbar_wait(smem_u32(&bar_tfull[acc]), acc_ph, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -918,6 +1078,8 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
         const uint32_t tmem_acc = tmem_base + acc * TILE_N;
         if (EPI == 3)      epilogue_swiglu(p, tmem_acc, quad, lane, m0, tn, sEpi + (uint32_t)quad * 8192u, n_boxes);
         else if (EPI == 5) { if (!(ok = epilogue_swiglu_bwd(p, tmem_acc, quad, lane, m0, n0, gl, abort_flag))) break; }
+        else if (EPI == 9) epilogue_swiglu_q8(p, tmem_acc, quad, lane, m0, tn, sEpi + (uint32_t)quad * 8192u, n_boxes);
+        else if (EPI == 10) { if (!(ok = epilogue_swiglu_bwd_q8(p, tmem_acc, quad, lane, m0, n0, cl, sEpi + (uint32_t)quad * 16384u + 8192u, n_boxes, abort_flag))) break; }
         else if (EPI == 6) epilogue_attn_dout(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
         else if (EPI == 4 && p.rope_dh == 128 && p.rope_cols % 128 == 0)
           epilogue_rope<128>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
@@ -934,6 +1096,10 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
       if (EPI == 5) {
         Drain drain;
         for (; gl.used < gl.issued; ++gl.used) drain.wait(gl.bar + 8u * (gl.used & 1u), (gl.used >> 1) & 1u);
+      }
+      if (EPI == 10) {
+        Drain drain;
+        for (; cl.used < cl.issued; ++cl.used) drain.wait(cl.bar + 8u * (cl.used & 1u), (cl.used >> 1) & 1u);
       }
       if (lane == 0) {
         bulk_wait0();                // staging buffers are read out and the stores / reductions are performed
@@ -1022,7 +1188,7 @@ int launch2(Gemm2Params& p, int n_comm_pairs, int max_pairs, cudaStream_t st) {
   attr[1] = pdl_attr(p.world == 1);
   cfg.attrs = attr; cfg.numAttrs = 2;
   // all CTAs must be resident at once: compute CTAs wait for comm CTAs of the same launch
-  static int max_clusters[2][2][9] = {};
+  static int max_clusters[2][2][11] = {};
   int& mc = max_clusters[A_MN][B_MN][EPI];
   if (mc == 0) {
     cfg.gridDim = dim3(2 * (tplr_sm_count() / 2));
@@ -1052,7 +1218,7 @@ int dispatch2(Gemm2Params& p, int a_mn, int b_mn, int epi, int n_comm_pairs, int
   TPLR_GEMM2_CASE(1, 1, 0) TPLR_GEMM2_CASE(1, 1, 1) TPLR_GEMM2_CASE(1, 1, 2)
   TPLR_GEMM2_CASE(1, 0, 0) TPLR_GEMM2_CASE(1, 0, 1) TPLR_GEMM2_CASE(1, 0, 2)
   TPLR_GEMM2_CASE(0, 0, 3) TPLR_GEMM2_CASE(0, 0, 4) TPLR_GEMM2_CASE(0, 1, 5) TPLR_GEMM2_CASE(0, 1, 6)
-  TPLR_GEMM2_CASE(0, 0, 7) TPLR_GEMM2_CASE(0, 0, 8)
+  TPLR_GEMM2_CASE(0, 0, 7) TPLR_GEMM2_CASE(0, 0, 8) TPLR_GEMM2_CASE(0, 0, 9) TPLR_GEMM2_CASE(0, 1, 10)
 #undef TPLR_GEMM2_CASE
   return -104;
 }
@@ -1350,6 +1516,42 @@ TPLR_API int tplr_gemm2_swiglu_bwd(const void* dY, const void* W2, const void* G
   if (!make_map(&p.tmGU, GU, 2LL * F, M, ldgu, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, false)) return -110;
   p.swiglu_f = F;
   return dispatch2(p, 0, 1, 5, 0, 0, (cudaStream_t)stream);
+}
+
+// tplr_gemm2_swiglu with the packed projection kept in 8 bits instead of in bf16: Q [M, 2F] codes (rows of ldq bytes, a multiple of 16) and
+// scale[group * ld_scale + row], F / 64 groups of the gate values, then as many of the up values (see epilogue_swiglu_q8).  -111: shapes or
+// alignment that this entry does not take.
+TPLR_API int tplr_gemm2_swiglu_saved8(const void* X, const void* W, void* Q, float* scale, void* H, int M, int F, int K, long long ldx,
+                                      long long ldw, long long ldq, long long ld_scale, long long ldh, unsigned int* status, void* stream) {
+  TPLR_ENTER();
+  if (M <= 0 || F <= 0 || K <= 0) return 0;
+  if (F % CTA_N || (((uintptr_t)Q | (uintptr_t)H) & 15) || (ldq % 16) || (ldh % 8)) return -111;
+  Gemm2Params p = {};
+  if (int r = fill_common(p, X, W, nullptr, M, 2 * F, K, ldx, ldw, ldh, 0, 0, 0, status, pick_tile(M, 2 * F, K, false, false, 3, 1, 128))) return r;
+  if (!make_map_u8(&p.tmC, Q, 2LL * F, M, ldq, 64, 32, CU_TENSOR_MAP_SWIZZLE_64B)) return -110;
+  if (!make_map(&p.tmCr[0], H, F, M, ldh, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, false)) return -110;
+  p.swiglu_f = F;
+  p.q8_scale = scale; p.q8_ld = ld_scale;
+  return dispatch2(p, 0, 0, 9, 0, 0, (cudaStream_t)stream);
+}
+
+// tplr_gemm2_swiglu_bwd from the projection kept in 8 bits by tplr_gemm2_swiglu_saved8, which also writes the activation
+// H[M, F] = silu(gate) * up of the kept values (see epilogue_swiglu_bwd_q8).  -111 when this entry does not take the arguments.
+TPLR_API int tplr_gemm2_swiglu_bwd_saved8(const void* dY, const void* W2, const void* Q, const float* scale, void* dGU, void* H, int M, int F,
+                                          int K, long long lddy, long long ldw2, long long ldq, long long ld_scale, long long lddgu,
+                                          long long ldh, unsigned int* status, void* stream) {
+  TPLR_ENTER();
+  if (M <= 0 || F <= 0 || K <= 0) return 0;
+  if (F % 64 || (((uintptr_t)Q | (uintptr_t)H | (uintptr_t)dGU) & 15) || (ldq % 16) || (ldh % 8) || (lddgu % 8)) return -111;
+  Gemm2Params p = {};
+  if (int r = fill_common(p, dY, W2, dGU, M, F, K, lddy, ldw2, lddgu, 0, 1, 0, status, pick_tile(M, F, K, false, true, 5))) return r;
+  if (!p.c_tma) return -111;
+  if (!make_map(&p.tmC, dGU, 2LL * F, M, lddgu, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, false)) return -110;
+  if (!make_map(&p.tmCr[0], H, F, M, ldh, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, false)) return -110;
+  if (!make_map_u8(&p.tmGU, Q, 2LL * F, M, ldq, 64, 32, CU_TENSOR_MAP_SWIZZLE_64B)) return -110;
+  p.swiglu_f = F;
+  p.q8_scale = const_cast<float*>(scale); p.q8_ld = ld_scale;
+  return dispatch2(p, 0, 1, 10, 0, 0, (cudaStream_t)stream);
 }
 
 // dO[M, N] = dY Wo (dY [M, K] bf16 K-major, Wo [K, N] bf16 with N contiguous: the attention output projection's weight

@@ -5,21 +5,13 @@
 // with IEEE division, in fp32.  A group below 2^-100 (127 / a would overflow not far below) is zero with scale zero; a group with a
 // member that is not finite has scale NaN and q zero, so that all that is made of it is NaN and nothing is hidden.  Magnitudes are
 // compared by their bits, where NaN is above infinity and both above every number.
-#include "common.cuh"
+#include "quant.cuh"
 
 namespace {
 typedef __nv_bfloat16 bf16;
 typedef long long ll;
 
-struct Codes { float inv, scale; };
-__device__ __forceinline__ Codes codes_of(uint32_t top) {
-  const float a = __uint_as_float(top);
-  if (top >= 0x7f800000u) return {0.f, __uint_as_float(0x7fc00000u)};
-  if (a < 0x1p-100f) return {0.f, 0.f};
-  return {127.f / a, a / 127.f};
-}
-__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-// x * inv is at most 127 (1 + 2^-23): it never rounds to 128; what is not finite converts to 0
+// what is not finite converts to 0
 __device__ __forceinline__ int code(float x, float inv) { return __float2int_rn(x * inv); }
 
 // ------------------------------------------------------------------------------------------ rows -> 8 bits
@@ -30,7 +22,7 @@ enum Mode {
   NORM_SAVED = 3,    // h = a + b, y = h * rstd * w in bf16, rows h * rstd with a scale for every 64 columns, rstd
   SWIGLU_ROWS = 4,   // a: bf16 [gate | up] rows of 2 D, rows silu(gate) * up, one scale a row
 };
-constexpr int GROUP = 64;
+constexpr int GROUP = QUANT_GROUP;
 
 struct RowsArgs {
   const bf16 *a, *b, *w;
@@ -117,21 +109,11 @@ __device__ __forceinline__ bf16x8 pack8(const float* f) {
   for (int i = 0; i < 4; ++i) p.v[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
   return p;
 }
-__device__ __forceinline__ uint2 codes8(const float* x, float inv) {
-  uint2 r = make_uint2(0, 0);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    r.x |= (uint32_t)(code(x[i], inv) & 255) << (8 * i);
-    r.y |= (uint32_t)(code(x[4 + i], inv) & 255) << (8 * i);
-  }
-  return r;
-}
+__device__ __forceinline__ uint2 codes8(const float* x, float inv) { return make_uint2(codes4(x, inv), codes4(x + 4, inv)); }
 __device__ __forceinline__ void values8(const uint2& q, float scale, float* f) {
+  numbers4(q.x, f); numbers4(q.y, f + 4);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[i] = (float)(int8_t)(q.x >> (8 * i)) * scale;
-    f[4 + i] = (float)(int8_t)(q.y >> (8 * i)) * scale;
-  }
+  for (int i = 0; i < 8; ++i) f[i] *= scale;
 }
 
 // The same from registers, for rows of whole 16-byte pieces: `tpr` threads (a power of two) share a row, VPL pieces each, so a row is

@@ -1,0 +1,32 @@
+// Values in 8 bits: what the kernels that write codes and those that read them share (the format is described in quant.cu).
+#pragma once
+#include "common.cuh"
+
+constexpr int QUANT_GROUP = 64;      // columns that share a scale in what a backward pass reads
+
+struct Codes { float inv, scale; };
+// From the bits of a group's largest magnitude.
+static __device__ __forceinline__ Codes codes_of(uint32_t top) {
+  const float a = __uint_as_float(top);
+  if (top >= 0x7f800000u) return {0.f, __uint_as_float(0x7fc00000u)};
+  if (a < 0x1p-100f) return {0.f, 0.f};
+  return {127.f / a, a / 127.f};
+}
+static __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// Four codes in a word.  Added to 1.5 * 2^23, a number's last bits are its nearest whole number (ties to even, as rint) in two's
+// complement: conversion instructions run at a sixteenth of the rate.  |x * inv| is at most 127 (1 + 2^-23) and never rounds to
+// 128.  Multiplied and added one after the other: a fused sum would round ties of x * inv another way than rint(x * inv).
+static __device__ __forceinline__ uint32_t codes4(const float* x, float inv) {
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inv), 12582912.f));
+  const uint32_t w = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+  return inv != 0.f ? w : 0u;        // a group that is not finite has codes of zero
+}
+// The codes of a word as numbers: byte b + 128 in the last place of 2^23.
+static __device__ __forceinline__ void numbers4(uint32_t w, float* f) {
+  w ^= 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | i)) - 8388736.f;
+}

@@ -544,6 +544,15 @@ class _FeedForward(torch.autograd.Function):
         return dx, dw13, dw2, None, None
 
 
+def _feed_forward_fused(x2, w13, w2) -> bool:
+    """Whether both projections run on the own GEMM with the activation and its backward in their epilogues."""
+    Fd = w13.shape[0] // 2
+    return (FUSED_PROJECTIONS and _GEMM_BACKEND == "tcgen05_2sm" and _native_ok(x2, w13, w2) and x2.dtype == torch.bfloat16
+            and Fd % 128 == 0 and x2.is_contiguous() and w13.stride(1) == 1 and w2.stride(1) == 1 and w13.stride(0) % 8 == 0
+            and w2.stride(0) % 8 == 0 and x2.shape[1] % 8 == 0 and w2.shape[0] % 8 == 0 and w13.shape[1] == x2.shape[1]
+            and w2.shape[1] == Fd and _aligned(x2, w13, w2))
+
+
 def feed_forward(x, w13, w2, main_grad13=None, main_grad2=None):
     """``(silu(x w1^T) * (x w3^T)) w2^T`` for the packed ``w13 = [w1; w3]`` ([2F, D]) and ``w2`` [D, F]."""
     if main_grad13 is None:
@@ -552,10 +561,7 @@ def feed_forward(x, w13, w2, main_grad13=None, main_grad2=None):
         main_grad2 = getattr(w2, "main_grad", None)
     Fd = w13.shape[0] // 2
     x2 = x.reshape(-1, x.shape[-1])
-    if (FUSED_PROJECTIONS and _GEMM_BACKEND == "tcgen05_2sm" and _native_ok(x2, w13, w2) and x.dtype == torch.bfloat16
-            and Fd % 128 == 0 and x2.is_contiguous() and w13.stride(1) == 1 and w2.stride(1) == 1 and w13.stride(0) % 8 == 0
-            and w2.stride(0) % 8 == 0 and x2.shape[1] % 8 == 0 and w2.shape[0] % 8 == 0 and w13.shape[1] == x2.shape[1]
-            and w2.shape[1] == Fd and _aligned(x2, w13, w2)):
+    if _feed_forward_fused(x2, w13, w2):
         if not torch.is_grad_enabled():          # nothing will ask for the packed projection: it is not stored
             h = torch.empty(x2.shape[0], Fd, dtype=x.dtype, device=x.device)
             native.check(native.lib().tplr_gemm2_swiglu(x2.data_ptr(), w13.data_ptr(), None, h.data_ptr(), x2.shape[0], Fd,

@@ -114,6 +114,8 @@ def _declare(L: ctypes.CDLL) -> None:
         "tplr_swiglu_q8": [vp, ll, vp, ll, vp, ll, i, vp],
         "tplr_gemm_q8": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, i, vp, vp],
         "tplr_gemm_q8_stream": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, i, vp, vp],
+        "tplr_gemm2_swiglu_saved8": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, ll, ll, vp, vp],
+        "tplr_gemm2_swiglu_bwd_saved8": [vp, vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, ll, ll, ll, vp, vp],
         "tplr_gemm2_q8": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, i, vp, vp],
         "tplr_add_rmsnorm_saved8": [vp, vp, vp, vp, vp, vp, ll, vp, ll, ll, vp, ll, i, f, vp],
         "tplr_rmsnorm_saved8_parts": [ll, i],

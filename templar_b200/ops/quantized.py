@@ -397,8 +397,18 @@ class _FeedForwardSaved8(torch.autograd.Function):
         x2 = x.reshape(-1, x.shape[-1])
         T, Fd = x2.shape[0], w13.shape[0] // 2
         ctx.native = _native_rows(x, w13, w2)
-        gu = OF.gemm(x2, w13, out_dtype=torch.float32) if ctx.native else x2.float() @ w13.float().t()
-        if ctx.native:
+        ctx.fused = OF._feed_forward_fused(x2, w13, w2)
+        gu = None
+        if not ctx.fused:
+            gu = OF.gemm(x2, w13, out_dtype=torch.float32) if ctx.native else x2.float() @ w13.float().t()
+        if ctx.fused:                 # activation and codes in the projection's epilogue
+            act = torch.empty(T, Fd, dtype=x.dtype, device=x.device)
+            q, scale = _empty_halves(T, Fd, x.device)
+            native.check(native.lib().tplr_gemm2_swiglu_saved8(x2.data_ptr(), w13.data_ptr(), q.data_ptr(), scale.data_ptr(), act.data_ptr(),
+                                                               T, Fd, x2.shape[1], x2.stride(0), w13.stride(0), q.stride(0),
+                                                               scale.stride(1), Fd, OF.status_word(x.device).data_ptr(),
+                                                               native.stream_ptr()), "gemm2_swiglu_saved8")
+        elif ctx.native:
             act = torch.empty(T, Fd, dtype=x.dtype, device=x.device)
             q, scale = _empty_halves(T, Fd, x.device)
             native.check(native.lib().tplr_swiglu_saved8(gu.data_ptr(), act.data_ptr(), q.data_ptr(), q.stride(0), scale.data_ptr(),
@@ -420,8 +430,19 @@ class _FeedForwardSaved8(torch.autograd.Function):
         mg13, mg2 = ctx.mg
         dy2 = dy.reshape(-1, dy.shape[-1]).contiguous()
         T, Fd = dy2.shape[0], w13.shape[0] // 2
-        dact = OF.gemm(dy2, w2, b_mn=True, out_dtype=torch.float32) if ctx.native else dy2.float() @ w2.float()
-        if ctx.native:
+        dact = None
+        if not ctx.fused:
+            dact = OF.gemm(dy2, w2, b_mn=True, out_dtype=torch.float32) if ctx.native else dy2.float() @ w2.float()
+        if ctx.fused:
+            dy2 = OF._dense(dy2)
+            dgu = torch.empty(T, 2 * Fd, dtype=dy.dtype, device=dy.device)
+            act = torch.empty(T, Fd, dtype=dy.dtype, device=dy.device)
+            native.check(native.lib().tplr_gemm2_swiglu_bwd_saved8(dy2.data_ptr(), w2.data_ptr(), q.data_ptr(), scale.data_ptr(), dgu.data_ptr(),
+                                                                   act.data_ptr(), T, Fd, dy2.shape[1], dy2.stride(0), w2.stride(0),
+                                                                   q.stride(0), scale.stride(1), 2 * Fd, Fd,
+                                                                   OF.status_word(dy.device).data_ptr(), native.stream_ptr()),
+                         "gemm2_swiglu_bwd_saved8")
+        elif ctx.native:
             dgu = torch.empty(T, 2 * Fd, dtype=dy.dtype, device=dy.device)
             act = torch.empty(T, Fd, dtype=dy.dtype, device=dy.device)
             native.check(native.lib().tplr_swiglu_saved8_bwd(dact.data_ptr(), q.data_ptr(), q.stride(0), scale.data_ptr(), scale.stride(0),
