@@ -41,7 +41,11 @@ constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_STAGE_BYTES + 1024;
 constexpr int EPI5_STAGES = STAGES - 1;            // the SwiGLU backward has a second pair of staging buffers per warp instead
 constexpr int MAX_STAGES = 8;                      // narrower tiles have smaller stages, so more of them fit the ring
 static_assert(4 * 8192 <= STAGE_BYTES, "the freed stage holds four warps' second pair");
-constexpr int NUM_THREADS = 192;
+// Warps that drain the accumulator: one a quadrant of tensor memory, or two where the epilogue is as long as the main loop of a short K,
+// so that one has instructions while the other waits.  What they stage beyond 32 KB takes a stage of the ring.
+constexpr int epi_warps(int epi) { return epi == 7 || epi == 8 || epi == 10 ? 8 : 4; }
+constexpr int num_threads(int epi) { return 64 + 32 * epi_warps(epi); }
+constexpr int ring_stages(int epi) { return epi == 5 || epi == 7 || epi == 8 || epi == 10 ? EPI5_STAGES : STAGES; }
 constexpr int MAX_RANKS = 8;
 constexpr int CHUNK_ROWS = 128;                    // gather / scatter flag granularity (rows)
 
@@ -656,7 +660,7 @@ __device__ __forceinline__ void epilogue_attn_dout(const Gemm2Params& p, uint32_
 // no TMA store (a row stride that is not a multiple of 16 bytes) a warp writes its staged box row by row, 32 columns of one row at a
 // time, since a lane that stores its own row touches 32 lines an instruction.
 template <bool F32>
-__device__ __forceinline__ void epilogue_q8(const Gemm2Params& p, uint32_t tmem_acc, int quad, int lane, int m0, int n0,
+__device__ __forceinline__ void epilogue_q8(const Gemm2Params& p, uint32_t tmem_acc, int quad, int turn, int lane, int m0, int n0,
                                             uint32_t stage_base, uint32_t& n_boxes) {
   constexpr int COLS = F32 ? 32 : 64;
   const int row0 = m0 + quad * 32;
@@ -664,7 +668,7 @@ __device__ __forceinline__ void epilogue_q8(const Gemm2Params& p, uint32_t tmem_
   const uint32_t lane_sel = (uint32_t)(quad * 32) << 16;
   const float sr = p.q8_row[min(row0 + lane, p.M - 1)];
 #pragma unroll 1
-  for (int c = 0; c < p.tile_n / COLS; ++c) {
+  for (int c = turn; c < p.tile_n / COLS; c += 2) {
     const int col0 = n0 + c * COLS;
     if (col0 >= p.N) break;                          // warp-uniform
     const uint32_t buf = box_begin(lane, stage_base, n_boxes);
@@ -786,25 +790,34 @@ __device__ __forceinline__ void epilogue_swiglu_q8(const Gemm2Params& p, uint32_
 }
 
 // Backward of the SwiGLU on the down projection's data gradient from the projection kept in 8 bits (EPI 10): as
-// epilogue_swiglu_bwd, with g and u as boxes of 32 rows x 64 codes (a quarter of that epilogue's loads), and the activation
-// s * g * u formed again as a third output for the down projection's weight gradient, which no pass stored.  The 64 columns' three outputs wait
-// packed in registers for the two buffers of the warp: the codes are read, and each exponential taken, once.
-// 16384 x 2048 -> 8192: XX us, where the bf16 form takes XX and forms no activation.
+// epilogue_swiglu_bwd, with g and u as boxes of 32 rows x 64 codes (half the bytes of that epilogue's loads), and the activation
+// s * g * u formed again as a third output for the down projection's weight gradient, which no pass stored.  The two warps of a
+// quadrant share a box of codes and the three boxes that leave, half the columns each: the first one's first lane moves them.
+// One warp a quadrant that did both halves was the longest part of the kernel (4096 x 2048 -> 8192: 128 us, the tensor pipe busy
+// for 55 % of them); with boxes of 32 columns for each warp alone the stores' 64-byte pieces were (16384 rows: 539 -> 670 us).
+// 16384 x 2048 -> 8192: XX us, the bf16 form 450 without the activation.
+constexpr uint32_t CODE_STAGE = 4096 + 3 * 4096;     // a quadrant's codes of 64 columns, gate and up; three boxes of 64 columns
 struct CodeLoads {
-  uint32_t bar;                      // two mbarriers of this warp
-  uint32_t base;                     // two pairs of 2 KB buffers
-  uint32_t issued, used;             // box pairs asked for and consumed so far
-  float sg, su;                      // scales of this lane's row in the pair asked for last
+  uint32_t bar;                      // the quadrant's mbarrier
+  uint32_t base;                     // its CODE_STAGE bytes
+  uint32_t issued, used;             // boxes of codes asked for and consumed so far, the same in both warps
+  float sg, su;                      // scales of this lane's row in the box asked for last
 };
-__device__ __forceinline__ void codes_issue(const Gemm2Params& p, CodeLoads& L, int lane, int f0, int row0) {
+__device__ __forceinline__ void quadrant_sync(int quad) { asm volatile("bar.sync %0, 64;" ::"r"(quad + 1) : "memory"); }
+// Both warps of a quadrant leave with one answer: neither waits at a barrier for another that has given up.
+__device__ __forceinline__ bool quadrant_agrees(bool ok, int quad, int lane, volatile int* given_up) {
+  if (!ok && lane == 0) given_up[quad] = 1;
+  quadrant_sync(quad);
+  return given_up[quad] == 0;
+}
+__device__ __forceinline__ void codes_issue(const Gemm2Params& p, CodeLoads& L, bool mover, int lane, int f0, int row0) {
   const long long row = min(row0 + lane, p.M - 1);
   L.sg = p.q8_scale[(long long)(f0 / QUANT_GROUP) * p.q8_ld + row];
   L.su = p.q8_scale[(long long)((p.swiglu_f + f0) / QUANT_GROUP) * p.q8_ld + row];
-  if (lane == 0) {
-    const uint32_t s = L.issued & 1u, bar = L.bar + 8u * s, buf = L.base + s * 4096u;
-    mbar_expect_tx(bar, 4096);
-    tma_load_2d(buf, &p.tmGU, bar, f0, row0);
-    tma_load_2d(buf + 2048u, &p.tmGU, bar, p.swiglu_f + f0, row0);
+  if (mover) {
+    mbar_expect_tx(L.bar, 4096);
+    tma_load_2d(L.base, &p.tmGU, L.bar, f0, row0);
+    tma_load_2d(L.base + 2048u, &p.tmGU, L.bar, p.swiglu_f + f0, row0);
   }
   ++L.issued;
 }
@@ -812,70 +825,68 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ void box_words(uint32_t buf, int lane, const uint32_t* w) {
-  const uint32_t rowaddr = buf + (uint32_t)lane * 128u, sw = (uint32_t)(lane & 7);
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + (((uint32_t)j ^ sw) << 4)), "r"(w[4 * j]), "r"(w[4 * j + 1]),
-                 "r"(w[4 * j + 2]), "r"(w[4 * j + 3]) : "memory");
-}
-__device__ __forceinline__ bool epilogue_swiglu_bwd_q8(const Gemm2Params& p, uint32_t tmem_acc, int quad, int lane, int m0, int n0,
-                                                       CodeLoads& L, uint32_t stage_base, uint32_t& n_boxes, volatile int* abort_flag) {
+__device__ __forceinline__ bool epilogue_swiglu_bwd_q8(const Gemm2Params& p, uint32_t tmem_acc, int quad, int turn, int lane, int m0, int n0,
+                                                       CodeLoads& L, volatile int* given_up, volatile int* abort_flag) {
   const int row0 = m0 + quad * 32;
-  if (row0 >= p.M || n0 >= p.swiglu_f) return true;  // warp-uniform; nothing was asked for
-  const uint32_t lane_sel = (uint32_t)(quad * 32) << 16;
+  if (row0 >= p.M || n0 >= p.swiglu_f) return true;  // the same in both warps; nothing was asked for
+  const bool mover = turn == 0 && lane == 0;
+  const uint32_t acc = tmem_acc + turn * 32 + ((uint32_t)(quad * 32) << 16);
+  const uint32_t grow = box64_row(L.base, lane), out = L.base + 4096u, orow = out + (uint32_t)lane * 128u;
 #pragma unroll 1
   for (int c = 0; c < p.tile_n / 64; ++c) {
     const int f0 = n0 + c * 64;
-    if (f0 >= p.swiglu_f) break;                     // warp-uniform (swiglu_f is a multiple of 64)
+    if (f0 >= p.swiglu_f) break;                     // swiglu_f is a multiple of 64
     const float sg = L.sg, su = L.su;
-    if (c + 1 < p.tile_n / 64 && f0 + 64 < p.swiglu_f) codes_issue(p, L, lane, f0 + 64, row0);
-    const uint32_t s = L.used & 1u;
-    const bool ok = mbar_wait(L.bar + 8u * s, (L.used >> 1) & 1u, abort_flag);
-    if (!__all_sync(0xffffffffu, ok)) return false;
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(L.bar, L.used & 1u, abort_flag));
     ++L.used;
-    const uint32_t grow = box64_row(L.base + s * 4096u, lane), urow = grow + 2048u;
-    uint32_t dg[32], du[32], act[32];
+    uint32_t gw[8], uw[8], r[32];
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      uint32_t r[32];
-      tmem_ld32(tmem_acc + c * 64 + hh * 32 + lane_sel, r);
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int j = hh * 2 + q;                    // 16 columns
-        uint32_t gw[4], uw[4];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(gw[0]), "=r"(gw[1]), "=r"(gw[2]), "=r"(gw[3]) : "r"(grow + box64_at(lane, j)) : "memory");
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(uw[0]), "=r"(uw[1]), "=r"(uw[2]), "=r"(uw[3]) : "r"(urow + box64_at(lane, j)) : "memory");
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          float g[4], u[4], a[4];
-          numbers4(gw[w], g); numbers4(uw[w], u);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float dh = __uint_as_float(r[q * 16 + w * 4 + e]);
-            const float gv = g[e] * sg, uv = u[e] * su;
-            const float sig = __fdividef(1.f, 1.f + __expf(-gv)), silu = gv * sig;
-            a[e] = silu * uv;
-            g[e] = dh * uv * (sig + silu * (1.f - sig));
-            u[e] = dh * silu;
-          }
-          const int at = j * 8 + w * 2;
-          dg[at] = pack2(g[0], g[1]); dg[at + 1] = pack2(g[2], g[3]);
-          du[at] = pack2(u[0], u[1]); du[at + 1] = pack2(u[2], u[3]);
-          act[at] = pack2(a[0], a[1]); act[at + 1] = pack2(a[2], a[3]);
-        }
-      }
+    for (int q = 0; q < 2; ++q) {
+      const uint32_t at = grow + box64_at(lane, turn * 2 + q);
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(gw[4 * q]), "=r"(gw[4 * q + 1]), "=r"(gw[4 * q + 2]), "=r"(gw[4 * q + 3]) : "r"(at) : "memory");
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(uw[4 * q]), "=r"(uw[4 * q + 1]), "=r"(uw[4 * q + 2]), "=r"(uw[4 * q + 3]) : "r"(at + 2048u) : "memory");
     }
-    __syncwarp();                                    // every lane has read its codes: their buffer may be asked for again
-    uint32_t buf = box_begin(lane, stage_base, n_boxes);
-    box_words(buf, lane, dg);
-    box_store(&p.tmC, buf, lane, n_boxes, f0, row0);
-    buf = box_begin(lane, stage_base, n_boxes);
-    box_words(buf, lane, du);
-    box_store(&p.tmC, buf, lane, n_boxes, p.swiglu_f + f0, row0);
-    buf = box_begin(lane, stage_base, n_boxes);
-    box_words(buf, lane, act);
-    box_store(&p.tmCr[0], buf, lane, n_boxes, f0, row0);
+    tmem_ld32(acc + c * 64, r);
+    uint32_t dg[16], du[16], act[16];
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      float g[4], u[4], a[4];
+      numbers4(gw[w], g); numbers4(uw[w], u);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float dh = __uint_as_float(r[w * 4 + e]);
+        const float gv = g[e] * sg, uv = u[e] * su;
+        const float sig = __fdividef(1.f, 1.f + __expf(-gv)), silu = gv * sig;
+        a[e] = silu * uv;
+        g[e] = dh * uv * (sig + silu * (1.f - sig));
+        u[e] = dh * silu;
+      }
+      dg[2 * w] = pack2(g[0], g[1]); dg[2 * w + 1] = pack2(g[2], g[3]);
+      du[2 * w] = pack2(u[0], u[1]); du[2 * w + 1] = pack2(u[2], u[3]);
+      act[2 * w] = pack2(a[0], a[1]); act[2 * w + 1] = pack2(a[2], a[3]);
+    }
+    if (mover) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");            // the last boxes are read out
+    __syncwarp();
+    // both warps have read their codes, and the boxes are free
+    if (!quadrant_agrees(ok, quad, lane, given_up)) return false;
+    if (c + 1 < p.tile_n / 64 && f0 + 64 < p.swiglu_f) codes_issue(p, L, mover, lane, f0 + 64, row0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t at = orow + (((uint32_t)(turn * 4 + j) ^ (uint32_t)(lane & 7)) << 4);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(dg[4 * j]), "r"(dg[4 * j + 1]), "r"(dg[4 * j + 2]), "r"(dg[4 * j + 3]) : "memory");
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + 4096u), "r"(du[4 * j]), "r"(du[4 * j + 1]), "r"(du[4 * j + 2]), "r"(du[4 * j + 3]) : "memory");
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + 8192u), "r"(act[4 * j]), "r"(act[4 * j + 1]), "r"(act[4 * j + 2]), "r"(act[4 * j + 3]) : "memory");
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    quadrant_sync(quad);
+    if (mover) {
+      tma_store_2d(&p.tmC, out, f0, row0);
+      tma_store_2d(&p.tmC, out + 4096u, p.swiglu_f + f0, row0);
+      tma_store_2d(&p.tmCr[0], out + 8192u, f0, row0);
+      bulk_commit();
+    }
+    __syncwarp();
   }
   return true;
 }
@@ -885,17 +896,17 @@ __device__ __forceinline__ bool epilogue_swiglu_bwd_q8(const Gemm2Params& p, uin
 // of the down projection, 6 data gradient of the attention output projection with the attention backward's delta term,
 // 7 / 8 product of 8-bit rows stored as bf16 / fp32, 9 as 3 with the projection kept in 8 bits, 10 as 5 from it
 template <bool A_MN, bool B_MN, int EPI>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+__global__ void __launch_bounds__(num_threads(EPI), 1)
 gemm2_kernel(const __grid_constant__ Gemm2Params p) {
-  constexpr int RING_BYTES = (EPI == 5 || EPI == 10 ? EPI5_STAGES : STAGES) * STAGE_BYTES;
+  constexpr int RING_BYTES = ring_stages(EPI) * STAGE_BYTES;
   constexpr bool I8 = EPI == 7 || EPI == 8;
   constexpr int KB = I8 ? 2 * BK : BK;               // elements of a k block: 128 bytes of a row
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t bar_full[MAX_STAGES], bar_empty[MAX_STAGES], bar_tfull[2], bar_tempty[2];
   __shared__ uint32_t s_tmem_base;
-  __shared__ int s_abort;
-  __shared__ __align__(8) uint64_t bar_gu[EPI == 5 || EPI == 10 ? 8 : 1];      // EPI 5 and 10: two per epilogue warp
+  __shared__ int s_abort, s_given_up[EPI == 10 ? 4 : 1];
+  __shared__ __align__(8) uint64_t bar_gu[EPI == 5 || EPI == 10 ? 8 : 1];      // EPI 5: two per epilogue warp, 10: one a quadrant
   __shared__ uint32_t s_ready[32];   // gather: bit c set once chunk c was seen ready (1024 chunks)
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
@@ -913,11 +924,12 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
 
   if (threadIdx.x == 0) {
     s_abort = 0;
+    for (int& g : s_given_up) g = 0;
     for (int s = 0; s < MAX_STAGES; ++s) {
       mbar_init(smem_u32(&bar_full[s]), 1);
       mbar_init(smem_u32(&bar_empty[s]), 1);
     }
-    for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&bar_tfull[s]), 1); mbar_init(smem_u32(&bar_tempty[s]), 8); }
+    for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&bar_tfull[s]), 1); mbar_init(smem_u32(&bar_tempty[s]), 2 * epi_warps(EPI)); }
     if (EPI == 5 || EPI == 10)
       for (int s = 0; s < 8; ++s) mbar_init(smem_u32(&bar_gu[s]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1054,13 +1066,13 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
         }
       }
     } else {
-      // ----------------------------- epilogue (warps 2..5 of both CTAs) --------------
-      const int quad = warp & 3;
+      // ----------------------------- epilogue (warps 2.. of both CTAs) ---------------
+      const int quad = warp & 3, turn = (warp - 2) >> 2;      // turn: 0, or 1 in the second warp of a quadrant
       uint32_t tile_i = 0, n_boxes = 0;
       GuLoads gl = {};
       if (EPI == 5) gl = {smem_u32(&bar_gu[EPI == 5 ? 2 * quad : 0]), sEpi + (uint32_t)quad * 16384u, 0u, 0u};
       CodeLoads cl = {};
-      if (EPI == 10) cl = {smem_u32(&bar_gu[EPI == 10 ? 2 * quad : 0]), sEpi + (uint32_t)quad * 16384u, 0u, 0u, 0.f, 0.f};
+      if (EPI == 10) cl = {smem_u32(&bar_gu[EPI == 10 ? quad : 0]), sEpi + (uint32_t)quad * CODE_STAGE, 0u, 0u, 0.f, 0.f};
       bool ok = true;
       Work w;
       work_init(p, w, pair);
@@ -1070,22 +1082,23 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
         const int m0 = tm * TILE_M + (int)cr * CTA_M, n0 = tn * tile_n;
         const uint32_t acc = tile_i & 1, acc_ph = (tile_i >> 1) & 1;
         if (EPI == 5 && m0 + quad * 32 < p.M && n0 < p.swiglu_f) gu_issue(p, gl, lane, n0, m0 + quad * 32);   // while the main loop runs
-        if (EPI == 10 && m0 + quad * 32 < p.M && n0 < p.swiglu_f) codes_issue(p, cl, lane, n0, m0 + quad * 32);
+        if (EPI == 10 && m0 + quad * 32 < p.M && n0 < p.swiglu_f) codes_issue(p, cl, turn == 0 && lane == 0, lane, n0, m0 + quad * 32);
         ok = mbar_wait(smem_u32(&bar_tfull[acc]), acc_ph, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
+        if (EPI == 10) ok = quadrant_agrees(ok, quad, lane, s_given_up);
         if (!ok) break;
         tcgen05_fence_after();
         const uint32_t tmem_acc = tmem_base + acc * TILE_N;
         if (EPI == 3)      epilogue_swiglu(p, tmem_acc, quad, lane, m0, tn, sEpi + (uint32_t)quad * 8192u, n_boxes);
         else if (EPI == 5) { if (!(ok = epilogue_swiglu_bwd(p, tmem_acc, quad, lane, m0, n0, gl, abort_flag))) break; }
         else if (EPI == 9) epilogue_swiglu_q8(p, tmem_acc, quad, lane, m0, tn, sEpi + (uint32_t)quad * 8192u, n_boxes);
-        else if (EPI == 10) { if (!(ok = epilogue_swiglu_bwd_q8(p, tmem_acc, quad, lane, m0, n0, cl, sEpi + (uint32_t)quad * 16384u + 8192u, n_boxes, abort_flag))) break; }
+        else if (EPI == 10) { if (!(ok = epilogue_swiglu_bwd_q8(p, tmem_acc, quad, turn, lane, m0, n0, cl, s_given_up, abort_flag))) break; }
         else if (EPI == 6) epilogue_attn_dout(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
         else if (EPI == 4 && p.rope_dh == 128 && p.rope_cols % 128 == 0)
           epilogue_rope<128>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
         else if (EPI == 4 && p.rope_dh == 64 && p.rope_cols % 64 == 0)
           epilogue_rope<64>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
-        else if (I8)       epilogue_q8<EPI == 8>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
+        else if (I8)       epilogue_q8<EPI == 8>(p, tmem_acc, quad, turn, lane, m0, n0, sEpi + (uint32_t)(warp - 2) * 8192u, n_boxes);
         else if (p.c_tma)  epilogue_tma<EPI>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes, w.t % p.k_splits);
         else               epilogue_direct<EPI>(p, tmem_acc, quad, lane, m0, n0);
         tcgen05_fence_before();
@@ -1099,7 +1112,7 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
       }
       if (EPI == 10) {
         Drain drain;
-        for (; cl.used < cl.issued; ++cl.used) drain.wait(cl.bar + 8u * (cl.used & 1u), (cl.used >> 1) & 1u);
+        for (; cl.used < cl.issued; ++cl.used) drain.wait(cl.bar, cl.used & 1u);
       }
       if (lane == 0) {
         bulk_wait0();                // staging buffers are read out and the stores / reductions are performed
@@ -1181,7 +1194,7 @@ int launch2(Gemm2Params& p, int n_comm_pairs, int max_pairs, cudaStream_t st) {
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(NUM_THREADS);
+  cfg.blockDim = dim3(num_threads(EPI));
   cfg.dynamicSmemBytes = SMEM_BYTES;
   cfg.stream = st;
   // not for the fused collectives: their CTAs wait for other ranks' kernels and start as one
@@ -1546,8 +1559,8 @@ TPLR_API int tplr_gemm2_swiglu_bwd_saved8(const void* dY, const void* W2, const 
   Gemm2Params p = {};
   if (int r = fill_common(p, dY, W2, dGU, M, F, K, lddy, ldw2, lddgu, 0, 1, 0, status, pick_tile(M, F, K, false, true, 5))) return r;
   if (!p.c_tma) return -111;
-  if (!make_map(&p.tmC, dGU, 2LL * F, M, lddgu, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, false)) return -110;
-  if (!make_map(&p.tmCr[0], H, F, M, ldh, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, false)) return -110;
+  if (!make_map(&p.tmC, dGU, 2LL * F, M, lddgu, 64, 32)) return -110;
+  if (!make_map(&p.tmCr[0], H, F, M, ldh, 64, 32)) return -110;
   if (!make_map_u8(&p.tmGU, Q, 2LL * F, M, ldq, 64, 32, CU_TENSOR_MAP_SWIZZLE_64B)) return -110;
   p.swiglu_f = F;
   p.q8_scale = const_cast<float*>(scale); p.q8_ld = ld_scale;
