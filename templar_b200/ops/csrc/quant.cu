@@ -38,7 +38,7 @@ struct RowsArgs {
   float eps;
 };
 
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + __expf(-g)) * u; }
+__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
 // One CTA a row, element by element: every width and alignment.
 template <int MODE>
@@ -170,6 +170,12 @@ __global__ void __launch_bounds__(BLOCK) rows_q8_kernel(const RowsArgs p, const 
     for (int j = 0; j < VPL; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss = fmaf(v[j][e], v[j][e], ss);
+    bf16x8 wp[VPL];
+    if (MODE == NORM_SAVED) {                                            // all asked for here: no load passes the stores below
+#pragma unroll
+      for (int j = 0; j < VPL; ++j)
+        if (t + tpr * j < nv) wp[j] = reinterpret_cast<const bf16x8*>(p.w)[t + tpr * j];
+    }
     ss = warp_sum(ss);
     if (warps > 1) {
       if (lane == 0) s_sum[warp] = ss;
@@ -182,9 +188,9 @@ __global__ void __launch_bounds__(BLOCK) rows_q8_kernel(const RowsArgs p, const 
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
       const int i = t + tpr * j;
-      if (i >= nv) continue;
+      if (!live || i >= nv) continue;
       float w[8];
-      unpack8(reinterpret_cast<const bf16x8*>(p.w)[i], w);
+      unpack8(MODE == NORM_SAVED ? wp[j] : reinterpret_cast<const bf16x8*>(p.w)[i], w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v[j][e] *= r;
@@ -193,7 +199,7 @@ __global__ void __launch_bounds__(BLOCK) rows_q8_kernel(const RowsArgs p, const 
       if (MODE == NORM_ROWS) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[j][e] = w[e];
-      } else if (live) {
+      } else {
         reinterpret_cast<bf16x8*>(p.y + row * D)[i] = pack8(w);
       }
     }
@@ -219,18 +225,26 @@ __global__ void __launch_bounds__(BLOCK) rows_q8_kernel(const RowsArgs p, const 
     all = codes_of(top);
     if (live && t == 0) p.scale[row * p.scale_row] = all.scale;
   }
+  if (BY_GROUP) {                                                        // eight lanes hold a group's 64 columns
+#pragma unroll
+    for (int j = 0; j < VPL; ++j)
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) tops[j] = max(tops[j], __shfl_xor_sync(0xffffffffu, tops[j], o));
+    // lane j of the eight divides for their j-th group
+    const int k = lane & 7;
+    uint32_t top = tops[0];
+#pragma unroll
+    for (int j = 1; j < VPL; ++j) top = k == j ? tops[j] : top;
+    all = codes_of(top);
+    const int i = t - k + tpr * k;
+    if (live && k < VPL && i < nv) p.scale[row * p.scale_row + (i >> 3) * p.scale_group] = all.scale;
+  }
 #pragma unroll
   for (int j = 0; j < VPL; ++j) {
     const int i = t + tpr * j;
-    Codes c = all;
-    if (BY_GROUP) {                                                      // eight lanes hold a group's 64 columns
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) tops[j] = max(tops[j], __shfl_xor_sync(0xffffffffu, tops[j], o));
-      c = codes_of(tops[j]);
-      if (live && (i & 7) == 0 && i < nv) p.scale[row * p.scale_row + (i >> 3) * p.scale_group] = c.scale;
-    }
+    const float inv = BY_GROUP ? __shfl_sync(0xffffffffu, all.inv, (lane & ~7) + j) : all.inv;
     if (live && (ll)i * 8 < p.ldq)                                       // zeros behind the row: v is 0 there
-      reinterpret_cast<uint2*>(p.q + row * p.ldq)[i] = codes8(v[j], i < nv ? c.inv : 0.f);
+      reinterpret_cast<uint2*>(p.q + row * p.ldq)[i] = codes8(v[j], i < nv ? inv : 0.f);
   }
 }
 
@@ -250,26 +264,43 @@ __global__ void __launch_bounds__(256) dequantize_any_kernel(const int8_t* q, ll
   }
 }
 
-// The same for whole 16-byte pieces of y and groups of whole pieces: eight columns a thread, `lanes` threads (a power of two) on a row.
-__global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* q, ll ldq, const float* scale, ll scale_row, ll scale_group, int group,
-                                                         const bf16* w, bf16* y, ll T, int D, int lanes) {
+// The same for whole 16-byte pieces of y, a scale for a row or for 64 columns: `tpr` threads (a power of two) on a row, four pieces each,
+// all asked for before the first is written.
+__global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* q, ll ldq, const float* scale, ll scale_row, ll scale_group,
+                                                         const bf16* w, bf16* y, ll T, int D, int tpr) {
   grid_wait();
   grid_release();
-  const int nv = D / 8, rows = 256 / lanes;
-  for (ll row = (ll)blockIdx.x * rows + threadIdx.x / lanes; row < T; row += (ll)gridDim.x * rows) {
-    const uint2* src = reinterpret_cast<const uint2*>(q + row * ldq);
-    const float* s = scale + row * scale_row;
-#pragma unroll 4
-    for (int i = threadIdx.x & (lanes - 1); i < nv; i += lanes) {
-      float f[8];
-      values8(src[i], s[i * 8 / group * scale_group], f);
-      if (w) {
-        float m[8];
-        unpack8(reinterpret_cast<const bf16x8*>(w)[i], m);
+  const int nv = D / 8, t = threadIdx.x & (tpr - 1);
+  const ll row = (ll)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
+  if (row >= T) return;
+  const uint2* src = reinterpret_cast<const uint2*>(q + row * ldq);
+  bf16x8* dst = reinterpret_cast<bf16x8*>(y + row * D);
+  for (int i0 = t; i0 < nv; i0 += 4 * tpr) {
+    uint2 c[4];
+    float s[4];
+    bf16x8 m[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= m[e];
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + tpr * j;
+      if (i < nv) {
+        c[j] = src[i];
+        s[j] = scale[row * scale_row + (i >> 3) * scale_group];
+        if (w) m[j] = reinterpret_cast<const bf16x8*>(w)[i];
       }
-      reinterpret_cast<bf16x8*>(y + row * D)[i] = pack8(f);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + tpr * j;
+      if (i >= nv) continue;
+      float f[8];
+      values8(c[j], s[j], f);
+      if (w) {
+        float g[8];
+        unpack8(m[j], g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= g[e];
+      }
+      dst[i] = pack8(f);
     }
   }
 }
@@ -303,55 +334,90 @@ __global__ void __launch_bounds__(256) rmsnorm_saved8_bwd_any_kernel(const bf16*
   }
 }
 
-// The same for whole 16-byte pieces: `tpr` threads on a row, VPL pieces each, the row in registers between its sum and its output, the weight
-// gradient's sums of a thread's columns in registers over all rows of the CTA.
-template <int VPL>
-__global__ void __launch_bounds__(256, VPL == 2 ? 3 : 2)
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory"); }
+
+// The same for whole 16-byte pieces: `tpr` threads on a row, VPL pieces each, the weight gradient's sums of a thread's columns in registers
+// over all rows of the CTA.  What keeps the memory busy are the copies of the two rows after the present one, each thread's own
+// pieces into its own shared memory, so that no barrier stands between them and their use.
+// Counters of a first form (16384 x 2048): the memory 45 % busy, an instruction issued in 72 % of the cycles; so the weight stays unpacked, the
+// products and the codes' numbers of a piece stay for its output, and a scale multiplies once a piece where it can, and the next row's scales are asked for a row ahead: 57 -> 47 us.
+constexpr int BWD_STAGES = 3, BWD_VPL = 2;
+template <int BLOCK>
+__global__ void __launch_bounds__(BLOCK, 512 / BLOCK)
 rmsnorm_saved8_bwd_kernel(const bf16* dy, const int8_t* q, ll ldq, const float* scale, ll scale_row, ll scale_group, const float* rstd, const bf16* w,
                           const bf16* dres, bf16* dx, float* part, ll T, int D, int tpr) {
-  __shared__ float s_dot[2][32];
-  __shared__ float s_dw[256 * 8];
+  constexpr int VPL = BWD_VPL, PIECE = 40 * BLOCK, STAGE = VPL * PIECE;
+  extern __shared__ uint8_t pieces[];        // [stage][piece][dy 16 | dres 16 | codes 8][thread]
+  __shared__ float s_dot[2][BLOCK / 32];
+  __shared__ float s_dw[BLOCK * 8];
   grid_wait();
   grid_release();
   const int t = threadIdx.x & (tpr - 1), slot = threadIdx.x / tpr, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nv = D / 8;
-  const int warps = tpr >> 5, rows = 256 / tpr;
-  bf16x8 wp[VPL];
-  float dw[VPL][8];
+  const int warps = tpr >> 5, rows = BLOCK / tpr;
+  const uint32_t mine16 = (uint32_t)__cvta_generic_to_shared(pieces) + threadIdx.x * 16u;
+  const uint32_t mine8 = (uint32_t)__cvta_generic_to_shared(pieces) + 32u * BLOCK + threadIdx.x * 8u;
+  float m[VPL][8], dw[VPL][8];
 #pragma unroll
   for (int j = 0; j < VPL; ++j) {
+    if (t + tpr * j < nv) unpack8(reinterpret_cast<const bf16x8*>(w)[t + tpr * j], m[j]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[j][e] = 0.f;
-    if (t + tpr * j < nv) wp[j] = reinterpret_cast<const bf16x8*>(w)[t + tpr * j];
   }
-  int turn = 0;
-  for (ll first = (ll)blockIdx.x * rows; first < T; first += (ll)gridDim.x * rows, turn ^= 1) {
-    const ll row = first + slot;
-    const bool live = row < T;
-    bf16x8 g[VPL], a[VPL];
-    uint2 c[VPL];
-    float sc[VPL];
+  auto ask = [&](ll row, int stage) {
+    if (row < T) {
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) {
-      const int i = t + tpr * j;
-      if (live && i < nv) {
-        g[j] = reinterpret_cast<const bf16x8*>(dy + row * D)[i];
-        c[j] = reinterpret_cast<const uint2*>(q + row * ldq)[i];
-        sc[j] = scale[row * scale_row + (i >> 3) * scale_group];
-        if (dres) a[j] = reinterpret_cast<const bf16x8*>(dres + row * D)[i];
+      for (int j = 0; j < VPL; ++j) {
+        const int i = t + tpr * j;
+        if (i < nv) {
+          const uint32_t at = stage * STAGE + j * PIECE;
+          copy16(mine16 + at, dy + row * D + i * 8);
+          if (dres) copy16(mine16 + at + 16 * BLOCK, dres + row * D + i * 8);
+          copy8(mine8 + at, q + row * ldq + i * 8);
+        }
       }
     }
-    const float r = live ? rstd[row] : 0.f;
-    float dot = 0.f;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  float sc2[VPL] = {}, r2 = 0.f;                                           // the next row's scales: their latency would be in every turn
+  auto ask_scales = [&](ll row) {
+    if (row >= T) return;
+    r2 = rstd[row];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j)
+      if (t + tpr * j < nv) sc2[j] = scale[row * scale_row + ((t + tpr * j) >> 3) * scale_group];
+  };
+  const ll step = (ll)gridDim.x * rows;
+  ask((ll)blockIdx.x * rows + slot, 0);
+  ask((ll)blockIdx.x * rows + slot + step, 1);
+  ask_scales((ll)blockIdx.x * rows + slot);
+  int turn = 0, stage = 0;
+  for (ll first = (ll)blockIdx.x * rows; first < T; first += step, turn ^= 1, stage = stage == BWD_STAGES - 1 ? 0 : stage + 1) {
+    const ll row = first + slot;
+    const bool live = row < T;
+    float sc[VPL];
+    const float r = r2;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) sc[j] = sc2[j];
+    ask_scales(row + step);
+    ask(row + 2 * step, stage == 0 ? 2 : stage - 1);
+    asm volatile("cp.async.wait_group 2;" ::: "memory");
+    float gm[VPL][8], x[VPL][8], dot = 0.f;
 #pragma unroll
     for (int j = 0; j < VPL; ++j)
       if (live && t + tpr * j < nv) {
-        float d[8], x[8], m[8];
-        unpack8(g[j], d); unpack8(wp[j], m); values8(c[j], sc[j], x);
+        const uint8_t* at = pieces + stage * STAGE + j * PIECE;
+        const uint2 c = reinterpret_cast<const uint2*>(at + 32 * BLOCK)[threadIdx.x];
+        float d[8], sum = 0.f;
+        unpack8(reinterpret_cast<const bf16x8*>(at)[threadIdx.x], d);
+        numbers4(c.x, x[j]); numbers4(c.y, x[j] + 4);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          dw[j][e] = fmaf(d[e], x[e], dw[j][e]);
-          dot = fmaf(d[e] * m[e], x[e], dot);
+          gm[j][e] = d[e] * m[j][e];
+          dw[j][e] = fmaf(d[e] * sc[j], x[j][e], dw[j][e]);
+          sum = fmaf(gm[j][e], x[j][e], sum);
         }
+        dot = fmaf(sum, sc[j], dot);
       }
     dot = warp_sum(dot);
     if (warps > 1) {                                                     // two buffers: one barrier a row
@@ -360,24 +426,28 @@ rmsnorm_saved8_bwd_kernel(const bf16* dy, const int8_t* q, ll ldq, const float* 
       dot = 0.f;
       for (int k = 0; k < warps; ++k) dot += s_dot[turn][slot * warps + k];
     }
-    dot /= (float)D;
+    dot *= r / (float)D;
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
       const int i = t + tpr * j;
       if (live && i < nv) {
-        float d[8], x[8], m[8], o[8];
-        unpack8(g[j], d); unpack8(wp[j], m); values8(c[j], sc[j], x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = r * (d[e] * m[e] - x[e] * dot);
+        const float k = dot * sc[j];
+        float o[8];
         if (dres) {
-          unpack8(a[j], d);
+          unpack8(reinterpret_cast<const bf16x8*>(pieces + stage * STAGE + j * PIECE + 16 * BLOCK)[threadIdx.x], o);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] += d[e];
+          for (int e = 0; e < 8; ++e) o[e] = fmaf(r, gm[j][e], o[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = r * gm[j][e];
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = fmaf(-k, x[j][e], o[e]);
         reinterpret_cast<bf16x8*>(dx + row * D)[i] = pack8(o);
       }
     }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   float* mine = part + (ll)blockIdx.x * D;
 #pragma unroll
   for (int j = 0; j < VPL; ++j) {
@@ -385,12 +455,12 @@ rmsnorm_saved8_bwd_kernel(const bf16* dy, const int8_t* q, ll ldq, const float* 
     if (rows > 1) {
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s_dw[e * 256 + threadIdx.x] = dw[j][e];
+      for (int e = 0; e < 8; ++e) s_dw[e * BLOCK + threadIdx.x] = dw[j][e];
       __syncthreads();
       if (slot == 0)
         for (int k = 1; k < rows; ++k)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) dw[j][e] += s_dw[e * 256 + k * tpr + t];
+          for (int e = 0; e < 8; ++e) dw[j][e] += s_dw[e * BLOCK + k * tpr + t];
     }
     if (slot == 0 && i < nv) {
       reinterpret_cast<float4*>(mine + i * 8)[0] = make_float4(dw[j][0], dw[j][1], dw[j][2], dw[j][3]);
@@ -400,18 +470,21 @@ rmsnorm_saved8_bwd_kernel(const bf16* dy, const int8_t* q, ll ldq, const float* 
 }
 
 // Sum of the CTAs' parts in their order, the same on every run: added into an fp32 buffer or stored in bf16.
-__global__ void __launch_bounds__(256) sum_parts_kernel(const float* part, int n, int D, float* add, bf16* out) {
-  __shared__ float s[8][33];
+__global__ void __launch_bounds__(1024) sum_parts_kernel(const float* part, int n, int D, float* add, bf16* out) {
+  __shared__ float s[32][33];
   grid_wait();
   grid_release();
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float v = 0.f;
-  if (c < D)
-    for (int k = slice; k < n; k += 8) v += part[(ll)k * D + c];
+  if (c < D) {
+#pragma unroll 8
+    for (int k = slice; k < n; k += 32) v += part[(ll)k * D + c];
+  }
   s[slice][lane] = v;
   __syncthreads();
   if (slice == 0 && c < D) {
-    for (int k = 1; k < 8; ++k) v += s[k][lane];
+#pragma unroll
+    for (int k = 1; k < 32; ++k) v += s[k][lane];
     if (add) add[c] += v;
     else out[c] = __float2bfloat16(v);
   }
@@ -612,11 +685,12 @@ TPLR_API int tplr_dequantize_rows(const void* q, ll ldq, const float* scale, ll 
   TPLR_ENTER();
   if (T <= 0) return 0;
   if (D <= 0 || group <= 0) return (int)cudaErrorInvalidValue;
-  if (D % 8 == 0 && ldq % 8 == 0 && (group % 8 == 0 || group >= D) && whole_pieces(q, w, y)) {
-    int lanes = 32;
-    while (lanes < 256 && lanes * 8 < D) lanes *= 2;
-    return (int)launch_pdl(dequantize_kernel, waves((T + 256 / lanes - 1) / (256 / lanes), 32), 256, 0, (cudaStream_t)stream, (const int8_t*)q,
-                           ldq, scale, scale_row, scale_group, group, (const bf16*)w, (bf16*)y, T, D, lanes);
+  if (D % 8 == 0 && ldq % 8 == 0 && (group == GROUP || group >= D) && T <= 0x7fffffffLL && whole_pieces(q, w, y)) {
+    int tpr = row_threads(D / 8, 4);
+    if (tpr > 256) tpr = 256;
+    const int rows = 256 / tpr;
+    return (int)launch_pdl(dequantize_kernel, (unsigned)((T + rows - 1) / rows), 256, 0, (cudaStream_t)stream, (const int8_t*)q, ldq, scale,
+                           scale_row, group >= D ? 0 : scale_group, (const bf16*)w, (bf16*)y, T, D, tpr);
   }
   return (int)launch_pdl(dequantize_any_kernel, waves((T * D + 255) / 256, 16), 256, 0, (cudaStream_t)stream, (const int8_t*)q, ldq, scale,
                          scale_row, scale_group, group, (const bf16*)w, (bf16*)y, T, D);
@@ -642,13 +716,15 @@ TPLR_API int tplr_rmsnorm_saved8_bwd(const void* dy, const void* q, ll ldq, cons
     n = (int)waves(T, 4);
     e = launch_pdl(rmsnorm_saved8_bwd_any_kernel, n, 256, 0, st, g, c, ldq, scale, scale_row, scale_group, rstd, wp, a, (bf16*)dx, part, T, D);
   } else {
-    const int vpl = D <= 4096 ? 2 : 4, tpr = row_threads(D / 8, vpl), rows = 256 / tpr;
-    n = (int)waves((T + rows - 1) / rows, vpl == 2 ? 3 : 2);
-    e = launch_pdl(vpl == 2 ? rmsnorm_saved8_bwd_kernel<2> : rmsnorm_saved8_bwd_kernel<4>, n, 256, 0, st, g, c, ldq, scale, scale_row, scale_group,
-                   rstd, wp, a, (bf16*)dx, part, T, D, tpr);
+    const int tpr = row_threads(D / 8, BWD_VPL), block = tpr > 256 ? 512 : 256, rows = block / tpr;
+    n = (int)waves((T + rows - 1) / rows, 512 / block);
+    auto kern = block == 512 ? rmsnorm_saved8_bwd_kernel<512> : rmsnorm_saved8_bwd_kernel<256>;
+    const size_t smem = (size_t)BWD_STAGES * BWD_VPL * 40 * block;
+    if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return (int)e;
+    e = launch_pdl(kern, n, block, smem, st, g, c, ldq, scale, scale_row, scale_group, rstd, wp, a, (bf16*)dx, part, T, D, tpr);
   }
   if (e != cudaSuccess || (!dw_add && !dw_out)) return (int)e;
-  return (int)launch_pdl(sum_parts_kernel, (D + 31) / 32, 256, 0, st, part, n, D, dw_add, (bf16*)dw_out);
+  return (int)launch_pdl(sum_parts_kernel, (D + 31) / 32, 1024, 0, st, part, n, D, dw_add, (bf16*)dw_out);
 }
 
 // The activation of a dense fp32 [gate | up] projection, and the projection in 8 bits (rows of ldq >= 2 F bytes) by 64 columns of each half.
