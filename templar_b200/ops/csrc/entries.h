@@ -32,4 +32,24 @@ int tplr_attention_bwd_scratch_cols(int B, int S, int H, int KV, int head_dim);
 int tplr_attention_bwd_unrope_delta(const void* qkv, const void* out, const void* dout, const float* lse, float* delta, float* dq32,
                                     void* dqkv, int B, int S, int H, int KV, int head_dim, long long ld_qkv, long long ld_o,
                                     float scale, const float* cosb, const float* sinb, unsigned int* status, void* stream);
+// rows in 8 bits
+int tplr_quantize_rows(const void* x, long long ldx, void* q, long long ldq, float* scale, long long scale_row, long long scale_group,
+                       long long T, int D, int group, void* stream);
+int tplr_dequantize_rows(const void* q, long long ldq, const float* scale, long long scale_row, long long scale_group, int group,
+                         const void* w, void* y, long long T, int D, void* stream);
+int tplr_add_rmsnorm_q8(const void* res, const void* delta, const void* w, void* h_out, void* q, long long ldq, float* scale, long long T,
+                        int D, float eps, void* stream);
+int tplr_add_rmsnorm_saved8(const void* res, const void* delta, const void* w, void* h_out, void* y, void* q, long long ldq, float* scale,
+                            long long scale_row, long long scale_group, float* rstd, long long T, int D, float eps, void* stream);
+int tplr_rmsnorm_saved8_parts(long long T, int D);
+int tplr_rmsnorm_saved8_bwd(const void* dy, const void* q, long long ldq, const float* scale, long long scale_row, long long scale_group,
+                            const float* rstd, const void* w, const void* dres, void* dx, float* part, float* dw_add, void* dw_out,
+                            long long T, int D, void* stream);
+int tplr_gemm_q8(const void* x, const void* w, const float* sx, const float* sw, void* y, int T, int N, int K, long long ldx, long long ldw,
+                 long long ldy, int out_fp32, unsigned int* status, void* stream);
+int tplr_gemm2_swiglu_saved8(const void* X, const void* W, void* Q, float* scale, void* H, int M, int F, int K, long long ldx, long long ldw,
+                             long long ldq, long long ld_scale, long long ldh, unsigned int* status, void* stream);
+int tplr_gemm2_swiglu_bwd_saved8(const void* dY, const void* W2, const void* Q, const float* scale, void* dGU, void* H, int M, int F, int K,
+                                 long long lddy, long long ldw2, long long ldq, long long ld_scale, long long lddgu, long long ldh,
+                                 unsigned int* status, void* stream);
 }

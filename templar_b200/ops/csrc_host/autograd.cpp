@@ -43,6 +43,15 @@ struct Entries {
   decltype(&tplr_gemm2_attn_dout) attn_dout;
   decltype(&tplr_attention_bwd_scratch_cols) bwd_scratch_cols;
   decltype(&tplr_attention_bwd_unrope_delta) attention_bwd;
+  decltype(&tplr_quantize_rows) quantize;
+  decltype(&tplr_dequantize_rows) dequantize;
+  decltype(&tplr_add_rmsnorm_q8) add_rmsnorm_q8;
+  decltype(&tplr_add_rmsnorm_saved8) add_rmsnorm_saved8;
+  decltype(&tplr_rmsnorm_saved8_parts) rmsnorm_saved8_parts;
+  decltype(&tplr_rmsnorm_saved8_bwd) rmsnorm_saved8_bwd;
+  decltype(&tplr_gemm_q8) gemm_q8;
+  decltype(&tplr_gemm2_swiglu_saved8) swiglu_saved8;
+  decltype(&tplr_gemm2_swiglu_bwd_saved8) swiglu_bwd_saved8;
 } E;
 
 void bind(const std::string& path) {
@@ -70,6 +79,15 @@ void bind(const std::string& path) {
   get(E.attn_dout, "tplr_gemm2_attn_dout");
   get(E.bwd_scratch_cols, "tplr_attention_bwd_scratch_cols");
   get(E.attention_bwd, "tplr_attention_bwd_unrope_delta");
+  get(E.quantize, "tplr_quantize_rows");
+  get(E.dequantize, "tplr_dequantize_rows");
+  get(E.add_rmsnorm_q8, "tplr_add_rmsnorm_q8");
+  get(E.add_rmsnorm_saved8, "tplr_add_rmsnorm_saved8");
+  get(E.rmsnorm_saved8_parts, "tplr_rmsnorm_saved8_parts");
+  get(E.rmsnorm_saved8_bwd, "tplr_rmsnorm_saved8_bwd");
+  get(E.gemm_q8, "tplr_gemm_q8");
+  get(E.swiglu_saved8, "tplr_gemm2_swiglu_saved8");
+  get(E.swiglu_bwd_saved8, "tplr_gemm2_swiglu_bwd_saved8");
 }
 
 void check(int err, const char* what) {
@@ -319,6 +337,195 @@ struct AttentionBlock : Function<AttentionBlock> {
   }
 };
 
+// ------------------------------------------------------------------------------------------ rows in 8 bits
+// The same calls as ops/quantized.py makes, for the operands that it hands here: bf16 CUDA tensors with contiguous columns.
+constexpr ll GROUP = 64;
+ll padded(ll n) { return (n + 15) / 16 * 16; }
+Tensor int8(at::IntArrayRef shape, const Tensor& like) { return at::empty(shape, like.options().dtype(at::kChar)); }
+// x as rows of D with contiguous columns
+Tensor dense_rows(const Tensor& x) {
+  Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+  return x2.stride(1) == 1 ? x2 : x2.contiguous();
+}
+// codes [T, D rounded up to 16] and scales [T, 1] or [T, groups]
+std::pair<Tensor, Tensor> quantize(const Tensor& x, int group) {
+  const Tensor x2 = dense_rows(x);
+  const ll T = x2.size(0), D = x2.size(1);
+  Tensor q = int8({T, padded(D)}, x), scale = f32({T, group ? (D + group - 1) / group : 1}, x);
+  check(E.quantize(x2.data_ptr(), x2.stride(0), q.data_ptr(), q.stride(0), scale.data_ptr<float>(), scale.stride(0), scale.stride(1), T,
+                   (int)D, group, stream()),
+        "quantize_rows");
+  return {q, scale};
+}
+// the values of codes, in bf16: `shape` is that of the result, w may be undefined
+Tensor dequantize(const Tensor& q, const Tensor& scale, ll group, at::IntArrayRef shape, const Tensor& w) {
+  const ll D = shape.back();
+  Tensor y = at::empty(shape, q.options().dtype(at::kBFloat16));
+  const Tensor wc = w.defined() ? w.contiguous() : w;
+  check(E.dequantize(q.data_ptr(), q.stride(0), scale.data_ptr<float>(), scale.stride(0), group ? scale.stride(1) : 0,
+                     (int)(group ? group : D), wc.defined() ? wc.data_ptr() : nullptr, y.data_ptr(), q.size(0), (int)D, stream()),
+        "dequantize_rows");
+  return y;
+}
+// x in 8 bits by rows, times an 8-bit weight; the codes live for this call alone, with their scales behind them
+Tensor linear_q8(const Tensor& x, const Tensor& wq, const Tensor& ws, const Tensor& status) {
+  const Tensor x2 = dense_rows(x);
+  const ll T = x2.size(0), K = x2.size(1), N = wq.size(0), ldq = padded(K);
+  auto shape = x.sizes().vec();
+  shape.back() = N;
+  Tensor y = bf16(shape, x);
+  Tensor codes = int8({T * (ldq + 4)}, x);
+  char* q = static_cast<char*>(codes.data_ptr());
+  float* scale = reinterpret_cast<float*>(q + T * ldq);
+  check(E.quantize(x2.data_ptr(), x2.stride(0), q, ldq, scale, 1, 1, T, (int)K, 0, stream()), "quantize_rows");
+  check(E.gemm_q8(q, wq.data_ptr(), scale, ws.data_ptr<float>(), y.data_ptr(), (int)T, (int)N, (int)K, ldq, wq.stride(0), N, 0, word(status),
+                  stream()),
+        "gemm_q8");
+  return y;
+}
+// rows of codes that are there already: sx one scale a row, dense
+Tensor linear_q8_rows(const Tensor& q, const Tensor& sx, at::IntArrayRef shape, const Tensor& wq, const Tensor& ws, const Tensor& status) {
+  auto out = shape.vec();
+  out.back() = wq.size(0);
+  Tensor y = at::empty(out, q.options().dtype(at::kBFloat16));
+  check(E.gemm_q8(q.data_ptr(), wq.data_ptr(), sx.data_ptr<float>(), ws.data_ptr<float>(), y.data_ptr(), (int)q.size(0), (int)wq.size(0),
+                  (int)shape.back(), q.stride(0), wq.stride(0), wq.size(0), 0, word(status), stream()),
+        "gemm_q8");
+  return y;
+}
+// codes [N, K] and scales [N] that the product takes as they are: rows, and every 16-byte piece of a row, inside the storage
+bool weight_as_it_is(const Tensor& q, const Tensor& scale) {
+  if (q.scalar_type() != at::kChar || q.dim() != 2 || scale.scalar_type() != at::kFloat || scale.dim() != 1 || q.device() != scale.device())
+    return false;
+  const ll N = q.size(0), K = q.size(1), ld = q.stride(0), wide = padded(K);
+  return K > 0 && K <= 131072 && scale.size(0) == N && q.stride(1) == 1 && ld % 16 == 0 && ld >= wide && scale.is_contiguous() &&
+         reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(scale.data_ptr()) % 16 == 0 &&
+         q.storage_offset() + (N - 1) * ld + wide <= (ll)q.storage().nbytes();
+}
+std::tuple<Tensor, Tensor, Tensor> add_rmsnorm_q8(const Tensor& res, const std::optional<Tensor>& delta, const Tensor& w, double eps) {
+  const Tensor x2 = rows(res).contiguous(), wc = w.contiguous(), d = delta ? delta->contiguous() : Tensor();
+  const ll T = x2.size(0), D = x2.size(1);
+  Tensor h = delta ? bf16(res.sizes(), res) : res, q = int8({T, padded(D)}, res), scale = f32({T, 1}, res);
+  check(E.add_rmsnorm_q8(x2.data_ptr(), delta ? d.data_ptr() : nullptr, wc.data_ptr(), delta ? h.data_ptr() : nullptr, q.data_ptr(),
+                         q.stride(0), scale.data_ptr<float>(), T, (int)D, (float)eps, stream()),
+        "add_rmsnorm_q8");
+  return {h, q, scale};
+}
+
+// (h, y, codes, scales) of the training norm; delta undefined: h is the input's and not a result
+struct Saved8 { Tensor h, y, q, scale, rstd; };
+Saved8 add_rmsnorm_saved8(const Tensor& res, const Tensor& delta, const Tensor& w, double eps) {
+  const Tensor x2 = rows(res).contiguous(), d = delta.defined() ? delta.contiguous() : delta;
+  const ll T = x2.size(0), D = x2.size(1);
+  Saved8 s;
+  if (d.defined()) s.h = bf16(res.sizes(), res);
+  s.y = bf16(res.sizes(), res);
+  s.q = int8({T, padded(D)}, res);
+  s.scale = f32({T, (D + GROUP - 1) / GROUP}, res);
+  s.rstd = f32({T}, res);
+  check(E.add_rmsnorm_saved8(x2.data_ptr(), d.defined() ? d.data_ptr() : nullptr, w.data_ptr(), d.defined() ? s.h.data_ptr() : nullptr,
+                             s.y.data_ptr(), s.q.data_ptr(), s.q.stride(0), s.scale.data_ptr<float>(), s.scale.stride(0), s.scale.stride(1),
+                             s.rstd.data_ptr<float>(), T, (int)D, (float)eps, stream()),
+        "add_rmsnorm_saved8");
+  return s;
+}
+// dx, dw (undefined where it went into the buffer or nothing asks for it) from the saved (q, scale, rstd, w)
+std::pair<Tensor, Tensor> norm_saved8_backward(AutogradContext* ctx, const Tensor& dh, const Tensor& dy, int w_index) {
+  auto s = ctx->get_saved_variables();
+  const Tensor &q = s[0], &scale = s[1], &rstd = s[2], &w = s[3];
+  if (!dy.defined()) return {dh, Tensor()};                  // only the sum was used
+  const Tensor buffer = aside(ctx, "buffer"), g = dy.contiguous(), dres = dh.defined() ? dh.contiguous() : dh;
+  const ll T = q.size(0), D = w.size(0);
+  Tensor dx = bf16(dy.sizes(), dy), part = f32({E.rmsnorm_saved8_parts(T, (int)D) * D}, dy);
+  Tensor dw;
+  if (!buffer.defined() && ctx->needs_input_grad(w_index)) dw = T ? at::empty_like(w) : at::zeros_like(w);
+  check(E.rmsnorm_saved8_bwd(g.data_ptr(), q.data_ptr(), q.stride(0), scale.data_ptr<float>(), scale.stride(0), scale.stride(1),
+                             rstd.data_ptr<float>(), w.data_ptr(), dres.defined() ? dres.data_ptr() : nullptr, dx.data_ptr(),
+                             part.data_ptr<float>(), buffer.defined() ? buffer.data_ptr<float>() : nullptr,
+                             dw.defined() ? dw.data_ptr() : nullptr, T, (int)D, stream()),
+        "rmsnorm_saved8_bwd");
+  return {dx, dw};
+}
+struct RMSNormSaved8 : Function<RMSNormSaved8> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, Aside buffer, double eps) {
+    ctx->set_materialize_grads(false);
+    const Tensor wc = w.contiguous();
+    Saved8 s = add_rmsnorm_saved8(x, Tensor(), wc, eps);
+    ctx->save_for_backward({s.q, s.scale, s.rstd, wc});
+    ctx->mark_non_differentiable({s.q, s.scale});
+    keep(ctx, "buffer", buffer);
+    return {s.y, s.q, s.scale};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    auto r = norm_saved8_backward(ctx, Tensor(), g[0], 1);
+    return {r.first, r.second, Tensor(), Tensor()};
+  }
+};
+struct AddRMSNormSaved8 : Function<AddRMSNormSaved8> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& res, const Tensor& delta, const Tensor& w, Aside buffer, double eps) {
+    ctx->set_materialize_grads(false);
+    const Tensor wc = w.contiguous();
+    Saved8 s = add_rmsnorm_saved8(res, delta, wc, eps);
+    ctx->save_for_backward({s.q, s.scale, s.rstd, wc});
+    ctx->mark_non_differentiable({s.q, s.scale});
+    keep(ctx, "buffer", buffer);
+    return {s.h, s.y, s.q, s.scale};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    auto r = norm_saved8_backward(ctx, g[0], g[1], 2);
+    return {r.first, r.first, r.second, Tensor(), Tensor()};
+  }
+};
+
+// xq, xscale and, where the codes are those of a norm's rows, its weight stand for x until the backward pass
+struct FeedForwardSaved8 : Function<FeedForwardSaved8> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w13, const Tensor& w2, Aside buffer13, Aside buffer2,
+                        Aside status, Aside xq, Aside xscale, Aside xweight) {
+    const Tensor x2 = rows(x);
+    const ll T = x2.size(0), F2 = w13.size(0), F = F2 / 2;
+    if (!xq.t.defined()) std::tie(xq.t, xscale.t) = quantize(x2, GROUP);
+    // scales of a group side by side for consecutive rows
+    Tensor q = int8({T, F2}, x), scale = f32({2 * ((F + GROUP - 1) / GROUP), T}, x), h = bf16({T, F}, x);
+    check(E.swiglu_saved8(x2.data_ptr(), w13.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), h.data_ptr(), (int)T, (int)F,
+                          (int)x2.size(1), x2.stride(0), w13.stride(0), F2, T, F, word(status.t), stream()),
+          "gemm2_swiglu_saved8");
+    auto shape = x.sizes().vec();
+    shape.back() = w2.size(0);
+    Tensor y = bf16(shape, x);
+    gemm(h, w2, y.view({-1, w2.size(0)}), false, false, 0, status.t);
+    ctx->save_for_backward({xq.t, xscale.t, xweight.t, w13, w2, q, scale});
+    keep(ctx, "buffer13", buffer13);
+    keep(ctx, "buffer2", buffer2);
+    keep(ctx, "status", status);
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    auto s = ctx->get_saved_variables();
+    const Tensor &xq = s[0], &xscale = s[1], &xweight = s[2], &w13 = s[3], &w2 = s[4], &q = s[5], &scale = s[6];
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    const Tensor status = aside(ctx, "status"), buffer13 = aside(ctx, "buffer13");
+    const Tensor dy2 = dense(rows(g[0]));
+    const ll T = q.size(0), F2 = q.size(1), F = F2 / 2;
+    Tensor dgu = bf16({T, F2}, dy2), dw2;
+    {
+      Tensor h = bf16({T, F}, dy2);
+      check(E.swiglu_bwd_saved8(dy2.data_ptr(), w2.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), dgu.data_ptr(), h.data_ptr(), (int)T,
+                                (int)F, (int)dy2.size(1), dy2.stride(0), w2.stride(0), F2, T, F2, F, word(status), stream()),
+            "gemm2_swiglu_bwd_saved8");
+      dw2 = weight_grad(aside(ctx, "buffer2"), dy2, h, w2, ctx->needs_input_grad(2), status);
+    }
+    Tensor dx, dw13;
+    if (ctx->needs_input_grad(0)) {
+      dx = bf16(shape, dy2);
+      gemm(dgu, w13, dx.view({-1, w13.size(1)}), false, true, 0, status);
+    }
+    if (buffer13.defined() || ctx->needs_input_grad(1))
+      dw13 = weight_grad(buffer13, dgu, dequantize(xq, xscale, GROUP, {T, w13.size(1)}, xweight), w13, true, status);
+    return {dx, dw13, dw2, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
 Aside opt(const std::optional<Tensor>& t) { return Aside{t ? *t : Tensor()}; }
 
 }  // namespace
@@ -346,5 +553,26 @@ PYBIND11_MODULE(tplr_host, m) {
                               const std::optional<Tensor>& bo, const Tensor& cos, const Tensor& sin, int64_t heads, int64_t kv,
                               int64_t hd, const Tensor& status) {
     return AttentionBlock::apply(x, wqkv, wo, opt(bq), opt(bo), Aside{cos}, Aside{sin}, heads, kv, hd, Aside{status});
+  }, nogil());
+  m.def("quantize_rows", &quantize, nogil());
+  m.def("dequantize_rows", [](const Tensor& q, const Tensor& scale, int64_t group, const std::vector<int64_t>& shape,
+                              const std::optional<Tensor>& w) { return dequantize(q, scale, group, shape, w ? *w : Tensor()); }, nogil());
+  m.def("linear_q8", &linear_q8, nogil());
+  m.def("linear_q8_rows", [](const Tensor& q, const Tensor& sx, const std::vector<int64_t>& shape, const Tensor& wq, const Tensor& ws,
+                             const Tensor& status) { return linear_q8_rows(q, sx, shape, wq, ws, status); }, nogil());
+  m.def("weight_as_it_is", &weight_as_it_is);
+  m.def("add_rmsnorm_q8", &add_rmsnorm_q8, nogil());
+  m.def("rmsnorm_saved8", [](const Tensor& x, const Tensor& w, const std::optional<Tensor>& buffer, double eps) {
+    auto r = RMSNormSaved8::apply(x, w, opt(buffer), eps);
+    return std::make_tuple(r[0], r[1], r[2]);
+  }, nogil());
+  m.def("add_rmsnorm_saved8", [](const Tensor& res, const Tensor& delta, const Tensor& w, const std::optional<Tensor>& buffer, double eps) {
+    auto r = AddRMSNormSaved8::apply(res, delta, w, opt(buffer), eps);
+    return std::make_tuple(r[0], r[1], r[2], r[3]);
+  }, nogil());
+  m.def("feed_forward_saved8", [](const Tensor& x, const Tensor& w13, const Tensor& w2, const std::optional<Tensor>& b13,
+                                  const std::optional<Tensor>& b2, const Tensor& status, const std::optional<Tensor>& xq,
+                                  const std::optional<Tensor>& xscale, const std::optional<Tensor>& xweight) {
+    return FeedForwardSaved8::apply(x, w13, w2, opt(b13), opt(b2), Aside{status}, opt(xq), opt(xscale), opt(xweight));
   }, nogil());
 }

@@ -29,7 +29,10 @@ def _padded(n: int) -> int:
 
 
 def _native_rows(*ts) -> bool:
-    return all(t is None or (t.is_cuda and t.dtype == torch.bfloat16) for t in ts)
+    for t in ts:
+        if t is not None and not (t.is_cuda and t.dtype == torch.bfloat16):
+            return False
+    return True
 
 
 def _rows_of(x: torch.Tensor) -> torch.Tensor:
@@ -66,6 +69,13 @@ class QuantRows:
                              f"{scale.dtype} {tuple(scale.shape)} on {scale.device}")
         self.q, self.scale, self.group, self.shape = q, scale, int(group), torch.Size(shape)
 
+    @classmethod
+    def _of(cls, q, scale, group: int, shape):
+        """From the operators themselves, whose codes and scales need no look."""
+        r = cls.__new__(cls)
+        r.q, r.scale, r.group, r.shape = q, scale, group, shape
+        return r
+
     @property
     def width(self) -> int:
         return self.shape[-1]
@@ -92,14 +102,16 @@ def quantize_rows(x: torch.Tensor, group: int = 0) -> QuantRows:
         raise ValueError(f"quantize_rows: group is 0 (the row) or {GROUP}, got {group}")
     x2 = _rows_of(x.detach())
     if not _native_rows(x2):
-        return QuantRows(*_plain_rows(x2.float(), group), group, x.shape)
+        return QuantRows._of(*_plain_rows(x2.float(), group), group, x.shape)
+    if host := native.host():
+        return QuantRows._of(*host.quantize_rows(x2, group), group, x.shape)
     if x2.stride(1) != 1:
         x2 = x2.contiguous()
     T, D = x2.shape
     q, scale = _empty_rows((T, D), group, x.device)
     native.check(native.lib().tplr_quantize_rows(x2.data_ptr(), x2.stride(0), q.data_ptr(), q.stride(0), scale.data_ptr(), scale.stride(0),
                                                  scale.stride(1), T, D, group, native.stream_ptr()), "quantize_rows")
-    return QuantRows(q, scale, group, x.shape)
+    return QuantRows._of(q, scale, group, x.shape)
 
 
 def dequantize_rows(rows: QuantRows, dtype: torch.dtype = torch.bfloat16, weight: torch.Tensor | None = None) -> torch.Tensor:
@@ -112,6 +124,8 @@ def dequantize_rows(rows: QuantRows, dtype: torch.dtype = torch.bfloat16, weight
 def _values(q, scale, group: int, shape, dtype, weight=None):
     T, D = q.shape[0], shape[-1]
     if q.is_cuda and dtype == torch.bfloat16 and _native_rows(weight):
+        if host := native.host():
+            return host.dequantize_rows(q, scale, group, shape, None if weight is None else weight.detach())
         y = torch.empty(shape, dtype=dtype, device=q.device)
         w = None if weight is None else weight.detach().contiguous()
         native.check(native.lib().tplr_dequantize_rows(q.data_ptr(), q.stride(0), scale.data_ptr(), scale.stride(0),
@@ -135,6 +149,9 @@ class QuantWeight:
     __slots__ = ("q", "scale")
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor):
+        if q.is_cuda and (host := native.host()) and host.weight_as_it_is(q, scale):
+            self.q, self.scale = q, scale
+            return
         if q.dim() != 2 or q.dtype != torch.int8 or q.shape[1] == 0:
             raise ValueError(f"QuantWeight: int8 codes [N, K] expected, got {q.dtype} {tuple(q.shape)}")
         if q.shape[1] > MAX_INNER:
@@ -175,24 +192,28 @@ def _no_grad_asked(what: str, *ts) -> None:
 def add_rmsnorm_q8(res: torch.Tensor, delta: torch.Tensor | None, w: torch.Tensor, eps: float = 1e-5) -> tuple[torch.Tensor, QuantRows]:
     """``(res + delta, rmsnorm(res + delta) * w)``, the second in 8 bits with one scale a row (``delta`` None: of ``res``)."""
     _no_grad_asked("add_rmsnorm_q8", res, delta, w)
-    x2 = _rows_of(res)
-    T, D = x2.shape
     _norm_args("add_rmsnorm_q8", res, delta, w)
     if not _native_rows(res, delta, w):
         h = res if delta is None else res + delta
-        hf = h.float().reshape(T, D)
+        hf = _rows_of(h.float())
         y = hf * torch.rsqrt(hf.pow(2).mean(-1, keepdim=True) + eps) * w.float()
-        return h, QuantRows(*_plain_rows(y, 0), 0, res.shape)
-    x2, w = x2.contiguous(), w.contiguous()
+        return h, QuantRows._of(*_plain_rows(y, 0), 0, res.shape)
+    if host := native.host():
+        h, q, scale = host.add_rmsnorm_q8(res, delta, w, eps)
+        return (res if delta is None else h), QuantRows._of(q, scale, 0, res.shape)
+    x2, w = _rows_of(res).contiguous(), w.contiguous()
+    T, D = x2.shape
     d2 = None if delta is None else delta.contiguous()
     h = res if delta is None else torch.empty(res.shape, dtype=res.dtype, device=res.device)
     q, scale = _empty_rows((T, D), 0, res.device)
     native.check(native.lib().tplr_add_rmsnorm_q8(x2.data_ptr(), native.ptr(d2), w.data_ptr(), h.data_ptr(), q.data_ptr(), q.stride(0),
                                                   scale.data_ptr(), T, D, eps, native.stream_ptr()), "add_rmsnorm_q8")
-    return h, QuantRows(q, scale, 0, res.shape)
+    return h, QuantRows._of(q, scale, 0, res.shape)
 
 
 def _norm_args(what: str, res, delta, w) -> None:
+    if res.dim() == 0 or res.shape[-1] == 0:
+        raise ValueError(f"{what}: rows of no elements: shape {tuple(res.shape)}")
     if w.dim() != 1 or w.shape[0] != res.shape[-1]:
         raise ValueError(f"{what}: {tuple(w.shape)} weights for rows of {res.shape[-1]}")
     if delta is not None and delta.shape != res.shape:
@@ -208,24 +229,29 @@ def swiglu_q8(gu: torch.Tensor) -> QuantRows:
     T, Fd = g2.shape[0], g2.shape[1] // 2
     shape = (*gu.shape[:-1], Fd)
     if not _native_rows(gu):
-        return QuantRows(*_plain_rows(F.silu(g2[:, :Fd].float()) * g2[:, Fd:].float(), 0), 0, shape)
+        return QuantRows._of(*_plain_rows(F.silu(g2[:, :Fd].float()) * g2[:, Fd:].float(), 0), 0, torch.Size(shape))
     if g2.stride(1) != 1:
         g2 = g2.contiguous()
     q, scale = _empty_rows((T, Fd), 0, gu.device)
     native.check(native.lib().tplr_swiglu_q8(g2.data_ptr(), g2.stride(0), q.data_ptr(), q.stride(0), scale.data_ptr(), T, Fd,
                                              native.stream_ptr()), "swiglu_q8")
-    return QuantRows(q, scale, 0, shape)
+    return QuantRows._of(q, scale, 0, torch.Size(shape))
 
 
 def linear_q8(x: torch.Tensor | QuantRows, w: QuantWeight, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``x @ w.T`` from 8-bit rows and an 8-bit weight: exact sums in 32-bit integers, one scale for each row times one for each
     channel, rounded once to ``out_dtype`` (bf16 or fp32; default: that of ``x``, bf16 for rows in 8 bits).  A tensor ``x`` is
     quantised first, by rows.  Forward passes only."""
+    bf16_out = out_dtype is None or out_dtype is torch.bfloat16
     if not isinstance(x, QuantRows):
         _no_grad_asked("linear_q8", x)
+        if x.dim() == 0 or x.shape[-1] != w.q.shape[1]:
+            raise ValueError(f"linear_q8: inner dimensions of {tuple(x.shape)} and {tuple(w.shape)} differ")
+        if x.device != w.q.device:
+            raise ValueError(f"linear_q8: rows on {x.device}, weight on {w.q.device}")
+        if bf16_out and _native_rows(x) and (host := native.host()):
+            return host.linear_q8(x, w.q, w.scale, OF.status_word(x.device))
         out_dtype = out_dtype or x.dtype
-        if x.shape[-1] != w.shape[1]:
-            raise ValueError(f"linear_q8: inner dimensions {x.shape[-1]} and {w.shape[1]} differ")
         x = quantize_rows(x)
     out_dtype = out_dtype or torch.bfloat16
     if x.group:
@@ -235,6 +261,8 @@ def linear_q8(x: torch.Tensor | QuantRows, w: QuantWeight, out_dtype: torch.dtyp
         raise ValueError(f"linear_q8: inner dimensions {x.width} and {w.shape[1]} differ")
     if x.q.device != w.q.device:
         raise ValueError(f"linear_q8: rows on {x.q.device}, weight on {w.q.device}")
+    if bf16_out and x.q.is_cuda and (host := native.host()):
+        return host.linear_q8_rows(x.q, x.scale.contiguous(), x.shape, w.q, w.scale, OF.status_word(x.q.device))
     T, N, K = x.q.shape[0], w.shape[0], w.shape[1]
     if x.q.is_cuda and out_dtype in (torch.bfloat16, torch.float32):
         y = torch.empty(*x.shape[:-1], N, dtype=out_dtype, device=x.q.device)
@@ -337,8 +365,14 @@ def add_rmsnorm_saved8(res: torch.Tensor, delta: torch.Tensor | None, w: torch.T
     if main_grad is None:
         main_grad = getattr(w, "main_grad", None)
     _norm_args("add_rmsnorm_saved8", res, delta, w)
+    if _native_rows(res, delta, w) and OF._buffers_ok((main_grad, w)) and (host := native.host()):
+        if delta is None:
+            h, (y, q, scale) = res, host.rmsnorm_saved8(res, w, main_grad, eps)
+        else:
+            h, y, q, scale = host.add_rmsnorm_saved8(res, delta, w, main_grad, eps)
+        return h, y, QuantRows._of(q, scale, GROUP, res.shape)
     h, y, q, scale = _AddRMSNormSaved8.apply(res, delta, w, eps, main_grad)
-    return (res if delta is None else h), y, QuantRows(q, scale, GROUP, res.shape)
+    return (res if delta is None else h), y, QuantRows._of(q, scale, GROUP, res.shape)
 
 
 def _kept_input(x, rows: QuantRows | None, weight):
@@ -484,6 +518,10 @@ def feed_forward_saved8(x, w13, w2, rows: QuantRows | None = None, weight=None, 
         raise ValueError(f"feed_forward_saved8: weights {tuple(w13.shape)} and {tuple(w2.shape)} do not fit rows of {x.shape[-1]}")
     if not torch.is_grad_enabled():
         return OF.feed_forward(x, w13, w2, main_grad13, main_grad2)
+    if (OF._feed_forward_fused(x.reshape(-1, x.shape[-1]), w13, w2) and OF._buffers_ok((main_grad13, w13), (main_grad2, w2))
+            and (host := native.host())):
+        q, scale, weight = (None, None, None) if rows is None else _kept_input(x, rows, weight)
+        return host.feed_forward_saved8(x, w13, w2, main_grad13, main_grad2, OF.status_word(x.device), q, scale, weight)
     return _FeedForwardSaved8.apply(x, w13, w2, main_grad13, main_grad2, *_kept_input(x, rows, weight))
 
 

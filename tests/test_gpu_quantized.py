@@ -11,6 +11,7 @@ from templar_b200 import ops
 from templar_b200.models.llama import ModelArgs, build_model
 from templar_b200.models.llama_int8 import Int8Llama
 from templar_b200.ops import functional as OF
+from templar_b200.ops import native
 from templar_b200.ops import quantized as OQ
 from templar_b200.parallel.window_engine import EngineConfig, WindowEngine
 
@@ -320,3 +321,31 @@ def test_scoring_in_8_bits_is_near_the_model():
     one = q(tok[:1, :1]).float()
     assert (one - want[:1, :1]).norm() < 0.06 * want[:1, :1].norm()
     healthy()
+
+
+@pytest.mark.parametrize("T,D,Fd", [(5, 72, 40), (300, 256, 384)])
+def test_the_python_nodes_give_the_bits_of_those_in_cpp(T, D, Fd, monkeypatch):
+    res, delta, wn = bf(T, D).requires_grad_(), bf(T, D, seed=1).requires_grad_(), bf(D, seed=2).requires_grad_()
+    w13, w2 = bf(2 * Fd, D, std=D ** -0.5, seed=3).requires_grad_(), bf(D, Fd, std=Fd ** -0.5, seed=4).requires_grad_()
+    dh, dy = bf(T, D, seed=5), bf(T, D, seed=6)
+    qw = ops.quantize_weight(w13)
+
+    def everything():
+        out = []
+        for d in (delta, None):
+            h, y, rows = ops.add_rmsnorm_saved8(res, d, wn)
+            z = ops.feed_forward_saved8(y, w13, w2, rows, wn)
+            out += [h, y, rows.q, rows.scale, z, *torch.autograd.grad((h, z), (res, wn, w13, w2), (dh, dy))]
+            out += torch.autograd.grad(ops.feed_forward_saved8(res, w13, w2), (res, w13), dy)
+            with torch.no_grad():
+                h, rows = ops.add_rmsnorm_q8(res, d, wn)
+                gu = ops.linear_q8(rows, qw)
+                out += [h, rows.q, rows.scale, gu, ops.linear_q8(res, qw), rows.dequantize(weight=wn), ops.swiglu_q8(gu).q]
+        out += [ops.quantize_rows(res, g).q for g in (0, 64)]
+        return out
+
+    want = everything()
+    assert native.host()
+    monkeypatch.setattr(native, "host", lambda: None)
+    got = everything()
+    assert len(got) == len(want) and all(a.equal(b) for a, b in zip(got, want))
