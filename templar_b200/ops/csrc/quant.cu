@@ -40,62 +40,105 @@ struct RowsArgs {
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
-// One CTA a row, element by element: every width and alignment.
-template <int MODE>
+// One CTA a row, element by element: every width and alignment.  A row of up to 256 * EPT elements stays in registers, EPT a
+// thread, 32 * EPT consecutive ones a warp, so that a group of 64 columns is two values of every lane; EPT 0: it is read again for each
+// pass.  1111 x 1001, norm in 8 bits: 7.0 us read three times, 4.8 from registers.
+template <int MODE, int EPT>
 __global__ void __launch_bounds__(256) rows_q8_any_kernel(const RowsArgs p) {
+  constexpr bool NORM = MODE == NORM_ROWS || MODE == NORM_SAVED, BY_GROUP = MODE == GROUPS || MODE == NORM_SAVED;
+  constexpr int HELD = EPT ? EPT : 1;
   __shared__ float red[32];
   __shared__ uint32_t s_top[8];
   grid_wait();
   grid_release();
   const ll row = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = p.D;
-  constexpr bool NORM = MODE == NORM_ROWS || MODE == NORM_SAVED;
   const bf16 *a = p.a + row * p.lda, *b = p.b ? p.b + row * p.ldb : nullptr;
+  int8_t* q = p.q + row * p.ldq;
   auto in = [&](int i) -> float {
     if (MODE == SWIGLU_ROWS) return silu_mul(__bfloat162float(a[i]), __bfloat162float(a[D + i]));
     if (!NORM || !b) return __bfloat162float(a[i]);
     return __bfloat162float(__float2bfloat16(__bfloat162float(a[i]) + __bfloat162float(b[i])));   // as the residual stream stores it
   };
+  auto column = [&](int c) { return (warp * HELD + c) * 32 + lane; };
+  float v[HELD];
   float r = 1.f;
+  if (EPT) {
+#pragma unroll
+    for (int c = 0; c < HELD; ++c) v[c] = column(c) < D ? in(column(c)) : 0.f;
+  }
   if (NORM) {
     float ss = 0.f;
-    for (int i = threadIdx.x; i < D; i += 256) {
-      const float x = in(i);
-      if (p.h) p.h[row * D + i] = __float2bfloat16(x);
-      ss = fmaf(x, x, ss);
+    if (EPT) {
+#pragma unroll
+      for (int c = 0; c < HELD; ++c) {
+        if (p.h && column(c) < D) p.h[row * D + column(c)] = __float2bfloat16(v[c]);
+        ss = fmaf(v[c], v[c], ss);
+      }
+    } else {
+      for (int i = threadIdx.x; i < D; i += 256) {
+        const float x = in(i);
+        if (p.h) p.h[row * D + i] = __float2bfloat16(x);
+        ss = fmaf(x, x, ss);
+      }
     }
     r = rsqrtf(block_sum(ss, red) / (float)D + p.eps);
     if (MODE == NORM_SAVED && threadIdx.x == 0) p.rstd[row] = r;
+    if (EPT) {
+#pragma unroll
+      for (int c = 0; c < HELD; ++c) {
+        v[c] *= r;
+        if (MODE == NORM_ROWS && column(c) < D) v[c] *= __bfloat162float(p.w[column(c)]);
+      }
+    }
   }
-  int8_t* q = p.q + row * p.ldq;
-  auto value = [&](int i) -> float {
+  auto value = [&](int i) -> float {                                     // of a column that is not held
     const float x = NORM ? in(i) * r : in(i);
     return MODE == NORM_ROWS ? x * __bfloat162float(p.w[i]) : x;
   };
-  if (MODE == GROUPS || MODE == NORM_SAVED) {
-    for (int g = warp; g * GROUP < D; g += 8) {
-      const int i0 = g * GROUP + lane, i1 = i0 + 32;
-      const float x0 = i0 < D ? value(i0) : 0.f, x1 = i1 < D ? value(i1) : 0.f;
-      const Codes c = codes_of(__reduce_max_sync(0xffffffffu, max(magnitude(x0), magnitude(x1))));
-      if (lane == 0) p.scale[row * p.scale_row + g * p.scale_group] = c.scale;
-      if (i0 < p.ldq) q[i0] = (int8_t)code(x0, c.inv);
-      if (i1 < p.ldq) q[i1] = (int8_t)code(x1, c.inv);
+  if (BY_GROUP) {
+    auto group = [&](int i0, float x0, float x1) {                       // columns i0 and i0 + 32 of a group
+      const Codes k = codes_of(__reduce_max_sync(0xffffffffu, max(magnitude(x0), magnitude(x1))));
+      const int i1 = i0 + 32;
+      if (lane == 0 && i0 < D) p.scale[row * p.scale_row + (i0 >> 6) * p.scale_group] = k.scale;
+      if (i0 < p.ldq) q[i0] = (int8_t)code(x0, k.inv);
+      if (i1 < p.ldq) q[i1] = (int8_t)code(x1, k.inv);
       if (MODE == NORM_SAVED) {
         if (i0 < D) p.y[row * D + i0] = __float2bfloat16(x0 * __bfloat162float(p.w[i0]));
         if (i1 < D) p.y[row * D + i1] = __float2bfloat16(x1 * __bfloat162float(p.w[i1]));
+      }
+    };
+    if (EPT) {
+#pragma unroll
+      for (int c = 0; c + 1 < HELD; c += 2) group(column(c), v[c], v[c + 1]);
+    } else {
+      for (int g = warp; g * GROUP < D; g += 8) {
+        const int i0 = g * GROUP + lane;
+        group(i0, i0 < D ? value(i0) : 0.f, i0 + 32 < D ? value(i0 + 32) : 0.f);
       }
     }
     return;
   }
   uint32_t top = 0;
-  for (int i = threadIdx.x; i < D; i += 256) top = max(top, magnitude(value(i)));
+  if (EPT) {
+#pragma unroll
+    for (int c = 0; c < HELD; ++c) top = max(top, magnitude(v[c]));
+  } else {
+    for (int i = threadIdx.x; i < D; i += 256) top = max(top, magnitude(value(i)));
+  }
   top = __reduce_max_sync(0xffffffffu, top);
   if (lane == 0) s_top[warp] = top;
   __syncthreads();
   for (int k = 0; k < 8; ++k) top = max(top, s_top[k]);
-  const Codes c = codes_of(top);
-  if (threadIdx.x == 0) p.scale[row * p.scale_row] = c.scale;
-  for (int i = threadIdx.x; i < p.ldq; i += 256) q[i] = i < D ? (int8_t)code(value(i), c.inv) : 0;
+  const Codes k = codes_of(top);
+  if (threadIdx.x == 0) p.scale[row * p.scale_row] = k.scale;
+  if (EPT) {
+#pragma unroll
+    for (int c = 0; c < HELD; ++c)
+      if (column(c) < p.ldq) q[column(c)] = (int8_t)code(v[c], k.inv);   // zeros behind column D
+  } else {
+    for (int i = threadIdx.x; i < p.ldq; i += 256) q[i] = i < D ? (int8_t)code(value(i), k.inv) : 0;
+  }
 }
 
 struct alignas(16) bf16x8 { __nv_bfloat162 v[4]; };
@@ -249,18 +292,25 @@ __global__ void __launch_bounds__(BLOCK) rows_q8_kernel(const RowsArgs p, const 
 }
 
 // ------------------------------------------------------------------------------------------ 8 bits -> rows
-// y = q * scale (* w of the column), rows of D; a scale for every `group` columns.
-__global__ void __launch_bounds__(256) dequantize_any_kernel(const int8_t* q, ll ldq, const float* scale, ll scale_row, ll scale_group, int group,
-                                                             const bf16* w, bf16* y, ll T, int D) {
+// y = q * scale (* w of the column), rows of D; a scale for the row or for every 64 columns.
+__global__ void __launch_bounds__(256) dequantize_any_kernel(const int8_t* q, ll ldq, const float* scale, ll scale_row, ll scale_group,
+                                                             bool by_group, const bf16* w, bf16* y, ll T, int D) {
   grid_wait();
   grid_release();
-  const ll total = T * D;
-  for (ll i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-    const ll row = i / D;
-    const int c = (int)(i - row * D);
-    float v = (float)q[row * ldq + c] * scale[row * scale_row + c / group * scale_group];
-    if (w) v *= __bfloat162float(w[c]);
-    y[i] = __float2bfloat16(v);
+  for (ll row = blockIdx.x; row < T; row += gridDim.x) {
+    const float* s = scale + row * scale_row;
+    for (int c0 = threadIdx.x; c0 < D; c0 += 4 * 256) {
+      float v[4], m[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = c0 + 256 * j;
+        v[j] = c < D ? (float)q[row * ldq + c] * s[by_group ? c / GROUP * scale_group : 0] : 0.f;
+        m[j] = w && c < D ? __bfloat162float(w[c]) : 1.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c0 + 256 * j < D) y[row * D + c0 + 256 * j] = __float2bfloat16(w ? v[j] * m[j] : v[j]);
+    }
   }
 }
 
@@ -306,29 +356,62 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* q, ll ldq
 }
 
 // ------------------------------------------------------------------------------------------ norm, backward from 8 bits
-// xn = q * scale; g = dy * w; dx = dres + rstd * (g - xn * mean(g * xn)); the CTA's sum of dy * xn goes to part[blockIdx.x].
-__global__ void __launch_bounds__(256) rmsnorm_saved8_bwd_any_kernel(const bf16* dy, const int8_t* q, ll ldq, const float* scale, ll scale_row,
-                                                                     ll scale_group, const float* rstd, const bf16* w, const bf16* dres,
-                                                                     bf16* dx, float* part, ll T, int D) {
+// xn = q * scale; g = dy * w; dx = dres + rstd * (g - xn * mean(g * xn)); the CTA's sum of dy * xn goes to part[blockIdx.x].  Every width and
+// alignment; a row of up to BLOCK * EPT elements stays in registers, and so do the sums (EPT 0: read again, sums in memory).
+template <int EPT, int BLOCK>
+__global__ void __launch_bounds__(BLOCK) rmsnorm_saved8_bwd_any_kernel(const bf16* dy, const int8_t* q, ll ldq, const float* scale, ll scale_row,
+                                                                       ll scale_group, const float* rstd, const bf16* w, const bf16* dres,
+                                                                       bf16* dx, float* part, ll T, int D) {
+  constexpr int HELD = EPT ? EPT : 1;
   __shared__ float red[32];
   grid_wait();
   grid_release();
   float* mine = part + (ll)blockIdx.x * D;
-  for (int i = threadIdx.x; i < D; i += 256) mine[i] = 0.f;
+  auto xn = [&](ll row, int i) { return (float)q[row * ldq + i] * scale[row * scale_row + i / GROUP * scale_group]; };
+  if (EPT) {
+    float dw[HELD] = {}, m[HELD];
+#pragma unroll
+    for (int c = 0; c < HELD; ++c) m[c] = threadIdx.x + BLOCK * c < D ? __bfloat162float(w[threadIdx.x + BLOCK * c]) : 0.f;
+    for (ll row = blockIdx.x; row < T; row += gridDim.x) {
+      float dot = 0.f, x[HELD], g[HELD], a[HELD];
+      const float r = rstd[row];
+#pragma unroll
+      for (int c = 0; c < HELD; ++c) {
+        const int i = threadIdx.x + BLOCK * c;
+        g[c] = i < D ? __bfloat162float(dy[row * D + i]) : 0.f;
+        x[c] = i < D ? xn(row, i) : 0.f;
+        a[c] = dres && i < D ? __bfloat162float(dres[row * D + i]) : 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < HELD; ++c) {
+        dw[c] = fmaf(g[c], x[c], dw[c]);
+        g[c] *= m[c];
+        dot = fmaf(g[c], x[c], dot);
+      }
+      dot = block_sum(dot, red) / (float)D;
+#pragma unroll
+      for (int c = 0; c < HELD; ++c)
+        if (threadIdx.x + BLOCK * c < D) dx[row * D + threadIdx.x + BLOCK * c] = __float2bfloat16(fmaf(r, g[c] - x[c] * dot, a[c]));
+      __syncthreads();
+    }
+#pragma unroll
+    for (int c = 0; c < HELD; ++c)
+      if (threadIdx.x + BLOCK * c < D) mine[threadIdx.x + BLOCK * c] = dw[c];
+    return;
+  }
+  for (int i = threadIdx.x; i < D; i += BLOCK) mine[i] = 0.f;            // this thread's own columns
   for (ll row = blockIdx.x; row < T; row += gridDim.x) {
-    auto xn = [&](int i) { return (float)q[row * ldq + i] * scale[row * scale_row + i / GROUP * scale_group]; };
     float dot = 0.f;
-    for (int i = threadIdx.x; i < D; i += 256) {
-      const float d = __bfloat162float(dy[row * D + i]), x = xn(i);
-      mine[i] += d * x;                                                  // this thread's own columns
-      dot = fmaf(d * __bfloat162float(w[i]), x, dot);
+    for (int i = threadIdx.x; i < D; i += BLOCK) {
+      const float d = __bfloat162float(dy[row * D + i]), xi = xn(row, i);
+      mine[i] += d * xi;
+      dot = fmaf(d * __bfloat162float(w[i]), xi, dot);
     }
     dot = block_sum(dot, red) / (float)D;
     const float r = rstd[row];
-    for (int i = threadIdx.x; i < D; i += 256) {
-      float o = r * (__bfloat162float(dy[row * D + i]) * __bfloat162float(w[i]) - xn(i) * dot);
-      if (dres) o += __bfloat162float(dres[row * D + i]);
-      dx[row * D + i] = __float2bfloat16(o);
+    for (int i = threadIdx.x; i < D; i += BLOCK) {
+      const float o = r * (__bfloat162float(dy[row * D + i]) * __bfloat162float(w[i]) - xn(row, i) * dot);
+      dx[row * D + i] = __float2bfloat16(dres ? o + __bfloat162float(dres[row * D + i]) : o);
     }
     __syncthreads();
   }
@@ -622,7 +705,8 @@ int rows_q8(const RowsArgs& p, void* stream) {
   cudaStream_t st = (cudaStream_t)stream;
   const int pieces = (int)((p.ldq + 7) / 8);
   if (p.D % 8 || p.ldq % 8 || p.lda % 8 || (p.b && p.ldb % 8) || p.D > 32760 || !whole_pieces(p.a, p.b, p.w, p.h, p.y, p.q))
-    return (int)launch_pdl(rows_q8_any_kernel<MODE>, (unsigned)p.T, 256, 0, st, p);
+    return (int)launch_pdl(p.D <= 1024 ? rows_q8_any_kernel<MODE, 4> : p.D <= 2048 ? rows_q8_any_kernel<MODE, 8> : p.D <= 4096 ? rows_q8_any_kernel<MODE, 16>
+                           : p.D <= 8192 ? rows_q8_any_kernel<MODE, 32> : rows_q8_any_kernel<MODE, 0>, (unsigned)p.T, 256, 0, st, p);
   // one piece a thread while that leaves threads to spare on the chip, four where rows are many
   const int vpl = p.T * pieces <= 2048LL * tplr_sm_count() && pieces <= 1024 ? 1 : 4;
   const int tpr = row_threads(pieces, vpl), block = tpr > 256 ? 1024 : 256;
@@ -679,21 +763,21 @@ TPLR_API int tplr_swiglu_q8(const void* gu, ll ldgu, void* q, ll ldq, float* sca
   return rows_q8<SWIGLU_ROWS>(p, stream);
 }
 
-// y[T, D] (dense bf16) = q * scale, times w[column] where w is given; a scale for every `group` columns.
+// y[T, D] (dense bf16) = q * scale, times w[column] where w is given; a scale for the row (group D or more) or for every 64 columns.
 TPLR_API int tplr_dequantize_rows(const void* q, ll ldq, const float* scale, ll scale_row, ll scale_group, int group, const void* w, void* y,
                                   ll T, int D, void* stream) {
   TPLR_ENTER();
   if (T <= 0) return 0;
-  if (D <= 0 || group <= 0) return (int)cudaErrorInvalidValue;
-  if (D % 8 == 0 && ldq % 8 == 0 && (group == GROUP || group >= D) && T <= 0x7fffffffLL && whole_pieces(q, w, y)) {
+  if (D <= 0 || (group != GROUP && group < D)) return (int)cudaErrorInvalidValue;
+  if (D % 8 == 0 && ldq % 8 == 0 && T <= 0x7fffffffLL && whole_pieces(q, w, y)) {
     int tpr = row_threads(D / 8, 4);
     if (tpr > 256) tpr = 256;
     const int rows = 256 / tpr;
     return (int)launch_pdl(dequantize_kernel, (unsigned)((T + rows - 1) / rows), 256, 0, (cudaStream_t)stream, (const int8_t*)q, ldq, scale,
-                           scale_row, group >= D ? 0 : scale_group, (const bf16*)w, (bf16*)y, T, D, tpr);
+                           scale_row, group == GROUP ? scale_group : 0, (const bf16*)w, (bf16*)y, T, D, tpr);
   }
-  return (int)launch_pdl(dequantize_any_kernel, waves((T * D + 255) / 256, 16), 256, 0, (cudaStream_t)stream, (const int8_t*)q, ldq, scale,
-                         scale_row, scale_group, group, (const bf16*)w, (bf16*)y, T, D);
+  return (int)launch_pdl(dequantize_any_kernel, waves(T, 64), 256, 0, (cudaStream_t)stream, (const int8_t*)q, ldq, scale,
+                         scale_row, scale_group, group == GROUP, (const bf16*)w, (bf16*)y, T, D);
 }
 
 // Rows (each of D elements) of the fp32 workspace that tplr_rmsnorm_saved8_bwd takes: its CTAs at most.
@@ -713,8 +797,11 @@ TPLR_API int tplr_rmsnorm_saved8_bwd(const void* dy, const void* q, ll ldq, cons
   int n;
   cudaError_t e;
   if (D % 8 || D > 8192 || ldq % 8 || !whole_pieces(dy, q, w, dres, dx, part)) {
-    n = (int)waves(T, 4);
-    e = launch_pdl(rmsnorm_saved8_bwd_any_kernel, n, 256, 0, st, g, c, ldq, scale, scale_row, scale_group, rstd, wp, a, (bf16*)dx, part, T, D);
+    const int block = D <= 1024 ? 256 : D <= 2048 ? 512 : 1024;
+    n = (int)waves(T, block == 256 ? 4 : 2048 / block);
+    auto kern = block == 256 ? rmsnorm_saved8_bwd_any_kernel<4, 256> : block == 512 ? rmsnorm_saved8_bwd_any_kernel<4, 512>
+                : D <= 4096 ? rmsnorm_saved8_bwd_any_kernel<4, 1024> : D <= 8192 ? rmsnorm_saved8_bwd_any_kernel<8, 1024> : rmsnorm_saved8_bwd_any_kernel<0, 1024>;
+    e = launch_pdl(kern, n, block, 0, st, g, c, ldq, scale, scale_row, scale_group, rstd, wp, a, (bf16*)dx, part, T, D);
   } else {
     const int tpr = row_threads(D / 8, BWD_VPL), block = tpr > 256 ? 512 : 256, rows = block / tpr;
     n = (int)waves((T + rows - 1) / rows, 512 / block);
