@@ -47,6 +47,8 @@ int tplr_rmsnorm_saved8_bwd(const void* dy, const void* q, long long ldq, const 
                             long long T, int D, void* stream);
 int tplr_gemm_q8(const void* x, const void* w, const float* sx, const float* sw, void* y, int T, int N, int K, long long ldx, long long ldw,
                  long long ldy, int out_fp32, unsigned int* status, void* stream);
+int tplr_linear_q8_few(const void* x, const void* w, const float* sw, void* y, int T, int N, int K, long long ldx, long long ldw,
+                       long long ldy, void* stream);
 int tplr_gemm2_swiglu_saved8(const void* X, const void* W, void* Q, float* scale, void* H, int M, int F, int K, long long ldx, long long ldw,
                              long long ldq, long long ld_scale, long long ldh, unsigned int* status, void* stream);
 int tplr_gemm2_swiglu_bwd_saved8(const void* dY, const void* W2, const void* Q, const float* scale, void* dGU, void* H, int M, int F, int K,

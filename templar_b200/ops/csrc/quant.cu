@@ -627,7 +627,8 @@ __global__ void __launch_bounds__(256) swiglu_saved8_bwd_kernel(const float* dac
 // straight into the operands of mma.m16n8k32: nothing is set up before the first load, which for 2048 x 2048 is a third of
 // the time.  The sum over k may be taken in any order, so a lane's 16 bytes of a row are its words of two instructions as they lie:
 // word j of a weight row and word j of a token are multiplied wherever the instruction thinks they are.  A CTA's eight warps take
-// 64-byte pieces of 16 rows in turn, 512 bytes of a row together, and add their sums in shared memory.
+// 64-byte pieces of 16 rows in turn, 512 bytes of a row together, and add their sums in shared memory, while the next rows' are on
+// their way.
 __device__ __forceinline__ uint4 ld_once(const int8_t* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
@@ -637,56 +638,114 @@ __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <class Out>
-__global__ void __launch_bounds__(256) gemm_q8_few_kernel(const int8_t* x, const int8_t* w, const float* sx, const float* sw, Out* y, int T,
-                                                          int N, int K, ll ldx, ll ldw, ll ldy) {
-  constexpr int UNROLL = 4;
-  __shared__ int s_sum[8][8][17];
+//
+// HELD: x is bf16 and its rows are put in 8 bits here, by every CTA for itself, while its first pieces of the weight are on their way: as
+// many values as the threads hold, HELD_MOST; one launch instead of two.
+constexpr int FEW = 8, FEW_UNROLL = 4, HELD_MOST = 4096, HELD_PIECES = HELD_MOST / 2048;
+__host__ __device__ constexpr int held_stride(int kp) { return (kp + 511) / 512 * 512 + 64; }          // rows 64 bytes apart in the banks
+template <class Out, bool HELD>
+__global__ void __launch_bounds__(256, 3) gemm_q8_few_kernel(const void* x, const int8_t* w, const float* sx, const float* sw, Out* y, int T, int N,
+                                                          int K, ll ldx, ll ldw, ll ldy) {
+  __shared__ int s_sum[2][8][8][17];
+  __shared__ __align__(16) int8_t s_x[HELD ? HELD_MOST + FEW * (512 + 64) : 16];
+  __shared__ float s_sx[FEW];
+  __shared__ uint32_t s_top[8];
   grid_wait();
   grid_release();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n0 = blockIdx.x * 16, kp = (K + 15) / 16 * 16, tok = lane >> 2;
-  int acc[4] = {};
-  const int8_t* wr[2];
-  bool wok[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int n = n0 + h * 8 + (lane >> 2);
-    wok[h] = n < N;
-    wr[h] = w + (ll)(n < N ? n : N - 1) * ldw;
-  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kp = (K + 15) / 16 * 16, tok = lane >> 2;
+  const int stride = held_stride(kp), blocks = (N + 15) / 16;
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  for (int k0 = warp * 64; k0 < kp; k0 += 512 * UNROLL) {
-    uint4 a[UNROLL][2], b[UNROLL];
+  uint4 a[FEW_UNROLL][2];
+  auto ask = [&](int block, int k0) {
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int k = k0 + u * 512 + (lane & 3) * 16;
-      const bool in = k < kp;
+    for (int h = 0; h < 2; ++h) {
+      const int n = block * 16 + h * 8 + (lane >> 2);
+      const int8_t* row = w + (ll)min(n, N - 1) * ldw;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) a[u][h] = in && wok[h] ? ld_once(wr[h] + k) : zero;
-      b[u] = in && tok < T ? *reinterpret_cast<const uint4*>(x + tok * ldx + k) : zero;
+      for (int u = 0; u < FEW_UNROLL; ++u) {
+        const int k = k0 + u * 512 + (lane & 3) * 16;
+        a[u][h] = k < kp && n < N ? ld_once(row + k) : zero;
+      }
     }
+  };
+  ask(blockIdx.x, warp * 64);
+  if (HELD) {
+    int share = 256;                                                     // threads of a token
+    while (share * T > 256) share /= 2;
+    const int t = threadIdx.x / share, i0 = threadIdx.x & (share - 1), nv = K / 8;
+    const bf16x8* row = reinterpret_cast<const bf16x8*>(static_cast<const bf16*>(x) + (t < T ? t : 0) * ldx);
+    bf16x8 p[HELD_PIECES];
+    uint32_t top = 0;
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      mma_s8(acc, a[u][0].x, a[u][1].x, a[u][0].y, a[u][1].y, b[u].x, b[u].y);
-      mma_s8(acc, a[u][0].z, a[u][1].z, a[u][0].w, a[u][1].w, b[u].z, b[u].w);
+    for (int j = 0; j < HELD_PIECES; ++j)
+      if (t < T && i0 + share * j < nv) p[j] = row[i0 + share * j];
+#pragma unroll
+    for (int j = 0; j < HELD_PIECES; ++j)
+      if (t < T && i0 + share * j < nv) {
+        float f[8];
+        unpack8(p[j], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, magnitude(f[e]));
+      }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (share > 32) {
+      if (lane == 0) s_top[warp] = top;
+      __syncthreads();
+      const int first = t * (share >> 5);
+      for (int k = 0; k < (share >> 5); ++k) top = max(top, s_top[first + k]);
+    }
+    const Codes c = codes_of(top);
+    if (t < T) {
+      if (i0 == 0) s_sx[t] = c.scale;
+#pragma unroll
+      for (int j = 0; j < HELD_PIECES; ++j) {
+        const int i = i0 + share * j;
+        if (i * 8 >= kp) continue;
+        float f[8] = {};
+        if (i < nv) unpack8(p[j], f);
+        *reinterpret_cast<uint2*>(s_x + t * stride + i * 8) = codes8(f, i < nv ? c.inv : 0.f);
+      }
+    }
+    __syncthreads();
+  }
+  int turn = 0;
+  for (int block = blockIdx.x; block < blocks; block += gridDim.x, turn ^= 1) {
+    int acc[4] = {};
+    for (int k0 = warp * 64; k0 < kp; k0 += 512 * FEW_UNROLL) {
+      if (k0 != warp * 64) ask(block, k0);
+      uint4 b[FEW_UNROLL];
+#pragma unroll
+      for (int u = 0; u < FEW_UNROLL; ++u) {
+        const int k = k0 + u * 512 + (lane & 3) * 16;
+        b[u] = zero;
+        if (k < kp && tok < T)
+          b[u] = HELD ? *reinterpret_cast<const uint4*>(s_x + tok * stride + k) : *reinterpret_cast<const uint4*>(static_cast<const int8_t*>(x) + tok * ldx + k);
+      }
+#pragma unroll
+      for (int u = 0; u < FEW_UNROLL; ++u) {
+        mma_s8(acc, a[u][0].x, a[u][1].x, a[u][0].y, a[u][1].y, b[u].x, b[u].y);
+        mma_s8(acc, a[u][0].z, a[u][1].z, a[u][0].w, a[u][1].w, b[u].z, b[u].w);
+      }
+    }
+    if (block + (int)gridDim.x < blocks) ask(block + gridDim.x, warp * 64);          // on their way while the sums meet
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s_sum[turn][warp][(lane & 3) * 2 + (e & 1)][(lane >> 2) + (e >> 1) * 8] = acc[e];
+    __syncthreads();                                                     // two buffers: one barrier a block
+    const int t = threadIdx.x >> 4, c = threadIdx.x & 15, n = block * 16 + c;
+    if (t < T && n < N) {                                                // 16 threads a token: those from 8 on have none
+      int sum = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += s_sum[turn][k][t][c];
+      y[t * ldy + n] = (Out)((float)sum * ((HELD ? s_sx[t] : sx[t]) * sw[n]));
     }
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) s_sum[warp][(lane & 3) * 2 + (e & 1)][(lane >> 2) + (e >> 1) * 8] = acc[e];
-  __syncthreads();
-  const int t = threadIdx.x >> 4, c = threadIdx.x & 15, n = n0 + c;
-  if (t >= T || n >= N) return;                                          // 16 threads a token: those from 8 on have none
-  int sum = 0;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) sum += s_sum[k][t][c];
-  y[t * ldy + n] = (Out)((float)sum * (sx[t] * sw[n]));
 }
 
-constexpr int FEW = 8;         // tokens of one instruction
-template <class Out>
-int gemm_q8_few(const int8_t* x, const int8_t* w, const float* sx, const float* sw, Out* y, int T, int N, int K, ll ldx, ll ldw, ll ldy,
-                cudaStream_t st) {
-  return (int)launch_pdl(gemm_q8_few_kernel<Out>, (N + 15) / 16, 256, 0, st, x, w, sx, sw, y, T, N, K, ldx, ldw, ldy);
+template <class Out, bool HELD>
+int gemm_q8_few(const void* x, const void* w, const float* sx, const float* sw, void* y, int T, int N, int K, ll ldx, ll ldw, ll ldy, void* st) {
+  const int blocks = (N + 15) / 16, resident = 3 * tplr_sm_count(), turns = (blocks + resident - 1) / resident;
+  return (int)launch_pdl(gemm_q8_few_kernel<Out, HELD>, (blocks + turns - 1) / turns, 256, 0, (cudaStream_t)st, x, (const int8_t*)w, sx, sw, (Out*)y, T, N, K, ldx,
+                         ldw, ldy);
 }
 
 template <class... P>
@@ -855,7 +914,17 @@ TPLR_API int tplr_gemm_q8(const void* x, const void* w, const float* sx, const f
   if (K <= 0 || K > 131072 || (ldx | ldw) % 16 || (((uintptr_t)x | (uintptr_t)w) & 15)) return (int)cudaErrorInvalidValue;
   if (T > FEW) return (T <= (K >= 8192 ? 128 : 64) ? tplr_gemm_q8_stream : tplr_gemm2_q8)(x, w, sx, sw, y, T, N, K, ldx, ldw, ldy, out_fp32,
                                                                                           status, stream);
-  cudaStream_t st = (cudaStream_t)stream;
-  if (out_fp32) return gemm_q8_few((const int8_t*)x, (const int8_t*)w, sx, sw, (float*)y, T, N, K, ldx, ldw, ldy, st);
-  return gemm_q8_few((const int8_t*)x, (const int8_t*)w, sx, sw, (bf16*)y, T, N, K, ldx, ldw, ldy, st);
+  return (out_fp32 ? gemm_q8_few<float, false> : gemm_q8_few<bf16, false>)(x, w, sx, sw, y, T, N, K, ldx, ldw, ldy, stream);
+}
+
+// tplr_quantize_rows (one scale a row) of bf16 x and tplr_gemm_q8 in one launch, the same bits; y bf16.  -111: more tokens or values than a
+// CTA holds, or rows that are not whole 16-byte pieces.
+TPLR_API int tplr_linear_q8_few(const void* x, const void* w, const float* sw, void* y, int T, int N, int K, ll ldx, ll ldw, ll ldy, void* stream) {
+  TPLR_ENTER();
+  if (T <= 0 || N <= 0) return 0;
+  if (T > FEW || K <= 0 || (ll)T * K > HELD_MOST || K % 8 || ldx % 8 || ldw % 16 || !whole_pieces(x, w)) return -111;
+  int share = 256;
+  while (share * T > 256) share /= 2;
+  if ((K + 15) / 16 * 2 > share * HELD_PIECES) return -111;
+  return gemm_q8_few<bf16, true>(x, w, nullptr, sw, y, T, N, K, ldx, ldw, ldy, stream);
 }

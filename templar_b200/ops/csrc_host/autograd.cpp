@@ -50,6 +50,7 @@ struct Entries {
   decltype(&tplr_rmsnorm_saved8_parts) rmsnorm_saved8_parts;
   decltype(&tplr_rmsnorm_saved8_bwd) rmsnorm_saved8_bwd;
   decltype(&tplr_gemm_q8) gemm_q8;
+  decltype(&tplr_linear_q8_few) linear_q8_few;
   decltype(&tplr_gemm2_swiglu_saved8) swiglu_saved8;
   decltype(&tplr_gemm2_swiglu_bwd_saved8) swiglu_bwd_saved8;
 } E;
@@ -86,6 +87,7 @@ void bind(const std::string& path) {
   get(E.rmsnorm_saved8_parts, "tplr_rmsnorm_saved8_parts");
   get(E.rmsnorm_saved8_bwd, "tplr_rmsnorm_saved8_bwd");
   get(E.gemm_q8, "tplr_gemm_q8");
+  get(E.linear_q8_few, "tplr_linear_q8_few");
   get(E.swiglu_saved8, "tplr_gemm2_swiglu_saved8");
   get(E.swiglu_bwd_saved8, "tplr_gemm2_swiglu_bwd_saved8");
 }
@@ -374,6 +376,14 @@ Tensor linear_q8(const Tensor& x, const Tensor& wq, const Tensor& ws, const Tens
   auto shape = x.sizes().vec();
   shape.back() = N;
   Tensor y = bf16(shape, x);
+  if (T <= 8) {
+    const int err = E.linear_q8_few(x2.data_ptr(), wq.data_ptr(), ws.data_ptr<float>(), y.data_ptr(), (int)T, (int)N, (int)K, x2.stride(0),
+                                    wq.stride(0), N, stream());
+    if (err != -111) {
+      check(err, "linear_q8_few");
+      return y;
+    }
+  }
   Tensor codes = int8({T * (ldq + 4)}, x);
   char* q = static_cast<char*>(codes.data_ptr());
   float* scale = reinterpret_cast<float*>(q + T * ldq);

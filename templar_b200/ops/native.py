@@ -113,6 +113,7 @@ def _declare(L: ctypes.CDLL) -> None:
         "tplr_add_rmsnorm_q8": [vp, vp, vp, vp, vp, ll, vp, ll, i, f, vp],
         "tplr_swiglu_q8": [vp, ll, vp, ll, vp, ll, i, vp],
         "tplr_gemm_q8": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, i, vp, vp],
+        "tplr_linear_q8_few": [vp, vp, vp, vp, i, i, i, ll, ll, ll, vp],
         "tplr_gemm_q8_stream": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, i, vp, vp],
         "tplr_gemm2_swiglu_saved8": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, ll, ll, vp, vp],
         "tplr_gemm2_swiglu_bwd_saved8": [vp, vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, ll, ll, ll, vp, vp],
