@@ -242,18 +242,16 @@ def linear_q8(x: torch.Tensor | QuantRows, w: QuantWeight, out_dtype: torch.dtyp
     """``x @ w.T`` from 8-bit rows and an 8-bit weight: exact sums in 32-bit integers, one scale for each row times one for each
     channel, rounded once to ``out_dtype`` (bf16 or fp32; default: that of ``x``, bf16 for rows in 8 bits).  A tensor ``x`` is
     quantised first, by rows.  Forward passes only."""
-    bf16_out = out_dtype is None or out_dtype is torch.bfloat16
+    out_dtype = out_dtype or (torch.bfloat16 if isinstance(x, QuantRows) else x.dtype)
     if not isinstance(x, QuantRows):
         _no_grad_asked("linear_q8", x)
         if x.dim() == 0 or x.shape[-1] != w.q.shape[1]:
             raise ValueError(f"linear_q8: inner dimensions of {tuple(x.shape)} and {tuple(w.shape)} differ")
         if x.device != w.q.device:
             raise ValueError(f"linear_q8: rows on {x.device}, weight on {w.q.device}")
-        if bf16_out and _native_rows(x) and (host := native.host()):
+        if out_dtype is torch.bfloat16 and _native_rows(x) and (host := native.host()):
             return host.linear_q8(x, w.q, w.scale, OF.status_word(x.device))
-        out_dtype = out_dtype or x.dtype
         x = quantize_rows(x)
-    out_dtype = out_dtype or torch.bfloat16
     if x.group:
         raise ValueError("linear_q8: rows with one scale each are multiplied, got rows with a scale for every "
                          f"{x.group} columns")
@@ -261,7 +259,7 @@ def linear_q8(x: torch.Tensor | QuantRows, w: QuantWeight, out_dtype: torch.dtyp
         raise ValueError(f"linear_q8: inner dimensions {x.width} and {w.shape[1]} differ")
     if x.q.device != w.q.device:
         raise ValueError(f"linear_q8: rows on {x.q.device}, weight on {w.q.device}")
-    if bf16_out and x.q.is_cuda and (host := native.host()):
+    if out_dtype is torch.bfloat16 and x.q.is_cuda and (host := native.host()):
         return host.linear_q8_rows(x.q, x.scale.contiguous(), x.shape, w.q, w.scale, OF.status_word(x.q.device))
     T, N, K = x.q.shape[0], w.shape[0], w.shape[1]
     if x.q.is_cuda and out_dtype in (torch.bfloat16, torch.float32):
@@ -379,15 +377,22 @@ def _kept_input(x, rows: QuantRows | None, weight):
     """(codes, scales, weight) that stand for ``x`` until the backward pass."""
     if rows is None:
         rows, weight = quantize_rows(x, GROUP), None
-    if rows.group != GROUP or rows.shape != x.shape:
-        raise ValueError(f"rows by {GROUP} columns in the shape {tuple(x.shape)} of the input expected, got {tuple(rows.shape)} by "
-                         f"{rows.group or 'row'}")
+    if rows.group != GROUP or rows.shape != x.shape or rows.q.device != x.device:
+        raise ValueError(f"rows by {GROUP} columns in the shape {tuple(x.shape)} of the input on {x.device} expected, got "
+                         f"{tuple(rows.shape)} by {rows.group or 'row'} on {rows.q.device}")
+    if weight is not None and (weight.shape != x.shape[-1:] or weight.device != x.device):
+        raise ValueError(f"{tuple(weight.shape)} weights on {weight.device} for rows of {x.shape[-1]} on {x.device}")
     return rows.q, rows.scale, None if weight is None else weight.detach()
 
 
 def _input_again(q, scale, weight, shape, dtype):
     """The rows that a projection multiplied, from what was kept of them: [T, K]."""
     return _values(q, scale, GROUP, (q.shape[0], shape[-1]), dtype, weight)
+
+
+def _linear_of_nothing(x, w, main_grad):
+    """A projection of no rows; the weight's gradient is zero, so a gradient buffer stays as it is."""
+    return F.linear(x, w if main_grad is None else w.detach())
 
 
 class _LinearSaved8(torch.autograd.Function):
@@ -419,6 +424,8 @@ def linear_saved8(x, w, rows: QuantRows | None = None, weight=None, main_grad=No
         main_grad = getattr(w, "main_grad", None)
     if not torch.is_grad_enabled():
         return OF.linear(x, w, main_grad)
+    if x.numel() == 0:
+        return _linear_of_nothing(x, w, main_grad)
     return _LinearSaved8.apply(x, w, main_grad, *_kept_input(x, rows, weight))
 
 
@@ -518,8 +525,11 @@ def feed_forward_saved8(x, w13, w2, rows: QuantRows | None = None, weight=None, 
         raise ValueError(f"feed_forward_saved8: weights {tuple(w13.shape)} and {tuple(w2.shape)} do not fit rows of {x.shape[-1]}")
     if not torch.is_grad_enabled():
         return OF.feed_forward(x, w13, w2, main_grad13, main_grad2)
+    if x.numel() == 0:
+        gu = _linear_of_nothing(x, w13, main_grad13)
+        return _linear_of_nothing(F.silu(gu[..., :w2.shape[1]]) * gu[..., w2.shape[1]:], w2, main_grad2)
     if (OF._feed_forward_fused(x.reshape(-1, x.shape[-1]), w13, w2) and OF._buffers_ok((main_grad13, w13), (main_grad2, w2))
-            and (host := native.host())):
+            and _native_rows(weight) and (host := native.host())):
         q, scale, weight = (None, None, None) if rows is None else _kept_input(x, rows, weight)
         return host.feed_forward_saved8(x, w13, w2, main_grad13, main_grad2, OF.status_word(x.device), q, scale, weight)
     return _FeedForwardSaved8.apply(x, w13, w2, main_grad13, main_grad2, *_kept_input(x, rows, weight))

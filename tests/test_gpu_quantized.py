@@ -96,6 +96,27 @@ def test_rows_without_tokens_views_and_other_streams():
     assert got.equal(want)
 
 
+@pytest.mark.parametrize("group", [0, 64])
+def test_rows_beyond_32_bit_offsets(group):
+    T, D = 65552, 32768                                    # 2^31 elements and 16 rows more
+    x = torch.zeros(T, D, dtype=torch.bfloat16, device=DEV)
+    x[-16:] = bf(16, D)
+    r = ops.quantize_rows(x, group)
+    q, scale = OQ._codes(x[-16:].float(), group or D)
+    assert r.q[-16:].equal(q) and r.scale[-16:].equal(scale) and not r.q[:16].any()
+    del x
+    v = r.dequantize()
+    assert v[-16:].equal(ops.QuantRows(r.q[-16:].clone(), r.scale[-16:].clone(), group, (16, D)).dequantize())
+
+
+def test_products_beyond_32_bit_offsets():
+    T, K, N = 65552, 64, 32768
+    rows, w = ops.quantize_rows(bf(T, K)), ops.quantize_weight(bf(N, K, seed=1))
+    y = ops.linear_q8(rows, w)
+    want = (rows.q[-16:].double() @ w.q.double().t()) * rows.scale[-16:].double() * w.scale.double()
+    assert ((y[-16:].double() - want).abs() <= want.abs() * HALF).all()
+
+
 def norm64(res, delta):
     h = res if delta is None else (res.float() + delta.float()).to(torch.bfloat16)
     hd = h.double()
@@ -223,6 +244,27 @@ def ffn64(x, w13, w2, dy):
     return y, dgu @ w13, dgu.t() @ kept(x, 64), dy.t() @ act.detach()
 
 
+def test_no_tokens():
+    w13, w2, wn = bf(256, 64).requires_grad_(), bf(64, 128).requires_grad_(), bf(64).requires_grad_()
+    x = bf(0, 64).requires_grad_()
+    for res, delta in ((x, None), (x, bf(0, 64))):
+        h, y, rows = ops.add_rmsnorm_saved8(res, delta, wn)
+        out = ops.feed_forward_saved8(y, w13, w2, rows, wn)
+        grads = torch.autograd.grad(out.sum() + ops.linear_saved8(y, w13).sum() + y.sum(), (w13, w2, wn))
+        assert out.shape == (0, 64) and not any(g.any() for g in grads)
+
+
+def test_fp32_rows_take_the_formulas():
+    x, w = torch.randn(5, 48, device=DEV), ops.quantize_weight(torch.randn(7, 48, device=DEV))
+    rows = ops.quantize_rows(x)
+    y = ops.linear_q8(x, w)
+    want = (rows.q[:, :48].double() @ w.q.double().t()) * rows.scale.double() * w.scale.double()
+    assert y.dtype == torch.float32 and ((y.double() - want).abs() <= want.abs() * 2.0 ** -22).all()
+    assert ((rows.dequantize(torch.float32) - x).abs() <= rows.scale * 0.501).all()
+    h, y, _ = ops.add_rmsnorm_saved8(x, x, torch.ones(48, device=DEV))
+    assert h.dtype == torch.float32 and y.dtype == torch.float32
+
+
 FFN = [(1, 64, 128), (5, 72, 40), (100, 128, 256), (130, 256, 384), (257, 200, 136), (300, 1024, 2816), (513, 512, 1000), (1000, 768, 2048)]
 
 
@@ -290,19 +332,22 @@ ARGS = ModelArgs(dim=256, n_layers=3, n_heads=2, n_kv_heads=1, vocab_size=512, i
 def test_a_training_step_with_saved_activations_in_8_bits():
     tok = torch.randint(0, 512, (4, 129), generator=torch.Generator().manual_seed(0)).to(DEV)
 
-    def step(mode):
+    def step(mode, shard=False):
         m = build_model(ARGS, device=DEV, dtype=torch.bfloat16, seed=3)
         m.activation_checkpointing = mode
-        eng = WindowEngine(m, EngineConfig(), device=DEV)
+        eng = WindowEngine(m, EngineConfig(shard_params=shard), device=DEV)
         torch.cuda.synchronize()
         base = torch.cuda.memory_allocated()
         loss = m.loss(tok[:, :-1], tok[:, 1:])
         held = torch.cuda.memory_allocated() - base
         loss.backward()
-        return float(loss.detach()), eng.store.grad.clone(), held
+        return float(loss.detach()), (eng.store.grad_shard if shard else eng.store.grad).clone(), held
     l0, g0, b0 = step("none")
     l1, g1, b1 = step("int8")
     assert abs(l1 - l0) < 5e-3 and (g1 - g0).norm() < 0.03 * g0.norm() and b1 < 0.75 * b0
+    l0, g0, _ = step("none", True)                                         # gradient targets with a method of their own: the Python nodes
+    l1, g1, _ = step("int8", True)
+    assert abs(l1 - l0) < 5e-3 and (g1 - g0).norm() < 0.03 * g0.norm()
     healthy()
 
 

@@ -169,6 +169,16 @@ def test_feed_forward_keeps_a_third_of_the_bytes_and_takes_the_norms_rows():
     assert (dw - dw0).norm() < 0.02 * dw0.norm()
 
 
+def test_no_tokens():
+    w13, w2, wn = rand(16, 8).requires_grad_(), rand(8, 8).requires_grad_(), rand(8).requires_grad_()
+    x = rand(0, 8).requires_grad_()
+    h, y, rows = ops.add_rmsnorm_saved8(x, None, wn)
+    out = ops.feed_forward_saved8(y, w13, w2, rows, wn)
+    assert out.shape == (0, 8)
+    for g in torch.autograd.grad(out.sum() + ops.linear_saved8(y, w13).sum(), (w13, w2, wn)):
+        assert not g.any()
+
+
 def test_refusals():
     x, w = rand(4, 32), ops.quantize_weight(rand(8, 32, seed=1))
     with pytest.raises(ValueError, match="inner dimensions"):
@@ -203,6 +213,8 @@ def test_refusals():
         ops.QuantRows(torch.zeros(3, 80, dtype=torch.int8), torch.zeros(3, 1), 64, (3, 80))
     with pytest.raises(ValueError, match="do not fit"):
         ops.feed_forward_saved8(x, rand(16, 32), rand(32, 9))
+    with pytest.raises(ValueError, match="weights on"):
+        ops.feed_forward_saved8(x, rand(16, 32), rand(32, 8), ops.quantize_rows(x, 64), torch.ones(31))
     with pytest.raises(ValueError, match="by 64 columns"):
         ops.feed_forward_saved8(x, rand(16, 32), rand(32, 8), ops.quantize_rows(x))
 
@@ -217,10 +229,10 @@ def test_weight_codes_that_end_with_their_storage_are_copied():
     assert ops.QuantWeight(q, torch.ones(3)).q.data_ptr() == q.data_ptr()
 
 
-def _step(mode, packed=True):
+def _step(mode, packed=True, shard=False):
     m = build_model(ARGS, seed=3)
     m.activation_checkpointing = mode
-    eng = WindowEngine(m, EngineConfig(), device="cpu") if packed else None
+    eng = WindowEngine(m, EngineConfig(shard_params=shard), device="cpu") if packed else None
     tok = torch.randint(0, 256, (3, 33), generator=torch.Generator().manual_seed(0))
     stored = [0]
 
@@ -230,13 +242,15 @@ def _step(mode, packed=True):
     with ag.saved_tensors_hooks(pack, lambda t: t):
         loss = m.loss(tok[:, :-1], tok[:, 1:])
     loss.backward()
+    if shard:
+        return float(loss.detach()), eng.store.stage.clone(), stored[0]
     return float(loss.detach()), eng.store.grad.clone() if packed else torch.cat([p.grad.flatten() for p in m.parameters()]), stored[0]
 
 
-@pytest.mark.parametrize("packed", [True, False])
-def test_a_training_step_with_saved_activations_in_8_bits(packed):
-    l0, g0, b0 = _step("none", packed)
-    l1, g1, b1 = _step("int8", packed)
+@pytest.mark.parametrize("packed,shard", [(True, False), (False, False), (True, True)])
+def test_a_training_step_with_saved_activations_in_8_bits(packed, shard):
+    l0, g0, b0 = _step("none", packed, shard)
+    l1, g1, b1 = _step("int8", packed, shard)
     # the forward pass computes the same thing; gradients are off by what 8 bits leave out
     assert abs(l1 - l0) < 1e-5 and (g1 - g0).norm() < 0.02 * g0.norm() and b1 < b0
 
