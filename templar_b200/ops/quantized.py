@@ -13,6 +13,8 @@ PyTorch, as in :mod:`templar_b200.ops.functional`.
 
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as F
 
@@ -64,6 +66,8 @@ class QuantRows:
         D = shape[-1]
         if q.dtype != torch.int8 or q.dim() != 2 or q.shape[1] != _padded(D) or q.stride() != (q.shape[1], 1):
             raise ValueError(f"QuantRows: dense int8 codes [T, {_padded(D)}] expected, got {q.dtype} {tuple(q.shape)}, strides {q.stride()}")
+        if math.prod(shape[:-1]) != q.shape[0]:
+            raise ValueError(f"QuantRows: {q.shape[0]} rows of codes for the shape {tuple(shape)}")
         if scale.dtype != torch.float32 or scale.shape != (q.shape[0], -(-D // group) if group else 1) or scale.device != q.device:
             raise ValueError(f"QuantRows: fp32 scales [{q.shape[0]}, {-(-D // group) if group else 1}] on {q.device} expected, got "
                              f"{scale.dtype} {tuple(scale.shape)} on {scale.device}")

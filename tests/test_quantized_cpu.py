@@ -209,6 +209,8 @@ def test_refusals():
         ops.QuantWeight(torch.zeros(1, 131088, dtype=torch.int8), torch.zeros(1))
     with pytest.raises(ValueError, match="dense int8 codes"):
         ops.QuantRows(torch.zeros(3, 20, dtype=torch.int8), torch.zeros(3, 1), 0, (3, 20))
+    with pytest.raises(ValueError, match="3 rows of codes"):
+        ops.QuantRows(torch.zeros(3, 32, dtype=torch.int8), torch.zeros(3, 1), 0, (4, 20))
     with pytest.raises(ValueError, match="fp32 scales"):
         ops.QuantRows(torch.zeros(3, 80, dtype=torch.int8), torch.zeros(3, 1), 64, (3, 80))
     with pytest.raises(ValueError, match="do not fit"):
