@@ -154,7 +154,7 @@ Tensor weight_grad(const Tensor& buffer, const Tensor& dy2, const Tensor& x2, co
   gemm(dy2, x2, dw, true, true, 0, status);
   return dw;
 }
-Tensor rows(const Tensor& t) { return t.reshape({-1, t.size(-1)}); }
+Tensor rows(const Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
 // rows of a tensor whose last dimension is D; an integer division by zero would end the process
 ll count_rows(const Tensor& t, ll D) {
   TORCH_CHECK(D > 0, "rows of no elements");
@@ -361,6 +361,7 @@ std::pair<Tensor, Tensor> quantize(const Tensor& x, int group) {
 }
 // the values of codes, in bf16: `shape` is that of the result, w may be undefined
 Tensor dequantize(const Tensor& q, const Tensor& scale, ll group, at::IntArrayRef shape, const Tensor& w) {
+  const at::AutoDispatchBelowADInplaceOrView guard;
   const ll D = shape.back();
   Tensor y = at::empty(shape, q.options().dtype(at::kBFloat16));
   const Tensor wc = w.defined() ? w.contiguous() : w;
@@ -371,6 +372,7 @@ Tensor dequantize(const Tensor& q, const Tensor& scale, ll group, at::IntArrayRe
 }
 // x in 8 bits by rows, times an 8-bit weight; the codes live for this call alone, with their scales behind them
 Tensor linear_q8(const Tensor& x, const Tensor& wq, const Tensor& ws, const Tensor& status) {
+  const at::AutoDispatchBelowADInplaceOrView guard;
   const Tensor x2 = dense_rows(x);
   const ll T = x2.size(0), K = x2.size(1), N = wq.size(0), ldq = padded(K);
   auto shape = x.sizes().vec();
@@ -412,14 +414,21 @@ bool weight_as_it_is(const Tensor& q, const Tensor& scale) {
          reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(scale.data_ptr()) % 16 == 0 &&
          q.storage_offset() + (N - 1) * ld + wide <= (ll)q.storage().nbytes();
 }
-std::tuple<Tensor, Tensor, Tensor> add_rmsnorm_q8(const Tensor& res, const std::optional<Tensor>& delta, const Tensor& w, double eps) {
+bool bf16_cuda(const Tensor& t) { return t.is_cuda() && t.scalar_type() == at::kBFloat16; }
+// nothing: operands that are not for the kernels, or not for this call, of which ops/quantized.py says more
+std::optional<std::tuple<Tensor, Tensor, Tensor>> add_rmsnorm_q8(const Tensor& res, const std::optional<Tensor>& delta, const Tensor& w,
+                                                                 double eps) {
+  if (!bf16_cuda(res) || !bf16_cuda(w) || (delta && !(bf16_cuda(*delta) && delta->sizes() == res.sizes()))) return std::nullopt;
+  if (res.dim() == 0 || res.size(-1) == 0 || w.dim() != 1 || w.size(0) != res.size(-1)) return std::nullopt;
+  if (at::GradMode::is_enabled() && (res.requires_grad() || w.requires_grad() || (delta && delta->requires_grad()))) return std::nullopt;
+  const at::AutoDispatchBelowADInplaceOrView guard;
   const Tensor x2 = rows(res).contiguous(), wc = w.contiguous(), d = delta ? delta->contiguous() : Tensor();
   const ll T = x2.size(0), D = x2.size(1);
   Tensor h = delta ? bf16(res.sizes(), res) : res, q = int8({T, padded(D)}, res), scale = f32({T, 1}, res);
   check(E.add_rmsnorm_q8(x2.data_ptr(), delta ? d.data_ptr() : nullptr, wc.data_ptr(), delta ? h.data_ptr() : nullptr, q.data_ptr(),
                          q.stride(0), scale.data_ptr<float>(), T, (int)D, (float)eps, stream()),
         "add_rmsnorm_q8");
-  return {h, q, scale};
+  return std::make_tuple(h, q, scale);
 }
 
 // (h, y, codes, scales) of the training norm; delta undefined: h is the input's and not a result

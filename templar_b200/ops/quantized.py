@@ -85,7 +85,10 @@ class QuantRows:
         return self.shape[-1]
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16, weight: torch.Tensor | None = None) -> torch.Tensor:
-        return dequantize_rows(self, dtype, weight)
+        """:func:`dequantize_rows`."""
+        if weight is not None:
+            return dequantize_rows(self, dtype, weight)
+        return _values(self.q, self.scale, self.group, self.shape, dtype)
 
 
 def _empty_rows(shape, group: int, device) -> tuple[torch.Tensor, torch.Tensor]:
@@ -195,6 +198,8 @@ def _no_grad_asked(what: str, *ts) -> None:
 
 def add_rmsnorm_q8(res: torch.Tensor, delta: torch.Tensor | None, w: torch.Tensor, eps: float = 1e-5) -> tuple[torch.Tensor, QuantRows]:
     """``(res + delta, rmsnorm(res + delta) * w)``, the second in 8 bits with one scale a row (``delta`` None: of ``res``)."""
+    if res.is_cuda and (host := native.host()) and (made := host.add_rmsnorm_q8(res, delta, w, eps)) is not None:
+        return (res if delta is None else made[0]), QuantRows._of(made[1], made[2], 0, res.shape)
     _no_grad_asked("add_rmsnorm_q8", res, delta, w)
     _norm_args("add_rmsnorm_q8", res, delta, w)
     if not _native_rows(res, delta, w):
@@ -202,9 +207,6 @@ def add_rmsnorm_q8(res: torch.Tensor, delta: torch.Tensor | None, w: torch.Tenso
         hf = _rows_of(h.float())
         y = hf * torch.rsqrt(hf.pow(2).mean(-1, keepdim=True) + eps) * w.float()
         return h, QuantRows._of(*_plain_rows(y, 0), 0, res.shape)
-    if host := native.host():
-        h, q, scale = host.add_rmsnorm_q8(res, delta, w, eps)
-        return (res if delta is None else h), QuantRows._of(q, scale, 0, res.shape)
     x2, w = _rows_of(res).contiguous(), w.contiguous()
     T, D = x2.shape
     d2 = None if delta is None else delta.contiguous()
