@@ -759,10 +759,10 @@ __device__ __forceinline__ void epilogue_swiglu_q8(const Gemm2Params& p, uint32_
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[hh * 32 + e] = __uint_as_float(r[e]);
       }
-      uint32_t top = 0;
+      float top = 0.f;
 #pragma unroll
-      for (int e = 0; e < 64; ++e) top = max(top, magnitude(v[e]));
-      const Codes q = codes_of(top);
+      for (int e = 0; e < 64; e += 2) top = top3(top, v[e], v[e + 1]);
+      const Codes q = codes_of(magnitude(top));
       if (row0 + lane < p.M) p.q8_scale[(long long)((part * p.swiglu_f + f0) / QUANT_GROUP) * p.q8_ld + row0 + lane] = q.scale;
       const uint32_t buf = box_begin(lane, stage_base, n_boxes), rowaddr = box64_row(buf, lane);
 #pragma unroll

@@ -163,7 +163,7 @@ __device__ __forceinline__ void values8(const uint2& q, float scale, float* f) {
 // read once and its two reductions (the squares, the largest magnitude) run on values that are already there.  Several rows a CTA
 // share its barriers.  Memory bounds it: a thread asks for all its pieces before it waits for the first.
 template <int MODE, int VPL, int BLOCK>
-__global__ void __launch_bounds__(BLOCK) rows_q8_kernel(const RowsArgs p, const int tpr) {
+__global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) rows_q8_kernel(const RowsArgs p, const int tpr) {
   constexpr bool NORM = MODE == NORM_ROWS || MODE == NORM_SAVED, BY_GROUP = MODE == GROUPS || MODE == NORM_SAVED;
   __shared__ float s_sum[32];
   __shared__ uint32_t s_top[32];
@@ -193,17 +193,17 @@ __global__ void __launch_bounds__(BLOCK) rows_q8_kernel(const RowsArgs p, const 
         for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
         continue;
       }
+      if (NORM && two) {                                                 // the norm sees the sum as the residual stream stores it
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ra[j].v[e] = __hadd2(ra[j].v[e], rb[j].v[e]);
+        reinterpret_cast<bf16x8*>(p.h + row * D)[i] = ra[j];
+      }
       unpack8(ra[j], v[j]);
-      if (two) {
+      if (MODE == SWIGLU_ROWS) {
         float o[8];
         unpack8(rb[j], o);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] = MODE == SWIGLU_ROWS ? silu_mul(v[j][e], o[e]) : v[j][e] + o[e];
-        if (NORM) {                                                      // the norm sees the sum as the residual stream stores it
-          const bf16x8 h = pack8(v[j]);
-          reinterpret_cast<bf16x8*>(p.h + row * D)[i] = h;
-          unpack8(h, v[j]);
-        }
+        for (int e = 0; e < 8; ++e) v[j][e] = silu_mul(v[j][e], o[e]);
       }
     }
   }
@@ -250,9 +250,10 @@ __global__ void __launch_bounds__(BLOCK) rows_q8_kernel(const RowsArgs p, const 
   uint32_t tops[VPL];
 #pragma unroll
   for (int j = 0; j < VPL; ++j) {
-    tops[j] = 0;
+    float top = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) tops[j] = max(tops[j], magnitude(v[j][e]));
+    for (int e = 0; e < 8; e += 2) top = top3(top, v[j][e], v[j][e + 1]);
+    tops[j] = magnitude(top);
   }
   Codes all = {};
   if (!BY_GROUP) {

@@ -13,6 +13,12 @@ static __device__ __forceinline__ Codes codes_of(uint32_t top) {
   return {127.f / a, a / 127.f};
 }
 static __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// The largest magnitude of three, one of them a largest magnitude already; NaN where one is NaN.
+static __device__ __forceinline__ float top3(float t, float x, float y) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(t), "f"(x), "f"(y));
+  return r;
+}
 
 // Four codes in a word.  Added to 1.5 * 2^23, a number's last bits are its nearest whole number (ties to even, as rint) in two's
 // complement: conversion instructions run at a sixteenth of the rate.  |x * inv| is at most 127 (1 + 2^-23) and never rounds to
