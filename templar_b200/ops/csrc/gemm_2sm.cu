@@ -45,7 +45,7 @@ static_assert(4 * 8192 <= STAGE_BYTES, "the freed stage holds four warps' second
 // so that one has instructions while the other waits.  What they stage beyond 32 KB takes a stage of the ring.
 constexpr int epi_warps(int epi) { return epi == 7 || epi == 8 || epi == 10 ? 8 : 4; }
 constexpr int num_threads(int epi) { return 64 + 32 * epi_warps(epi); }
-constexpr int ring_stages(int epi) { return epi == 5 || epi == 7 || epi == 8 || epi == 10 ? EPI5_STAGES : STAGES; }
+constexpr int ring_stages(int epi) { return epi == 5 || epi == 10 ? EPI5_STAGES : STAGES; }
 constexpr int MAX_RANKS = 8;
 constexpr int CHUNK_ROWS = 128;                    // gather / scatter flag granularity (rows)
 
@@ -657,11 +657,13 @@ __device__ __forceinline__ void epilogue_attn_dout(const Gemm2Params& p, uint32_
 
 // Epilogue of a product of 8-bit rows (EPI 7 stores bf16, EPI 8 fp32): the int32 accumulator times the scales of its row (one a
 // lane) and its column (the same for all lanes: 16-byte loads that the L1 answers).  Columns from N on are not stored; where C takes
-// no TMA store (a row stride that is not a multiple of 16 bytes) a warp writes its staged box row by row, 32 columns of one row at a
-// time, since a lane that stores its own row touches 32 lines an instruction.
+// no TMA store (a row stride that is not a multiple of 16 bytes) a warp writes its staged box eight rows at a time, 32 columns
+// of a row an instruction, since a lane that stores its own row touches 32 lines: 777 x 1003 x 1111 9.2 us, 777 x 1008 x 1112 by TMA 7.5.
+// K of 2048 and more is bound by the main loop (4096 x 2048 x 16384: 94 us, 2918 T/s, tensor pipe 82 % busy at the 1.67 GHz that the
+// power cap leaves; 2048 x 8192 x 8192 3130 T/s); shorter ones by this, the proxy fence and the loads of a box: 8192 x 512 x 4096 27 us.
 template <bool F32>
 __device__ __forceinline__ void epilogue_q8(const Gemm2Params& p, uint32_t tmem_acc, int quad, int turn, int lane, int m0, int n0,
-                                            uint32_t stage_base, uint32_t& n_boxes) {
+                                            uint32_t buf, uint32_t& n_boxes) {
   constexpr int COLS = F32 ? 32 : 64;
   const int row0 = m0 + quad * 32;
   if (row0 >= p.M) return;                           // warp-uniform
@@ -671,24 +673,31 @@ __device__ __forceinline__ void epilogue_q8(const Gemm2Params& p, uint32_t tmem_
   for (int c = turn; c < p.tile_n / COLS; c += 2) {
     const int col0 = n0 + c * COLS;
     if (col0 >= p.N) break;                          // warp-uniform
-    const uint32_t buf = box_begin(lane, stage_base, n_boxes);
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // one box a warp: the other warp of the quadrant works meanwhile
+    __syncwarp();
 #pragma unroll
     for (int hh = 0; hh < COLS / 32; ++hh) {
       const int col = col0 + hh * 32;
+      float4 sc[8];                                  // asked for in front of the accumulator: nothing passes its wait
+      if (col + 32 <= p.N) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sc[e] = reinterpret_cast<const float4*>(p.q8_col + col)[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          sc[e].x = col + 4 * e < p.N ? p.q8_col[col + 4 * e] : 0.f;
+          sc[e].y = col + 4 * e + 1 < p.N ? p.q8_col[col + 4 * e + 1] : 0.f;
+          sc[e].z = col + 4 * e + 2 < p.N ? p.q8_col[col + 4 * e + 2] : 0.f;
+          sc[e].w = col + 4 * e + 3 < p.N ? p.q8_col[col + 4 * e + 3] : 0.f;
+        }
+      }
       uint32_t r[32];
       float v[32];
       tmem_ld32(tmem_acc + c * COLS + hh * 32 + lane_sel, r);
-      if (col + 32 <= p.N) {
-        const float4* sc = reinterpret_cast<const float4*>(p.q8_col + col);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float4 q = sc[e];
-          v[4 * e] = (float)(int)r[4 * e] * (sr * q.x); v[4 * e + 1] = (float)(int)r[4 * e + 1] * (sr * q.y);
-          v[4 * e + 2] = (float)(int)r[4 * e + 2] * (sr * q.z); v[4 * e + 3] = (float)(int)r[4 * e + 3] * (sr * q.w);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = col + e < p.N ? (float)(int)r[e] * (sr * p.q8_col[col + e]) : 0.f;
+      for (int e = 0; e < 8; ++e) {
+        v[4 * e] = (float)(int)r[4 * e] * (sr * sc[e].x); v[4 * e + 1] = (float)(int)r[4 * e + 1] * (sr * sc[e].y);
+        v[4 * e + 2] = (float)(int)r[4 * e + 2] * (sr * sc[e].z); v[4 * e + 3] = (float)(int)r[4 * e + 3] * (sr * sc[e].w);
       }
       if (F32) {
         const uint32_t rowaddr = buf + (uint32_t)lane * 128u, sw = (uint32_t)(lane & 7);
@@ -735,8 +744,8 @@ __device__ __forceinline__ void epilogue_q8(const Gemm2Params& p, uint32_t tmem_
 // Epilogue of the fused [w1; w3] projection whose gate and up values are kept in 8 bits for the backward pass (EPI 9): as
 // epilogue_swiglu, but a row's 64 values of either half, a group, leave as codes with one scale instead of as bf16: half the
 // bytes of its two larger outputs.  The codes are made from the fp32 accumulators.  A lane has a row, so a group's largest
-// magnitude needs no exchange, and 32 rows' scales of a group lie side by side.
-// 16384 x 2048 -> 8192: XX us, where the bf16 form takes XX.
+// magnitude needs no exchange, and 32 rows' scales of a group lie side by side.  The main loop bounds it (the tensor pipe 86 % busy), so
+// what is gained is memory: in turn with the bf16 form, 16384 x 2048 -> 8192 797 and 815 us, 2048 x 768 -> 2048 25.8 and 27.4.
 __device__ __forceinline__ uint32_t box64_row(uint32_t buf, int row) { return buf + (uint32_t)row * 64u; }      // box of 64 bytes a row,
 __device__ __forceinline__ uint32_t box64_at(int row, int j) { return (uint32_t)(j ^ ((row >> 1) & 3)) << 4; }  // 64-byte swizzle
 __device__ __forceinline__ void epilogue_swiglu_q8(const Gemm2Params& p, uint32_t tmem_acc, int quad, int lane, int m0, int tn,
@@ -795,7 +804,9 @@ __device__ __forceinline__ void epilogue_swiglu_q8(const Gemm2Params& p, uint32_
 // quadrant share a box of codes and the three boxes that leave, half the columns each: the first one's first lane moves them.
 // One warp a quadrant that did both halves was the longest part of the kernel (4096 x 2048 -> 8192: 128 us, the tensor pipe busy
 // for 55 % of them); with boxes of 32 columns for each warp alone the stores' 64-byte pieces were (16384 rows: 539 -> 670 us).
-// 16384 x 2048 -> 8192: XX us, the bf16 form 450 without the activation.
+// In turn with the bf16 form, which forms no activation: 16384 x 2048 -> 8192 558 and 468 us, 4096 x 4096 -> 14336 397 and 377, 2048 x 768 ->
+// 2048 22.9 and 22.9.  Left: the third output's bytes, and fixed latencies of a step (tensor pipe 57 % busy, an instruction in 16 % of
+// the cycles).
 constexpr uint32_t CODE_STAGE = 4096 + 3 * 4096;     // a quadrant's codes of 64 columns, gate and up; three boxes of 64 columns
 struct CodeLoads {
   uint32_t bar;                      // the quadrant's mbarrier
@@ -1098,7 +1109,7 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
           epilogue_rope<128>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
         else if (EPI == 4 && p.rope_dh == 64 && p.rope_cols % 64 == 0)
           epilogue_rope<64>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
-        else if (I8)       epilogue_q8<EPI == 8>(p, tmem_acc, quad, turn, lane, m0, n0, sEpi + (uint32_t)(warp - 2) * 8192u, n_boxes);
+        else if (I8)       epilogue_q8<EPI == 8>(p, tmem_acc, quad, turn, lane, m0, n0, sEpi + (uint32_t)(warp - 2) * 4096u, n_boxes);
         else if (p.c_tma)  epilogue_tma<EPI>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes, w.t % p.k_splits);
         else               epilogue_direct<EPI>(p, tmem_acc, quad, lane, m0, n0);
         tcgen05_fence_before();
