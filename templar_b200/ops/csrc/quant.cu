@@ -161,7 +161,9 @@ __device__ __forceinline__ void values8(const uint2& q, float scale, float* f) {
 
 // The same from registers, for rows of whole 16-byte pieces: `tpr` threads (a power of two) share a row, VPL pieces each, so a row is
 // read once and its two reductions (the squares, the largest magnitude) run on values that are already there.  Several rows a CTA
-// share its barriers.  Memory bounds it: a thread asks for all its pieces before it waits for the first.
+// share its barriers.  A thread asks for all its pieces before it waits for the first.  16384 x 2048: norm in 8 bits 45 us, its training form
+// 56, codes by row 21, the activation of 16384 x 1024 in 8 bits 17: 4.9 to 5.4 TB/s, 75 to 83 % of what a plain copy of 2 GB moves; what is left
+// are a CTA's loads, barriers and stores in turn (in the training form an instruction is issued in 55 % of the cycles).
 template <int MODE, int VPL, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) rows_q8_kernel(const RowsArgs p, const int tpr) {
   constexpr bool NORM = MODE == NORM_ROWS || MODE == NORM_SAVED, BY_GROUP = MODE == GROUPS || MODE == NORM_SAVED;
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(256) dequantize_any_kernel(const int8_t* q, ll
 }
 
 // The same for whole 16-byte pieces of y, a scale for a row or for 64 columns: `tpr` threads (a power of two) on a row, four pieces each,
-// all asked for before the first is written.
+// all asked for before the first is written.  16384 x 2048 by 64 columns: 21 us (4.7 TB/s), 32 in a loop whose loads stood behind its stores.
 __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* q, ll ldq, const float* scale, ll scale_row, ll scale_group,
                                                          const bf16* w, bf16* y, ll T, int D, int tpr) {
   grid_wait();
@@ -425,7 +427,8 @@ __device__ __forceinline__ void copy8(uint32_t dst, const void* src) { asm volat
 // over all rows of the CTA.  What keeps the memory busy are the copies of the two rows after the present one, each thread's own
 // pieces into its own shared memory, so that no barrier stands between them and their use.
 // Counters of a first form (16384 x 2048): the memory 45 % busy, an instruction issued in 72 % of the cycles; so the weight stays unpacked, the
-// products and the codes' numbers of a piece stay for its output, and a scale multiplies once a piece where it can, and the next row's scales are asked for a row ahead: 57 -> 47 us.
+// products and the codes' numbers of a piece stay for its output, and a scale multiplies once a piece where it can, and the next row's scales are asked for
+// a row ahead: 57 -> 47 us, 5.0 TB/s.
 constexpr int BWD_STAGES = 3, BWD_VPL = 2;
 template <int BLOCK>
 __global__ void __launch_bounds__(BLOCK, 512 / BLOCK)
@@ -641,7 +644,8 @@ __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_
 }
 //
 // HELD: x is bf16 and its rows are put in 8 bits here, by every CTA for itself, while its first pieces of the weight are on their way: as
-// many values as the threads hold, HELD_MOST; one launch instead of two.
+// many values as the threads hold, HELD_MOST; one launch instead of two.  One token, one launch and two: 2048 x 2048 3.1 and 4.1 us, 4096 x 6144
+// 6.9 and 8.5, 2048 x 16384 8.5 and 9.8 (4.0 TB/s); with 16384 values held a call of the last took 13.7, two CTAs an SM.
 constexpr int FEW = 8, FEW_UNROLL = 4, HELD_MOST = 4096, HELD_PIECES = HELD_MOST / 2048;
 __host__ __device__ constexpr int held_stride(int kp) { return (kp + 511) / 512 * 512 + 64; }          // rows 64 bytes apart in the banks
 template <class Out, bool HELD>
@@ -767,11 +771,14 @@ int rows_q8(const RowsArgs& p, void* stream) {
   if (p.D % 8 || p.ldq % 8 || p.lda % 8 || (p.b && p.ldb % 8) || p.D > 32760 || !whole_pieces(p.a, p.b, p.w, p.h, p.y, p.q))
     return (int)launch_pdl(p.D <= 1024 ? rows_q8_any_kernel<MODE, 4> : p.D <= 2048 ? rows_q8_any_kernel<MODE, 8> : p.D <= 4096 ? rows_q8_any_kernel<MODE, 16>
                            : p.D <= 8192 ? rows_q8_any_kernel<MODE, 32> : rows_q8_any_kernel<MODE, 0>, (unsigned)p.T, 256, 0, st, p);
-  // one piece a thread while that leaves threads to spare on the chip, four where rows are many
-  const int vpl = p.T * pieces <= 2048LL * tplr_sm_count() && pieces <= 1024 ? 1 : 4;
-  const int tpr = row_threads(pieces, vpl), block = tpr > 256 ? 1024 : 256;
+  // One piece a thread while rows are few, four where they are many.  Microseconds with one and with four: norm in 8 bits 1 x 2048 2.3 and 3.3,
+  // 128 x 2048 2.4 and 4.0, 512 x 2048 3.6 and 4.1, 1024 x 2048 6.1 and 5.9, 4096 x 768 8.2 and 7.3; codes alone 64 x 768 1.6 and 2.0, 128 x 2048
+  // 1.8 and 2.1, 512 x 2048 2.7 and 2.2.
+  const bool codes_alone = MODE == ROWS || MODE == GROUPS;
+  const int vpl = p.T * pieces <= (codes_alone ? 512LL : 1024LL) * tplr_sm_count() && pieces <= 1024 ? 1 : 4;
+  const int tpr = row_threads(pieces, vpl), block = tpr > 256 ? tpr : 256;
   const unsigned grid = (unsigned)((p.T + block / tpr - 1) / (block / tpr));
-  if (block == 1024) return (int)(vpl == 1 ? launch_pdl(rows_q8_kernel<MODE, 1, 1024>, grid, block, 0, st, p, tpr)
+  if (block > 256) return (int)(vpl == 1 ? launch_pdl(rows_q8_kernel<MODE, 1, 1024>, grid, block, 0, st, p, tpr)
                                            : launch_pdl(rows_q8_kernel<MODE, 4, 1024>, grid, block, 0, st, p, tpr));
   return (int)(vpl == 1 ? launch_pdl(rows_q8_kernel<MODE, 1, 256>, grid, block, 0, st, p, tpr)
                         : launch_pdl(rows_q8_kernel<MODE, 4, 256>, grid, block, 0, st, p, tpr));
