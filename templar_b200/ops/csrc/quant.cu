@@ -662,15 +662,13 @@ __global__ void __launch_bounds__(256, 3) gemm_q8_few_kernel(const void* x, cons
   const uint4 zero = make_uint4(0, 0, 0, 0);
   uint4 a[FEW_UNROLL][2];
   auto ask = [&](int block, int k0) {
+    const int n = block * 16 + (lane >> 2);
+    const int8_t *r0 = w + (ll)min(n, N - 1) * ldw, *r1 = w + (ll)min(n + 8, N - 1) * ldw;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int n = block * 16 + h * 8 + (lane >> 2);
-      const int8_t* row = w + (ll)min(n, N - 1) * ldw;
-#pragma unroll
-      for (int u = 0; u < FEW_UNROLL; ++u) {
-        const int k = k0 + u * 512 + (lane & 3) * 16;
-        a[u][h] = k < kp && n < N ? ld_once(row + k) : zero;
-      }
+    for (int u = 0; u < FEW_UNROLL; ++u) {
+      const int k = k0 + u * 512 + (lane & 3) * 16;
+      a[u][0] = k < kp && n < N ? ld_once(r0 + k) : zero;
+      a[u][1] = k < kp && n + 8 < N ? ld_once(r1 + k) : zero;
     }
   };
   ask(blockIdx.x, warp * 64);
@@ -911,16 +909,17 @@ extern "C" int tplr_gemm_q8_stream(const void* X, const void* W, const float* sx
 // bytes of a row from K to the next 16-byte boundary are read: zeros in x, anything in w.
 //
 // Which kernel: up to 8 tokens the one that loads the weight into registers, up to 64 the weight's rows as the tensor core's long side
-// with K cut over clusters, more on CTA pairs; up to 128 tokens the cut still wins where K is long.  Microseconds, the
-// three in that order, inner dimension x channels at 8 | 32 | 64 | 128 tokens: 2048 x 2048 2.8, 3.9, 7.5 | 7.4, 4.9, 7.5 | -, 6.7, 7.5 |
-// -, 10.4, 8.0; 4096 x 6144 6.5, 8.8, 14.5 | 15.6, 9.6, 11.5 | -, 11.7, 11.5 | -, 18.5, 12.1; 2048 x 16384 8.9, 9.2, 14.8 | 17.3, 9.9, 14.4 |
-// -, 12.0, 13.9 | -, 16.0, 14.5; 14336 x 4096 13.7, 13.4, 34.1 | 42.5, 13.8, 24.4 | -, 15.2, 24.6 | -, 19.0, 25.2; 8192 x 2048 at 128: 13.7, 16.1.
+// with K cut over clusters, more on CTA pairs; where K is long the cut wins earlier and longer.  Microseconds, the three in that
+// order, inner dimension x channels, at 8 | 32 | 64 | 128 tokens: 2048 x 2048 2.8, 3.9, 6.9 | -, 4.9, 7.0 | -, 6.7, 7.3 | -, 10.4, 7.8;
+// 4096 x 6144 6.9, 8.7, 14.0 | -, 9.7, 10.7 | -, 11.9, 11.1 | -, 18.5, 11.6; 2048 x 16384 9.2, 9.4, 12.9 | -, 10.1, 12.5 | -, 12.2, 12.3 | -, 16.2,
+// 12.7; 8192 x 2048 7.3, 7.5, 15.1 | -, 8.2, 15.2 | -, 9.9, 15.6 | -, 13.8, 16.1; 14336 x 4096 15.6, 13.6, 30.9 | -, 13.9, 23.5 | -, 15.3, 24.2 | -,
+// 19.3, 24.6.  The bytes of the weight alone take 5.1 us at 2048 x 16384 and 9.0 at 14336 x 4096.
 TPLR_API int tplr_gemm_q8(const void* x, const void* w, const float* sx, const float* sw, void* y, int T, int N, int K, ll ldx, ll ldw,
                           ll ldy, int out_fp32, unsigned int* status, void* stream) {
   TPLR_ENTER();
   if (T <= 0 || N <= 0) return 0;
   if (K <= 0 || K > 131072 || (ldx | ldw) % 16 || (((uintptr_t)x | (uintptr_t)w) & 15)) return (int)cudaErrorInvalidValue;
-  if (T > FEW) return (T <= (K >= 8192 ? 128 : 64) ? tplr_gemm_q8_stream : tplr_gemm2_q8)(x, w, sx, sw, y, T, N, K, ldx, ldw, ldy, out_fp32,
+  if (T > FEW || K > 8192) return (T <= (K >= 8192 ? 128 : 64) ? tplr_gemm_q8_stream : tplr_gemm2_q8)(x, w, sx, sw, y, T, N, K, ldx, ldw, ldy, out_fp32,
                                                                                           status, stream);
   return (out_fp32 ? gemm_q8_few<float, false> : gemm_q8_few<bf16, false>)(x, w, sx, sw, y, T, N, K, ldx, ldw, ldy, stream);
 }
