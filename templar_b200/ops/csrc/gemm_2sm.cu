@@ -803,7 +803,8 @@ __device__ __forceinline__ void epilogue_swiglu_q8(const Gemm2Params& p, uint32_
 // s * g * u formed again as a third output for the down projection's weight gradient, which no pass stored.  The two warps of a
 // quadrant share a box of codes and the three boxes that leave, half the columns each: the first one's first lane moves them.
 // One warp a quadrant that did both halves was the longest part of the kernel (4096 x 2048 -> 8192: 128 us, the tensor pipe busy
-// for 55 % of them); with boxes of 32 columns for each warp alone the stores' 64-byte pieces were (16384 rows: 539 -> 670 us).
+// for 55 % of them); with boxes of 32 columns for each warp alone the stores' 64-byte pieces were (16384 rows: 539 -> 670 us); outputs
+// turned around in shared memory and stored by rows, without fences and barriers, take 4 % longer than this.
 // In turn with the bf16 form, which forms no activation: 16384 x 2048 -> 8192 558 and 468 us, 4096 x 4096 -> 14336 397 and 377, 2048 x 768 ->
 // 2048 22.9 and 22.9.  Left: the third output's bytes, and fixed latencies of a step (tensor pipe 57 % busy, an instruction in 16 % of
 // the cycles).
