@@ -182,7 +182,8 @@ def test_activation_in_8_bits(T, Fd):
     assert ops.swiglu_q8(strided).q.equal(rows.q)
 
 
-PRODUCTS = [(1, 1, 1), (1, 16, 8), (1, 8, 3), (1, 16384, 40), (1, 16392, 40), (3, 5456, 100), (5, 2040, 48), (7, 2336, 17), (8, 2056, 33), (2, 8192, 512), (3, 1003, 65), (8, 2048, 1111), (9, 4096, 640), (17, 100, 24), (24, 4096, 1544), (31, 777, 33),
+# (9 to 64 tokens: inner dimensions of 3, 5 and 9 blocks of 128 make clusters of 3 and 5; 8 tokens: both sides of an inner dimension of 8192)
+PRODUCTS = [(24, 1152, 100), (64, 640, 130), (9, 384, 1000), (40, 1100, 17), (128, 8192, 136), (8, 8192, 40), (8, 8208, 40), (1, 1, 1), (1, 16, 8), (1, 8, 3), (1, 16384, 40), (1, 16392, 40), (3, 5456, 100), (5, 2040, 48), (7, 2336, 17), (8, 2056, 33), (2, 8192, 512), (3, 1003, 65), (8, 2048, 1111), (9, 4096, 640), (17, 100, 24), (24, 4096, 1544), (31, 777, 33),
             (32, 14336, 256), (33, 256, 512), (64, 2048, 640), (65, 2048, 2048), (100, 1000, 1000), (129, 384, 257), (256, 4096, 256), (300, 72, 5000),
             (777, 1003, 1111), (1500, 2048, 1024), (2049, 128, 96)]
 
