@@ -429,12 +429,15 @@ __device__ __forceinline__ void copy8(uint32_t dst, const void* src) { asm volat
 // Counters of a first form (16384 x 2048): the memory 45 % busy, an instruction issued in 72 % of the cycles; so the weight stays unpacked, the
 // products and the codes' numbers of a piece stay for its output, and a scale multiplies once a piece where it can, and the next row's scales are asked for
 // a row ahead: 57 -> 47 us, 5.0 TB/s.
-constexpr int BWD_STAGES = 3, BWD_VPL = 2;
-template <int BLOCK>
-__global__ void __launch_bounds__(BLOCK, 512 / BLOCK)
+// Two pieces a thread, or three where two leave more threads idle (widths of three times a power of two): 16384 x 768 21.5 us against
+// 24.5, x 1536 38.2 against 45.9; at 2048 two take 48.8, three 53.3, one (24 warps an SM) 54.1, four 52.9.
+constexpr int BWD_STAGES = 3;
+constexpr int bwd_ctas(int vpl, int block) { return vpl == 3 ? 3 : 512 / block; }                      // resident on an SM
+template <int VPL, int BLOCK>
+__global__ void __launch_bounds__(BLOCK, bwd_ctas(VPL, BLOCK))
 rmsnorm_saved8_bwd_kernel(const bf16* dy, const int8_t* q, ll ldq, const float* scale, ll scale_row, ll scale_group, const float* rstd, const bf16* w,
                           const bf16* dres, bf16* dx, float* part, ll T, int D, int tpr) {
-  constexpr int VPL = BWD_VPL, PIECE = 40 * BLOCK, STAGE = VPL * PIECE;
+  constexpr int PIECE = 40 * BLOCK, STAGE = VPL * PIECE;
   extern __shared__ uint8_t pieces[];        // [stage][piece][dy 16 | dres 16 | codes 8][thread]
   __shared__ float s_dot[2][BLOCK / 32];
   __shared__ float s_dw[BLOCK * 8];
@@ -868,10 +871,12 @@ TPLR_API int tplr_rmsnorm_saved8_bwd(const void* dy, const void* q, ll ldq, cons
                 : D <= 4096 ? rmsnorm_saved8_bwd_any_kernel<4, 1024> : D <= 8192 ? rmsnorm_saved8_bwd_any_kernel<8, 1024> : rmsnorm_saved8_bwd_any_kernel<0, 1024>;
     e = launch_pdl(kern, n, block, 0, st, g, c, ldq, scale, scale_row, scale_group, rstd, wp, a, (bf16*)dx, part, T, D);
   } else {
-    const int tpr = row_threads(D / 8, BWD_VPL), block = tpr > 256 ? 512 : 256, rows = block / tpr;
-    n = (int)waves((T + rows - 1) / rows, 512 / block);
-    auto kern = block == 512 ? rmsnorm_saved8_bwd_kernel<512> : rmsnorm_saved8_bwd_kernel<256>;
-    const size_t smem = (size_t)BWD_STAGES * BWD_VPL * 40 * block;
+    const int two = row_threads(D / 8, 2), three = row_threads(D / 8, 3);
+    const int vpl = three <= 128 && 3 * three < 2 * two ? 3 : 2, tpr = vpl == 3 ? three : two, block = vpl == 3 ? 128 : tpr > 256 ? 512 : 256;
+    const int rows = block / tpr;
+    n = (int)waves((T + rows - 1) / rows, bwd_ctas(vpl, block));
+    auto kern = vpl == 3 ? rmsnorm_saved8_bwd_kernel<3, 128> : block == 512 ? rmsnorm_saved8_bwd_kernel<2, 512> : rmsnorm_saved8_bwd_kernel<2, 256>;
+    const size_t smem = (size_t)BWD_STAGES * vpl * 40 * block;
     if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return (int)e;
     e = launch_pdl(kern, n, block, smem, st, g, c, ldq, scale, scale_row, scale_group, rstd, wp, a, (bf16*)dx, part, T, D, tpr);
   }

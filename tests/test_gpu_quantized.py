@@ -44,7 +44,7 @@ def healthy():
     assert int(OF.status_word(DEV).item()) == 0
 
 
-WIDTHS = [(1, 1), (3, 63), (5, 64), (2, 65), (1, 72), (9, 136), (7, 768), (4, 1001), (300, 2048), (65, 4096), (33, 8192), (3, 28672), (2, 40001)]
+WIDTHS = [(600, 384), (40, 1536), (9, 2560), (5, 6144), (1, 1), (3, 63), (5, 64), (2, 65), (1, 72), (9, 136), (7, 768), (4, 1001), (300, 2048), (65, 4096), (33, 8192), (3, 28672), (2, 40001)]
 
 
 @pytest.mark.parametrize("T,D", WIDTHS)
