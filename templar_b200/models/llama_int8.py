@@ -18,6 +18,8 @@ from .llama import LlamaModel
 
 class Int8Llama:
     def __init__(self, model: LlamaModel):
+        if getattr(model, "_param_gather", None) is not None:
+            raise ValueError("Int8Llama: the model's weights are sharded and only present while a block runs; load them whole first")
         self.args = model.args
         self._model = model
         with torch.no_grad():

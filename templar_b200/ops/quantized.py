@@ -7,8 +7,8 @@ A group of a row with the largest magnitude ``a`` is held as whole numbers ``q =
 magnitude is below 2^-100 is zero with scale zero; one with a member that is not finite has scale NaN, so that everything made
 of it is NaN.
 
-bf16 CUDA tensors go to the kernels of ``csrc/quant.cu`` and ``csrc/gemm_2sm.cu``, everything else to the same formulas in
-PyTorch, as in :mod:`templar_b200.ops.functional`.
+bf16 CUDA tensors go to the kernels of ``csrc/quant.cu``, ``csrc/gemm_2sm.cu`` and ``csrc/gemm_q8_stream.cu``, everything else to the
+same formulas in PyTorch, as in :mod:`templar_b200.ops.functional`.
 """
 
 from __future__ import annotations

@@ -265,6 +265,13 @@ def test_model_factory_reads_the_mode():
     assert mf.initialize_torchtitan_model(hp, role="miner", device="cpu", world_size=1).activation_checkpointing == "int8"
 
 
+def test_scoring_refuses_sharded_weights():
+    m = build_model(ARGS, seed=3)
+    WindowEngine(m, EngineConfig(shard_params=True), device="cpu")
+    with pytest.raises(ValueError, match="sharded"):
+        Int8Llama(m)
+
+
 def test_scoring_in_8_bits_is_near_the_model():
     m = build_model(ARGS, seed=3)
     tok = torch.randint(0, 256, (2, 33), generator=torch.Generator().manual_seed(1))
