@@ -45,8 +45,9 @@ int tplr_rmsnorm_saved8_parts(long long T, int D);
 int tplr_rmsnorm_saved8_bwd(const void* dy, const void* q, long long ldq, const float* scale, long long scale_row, long long scale_group,
                             const float* rstd, const void* w, const void* dres, void* dx, float* part, float* dw_add, void* dw_out,
                             long long T, int D, void* stream);
-int tplr_gemm_q8(const void* x, const void* w, const float* sx, const float* sw, void* y, int T, int N, int K, long long ldx, long long ldw,
-                 long long ldy, int out_fp32, unsigned int* status, void* stream);
+long long tplr_gemm_q8_workspace(int T, int N, int K);
+int tplr_gemm_q8(const void* x, const void* w, const float* sx, const float* sw, void* y, void* ws, int T, int N, int K, long long ldx,
+                 long long ldw, long long ldy, int out_fp32, unsigned int* status, void* stream);
 int tplr_linear_q8_few(const void* x, const void* w, const float* sw, void* y, int T, int N, int K, long long ldx, long long ldw,
                        long long ldy, void* stream);
 int tplr_gemm2_swiglu_saved8(const void* X, const void* W, void* Q, float* scale, void* H, int M, int F, int K, long long ldx, long long ldw,

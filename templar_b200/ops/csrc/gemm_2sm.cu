@@ -906,12 +906,13 @@ __device__ __forceinline__ bool epilogue_swiglu_bwd_q8(const Gemm2Params& p, uin
 // EPI: 0 store bf16, 1 fp32 accumulate (C += acc), 2 store fp32, 3 fused SwiGLU of a packed [w1; w3] projection,
 // 4 store bf16 with the rotary embedding applied to the leading columns, 5 backward of the SwiGLU on the data gradient
 // of the down projection, 6 data gradient of the attention output projection with the attention backward's delta term,
-// 7 / 8 product of 8-bit rows stored as bf16 / fp32, 9 as 3 with the projection kept in 8 bits, 10 as 5 from it
+// 7 / 8 product of 8-bit rows stored as bf16 / fp32, 9 as 3 with the projection kept in 8 bits, 10 as 5 from it,
+// 11 product of 8-bit rows, int32 sums of a part of K to a plane of its own
 template <bool A_MN, bool B_MN, int EPI>
 __global__ void __launch_bounds__(num_threads(EPI), 1)
 gemm2_kernel(const __grid_constant__ Gemm2Params p) {
   constexpr int RING_BYTES = ring_stages(EPI) * STAGE_BYTES;
-  constexpr bool I8 = EPI == 7 || EPI == 8;
+  constexpr bool I8 = EPI == 7 || EPI == 8 || EPI == 11;
   constexpr int KB = I8 ? 2 * BK : BK;               // elements of a k block: 128 bytes of a row
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -1110,6 +1111,7 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
           epilogue_rope<128>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
         else if (EPI == 4 && p.rope_dh == 64 && p.rope_cols % 64 == 0)
           epilogue_rope<64>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
+        else if (EPI == 11) epilogue_tma<2>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes, w.t % p.k_splits);
         else if (I8)       epilogue_q8<EPI == 8>(p, tmem_acc, quad, turn, lane, m0, n0, sEpi + (uint32_t)(warp - 2) * 4096u, n_boxes);
         else if (p.c_tma)  epilogue_tma<EPI>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes, w.t % p.k_splits);
         else               epilogue_direct<EPI>(p, tmem_acc, quad, lane, m0, n0);
@@ -1213,7 +1215,7 @@ int launch2(Gemm2Params& p, int n_comm_pairs, int max_pairs, cudaStream_t st) {
   attr[1] = pdl_attr(p.world == 1);
   cfg.attrs = attr; cfg.numAttrs = 2;
   // all CTAs must be resident at once: compute CTAs wait for comm CTAs of the same launch
-  static int max_clusters[2][2][11] = {};
+  static int max_clusters[2][2][12] = {};
   int& mc = max_clusters[A_MN][B_MN][EPI];
   if (mc == 0) {
     cfg.gridDim = dim3(2 * (tplr_sm_count() / 2));
@@ -1243,7 +1245,7 @@ int dispatch2(Gemm2Params& p, int a_mn, int b_mn, int epi, int n_comm_pairs, int
   TPLR_GEMM2_CASE(1, 1, 0) TPLR_GEMM2_CASE(1, 1, 1) TPLR_GEMM2_CASE(1, 1, 2)
   TPLR_GEMM2_CASE(1, 0, 0) TPLR_GEMM2_CASE(1, 0, 1) TPLR_GEMM2_CASE(1, 0, 2)
   TPLR_GEMM2_CASE(0, 0, 3) TPLR_GEMM2_CASE(0, 0, 4) TPLR_GEMM2_CASE(0, 1, 5) TPLR_GEMM2_CASE(0, 1, 6)
-  TPLR_GEMM2_CASE(0, 0, 7) TPLR_GEMM2_CASE(0, 0, 8) TPLR_GEMM2_CASE(0, 0, 9) TPLR_GEMM2_CASE(0, 1, 10)
+  TPLR_GEMM2_CASE(0, 0, 7) TPLR_GEMM2_CASE(0, 0, 8) TPLR_GEMM2_CASE(0, 0, 9) TPLR_GEMM2_CASE(0, 1, 10) TPLR_GEMM2_CASE(0, 0, 11)
 #undef TPLR_GEMM2_CASE
   return -104;
 }
@@ -1323,6 +1325,30 @@ int pick_parts(int M, int N, int K, int epi) {
   return best;
 }
 
+// Parts of K of a product of 8-bit rows: their sums go to int32 planes and a second kernel adds and scales them, so that few tokens and
+// few channels do not leave most pairs idle over a long K; the sum of integers is the same in any order.  The costs above hold: a k block
+// of 128 bytes a row takes what one of bf16 takes.  Microseconds whole, as cut: 256 x 8192 x 2048 16.6, 12.1 in four; 256 x 14336 x 4096
+// 25.3, 20.5 in two; 333 x 5001 x 1004 17.6, 11.4 in four; 100 x 4096 x 768 10.1, 7.8 in eight.  Left whole: 512 x 8192 x 2048 16.8 (15.2
+// in two), 256 x 4096 x 2048 11.0 (10.2 in four), 1024 x 8192 x 2048 18.2 (21.5 in two), 256 x 2048 x 2048 7.8 (8.6).
+int pick_parts_q8(int M, int N, int K) {
+  const long long kb = (K + 2 * BK - 1) / (2 * BK), tiles = (long long)((M + TILE_M - 1) / TILE_M) * ((N + TILE_N - 1) / TILE_N);
+  const int pairs = tplr_sm_count() / 2;
+  if (N % 4 || kb < 16) return 1;
+  auto cost = [&](int parts) {
+    const double wide = plan_cost(M, N, (K + 1) / 2, false, false, 0, 256, parts), narrow = plan_cost(M, N, (K + 1) / 2, false, false, 0, 128, parts);
+    return wide < narrow ? wide : narrow;
+  };
+  int best = 1;
+  double best_cost = 0.90 * cost(1);
+  for (int parts = 2; parts <= 8 && parts <= kb; ++parts) {
+    const long long per = (kb + parts - 1) / parts;
+    if ((parts - 1) * per >= kb || tiles * parts > 4 * pairs) continue;      // every unit has work
+    const double c = cost(parts);
+    if (c < best_cost) { best = parts; best_cost = c; }
+  }
+  return best;
+}
+
 // Parts of K of the triangle product for Newton-Schulz, by the same count of waves.  Two at most: replicas orthogonalise the
 // same matrix each for itself, so the result must not depend on the order in which the parts arrive, and two parts added into
 // zeros give the same sum in either order.
@@ -1385,6 +1411,30 @@ __global__ void __launch_bounds__(256) round_rows_kernel(const float* __restrict
                                  __floats2bfloat162_rn(b.z, b.w)};
     const long long row = i / n8;
     *reinterpret_cast<uint4*>(y + row * ldc + (i - row * n8) * 8) = *reinterpret_cast<const uint4*>(h);
+  }
+}
+
+// y = sx[row] * sw[column] * the sum of the parts' int32 planes ([parts][plane], rows of N elements, N a multiple of 4), which are still in
+// L2: the launch is most of what it costs.
+template <class Out>
+__global__ void __launch_bounds__(256) join_q8_kernel(const int* x, const float* sx, const float* sw, Out* y, long long M, int n4, long long ldc,
+                                                      int parts, long long plane) {
+  grid_wait();
+  grid_release();
+  const long long total = M * n4;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+    const long long row = i / n4;
+    const int c = (int)(i - row * n4);
+    int4 a = reinterpret_cast<const int4*>(x)[i];
+    for (int s = 1; s < parts; ++s) {
+      const int4 b = reinterpret_cast<const int4*>(x + s * plane)[i];
+      a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+    }
+    const float r = sx[row];
+    const float4 q = reinterpret_cast<const float4*>(sw)[c];
+    Out* p = y + row * ldc + 4LL * c;                // rows of any stride and alignment
+    p[0] = (Out)((float)a.x * (r * q.x)); p[1] = (Out)((float)a.y * (r * q.y));
+    p[2] = (Out)((float)a.z * (r * q.z)); p[3] = (Out)((float)a.w * (r * q.w));
   }
 }
 
@@ -1613,19 +1663,40 @@ TPLR_API int tplr_gemm2_rope(const void* X, const void* W, void* QKV, int M, int
   return dispatch2(p, 0, 0, 4, 0, 0, (cudaStream_t)stream);
 }
 
+// int32 elements of the workspace that tplr_gemm2_q8 takes for this size (0: none).
+TPLR_API long long tplr_gemm2_q8_workspace(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const int parts = pick_parts_q8(M, N, K);
+  return parts > 1 ? (long long)parts * ((M + 31) / 32 * 32) * N : 0;
+}
+
 // C[M, N] = sx[m] * sw[n] * (X W^T) for 8-bit rows X [M, K] and W [N, K] (bases and row strides multiples of 16 bytes), C bf16 or fp32
 // with any row stride and alignment.  The sums are exact for K up to 131072.  A k block holds 128 values where a bf16 one holds 64,
-// at the same bytes and the same 500 cycles, so the tile rule is asked for half the K.
-TPLR_API int tplr_gemm2_q8(const void* X, const void* W, const float* sx, const float* sw, void* C, int M, int N, int K, long long ldx,
+// at the same bytes and the same 500 cycles, so the tile rule is asked for half the K.  ws: tplr_gemm2_q8_workspace elements, 16-byte
+// aligned, contents irrelevant.
+TPLR_API int tplr_gemm2_q8(const void* X, const void* W, const float* sx, const float* sw, void* C, int* ws, int M, int N, int K, long long ldx,
                            long long ldw, long long ldc, int out_fp32, unsigned int* status, void* stream) {
   TPLR_ENTER();
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  if (K > 131072 || (ldx % 16) || (ldw % 16) || (((uintptr_t)X | (uintptr_t)W | (uintptr_t)sw) & 15)) return -101;
+  if (K > 131072 || (ldx % 16) || (ldw % 16) || (((uintptr_t)X | (uintptr_t)W | (uintptr_t)sw | (uintptr_t)ws) & 15)) return -101;
+  const int parts = pick_parts_q8(M, N, K);
+  if (parts > 1 && !ws) return -101;
   Gemm2Params p = {};
-  const int tile_n = pick_tile(M, N, (K + 1) / 2, false, false, out_fp32 ? 2 : 0);
+  const int tile_n = pick_tile(M, N, (K + 1) / 2, false, false, out_fp32 && parts == 1 ? 2 : 0, parts);
   if (!make_map_u8(&p.tmA, X, K, M, ldx, 2 * BK, CTA_M)) return -102;
   if (!make_map_u8(&p.tmB, W, K, N, ldw, 2 * BK, tile_n / 2)) return -103;
   plain_fields(p, C, M, N, K, ldc, status, tile_n);
+  if (parts > 1) {
+    p.k_splits = parts;
+    p.plane_rows = (M + 31) / 32 * 32;               // a warp's box of 32 rows stays inside its plane
+    // int32 sums, moved as 32-bit words
+    if (!make_map(&p.tmC, ws, N, (long long)parts * p.plane_rows, N, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B, true)) return -110;
+    if (int r = dispatch2(p, 0, 0, 11, 0, 0, (cudaStream_t)stream)) return r;
+    const long long ctas = ((long long)M * (N / 4) + 255) / 256, most = 8LL * tplr_sm_count(), plane = (long long)p.plane_rows * N;
+    const unsigned grid = (unsigned)(ctas < most ? ctas : most);
+    if (out_fp32) return (int)launch_pdl(join_q8_kernel<float>, grid, 256, 0, (cudaStream_t)stream, ws, sx, sw, (float*)C, M, N / 4, ldc, parts, plane);
+    return (int)launch_pdl(join_q8_kernel<__nv_bfloat16>, grid, 256, 0, (cudaStream_t)stream, ws, sx, sw, (__nv_bfloat16*)C, M, N / 4, ldc, parts, plane);
+  }
   p.q8_row = sx; p.q8_col = sw;
   p.c_tma = !((uintptr_t)C & 15) && (ldc * (out_fp32 ? 4 : 2)) % 16 == 0;
   if (p.c_tma && !make_map(&p.tmC, C, N, M, ldc, out_fp32 ? 32 : 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, out_fp32 != 0)) return -110;

@@ -1,15 +1,15 @@
 // Product of few tokens with an 8-bit weight (sm_100a): the weight's bytes, read once, are what it costs.
 //
-//   y[t, n] = sx[t] * sw[n] * sum_k x[t, k] w[n, k]        T up to 128
+//   y[t, n] = sx[t] * sw[n] * sum_k x[t, k] w[n, k]        T up to 64
 //
 // The weight takes the tensor core's long side: a CTA's tile is 128 output channels (rows of w, lanes of tensor memory) by all the
-// tokens (8 to 128 columns), so no instruction multiplies rows that are not there, as a 256-row tile of tokens would.  A ring of up to
+// tokens (8 to 64 columns), so no instruction multiplies rows that are not there, as a 256-row tile of tokens would.  A ring of up to
 // 221 KB per SM is in flight all the time.  Where the blocks of 128 channels leave SMs idle, K is cut over the two, four or eight CTAs of a
 // cluster; each sends the int32 sums of a token to the CTA that owns it, 16 bytes a store into its shared memory, and the owners add
 // and scale: the sum of integers is the same in any order, and no workspace or second launch is needed.
 // 24 x 4096 x 6144 (two CTAs a block) 9.2 us, 32 x 14336 x 4096 (four) 13.9, 64 x 2048 x 16384 (one) 12.2: 2.6 to 4.2 TB/s of weight; 3 us of
 // each are launch, barriers, tensor memory, first loads and the last sums.  With the owners loading from the others' memory instead, one
-// word at a time, 128 tokens of 2048 x 2048 took 49 us, 10.4 here.
+// word at a time, 128 tokens of 2048 x 2048 took 49 us, 10.4 in this form; from 65 on CTA pairs are as fast or faster.
 // No load carries a cluster-multicast qualifier.  Every wait is bounded; on expiry TPLR_ST_WAIT_TIMEOUT is set and all roles return.
 #include "tcgen05.cuh"
 
@@ -17,14 +17,14 @@ namespace {
 using namespace tplr_tc;
 typedef long long ll;
 
-constexpr int ROWS = 128, KB = 128, W_STAGE = ROWS * KB, SMEM = 225 * 1024, MAX_STAGES = 13, THREADS = 192, MAX_TOKENS = 128, MAX_SPLIT = 8;
+constexpr int ROWS = 128, KB = 128, W_STAGE = ROWS * KB, SMEM = 225 * 1024, MAX_STAGES = 13, THREADS = 192, MAX_TOKENS = 64, MAX_SPLIT = 8;
 
 struct StreamParams {
   CUtensorMap tmW, tmX;
   const float *sx, *sw;
   void* y;
   ll ldy;
-  int T, N, K, tn;             // tn: columns of the tile, T rounded up to 8, 16, 32, 64 or 128
+  int T, N, K, tn;             // tn: columns of the tile, T rounded up to 8, 16, 32 or 64
   int split, k_per;            // CTAs of a cluster, k blocks of each
   int n_stages;
   int mine;                    // tokens whose sums meet in one CTA of a cluster, a multiple of 4
@@ -143,16 +143,16 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q8_stream_kernel(const __grid
   // of the cluster, four of a channel in 16 bytes: [sender][four tokens][channel][4] behind the ring.
   const int c = (warp & 3) * 32 + lane, n = n0 + c, first = p.split > 1 ? (int)rank * p.mine : 0;
   const uint32_t part = sX + n_stages * x_stage, part_cta = (uint32_t)p.mine * ROWS * 4u;
-  float sn = 0.f, st[4] = {};
+  float sn = 0.f, st[2] = {};
   if (warp >= 2) {
     sn = n < p.N ? p.sw[n] : 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 2; ++j)
       if (first + j * 32 + lane < p.T) st[j] = p.sx[first + j * 32 + lane];
     const bool ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_done), 0, abort_flag));
     tcgen05_fence_after();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 2; ++j) {
       if (!ok || j * 32 >= p.T) break;
       uint32_t r[32];
       tmem_ld32(tmem + j * 32 + ((uint32_t)((warp & 3) * 32) << 16), r);
@@ -176,24 +176,22 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q8_stream_kernel(const __grid
   if (p.split > 1) {
     cluster_sync_all();
     if (warp >= 2) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)                   // 64 tokens at most: two CTAs or more
-        for (int e = 0; e < 32 && j * 32 + e < p.mine && first + j * 32 + e < p.T; e += 4) {
-          int sum[4] = {};
+      for (int e = 0; e < p.mine && first + e < p.T; e += 4) {     // 32 tokens at most: two CTAs or more
+        int sum[4] = {};
 #pragma unroll 4
-          for (int k = 0; k < p.split; ++k) {
-            int v[4];
-            asm volatile("ld.shared.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                         : "r"(part + (uint32_t)k * part_cta + (uint32_t)((j * 32 + e) * ROWS + c * 4) * 4u));
+        for (int k = 0; k < p.split; ++k) {
+          int v[4];
+          asm volatile("ld.shared.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                       : "r"(part + (uint32_t)k * part_cta + (uint32_t)(e * ROWS + c * 4) * 4u));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] += v[i];
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float sc = __shfl_sync(0xffffffffu, st[j], e + i) * sn;
-            if (first + j * 32 + e + i < p.T && n < p.N) store(p, first + j * 32 + e + i, n, (float)sum[i] * sc);
-          }
+          for (int i = 0; i < 4; ++i) sum[i] += v[i];
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float sc = __shfl_sync(0xffffffffu, st[0], e + i) * sn;
+          if (first + e + i < p.T && n < p.N) store(p, first + e + i, n, (float)sum[i] * sc);
+        }
+      }
     }
     __syncwarp();
   }
@@ -206,14 +204,14 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q8_stream_kernel(const __grid
 }
 }  // namespace
 
-// tplr_gemm2_q8 for T <= 128 tokens.
+// tplr_gemm2_q8 for T <= 64 tokens.
 TPLR_API int tplr_gemm_q8_stream(const void* X, const void* W, const float* sx, const float* sw, void* C, int T, int N, int K, ll ldx, ll ldw,
                                  ll ldc, int out_fp32, unsigned int* status, void* stream) {
   TPLR_ENTER();
   if (T <= 0 || N <= 0 || K <= 0) return 0;
   if (T > MAX_TOKENS || K > 131072 || (ldx % 16) || (ldw % 16) || (((uintptr_t)X | (uintptr_t)W) & 15)) return -101;
   StreamParams p = {};
-  p.tn = T <= 8 ? 8 : T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
+  p.tn = T <= 8 ? 8 : T <= 16 ? 16 : T <= 32 ? 32 : 64;
   if (!make_map_u8(&p.tmW, W, K, N, ldw, KB, ROWS) || !make_map_u8(&p.tmX, X, K, T, ldx, KB, p.tn)) return -102;
   p.sx = sx; p.sw = sw; p.y = C; p.ldy = ldc; p.T = T; p.N = N; p.K = K; p.fp32 = out_fp32; p.status = status;
   const int blocks = (N + ROWS - 1) / ROWS, k_all = (K + KB - 1) / KB;

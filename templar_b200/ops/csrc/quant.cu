@@ -905,28 +905,35 @@ TPLR_API int tplr_swiglu_saved8_bwd(const float* dact, const void* q, ll ldq, co
                          scale, scale_row, scale_group, (bf16*)dgu, (bf16*)act, T, F);
 }
 
-extern "C" int tplr_gemm2_q8(const void* X, const void* W, const float* sx, const float* sw, void* C, int M, int N, int K, ll ldx, ll ldw,
+extern "C" ll tplr_gemm2_q8_workspace(int M, int N, int K);
+extern "C" int tplr_gemm2_q8(const void* X, const void* W, const float* sx, const float* sw, void* C, int* ws, int M, int N, int K, ll ldx, ll ldw,
                              ll ldc, int out_fp32, unsigned int* status, void* stream);
 extern "C" int tplr_gemm_q8_stream(const void* X, const void* W, const float* sx, const float* sw, void* C, int T, int N, int K, ll ldx, ll ldw,
                                    ll ldc, int out_fp32, unsigned int* status, void* stream);
 
+// Which kernel multiplies 8-bit rows: up to 8 tokens the one that loads the weight into registers, up to 64 (or with a longer K) the weight's
+// rows as the tensor core's long side with K cut over clusters, more on CTA pairs.  Microseconds, the three in that order, inner dimension x
+// channels, at 8 | 32 | 64 | 128 tokens: 2048 x 2048 2.8, 3.9, 6.9 | -, 4.9, 7.0 | -, 6.8, 7.4 | -, 10.4, 7.9; 4096 x 6144 6.9, 8.7, 14.0 | -, 9.7,
+// 11.1 | -, 12.2, 11.5 | -, 18.9, 11.9; 2048 x 16384 9.2, 9.4, 12.9 | -, 10.1, 12.5 | -, 12.2, 12.3 | -, 16.2, 12.7; 8192 x 2048 7.3, 7.5, 10.0 | -,
+// 8.4, 10.2 | -, 10.2, 10.7 | -, 14.1, 11.8; 14336 x 4096 15.6, 13.6, 18.0 | -, 14.3, 18.2 | -, 15.7, 18.6 | -, 19.6, 19.8.  The bytes of the weight
+// alone take 5.1 us at 2048 x 16384 and 9.0 at 14336 x 4096.
+static bool few_tokens(int T, int K) { return T <= FEW && K <= 8192; }
+static bool streamed(int T) { return T <= 64; }
+
+// int32 elements of the workspace that tplr_gemm_q8 takes for this size (0: none).
+TPLR_API ll tplr_gemm_q8_workspace(int T, int N, int K) { return streamed(T) ? 0 : tplr_gemm2_q8_workspace(T, N, K); }
+
 // y[T, N] = sx[t] * sw[n] * (x w^T) for int8 rows x [T, K] and w [N, K] on 16-byte boundaries, y bf16 or fp32 with row stride ldy.  The
-// bytes of a row from K to the next 16-byte boundary are read: zeros in x, anything in w.
-//
-// Which kernel: up to 8 tokens the one that loads the weight into registers, up to 64 the weight's rows as the tensor core's long side
-// with K cut over clusters, more on CTA pairs; where K is long the cut wins earlier and longer.  Microseconds, the three in that
-// order, inner dimension x channels, at 8 | 32 | 64 | 128 tokens: 2048 x 2048 2.8, 3.9, 6.9 | -, 4.9, 7.0 | -, 6.7, 7.3 | -, 10.4, 7.8;
-// 4096 x 6144 6.9, 8.7, 14.0 | -, 9.7, 10.7 | -, 11.9, 11.1 | -, 18.5, 11.6; 2048 x 16384 9.2, 9.4, 12.9 | -, 10.1, 12.5 | -, 12.2, 12.3 | -, 16.2,
-// 12.7; 8192 x 2048 7.3, 7.5, 15.1 | -, 8.2, 15.2 | -, 9.9, 15.6 | -, 13.8, 16.1; 14336 x 4096 15.6, 13.6, 30.9 | -, 13.9, 23.5 | -, 15.3, 24.2 | -,
-// 19.3, 24.6.  The bytes of the weight alone take 5.1 us at 2048 x 16384 and 9.0 at 14336 x 4096.
-TPLR_API int tplr_gemm_q8(const void* x, const void* w, const float* sx, const float* sw, void* y, int T, int N, int K, ll ldx, ll ldw,
+// bytes of a row from K to the next 16-byte boundary are read: zeros in x, anything in w.  ws: tplr_gemm_q8_workspace elements, 16-byte
+// aligned.
+TPLR_API int tplr_gemm_q8(const void* x, const void* w, const float* sx, const float* sw, void* y, void* ws, int T, int N, int K, ll ldx, ll ldw,
                           ll ldy, int out_fp32, unsigned int* status, void* stream) {
   TPLR_ENTER();
   if (T <= 0 || N <= 0) return 0;
   if (K <= 0 || K > 131072 || (ldx | ldw) % 16 || (((uintptr_t)x | (uintptr_t)w) & 15)) return (int)cudaErrorInvalidValue;
-  if (T > FEW || K > 8192) return (T <= (K >= 8192 ? 128 : 64) ? tplr_gemm_q8_stream : tplr_gemm2_q8)(x, w, sx, sw, y, T, N, K, ldx, ldw, ldy, out_fp32,
-                                                                                          status, stream);
-  return (out_fp32 ? gemm_q8_few<float, false> : gemm_q8_few<bf16, false>)(x, w, sx, sw, y, T, N, K, ldx, ldw, ldy, stream);
+  if (few_tokens(T, K)) return (out_fp32 ? gemm_q8_few<float, false> : gemm_q8_few<bf16, false>)(x, w, sx, sw, y, T, N, K, ldx, ldw, ldy, stream);
+  if (streamed(T)) return tplr_gemm_q8_stream(x, w, sx, sw, y, T, N, K, ldx, ldw, ldy, out_fp32, status, stream);
+  return tplr_gemm2_q8(x, w, sx, sw, y, (int*)ws, T, N, K, ldx, ldw, ldy, out_fp32, status, stream);
 }
 
 // tplr_quantize_rows (one scale a row) of bf16 x and tplr_gemm_q8 in one launch, the same bits; y bf16.  -111: more tokens or values than a

@@ -49,6 +49,7 @@ struct Entries {
   decltype(&tplr_add_rmsnorm_saved8) add_rmsnorm_saved8;
   decltype(&tplr_rmsnorm_saved8_parts) rmsnorm_saved8_parts;
   decltype(&tplr_rmsnorm_saved8_bwd) rmsnorm_saved8_bwd;
+  decltype(&tplr_gemm_q8_workspace) gemm_q8_workspace;
   decltype(&tplr_gemm_q8) gemm_q8;
   decltype(&tplr_linear_q8_few) linear_q8_few;
   decltype(&tplr_gemm2_swiglu_saved8) swiglu_saved8;
@@ -86,6 +87,7 @@ void bind(const std::string& path) {
   get(E.add_rmsnorm_saved8, "tplr_add_rmsnorm_saved8");
   get(E.rmsnorm_saved8_parts, "tplr_rmsnorm_saved8_parts");
   get(E.rmsnorm_saved8_bwd, "tplr_rmsnorm_saved8_bwd");
+  get(E.gemm_q8_workspace, "tplr_gemm_q8_workspace");
   get(E.gemm_q8, "tplr_gemm_q8");
   get(E.linear_q8_few, "tplr_linear_q8_few");
   get(E.swiglu_saved8, "tplr_gemm2_swiglu_saved8");
@@ -370,6 +372,13 @@ Tensor dequantize(const Tensor& q, const Tensor& scale, ll group, at::IntArrayRe
         "dequantize_rows");
   return y;
 }
+void multiply_q8(const void* q, ll ldq, const float* sx, const Tensor& wq, const Tensor& ws, const Tensor& y, ll T, ll K, const Tensor& status) {
+  const ll N = wq.size(0), n = E.gemm_q8_workspace((int)T, (int)N, (int)K);
+  const Tensor parts = n ? at::empty({n}, y.options().dtype(at::kInt)) : Tensor();            // of a long inner dimension
+  check(E.gemm_q8(q, wq.data_ptr(), sx, ws.data_ptr<float>(), y.data_ptr(), n ? parts.data_ptr() : nullptr, (int)T, (int)N, (int)K, ldq,
+                  wq.stride(0), N, 0, word(status), stream()),
+        "gemm_q8");
+}
 // x in 8 bits by rows, times an 8-bit weight; the codes live for this call alone, with their scales behind them
 Tensor linear_q8(const Tensor& x, const Tensor& wq, const Tensor& ws, const Tensor& status) {
   const at::AutoDispatchBelowADInplaceOrView guard;
@@ -390,9 +399,7 @@ Tensor linear_q8(const Tensor& x, const Tensor& wq, const Tensor& ws, const Tens
   char* q = static_cast<char*>(codes.data_ptr());
   float* scale = reinterpret_cast<float*>(q + T * ldq);
   check(E.quantize(x2.data_ptr(), x2.stride(0), q, ldq, scale, 1, 1, T, (int)K, 0, stream()), "quantize_rows");
-  check(E.gemm_q8(q, wq.data_ptr(), scale, ws.data_ptr<float>(), y.data_ptr(), (int)T, (int)N, (int)K, ldq, wq.stride(0), N, 0, word(status),
-                  stream()),
-        "gemm_q8");
+  multiply_q8(q, ldq, scale, wq, ws, y, T, K, status);
   return y;
 }
 // rows of codes that are there already: sx one scale a row, dense
@@ -400,9 +407,7 @@ Tensor linear_q8_rows(const Tensor& q, const Tensor& sx, at::IntArrayRef shape, 
   auto out = shape.vec();
   out.back() = wq.size(0);
   Tensor y = at::empty(out, q.options().dtype(at::kBFloat16));
-  check(E.gemm_q8(q.data_ptr(), wq.data_ptr(), sx.data_ptr<float>(), ws.data_ptr<float>(), y.data_ptr(), (int)q.size(0), (int)wq.size(0),
-                  (int)shape.back(), q.stride(0), wq.stride(0), wq.size(0), 0, word(status), stream()),
-        "gemm_q8");
+  multiply_q8(q.data_ptr(), q.stride(0), sx.data_ptr<float>(), wq, ws, y, q.size(0), shape.back(), status);
   return y;
 }
 // codes [N, K] and scales [N] that the product takes as they are: rows, and every 16-byte piece of a row, inside the storage

@@ -112,12 +112,12 @@ def _declare(L: ctypes.CDLL) -> None:
         "tplr_dequantize_rows": [vp, ll, vp, ll, ll, i, vp, vp, ll, i, vp],
         "tplr_add_rmsnorm_q8": [vp, vp, vp, vp, vp, ll, vp, ll, i, f, vp],
         "tplr_swiglu_q8": [vp, ll, vp, ll, vp, ll, i, vp],
-        "tplr_gemm_q8": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, i, vp, vp],
+        "tplr_gemm_q8": [vp, vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, i, vp, vp],
         "tplr_linear_q8_few": [vp, vp, vp, vp, i, i, i, ll, ll, ll, vp],
         "tplr_gemm_q8_stream": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, i, vp, vp],
         "tplr_gemm2_swiglu_saved8": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, ll, ll, vp, vp],
         "tplr_gemm2_swiglu_bwd_saved8": [vp, vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, ll, ll, ll, vp, vp],
-        "tplr_gemm2_q8": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, i, vp, vp],
+        "tplr_gemm2_q8": [vp, vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, i, vp, vp],
         "tplr_add_rmsnorm_saved8": [vp, vp, vp, vp, vp, vp, ll, vp, ll, ll, vp, ll, i, f, vp],
         "tplr_rmsnorm_saved8_parts": [ll, i],
         "tplr_rmsnorm_saved8_bwd": [vp, vp, ll, vp, ll, ll, vp, vp, vp, vp, vp, vp, vp, ll, i, vp],
@@ -179,6 +179,8 @@ def _declare(L: ctypes.CDLL) -> None:
             continue
         fn.argtypes = args
         fn.restype = c_int
+    for name in ("tplr_gemm_q8_workspace", "tplr_gemm2_q8_workspace"):
+        getattr(L, name).argtypes, getattr(L, name).restype = [i, i, i], ll
 
 
 def stream_ptr() -> int:

@@ -270,10 +270,12 @@ def linear_q8(x: torch.Tensor | QuantRows, w: QuantWeight, out_dtype: torch.dtyp
     T, N, K = x.q.shape[0], w.shape[0], w.shape[1]
     if x.q.is_cuda and out_dtype in (torch.bfloat16, torch.float32):
         y = torch.empty(*x.shape[:-1], N, dtype=out_dtype, device=x.q.device)
-        sx = x.scale.contiguous()
-        native.check(native.lib().tplr_gemm_q8(x.q.data_ptr(), w.q.data_ptr(), sx.data_ptr(), w.scale.data_ptr(), y.data_ptr(), T, N, K,
-                                               x.q.stride(0), w.q.stride(0), N, int(out_dtype == torch.float32),
-                                               OF.status_word(y.device).data_ptr(), native.stream_ptr()), "gemm_q8")
+        sx, L = x.scale.contiguous(), native.lib()
+        n = L.tplr_gemm_q8_workspace(T, N, K)                 # parts of a long inner dimension
+        ws = torch.empty(n, dtype=torch.int32, device=y.device) if n else None
+        native.check(L.tplr_gemm_q8(x.q.data_ptr(), w.q.data_ptr(), sx.data_ptr(), w.scale.data_ptr(), y.data_ptr(), native.ptr(ws), T, N, K,
+                                    x.q.stride(0), w.q.stride(0), N, int(out_dtype == torch.float32), OF.status_word(y.device).data_ptr(),
+                                    native.stream_ptr()), "gemm_q8")
         return y
     y = (x.q[:, :K].double() @ w.q.double().t()).float() * (x.scale * w.scale)
     return y.to(out_dtype).view(*x.shape[:-1], N)

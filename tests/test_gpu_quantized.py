@@ -201,6 +201,27 @@ def test_product(T, K, N, out):
     healthy()
 
 
+# inner dimensions that are cut into parts (4, 4, 8, 4, 6, 8 of them, the last of fewer blocks), rows that do not end with a plane's last box of 32
+@pytest.mark.parametrize("T,K,N", [(256, 8192, 2048), (333, 5001, 1004), (100, 4096, 768), (130, 14336, 4096), (65, 6000, 1536), (65, 131072, 12)])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_product_with_the_inner_dimension_in_parts(T, K, N, out):
+    L = native.lib()
+    assert L.tplr_gemm_q8_workspace(T, N, K) > 0 and L.tplr_gemm_q8_workspace(T, N - 1, K) == 0
+    x, w = bf(T, K), ops.quantize_weight(bf(N, K, seed=1))
+    x[T - 2] = 0
+    rows = ops.quantize_rows(x)
+    y = ops.linear_q8(rows, w, out)
+    want = (rows.q[:, :K].double() @ w.q.double().t()) * rows.scale.double() * w.scale.double()
+    assert ((y.double() - want).abs() <= want.abs() * (HALF if out == torch.bfloat16 else 2.0 ** -22)).all()
+    assert ops.linear_q8(x, w, out).equal(y)
+    less = ops.linear_q8(rows, ops.QuantWeight(w.q[:N - 1], w.scale[:N - 1]), out)       # whole: channels that make no 16-byte pieces
+    assert less.equal(y[:, :N - 1])
+    x[3, 5] = float("nan")
+    z = ops.linear_q8(x, w, out)
+    assert z[3].isnan().all() and z[:3].equal(y[:3]) and z[4:].equal(y[4:])
+    healthy()
+
+
 @pytest.mark.parametrize("T", [1, 5, 40, 300])
 def test_longest_sums_are_exact(T):
     K, N = OQ.MAX_INNER, 40
