@@ -159,138 +159,188 @@ __device__ __forceinline__ void values8(const uint2& q, float scale, float* f) {
   for (int i = 0; i < 8; ++i) f[i] *= scale;
 }
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+
 // The same from registers, for rows of whole 16-byte pieces: `tpr` threads (a power of two) share a row, VPL pieces each, so a row is
 // read once and its two reductions (the squares, the largest magnitude) run on values that are already there.  Several rows a CTA
-// share its barriers.  A thread asks for all its pieces before it waits for the first.  16384 x 2048: norm in 8 bits 45 us, its training form
-// 56, codes by row 21, the activation of 16384 x 1024 in 8 bits 17: 4.9 to 5.4 TB/s, 75 to 83 % of what a plain copy of 2 GB moves; what is left
-// are a CTA's loads, barriers and stores in turn (in the training form an instruction is issued in 55 % of the cycles).
-template <int MODE, int VPL, int BLOCK>
-__global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) rows_q8_kernel(const RowsArgs p, const int tpr) {
+// share its barriers.  A thread asks for all its pieces before it waits for the first.
+//
+// RING: CTAs that stay, RING of them on an SM, and ask for the next row while they work on one, each thread's own pieces into its own
+// shared memory, so that no barrier stands between a copy and its use and a CTA's loads, barriers and stores do not come in turn.  Without
+// and with it: norm in 8 bits 4096 x 4096 26.4 and 21.6 us, 16384 x 2048 45.4 and 39.0 (6.0 TB/s, 92 % of what a plain copy of 2 GB moves), its training
+// form 31.1 and 28.1, 56.2 and 50.6; codes by row 12.2 and 10.8, 21.8 and 19.3.  Three rows in flight, CTAs of 128 threads, two pieces a thread and
+// neighbouring rows to a CTA were even or slower.  Not faster: a norm without a residual to add (17.7 and 18.7, 31.5 and 35.3) and the activation of
+// [gate | up] rows (16384 x 1024 17.5 and 17.4, 4096 x 2048 10.9 and 12.2).
+template <int MODE, int VPL, int BLOCK, int RING>
+__global__ void __launch_bounds__(BLOCK, RING ? RING : 1024 / BLOCK) rows_q8_kernel(const RowsArgs p, const int tpr) {
   constexpr bool NORM = MODE == NORM_ROWS || MODE == NORM_SAVED, BY_GROUP = MODE == GROUPS || MODE == NORM_SAVED;
-  __shared__ float s_sum[32];
-  __shared__ uint32_t s_top[32];
+  constexpr int OPERANDS = NORM ? 2 : 1, PIECE = BLOCK * 16, STAGE = OPERANDS * VPL * PIECE;
+  extern __shared__ __align__(16) uint8_t ring[];                                   // [this row, the next][operand][piece][thread]
+  __shared__ float s_sum[RING ? 2 : 1][32];                              // by row in turn: the next row's are written while this one's are read
+  __shared__ uint32_t s_top[RING ? 2 : 1][32];
   grid_wait();
   grid_release();
   const int t = threadIdx.x & (tpr - 1), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.D, nv = D / 8, warps = tpr >> 5;
   const int row_warp = threadIdx.x / tpr * warps;                        // first warp of this thread's row
-  const ll row = (ll)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
-  const bool live = row < p.T;
-  const bf16x8* a = reinterpret_cast<const bf16x8*>(p.a + (live ? row : 0) * p.lda);
-  const bf16x8* b = MODE == SWIGLU_ROWS ? a + nv : p.b ? reinterpret_cast<const bf16x8*>(p.b + (live ? row : 0) * p.ldb) : nullptr;
   const bool two = MODE == SWIGLU_ROWS || (NORM && p.b);
-  float v[VPL][8];
-  {
-    bf16x8 ra[VPL], rb[VPL];
+  const ll rows = blockDim.x / tpr, step = (ll)gridDim.x * rows;
+  uint8_t* mine = ring + threadIdx.x * 16;
+  auto ask = [&](ll row, int stage) {
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(mine) + stage * STAGE;
+    if (row < p.T) {
 #pragma unroll
-    for (int j = 0; j < VPL; ++j)
-      if (live && t + tpr * j < nv) {
-        ra[j] = a[t + tpr * j];
-        if (two) rb[j] = b[t + tpr * j];
-      }
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) {
-      const int i = t + tpr * j;
-      if (!live || i >= nv) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
-        continue;
-      }
-      if (NORM && two) {                                                 // the norm sees the sum as the residual stream stores it
-#pragma unroll
-        for (int e = 0; e < 4; ++e) ra[j].v[e] = __hadd2(ra[j].v[e], rb[j].v[e]);
-        reinterpret_cast<bf16x8*>(p.h + row * D)[i] = ra[j];
-      }
-      unpack8(ra[j], v[j]);
-      if (MODE == SWIGLU_ROWS) {
-        float o[8];
-        unpack8(rb[j], o);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] = silu_mul(v[j][e], o[e]);
-      }
+      for (int j = 0; j < VPL; ++j)
+        if (t + tpr * j < nv) {
+          copy16(to + j * PIECE, p.a + row * p.lda + (t + tpr * j) * 8);
+          if (OPERANDS == 2) copy16(to + (VPL + j) * PIECE, p.b + row * p.ldb + (t + tpr * j) * 8);
+        }
     }
-  }
-  if (NORM) {
-    float ss = 0.f;
-#pragma unroll
-    for (int j = 0; j < VPL; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(v[j][e], v[j][e], ss);
-    bf16x8 wp[VPL];
-    if (MODE == NORM_SAVED) {                                            // all asked for here: no load passes the stores below
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  bf16x8 wp[VPL];
+  if (RING) {
+    if (NORM) {
 #pragma unroll
       for (int j = 0; j < VPL; ++j)
         if (t + tpr * j < nv) wp[j] = reinterpret_cast<const bf16x8*>(p.w)[t + tpr * j];
     }
-    ss = warp_sum(ss);
-    if (warps > 1) {
-      if (lane == 0) s_sum[warp] = ss;
-      __syncthreads();
-      ss = 0.f;
-      for (int k = 0; k < warps; ++k) ss += s_sum[row_warp + k];
+    ask((ll)blockIdx.x * rows + threadIdx.x / tpr, 0);
+  }
+  int stage = 0;
+  for (ll first = (ll)blockIdx.x * rows; first < p.T; first += step, stage ^= 1) {   // once without a ring
+    const ll row = first + threadIdx.x / tpr;
+    const bool live = row < p.T;
+    if (RING) {
+      ask(row + step, stage ^ 1);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
     }
-    const float r = rsqrtf(ss / (float)D + p.eps);
-    if (MODE == NORM_SAVED && live && t == 0) p.rstd[row] = r;
+    const int at = RING ? stage : 0;
+    float v[VPL][8];
+    {
+      bf16x8 ra[VPL], rb[VPL];
+      if (RING) {
+        const bf16x8* from = reinterpret_cast<const bf16x8*>(mine + stage * STAGE);
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+          if (live && t + tpr * j < nv) {
+            ra[j] = from[j * BLOCK];
+            if (OPERANDS == 2) rb[j] = from[(VPL + j) * BLOCK];
+          }
+      } else {
+        const bf16x8* a = reinterpret_cast<const bf16x8*>(p.a + (live ? row : 0) * p.lda);
+        const bf16x8* b = MODE == SWIGLU_ROWS ? a + nv : p.b ? reinterpret_cast<const bf16x8*>(p.b + (live ? row : 0) * p.ldb) : nullptr;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+          if (live && t + tpr * j < nv) {
+            ra[j] = a[t + tpr * j];
+            if (two) rb[j] = b[t + tpr * j];
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        const int i = t + tpr * j;
+        if (!live || i >= nv) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
+          continue;
+        }
+        if (NORM && two) {                                               // the norm sees the sum as the residual stream stores it
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ra[j].v[e] = __hadd2(ra[j].v[e], rb[j].v[e]);
+          reinterpret_cast<bf16x8*>(p.h + row * D)[i] = ra[j];
+        }
+        unpack8(ra[j], v[j]);
+        if (MODE == SWIGLU_ROWS) {
+          float o[8];
+          unpack8(rb[j], o);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[j][e] = silu_mul(v[j][e], o[e]);
+        }
+      }
+    }
+    if (NORM) {
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(v[j][e], v[j][e], ss);
+      if (MODE == NORM_SAVED && !RING) {                                 // all asked for here: no load passes the stores below
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+          if (t + tpr * j < nv) wp[j] = reinterpret_cast<const bf16x8*>(p.w)[t + tpr * j];
+      }
+      ss = warp_sum(ss);
+      if (warps > 1) {
+        if (lane == 0) s_sum[at][warp] = ss;
+        __syncthreads();
+        ss = 0.f;
+        for (int k = 0; k < warps; ++k) ss += s_sum[at][row_warp + k];
+      }
+      const float r = rsqrtf(ss / (float)D + p.eps);
+      if (MODE == NORM_SAVED && live && t == 0) p.rstd[row] = r;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        const int i = t + tpr * j;
+        if (!live || i >= nv) continue;
+        float w[8];
+        unpack8(RING || MODE == NORM_SAVED ? wp[j] : reinterpret_cast<const bf16x8*>(p.w)[i], w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[j][e] *= r;
+          w[e] *= v[j][e];
+        }
+        if (MODE == NORM_ROWS) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[j][e] = w[e];
+        } else {
+          reinterpret_cast<bf16x8*>(p.y + row * D)[i] = pack8(w);
+        }
+      }
+    }
+    uint32_t tops[VPL];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      float top = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) top = top3(top, v[j][e], v[j][e + 1]);
+      tops[j] = magnitude(top);
+    }
+    Codes all = {};
+    if (!BY_GROUP) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) top = max(top, tops[j]);
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (warps > 1) {
+        if (lane == 0) s_top[at][warp] = top;
+        __syncthreads();
+        for (int k = 0; k < warps; ++k) top = max(top, s_top[at][row_warp + k]);
+      }
+      all = codes_of(top);
+      if (live && t == 0) p.scale[row * p.scale_row] = all.scale;
+    }
+    if (BY_GROUP) {                                                      // eight lanes hold a group's 64 columns
+#pragma unroll
+      for (int j = 0; j < VPL; ++j)
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) tops[j] = max(tops[j], __shfl_xor_sync(0xffffffffu, tops[j], o));
+      // lane j of the eight divides for their j-th group
+      const int k = lane & 7;
+      uint32_t top = tops[0];
+#pragma unroll
+      for (int j = 1; j < VPL; ++j) top = k == j ? tops[j] : top;
+      all = codes_of(top);
+      const int i = t - k + tpr * k;
+      if (live && k < VPL && i < nv) p.scale[row * p.scale_row + (i >> 3) * p.scale_group] = all.scale;
+    }
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
       const int i = t + tpr * j;
-      if (!live || i >= nv) continue;
-      float w[8];
-      unpack8(MODE == NORM_SAVED ? wp[j] : reinterpret_cast<const bf16x8*>(p.w)[i], w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[j][e] *= r;
-        w[e] *= v[j][e];
-      }
-      if (MODE == NORM_ROWS) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] = w[e];
-      } else {
-        reinterpret_cast<bf16x8*>(p.y + row * D)[i] = pack8(w);
-      }
+      const float inv = BY_GROUP ? __shfl_sync(0xffffffffu, all.inv, (lane & ~7) + j) : all.inv;
+      if (live && (ll)i * 8 < p.ldq)                                     // zeros behind the row: v is 0 there
+        reinterpret_cast<uint2*>(p.q + row * p.ldq)[i] = codes8(v[j], i < nv ? inv : 0.f);
     }
-  }
-  uint32_t tops[VPL];
-#pragma unroll
-  for (int j = 0; j < VPL; ++j) {
-    float top = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) top = top3(top, v[j][e], v[j][e + 1]);
-    tops[j] = magnitude(top);
-  }
-  Codes all = {};
-  if (!BY_GROUP) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) top = max(top, tops[j]);
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (warps > 1) {
-      if (lane == 0) s_top[warp] = top;
-      __syncthreads();
-      for (int k = 0; k < warps; ++k) top = max(top, s_top[row_warp + k]);
-    }
-    all = codes_of(top);
-    if (live && t == 0) p.scale[row * p.scale_row] = all.scale;
-  }
-  if (BY_GROUP) {                                                        // eight lanes hold a group's 64 columns
-#pragma unroll
-    for (int j = 0; j < VPL; ++j)
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) tops[j] = max(tops[j], __shfl_xor_sync(0xffffffffu, tops[j], o));
-    // lane j of the eight divides for their j-th group
-    const int k = lane & 7;
-    uint32_t top = tops[0];
-#pragma unroll
-    for (int j = 1; j < VPL; ++j) top = k == j ? tops[j] : top;
-    all = codes_of(top);
-    const int i = t - k + tpr * k;
-    if (live && k < VPL && i < nv) p.scale[row * p.scale_row + (i >> 3) * p.scale_group] = all.scale;
-  }
-#pragma unroll
-  for (int j = 0; j < VPL; ++j) {
-    const int i = t + tpr * j;
-    const float inv = BY_GROUP ? __shfl_sync(0xffffffffu, all.inv, (lane & ~7) + j) : all.inv;
-    if (live && (ll)i * 8 < p.ldq)                                       // zeros behind the row: v is 0 there
-      reinterpret_cast<uint2*>(p.q + row * p.ldq)[i] = codes8(v[j], i < nv ? inv : 0.f);
+    if (!RING) break;
   }
 }
 
@@ -420,7 +470,6 @@ __global__ void __launch_bounds__(BLOCK) rmsnorm_saved8_bwd_any_kernel(const bf1
   }
 }
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy8(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory"); }
 
 // The same for whole 16-byte pieces: `tpr` threads on a row, VPL pieces each, the weight gradient's sums of a thread's columns in registers
@@ -763,6 +812,20 @@ int row_threads(int pieces, int vpl) {
   return n;
 }
 
+unsigned waves(ll ctas, int resident) {
+  const ll most = (ll)tplr_sm_count() * resident;
+  return (unsigned)(ctas < most ? ctas : most);
+}
+
+template <int MODE, int BLOCK, int RING>
+int rows_q8_ring(const RowsArgs& p, int tpr, cudaStream_t st) {
+  constexpr int OPERANDS = MODE == NORM_ROWS || MODE == NORM_SAVED ? 2 : 1, SMEM = 2 * OPERANDS * 4 * BLOCK * 16;
+  auto kern = rows_q8_kernel<MODE, 4, BLOCK, RING>;
+  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM)) return (int)e;
+  const ll groups = (p.T + BLOCK / tpr - 1) / (BLOCK / tpr);
+  return (int)launch_pdl(kern, waves(groups, RING), BLOCK, SMEM, st, p, tpr);
+}
+
 template <int MODE>
 int rows_q8(const RowsArgs& p, void* stream) {
   if (p.T <= 0) return 0;
@@ -779,14 +842,17 @@ int rows_q8(const RowsArgs& p, void* stream) {
   const int vpl = p.T * pieces <= (codes_alone ? 512LL : 1024LL) * tplr_sm_count() && pieces <= 1024 ? 1 : 4;
   const int tpr = row_threads(pieces, vpl), block = tpr > 256 ? tpr : 256;
   const unsigned grid = (unsigned)((p.T + block / tpr - 1) / (block / tpr));
-  if (block > 256) return (int)(vpl == 1 ? launch_pdl(rows_q8_kernel<MODE, 1, 1024>, grid, block, 0, st, p, tpr)
-                                           : launch_pdl(rows_q8_kernel<MODE, 4, 1024>, grid, block, 0, st, p, tpr));
-  return (int)(vpl == 1 ? launch_pdl(rows_q8_kernel<MODE, 1, 256>, grid, block, 0, st, p, tpr)
-                        : launch_pdl(rows_q8_kernel<MODE, 4, 256>, grid, block, 0, st, p, tpr));
-}
-unsigned waves(ll ctas, int resident) {
-  const ll most = (ll)tplr_sm_count() * resident;
-  return (unsigned)(ctas < most ? ctas : most);
+  if constexpr (MODE == NORM_SAVED)
+    // Four arrays are written: beyond twice the L2, fewer CTAs keep longer runs of each together.  Microseconds with two of 256 threads an SM and with
+    // one of 512: 12000 x 2048 38.2 and 39.9, 16384 x 1536 39.9 and 41.1, 16000 x 2048 53.5 and 50.4, 32768 x 2048 106.6 and 95.8.
+    if (vpl == 4 && block == 256 && p.b && p.T * p.D > 28LL << 20) return rows_q8_ring<MODE, 512, 1>(p, tpr, st);
+  if constexpr (MODE != SWIGLU_ROWS)
+    if (vpl == 4 && block == 256 && (codes_alone || p.b)) return rows_q8_ring<MODE, 256, 2>(p, tpr, st);
+  if (block > 256) return (int)(vpl == 1 ? launch_pdl(rows_q8_kernel<MODE, 1, 1024, 0>, grid, block, 0, st, p, tpr)
+                                         : launch_pdl(rows_q8_kernel<MODE, 4, 1024, 0>, grid, block, 0, st, p, tpr));
+  if constexpr (MODE != ROWS && MODE != GROUPS)
+    if (vpl == 4) return (int)launch_pdl(rows_q8_kernel<MODE, 4, 256, 0>, grid, block, 0, st, p, tpr);
+  return (int)launch_pdl(rows_q8_kernel<MODE, 1, 256, 0>, grid, block, 0, st, p, tpr);
 }
 }  // namespace
 

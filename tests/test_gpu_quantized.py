@@ -171,6 +171,23 @@ def test_saved_norm_and_its_gradient(T, D, add):
     assert ((mg.double() - 1 - dw).abs() <= (dy.double() * xn).abs().sum(0) * NOISE + (1 + dw.abs()) * 2.0 ** -23).all()
 
 
+# many rows: CTAs that stay and take several in turn, the last turn with fewer; more than 2^20 * 28 values
+@pytest.mark.parametrize("T,D", [(2501, 2008), (1201, 4096), (5003, 768), (700, 8192), (14401, 2048)])
+def test_many_rows(T, D):
+    for group in (0, 64):
+        test_rows(T, D, group)
+    for add in (True, False):
+        test_norm_in_8_bits(T, D, add)
+        test_saved_norm_and_its_gradient(T, D, add)
+    x = bf(T, D)
+    want = ops.quantize_rows(x)
+    x[T // 2, D - 1] = float("inf")
+    got = ops.quantize_rows(x)
+    rest = torch.arange(T, device=DEV) != T // 2
+    assert got.scale[T // 2].isnan().all() and not got.q[T // 2].any()
+    assert got.q[rest].equal(want.q[rest]) and got.scale[rest].equal(want.scale[rest])
+
+
 @pytest.mark.parametrize("T,Fd", [(1, 1), (3, 100), (5, 64), (4, 1001), (200, 2816), (17, 8192), (2, 28672), (1, 40000)])
 def test_activation_in_8_bits(T, Fd):
     gu = bf(T, 2 * Fd)
