@@ -816,11 +816,14 @@ struct CodeLoads {
   float sg, su;                      // scales of this lane's row in the box asked for last
 };
 __device__ __forceinline__ void quadrant_sync(int quad) { asm volatile("bar.sync %0, 64;" ::"r"(quad + 1) : "memory"); }
-// Both warps of a quadrant leave with one answer: neither waits at a barrier for another that has given up.
-__device__ __forceinline__ bool quadrant_agrees(bool ok, int quad, int lane, volatile int* given_up) {
-  if (!ok && lane == 0) given_up[quad] = 1;
-  quadrant_sync(quad);
-  return given_up[quad] == 0;
+// Both warps of a quadrant leave with one answer, and neither waits at a barrier for another that has given up: the barrier itself joins
+// their answers.  A flag in shared memory, written in front of the barrier and read behind it, is the next call's as well: one warp could
+// raise it there before the other had read this call's.
+__device__ __forceinline__ bool quadrant_agrees(bool ok, int quad) {
+  uint32_t both;
+  asm volatile("{\n\t.reg .pred mine, all;\n\tsetp.ne.u32 mine, %2, 0;\n\tbar.red.and.pred all, %1, 64, mine;\n\tselp.u32 %0, 1, 0, all;\n\t}"
+               : "=r"(both) : "r"(quad + 1), "r"((uint32_t)ok) : "memory");
+  return both != 0;
 }
 __device__ __forceinline__ void codes_issue(const Gemm2Params& p, CodeLoads& L, bool mover, int lane, int f0, int row0) {
   const long long row = min(row0 + lane, p.M - 1);
@@ -838,7 +841,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ bool epilogue_swiglu_bwd_q8(const Gemm2Params& p, uint32_t tmem_acc, int quad, int turn, int lane, int m0, int n0,
-                                                       CodeLoads& L, volatile int* given_up, volatile int* abort_flag) {
+                                                       CodeLoads& L, volatile int* abort_flag) {
   const int row0 = m0 + quad * 32;
   if (row0 >= p.M || n0 >= p.swiglu_f) return true;  // the same in both warps; nothing was asked for
   const bool mover = turn == 0 && lane == 0;
@@ -880,7 +883,7 @@ __device__ __forceinline__ bool epilogue_swiglu_bwd_q8(const Gemm2Params& p, uin
     if (mover) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");            // the last boxes are read out
     __syncwarp();
     // both warps have read their codes, and the boxes are free
-    if (!quadrant_agrees(ok, quad, lane, given_up)) return false;
+    if (!quadrant_agrees(ok, quad)) return false;
     if (c + 1 < p.tile_n / 64 && f0 + 64 < p.swiglu_f) codes_issue(p, L, mover, lane, f0 + 64, row0);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -918,7 +921,7 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t bar_full[MAX_STAGES], bar_empty[MAX_STAGES], bar_tfull[2], bar_tempty[2];
   __shared__ uint32_t s_tmem_base;
-  __shared__ int s_abort, s_given_up[EPI == 10 ? 4 : 1];
+  __shared__ int s_abort;
   __shared__ __align__(8) uint64_t bar_gu[EPI == 5 || EPI == 10 ? 8 : 1];      // EPI 5: two per epilogue warp, 10: one a quadrant
   __shared__ uint32_t s_ready[32];   // gather: bit c set once chunk c was seen ready (1024 chunks)
 
@@ -937,7 +940,6 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
 
   if (threadIdx.x == 0) {
     s_abort = 0;
-    for (int& g : s_given_up) g = 0;
     for (int s = 0; s < MAX_STAGES; ++s) {
       mbar_init(smem_u32(&bar_full[s]), 1);
       mbar_init(smem_u32(&bar_empty[s]), 1);
@@ -1098,14 +1100,14 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
         if (EPI == 10 && m0 + quad * 32 < p.M && n0 < p.swiglu_f) codes_issue(p, cl, turn == 0 && lane == 0, lane, n0, m0 + quad * 32);
         ok = mbar_wait(smem_u32(&bar_tfull[acc]), acc_ph, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
-        if (EPI == 10) ok = quadrant_agrees(ok, quad, lane, s_given_up);
+        if (EPI == 10) ok = quadrant_agrees(ok, quad);
         if (!ok) break;
         tcgen05_fence_after();
         const uint32_t tmem_acc = tmem_base + acc * TILE_N;
         if (EPI == 3)      epilogue_swiglu(p, tmem_acc, quad, lane, m0, tn, sEpi + (uint32_t)quad * 8192u, n_boxes);
         else if (EPI == 5) { if (!(ok = epilogue_swiglu_bwd(p, tmem_acc, quad, lane, m0, n0, gl, abort_flag))) break; }
         else if (EPI == 9) epilogue_swiglu_q8(p, tmem_acc, quad, lane, m0, tn, sEpi + (uint32_t)quad * 8192u, n_boxes);
-        else if (EPI == 10) { if (!(ok = epilogue_swiglu_bwd_q8(p, tmem_acc, quad, turn, lane, m0, n0, cl, s_given_up, abort_flag))) break; }
+        else if (EPI == 10) { if (!(ok = epilogue_swiglu_bwd_q8(p, tmem_acc, quad, turn, lane, m0, n0, cl, abort_flag))) break; }
         else if (EPI == 6) epilogue_attn_dout(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
         else if (EPI == 4 && p.rope_dh == 128 && p.rope_cols % 128 == 0)
           epilogue_rope<128>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);

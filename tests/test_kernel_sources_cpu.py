@@ -65,3 +65,73 @@ def test_every_exit_of_a_loss_kernel_has_written_its_row():
         assert "mbar_wait" not in body, name
         for exit_at in re.finditer(r"\breturn;", body):
             assert re.search(r"\blosses\[row\] = ", body[:exit_at.start()]), name
+
+
+def _agreement_steps(text):
+    """What one warp does in ``quadrant_agrees``, in order: "raise" its flag where its wait gave up, "meet" at the barrier (and
+    "reduce" its answer there), "look" at the flag."""
+    body = re.search(r"bool quadrant_agrees\([^)]*\)\s*\{(.*?)\n\}", text, re.S).group(1)
+    body = body.replace("quadrant_sync(quad);", "bar.sync;")
+    marks = [(m.start(), s) for pattern, s in ((r"given_up\[[^\]]*\] = 1", "raise"), (r"bar\.sync", "meet"), (r"bar\.red\.and\.pred", "reduce"),
+                                               (r"return given_up", "look")) for m in re.finditer(pattern, body)]
+    return [s for _, s in sorted(marks)]
+
+
+def _answers(steps, waits):
+    """Every pair of answer lists that two warps can leave with, over all orders of their steps: each goes through the waits of its
+    list until one gives up or the two of them do not agree."""
+    flat = [(call, s) for call in range(len(waits[0])) for s in steps]
+    ends, seen = set(), set()
+
+    def go(at, met, joined, flag, answers):
+        key = (at, met, joined, flag, answers)
+        if key in seen:
+            return
+        seen.add(key)
+        moved = False
+        for w in (0, 1):
+            if at[w] == len(flat) or answers[w][-1:] == (False,):
+                continue
+            call, step = flat[at[w]]
+            m, j, f, a, n = met, joined, flag, answers, at[w] + 1
+            if step in ("meet", "reduce"):
+                if met[w] == call:                               # arrives
+                    m = tuple(call + 1 if k == w else met[k] for k in (0, 1))
+                    j = tuple(x and waits[w][c] if c == call else x for c, x in enumerate(joined))
+                    n = at[w]
+                elif met[1 - w] <= call:
+                    continue                                     # waits for the other
+                elif step == "reduce":
+                    a = tuple(answers[k] + (joined[call],) if k == w else answers[k] for k in (0, 1))
+            elif step == "raise":
+                f = flag or not waits[w][call]
+            else:
+                a = tuple(answers[k] + (not flag,) if k == w else answers[k] for k in (0, 1))
+            moved = True
+            go(tuple(n if k == w else at[k] for k in (0, 1)), m, j, f, a)
+        if not moved:
+            ends.add(answers)
+
+    go((0, 0), (0, 0), (True,) * len(waits[0]), False, ((), ()))
+    return ends
+
+
+@pytest.mark.parametrize("waits", [((True, True), (True, True)), ((False, True), (True, True)), ((True, True), (True, False)),
+                                   ((True, True, False), (True, True, True)), ((True, False), (True, False))])
+def test_two_warps_that_share_boxes_leave_together(waits):
+    """Two warps share the boxes of a quadrant of the SwiGLU backward from codes and its barriers.  One that leaves while the
+    other goes on would be waited for without end, so in every order of their steps both give the same answers."""
+    steps = _agreement_steps(re.sub(r"//[^\n]*", "", (CSRC / "gemm_2sm.cu").read_text()))
+    assert "meet" in steps or "reduce" in steps
+    # the model tells a sound exchange from one whose flag is the next call's as well
+    assert all(a == b for a, b in _answers(["reduce"], waits))
+    for a, b in _answers(steps, waits):
+        assert a == b, (steps, a, b)
+    want = [all(w) for w in zip(*waits)]
+    want = tuple(want[:want.index(False) + 1] if False in want else want)
+    assert {a for a, _ in _answers(steps, waits)} == {want}
+
+
+def test_the_model_of_two_warps_finds_a_flag_that_is_read_late():
+    ends = _answers(["raise", "meet", "look"], ((True, True), (True, False)))
+    assert any(a != b for a, b in ends)
