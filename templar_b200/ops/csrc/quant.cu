@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(BLOCK, bwd_ctas(VPL, BLOCK))
 rmsnorm_saved8_bwd_kernel(const bf16* dy, const int8_t* q, ll ldq, const float* scale, ll scale_row, ll scale_group, const float* rstd, const bf16* w,
                           const bf16* dres, bf16* dx, float* part, ll T, int D, int tpr) {
   constexpr int PIECE = 40 * BLOCK, STAGE = VPL * PIECE;
-  extern __shared__ uint8_t pieces[];        // [stage][piece][dy 16 | dres 16 | codes 8][thread]
+  extern __shared__ __align__(16) uint8_t pieces[];        // [stage][piece][dy 16 | dres 16 | codes 8][thread]
   __shared__ float s_dot[2][BLOCK / 32];
   __shared__ float s_dw[BLOCK * 8];
   grid_wait();

@@ -135,3 +135,15 @@ def test_two_warps_that_share_boxes_leave_together(waits):
 def test_the_model_of_two_warps_finds_a_flag_that_is_read_late():
     ends = _answers(["raise", "meet", "look"], ((True, True), (True, False)))
     assert any(a != b for a, b in ends)
+
+
+@pytest.mark.parametrize("src", sorted(p.name for p in CSRC.glob("*.cu") if "extern __shared__" in p.read_text()))
+def test_buffers_of_bytes_in_shared_memory_are_aligned_by_declaration_or_by_hand(src):
+    """A dynamic buffer lies behind the kernel's static arrays.  One of bytes has no alignment of its own, and copies of 16 bytes
+    fault on another: it is declared with one, or used through a pointer that was rounded up."""
+    text = re.sub(r"//[^\n]*", "", (CSRC / src).read_text())
+    for name, _, body in _kernels(src):
+        for buf in re.findall(r"extern __shared__ (?:uint8_t|int8_t|char) (\w+)\[\];", body):
+            uses = re.findall(rf"[^;]*\b{buf}\b[^;]*;", body.split(f"{buf}[];", 1)[1])
+            assert uses and all(re.search(rf"\(reinterpret_cast<uintptr_t>\({buf}\) \+ \d+\) & ~", u) for u in uses), (name, buf)
+    assert "extern __shared__" in text
