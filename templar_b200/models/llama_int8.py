@@ -20,6 +20,9 @@ class Int8Llama:
     def __init__(self, model: LlamaModel):
         if getattr(model, "_param_gather", None) is not None:
             raise ValueError("Int8Llama: the model's weights are sharded and only present while a block runs; load them whole first")
+        if getattr(model, "tp_world", 1) > 1 or model.output.weight.shape[0] != model.args.vocab_size:
+            raise ValueError("Int8Llama: the model holds one rank's part of its heads, hidden units and (padded) vocabulary; "
+                             "load the whole weights into a LlamaModel first")
         self.args = model.args
         self._model = model
         with torch.no_grad():

@@ -10,6 +10,7 @@ from templar_b200 import model_factory as mf
 from templar_b200 import ops
 from templar_b200.models.llama import ModelArgs, build_model
 from templar_b200.models.llama_int8 import Int8Llama
+from templar_b200.models.llama_tp import TPLlamaModel
 from templar_b200.parallel.window_engine import EngineConfig, WindowEngine
 
 ARGS = ModelArgs(dim=128, n_layers=3, n_heads=2, n_kv_heads=1, vocab_size=256, intermediate_size=192, max_seq_len=32)
@@ -269,6 +270,18 @@ def test_scoring_refuses_sharded_weights():
     m = build_model(ARGS, seed=3)
     WindowEngine(m, EngineConfig(shard_params=True), device="cpu")
     with pytest.raises(ValueError, match="sharded"):
+        Int8Llama(m)
+
+
+# two ranks; one rank whose vocabulary is padded, so that its logits have columns of no entry
+@pytest.mark.parametrize("world,vocab", [(2, 256), (1, 200)])
+def test_scoring_refuses_one_ranks_part_of_a_model(world, vocab):
+    args = ModelArgs(dim=128, n_layers=2, n_heads=4, n_kv_heads=2, vocab_size=vocab, intermediate_size=256, max_seq_len=32)
+    full = build_model(args, seed=3)
+    m = TPLlamaModel(args, 0, world)
+    m.freqs_cis = full.freqs_cis
+    m.load_from_full(full)
+    with pytest.raises(ValueError, match="one rank's part"):
         Int8Llama(m)
 
 
