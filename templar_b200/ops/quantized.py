@@ -169,7 +169,9 @@ class QuantWeight:
         wide = _padded(q.shape[1])
         behind = q.storage_offset() + (q.shape[0] - 1) * q.stride(0) + wide       # the last row's last 16-byte piece
         if q.stride(1) != 1 or q.stride(0) % 16 or q.stride(0) < wide or q.data_ptr() % 16 or behind > q.untyped_storage().nbytes():
-            q = F.pad(q, (0, wide - q.shape[1]))[:, :q.shape[1]]
+            rows = q.new_zeros(q.shape[0], wide)             # F.pad by nothing would keep the strides of a transposed matrix
+            rows[:, :q.shape[1]] = q
+            q = rows[:, :q.shape[1]]
         self.q, self.scale = q, OF._dense(scale)
 
     @property

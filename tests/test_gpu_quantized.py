@@ -271,6 +271,16 @@ def test_weight_codes_as_a_view_and_what_lies_behind_them(T):
     assert ((ops.linear_q8(rows, w, torch.float32).double() - want).abs() <= want.abs() * 2.0 ** -22).all()
 
 
+@pytest.mark.parametrize("T", [1, 20, 200])
+@pytest.mark.parametrize("K", [1003, 1024])
+def test_weight_codes_stored_by_input_channel(T, K):
+    codes = torch.randint(-127, 128, (K, 264), device=DEV, dtype=torch.int8)
+    w = ops.QuantWeight(codes.t(), torch.rand(264, device=DEV))
+    rows = ops.quantize_rows(bf(T, K))
+    want = (rows.q[:, :K].double() @ codes.double()) * rows.scale.double() * w.scale.double()
+    assert ((ops.linear_q8(rows, w, torch.float32).double() - want).abs() <= want.abs() * 2.0 ** -22).all()
+
+
 def ffn64(x, w13, w2, dy):
     """(y, dx, dw13, dw2) in 64 bits with x and the projection held in 8 bits for the gradients."""
     x, w13, w2, dy = (t.detach().double() for t in (x, w13, w2, dy))

@@ -232,6 +232,18 @@ def test_weight_codes_that_end_with_their_storage_are_copied():
     assert ops.QuantWeight(q, torch.ones(3)).q.data_ptr() == q.data_ptr()
 
 
+# codes stored by input channel, a column of a wider matrix, one channel for all: of inner dimensions that are whole 16-byte pieces and not
+@pytest.mark.parametrize("K", [16, 19, 48, 64])
+def test_weight_codes_in_every_layout_become_dense_rows(K):
+    q = torch.randint(-127, 128, (24, K), dtype=torch.int8, generator=torch.Generator().manual_seed(K))
+    wide = torch.zeros(24, K, 5, dtype=torch.int8)
+    wide[:, :, 2] = q
+    for view in (q.t().contiguous().t(), wide[:, :, 2], q[:1].expand(24, K), q.flip(0)[::2]):
+        w = ops.QuantWeight(view, torch.ones(view.shape[0]))
+        assert w.q.equal(view) and w.q.stride(1) == 1 and w.q.stride(0) % 16 == 0 and w.q.stride(0) >= K
+        assert w.q.data_ptr() % 16 == 0 and w.q.untyped_storage().nbytes() >= (w.q.shape[0] - 1) * w.q.stride(0) + -(-K // 16) * 16
+
+
 def _step(mode, packed=True, shard=False):
     m = build_model(ARGS, seed=3)
     m.activation_checkpointing = mode
