@@ -661,6 +661,19 @@ __device__ __forceinline__ void epilogue_attn_dout(const Gemm2Params& p, uint32_
 // of a row an instruction, since a lane that stores its own row touches 32 lines: 777 x 1003 x 1111 9.2 us, 777 x 1008 x 1112 by TMA 7.5.
 // K of 2048 and more is bound by the main loop (4096 x 2048 x 16384: 94 us, 2918 T/s, tensor pipe 82 % busy at the 1.67 GHz that the
 // power cap leaves; 2048 x 8192 x 8192 3130 T/s); shorter ones by this, the proxy fence and the loads of a box: 8192 x 512 x 4096 27 us.
+// A box some of whose scales multiply out of the normal numbers: column by column, since code that few tiles need is short rather than fast.
+template <bool F32>
+__device__ __forceinline__ void box_q8_far(const Gemm2Params& p, uint32_t acc, int lane, float sr, int col0, uint32_t buf) {
+  const uint32_t rowaddr = buf + (uint32_t)lane * 128u, sw = (uint32_t)(lane & 7);
+#pragma unroll 1
+  for (uint32_t e = 0; e < (F32 ? 32u : 64u); ++e) {
+    uint32_t sum;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;" : "=r"(sum) : "r"(acc + e));
+    const float v = scaled((int)sum, sr, col0 + (int)e < p.N ? p.q8_col[col0 + e] : 0.f);
+    if (F32) asm volatile("st.shared.f32 [%0], %1;" ::"r"(rowaddr + (((e >> 2) ^ sw) << 4) + (e & 3u) * 4u), "f"(v) : "memory");
+    else     asm volatile("st.shared.b16 [%0], %1;" ::"r"(rowaddr + (((e >> 3) ^ sw) << 4) + (e & 7u) * 2u), "h"(__bfloat16_as_ushort(__float2bfloat16(v))) : "memory");
+  }
+}
 template <bool F32>
 __device__ __forceinline__ void epilogue_q8(const Gemm2Params& p, uint32_t tmem_acc, int quad, int turn, int lane, int m0, int n0,
                                             uint32_t buf, uint32_t& n_boxes) {
@@ -673,6 +686,9 @@ __device__ __forceinline__ void epilogue_q8(const Gemm2Params& p, uint32_t tmem_
   for (int c = turn; c < p.tile_n / COLS; c += 2) {
     const int col0 = n0 + c * COLS;
     if (col0 >= p.N) break;                          // warp-uniform
+    float own[COLS / 32];                            // a lane looks at one column of each half for all
+#pragma unroll
+    for (int hh = 0; hh < COLS / 32; ++hh) own[hh] = col0 + hh * 32 + lane < p.N ? p.q8_col[col0 + hh * 32 + lane] : 0.f;
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // one box a warp: the other warp of the quadrant works meanwhile
     __syncwarp();
 #pragma unroll
@@ -689,6 +705,15 @@ __device__ __forceinline__ void epilogue_q8(const Gemm2Params& p, uint32_t tmem_
           sc[e].y = col + 4 * e + 1 < p.N ? p.q8_col[col + 4 * e + 1] : 0.f;
           sc[e].z = col + 4 * e + 2 < p.N ? p.q8_col[col + 4 * e + 2] : 0.f;
           sc[e].w = col + 4 * e + 3 < p.N ? p.q8_col[col + 4 * e + 3] : 0.f;
+        }
+      }
+      if (hh == 0) {                                 // behind the loads, in one latency with them
+        const ScaleRange rows = scale_range(sr);
+        bool plain = in_range(rows, own[0]);
+        if (!F32) plain = plain && in_range(rows, own[COLS / 32 - 1]);
+        if (!__all_sync(0xffffffffu, plain)) {
+          box_q8_far<F32>(p, tmem_acc + c * COLS + lane_sel, lane, sr, col0, buf);
+          break;
         }
       }
       uint32_t r[32];
@@ -1435,8 +1460,8 @@ __global__ void __launch_bounds__(256) join_q8_kernel(const int* x, const float*
     const float r = sx[row];
     const float4 q = reinterpret_cast<const float4*>(sw)[c];
     Out* p = y + row * ldc + 4LL * c;                // rows of any stride and alignment
-    p[0] = (Out)((float)a.x * (r * q.x)); p[1] = (Out)((float)a.y * (r * q.y));
-    p[2] = (Out)((float)a.z * (r * q.z)); p[3] = (Out)((float)a.w * (r * q.w));
+    p[0] = (Out)scaled(a.x, r, q.x); p[1] = (Out)scaled(a.y, r, q.y);
+    p[2] = (Out)scaled(a.z, r, q.z); p[3] = (Out)scaled(a.w, r, q.w);
   }
 }
 

@@ -11,6 +11,7 @@
 // each are launch, barriers, tensor memory, first loads and the last sums.  With the owners loading from the others' memory instead, one
 // word at a time, 128 tokens of 2048 x 2048 took 49 us, 10.4 in this form; from 65 on CTA pairs are as fast or faster.
 // No load carries a cluster-multicast qualifier.  Every wait is bounded; on expiry TPLR_ST_WAIT_TIMEOUT is set and all roles return.
+#include "quant.cuh"
 #include "tcgen05.cuh"
 
 namespace {
@@ -144,11 +145,15 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q8_stream_kernel(const __grid
   const int c = (warp & 3) * 32 + lane, n = n0 + c, first = p.split > 1 ? (int)rank * p.mine : 0;
   const uint32_t part = sX + n_stages * x_stage, part_cta = (uint32_t)p.mine * ROWS * 4u;
   float sn = 0.f, st[2] = {};
+  bool plain = true;                               // every product of this warp's scales is a normal number or zero
+  auto value = [&](uint32_t sum, float t) { return plain ? (float)(int)sum * (t * sn) : scaled_far((int)sum, t, sn); };
   if (warp >= 2) {
     sn = n < p.N ? p.sw[n] : 0.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
       if (first + j * 32 + lane < p.T) st[j] = p.sx[first + j * 32 + lane];
+    const ScaleRange r0 = scale_range(st[0]), r1 = scale_range(st[1]);
+    plain = __all_sync(0xffffffffu, in_range(r0, sn) && in_range(r1, sn));
     const bool ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_done), 0, abort_flag));
     tcgen05_fence_after();
 #pragma unroll
@@ -165,8 +170,8 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q8_stream_kernel(const __grid
       } else {
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const float sc = __shfl_sync(0xffffffffu, st[j], e) * sn;
-          if (j * 32 + e < p.T && n < p.N) store(p, j * 32 + e, n, (float)(int)r[e] * sc);
+          const float t = __shfl_sync(0xffffffffu, st[j], e);
+          if (j * 32 + e < p.T && n < p.N) store(p, j * 32 + e, n, value(r[e], t));
         }
       }
     }
@@ -188,8 +193,8 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q8_stream_kernel(const __grid
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float sc = __shfl_sync(0xffffffffu, st[0], e + i) * sn;
-          if (first + e + i < p.T && n < p.N) store(p, first + e + i, n, (float)sum[i] * sc);
+          const float t = __shfl_sync(0xffffffffu, st[0], e + i);
+          if (first + e + i < p.T && n < p.N) store(p, first + e + i, n, value((uint32_t)sum[i], t));
         }
       }
     }

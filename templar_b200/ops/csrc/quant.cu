@@ -791,7 +791,7 @@ __global__ void __launch_bounds__(256, 3) gemm_q8_few_kernel(const void* x, cons
       int sum = 0;
 #pragma unroll
       for (int k = 0; k < 8; ++k) sum += s_sum[turn][k][t][c];
-      y[t * ldy + n] = (Out)((float)sum * ((HELD ? s_sx[t] : sx[t]) * sw[n]));
+      y[t * ldy + n] = (Out)scaled(sum, HELD ? s_sx[t] : sx[t], sw[n]);
     }
   }
 }

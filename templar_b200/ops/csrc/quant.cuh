@@ -36,3 +36,30 @@ static __device__ __forceinline__ void numbers4(uint32_t w, float* f) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | i)) - 8388736.f;
 }
+
+// A sum of integers times the scales of its row and its column.  The scales multiply one another first; where that leaves the normal
+// numbers although the result may be one (groups are held down to 2^-100 and up to what fp32 holds), half of each scale's exponent
+// waits for the end: with s = h * t and t a power of two near sqrt(s), the product h * h' and its product with the sum are normal wherever
+// the result is, and a power of two changes no bit of it.  Where both ways stay normal they give the same bits.
+static __device__ __forceinline__ float power_near_root(uint32_t s) { return __uint_as_float(((s >> 1) & 0x3f800000u) + 0x20000000u); }
+static __device__ __forceinline__ float scaled_far(int sum, float row, float col) {
+  const float tr = power_near_root(magnitude(row)), tc = power_near_root(magnitude(col));        // 2^-63 to 2^64
+  const float hr = row * __uint_as_float(0x7f000000u - __float_as_uint(tr)), hc = col * __uint_as_float(0x7f000000u - __float_as_uint(tc));
+  return (float)sum * (hr * hc) * fminf(tr * tc, 0x1p127f);      // 2^128 only where every sum but 0 gives infinity
+}
+static __device__ __forceinline__ float scaled(int sum, float row, float col) {
+  const float s = row * col;
+  return magnitude(s) - 0x00800000u < 0x7f000000u ? (float)sum * s : scaled_far(sum, row, col);
+}
+// The least and the largest magnitude of a warp's scales, zeros and what is not finite left out, and whether all their products with
+// another scale are normal numbers, or zero because that one is.
+struct ScaleRange { float least, most; };
+static __device__ __forceinline__ ScaleRange scale_range(float s) {
+  const uint32_t m = magnitude(s);
+  const bool in = m - 1u < 0x7f7fffffu;
+  return {__uint_as_float(__reduce_min_sync(0xffffffffu, in ? m : 0x7f800000u)), __uint_as_float(__reduce_max_sync(0xffffffffu, in ? m : 0u))};
+}
+static __device__ __forceinline__ bool in_range(const ScaleRange& r, float s) {
+  const float m = fabsf(s);
+  return m == 0.f || (m * r.least >= 0x1p-126f && m * r.most < __uint_as_float(0x7f800000u));
+}

@@ -247,8 +247,9 @@ def swiglu_q8(gu: torch.Tensor) -> QuantRows:
 
 
 def linear_q8(x: torch.Tensor | QuantRows, w: QuantWeight, out_dtype: torch.dtype | None = None) -> torch.Tensor:
-    """``x @ w.T`` from 8-bit rows and an 8-bit weight: exact sums in 32-bit integers, one scale for each row times one for each
-    channel, rounded once to ``out_dtype`` (bf16 or fp32; default: that of ``x``, bf16 for rows in 8 bits).  A tensor ``x`` is
+    """``x @ w.T`` from 8-bit rows and an 8-bit weight: exact sums in 32-bit integers, times one scale for each row and one for each
+    channel in fp32 (the sum, the scales' product and the result are rounded to 24 bits; no step leaves the range where the result
+    does not), rounded to ``out_dtype`` (bf16 or fp32; default: that of ``x``, bf16 for rows in 8 bits).  A tensor ``x`` is
     quantised first, by rows.  Forward passes only."""
     out_dtype = out_dtype or (torch.bfloat16 if isinstance(x, QuantRows) else x.dtype)
     if not isinstance(x, QuantRows):
@@ -279,7 +280,7 @@ def linear_q8(x: torch.Tensor | QuantRows, w: QuantWeight, out_dtype: torch.dtyp
                                     x.q.stride(0), w.q.stride(0), N, int(out_dtype == torch.float32), OF.status_word(y.device).data_ptr(),
                                     native.stream_ptr()), "gemm_q8")
         return y
-    y = (x.q[:, :K].double() @ w.q.double().t()).float() * (x.scale * w.scale)
+    y = (x.q[:, :K].double() @ w.q.double().t()) * x.scale.double() * w.scale.double()       # 64 bits: the scales may multiply out of 32
     return y.to(out_dtype).view(*x.shape[:-1], N)
 
 

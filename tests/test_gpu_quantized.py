@@ -271,6 +271,36 @@ def test_weight_codes_as_a_view_and_what_lies_behind_them(T):
     assert ((ops.linear_q8(rows, w, torch.float32).double() - want).abs() <= want.abs() * 2.0 ** -22).all()
 
 
+# a few tokens, streamed in one CTA a block and in clusters, on CTA pairs with and without TMA stores, the inner dimension in parts
+@pytest.mark.parametrize("T,K,N", [(3, 256, 40), (20, 256, 40), (40, 4096, 130), (200, 256, 320), (200, 256, 333), (100, 4096, 768)])
+@pytest.mark.parametrize("sx,sw", [(2.0 ** -73, 2.0 ** -60), (2.0 ** -87, 2.0 ** -64), (2.0 ** -107, 2.0 ** -40), (2.0 ** -107, 2.0 ** 121),
+                                   (2.0 ** 90, 2.0 ** 60), (2.0 ** 121, 2.0 ** -140)])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+def test_products_whose_scales_multiply_out_of_range(T, K, N, sx, sw, out):
+    g = torch.Generator(device=DEV).manual_seed(0)
+    q, wq = (torch.randint(64, 128, (n, K), dtype=torch.int8, generator=g, device=DEV) for n in (T, N))
+    wq[1] = 0
+    spread = lambda n: torch.linspace(1, 2, n, device=DEV)  # noqa: E731
+    rows = ops.QuantRows(q, (sx * spread(T))[:, None].contiguous(), 0, (T, K))
+    rows.scale[0], rows.scale[T - 1] = 0, float("nan")
+    w = ops.QuantWeight(wq, sw * spread(N))
+    y = ops.linear_q8(rows, w, out)
+    want = (q.double() @ wq.double().t()) * rows.scale.double() * w.scale.double()
+    assert y[T - 1].isnan().all() and (y[0] == 0).all() and (y[:T - 1, 1] == 0).all()
+    rel, tiny = (2.0 ** -22, 2.0 ** -148) if out == torch.float32 else (HALF, 2.0 ** -132)
+    y, want = y[:T - 1].double(), want[:T - 1]
+    far = want.abs() > 2.0 ** 128
+    assert y[far].isinf().all() and ((y - want).abs() <= want.abs() * rel + tiny)[~far].all()
+    # scales of both kinds side by side: a result does not depend on its neighbours
+    near = ops.QuantRows(q, rows.scale.clone(), 0, (T, K))
+    near.scale[1::2], wn = 1.0, w.scale.clone()
+    wn[::2] = 0.5
+    z = ops.linear_q8(near, ops.QuantWeight(wq, wn), out)
+    assert z[2:T - 1:2, 1::2].double().equal(y[2::2, 1::2])
+    assert z[1::2, ::2].equal(ops.linear_q8(ops.QuantRows(q, torch.ones(T, 1, device=DEV), 0, (T, K)), ops.QuantWeight(wq, torch.full((N,), 0.5, device=DEV)), out)[1::2, ::2])
+    healthy()
+
+
 @pytest.mark.parametrize("T", [1, 20, 200])
 @pytest.mark.parametrize("K", [1003, 1024])
 def test_weight_codes_stored_by_input_channel(T, K):

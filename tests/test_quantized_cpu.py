@@ -77,6 +77,26 @@ def test_product_is_the_one_of_the_kept_values(T, K, N):
     assert (qw.dequantize(torch.float32) - w).abs().max() <= qw.scale.max() * 0.50001
 
 
+# (rows' scale, channels' scale): products of the two below and above the normal numbers, whose results are normal, tiny or zero
+@pytest.mark.parametrize("sx,sw", [(2.0 ** -73, 2.0 ** -60), (2.0 ** -87, 2.0 ** -64), (2.0 ** -107, 2.0 ** -40), (2.0 ** -107, 2.0 ** 121),
+                                   (2.0 ** 90, 2.0 ** 60), (2.0 ** 121, 2.0 ** -140)])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+def test_products_whose_scales_multiply_out_of_range(sx, sw, out):
+    T, K, N = 4, 4096, 6
+    g = torch.Generator().manual_seed(0)
+    q = torch.randint(64, 128, (T, K), dtype=torch.int8, generator=g)
+    wq = torch.randint(64, 128, (N, K), dtype=torch.int8, generator=g)
+    wq[1] = 0
+    rows = ops.QuantRows(q, torch.full((T, 1), sx) * torch.tensor([[1.0], [1.3], [0.0], [float("nan")]]), 0, (T, K))
+    y = ops.linear_q8(rows, ops.QuantWeight(wq, torch.full((N,), sw) * 1.7), out)
+    want = (q.double() @ wq.double().t()) * rows.scale.double() * torch.full((N,), sw).mul(1.7).double()
+    assert y[3].isnan().all() and (y[2] == 0).all() and (y[:3, 1] == 0).all()
+    # one rounding to 24 or 8 bits after three of 24, and half a step of the smallest numbers at each
+    rel, tiny = (2.0 ** -22, 2.0 ** -148) if out == torch.float32 else (2.0 ** -8, 2.0 ** -132)
+    far = want[:3].abs() > 2.0 ** 128
+    assert y[:3][far].isinf().all() and ((y[:3].double() - want[:3]).abs() <= want[:3].abs() * rel + tiny)[~far].all()
+
+
 def test_forward_operators_against_their_formulas():
     res, delta, w = rand(5, 96), rand(5, 96, seed=1), rand(96, seed=2)
     h, rows = ops.add_rmsnorm_q8(res, delta, w)
