@@ -694,13 +694,15 @@ __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ uint32_t first_bytes(int n) { return n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u; }
 //
 // HELD: x is bf16 and its rows are put in 8 bits here, by every CTA for itself, while its first pieces of the weight are on their way: as
 // many values as the threads hold, HELD_MOST; one launch instead of two.  One token, one launch and two: 2048 x 2048 3.1 and 4.1 us, 4096 x 6144
 // 6.9 and 8.5, 2048 x 16384 8.5 and 9.8 (4.0 TB/s); with 16384 values held a call of the last took 13.7, two CTAs an SM.
+// TAIL: K is not whole 16-byte pieces, and codes behind it, which are the caller's, are masked; in one form for both 1 x 4096 x 6144 took 4.8 us, not 4.4.
 constexpr int FEW = 8, FEW_UNROLL = 4, HELD_MOST = 4096, HELD_PIECES = HELD_MOST / 2048;
 __host__ __device__ constexpr int held_stride(int kp) { return (kp + 511) / 512 * 512 + 64; }          // rows 64 bytes apart in the banks
-template <class Out, bool HELD>
+template <class Out, bool HELD, bool TAIL>
 __global__ void __launch_bounds__(256, 3) gemm_q8_few_kernel(const void* x, const int8_t* w, const float* sx, const float* sw, Out* y, int T, int N,
                                                           int K, ll ldx, ll ldw, ll ldy) {
   __shared__ int s_sum[2][8][8][17];
@@ -775,6 +777,10 @@ __global__ void __launch_bounds__(256, 3) gemm_q8_few_kernel(const void* x, cons
         b[u] = zero;
         if (k < kp && tok < T)
           b[u] = HELD ? *reinterpret_cast<const uint4*>(s_x + tok * stride + k) : *reinterpret_cast<const uint4*>(static_cast<const int8_t*>(x) + tok * ldx + k);
+        if (TAIL && k < K && k + 16 > K) {                              // what lies behind a row's last column counts for nothing
+          b[u].x &= first_bytes(K - k); b[u].y &= first_bytes(K - k - 4);
+          b[u].z &= first_bytes(K - k - 8); b[u].w &= first_bytes(K - k - 12);
+        }
       }
 #pragma unroll
       for (int u = 0; u < FEW_UNROLL; ++u) {
@@ -796,10 +802,10 @@ __global__ void __launch_bounds__(256, 3) gemm_q8_few_kernel(const void* x, cons
   }
 }
 
-template <class Out, bool HELD>
+template <class Out, bool HELD, bool TAIL>
 int gemm_q8_few(const void* x, const void* w, const float* sx, const float* sw, void* y, int T, int N, int K, ll ldx, ll ldw, ll ldy, void* st) {
   const int blocks = (N + 15) / 16, resident = 3 * tplr_sm_count(), turns = (blocks + resident - 1) / resident;
-  return (int)launch_pdl(gemm_q8_few_kernel<Out, HELD>, (blocks + turns - 1) / turns, 256, 0, (cudaStream_t)st, x, (const int8_t*)w, sx, sw, (Out*)y, T, N, K, ldx,
+  return (int)launch_pdl(gemm_q8_few_kernel<Out, HELD, TAIL>, (blocks + turns - 1) / turns, 256, 0, (cudaStream_t)st, x, (const int8_t*)w, sx, sw, (Out*)y, T, N, K, ldx,
                          ldw, ldy);
 }
 
@@ -990,14 +996,18 @@ static bool streamed(int T) { return T <= 64; }
 TPLR_API ll tplr_gemm_q8_workspace(int T, int N, int K) { return streamed(T) ? 0 : tplr_gemm2_q8_workspace(T, N, K); }
 
 // y[T, N] = sx[t] * sw[n] * (x w^T) for int8 rows x [T, K] and w [N, K] on 16-byte boundaries, y bf16 or fp32 with row stride ldy.  The
-// bytes of a row from K to the next 16-byte boundary are read: zeros in x, anything in w.  ws: tplr_gemm_q8_workspace elements, 16-byte
+// bytes of a row from K to the next 16-byte boundary may be read and count for nothing.  ws: tplr_gemm_q8_workspace elements, 16-byte
 // aligned.
 TPLR_API int tplr_gemm_q8(const void* x, const void* w, const float* sx, const float* sw, void* y, void* ws, int T, int N, int K, ll ldx, ll ldw,
                           ll ldy, int out_fp32, unsigned int* status, void* stream) {
   TPLR_ENTER();
   if (T <= 0 || N <= 0) return 0;
   if (K <= 0 || K > 131072 || (ldx | ldw) % 16 || (((uintptr_t)x | (uintptr_t)w) & 15)) return (int)cudaErrorInvalidValue;
-  if (few_tokens(T, K)) return (out_fp32 ? gemm_q8_few<float, false> : gemm_q8_few<bf16, false>)(x, w, sx, sw, y, T, N, K, ldx, ldw, ldy, stream);
+  if (few_tokens(T, K)) {
+    auto few = K % 16 ? (out_fp32 ? gemm_q8_few<float, false, true> : gemm_q8_few<bf16, false, true>)
+                      : (out_fp32 ? gemm_q8_few<float, false, false> : gemm_q8_few<bf16, false, false>);
+    return few(x, w, sx, sw, y, T, N, K, ldx, ldw, ldy, stream);
+  }
   if (streamed(T)) return tplr_gemm_q8_stream(x, w, sx, sw, y, T, N, K, ldx, ldw, ldy, out_fp32, status, stream);
   return tplr_gemm2_q8(x, w, sx, sw, y, (int*)ws, T, N, K, ldx, ldw, ldy, out_fp32, status, stream);
 }
@@ -1011,5 +1021,5 @@ TPLR_API int tplr_linear_q8_few(const void* x, const void* w, const float* sw, v
   int share = 256;
   while (share * T > 256) share /= 2;
   if ((K + 15) / 16 * 2 > share * HELD_PIECES) return -111;
-  return gemm_q8_few<bf16, true>(x, w, nullptr, sw, y, T, N, K, ldx, ldw, ldy, stream);
+  return gemm_q8_few<bf16, true, false>(x, w, nullptr, sw, y, T, N, K, ldx, ldw, ldy, stream);
 }

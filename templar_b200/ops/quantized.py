@@ -57,7 +57,7 @@ def _codes(x: torch.Tensor, group: int) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 class QuantRows:
-    """Rows in 8 bits.  ``q``: int8 [T, columns rounded up to 16], zeros behind the last column; ``scale``: fp32 [T, G] (any
+    """Rows in 8 bits.  ``q``: int8 [T, columns rounded up to 16], of which nothing behind the last column counts; ``scale``: fp32 [T, G] (any
     strides), one for the whole row (``group`` 0) or for every ``group`` columns; ``shape``: the rows' own shape."""
 
     __slots__ = ("q", "scale", "group", "shape")

@@ -311,6 +311,18 @@ def test_weight_codes_stored_by_input_channel(T, K):
     assert ((ops.linear_q8(rows, w, torch.float32).double() - want).abs() <= want.abs() * 2.0 ** -22).all()
 
 
+@pytest.mark.parametrize("T", [1, 8, 20, 200])
+@pytest.mark.parametrize("K", [1, 100, 1003, 2047])
+def test_codes_behind_the_last_column_are_not_looked_at(T, K):
+    g = torch.Generator(device=DEV).manual_seed(K)
+    q, full = (torch.randint(-127, 128, (n, -(-K // 16) * 16), generator=g, device=DEV, dtype=torch.int8) for n in (T, 40))
+    w, scale = ops.QuantWeight(full[:, :K], torch.rand(40, device=DEV)), torch.rand(T, 1, device=DEV)
+    assert w.q.data_ptr() == full.data_ptr()
+    want = (q[:, :K].double() @ full[:, :K].double().t()) * scale.double() * w.scale.double()
+    got = ops.linear_q8(ops.QuantRows(q, scale, 0, (T, K)), w, torch.float32)
+    assert ((got.double() - want).abs() <= want.abs() * 2.0 ** -22).all()
+
+
 def ffn64(x, w13, w2, dy):
     """(y, dx, dw13, dw2) in 64 bits with x and the projection held in 8 bits for the gradients."""
     x, w13, w2, dy = (t.detach().double() for t in (x, w13, w2, dy))
