@@ -142,7 +142,7 @@ def _values(q, scale, group: int, shape, dtype, weight=None):
     wide = scale if not group else scale.repeat_interleave(group, dim=1)[:, :D]
     v = q[:, :D].float() * wide
     if weight is not None:
-        v = v * weight.detach().float()
+        v = v * weight.detach().reshape(-1).float()
     return v.to(dtype).view(shape)
 
 

@@ -65,6 +65,17 @@ def test_leading_shapes_views_and_weights_of_the_columns():
     assert torch.equal(ops.dequantize_rows(r, torch.float32, w), r.dequantize(torch.float32) * w)
 
 
+def test_weights_of_the_columns_in_any_shape():
+    x, w = rand(40, 40), rand(40, seed=1)                      # as many rows as columns: a column of weights would multiply the rows
+    r = ops.quantize_rows(x, 64)
+    want = r.dequantize(torch.float32) * w
+    for shape in ((40,), (40, 1), (1, 40), (1, 40, 1)):
+        assert torch.equal(ops.dequantize_rows(r, torch.float32, w.view(shape)), want)
+        assert torch.equal(r.dequantize(weight=w.view(shape)), want.to(torch.bfloat16))
+    with pytest.raises(ValueError, match="weights for 40 columns"):
+        ops.dequantize_rows(r, torch.float32, w[:39])
+
+
 @pytest.mark.parametrize("T,K,N", [(1, 1, 1), (3, 17, 5), (8, 128, 64)])
 def test_product_is_the_one_of_the_kept_values(T, K, N):
     x, w = rand(T, K), rand(N, K, seed=1)
