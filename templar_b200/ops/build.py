@@ -32,6 +32,9 @@ NVCC_FLAGS = [
     "--expt-relaxed-constexpr",
 ]
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"]
+# The C++ library by the name that PyTorch's own libraries need: a compiler that finds only an archive beside it would put a second
+# copy into the module, and a number written to a stream of one copy with the other's locale, as in every error's message, ends the process.
+HOST_LIBS = ["-l:libstdc++.so.6", "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lc10_cuda"]
 # Approximate intrinsics and flush-to-zero only where the arithmetic is a softmax in base 2 (the flash
 # attention kernels).  The loss, the norms, the optimizer, the quantiser and the compression kernels are
 # compiled with IEEE division / square root and keep denormals; where they want a fast exponential they
@@ -86,7 +89,7 @@ def _host_key() -> str:
     """What the extension module depends on beside its sources: a module of another PyTorch must not be loaded."""
     import torch
 
-    return "\n".join([torch.__version__, sys.version, *HOST_FLAGS, _abi_flag()])
+    return "\n".join([torch.__version__, sys.version, *HOST_FLAGS, *HOST_LIBS, _abi_flag()])
 
 
 def _host_key_path() -> Path:
@@ -117,7 +120,7 @@ def build_host(force: bool = False) -> Path:
     inc = [x for p in [*include_paths("cuda"), sysconfig.get_paths()["include"]] for x in ("-isystem", p)]
     tmp = out.with_suffix(f".{os.getpid()}.tmp")       # ranks that start together may all build
     _run([os.environ.get("CXX", "g++"), *HOST_FLAGS, _abi_flag(), *inc, *map(str, srcs), "-o", str(tmp),
-          "-L" + str(Path(torch.__file__).parent / "lib"), "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lc10_cuda"])
+          "-L" + str(Path(torch.__file__).parent / "lib"), *HOST_LIBS])
     os.replace(tmp, out)
     _host_key_path().write_text(_host_key())
     return out

@@ -557,6 +557,8 @@ Aside opt(const std::optional<Tensor>& t) { return Aside{t ? *t : Tensor()}; }
 PYBIND11_MODULE(tplr_host, m) {
   typedef py::call_guard<py::gil_scoped_release> nogil;
   m.def("bind", &bind);
+  // what every call of an entry goes through
+  m.def("check", [](int err, const std::string& what) { check(err, what.c_str()); }, nogil());
   m.def("launches", [] { return g_launches.load(std::memory_order_relaxed); });
   m.def("rmsnorm", [](const Tensor& x, const Tensor& w, const std::optional<Tensor>& buffer, double eps, const Tensor& status) {
     return RMSNorm::apply(x, w, opt(buffer), eps, Aside{status});

@@ -1,6 +1,8 @@
 """The builder of the two native libraries, with scripts in the compilers' places."""
 
 import os
+import subprocess
+import sys
 import tomllib
 from pathlib import Path
 
@@ -152,3 +154,17 @@ def test_operators_keep_their_python_nodes_without_the_extension_module(monkeypa
         assert native.host() is None
     native.launch_count = 5
     assert native.launch_count == 5
+
+
+def test_an_error_of_an_entry_reaches_python_from_the_module():
+    """The message of an error holds a number.  In a process of its own: a module with a second copy of the C++ library died there."""
+    script = ("from templar_b200.ops import native\n"
+              "for what in ('one', 'another'):\n"
+              "    try:\n        native.host().check(719, what)\n"
+              "    except RuntimeError as e:\n        print(e)\n"
+              "native.host().check(0, 'nothing')\nprint('alive')\n")
+    if not B.host_usable():
+        pytest.skip("the module has not been built here")
+    r = subprocess.run([sys.executable, "-c", script], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert r.stdout.split("\n")[:3] == ["one failed with CUDA error 719", "another failed with CUDA error 719", "alive"]
