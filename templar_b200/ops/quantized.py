@@ -57,7 +57,8 @@ def _codes(x: torch.Tensor, group: int) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 class QuantRows:
-    """Rows in 8 bits.  ``q``: int8 [T, columns rounded up to 16], of which nothing behind the last column counts; ``scale``: fp32 [T, G] (any
+    """Rows in 8 bits.  ``q``: int8 [T, columns rounded up to 16], of which nothing behind the last column counts (copied from a
+    place that is not on a 16-byte boundary); ``scale``: fp32 [T, G] (any
     strides), one for the whole row (``group`` 0) or for every ``group`` columns; ``shape``: the rows' own shape."""
 
     __slots__ = ("q", "scale", "group", "shape")
@@ -71,6 +72,8 @@ class QuantRows:
         if scale.dtype != torch.float32 or scale.shape != (q.shape[0], -(-D // group) if group else 1) or scale.device != q.device:
             raise ValueError(f"QuantRows: fp32 scales [{q.shape[0]}, {-(-D // group) if group else 1}] on {q.device} expected, got "
                              f"{scale.dtype} {tuple(scale.shape)} on {scale.device}")
+        if q.data_ptr() % 16:
+            q = q.clone()
         self.q, self.scale, self.group, self.shape = q, scale, int(group), torch.Size(shape)
 
     @classmethod

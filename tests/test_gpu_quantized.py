@@ -323,6 +323,14 @@ def test_codes_behind_the_last_column_are_not_looked_at(T, K):
     assert ((got.double() - want).abs() <= want.abs() * 2.0 ** -22).all()
 
 
+@pytest.mark.parametrize("T", [2, 20, 200])
+def test_row_codes_off_a_16_byte_boundary(T):
+    buf = torch.randint(-127, 128, (T * 64 + 1,), device=DEV, dtype=torch.int8)
+    w = ops.quantize_weight(bf(40, 64))
+    rows = [ops.QuantRows(q, torch.ones(T, 1, device=DEV), 0, (T, 64)) for q in (buf[1:].view(T, 64), buf[1:].clone().view(T, 64))]
+    assert ops.linear_q8(rows[0], w).equal(ops.linear_q8(rows[1], w)) and rows[0].dequantize().equal(rows[1].dequantize())
+
+
 def ffn64(x, w13, w2, dy):
     """(y, dx, dw13, dw2) in 64 bits with x and the projection held in 8 bits for the gradients."""
     x, w13, w2, dy = (t.detach().double() for t in (x, w13, w2, dy))

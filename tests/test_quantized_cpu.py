@@ -65,6 +65,14 @@ def test_leading_shapes_views_and_weights_of_the_columns():
     assert torch.equal(ops.dequantize_rows(r, torch.float32, w), r.dequantize(torch.float32) * w)
 
 
+def test_row_codes_off_a_16_byte_boundary_are_copied():
+    buf = torch.randint(-127, 128, (3 * 32 + 1,), dtype=torch.int8, generator=torch.Generator().manual_seed(0))
+    for at in (0, 1):
+        q = buf[at:at + 96].view(3, 32)
+        r = ops.QuantRows(q, torch.ones(3, 1), 0, (3, 20))
+        assert r.q.equal(q) and r.q.data_ptr() % 16 == 0 and (r.q.data_ptr() == q.data_ptr()) == (q.data_ptr() % 16 == 0)
+
+
 def test_weights_of_the_columns_in_any_shape():
     x, w = rand(40, 40), rand(40, seed=1)                      # as many rows as columns: a column of weights would multiply the rows
     r = ops.quantize_rows(x, 64)
