@@ -133,7 +133,7 @@ def dequantize_rows(rows: QuantRows, dtype: torch.dtype = torch.bfloat16, weight
 
 def _values(q, scale, group: int, shape, dtype, weight=None):
     T, D = q.shape[0], shape[-1]
-    if q.is_cuda and dtype == torch.bfloat16 and _native_rows(weight):
+    if q.is_cuda and dtype == torch.bfloat16 and (group in (0, GROUP) or group >= D) and _native_rows(weight):
         if host := native.host():
             return host.dequantize_rows(q, scale, group, shape, None if weight is None else weight.detach())
         y = torch.empty(shape, dtype=dtype, device=q.device)

@@ -331,6 +331,17 @@ def test_row_codes_off_a_16_byte_boundary(T):
     assert ops.linear_q8(rows[0], w).equal(ops.linear_q8(rows[1], w)) and rows[0].dequantize().equal(rows[1].dequantize())
 
 
+@pytest.mark.parametrize("group", [32, 48, 100, 128])
+def test_rows_of_a_callers_own_groups(group):
+    T, D = 5, 112
+    q = torch.randint(-127, 128, (T, D), device=DEV, dtype=torch.int8)
+    scale, w = torch.rand(T, -(-D // group), device=DEV), bf(D)
+    want = q.double() * wide(scale, group, D).double()
+    rows = ops.QuantRows(q, scale, group, (T, D))
+    assert ((rows.dequantize().double() - want).abs() <= want.abs() * HALF).all()
+    assert ((rows.dequantize(weight=w).double() - want * w.double()).abs() <= (want * w.double()).abs() * HALF).all()
+
+
 def ffn64(x, w13, w2, dy):
     """(y, dx, dw13, dw2) in 64 bits with x and the projection held in 8 bits for the gradients."""
     x, w13, w2, dy = (t.detach().double() for t in (x, w13, w2, dy))
