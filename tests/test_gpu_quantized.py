@@ -218,6 +218,13 @@ def test_product(T, K, N, out):
     healthy()
 
 
+# 340 tiles of 256 x 256, with and without TMA stores: each pair has several in turn, the last turn not all of them
+@pytest.mark.parametrize("T,K,N", [(5003, 640, 4104), (5003, 333, 4101), (2900, 128, 9000)])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_product_of_several_tiles_a_pair(T, K, N, out):
+    test_product(T, K, N, out)
+
+
 # inner dimensions that are cut into parts (4, 4, 8, 4, 6, 8 of them, the last of fewer blocks), rows that do not end with a plane's last box of 32
 @pytest.mark.parametrize("T,K,N", [(256, 8192, 2048), (333, 5001, 1004), (100, 4096, 768), (130, 14336, 4096), (65, 6000, 1536), (65, 131072, 12)])
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
@@ -396,6 +403,21 @@ def test_feed_forward(T, D, Fd):
     assert dx.equal(got[1])
     for m, a in ((mg13, got[2]), (mg2, got[3])):
         assert ((m - 1 - a.float()).abs() <= a.float().abs() * HALF + 2.0 ** -18 * (1 + a.float().abs())).all()
+    healthy()
+
+
+# 320 and 160 tiles of 256 x 256 for half as many pairs as there are SMs, or more of narrower ones: each pair has several in turn, the last turn
+# not all of them, the last rows of tiles are cut off; with fewer hidden units than a tile's columns in the last one
+@pytest.mark.parametrize("T,D,Fd", [(5003, 256, 2048), (4390, 128, 2944)])
+def test_feed_forward_of_several_tiles_a_pair(T, D, Fd):
+    test_feed_forward(T, D, Fd)
+    x, w13, w2 = bf(T, D).requires_grad_(), bf(2 * Fd, D, std=D ** -0.5, seed=1).requires_grad_(), bf(D, Fd, std=Fd ** -0.5, seed=2).requires_grad_()
+    dy = bf(T, D, seed=3)
+    y = ops.feed_forward_saved8(x, w13, w2)
+    got = (y, *torch.autograd.grad(y, (x, w13, w2), dy))
+    # by token and by hidden unit, so that one box of 32 x 64 cannot hide: 0.003 in norm each, up to four times that where a row is short
+    for a, b, dim in zip(got, ffn64(x, w13, w2, dy), (1, 1, 1, 0)):
+        assert ((a.double() - b).norm(dim=dim) <= 0.012 * b.norm(dim=dim)).all()
     healthy()
 
 
