@@ -832,7 +832,9 @@ __device__ __forceinline__ void epilogue_swiglu_q8(const Gemm2Params& p, uint32_
 // turned around in shared memory and stored by rows, without fences and barriers, take 4 % longer than this.
 // In turn with the bf16 form, which forms no activation: 16384 x 2048 -> 8192 558 and 468 us, 4096 x 4096 -> 14336 397 and 377, 2048 x 768 ->
 // 2048 22.9 and 22.9.  Left: the third output's bytes, and fixed latencies of a step (tensor pipe 57 % busy, an instruction in 16 % of
-// the cycles).
+// the cycles).  All three outputs are bf16 because the products behind them take bf16 on the tensor cores; so are the rows read back for the
+// packed projection's weight gradient.  That gradient, with both operands rounded, is 0.0029 off in norm where one rounding of the
+// result leaves 0.0017; the codes themselves leave 0.006.
 constexpr uint32_t CODE_STAGE = 4096 + 3 * 4096;     // a quadrant's codes of 64 columns, gate and up; three boxes of 64 columns
 struct CodeLoads {
   uint32_t bar;                      // the quadrant's mbarrier
@@ -1355,8 +1357,9 @@ int pick_parts(int M, int N, int K, int epi) {
 // Parts of K of a product of 8-bit rows: their sums go to int32 planes and a second kernel adds and scales them, so that few tokens and
 // few channels do not leave most pairs idle over a long K; the sum of integers is the same in any order.  The costs above hold: a k block
 // of 128 bytes a row takes what one of bf16 takes.  Microseconds whole, as cut: 256 x 8192 x 2048 16.6, 12.1 in four; 256 x 14336 x 4096
-// 25.3, 20.5 in two; 333 x 5001 x 1004 17.6, 11.4 in four; 100 x 4096 x 768 10.1, 7.8 in eight.  Left whole: 512 x 8192 x 2048 16.8 (15.2
-// in two), 256 x 4096 x 2048 11.0 (10.2 in four), 1024 x 8192 x 2048 18.2 (21.5 in two), 256 x 2048 x 2048 7.8 (8.6).
+// 25.3, 20.5 in two; 333 x 5001 x 1004 17.6, 11.4 in four; 100 x 4096 x 768 10.1, 7.8 in eight.  Left whole, since the
+// count must promise a tenth: 512 x 8192 x 2048 16.8 (15.2 in two) and 256 x 4096 x 2048 11.0 (10.2 in four), which cutting would help all the same, and
+// 1024 x 8192 x 2048 18.2 (21.5 in two), 256 x 2048 x 2048 7.8 (8.6).  The count was fitted to bf16 shapes, not to these.
 int pick_parts_q8(int M, int N, int K) {
   const long long kb = (K + 2 * BK - 1) / (2 * BK), tiles = (long long)((M + TILE_M - 1) / TILE_M) * ((N + TILE_N - 1) / TILE_N);
   const int pairs = tplr_sm_count() / 2;

@@ -4,12 +4,13 @@
 //
 // The weight takes the tensor core's long side: a CTA's tile is 128 output channels (rows of w, lanes of tensor memory) by all the
 // tokens (8 to 64 columns), so no instruction multiplies rows that are not there, as a 256-row tile of tokens would.  A ring of up to
-// 221 KB per SM is in flight all the time.  Where the blocks of 128 channels leave SMs idle, K is cut over the two, four or eight CTAs of a
+// 221 KB per SM is in flight all the time.  Where the blocks of 128 channels leave SMs idle, K is cut over the two to eight CTAs of a
 // cluster; each sends the int32 sums of a token to the CTA that owns it, 16 bytes a store into its shared memory, and the owners add
 // and scale: the sum of integers is the same in any order, and no workspace or second launch is needed.
-// 24 x 4096 x 6144 (two CTAs a block) 9.2 us, 32 x 14336 x 4096 (four) 13.9, 64 x 2048 x 16384 (one) 12.2: 2.6 to 4.2 TB/s of weight; 3 us of
-// each are launch, barriers, tensor memory, first loads and the last sums.  With the owners loading from the others' memory instead, one
-// word at a time, 128 tokens of 2048 x 2048 took 49 us, 10.4 in this form; from 65 on CTA pairs are as fast or faster.
+// Weights in turn, so that each comes from memory: 32 x 4096 x 6144 (two CTAs a block) 9.8 us, 32 x 14336 x 4096 (four) 13.9, 64 x 2048 x 16384
+// (one) 13.3: 2.5 to 4.2 TB/s of weight; one weight again and again, out of L2: 7.6, 9.6 and 10.5.  3 us of each are launch, barriers, tensor memory, first
+// loads and the last sums.  With the owners loading from the others' memory instead, one word at a time, 128 tokens of 2048 x 2048 took
+// 49 us, 10.4 in this form; from 65 on CTA pairs are as fast or faster.
 // No load carries a cluster-multicast qualifier.  Every wait is bounded; on expiry TPLR_ST_WAIT_TIMEOUT is set and all roles return.
 #include "quant.cuh"
 #include "tcgen05.cuh"

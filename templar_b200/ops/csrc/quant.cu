@@ -698,7 +698,8 @@ __device__ __forceinline__ uint32_t first_bytes(int n) { return n >= 4 ? 0xfffff
 //
 // HELD: x is bf16 and its rows are put in 8 bits here, by every CTA for itself, while its first pieces of the weight are on their way: as
 // many values as the threads hold, HELD_MOST; one launch instead of two.  One token, one launch and two: 2048 x 2048 3.1 and 4.1 us, 4096 x 6144
-// 6.9 and 8.5, 2048 x 16384 8.5 and 9.8 (4.0 TB/s); with 16384 values held a call of the last took 13.7, two CTAs an SM.
+// 6.9 and 8.5, 2048 x 16384 8.5 and 9.8; with 16384 values held a call of the last took 13.7, two CTAs an SM.  Those are times of one weight,
+// which stays in L2; with weights in turn one launch takes 3.2, 6.9 and 8.6 us (1.3, 3.6 and 3.9 TB/s).
 // TAIL: K is not whole 16-byte pieces, and codes behind it, which are the caller's, are masked; in one form for both 1 x 4096 x 6144 took 4.8 us, not 4.4.
 constexpr int FEW = 8, FEW_UNROLL = 4, HELD_MOST = 4096, HELD_PIECES = HELD_MOST / 2048;
 __host__ __device__ constexpr int held_stride(int kp) { return (kp + 511) / 512 * 512 + 64; }          // rows 64 bytes apart in the banks
@@ -985,10 +986,11 @@ extern "C" int tplr_gemm_q8_stream(const void* X, const void* W, const float* sx
 
 // Which kernel multiplies 8-bit rows: up to 8 tokens the one that loads the weight into registers, up to 64 (or with a longer K) the weight's
 // rows as the tensor core's long side with K cut over clusters, more on CTA pairs.  Microseconds, the three in that order, inner dimension x
-// channels, at 8 | 32 | 64 | 128 tokens: 2048 x 2048 2.8, 3.9, 6.9 | -, 4.9, 7.0 | -, 6.8, 7.4 | -, 10.4, 7.9; 4096 x 6144 6.9, 8.7, 14.0 | -, 9.7,
-// 11.1 | -, 12.2, 11.5 | -, 18.9, 11.9; 2048 x 16384 9.2, 9.4, 12.9 | -, 10.1, 12.5 | -, 12.2, 12.3 | -, 16.2, 12.7; 8192 x 2048 7.3, 7.5, 10.0 | -,
-// 8.4, 10.2 | -, 10.2, 10.7 | -, 14.1, 11.8; 14336 x 4096 15.6, 13.6, 18.0 | -, 14.3, 18.2 | -, 15.7, 18.6 | -, 19.6, 19.8.  The bytes of the weight
-// alone take 5.1 us at 2048 x 16384 and 9.0 at 14336 x 4096.
+// channels, at 8 | 32 | 64 tokens, weights of 500 MB in turn as the layers of a model take theirs: 2048 x 2048 2.8, 4.1, 7.3 | -, 5.1, 7.4 | -, 7.0, 7.7;
+// 4096 x 6144 7.0, 8.8, 14.6 | -, 9.8, 11.1 | -, 12.1, 11.4; 2048 x 16384 9.4, 10.0, 15.0 | -, 10.8, 13.4 | -, 13.3, 13.2; 8192 x 2048 7.4, 7.3, 10.8 | -,
+// 8.1, 10.0 | -, 9.8, 10.4; 14336 x 4096 -, 13.6, 20.9 | -, 13.9, 18.1 | -, 15.8, 18.9.  One weight again and again, out of L2, the order is the same
+// (2048 x 16384: 7.1, 6.9, 13.2 | -, 7.6, 11.2 | -, 10.5, 10.6).  At 128 tokens, out of L2: the second 10.4 to 19.6, pairs 7.9 to 19.8.  The bytes of the
+// weight alone take 5.1 us at 2048 x 16384 and 9.0 at 14336 x 4096.
 static bool few_tokens(int T, int K) { return T <= FEW && K <= 8192; }
 static bool streamed(int T) { return T <= 64; }
 

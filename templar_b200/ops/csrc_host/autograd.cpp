@@ -544,7 +544,7 @@ struct FeedForwardSaved8 : Function<FeedForwardSaved8> {
       dx = bf16(shape, dy2);
       gemm(dgu, w13, dx.view({-1, w13.size(1)}), false, true, 0, status);
     }
-    if (buffer13.defined() || ctx->needs_input_grad(1))
+    if (buffer13.defined() || ctx->needs_input_grad(1))        // the product takes bf16: the values are rounded to it, as _input_again does
       dw13 = weight_grad(buffer13, dgu, dequantize(xq, xscale, GROUP, {T, w13.size(1)}, xweight), w13, true, status);
     return {dx, dw13, dw2, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
