@@ -156,7 +156,8 @@ Tensor weight_grad(const Tensor& buffer, const Tensor& dy2, const Tensor& x2, co
   gemm(dy2, x2, dw, true, true, 0, status);
   return dw;
 }
-Tensor rows(const Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
+// t as a matrix.  The stride of a single row may be anything (and the matrix counts as contiguous); reshape gives it the row's length.
+Tensor rows(const Tensor& t) { return t.dim() == 2 && t.size(0) != 1 ? t : t.reshape({-1, t.size(-1)}); }
 // rows of a tensor whose last dimension is D; an integer division by zero would end the process
 ll count_rows(const Tensor& t, ll D) {
   TORCH_CHECK(D > 0, "rows of no elements");

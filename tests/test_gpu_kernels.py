@@ -843,3 +843,27 @@ def test_cross_entropy_keeps_exponentials_below_the_smallest_normal_number(V):
                                                  V, -100, 1, st.data_ptr(), native.stream_ptr()), "cross_entropy")
     assert int(st) == 0
     assert ((z.double() - want).abs() <= want.abs() * 2 ** -8 + 2 * 2.0 ** -149 * scale / T / sums).all()
+
+
+@pytest.mark.parametrize("stride", [1, 0, 771])
+def test_projections_of_a_single_row_whatever_its_stride(stride):
+    """The stride of a dimension of one element means nothing, and PyTorch takes such a matrix for contiguous whatever it is."""
+    D, Fd = 768, 1024
+    bf = lambda *s: torch.randn(*s, device=DEV).to(torch.bfloat16)  # noqa: E731
+    x, g, gf = bf(1, D), bf(1, D), bf(1, Fd)
+    w, w13, w2 = bf(Fd, D).requires_grad_(), bf(2 * Fd, D).mul_(D ** -0.5).requires_grad_(), bf(D, Fd).mul_(Fd ** -0.5).requires_grad_()
+    odd = lambda t: torch.as_strided(t, t.shape, (stride, 1))  # noqa: E731
+    assert odd(x).is_contiguous() and odd(x).stride(0) == stride
+
+    def run(f):
+        out = []
+        for fn, ws, dy in ((lambda t: OF.linear(t, w), (w,), gf), (lambda t: OF.feed_forward(t, w13, w2), (w13, w2), g)):
+            t = f(x.detach()).requires_grad_()
+            y = fn(t)
+            out += [y, *torch.autograd.grad(y, (t, *ws), f(dy))]
+        with torch.no_grad():
+            out.append(OF.feed_forward(f(x), w13, w2))
+        return out
+
+    for a, b in zip(run(odd), run(lambda t: t)):
+        assert torch.equal(a, b)

@@ -421,6 +421,19 @@ def test_feed_forward_of_several_tiles_a_pair(T, D, Fd):
     healthy()
 
 
+@pytest.mark.parametrize("stride", [1, 0, 259])
+def test_feed_forward_of_a_single_row_whatever_its_stride(stride):
+    D, Fd = 256, 384
+    w13, w2 = bf(2 * Fd, D, std=D ** -0.5, seed=1).requires_grad_(), bf(D, Fd, std=Fd ** -0.5, seed=2).requires_grad_()
+
+    def run(f):
+        x = f(bf(1, D)).requires_grad_()
+        y = ops.feed_forward_saved8(x, w13, w2)
+        return y, *torch.autograd.grad(y, (x, w13, w2), f(bf(1, D, seed=3)))
+    for a, b in zip(run(lambda t: torch.as_strided(t, t.shape, (stride, 1))), run(lambda t: t)):
+        assert a.equal(b)
+
+
 def test_feed_forward_with_the_norms_rows_a_frozen_part_and_one_row_that_is_not_finite():
     T, D, Fd = 200, 256, 512
     x, wn = bf(T, D).requires_grad_(), (1 + 0.1 * bf(D, seed=5).float()).to(torch.bfloat16)
