@@ -444,6 +444,17 @@ def linear_saved8(x, w, rows: QuantRows | None = None, weight=None, main_grad=No
     return _LinearSaved8.apply(x, w, main_grad, *_kept_input(x, rows, weight))
 
 
+def _sums32(a: torch.Tensor, b: torch.Tensor, b_mn: bool = False) -> torch.Tensor:
+    """``a b^T`` (``a b`` with ``b_mn``) with its sums left in fp32.  Operands that the own kernels do not take are copied to where they
+    do; rows of no whole 16-byte pieces are multiplied in fp32, since a library product of bf16 operands rounds its sums to bf16."""
+    if _native_rows(a, b) and OF._GEMM_BACKEND != "cublas":
+        if a.shape[1] % 8 == 0 and b.shape[1] % 8 == 0:
+            a, b = (t if t.stride(1) == 1 and t.stride(0) % 8 == 0 and OF._aligned(t) else OF._dense(t) for t in (a, b))
+            return OF.gemm(a, b, b_mn=b_mn, out_dtype=torch.float32)
+        OF._library_gemm_fallback(a, b)
+    return a.float() @ (b.float() if b_mn else b.float().t())
+
+
 class _FeedForwardSaved8(torch.autograd.Function):
     """``(silu(x w1^T) * (x w3^T)) w2^T``; kept: ``x`` and the projection [gate | up] in 8 bits, quantised from its fp32 sums.
     The backward pass forms the activation again from the kept projection."""
@@ -456,7 +467,7 @@ class _FeedForwardSaved8(torch.autograd.Function):
         ctx.fused = OF._feed_forward_fused(x2, w13, w2)
         gu = None
         if not ctx.fused:
-            gu = OF.gemm(x2, w13, out_dtype=torch.float32) if ctx.native else x2.float() @ w13.float().t()
+            gu = _sums32(x2, w13)
         if ctx.fused:                 # activation and codes in the projection's epilogue
             act = torch.empty(T, Fd, dtype=x.dtype, device=x.device)
             q, scale = _empty_halves(T, Fd, x.device)
@@ -488,7 +499,7 @@ class _FeedForwardSaved8(torch.autograd.Function):
         T, Fd = dy2.shape[0], w13.shape[0] // 2
         dact = None
         if not ctx.fused:
-            dact = OF.gemm(dy2, w2, b_mn=True, out_dtype=torch.float32) if ctx.native else dy2.float() @ w2.float()
+            dact = _sums32(dy2, w2, b_mn=True)
         if ctx.fused:
             dy2 = OF._dense(dy2)
             dgu = torch.empty(T, 2 * Fd, dtype=dy.dtype, device=dy.device)

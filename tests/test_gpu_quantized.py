@@ -421,6 +421,32 @@ def test_feed_forward_of_several_tiles_a_pair(T, D, Fd):
     healthy()
 
 
+# rows of the kernels' kind, rows off their 16-byte boundary, widths that make no 16-byte pieces
+@pytest.mark.parametrize("D,Fd,off", [(256, 72, 0), (256, 72, 1), (256, 128, 3), (100, 72, 0), (256, 100, 0), (129, 65, 0)])
+def test_feed_forward_keeps_codes_of_fp32_sums(D, Fd, off):
+    T = 200
+    x = bf(T * D + 8)[off:off + T * D].view(T, D).requires_grad_()
+    w13, w2 = bf(2 * Fd, D, std=D ** -0.5, seed=1).requires_grad_(), bf(D, Fd, std=Fd ** -0.5, seed=2).requires_grad_()
+    codes = []
+
+    def pack(t):
+        if t.dtype == torch.int8 and t.shape[1] >= 2 * Fd:
+            codes.append(t)
+        return t
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        y = ops.feed_forward_saved8(x, w13, w2)
+    g, u = (x.detach().double() @ w13.detach().double().t()).chunk(2, -1)
+    want = torch.cat([OQ._codes(t.float(), 64)[0] for t in (g, u)], dim=1)
+    # sums of D products in fp32 are 2^-24 sqrt(D) of a group's largest off or less, a code 127 times that from its neighbour: one in 5000 at
+    # D = 256; sums rounded to bf16 (2^-9) change one in five
+    assert len(codes) >= 1 and (codes[-1][:, :2 * Fd] != want).double().mean() < 1e-3
+    assert ((y.double() - (F.silu(g) * u).to(torch.bfloat16).double() @ w2.detach().double().t()).norm() <= 2.5e-3 * y.double().norm())
+    dy = bf(T, D, seed=3)
+    got = torch.autograd.grad(y, (x, w13, w2), dy)
+    for a, b in zip(got, ffn64(x, w13, w2, dy)[1:]):
+        assert (a.double() - b).norm() <= 3.3e-3 * b.norm()        # three roundings to bf16 of 0.0017 each, 0.0029
+
+
 @pytest.mark.parametrize("stride", [1, 0, 259])
 def test_feed_forward_of_a_single_row_whatever_its_stride(stride):
     D, Fd = 256, 384
