@@ -20,6 +20,7 @@
 // (torchtitan models/llama3/model/model.py:203-206, :244-262).
 #include "tcgen05.cuh"
 #include <cuda/std/type_traits>
+#include <limits.h>
 #include <stdlib.h>
 
 namespace {
@@ -39,6 +40,10 @@ struct AttnFwdParams {
   int B, S, H, KV;
   float scale_log2;       // softmax scale * log2(e)
   unsigned int* status;
+  // documents: row s of sequence b sees the keys max(starts[b * S + s], 0) .. s only; blocks[b * nQ + i] takes the least start in
+  // query block i of a row that sees anything (INT_MAX: none does), which the backward kernel walks by
+  const int* starts;
+  int* blocks;
 };
 
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
@@ -200,6 +205,27 @@ __device__ __forceinline__ float attn_row_max(uint32_t ts_lane, int r) {
   }
   return mx;
 }
+// The same with the columns from lo to hi alone (documents).
+__device__ __forceinline__ float attn_row_max_range(uint32_t (&v)[128], int lo, int hi) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < 128; ++e) {
+    if (e < lo || e > hi) v[e] = 0xff800000u;
+    mx = fmaxf(mx, __uint_as_float(v[e]));
+  }
+  return mx;
+}
+__device__ __forceinline__ float attn_row_max_range(uint32_t ts_lane, int lo, int hi) {
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t v[32];
+    tmem_ld32(ts_lane + c * 32, v);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) mx = fmaxf(mx, (c * 32 + e < lo || c * 32 + e > hi) ? -INFINITY : __uint_as_float(v[e]));
+  }
+  return mx;
+}
 // P = exp2(S * scale - m) written as packed bf16 to 64 columns; returns the row sum of P.
 __device__ __forceinline__ float attn_row_exp(const uint32_t (&v)[128], uint32_t tp_lane, float sl2, float m_used) {
   const unsigned long long sl2x2 = pack_f32x2(__float_as_uint(sl2), __float_as_uint(sl2));
@@ -224,9 +250,9 @@ __device__ __forceinline__ float attn_row_exp(const uint32_t (&v)[128], uint32_t
   return s0 + s1;
 }
 
-// the same over the first 64 columns of S
-template <bool DIAG>
-__device__ __forceinline__ float attn_row_exp(uint32_t ts_lane, int r, float sl2, float m_used) {
+// the same over the first 64 columns of S; MASK 1: the columns up to hi, 2: from lo to hi, are kept
+template <int MASK>
+__device__ __forceinline__ float attn_row_exp(uint32_t ts_lane, int lo, int hi, float sl2, float m_used) {
   const unsigned long long sl2x2 = pack_f32x2(__float_as_uint(sl2), __float_as_uint(sl2));
   const unsigned long long negm = pack_f32x2(__float_as_uint(-m_used), __float_as_uint(-m_used));
   unsigned long long sum = 0ull;                         // (0.f, 0.f)
@@ -239,9 +265,9 @@ __device__ __forceinline__ float attn_row_exp(uint32_t ts_lane, int r, float sl2
       float a0, a1;
       unpack_f32x2(fma_f32x2(pack_f32x2(v[2 * e], v[2 * e + 1]), sl2x2, negm), a0, a1);
       float p0 = exp2f(a0), p1 = exp2f(a1);
-      if (DIAG) {
-        if (c * 32 + 2 * e > r) p0 = 0.f;
-        if (c * 32 + 2 * e + 1 > r) p1 = 0.f;
+      if (MASK) {
+        if (c * 32 + 2 * e > hi || (MASK == 2 && c * 32 + 2 * e < lo)) p0 = 0.f;
+        if (c * 32 + 2 * e + 1 > hi || (MASK == 2 && c * 32 + 2 * e + 1 < lo)) p1 = 0.f;
       }
       sum = add_f32x2(sum, pack_f32x2(__float_as_uint(p0), __float_as_uint(p1)));
       __nv_bfloat162 hh = __floats2bfloat162_rn(p0, p1);
@@ -254,7 +280,7 @@ __device__ __forceinline__ float attn_row_exp(uint32_t ts_lane, int r, float sl2
   return s0 + s1;
 }
 
-template <int DH>
+template <int DH, bool DOCS>
 __global__ void __launch_bounds__(FWD_THREADS, 2)
 attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
   constexpr int TILE_BYTES = tile_bytes<DH>();
@@ -263,6 +289,7 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
   __shared__ __align__(8) uint64_t bar_q, bar_k_full, bar_k_empty, bar_v_full, bar_v_empty, bar_s_full, bar_s_read, bar_p_full, bar_o_full;
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
+  __shared__ int s_least[4];                               // documents: the least start of each softmax warp's rows
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int nQ = (p.S + BQ - 1) / BQ;
@@ -271,7 +298,7 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
   const int qi = nQ - 1 - (int)(blockIdx.x / hb);
   const int h = (int)(blockIdx.x % hb) % p.H, b = (int)(blockIdx.x % hb) / p.H;
   const int g = h / (p.H / p.KV);
-  const int nb = qi + 1;                                   // causal: kv blocks 0..qi
+  int j0 = 0, nb = qi + 1;                                 // kv blocks j0 .. j0 + nb - 1; causal: 0 .. qi
   const int row0 = qi * BQ;                                // position of the first query row; rows past S read as zeros
   const int qcol = h * DH, kcol = (p.H + g) * DH, vcol = (p.H + p.KV + g) * DH;
   volatile int* abort_flag = &s_abort;
@@ -295,6 +322,22 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
   tcgen05_fence_after();
   grid_wait();
   grid_release();
+  int start = 0;                                           // first key of this softmax thread's row
+  if constexpr (DOCS) {
+    // documents: from the block of the least start of a row that sees anything; a row past the end or without a key asks for none
+    if (warp >= 2) {
+      const int r = (warp & 3) * 32 + lane, s = row0 + r;
+      start = s < p.S ? max(p.starts[(long long)b * p.S + s], 0) : INT_MAX;
+      if (start > s) start = INT_MAX;
+      const int least = __reduce_min_sync(0xffffffffu, start);
+      if (lane == 0) s_least[warp - 2] = least;
+    }
+    __syncthreads();
+    const int least = min(min(s_least[0], s_least[1]), min(s_least[2], s_least[3]));
+    j0 = least == INT_MAX ? 0 : least / BKV;
+    nb = least == INT_MAX ? 0 : qi - j0 + 1;
+    if (p.blocks && h == 0 && threadIdx.x == 0) p.blocks[(long long)b * nQ + qi] = least;
+  }
   const uint32_t tmem_base = s_tmem_base;
   // S columns 0..127, O from column 128.  P lies over S at DH = 128; at 64 it has the 64 columns that O leaves, so that the
   // next block's S is computed as soon as the softmax warps hold this one's in registers (AHEAD).
@@ -305,7 +348,8 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
   if (warp == 0) {
     {
       const bool leader = elect_one();
-      if (leader) {
+      const bool any = !DOCS || nb > 0;
+      if (leader && any) {
         mbar_expect_tx(smem_u32(&bar_q), TILE_BYTES);
         load_tile<DH>(sQ, &p.tmQKV, smem_u32(&bar_q), qcol, row0, b);
       }
@@ -313,7 +357,7 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
       int n_k = 0, n_v = 0;                                // tiles asked for
       for (int j = 0; j < nb && ok; ++j) {
         const uint32_t ph = j & 1;
-        const int krow = j * BKV;
+        const int krow = (j0 + j) * BKV;
         if (!(ok = mbar_wait_warp(smem_u32(&bar_k_empty), ph ^ 1, abort_flag))) break;
         if (leader) {
           mbar_expect_tx(smem_u32(&bar_k_full), TILE_BYTES);
@@ -329,7 +373,7 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
       }
       if (leader) {
         Drain drain;                                         // no load may land after the CTA has retired: a role may have given up
-        drain.wait(smem_u32(&bar_q), 0);
+        if (any) drain.wait(smem_u32(&bar_q), 0);
         if (n_k) drain.wait(smem_u32(&bar_k_full), (uint32_t)((n_k - 1) & 1));
         if (n_v) drain.wait(smem_u32(&bar_v_full), (uint32_t)((n_v - 1) & 1));
       }
@@ -353,7 +397,7 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
         }
         return true;
       };
-      bool ok = mbar_wait_warp(smem_u32(&bar_q), 0, abort_flag);
+      bool ok = (!DOCS || nb > 0) && mbar_wait_warp(smem_u32(&bar_q), 0, abort_flag);
       if (AHEAD && ok) ok = issue_s(0);
       for (int j = 0; j < nb && ok; ++j) {
         const uint32_t ph = j & 1;
@@ -386,7 +430,15 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tcgen05_fence_after();
-      const bool diag = j == qi;
+      const bool diag = j0 + j == qi;
+      // documents: the columns of this block that the row sees; without a mask where all rows of the warp see all of them
+      int lo = 0, hi = r;
+      bool masked = diag;
+      if constexpr (DOCS) {
+        lo = start == INT_MAX ? BKV : start - (j0 + j) * BKV;        // nothing: behind the last column
+        hi = diag ? r : BKV - 1;
+        masked = diag || __any_sync(0xffffffffu, lo > 0);
+      }
       uint32_t sv[AHEAD ? 128 : 1];                        // AHEAD: the row, loaded once
       float mx;
       if constexpr (AHEAD) {
@@ -394,9 +446,11 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_s_read));
-        mx = diag ? attn_row_max<true>(sv, r) : attn_row_max<false>(sv, r);
+        if constexpr (DOCS) mx = masked ? attn_row_max_range(sv, lo, hi) : attn_row_max<false>(sv, r);
+        else mx = diag ? attn_row_max<true>(sv, r) : attn_row_max<false>(sv, r);
       } else {
-        mx = diag ? attn_row_max<true>(tS + lane_off, r) : attn_row_max<false>(tS + lane_off, r);
+        if constexpr (DOCS) mx = masked ? attn_row_max_range(tS + lane_off, lo, hi) : attn_row_max<false>(tS + lane_off, r);
+        else mx = diag ? attn_row_max<true>(tS + lane_off, r) : attn_row_max<false>(tS + lane_off, r);
       }
       if (AHEAD && j > 0) {                // O and the P columns: the product of block j-1 has finished with them
         ok = mbar_wait(smem_u32(&bar_v_empty), (uint32_t)((j - 1) & 1), abort_flag);
@@ -421,18 +475,21 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
           }
         }
       }
-      if constexpr (AHEAD) l += attn_row_exp(sv, tP + lane_off, p.scale_log2, m_used);
-      else l += diag ? attn_row_exp<true>(tS + lane_off, r, p.scale_log2, m_used) : attn_row_exp<false>(tS + lane_off, r, p.scale_log2, m_used);
+      // documents: a row that has seen no key yet has no maximum, and all its scores here are masked
+      const float m_ref = DOCS && m_used == -INFINITY ? 0.f : m_used;
+      if constexpr (AHEAD) l += attn_row_exp(sv, tP + lane_off, p.scale_log2, m_ref);
+      else l += masked ? attn_row_exp<DOCS ? 2 : 1>(tS + lane_off, lo, hi, p.scale_log2, m_ref) : attn_row_exp<0>(tS + lane_off, lo, hi, p.scale_log2, m_ref);
       tmem_wait_st();
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bar_p_full));
     }
     // epilogue: O / l -> bf16 -> swizzled staging (the Q tile is no longer read) -> TMA store
-    if (ok) ok = mbar_wait(smem_u32(&bar_o_full), 0, abort_flag);
+    if (ok && (!DOCS || nb > 0)) ok = mbar_wait(smem_u32(&bar_o_full), 0, abort_flag);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tcgen05_fence_after();
+      const bool empty = DOCS && start == INT_MAX;           // a row that sees nothing is zero
       const float inv_l = 1.f / l;
       const uint32_t stage = sQ + (uint32_t)quad * (32u * DH * 2u);
       const int orow = row0 + quad * 32;
@@ -441,14 +498,19 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
       for (int c = 0; c < DH / 32; ++c) {
         uint32_t v[32];
         tmem_ld32(tO + c * 32 + lane_off, v);
+        if (DOCS && empty) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0u;
+        }
+        const float by = empty ? 1.f : inv_l;
         const uint32_t rowaddr = stage + (uint32_t)(c >> 1) * 4096u + (uint32_t)lane * 128u;
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
           uint32_t pw[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            __nv_bfloat162 hh = __floats2bfloat162_rn(__uint_as_float(v[8 * q4 + 2 * e]) * inv_l,
-                                                      __uint_as_float(v[8 * q4 + 2 * e + 1]) * inv_l);
+            __nv_bfloat162 hh = __floats2bfloat162_rn(__uint_as_float(v[8 * q4 + 2 * e]) * by,
+                                                      __uint_as_float(v[8 * q4 + 2 * e + 1]) * by);
             pw[e] = *reinterpret_cast<uint32_t*>(&hh);
           }
           const uint32_t jj = (uint32_t)((c & 1) * 4 + q4);
@@ -464,7 +526,8 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       }
-      if (p.lse && row0 + r < p.S) p.lse[((long long)b * p.H + h) * p.S + row0 + r] = (m_used + log2f(l)) * 0.6931471805599453f;
+      // an infinite sum makes the backward pass's weights of the row zero
+      if (p.lse && row0 + r < p.S) p.lse[((long long)b * p.H + h) * p.S + row0 + r] = empty ? INFINITY : (m_used + log2f(l)) * 0.6931471805599453f;
     }
   }
   __syncwarp();
@@ -480,19 +543,20 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
 }  // namespace
 
 namespace {
-template <int DH>
+template <int DH, bool DOCS>
 int launch_fwd(const void* qkv, void* out, float* lse, int B, int S, int H, int KV, long long ld_qkv, long long ld_o,
-               float scale, unsigned int* status, cudaStream_t st) {
+               float scale, unsigned int* status, cudaStream_t st, const int* starts = nullptr, int* blocks = nullptr) {
   AttnFwdParams p = {};
   if (!make_map3(&p.tmQKV, qkv, (long long)(H + 2 * KV) * DH, S, B, ld_qkv, 64, 128)) return -202;
   if (!make_map3(&p.tmO, out, (long long)H * DH, S, B, ld_o, 64, 32)) return -203;
   p.lse = lse; p.B = B; p.S = S; p.H = H; p.KV = KV;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = status;
-  cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, fwd_smem<DH>());
+  p.starts = starts; p.blocks = blocks;
+  cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<DH, DOCS>, cudaFuncAttributeMaxDynamicSharedMemorySize, fwd_smem<DH>());
   if (e != cudaSuccess) return (int)e;
   const unsigned grid = (unsigned)(((S + BQ - 1) / BQ) * H * B);
-  return (int)launch_pdl(attn_fwd_kernel<DH>, grid, FWD_THREADS, fwd_smem<DH>(), st, p);
+  return (int)launch_pdl(attn_fwd_kernel<DH, DOCS>, grid, FWD_THREADS, fwd_smem<DH>(), st, p);
 }
 }  // namespace
 
@@ -503,9 +567,22 @@ TPLR_API int tplr_attention_fwd(const void* qkv, void* out, float* lse, int B, i
   TPLR_ENTER();
   if (B <= 0 || S <= 0) return 0;
   if (H % KV || (ld_qkv % 8) || (ld_o % 8) || ((uintptr_t)qkv & 15) || ((uintptr_t)out & 15)) return -201;
-  if (head_dim == 128) return launch_fwd<128>(qkv, out, lse, B, S, H, KV, ld_qkv, ld_o, scale, status, (cudaStream_t)stream);
-  if (head_dim == 64) return launch_fwd<64>(qkv, out, lse, B, S, H, KV, ld_qkv, ld_o, scale, status, (cudaStream_t)stream);
+  if (head_dim == 128) return launch_fwd<128, false>(qkv, out, lse, B, S, H, KV, ld_qkv, ld_o, scale, status, (cudaStream_t)stream);
+  if (head_dim == 64) return launch_fwd<64, false>(qkv, out, lse, B, S, H, KV, ld_qkv, ld_o, scale, status, (cudaStream_t)stream);
   return -201;
+}
+
+// tplr_attention_fwd within documents: row s of sequence b sees the keys max(starts[b * S + s], 0) .. s; one whose start lies behind it
+// sees nothing, and its output is zero.  starts: [B, S] int32, any values.  blocks: [B, ceil(S / 128)] int32 for the backward
+// pass, or null.
+TPLR_API int tplr_attention_docs_fwd(const void* qkv, const int* starts, void* out, float* lse, int* blocks, int B, int S, int H, int KV,
+                                     int head_dim, long long ld_qkv, long long ld_o, float scale, unsigned int* status, void* stream) {
+  TPLR_ENTER();
+  if (B <= 0 || S <= 0) return 0;
+  if (KV <= 0 || H % KV || (ld_qkv % 8) || (ld_o % 8) || ((uintptr_t)qkv & 15) || ((uintptr_t)out & 15) || !starts) return -201;
+  auto run = head_dim == 128 ? launch_fwd<128, true> : launch_fwd<64, true>;
+  if (head_dim != 128 && head_dim != 64) return -201;
+  return run(qkv, out, lse, B, S, H, KV, ld_qkv, ld_o, scale, status, (cudaStream_t)stream, starts, blocks);
 }
 
 // ------------------------------------------------------------------------------------------ //
@@ -553,6 +630,8 @@ struct AttnBwdParams {
   // the gradient is wanted with respect to the un-rotated projection: dK is rotated back in the epilogue
   const float* rope_cos;
   const float* rope_sin;
+  const int* starts;    // documents: as in the forward kernel, which left `blocks`
+  const int* blocks;
 };
 
 __device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
@@ -564,7 +643,7 @@ __device__ __forceinline__ void tma_reduce_add_3d(const CUtensorMap* map, uint32
                ::"l"(map), "r"(src), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
-template <int DH>
+template <int DH, bool DOCS>
 __global__ void __launch_bounds__(bwd_threads<DH>(), 1)
 attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
   constexpr int TILE_BYTES = tile_bytes<DH>();
@@ -574,6 +653,7 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
       bar_p_ready, bar_ds_ready, bar_dq_full, bar_dq_free;
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
+  __shared__ int s_last;                                   // documents: the last query block that sees any key of this block
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int nQ = (p.S + BQ - 1) / BQ;
@@ -583,14 +663,14 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
   const int g = (int)(blockIdx.x % gb) / p.split % p.KV, b = (int)(blockIdx.x % gb) / p.split / p.KV;
   const int heads = p.H / p.KV / p.split;                  // query heads of this CTA
   const int h0 = (g * p.split + sub) * heads;
-  const int n_i = nQ - j;                                  // query blocks j..nQ-1
-  const int n_it = heads * n_i;
+  int n_i = nQ - j, n_it = heads * n_i;                    // query blocks j .. j + n_i - 1; causal: to the last
   const int kvrow0 = j * BKV;                              // position of the first key row; rows past S read as zeros
   const int kcol = (p.H + g) * DH, vcol = (p.H + p.KV + g) * DH;
   volatile int* abort_flag = &s_abort;
 
   if (threadIdx.x == 0) {
     s_abort = 0;
+    s_last = -1;
     mbar_init(smem_u32(&bar_kv), 1);
     for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&bar_q_full[s]), 1); mbar_init(smem_u32(&bar_q_empty[s]), 1); }
     mbar_init(smem_u32(&bar_do_full), 1); mbar_init(smem_u32(&bar_do_empty), 1);
@@ -609,6 +689,17 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
   tcgen05_fence_after();
   grid_wait();
   grid_release();
+  if constexpr (DOCS) {
+    // a block in between whose rows begin behind this one is walked with all its weights masked: starts that grow with the
+    // row, as documents' do, have none
+    int last = -1;
+    for (int i = j + (int)threadIdx.x; i < nQ; i += bwd_threads<DH>())
+      if (p.blocks[(long long)b * nQ + i] < kvrow0 + BKV) last = i;
+    if (last >= 0) atomicMax(&s_last, last);
+    __syncthreads();
+    n_i = max(s_last - j + 1, 0);
+    n_it = heads * n_i;
+  }
   const uint32_t tmem_base = s_tmem_base;
   // dQ of a step lies over its dP at DH = 128; at 64 it has columns of its own
   const uint32_t tS = tmem_base, tdP = tmem_base + 128, tdV = tmem_base + 256, tdK = tmem_base + 256 + DH, tdQ = DH == 64 ? tmem_base + 384 : tdP;
@@ -677,7 +768,7 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
         for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(tdP, kdO, TPLR_KOFF(kk), kV, TPLR_KOFF(kk), id_kk, kk > 0 ? 1u : 0u);
         umma_commit(smem_u32(&bar_dp_full));
       };
-      bool ok = mbar_wait_warp(smem_u32(&bar_kv), 0, abort_flag);
+      bool ok = (!DOCS || n_it > 0) && mbar_wait_warp(smem_u32(&bar_kv), 0, abort_flag);
       if (ok) ok = mbar_wait_warp(smem_u32(&bar_q_full[0]), 0, abort_flag);
       if (ok) { tcgen05_fence_after(); issue_s(0); }
       if (ok) ok = mbar_wait_warp(smem_u32(&bar_do_full), 0, abort_flag);
@@ -773,12 +864,13 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
     const uint32_t prow = sP + (uint32_t)ch * (PT_BYTES / 2) + (uint32_t)r * 128u;
     const uint32_t drow = sdS + (uint32_t)ch * (PT_BYTES / 2) + (uint32_t)r * 128u;
     // the row statistics of step t; a query row past the end of the sequence has no weight: lse = +inf makes its P zero
-    auto stats = [&](int t, float& lse2, float& dl) {
+    auto stats = [&](int t, float& lse2, float& dl, int& st) {
       const int h = h0 + t / n_i, row = (j + t % n_i) * BQ + r;
       const long long at = ((long long)b * p.H + h) * p.S + row;
       const bool live = row < p.S;
       lse2 = live ? p.lse[at] : INFINITY;
       dl = live ? p.delta[at] : 0.f;
+      if (DOCS) st = live ? max(p.starts[(long long)b * p.S + row], 0) : 0;
     };
     // DH = 128: dQ of step tt (fp32 in tensor memory) into the global fp32 dQ with TMA reduce-add: one group of copies for each box
     auto drain = [&](int tt) -> bool {
@@ -809,21 +901,23 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
       }
       return true;
     };
-    float lse_n, dl_n;
-    stats(0, lse_n, dl_n);
+    float lse_n = 0.f, dl_n = 0.f;
+    int st_n = 0;
+    if (!DOCS || n_it > 0) stats(0, lse_n, dl_n, st_n);
     bool ok = true;
     for (int t = 0; t < n_it && ok; ++t) {
       const int i = j + t % n_i;
       const float lse2 = lse_n * 1.4426950408889634f, dls = dl_n * p.scale;
-      if (t + 1 < n_it) stats(t + 1, lse_n, dl_n);           // in flight during this step
+      const int lo = DOCS ? st_n - kvrow0 : 0;               // documents: first column of this block that the row sees
+      if (t + 1 < n_it) stats(t + 1, lse_n, dl_n, st_n);     // in flight during this step
       ok = mbar_wait(smem_u32(&bar_s_full), t & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tcgen05_fence_after();
       // P of this warp's 64 columns, kept in fp32 for dS; the diagonal block runs the variant with the causal mask
       float pv[64];
-      auto exp_part = [&](auto DIAG) {
-        constexpr bool kDiag = decltype(DIAG)::value;
+      auto exp_part = [&](auto DIAG, auto LOW) {
+        constexpr bool kDiag = decltype(DIAG)::value, kLow = decltype(LOW)::value;
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
           uint32_t sv[32];
@@ -832,11 +926,16 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
           for (int e = 0; e < 32; ++e) {
             float x = exp2f(fmaf(__uint_as_float(sv[e]), p.scale_log2, -lse2));
             if (kDiag && ch * 64 + cc * 32 + e > r) x = 0.f;
+            if (kLow && ch * 64 + cc * 32 + e < lo) x = 0.f;
             pv[cc * 32 + e] = x;
           }
         }
       };
-      if (i == j) exp_part(cuda::std::true_type{}); else exp_part(cuda::std::false_type{});
+      using yes = cuda::std::true_type;
+      using no = cuda::std::false_type;
+      if (DOCS && __any_sync(0xffffffffu, lo > 0)) { if (i == j) exp_part(yes{}, yes{}); else exp_part(no{}, yes{}); }
+      else if (i == j) exp_part(yes{}, no{});
+      else exp_part(no{}, no{});
       if (t > 0) {
         if constexpr (DH == 128) {
           // dQ of the step before: its products ran while this step's exponentials were taken.  Its last commit covers every
@@ -916,6 +1015,10 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
           __syncwarp();
           uint32_t v[32];
           tmem_ld32((acc ? tdK : tdV) + col + lane_off, v);
+          if (DOCS && n_it == 0) {                       // keys that no row sees
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = 0u;
+          }
           const uint32_t rowaddr = buf + (uint32_t)lane * 128u;
 #pragma unroll
           for (int q8 = 0; q8 < 8; ++q8)
@@ -942,6 +1045,10 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
           for (int hf = 0; hf < 2; ++hf) {
             uint32_t v[32];
             tmem_ld32(tacc + col + hf * 32 + lane_off, v);
+            if (DOCS && n_it == 0) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = 0u;
+            }
             if (acc == 1 && p.rope_cos) {          // dK back through the rotation of this key row: the opposite angle
               const long long tb = (long long)min(orow0 + lane, p.S - 1) * (DH / 2) + (col + hf * 32) / 2;
               const float4* cp = reinterpret_cast<const float4*>(p.rope_cos + tb);
@@ -1440,12 +1547,13 @@ extern "C" int tplr_rope(void* buf, const float* cosb, const float* sinb, long l
                          long long row_stride, int inverse, void* stream);
 
 static int bwd_split(int B, int S, int H, int KV, int head_dim);
+static int bwd_split_walk(int B, int S, int H, int KV);
 
 namespace {
-template <int HD>
+template <int HD, bool DOCS>
 int launch_bwd(const void* qkv, const void* out, const void* dout, const float* lse, float* delta, float* dq32, void* dqkv, int B,
                int S, int H, int KV, long long ld_qkv, long long ld_o, float scale, const float* cosb, const float* sinb,
-               unsigned int* status, cudaStream_t st, bool delta_ready) {
+               unsigned int* status, cudaStream_t st, bool delta_ready, const int* starts = nullptr, const int* blocks = nullptr) {
   const long long tokens = (long long)B * S;
   const int C = (H + 2 * KV) * HD;
   if (!delta_ready) {
@@ -1453,7 +1561,7 @@ int launch_bwd(const void* qkv, const void* out, const void* dout, const float* 
     attn_delta_kernel<HD><<<(unsigned)((tokens * H + per_cta - 1) / per_cta), 256, 0, st>>>(
         (const __nv_bfloat16*)out, (const __nv_bfloat16*)dout, delta, tokens, S, H, ld_o);
   }
-  if (HD == 128 && S % 128 == 0 && g_bwd_variant == 2) {
+  if (!DOCS && HD == 128 && S % 128 == 0 && g_bwd_variant == 2) {
     // pipelined kernel: dq32 is used as the transposed scratch [B*H*128, S]
     AttnBwd2Params p = {};
     if (!make_map(&p.tmKV, qkv, C, tokens, ld_qkv, 64, 128)) return -202;
@@ -1474,7 +1582,7 @@ int launch_bwd(const void* qkv, const void* out, const void* dout, const float* 
   AttnBwdParams p = {};
   if (!make_map3(&p.tmQKV, qkv, C, S, B, ld_qkv, 64, 128)) return -202;
   if (!make_map3(&p.tmDO, dout, (long long)H * HD, S, B, (long long)H * HD, 64, 128)) return -203;
-  p.split = bwd_split(B, S, H, KV, HD);
+  p.split = DOCS ? bwd_split_walk(B, S, H, KV) : bwd_split(B, S, H, KV, HD);
   float* part = dq32 + tokens * H * HD;                        // the parts of dK and dV lie behind dQ
   const int kv_cols = p.split > 1 ? 2 * KV * HD : 0;
   if (!make_map3(&p.tmDQ, dq32, (long long)H * HD, S, B, (long long)H * HD, 32, 32, true)) return -204;
@@ -1483,9 +1591,10 @@ int launch_bwd(const void* qkv, const void* out, const void* dout, const float* 
   p.lse = lse; p.delta = delta; p.B = B; p.S = S; p.H = H; p.KV = KV;
   p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   p.rope_cos = cosb; p.rope_sin = sinb;
-  cudaError_t e = cudaFuncSetAttribute(attn_bwd_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, bwd_smem<HD>());
+  p.starts = starts; p.blocks = blocks;
+  cudaError_t e = cudaFuncSetAttribute(attn_bwd_kernel<HD, DOCS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bwd_smem<HD>());
   if (e != cudaSuccess) return (int)e;
-  e = launch_pdl(attn_bwd_kernel<HD>, (unsigned)(((S + BKV - 1) / BKV) * KV * B * p.split), bwd_threads<HD>(), bwd_smem<HD>(), st, p);
+  e = launch_pdl(attn_bwd_kernel<HD, DOCS>, (unsigned)(((S + BKV - 1) / BKV) * KV * B * p.split), bwd_threads<HD>(), bwd_smem<HD>(), st, p);
   if (e != cudaSuccess) return (int)e;
   auto cast = kv_cols ? attn_dq_cast_kernel<HD, true> : attn_dq_cast_kernel<HD, false>;
   return (int)launch_pdl(cast, tplr_sm_count() * 8, 256, 0, st, dq32, part, p.split, (__nv_bfloat16*)dqkv, tokens, H * HD, kv_cols, (H + KV) * HD, ld_qkv, cosb, sinb, S);
@@ -1499,7 +1608,10 @@ int launch_bwd(const void* qkv, const void* out, const void* dout, const float* 
 // (64 CTAs), 46 us in four parts (256 CTAs; the pass that adds them 2 us more); B 6, S 640 (240 CTAs) 103 us whole, 113 us in
 // two parts; B 4, S 1024 (256 CTAs) 151 us whole, 163 us in two.
 static int bwd_split(int B, int S, int H, int KV, int head_dim) {
-  if (KV <= 0 || H % KV || (head_dim == 128 && S % 128 == 0 && g_bwd_variant == 2)) return 1;
+  return head_dim == 128 && S % 128 == 0 && g_bwd_variant == 2 ? 1 : bwd_split_walk(B, S, H, KV);
+}
+static int bwd_split_walk(int B, int S, int H, int KV) {
+  if (KV <= 0 || H % KV) return 1;
   const int group = H / KV;
   const long long n = (S + BKV - 1) / BKV, ctas = n * KV * B;
   int split = 1;
@@ -1523,9 +1635,9 @@ static int attention_bwd_impl(const void* qkv, const void* out, const void* dout
   if ((head_dim != 128 && head_dim != 64) || H % KV || (ld_qkv % 8) || (ld_o % 8) || ((uintptr_t)qkv & 15) ||
       ((uintptr_t)dqkv & 15) || ((uintptr_t)dout & 15) || ((uintptr_t)out & 7) || ((uintptr_t)dq32 & 15))
     return -201;
-  auto run = head_dim == 128 ? launch_bwd<128> : launch_bwd<64>;
+  auto run = head_dim == 128 ? launch_bwd<128, false> : launch_bwd<64, false>;
   return run(qkv, out, dout, lse, delta, dq32, dqkv, B, S, H, KV, ld_qkv, ld_o, scale, cosb, sinb, status, (cudaStream_t)stream,
-             delta_ready);
+             delta_ready, nullptr, nullptr);
 }
 
 TPLR_API int tplr_attention_bwd(const void* qkv, const void* out, const void* dout, const float* lse, float* delta,
@@ -1560,3 +1672,22 @@ TPLR_API int tplr_attention_bwd_unrope_delta(const void* qkv, const void* out, c
                             true);
 }
 
+// Fp32 elements per token of the scratch that tplr_attention_docs_bwd needs, laid out as tplr_attention_bwd's.
+TPLR_API int tplr_attention_docs_bwd_scratch_cols(int B, int S, int H, int KV, int head_dim) {
+  const int split = bwd_split_walk(B, S, H, KV);
+  return (H + (split > 1 ? 2 * KV * split : 0)) * head_dim;
+}
+
+// Gradient of tplr_attention_docs_fwd, whose starts and blocks it takes; otherwise as tplr_attention_bwd.
+TPLR_API int tplr_attention_docs_bwd(const void* qkv, const int* starts, const int* blocks, const void* out, const void* dout,
+                                     const float* lse, float* delta, float* dq32, void* dqkv, int B, int S, int H, int KV, int head_dim,
+                                     long long ld_qkv, long long ld_o, float scale, unsigned int* status, void* stream) {
+  TPLR_ENTER();
+  if (B <= 0 || S <= 0) return 0;
+  if ((head_dim != 128 && head_dim != 64) || KV <= 0 || H % KV || (ld_qkv % 8) || (ld_o % 8) || ((uintptr_t)qkv & 15) || !starts || !blocks ||
+      ((uintptr_t)dqkv & 15) || ((uintptr_t)dout & 15) || ((uintptr_t)out & 7) || ((uintptr_t)dq32 & 15))
+    return -201;
+  auto run = head_dim == 128 ? launch_bwd<128, true> : launch_bwd<64, true>;
+  return run(qkv, out, dout, lse, delta, dq32, dqkv, B, S, H, KV, ld_qkv, ld_o, scale, nullptr, nullptr, status, (cudaStream_t)stream,
+             false, starts, blocks);
+}

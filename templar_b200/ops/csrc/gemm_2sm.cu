@@ -43,7 +43,7 @@ constexpr int MAX_STAGES = 8;                      // narrower tiles have smalle
 static_assert(4 * 8192 <= STAGE_BYTES, "the freed stage holds four warps' second pair");
 // Warps that drain the accumulator: one a quadrant of tensor memory, or two where the epilogue is as long as the main loop of a short K,
 // so that one has instructions while the other waits.  What they stage beyond 32 KB takes a stage of the ring.
-constexpr int epi_warps(int epi) { return epi == 7 || epi == 8 || epi == 10 ? 8 : 4; }
+constexpr int epi_warps(int epi) { return epi == 7 || epi == 8 || epi == 10 || epi >= 12 ? 8 : 4; }
 constexpr int num_threads(int epi) { return 64 + 32 * epi_warps(epi); }
 constexpr int ring_stages(int epi) { return epi == 5 || epi == 10 ? EPI5_STAGES : STAGES; }
 constexpr int MAX_RANKS = 8;
@@ -95,6 +95,12 @@ struct Gemm2Params {
   // q8_scale[g * q8_ld + m], gate groups first
   float* q8_scale;
   long long q8_ld;
+  // softmax over the columns in pieces (EPI 12, 13): a piece is half a tile's columns, sm_parts pieces a row; (largest logit, sum of
+  // exp(logit - it)) goes to sm_stats[row * sm_parts + piece], the logit of the row's label to sm_target[row]
+  const long long* sm_labels;
+  float2* sm_stats;
+  float* sm_target;
+  int sm_parts;
   int world, rank;
   unsigned int epoch;
   // gather
@@ -933,11 +939,81 @@ __device__ __forceinline__ bool epilogue_swiglu_bwd_q8(const Gemm2Params& p, uin
   return true;
 }
 
+// Epilogue of the output projection with the softmax over its columns (EPI 12, 13): a lane has a row, so its piece's largest logit
+// and sum need no exchange; the accumulator is read twice, once for each.  EPI 12 stores exp(logit - largest of the piece) as bf16,
+// which is off by a rounding of itself whatever the logit's size (the logit in bf16 would be off by 2^-9 of the logit,
+// and the weight by as much in its exponent); EPI 13 stores the numbers of the pieces alone.  Columns from N on count for nothing.
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+template <bool STORE>
+__device__ __forceinline__ void epilogue_softmax(const Gemm2Params& p, uint32_t tmem_acc, int quad, int turn, int lane, int m0, int n0,
+                                                 uint32_t buf, uint32_t& n_boxes) {
+  const int half = p.tile_n / 2;                     // columns of a piece
+  const int row0 = m0 + quad * 32, c0 = n0 + turn * half;
+  if (row0 >= p.M || c0 >= p.N) return;              // warp-uniform
+  const uint32_t acc = tmem_acc + turn * half + ((uint32_t)(quad * 32) << 16);
+  const int width = min(half, p.N - c0);
+  const bool live = row0 + lane < p.M;
+  const long long label = live ? p.sm_labels[row0 + lane] - c0 : -1;
+  const int mine = label >= 0 && label < width ? (int)label : -1;
+  float top = -INFINITY, target = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < width; c += 32) {
+    uint32_t r[32];
+    tmem_ld32(acc + c, r);
+    if (c + 32 > width) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) if (c + e >= width) r[e] = 0xff800000u;
+    }
+    if (__any_sync(0xffffffffu, (mine >> 5) == (c >> 5))) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) if (c + e == mine) target = __uint_as_float(r[e]);
+    }
+    float top2 = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) { top = fmaxf(top, __uint_as_float(r[e])); top2 = fmaxf(top2, __uint_as_float(r[e + 1])); }
+    top = fmaxf(top, top2);
+  }
+  constexpr float LOG2E = 1.4426950408889634f;
+  const float neg = top == -INFINITY ? 0.f : -top * LOG2E;
+  float sum = 0.f, sum2 = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < width; c += 64) {
+    if (STORE) {
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // one box a warp: the other warp of the quadrant works meanwhile
+      __syncwarp();
+    }
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      uint32_t r[32];
+      float v[32];
+      tmem_ld32(acc + c + hh * 32, r);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) v[e] = ex2(fmaf(__uint_as_float(r[e]), LOG2E, neg));
+      if (c + hh * 32 + 32 > width) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) if (c + hh * 32 + e >= width) v[e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) { sum += v[e]; sum2 += v[e + 1]; }
+      if (STORE) box_half(buf, lane, hh, v);
+    }
+    if (STORE) box_store(&p.tmC, buf, lane, n_boxes, c0 + c, row0);
+  }
+  if (live) {
+    p.sm_stats[(long long)(row0 + lane) * p.sm_parts + c0 / half] = make_float2(top, sum + sum2);
+    if (mine >= 0) p.sm_target[row0 + lane] = target;
+  }
+}
+
 // EPI: 0 store bf16, 1 fp32 accumulate (C += acc), 2 store fp32, 3 fused SwiGLU of a packed [w1; w3] projection,
 // 4 store bf16 with the rotary embedding applied to the leading columns, 5 backward of the SwiGLU on the data gradient
 // of the down projection, 6 data gradient of the attention output projection with the attention backward's delta term,
 // 7 / 8 product of 8-bit rows stored as bf16 / fp32, 9 as 3 with the projection kept in 8 bits, 10 as 5 from it,
-// 11 product of 8-bit rows, int32 sums of a part of K to a plane of its own
+// 11 product of 8-bit rows, int32 sums of a part of K to a plane of its own, 12 softmax over the columns in pieces, 13 their numbers alone
 template <bool A_MN, bool B_MN, int EPI>
 __global__ void __launch_bounds__(num_threads(EPI), 1)
 gemm2_kernel(const __grid_constant__ Gemm2Params p) {
@@ -1141,6 +1217,7 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
         else if (EPI == 4 && p.rope_dh == 64 && p.rope_cols % 64 == 0)
           epilogue_rope<64>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
         else if (EPI == 11) epilogue_tma<2>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes, w.t % p.k_splits);
+        else if (EPI >= 12) epilogue_softmax<EPI == 12>(p, tmem_acc, quad, turn, lane, m0, n0, sEpi + (uint32_t)(warp - 2) * 4096u, n_boxes);
         else if (I8)       epilogue_q8<EPI == 8>(p, tmem_acc, quad, turn, lane, m0, n0, sEpi + (uint32_t)(warp - 2) * 4096u, n_boxes);
         else if (p.c_tma)  epilogue_tma<EPI>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes, w.t % p.k_splits);
         else               epilogue_direct<EPI>(p, tmem_acc, quad, lane, m0, n0);
@@ -1244,7 +1321,7 @@ int launch2(Gemm2Params& p, int n_comm_pairs, int max_pairs, cudaStream_t st) {
   attr[1] = pdl_attr(p.world == 1);
   cfg.attrs = attr; cfg.numAttrs = 2;
   // all CTAs must be resident at once: compute CTAs wait for comm CTAs of the same launch
-  static int max_clusters[2][2][12] = {};
+  static int max_clusters[2][2][14] = {};
   int& mc = max_clusters[A_MN][B_MN][EPI];
   if (mc == 0) {
     cfg.gridDim = dim3(2 * (tplr_sm_count() / 2));
@@ -1275,6 +1352,7 @@ int dispatch2(Gemm2Params& p, int a_mn, int b_mn, int epi, int n_comm_pairs, int
   TPLR_GEMM2_CASE(1, 0, 0) TPLR_GEMM2_CASE(1, 0, 1) TPLR_GEMM2_CASE(1, 0, 2)
   TPLR_GEMM2_CASE(0, 0, 3) TPLR_GEMM2_CASE(0, 0, 4) TPLR_GEMM2_CASE(0, 1, 5) TPLR_GEMM2_CASE(0, 1, 6)
   TPLR_GEMM2_CASE(0, 0, 7) TPLR_GEMM2_CASE(0, 0, 8) TPLR_GEMM2_CASE(0, 0, 9) TPLR_GEMM2_CASE(0, 1, 10) TPLR_GEMM2_CASE(0, 0, 11)
+  TPLR_GEMM2_CASE(0, 0, 12) TPLR_GEMM2_CASE(0, 0, 13)
 #undef TPLR_GEMM2_CASE
   return -104;
 }
@@ -1691,6 +1769,27 @@ TPLR_API int tplr_gemm2_rope(const void* X, const void* W, void* QKV, int M, int
   if (!p.c_tma) return -111;
   p.rope_cos = cosb; p.rope_sin = sinb; p.rope_s = S; p.rope_cols = rope_cols; p.rope_dh = head_dim;
   return dispatch2(p, 0, 0, 4, 0, 0, (cudaStream_t)stream);
+}
+
+// Columns of a piece of tplr_gemm2_softmax for these sizes: a row has ceil(N / columns) pieces.
+static int softmax_tile(int M, int N, int K) { return pick_tile(M, N, K, false, false, 0, 1, 128); }
+TPLR_API int tplr_gemm2_softmax_columns(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? softmax_tile(M, N, K) / 2 : 128; }
+
+// The product Z = X W^T (X [M, K], W [N, K] bf16, K-major) with the softmax over its columns in pieces of tplr_gemm2_softmax_columns
+// columns (see epilogue_softmax); Z itself is not stored.  stats [M, pieces] pairs (largest logit, sum), target [M] the logit of the
+// row's label (not written where the label is not a column).  P, if given: [M, N] bf16, rows of ldp (a multiple of 8) elements, exp(Z - the
+// piece's largest).
+TPLR_API int tplr_gemm2_softmax(const void* X, const void* W, void* P, const long long* labels, float* stats, float* target, int M, int N, int K,
+                                long long ldx, long long ldw, long long ldp, unsigned int* status, void* stream) {
+  TPLR_ENTER();
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (((uintptr_t)P & 15) || (ldp % 8) || ((uintptr_t)stats & 7) || (P && ldp < N)) return -101;
+  Gemm2Params p = {};
+  const int tile_n = softmax_tile(M, N, K);
+  if (int r = fill_common(p, X, W, P, M, N, K, ldx, ldw, P ? ldp : 8, 0, 0, 0, status, tile_n)) return r;
+  p.sm_labels = labels; p.sm_stats = reinterpret_cast<float2*>(stats); p.sm_target = target;
+  p.sm_parts = (N + tile_n / 2 - 1) / (tile_n / 2);
+  return dispatch2(p, 0, 0, P ? 12 : 13, 0, 0, (cudaStream_t)stream);
 }
 
 // int32 elements of the workspace that tplr_gemm2_q8 takes for this size (0: none).

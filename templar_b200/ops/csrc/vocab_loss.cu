@@ -1,0 +1,215 @@
+// Cross entropy from the pieces that tplr_gemm2_softmax leaves of a row of logits: (m_i, s_i) of every piece i, the target's logit z, and
+// e_ij = exp(z_ij - m_i) of its columns in bf16.
+//   lse = m + log(sum_i s_i exp(m_i - m)),  m = max m_i;     loss = lse - z
+//   d_ij = g * e_ij * exp(m_i - lse), at the label's column g * (exp(z - lse) - 1)
+// with g the gradient of the row's loss.  The label's column is made from the fp32 logit: where the model is sure of it, the
+// difference of a rounded weight and 1 would be little more than the rounding.
+//
+// A row whose label is ignored, or is no column, has loss and gradient zero.  Sums over rows and pieces are taken in one order.
+#include "common.cuh"
+
+namespace {
+typedef __nv_bfloat16 bf16;
+constexpr int THREADS = 512;
+
+// out[0] = labels that count
+__global__ void __launch_bounds__(1024) vocab_count_kernel(const long long* labels, long long T, long long ignore, int V, int* out,
+                                                           unsigned int* status) {
+  __shared__ int total;
+  grid_wait();
+  grid_release();
+  if (threadIdx.x == 0) total = 0;
+  __syncthreads();
+  int n = 0;
+  bool bad = false;
+  for (long long i = threadIdx.x; i < T; i += blockDim.x) {
+    const long long l = labels[i];
+    if (l == ignore) continue;
+    if (l < 0 || l >= V) bad = true; else ++n;
+  }
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) atomicAdd(&total, n);               // whole numbers: the same in any order
+  if (bad && status) atomicOr(status, TPLR_ST_BAD_INDEX);
+  __syncthreads();
+  if (threadIdx.x == 0) out[0] = total;
+}
+
+// Loss of each row, a warp a row.
+__global__ void __launch_bounds__(256) vocab_losses_kernel(const float2* stats, const float* target, const long long* labels, float* losses,
+                                                           float* lse_out, long long T, int parts, int V, long long ignore) {
+  grid_wait();
+  grid_release();
+  const long long row = blockIdx.x * 8LL + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= T) return;
+  const long long label = labels[row];
+  const bool counts = label != ignore && label >= 0 && label < V;
+  float loss = 0.f, lse = 0.f;
+  if (counts) {                                      // the same in all lanes
+    const float2* st = stats + row * parts;
+    float m = -INFINITY;
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, st[i].x);
+    m = warp_max(m);
+    float s = 0.f;
+    for (int i = lane; i < parts; i += 32) { const float2 v = st[i]; s += v.y * __expf(v.x - m); }
+    lse = m + logf(warp_sum(s));
+    loss = lse - target[row];
+  }
+  if (lane == 0) {
+    losses[row] = loss;
+    if (lse_out) lse_out[row] = lse;
+  }
+}
+
+// Loss of each row, and its pieces turned into the gradient of the logits in place; a block a row.  g = row_grad[row], or
+// grad_scale / *n_valid.
+__global__ void __launch_bounds__(THREADS) vocab_grad_kernel(bf16* e, long long ld, const float2* stats, const float* target, const long long* labels,
+                                                             const float* row_grad, const int* n_valid, float grad_scale, float* losses, int parts,
+                                                             int columns, int V, long long ignore) {
+  __shared__ float red[32];
+  grid_wait();
+  grid_release();
+  const long long row = blockIdx.x;
+  const long long label = labels[row];
+  const int n = (V + 7) / 8;
+  uint4* d = reinterpret_cast<uint4*>(e + row * ld);
+  if (label == ignore || label < 0 || label >= V) {
+    for (int i = threadIdx.x; i < n; i += THREADS) d[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (threadIdx.x == 0 && losses) losses[row] = 0.f;
+    return;
+  }
+  const float2* st = stats + row * parts;
+  float m = -INFINITY;
+  for (int i = threadIdx.x; i < parts; i += THREADS) m = fmaxf(m, st[i].x);
+  m = block_max(m, red);
+  float s = 0.f;
+  for (int i = threadIdx.x; i < parts; i += THREADS) { const float2 v = st[i]; s += v.y * __expf(v.x - m); }
+  s = block_sum(s, red);
+  const float lse = m + logf(s), z = target[row];
+  if (threadIdx.x == 0 && losses) losses[row] = lse - z;
+  const float g = row_grad ? row_grad[row] : grad_scale / (float)max(n_valid[0], 1);
+  const float by = g / s;
+  const int lab8 = (int)(label >> 3), lab = (int)(label & 7);
+  const int per = columns / 8;
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const float f = __expf(st[i / per].x - m) * by;
+    const uint4 v = d[i];
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    float o[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { o[2 * k] = __uint_as_float(w[k] << 16) * f; o[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u) * f; }
+    if (i == lab8) {
+      const float own = g * (__expf(z - lse) - 1.f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) if (k == lab) o[k] = own;
+    }
+    uint32_t r[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * k], o[2 * k + 1]);
+      r[k] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    d[i] = make_uint4(r[0], r[1], r[2], r[3]);
+  }
+}
+
+// out = sum of x / max(*n_valid, 1)
+__global__ void __launch_bounds__(1024) vocab_mean_kernel(const float* x, long long T, const int* n_valid, float* out) {
+  __shared__ double red[32];
+  grid_wait();
+  grid_release();
+  double s = 0.0;                                    // many rows' losses
+  for (long long i = threadIdx.x; i < T; i += blockDim.x) s += (double)x[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  s = red[threadIdx.x];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (threadIdx.x == 0) out[0] = (float)(s / (double)max(n_valid[0], 1));
+}
+
+// y = x * (*by), from bf16 or fp32 to bf16, or onto fp32; eight values a thread
+template <class In, bool ADD>
+__global__ void __launch_bounds__(256) vocab_scale_kernel(const In* x, const float* by, void* y, long long n8) {
+  grid_wait();
+  grid_release();
+  const float f = *by;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n8; i += gridDim.x * 256LL) {
+    float v[8];
+    if (sizeof(In) == 2) {
+      const uint4 q = reinterpret_cast<const uint4*>(x)[i];
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { v[2 * k] = __uint_as_float(w[k] << 16); v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u); }
+    } else {
+      const float4 a = reinterpret_cast<const float4*>(x)[2 * i], b = reinterpret_cast<const float4*>(x)[2 * i + 1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+    if (ADD) {
+      float4* o = reinterpret_cast<float4*>(y) + 2 * i;
+      float4 a = o[0], b = o[1];
+      a.x += v[0] * f; a.y += v[1] * f; a.z += v[2] * f; a.w += v[3] * f;
+      b.x += v[4] * f; b.y += v[5] * f; b.z += v[6] * f; b.w += v[7] * f;
+      o[0] = a; o[1] = b;
+    } else {
+      uint32_t r[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * k] * f, v[2 * k + 1] * f);
+        r[k] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      reinterpret_cast<uint4*>(y)[i] = make_uint4(r[0], r[1], r[2], r[3]);
+    }
+  }
+}
+}  // namespace
+
+// n_valid[0] = labels that are columns and not `ignore`
+TPLR_API int tplr_vocab_count(const long long* labels, long long T, long long ignore, int V, int* n_valid, unsigned int* status, void* stream) {
+  TPLR_ENTER();
+  return (int)launch_pdl(vocab_count_kernel, 1, 1024, 0, (cudaStream_t)stream, labels, T, ignore, V, n_valid, status);
+}
+
+// losses [T] (and, if given, lse [T]) from tplr_gemm2_softmax's stats [T, parts] and target [T]
+TPLR_API int tplr_vocab_losses(const float* stats, const float* target, const long long* labels, float* losses, float* lse, long long T,
+                               int parts, int V, long long ignore, void* stream) {
+  TPLR_ENTER();
+  if (T <= 0) return 0;
+  return (int)launch_pdl(vocab_losses_kernel, (unsigned)((T + 7) / 8), 256, 0, (cudaStream_t)stream, reinterpret_cast<const float2*>(stats), target,
+                         labels, losses, lse, T, parts, V, ignore);
+}
+
+// E [T, V] of tplr_gemm2_softmax (rows of ld elements) becomes the gradient of the logits in place; losses [T] may be null.  row_grad [T]
+// the gradients of the rows' losses, or null: grad_scale / n_valid[0] for every row.  columns: of a piece.
+TPLR_API int tplr_vocab_grad(void* E, long long ld, const float* stats, const float* target, const long long* labels, const float* row_grad,
+                             const int* n_valid, float grad_scale, float* losses, long long T, int parts, int columns, int V, long long ignore,
+                             void* stream) {
+  TPLR_ENTER();
+  if (T <= 0) return 0;
+  if ((ld % 8) || ld < V || (columns % 8) || columns <= 0 || ((uintptr_t)E & 15) || T > 0x7fffffffLL) return -401;
+  return (int)launch_pdl(vocab_grad_kernel, (unsigned)T, THREADS, 0, (cudaStream_t)stream, (bf16*)E, ld, reinterpret_cast<const float2*>(stats),
+                         target, labels, row_grad, n_valid, grad_scale, losses, parts, columns, V, ignore);
+}
+
+// loss[0] = sum of losses [T] / max(n_valid[0], 1)
+TPLR_API int tplr_vocab_mean(const float* losses, long long T, const int* n_valid, float* loss, void* stream) {
+  TPLR_ENTER();
+  return (int)launch_pdl(vocab_mean_kernel, 1, 1024, 0, (cudaStream_t)stream, losses, T, n_valid, loss);
+}
+
+// y = x * by[0] for n (a multiple of 8) values, dense, on 16-byte boundaries: x bf16 or fp32, y bf16, or fp32 that is added onto
+TPLR_API int tplr_vocab_scale(const void* x, int x_fp32, const float* by, void* y, int add_fp32, long long n, void* stream) {
+  TPLR_ENTER();
+  if (n <= 0) return 0;
+  if ((n % 8) || (((uintptr_t)x | (uintptr_t)y) & 15)) return -401;
+  const long long blocks = (n / 8 + 255) / 256, most = 8LL * tplr_sm_count();
+  const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (x_fp32 && add_fp32) return (int)launch_pdl(vocab_scale_kernel<float, true>, grid, 256, 0, st, (const float*)x, by, y, n / 8);
+  if (x_fp32) return (int)launch_pdl(vocab_scale_kernel<float, false>, grid, 256, 0, st, (const float*)x, by, y, n / 8);
+  if (add_fp32) return (int)launch_pdl(vocab_scale_kernel<bf16, true>, grid, 256, 0, st, (const bf16*)x, by, y, n / 8);
+  return (int)launch_pdl(vocab_scale_kernel<bf16, false>, grid, 256, 0, st, (const bf16*)x, by, y, n / 8);
+}

@@ -145,6 +145,19 @@ def _declare(L: ctypes.CDLL) -> None:
         "tplr_attention_bwd_scratch_cols": [i, i, i, i, i],
         "tplr_attention_fwd": [vp, vp, vp, i, i, i, i, i, ll, ll, f, vp, vp],
         "tplr_attention_bwd": [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, ll, ll, f, vp, vp],
+        "tplr_attention_docs_fwd": [vp, vp, vp, vp, vp, i, i, i, i, i, ll, ll, f, vp, vp],
+        "tplr_attention_docs_bwd": [vp, vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, ll, ll, f, vp, vp],
+        "tplr_attention_docs_bwd_scratch_cols": [i, i, i, i, i],
+        "tplr_qk_norm_rope": [vp, ll, vp, vp, vp, vp, vp, vp, ll, i, i, i, i, i, f, vp, vp],
+        "tplr_qk_norm_rope_parts": [ll, i, i, i],
+        "tplr_qk_norm_rope_bwd": [vp, ll, vp, ll, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, ll, i, i, i, i, i, f, vp, vp],
+        "tplr_gemm2_softmax_columns": [i, i, i],
+        "tplr_gemm2_softmax": [vp, vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, vp, vp],
+        "tplr_vocab_count": [vp, ll, ll, i, vp, vp, vp],
+        "tplr_vocab_losses": [vp, vp, vp, vp, vp, ll, i, i, ll, vp],
+        "tplr_vocab_grad": [vp, ll, vp, vp, vp, vp, vp, f, vp, ll, i, i, i, ll, vp],
+        "tplr_vocab_mean": [vp, ll, vp, vp, vp],
+        "tplr_vocab_scale": [vp, i, vp, vp, i, ll, vp],
         "tplr_gemm_bf16": [vp, vp, vp, i, i, i, ll, ll, ll, i, i, i, vp, i, vp],
         "tplr_gemm2_bf16": [vp, vp, vp, i, i, i, ll, ll, ll, i, i, i, vp, i, vp],
         "tplr_gemm2_acc_splits": [i, i, i],

@@ -1,0 +1,399 @@
+"""Attention within documents, norms of query and key heads, and the loss from the output projection on the GPU, against the formulas in
+64 bits.  A tolerance is made of the roundings on the way: U is a bf16 rounding, half a step, relative to the value."""
+
+import pytest
+import torch
+
+from templar_b200 import ops
+from templar_b200.ops import documents as OD
+from templar_b200.ops import functional as OF
+
+pytestmark = pytest.mark.gpu
+U = torch.finfo(torch.bfloat16).eps / 2
+DEV = "cuda"
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def normal(g, *shape, std=1.0, dtype=torch.bfloat16):
+    return (torch.randn(*shape, generator=g, device=DEV) * std).to(dtype)
+
+
+def close(got, want, bound, what):
+    got, bad = got.double(), (got.double() - want).abs() - bound
+    assert torch.isfinite(got).all(), what
+    assert bad.max() <= 0, f"{what}: {int((bad > 0).sum())} of {bad.numel()} off, worst by {bad.max().item():.3g} beyond {bound.flatten()[bad.argmax()].item():.3g}"
+
+
+# ------------------------------------------------------------------------------------------ attention
+def starts_of(kind, B, S, g):
+    rows = torch.arange(S, device=DEV, dtype=torch.int32).expand(B, S)
+    if kind == "whole":
+        return torch.zeros(B, S, dtype=torch.int32, device=DEV)
+    if kind == "single":                                       # every token a document
+        return rows.clone()
+    if kind == "window":
+        return rows - 99                                       # negative at the front
+    if kind == "nothing":
+        return torch.full((B, S), S, dtype=torch.int32, device=DEV)
+    if kind == "any":                                          # any numbers, also behind the row and below zero
+        return torch.randint(-S, 2 * S, (B, S), generator=g, device=DEV, dtype=torch.int32)
+    if kind == "extremes":
+        return torch.where(torch.rand(B, S, generator=g, device=DEV) < 0.5, -2 ** 31, 2 ** 31 - 1).to(torch.int32)
+    ends = torch.rand(B, S, generator=g, device=DEV) < (1 / 40 if kind == "docs" else 1 / 500)
+    st = torch.where(torch.roll(ends, 1, 1), rows, 0).cummax(1).values.to(torch.int32)
+    if kind == "padded":
+        st[:, S - S // 3:] = S
+    return st
+
+
+def attention64(qkv, starts, H, KV, hd, dout):
+    """(out, bound), (dqkv, bound) by the formulas."""
+    B, S, C = qkv.shape
+    G = H // KV
+    q, k, v = qkv.double().split([H * hd, KV * hd, KV * hd], dim=2)
+    q, k, v = (t.view(B, S, -1, hd).transpose(1, 2) for t in (q, k, v))
+    k, v = (t.repeat_interleave(G, 1) for t in (k, v))
+    do = dout.double().view(B, S, H, hd).transpose(1, 2)
+    rows = torch.arange(S, device=DEV)
+    seen = ((rows[None, None] <= rows[None, :, None]) & (rows[None, None] >= starts.long()[:, :, None]))[:, None]
+    sc = hd ** -0.5
+    z = (q @ k.transpose(2, 3) * sc).masked_fill(~seen, float("-inf"))
+    top = z.amax(-1, keepdim=True)
+    e = torch.exp(z - torch.where(torch.isinf(top), 0.0, top))
+    p = e / e.sum(-1, keepdim=True).clamp(min=1e-300)
+    near = 1e-4                                                # fp32 scores and exponentials, relative to the weights
+    out = p @ v
+    eo = (U + near) * (p @ v.abs()) + U * out.abs()            # rounded weights, rounded output
+    delta = (do * out).sum(-1, keepdim=True)
+    ed = (do.abs() * eo).sum(-1, keepdim=True)
+    dp = do @ v.transpose(2, 3)
+    ds = p * (dp - delta) * sc
+    es = U * ds.abs() + p * (ed + near * (do.abs() @ v.abs().transpose(2, 3) + delta.abs())) * sc
+    dq, eq = ds @ k, es @ k.abs()
+    dk, ek = ds.transpose(2, 3) @ q, es.transpose(2, 3) @ q.abs()
+    dv, ev = p.transpose(2, 3) @ do, (U + near) * (p.transpose(2, 3) @ do.abs())
+    shared = lambda t: t.view(B, KV, G, S, hd).sum(2)          # noqa: E731
+    rowsof = lambda *ts: torch.cat([t.transpose(1, 2).reshape(B, S, -1) for t in ts], -1)  # noqa: E731
+    grad = rowsof(dq, shared(dk), shared(dv))
+    bound = rowsof(eq, shared(ek), shared(ev)) * 1.01 + U * grad.abs() + 1e-6
+    return (rowsof(out), rowsof(eo) * 1.01 + 1e-6), (grad, bound)
+
+
+ATTENTION = [
+    (1, 1, 1, 1, 64, "whole"), (1, 1, 2, 1, 128, "nothing"), (3, 2, 4, 2, 64, "single"), (1, 60, 12, 12, 64, "docs"),
+    (2, 127, 4, 4, 128, "docs"), (2, 128, 4, 2, 128, "single"), (2, 129, 4, 1, 64, "docs"), (2, 300, 6, 2, 128, "padded"),
+    (2, 511, 6, 2, 64, "padded"), (1, 640, 4, 4, 128, "any"), (2, 385, 4, 4, 64, "any"), (2, 700, 2, 2, 64, "window"),
+    (1, 1024, 8, 2, 128, "window"), (2, 260, 4, 4, 128, "nothing"), (2, 260, 4, 2, 64, "nothing"), (1, 1999, 3, 3, 64, "long"),
+    (1, 1536, 5, 5, 128, "long"), (2, 300, 4, 2, 128, "extremes"), (2, 300, 4, 2, 64, "extremes"), (16, 130, 32, 8, 128, "docs"),
+]
+
+
+@pytest.mark.parametrize("B,S,H,KV,hd,kind", ATTENTION)
+def test_attention_documents(B, S, H, KV, hd, kind):
+    g = gen(S * 31 + H)
+    qkv = normal(g, B, S, (H + 2 * KV) * hd, std=1.3).requires_grad_()
+    dout = normal(g, B, S, H * hd, std=0.3)
+    starts = starts_of(kind, B, S, g)
+    out = ops.attention_documents(qkv, starts, H, KV, hd)
+    (grad,) = torch.autograd.grad(out, qkv, dout)
+    with torch.no_grad():
+        alone = ops.attention_documents(qkv, starts, H, KV, hd)
+    assert torch.equal(alone, out)
+    (want, bound), (wgrad, gbound) = attention64(qkv.detach(), starts, H, KV, hd, dout)
+    close(out.detach(), want, bound, "out")
+    close(grad, wgrad, gbound, "gradient")
+    empty = starts.long() > torch.arange(S, device=DEV)
+    assert not out[empty].any() and not grad[..., :H * hd][empty].any()
+    assert int(OF.status_word(DEV).item()) == 0
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_whole_sequences_match_the_causal_kernels(hd):
+    g = gen(5)
+    qkv = normal(g, 2, 515, 6 * hd).requires_grad_()
+    dout = normal(g, 2, 515, 4 * hd)
+    a = OF._AttentionPacked.apply(qkv, 4, 1, hd)
+    b = ops.attention_documents(qkv, torch.zeros(2, 515, dtype=torch.int64, device=DEV), 4, 1, hd)
+    assert torch.equal(a, b)
+    (da,), (db,) = torch.autograd.grad(a, qkv, dout), torch.autograd.grad(b, qkv, dout)
+    assert torch.equal(da[..., 4 * hd:], db[..., 4 * hd:])
+    torch.testing.assert_close(da.float(), db.float(), rtol=2 * U, atol=1e-6)      # dq is added up in any order: one step of bf16
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_packed_documents_are_the_documents_alone(hd):
+    """Documents that begin at whole blocks meet the same tiles as in a sequence of their own, so their outputs have the same bits."""
+    g = gen(9)
+    H, KV, lens = 4, 2, (128, 384, 50)
+    qkv = normal(g, 1, sum(lens), (H + 2 * KV) * hd)
+    starts = torch.cat([torch.full((n,), sum(lens[:i]), dtype=torch.int32) for i, n in enumerate(lens)])[None].to(DEV)
+    out = ops.attention_documents(qkv, starts, H, KV, hd)
+    at = 0
+    for n in lens:
+        one = ops.attention_documents(qkv[:, at:at + n], torch.zeros(1, n, dtype=torch.int32, device=DEV), H, KV, hd)
+        assert torch.equal(out[:, at:at + n], one)
+        at += n
+
+
+def test_attention_takes_views():
+    g = gen(3)
+    H, KV, hd, B, S = 4, 2, 64, 2, 150
+    C = (H + 2 * KV) * hd
+    wide = normal(g, B, S, C + 24)
+    dout = normal(g, S, B, H * hd).transpose(0, 1)
+    starts = starts_of("docs", B, S, g)
+    plain = wide[..., 16:16 + C].contiguous().requires_grad_()
+    ref = ops.attention_documents(plain, starts, H, KV, hd)
+    (dref,) = torch.autograd.grad(ref, plain, dout.contiguous())
+    views = [wide[..., 16:16 + C], wide[..., 16:16 + C].transpose(0, 1).contiguous().transpose(0, 1)]
+    odd = torch.empty(B * S * C + 3, dtype=torch.bfloat16, device=DEV)[3:].view(B, S, C)
+    views.append(odd.copy_(plain.detach()))
+    for v in views:
+        v = v.detach().requires_grad_()
+        out = ops.attention_documents(v, starts.long().t().contiguous().t(), H, KV, hd)
+        assert torch.equal(out, ref)
+        (d,) = torch.autograd.grad(out, v, dout)
+        torch.testing.assert_close(d.float(), dref.float(), rtol=2 * U, atol=1e-6)
+        assert torch.equal(d[..., H * hd:], dref[..., H * hd:])
+
+
+# ------------------------------------------------------------------------------------------ norm of heads
+def qknorm64(qkv, wq, wk, cos, sin, at, H, KV, hd, eps, dy):
+    B, S, C = qkv.shape
+    R = H + KV
+    x, d = qkv.double()[..., :R * hd].reshape(B, S, R, hd), dy.double()[..., :R * hd].reshape(B, S, R, hd)
+    w = torch.cat((wq.double().expand(H, hd), wk.double().expand(KV, hd)))
+    c, s = cos.double()[at][:, :, None], sin.double()[at][:, :, None]
+    r = (x.pow(2).mean(-1, keepdim=True) + eps).rsqrt()
+    z = x * r * w
+    turn = lambda t, s: torch.stack((t[..., 0::2] * c - t[..., 1::2] * s, t[..., 0::2] * s + t[..., 1::2] * c), -1).view(B, S, R, hd)  # noqa: E731
+    size = lambda t: turn(t.abs(), 0 * s) * 0 + (t[..., 0::2].abs() + t[..., 1::2].abs()).repeat_interleave(2, -1)  # noqa: E731
+    out, near = turn(z, s), 2e-6                               # a few fp32 steps
+    u = turn(d, -s)
+    gr, xh = u * w, x * r
+    m = (gr * xh).mean(-1, keepdim=True)
+    dx = r * (gr - xh * m)
+    ex = near * r * (size(d) * w.abs() + xh.abs() * (size(d) * w.abs() * xh.abs()).mean(-1, keepdim=True))
+    dw, ew = (u * xh).sum((0, 1)), (1e-5 * (size(d) * xh.abs())).sum((0, 1))       # a sum in fp32
+    flat = lambda t: t.reshape(B, S, R * hd)                   # noqa: E731
+    return (flat(out), U * flat(out).abs() + near * flat(size(z))), (flat(dx), U * flat(dx).abs() + 4 * flat(ex) + 1e-30), \
+        [(dw[a:b].sum(0), U * dw[a:b].sum(0).abs() + ew[a:b].sum(0)) for a, b in ((0, H), (H, R))]
+
+
+@pytest.mark.parametrize("B,S,H,KV,hd,pos", [
+    (1, 1, 12, 12, 64, False), (1, 1, 1, 1, 8, True), (2, 7, 10, 5, 80, True), (3, 77, 3, 1, 128, False), (2, 130, 16, 16, 128, True),
+    (1, 33, 5, 5, 256, True), (2, 19, 7, 7, 96, False), (1, 50, 9, 3, 40, True), (1, 3, 4, 2, 200, True), (5, 1, 32, 8, 128, True),
+    (2, 700, 32, 8, 128, True), (1, 2500, 12, 12, 64, False)])
+def test_qk_norm_rope(B, S, H, KV, hd, pos):
+    g = gen(hd + S)
+    qkv = normal(g, B, S, (H + 2 * KV) * hd)
+    qkv[..., ::7] *= 9
+    qkv[0, 0, :hd] = 0                                         # a head of zeros
+    qkv.requires_grad_()
+    wq, wk = (normal(g, hd).requires_grad_() for _ in range(2))
+    cos, sin = ops.rope_tables(S + 9, hd, device=DEV)
+    at = torch.randint(0, S + 9, (B, S), generator=g, device=DEV) if pos else torch.arange(S, device=DEV).expand(B, S)
+    dy = normal(g, B, S, (H + 2 * KV) * hd)
+    out = ops.qk_norm_rope(qkv, wq, wk, cos, sin, H, KV, hd, 1e-5, positions=at.to(torch.int32) if pos else None)
+    dx, dwq, dwk = torch.autograd.grad(out, (qkv, wq, wk), dy)
+    R = (H + KV) * hd
+    (w1, b1), (w2, b2), dws = qknorm64(qkv.detach(), wq.detach(), wk.detach(), cos, sin, at, H, KV, hd, 1e-5, dy)
+    close(out.detach()[..., :R], w1, b1 + 1e-30, "out")
+    close(dx[..., :R], w2, b2, "dx")
+    for got, (want, bound), name in zip((dwq, dwk), dws, ("dwq", "dwk")):
+        close(got, want, bound, name)
+    assert torch.equal(out[..., R:], qkv[..., R:]) and torch.equal(dx[..., R:], dy[..., R:])
+    with torch.no_grad():
+        assert torch.equal(ops.qk_norm_rope(qkv, wq, wk, cos, sin, H, KV, hd, 1e-5, positions=at if pos else None), out)
+    again = torch.autograd.grad(ops.qk_norm_rope(qkv, wq, wk, cos, sin, H, KV, hd, 1e-5, positions=at if pos else None), (qkv, wq, wk), dy)
+    assert all(torch.equal(a, b) for a, b in zip(again, (dx, dwq, dwk)))
+    assert int(OF.status_word(DEV).item()) == 0
+
+
+def test_qk_norm_rope_views_main_grad_and_bad_positions():
+    g = gen(1)
+    B, S, H, KV, hd = 2, 40, 4, 2, 64
+    C = (H + 2 * KV) * hd
+    wide = normal(g, B, S, C + 40)
+    x = wide[..., 8:8 + C].detach().requires_grad_()
+    dense = x.detach().contiguous().requires_grad_()
+    wq, wk = (normal(g, hd).requires_grad_() for _ in range(2))
+    cos, sin = ops.rope_tables(S, hd, device=DEV)
+    dy = normal(g, S, B, C).transpose(0, 1)
+    a, b = (ops.qk_norm_rope(t, wq, wk, cos, sin, H, KV, hd) for t in (x, dense))
+    assert torch.equal(a, b)
+    ga, gb = (torch.autograd.grad(o, (t, wq, wk), d) for o, t, d in ((a, x, dy), (b, dense, dy.contiguous())))
+    assert all(torch.equal(s, t) for s, t in zip(ga, gb))
+    mq, mk = torch.full((hd,), 3.0, device=DEV), torch.full((hd,), 5.0, device=DEV)
+    out = ops.qk_norm_rope(dense, wq, wk, cos, sin, H, KV, hd, main_grad_q=mq, main_grad_k=mk)
+    (dx,) = torch.autograd.grad(out, (dense,), dy, retain_graph=True)
+    out.backward(dy)
+    assert wq.grad is None and wk.grad is None
+    torch.testing.assert_close(mq, 3 + 2 * gb[1].float(), rtol=2 * U, atol=1e-3)
+    torch.testing.assert_close(mk, 5 + 2 * gb[2].float(), rtol=2 * U, atol=1e-3)
+    word = OF.status_word(DEV)
+    assert int(word.item()) == 0
+    far = torch.full((B, S), S, dtype=torch.int32, device=DEV)
+    far[0, 0] = -1
+    edge = far.clamp(0, S - 1)
+    try:
+        with torch.no_grad():
+            got = ops.qk_norm_rope(dense, wq, wk, cos, sin, H, KV, hd, positions=far)
+            assert int(word.item()) == 1                       # TPLR_ST_BAD_INDEX
+            assert torch.equal(got, ops.qk_norm_rope(dense, wq, wk, cos, sin, H, KV, hd, positions=edge))
+    finally:
+        word.zero_()
+
+
+# ------------------------------------------------------------------------------------------ loss
+def loss64(x, w, labels, ignore=-100):
+    """(losses, bound), d logits of the sum, bound of d: by the formulas."""
+    xd, wd = x.double(), w.double()
+    V, D = wd.shape
+    z = xd @ wd.t()
+    # fp32 sums of products of 16 in the tensor cores: one step for each of them
+    ez = (D / 16 + 2) * 2.0 ** -23 * (xd.abs() @ wd.abs().t()).amax(1, keepdim=True)
+    counts = ((labels != ignore) & (labels >= 0) & (labels < V))[:, None]
+    at = labels.clamp(0, V - 1)[:, None]
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    losses = torch.where(counts, lse - z.gather(1, at), 0.0)
+    el = 2 * ez + 4 * 2.0 ** -23 * (lse.abs() + z.gather(1, at).abs() + 8)
+    p = torch.exp(z - lse)
+    d = p.scatter_add(1, at, -torch.ones_like(lse)) * counts
+    ed = (2.02 * U + 2 * ez + 1e-5) * p
+    ed = ed.scatter(1, at, (U * d.gather(1, at).abs() + (2 * ez + 1e-5) * p.gather(1, at) + 2.0 ** -22)) * counts
+    return (losses[:, 0], (el * counts)[:, 0] + 1e-30), d, ed, counts.sum()
+
+
+def rows_and_labels(g, T, D, V, ignored=0.1):
+    w = normal(g, V, D, std=2 * D ** -0.5)
+    labels = torch.randint(0, V, (T,), generator=g, device=DEV)
+    x = torch.randn(T, D, generator=g, device=DEV) + 4 * torch.rand(T, 1, generator=g, device=DEV) * w[labels].float()
+    labels[torch.rand(T, generator=g, device=DEV) < ignored] = -100
+    return x.to(torch.bfloat16), w, labels
+
+
+LOSS = [(1, 8, 1), (1, 64, 7), (3, 16, 8), (30, 768, 1000), (128, 64, 129), (129, 200, 513), (257, 128, 2000), (700, 256, 5003), (1111, 1000, 1237),
+        (2048, 64, 640), (300, 512, 32000)]
+
+
+def check_loss(x, w, labels, chunk=None):
+    (want, el), d, ed, n = loss64(x.detach(), w.detach(), labels)
+    n = n.clamp(min=1)
+    loss = ops.linear_cross_entropy(x, w, labels)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    close(loss.detach()[None], want.sum()[None] / n, el.sum()[None] / n + 1e-12, "loss")
+    xd, wd = x.detach().double(), w.detach().double()
+    for got, ref, b in ((dx, d @ wd / n, ed @ wd.abs() / n), (dw, d.t() @ xd / n, ed.t() @ xd.abs() / n)):
+        more = (ref.abs() + b) * 0 + 2.0 ** -18 * ((d.abs() @ wd.abs()) if got is dx else (d.abs().t() @ xd.abs())) / n      # fp32 sums
+        close(got, ref, 1.02 * b + U * ref.abs() + more + 1e-30, "dx" if got is dx else "dw")
+    with torch.no_grad():
+        each = ops.linear_cross_entropy(x, w, labels, reduction="none")
+        mean = ops.linear_cross_entropy(x, w, labels)
+    close(each, want, el, "losses")
+    close(mean[None], want.sum()[None] / n, el.sum()[None] / n + 1e-12, "loss alone")
+    return dx, dw
+
+
+@pytest.mark.parametrize("T,D,V", LOSS)
+def test_linear_cross_entropy(T, D, V):
+    g = gen(T + V)
+    x, w, labels = rows_and_labels(g, T, D, V)
+    labels[0] = V - 1
+    x.requires_grad_()
+    w.requires_grad_()
+    dx, dw = check_loss(x, w, labels)
+    again = torch.autograd.grad(ops.linear_cross_entropy(x, w, labels), (x, w))
+    assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
+    assert not dx[labels == -100].any()
+    assert int(OF.status_word(DEV).item()) == 0
+
+
+def test_loss_in_several_runs_of_tokens(monkeypatch):
+    g = gen(8)
+    x, w, labels = rows_and_labels(g, 1300, 128, 3001)
+    x.requires_grad_()
+    w.requires_grad_()
+    monkeypatch.setattr(OD, "CHUNK_BYTES", 2 * 3001 * 300)
+    assert len(OD._chunks(1300, 3001)) > 3
+    check_loss(x, w, labels)
+
+
+def test_loss_gradients_of_single_tokens():
+    g = gen(4)
+    T, D, V = 333, 264, 1501
+    x, w, labels = rows_and_labels(g, T, D, V)
+    x.requires_grad_()
+    w.requires_grad_()
+    by = torch.randn(9, 37, generator=g, device=DEV)
+    each = ops.linear_cross_entropy(x.view(9, 37, D), w, labels.view(9, 37), reduction="none", grad_scale=2.0)
+    assert each.shape == (9, 37)
+    dx, dw = torch.autograd.grad(each, (x, w), by)
+    _, d, ed, _ = loss64(x.detach(), w.detach(), labels)
+    k = 2 * by.double().reshape(-1, 1)
+    xd, wd = x.detach().double(), w.detach().double()
+    d, ed = d * k, (ed + U * 0) * k.abs()
+    close(dx, d @ wd, 1.02 * (ed @ wd.abs()) + U * (d @ wd).abs() + 2.0 ** -18 * (d.abs() @ wd.abs()), "dx")
+    close(dw, d.t() @ xd, 1.02 * (ed.t() @ xd.abs()) + U * (d.t() @ xd).abs() + 2.0 ** -18 * (d.abs().t() @ xd.abs()), "dw")
+
+
+def test_loss_scales_main_grad_and_graph_use():
+    g = gen(6)
+    x, w, labels = rows_and_labels(g, 200, 64, 777)
+    x.requires_grad_()
+    w.requires_grad_()
+    dx, dw = torch.autograd.grad(ops.linear_cross_entropy(x, w, labels), (x, w))
+    loss = ops.linear_cross_entropy(x, w, labels, grad_scale=4.0)
+    d4 = torch.autograd.grad(loss * 0.5, (x, w), retain_graph=True)
+    d8 = torch.autograd.grad(loss, (x, w))                     # a second time from the same graph
+    for one, two, four in zip((dx, dw), d4, d8):
+        assert torch.equal(one * 2, two) and torch.equal(one * 4, four)
+    main = torch.full((777, 64), 0.25, device=DEV)
+    loss = ops.linear_cross_entropy(x, w, labels, main_grad=main)
+    assert (main == 0.25).all()                                # nothing is added before the backward pass
+    loss.backward()
+    assert w.grad is None
+    torch.testing.assert_close(main - 0.25, dw.float(), rtol=2 * U, atol=1e-7)
+    fixed = w.detach()
+    (only,) = torch.autograd.grad(ops.linear_cross_entropy(x, fixed, labels), (x,))
+    assert torch.equal(only, dx)
+    (only,) = torch.autograd.grad(ops.linear_cross_entropy(x.detach(), w, labels), (w,))
+    assert torch.equal(only, dw)
+
+
+def test_loss_without_labels_far_logits_and_bad_labels():
+    g = gen(7)
+    x, w, labels = rows_and_labels(g, 150, 64, 500)
+    x.requires_grad_()
+    w.requires_grad_()
+    none = torch.full_like(labels, -100)
+    loss = ops.linear_cross_entropy(x, w, none)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    assert loss.item() == 0 and not dx.any() and not dw.any()
+    big = (x.detach() * 200).requires_grad_()                  # logits of thousands: all weights but a few are zero
+    check_loss(big, w, labels)
+    word = OF.status_word(DEV)
+    assert int(word.item()) == 0
+    bad = labels.clone()
+    bad[5], bad[6] = 500, -7
+    same = labels.clone()
+    same[5] = same[6] = -100
+    try:
+        a, b = (torch.autograd.grad(ops.linear_cross_entropy(x, w, t), (x, w)) for t in (bad, same))
+        assert int(word.item()) == 1                           # TPLR_ST_BAD_INDEX
+        assert all(torch.equal(s, t) for s, t in zip(a, b))
+    finally:
+        word.zero_()
+
+
+def test_loss_takes_views():
+    g = gen(12)
+    x, w, labels = rows_and_labels(g, 90, 72, 333)
+    want = ops.linear_cross_entropy(x, w, labels, reduction="none")
+    wide = torch.zeros(90, 100, dtype=torch.bfloat16, device=DEV)
+    wide[:, 5:77] = x
+    for xv, wv in ((wide[:, 5:77], w), (x.t().contiguous().t(), w.t().contiguous().t()), (x[:, None].expand(90, 1, 72)[:, 0], w)):
+        assert torch.equal(ops.linear_cross_entropy(xv, wv, labels.to(torch.int32), reduction="none"), want)
