@@ -43,7 +43,7 @@ constexpr int MAX_STAGES = 8;                      // narrower tiles have smalle
 static_assert(4 * 8192 <= STAGE_BYTES, "the freed stage holds four warps' second pair");
 // Warps that drain the accumulator: one a quadrant of tensor memory, or two where the epilogue is as long as the main loop of a short K,
 // so that one has instructions while the other waits.  What they stage beyond 32 KB takes a stage of the ring.
-constexpr int epi_warps(int epi) { return epi == 7 || epi == 8 || epi == 10 || epi >= 12 ? 8 : 4; }
+constexpr int epi_warps(int epi) { return epi == 7 || epi == 8 || epi == 10 || epi == 12 || epi == 13 ? 8 : 4; }
 constexpr int num_threads(int epi) { return 64 + 32 * epi_warps(epi); }
 constexpr int ring_stages(int epi) { return epi == 5 || epi == 10 ? EPI5_STAGES : STAGES; }
 constexpr int MAX_RANKS = 8;
@@ -95,12 +95,13 @@ struct Gemm2Params {
   // q8_scale[g * q8_ld + m], gate groups first
   float* q8_scale;
   long long q8_ld;
-  // softmax over the columns in pieces (EPI 12, 13): a piece is half a tile's columns, sm_parts pieces a row; (largest logit, sum of
+  // softmax over the columns in pieces (EPI 12, 13): a piece is half a tile's columns, sm_parts pieces a row; (reference, sum of
   // exp(logit - it)) goes to sm_stats[row * sm_parts + piece], the logit of the row's label to sm_target[row]
   const long long* sm_labels;
   float2* sm_stats;
   float* sm_target;
   int sm_parts;
+  const float* row_scale;            // EPI 14: as EPI 0, row m times row_scale[m]
   int world, rank;
   unsigned int epoch;
   // gather
@@ -317,7 +318,7 @@ struct RopeRow {
 template <int EPI>
 __device__ __forceinline__ void epilogue_tma(const Gemm2Params& p, uint32_t tmem_acc, int quad, int lane, int m0, int n0,
                                              uint32_t stage_base, uint32_t& n_boxes, int part) {
-  constexpr bool BF16_OUT = EPI == 0 || EPI == 4;
+  constexpr bool BF16_OUT = EPI == 0 || EPI == 4 || EPI == 14;
   constexpr int COLS = BF16_OUT ? 64 : 32;
   const int row0 = m0 + quad * 32;
   const uint32_t sw = (uint32_t)(lane & 7);
@@ -325,6 +326,7 @@ __device__ __forceinline__ void epilogue_tma(const Gemm2Params& p, uint32_t tmem
   int y = EPI == 2 ? row0 + part * p.plane_rows : row0;
   const bool plane = EPI == 1 && p.plane_rows > 0 && part > 0;
   if (plane) { map = &p.tmCr[0]; y = row0 + (part - 1) * p.plane_rows; }
+  const float row_scale = EPI == 14 ? p.row_scale[min(row0 + lane, p.M - 1)] : 1.f;
   if (p.rs_on && row0 < p.M) {                       // the 32 rows of a warp have one owner (32 | every bound)
     int owner = 0;
     while (owner + 1 < p.world && row0 >= p.rs_bound[owner + 1]) ++owner;
@@ -363,6 +365,10 @@ __device__ __forceinline__ void epilogue_tma(const Gemm2Params& p, uint32_t tmem
               r[8 * q + 2 * e + 1] = __float_as_uint(a * ss[e] + b * cc[e]);
             }
           }
+        }
+        if (EPI == 14) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * row_scale);
         }
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
@@ -940,9 +946,16 @@ __device__ __forceinline__ bool epilogue_swiglu_bwd_q8(const Gemm2Params& p, uin
 }
 
 // Epilogue of the output projection with the softmax over its columns (EPI 12, 13): a lane has a row, so its piece's largest logit
-// and sum need no exchange; the accumulator is read twice, once for each.  EPI 12 stores exp(logit - largest of the piece) as bf16,
-// which is off by a rounding of itself whatever the logit's size (the logit in bf16 would be off by 2^-9 of the logit,
-// and the weight by as much in its exponent); EPI 13 stores the numbers of the pieces alone.  Columns from N on count for nothing.
+// and sum need no exchange; the accumulator is read twice, once for each.  EPI 12 stores exp(logit - reference) as bf16, which is
+// off by a rounding of itself whatever the logit's size (the logit in bf16 would be off by up to 2^-8 of the logit, and the
+// weight by that many times itself); EPI 13 stores the numbers of the pieces alone.  Columns from N on count for nothing.
+//
+// The reference of a piece is zero while its largest logit is within SM_NEAR of zero, as those of language models are, else that logit: so
+// nearly always all pieces of a row have the same one, and the stored numbers are the row's softmax up to a factor of the row,
+// which the two products behind take along.  A pass over the [M, N] weights that brings every piece to the row's largest logit
+// instead took 197 us where this product takes 693 (8192 x 2048 x 32000).  Within SM_NEAR the sums stay far inside fp32:
+// exp(40) = 2e17, and a weight is only lost where it is below 1e-20 of the row's sum.
+constexpr float SM_NEAR = 40.f;
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -978,7 +991,8 @@ __device__ __forceinline__ void epilogue_softmax(const Gemm2Params& p, uint32_t 
     top = fmaxf(top, top2);
   }
   constexpr float LOG2E = 1.4426950408889634f;
-  const float neg = top == -INFINITY ? 0.f : -top * LOG2E;
+  const float ref = fabsf(top) <= SM_NEAR || top == -INFINITY ? 0.f : top;
+  const float neg = -ref * LOG2E;
   float sum = 0.f, sum2 = 0.f;
 #pragma unroll 1
   for (int c = 0; c < width; c += 64) {
@@ -1004,7 +1018,7 @@ __device__ __forceinline__ void epilogue_softmax(const Gemm2Params& p, uint32_t 
     if (STORE) box_store(&p.tmC, buf, lane, n_boxes, c0 + c, row0);
   }
   if (live) {
-    p.sm_stats[(long long)(row0 + lane) * p.sm_parts + c0 / half] = make_float2(top, sum + sum2);
+    p.sm_stats[(long long)(row0 + lane) * p.sm_parts + c0 / half] = make_float2(ref, sum + sum2);
     if (mine >= 0) p.sm_target[row0 + lane] = target;
   }
 }
@@ -1013,7 +1027,8 @@ __device__ __forceinline__ void epilogue_softmax(const Gemm2Params& p, uint32_t 
 // 4 store bf16 with the rotary embedding applied to the leading columns, 5 backward of the SwiGLU on the data gradient
 // of the down projection, 6 data gradient of the attention output projection with the attention backward's delta term,
 // 7 / 8 product of 8-bit rows stored as bf16 / fp32, 9 as 3 with the projection kept in 8 bits, 10 as 5 from it,
-// 11 product of 8-bit rows, int32 sums of a part of K to a plane of its own, 12 softmax over the columns in pieces, 13 their numbers alone
+// 11 product of 8-bit rows, int32 sums of a part of K to a plane of its own, 12 softmax over the columns in pieces, 13 their numbers alone,
+// 14 as 0 with a factor for each row
 template <bool A_MN, bool B_MN, int EPI>
 __global__ void __launch_bounds__(num_threads(EPI), 1)
 gemm2_kernel(const __grid_constant__ Gemm2Params p) {
@@ -1217,7 +1232,7 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
         else if (EPI == 4 && p.rope_dh == 64 && p.rope_cols % 64 == 0)
           epilogue_rope<64>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
         else if (EPI == 11) epilogue_tma<2>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes, w.t % p.k_splits);
-        else if (EPI >= 12) epilogue_softmax<EPI == 12>(p, tmem_acc, quad, turn, lane, m0, n0, sEpi + (uint32_t)(warp - 2) * 4096u, n_boxes);
+        else if (EPI == 12 || EPI == 13) epilogue_softmax<EPI == 12>(p, tmem_acc, quad, turn, lane, m0, n0, sEpi + (uint32_t)(warp - 2) * 4096u, n_boxes);
         else if (I8)       epilogue_q8<EPI == 8>(p, tmem_acc, quad, turn, lane, m0, n0, sEpi + (uint32_t)(warp - 2) * 4096u, n_boxes);
         else if (p.c_tma)  epilogue_tma<EPI>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes, w.t % p.k_splits);
         else               epilogue_direct<EPI>(p, tmem_acc, quad, lane, m0, n0);
@@ -1321,7 +1336,7 @@ int launch2(Gemm2Params& p, int n_comm_pairs, int max_pairs, cudaStream_t st) {
   attr[1] = pdl_attr(p.world == 1);
   cfg.attrs = attr; cfg.numAttrs = 2;
   // all CTAs must be resident at once: compute CTAs wait for comm CTAs of the same launch
-  static int max_clusters[2][2][14] = {};
+  static int max_clusters[2][2][15] = {};
   int& mc = max_clusters[A_MN][B_MN][EPI];
   if (mc == 0) {
     cfg.gridDim = dim3(2 * (tplr_sm_count() / 2));
@@ -1352,7 +1367,7 @@ int dispatch2(Gemm2Params& p, int a_mn, int b_mn, int epi, int n_comm_pairs, int
   TPLR_GEMM2_CASE(1, 0, 0) TPLR_GEMM2_CASE(1, 0, 1) TPLR_GEMM2_CASE(1, 0, 2)
   TPLR_GEMM2_CASE(0, 0, 3) TPLR_GEMM2_CASE(0, 0, 4) TPLR_GEMM2_CASE(0, 1, 5) TPLR_GEMM2_CASE(0, 1, 6)
   TPLR_GEMM2_CASE(0, 0, 7) TPLR_GEMM2_CASE(0, 0, 8) TPLR_GEMM2_CASE(0, 0, 9) TPLR_GEMM2_CASE(0, 1, 10) TPLR_GEMM2_CASE(0, 0, 11)
-  TPLR_GEMM2_CASE(0, 0, 12) TPLR_GEMM2_CASE(0, 0, 13)
+  TPLR_GEMM2_CASE(0, 0, 12) TPLR_GEMM2_CASE(0, 0, 13) TPLR_GEMM2_CASE(0, 1, 14)
 #undef TPLR_GEMM2_CASE
   return -104;
 }
@@ -1500,9 +1515,10 @@ __global__ void __launch_bounds__(256) add_planes_kernel(const float* __restrict
 }
 
 // The parts' planes ([parts][plane] fp32, rows of N elements) added in order -> bf16 rows of ldc elements; N, plane and ldc
-// multiples of 8, 16-byte aligned.
+// multiples of 8, 16-byte aligned.  SCALE: row m times row_scale[m].
+template <bool SCALE>
 __global__ void __launch_bounds__(256) round_rows_kernel(const float* __restrict__ x, __nv_bfloat16* __restrict__ y, long long M, int n8,
-                                                         long long ldc, int parts, long long plane) {
+                                                         long long ldc, int parts, long long plane, const float* row_scale) {
   grid_wait();
   grid_release();
   behind_grid_wait(x); behind_grid_wait(y);
@@ -1515,9 +1531,14 @@ __global__ void __launch_bounds__(256) round_rows_kernel(const float* __restrict
       a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
       b.x += d.x; b.y += d.y; b.z += d.z; b.w += d.w;
     }
+    const long long row = i / n8;
+    if (SCALE) {
+      const float f = row_scale[row];
+      a.x *= f; a.y *= f; a.z *= f; a.w *= f;
+      b.x *= f; b.y *= f; b.z *= f; b.w *= f;
+    }
     const __nv_bfloat162 h[4] = {__floats2bfloat162_rn(a.x, a.y), __floats2bfloat162_rn(a.z, a.w), __floats2bfloat162_rn(b.x, b.y),
                                  __floats2bfloat162_rn(b.z, b.w)};
-    const long long row = i / n8;
     *reinterpret_cast<uint4*>(y + row * ldc + (i - row * n8) * 8) = *reinterpret_cast<const uint4*>(h);
   }
 }
@@ -1659,8 +1680,34 @@ TPLR_API int tplr_gemm2_bf16_split(const void* A, const void* B, void* C, float*
   if (int r = dispatch2(p, a_mn, b_mn, 2, 0, 0, (cudaStream_t)stream)) return r;
   const long long n = (long long)M * (N / 8);
   const unsigned grid = (unsigned)((n + 255) / 256 < 8LL * tplr_sm_count() ? (n + 255) / 256 : 8LL * tplr_sm_count());
-  return (int)launch_pdl(round_rows_kernel, grid, 256, 0, (cudaStream_t)stream, ws, (__nv_bfloat16*)C, M, N / 8, ldc, p.k_splits,
-                         (long long)p.plane_rows * N);
+  return (int)launch_pdl(round_rows_kernel<false>, grid, 256, 0, (cudaStream_t)stream, ws, (__nv_bfloat16*)C, M, N / 8, ldc, p.k_splits,
+                         (long long)p.plane_rows * N, nullptr);
+}
+
+// C[M, N] = row_scale[m] * (A B) in bf16, A [M, K] K-major and B [K, N] with N contiguous; ws as in tplr_gemm2_bf16_split where
+// tplr_gemm2_out_splits cuts K.  C 16-byte aligned, ldc and N multiples of 8.
+TPLR_API int tplr_gemm2_rows(const void* A, const void* B, void* C, float* ws, const float* row_scale, int M, int N, int K, long long lda,
+                             long long ldb, long long ldc, unsigned int* status, void* stream) {
+  TPLR_ENTER();
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if ((N % 8) || (ldc % 8) || (((uintptr_t)C | (uintptr_t)ws) & 15)) return -101;
+  Gemm2Params p = {};
+  const int parts = pick_parts(M, N, K, 0);
+  if (parts == 1) {
+    if (int r = fill_common(p, A, B, C, M, N, K, lda, ldb, ldc, 0, 1, 0, status, pick_tile(M, N, K, false, true, 0))) return r;
+    p.row_scale = row_scale;
+    return dispatch2(p, 0, 1, 14, 0, 0, (cudaStream_t)stream);
+  }
+  if (!ws) return -101;
+  if (int r = fill_common(p, A, B, ws, M, N, K, lda, ldb, N, 0, 1, 2, status, pick_tile(M, N, K, false, true, 0, parts))) return r;
+  p.k_splits = parts;
+  p.plane_rows = (M + 31) / 32 * 32;
+  if (!make_map(&p.tmC, ws, N, (long long)p.k_splits * p.plane_rows, N, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B, true)) return -110;
+  if (int r = dispatch2(p, 0, 1, 2, 0, 0, (cudaStream_t)stream)) return r;
+  const long long n = ((long long)M * (N / 8) + 255) / 256;
+  const unsigned grid = (unsigned)(n < 8LL * tplr_sm_count() ? n : 8LL * tplr_sm_count());
+  return (int)launch_pdl(round_rows_kernel<true>, grid, 256, 0, (cudaStream_t)stream, ws, (__nv_bfloat16*)C, M, N / 8, ldc, p.k_splits,
+                         (long long)p.plane_rows * N, row_scale);
 }
 
 // GU[M, 2F] = X W^T for the packed weight W = [w1; w3] ([2F, K] bf16, K-major) and H[M, F] = silu(GU[:, :F]) * GU[:, F:]
@@ -1776,9 +1823,9 @@ static int softmax_tile(int M, int N, int K) { return pick_tile(M, N, K, false, 
 TPLR_API int tplr_gemm2_softmax_columns(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? softmax_tile(M, N, K) / 2 : 128; }
 
 // The product Z = X W^T (X [M, K], W [N, K] bf16, K-major) with the softmax over its columns in pieces of tplr_gemm2_softmax_columns
-// columns (see epilogue_softmax); Z itself is not stored.  stats [M, pieces] pairs (largest logit, sum), target [M] the logit of the
-// row's label (not written where the label is not a column).  P, if given: [M, N] bf16, rows of ldp (a multiple of 8) elements, exp(Z - the
-// piece's largest).
+// columns (see epilogue_softmax); Z itself is not stored.  stats [M, pieces] pairs (reference, sum of exp(Z - it)), target [M] the logit of
+// the row's label (not written where the label is not a column).  P, if given: [M, N] bf16, rows of ldp (a multiple of 8) elements,
+// exp(Z - the piece's reference).
 TPLR_API int tplr_gemm2_softmax(const void* X, const void* W, void* P, const long long* labels, float* stats, float* target, int M, int N, int K,
                                 long long ldx, long long ldw, long long ldp, unsigned int* status, void* stream) {
   TPLR_ENTER();

@@ -12,7 +12,7 @@
 namespace {
 typedef __nv_bfloat16 bf16;
 
-constexpr int WARPS = 8;             // of a block
+constexpr int WARPS = 4;             // of a block
 
 struct QkNorm {
   const bf16* x; long long ldx;      // packed projection
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(WARPS * 32) qk_norm_fwd_kernel(const QkNorm p)
 }
 
 template <int LANES, int STEPS>
-__global__ void __launch_bounds__(WARPS * 32) qk_norm_bwd_kernel(const QkNorm p) {
+__global__ void __launch_bounds__(WARPS * 32, 4) qk_norm_bwd_kernel(const QkNorm p) {
   __shared__ float sums[WARPS * (32 / LANES)][2][LANES * 8];
   grid_wait();
   grid_release();
@@ -229,7 +229,7 @@ bool fits(const QkNorm& p) {
          p.lddy % 8 == 0 && !(((uintptr_t)p.x | (uintptr_t)p.dy | (uintptr_t)p.y | (uintptr_t)p.wq | (uintptr_t)p.wk | (uintptr_t)p.cosb |
                                (uintptr_t)p.sinb) & 15);
 }
-constexpr int FWD_STEPS = 4, BWD_STEPS = 2;
+constexpr int FWD_STEPS = 4, BWD_STEPS = 4;
 int lanes_of(int hd) { return hd <= 64 ? 8 : hd <= 128 ? 16 : 32; }
 int chunks_of(int n_q, int n_k, int hd, int steps) {
   const int heads = steps * 32 / lanes_of(hd);

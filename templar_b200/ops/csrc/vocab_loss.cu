@@ -1,16 +1,18 @@
-// Cross entropy from the pieces that tplr_gemm2_softmax leaves of a row of logits: (m_i, s_i) of every piece i, the target's logit z, and
-// e_ij = exp(z_ij - m_i) of its columns in bf16.
-//   lse = m + log(sum_i s_i exp(m_i - m)),  m = max m_i;     loss = lse - z
-//   d_ij = g * e_ij * exp(m_i - lse), at the label's column g * (exp(z - lse) - 1)
-// with g the gradient of the row's loss.  The label's column is made from the fp32 logit: where the model is sure of it, the
-// difference of a rounded weight and 1 would be little more than the rounding.
+// Cross entropy from the pieces that tplr_gemm2_softmax leaves of a row of logits: (r_i, s_i) of every piece i, its reference and the sum of
+// its e_ij = exp(z_ij - r_i); the target's logit z; and the e_ij in bf16.  With c the largest reference of the row and
+// s = sum_i s_i exp(r_i - c):
+//   lse = c + log(s),   loss = lse - z,   d_ij = g * (exp(z_ij - lse) - [ij is the label])
+// with g the gradient of the row's loss.  d is the row's factor f = g / s times E, which is e_ij where the piece's reference is c, as
+// it nearly always is, e_ij exp(r_i - c) where it is not, and s (exp(z - lse) - 1) in the label's column, made from the
+// fp32 logit: where the model is sure of it, the difference of a rounded weight and 1 would be little more than the rounding.  So
+//   dx = f * (E w),   dw = E^T (f x)
+// and E is not read or written here but for the label's column and pieces of another reference.  f x is rounded to bf16, as d would be.
 //
 // A row whose label is ignored, or is no column, has loss and gradient zero.  Sums over rows and pieces are taken in one order.
 #include "common.cuh"
 
 namespace {
 typedef __nv_bfloat16 bf16;
-constexpr int THREADS = 512;
 
 // out[0] = labels that count
 __global__ void __launch_bounds__(1024) vocab_count_kernel(const long long* labels, long long T, long long ignore, int V, int* out,
@@ -61,55 +63,75 @@ __global__ void __launch_bounds__(256) vocab_losses_kernel(const float2* stats, 
   }
 }
 
-// Loss of each row, and its pieces turned into the gradient of the logits in place; a block a row.  g = row_grad[row], or
-// grad_scale / *n_valid.
-__global__ void __launch_bounds__(THREADS) vocab_grad_kernel(bf16* e, long long ld, const float2* stats, const float* target, const long long* labels,
-                                                             const float* row_grad, const int* n_valid, float grad_scale, float* losses, int parts,
-                                                             int columns, int V, long long ignore) {
-  __shared__ float red[32];
+// What both products need of a row (see above), a warp a row: f in row_scale, E in place of e, f x in xs (dense rows of D); and the
+// row's loss.  g = row_grad[row], or grad_scale / *n_valid.
+__global__ void __launch_bounds__(256) vocab_rows_kernel(bf16* e, long long ld, const float2* stats, const float* target, const long long* labels,
+                                                         const float* row_grad, const int* n_valid, float grad_scale, const bf16* x, long long ldx,
+                                                         bf16* xs, float* row_scale, float* losses, long long T, int parts, int columns, int V,
+                                                         int D, long long ignore) {
   grid_wait();
   grid_release();
-  const long long row = blockIdx.x;
-  const long long label = labels[row];
-  const int n = (V + 7) / 8;
-  uint4* d = reinterpret_cast<uint4*>(e + row * ld);
-  if (label == ignore || label < 0 || label >= V) {
-    for (int i = threadIdx.x; i < n; i += THREADS) d[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (threadIdx.x == 0 && losses) losses[row] = 0.f;
-    return;
-  }
+  const long long row = blockIdx.x * 8LL + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= T) return;
   const float2* st = stats + row * parts;
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < parts; i += THREADS) m = fmaxf(m, st[i].x);
-  m = block_max(m, red);
-  float s = 0.f;
-  for (int i = threadIdx.x; i < parts; i += THREADS) { const float2 v = st[i]; s += v.y * __expf(v.x - m); }
-  s = block_sum(s, red);
-  const float lse = m + logf(s), z = target[row];
-  if (threadIdx.x == 0 && losses) losses[row] = lse - z;
-  const float g = row_grad ? row_grad[row] : grad_scale / (float)max(n_valid[0], 1);
-  const float by = g / s;
-  const int lab8 = (int)(label >> 3), lab = (int)(label & 7);
-  const int per = columns / 8;
-  for (int i = threadIdx.x; i < n; i += THREADS) {
-    const float f = __expf(st[i / per].x - m) * by;
-    const uint4 v = d[i];
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    float o[8];
+  bf16* er = e + row * ld;
+  const long long label = labels[row];
+  const bool counts = label != ignore && label >= 0 && label < V;
+  float c = -INFINITY, low = INFINITY, s = 0.f;
+  for (int i = lane; i < parts; i += 32) { c = fmaxf(c, st[i].x); low = fminf(low, st[i].x); }
+  c = warp_max(c);
+  low = -warp_max(-low);
+  for (int i = lane; i < parts; i += 32) { const float2 v = st[i]; s += v.y * __expf(v.x - c); }
+  s = warp_sum(s);
+  const float g = !counts ? 0.f : row_grad ? row_grad[row] : grad_scale / (float)max(n_valid[0], 1);
+  const float f = counts ? g / s : 0.f;
+  if (counts) {
+    if (low < c) {                                   // the same in all lanes
+      for (int i = 0; i < parts; ++i) {
+        if (st[i].x == c) continue;
+        const float by = __expf(st[i].x - c);
+        for (int k = i * columns + lane * 8; k < min(i * columns + columns, V); k += 256) {      // the columns behind V are nobody's
+          uint4 q = *reinterpret_cast<uint4*>(er + k);
+          uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) { o[2 * k] = __uint_as_float(w[k] << 16) * f; o[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u) * f; }
-    if (i == lab8) {
-      const float own = g * (__expf(z - lse) - 1.f);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) if (k == lab) o[k] = own;
+          for (int j = 0; j < 4; ++j) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(w[j] << 16) * by, __uint_as_float(w[j] & 0xffff0000u) * by);
+            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          *reinterpret_cast<uint4*>(er + k) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      __syncwarp();
     }
-    uint32_t r[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * k], o[2 * k + 1]);
-      r[k] = *reinterpret_cast<const uint32_t*>(&h);
+    if (lane == 0) {
+      const float lse = c + logf(s), z = target[row];
+      er[label] = __float2bfloat16(s * (__expf(z - lse) - 1.f));
+      if (losses) losses[row] = lse - z;
     }
-    d[i] = make_uint4(r[0], r[1], r[2], r[3]);
+  } else {
+    // what the row holds is multiplied by zero, which takes numbers
+    if (!(s < INFINITY)) for (int k = lane * 8; k < V; k += 256) *reinterpret_cast<uint4*>(er + k) = make_uint4(0u, 0u, 0u, 0u);
+    if (lane == 0 && losses) losses[row] = 0.f;
+  }
+  if (lane == 0) row_scale[row] = f;
+  if (!xs) return;
+  const uint4* xr = reinterpret_cast<const uint4*>(x + row * ldx);
+  uint4* out = reinterpret_cast<uint4*>(xs + row * D);
+#pragma unroll 4
+  for (int i = lane; i < D / 8; i += 32) {
+    uint4 q = make_uint4(0u, 0u, 0u, 0u);
+    if (counts) {
+      q = xr[i];
+      uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xffff0000u) * f);
+        w[j] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      q = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    out[i] = q;
   }
 }
 
@@ -182,16 +204,18 @@ TPLR_API int tplr_vocab_losses(const float* stats, const float* target, const lo
                          labels, losses, lse, T, parts, V, ignore);
 }
 
-// E [T, V] of tplr_gemm2_softmax (rows of ld elements) becomes the gradient of the logits in place; losses [T] may be null.  row_grad [T]
-// the gradients of the rows' losses, or null: grad_scale / n_valid[0] for every row.  columns: of a piece.
-TPLR_API int tplr_vocab_grad(void* E, long long ld, const float* stats, const float* target, const long long* labels, const float* row_grad,
-                             const int* n_valid, float grad_scale, float* losses, long long T, int parts, int columns, int V, long long ignore,
-                             void* stream) {
+// What tplr_gemm2_softmax left of T rows, E [T, V] (rows of ld elements), made ready for the products of the gradients: dx = row_scale * (E w),
+// dw = E^T xs.  x [T, D] (rows of ldx elements), xs [T, D] dense or null; losses [T] may be null.  row_grad [T] the gradients of the rows'
+// losses, or null: grad_scale / n_valid[0] for every row.  columns: of a piece.
+TPLR_API int tplr_vocab_rows(void* E, long long ld, const float* stats, const float* target, const long long* labels, const float* row_grad,
+                             const int* n_valid, float grad_scale, const void* x, long long ldx, void* xs, float* row_scale, float* losses,
+                             long long T, int parts, int columns, int V, int D, long long ignore, void* stream) {
   TPLR_ENTER();
   if (T <= 0) return 0;
-  if ((ld % 8) || ld < V || (columns % 8) || columns <= 0 || ((uintptr_t)E & 15) || T > 0x7fffffffLL) return -401;
-  return (int)launch_pdl(vocab_grad_kernel, (unsigned)T, THREADS, 0, (cudaStream_t)stream, (bf16*)E, ld, reinterpret_cast<const float2*>(stats),
-                         target, labels, row_grad, n_valid, grad_scale, losses, parts, columns, V, ignore);
+  if ((ld % 8) || ld < V || (columns % 8) || columns <= 0 || (ldx % 8) || (D % 8) || (((uintptr_t)E | (uintptr_t)x | (uintptr_t)xs) & 15)) return -401;
+  return (int)launch_pdl(vocab_rows_kernel, (unsigned)((T + 7) / 8), 256, 0, (cudaStream_t)stream, (bf16*)E, ld,
+                         reinterpret_cast<const float2*>(stats), target, labels, row_grad, n_valid, grad_scale, (const bf16*)x, ldx, (bf16*)xs,
+                         row_scale, losses, T, parts, columns, V, D, ignore);
 }
 
 // loss[0] = sum of losses [T] / max(n_valid[0], 1)

@@ -17,7 +17,7 @@ import torch
 from . import functional as OF
 from . import native
 
-CHUNK_BYTES = 512 << 20         # of the weights exp(logit - largest) that are there at a time
+CHUNK_BYTES = 512 << 20         # of the weights exp(logit) that are there at a time
 
 
 def _on(t: torch.Tensor):
@@ -270,15 +270,15 @@ def _chunks(T: int, V: int) -> list[tuple[int, int]]:
 class _Pieces:
     """Workspaces of the product with the softmax in pieces, for up to ``rows`` tokens."""
 
-    def __init__(self, x2, w, rows: int, store: bool):
+    def __init__(self, x2, w, rows: int, store: bool, scaled_rows: bool = False):
         self.V, self.D = w.shape
         dev = x2.device
         self.ld = -(-self.V // 8) * 8
         self.e = torch.empty(rows, self.ld, dtype=torch.bfloat16, device=dev) if store else None
-        columns = native.lib().tplr_gemm2_softmax_columns(rows, self.V, self.D)
-        # a shorter last run may take narrower pieces: twice as many
-        self.stats = torch.empty(rows * -(-self.V // min(columns, 64)) * 2, dtype=torch.float32, device=dev)
+        self.stats = torch.empty(rows * -(-self.V // 64) * 2, dtype=torch.float32, device=dev)      # pieces of 64 columns or more
         self.target = torch.empty(rows, dtype=torch.float32, device=dev)
+        self.scale = torch.empty(rows, dtype=torch.float32, device=dev) if store else None
+        self.xs = torch.empty(rows, self.D, dtype=torch.bfloat16, device=dev) if scaled_rows else None
 
     def run(self, x, w, labels) -> tuple[int, int]:
         """(pieces of a row, columns of a piece)"""
@@ -308,25 +308,30 @@ def _gradients(x2, w, labels, ignore_index, row_grad, n_valid, grad_scale, losse
     T, D = x2.shape
     V = w.shape[0]
     runs = _chunks(T, V)
-    ws = _Pieces(x2, w, runs[0][1], True)
+    ws = _Pieces(x2, w, runs[0][1], True, want_w)
+    L, st = native.lib(), OF.status_word(x2.device).data_ptr()
     dx = torch.empty(T, D, dtype=x2.dtype, device=x2.device) if want_x else None
     dw = None
     for a, b in runs:
         x, e = x2[a:b], ws.e[:b - a, :V]
         parts, columns = ws.run(x, w, labels[a:b])
-        native.check(native.lib().tplr_vocab_grad(
+        native.check(L.tplr_vocab_rows(
             ws.e.data_ptr(), ws.ld, ws.stats.data_ptr(), ws.target.data_ptr(), labels[a:].data_ptr(),
-            None if row_grad is None else row_grad[a:].data_ptr(), native.ptr(n_valid), grad_scale,
-            None if losses is None else losses[a:].data_ptr(), b - a, parts, columns, V, ignore_index, native.stream_ptr()), "vocab_grad")
+            None if row_grad is None else row_grad[a:].data_ptr(), native.ptr(n_valid), grad_scale, x.data_ptr(), x.stride(0), native.ptr(ws.xs),
+            ws.scale.data_ptr(), None if losses is None else losses[a:].data_ptr(), b - a, parts, columns, V, D, ignore_index,
+            native.stream_ptr()), "vocab_rows")
         if want_x:
-            OF.gemm(e, w, b_mn=True, out=dx[a:b])
+            cuts = L.tplr_gemm2_out_splits(b - a, D, V)
+            planes = torch.empty(cuts * (-(-(b - a) // 32) * 32) * D, dtype=torch.float32, device=x2.device) if cuts > 1 else None
+            native.check(L.tplr_gemm2_rows(ws.e.data_ptr(), w.data_ptr(), dx[a:].data_ptr(), native.ptr(planes), ws.scale.data_ptr(), b - a, D, V,
+                                           ws.ld, w.stride(0), D, st, native.stream_ptr()), "gemm2_rows")
         if want_w:
             single = len(runs) == 1 and not keep32
             if dw is None:
                 dw = torch.empty(V, D, dtype=torch.bfloat16 if single else torch.float32, device=x2.device)
-                OF.gemm(e, x, a_mn=True, b_mn=True, out=dw)
+                OF.gemm(e, ws.xs[:b - a], a_mn=True, b_mn=True, out=dw)
             else:
-                OF.gemm(e, x, a_mn=True, b_mn=True, out=dw, accumulate=True)
+                OF.gemm(e, ws.xs[:b - a], a_mn=True, b_mn=True, out=dw, accumulate=True)
     return dx, dw
 
 
@@ -424,7 +429,7 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
     token's own, in the shape of ``labels``, zero where it is ignored.  A label that is neither ``ignore_index`` nor a column counts as ignored, and
     the kernels report it in the status word.  The gradient is ``grad_scale`` times the loss's, and the incoming one counts.
 
-    The kernels hold ``exp(logit - largest of its piece)`` for a run of tokens at a time (``CHUNK_BYTES``), from which the gradients of
+    The kernels hold ``exp(logit)`` (relative to a piece's largest where that is far from zero) for a run of tokens at a time (``CHUNK_BYTES``), from which the gradients of
     ``x`` and ``w`` are made at once; where nothing asks for a gradient, two numbers for every 64 or 128 columns.  A mean makes its gradients in the forward
     pass; one gradient of ``"none"`` costs the product a second time."""
     if reduction not in ("mean", "none"):

@@ -263,8 +263,10 @@ def loss64(x, w, labels, ignore=-100):
     el = 2 * ez + 4 * 2.0 ** -23 * (lse.abs() + z.gather(1, at).abs() + 8)
     p = torch.exp(z - lse)
     d = p.scatter_add(1, at, -torch.ones_like(lse)) * counts
+    # the products take every weight rounded, times a row of x times the row's factor, rounded: (1 + U)^2 - 1 < 2.02 U, in the label's
+    # column too, whose weight is made from exp(z - lse) - 1 in fp32
     ed = (2.02 * U + 2 * ez + 1e-5) * p
-    ed = ed.scatter(1, at, (U * d.gather(1, at).abs() + (2 * ez + 1e-5) * p.gather(1, at) + 2.0 ** -22)) * counts
+    ed = ed.scatter(1, at, (2.02 * U * d.gather(1, at).abs() + (2 * ez + 1e-5) * p.gather(1, at) + 2.0 ** -22)) * counts
     return (losses[:, 0], (el * counts)[:, 0] + 1e-30), d, ed, counts.sum()
 
 
@@ -387,6 +389,34 @@ def test_loss_without_labels_far_logits_and_bad_labels():
         assert all(torch.equal(s, t) for s, t in zip(a, b))
     finally:
         word.zero_()
+
+
+@pytest.mark.parametrize("shift,some", [(100.0, False), (-100.0, False), (90.0, True), (-90.0, True)])
+def test_loss_of_logits_far_from_zero(shift, some):
+    """All logits, or every fifth run of 200 columns, moved far away: pieces of several references in a row."""
+    g = gen(21)
+    x, w, labels = rows_and_labels(g, 270, 72, 2000)
+    x[:, 0] = 10
+    far = torch.arange(2000, device=DEV) // 200 % 5 == 2 if some else torch.ones(2000, dtype=torch.bool, device=DEV)
+    w[:, 0] = torch.where(far, shift / 10, 0.0)
+    x.requires_grad_()
+    w.requires_grad_()
+    check_loss(x, w, labels)
+
+
+def test_rows_that_count_for_nothing_may_hold_anything():
+    g = gen(22)
+    x, w, labels = rows_and_labels(g, 140, 64, 900)
+    labels[7] = labels[8] = -100
+    nan = x.clone()
+    nan[7], nan[8] = float("nan"), float("inf")
+    got, want = [], []
+    for t, out in ((nan, got), (x, want)):
+        t.requires_grad_()
+        w.requires_grad_()
+        loss = ops.linear_cross_entropy(t, w, labels)
+        out += [loss, *torch.autograd.grad(loss, (t, w)), ops.linear_cross_entropy(t, w, labels, reduction="none")]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_loss_takes_views():
