@@ -93,16 +93,23 @@ def get_titan_model_args(hparams: SimpleNamespace) -> ModelArgs:
     vocab = hparams.tokenizer.vocab_size if hasattr(hparams, "tokenizer") else hparams.model_config.vocab_size
     tt = getattr(hparams, "torchtitan", SimpleNamespace())
     tie = getattr(tt, "tie_embeddings", True)
+    # options of this package: norms of query and key heads, attention within documents, the loss without logits
+    own = {"qk_norm": bool(getattr(tt, "qk_norm", False)), "fused_loss": bool(getattr(tt, "fused_loss", False))}
+    if getattr(tt, "document_attention", False):
+        eos = getattr(getattr(hparams, "tokenizer", None), "eos_token_id", None)
+        if eos is None or eos < 0:
+            raise ValueError("torchtitan.document_attention needs a tokenizer with an end-of-text token")
+        own["document_eos"] = int(eos)
     if size in llama3_configs:
         base = llama3_configs[size]
-        return ModelArgs(**{**base.__dict__, "max_seq_len": seq, "vocab_size": vocab, "tie_embeddings": tie})
+        return ModelArgs(**{**base.__dict__, "max_seq_len": seq, "vocab_size": vocab, "tie_embeddings": tie, **own})
     mc = hparams.model_config
     return ModelArgs(dim=mc.hidden_size, n_layers=mc.num_hidden_layers, n_heads=mc.num_attention_heads,
                      n_kv_heads=getattr(mc, "num_key_value_heads", mc.num_attention_heads), vocab_size=vocab,
                      intermediate_size=mc.intermediate_size, multiple_of=256,
                      ffn_dim_multiplier=mc.intermediate_size / max(int(8 * mc.hidden_size / 3), 1),
                      norm_eps=getattr(mc, "rms_norm_eps", 1e-5), rope_theta=getattr(mc, "rope_theta", 10000.0),
-                     max_seq_len=seq, tie_embeddings=tie)
+                     max_seq_len=seq, tie_embeddings=tie, **own)
 
 
 def create_job_config(hparams: SimpleNamespace, role: Literal["miner", "validator", "evaluator"] = "miner") -> JobConfig:
@@ -246,6 +253,8 @@ def _interleaved_to_half_rotation(w: torch.Tensor, n_heads: int) -> torch.Tensor
 
 
 def titan_to_hf_state_dict(sd: dict, args: ModelArgs) -> dict:
+    if args.qk_norm:
+        raise ValueError("the HuggingFace LLaMA layout has no norms of query and key heads: a model with qk_norm cannot be converted")
     out = {}
     for k, v in sd.items():
         if "freqs_cis" in k:

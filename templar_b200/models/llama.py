@@ -21,6 +21,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 
+from ..ops import documents as OD
 from ..ops import functional as OF
 from ..ops import quantized as OQ
 
@@ -40,6 +41,9 @@ class ModelArgs:
     max_seq_len: int = 2048
     depth_init: bool = True
     tie_embeddings: bool = False
+    qk_norm: bool = False          # norm of every query and key head, in front of the rotary embedding
+    document_eos: int = -1         # >= 0: a sequence holds documents that end with this token, and attention stays within them
+    fused_loss: bool = False       # the loss from the output projection, without the logits in memory
 
     @property
     def kv_heads(self) -> int:
@@ -60,7 +64,7 @@ class ModelArgs:
 
     def num_params(self) -> int:
         d, f, v, kv = self.dim, self.ffn_hidden, self.vocab_size, self.kv_heads * self.head_dim
-        per_layer = 2 * d * d + 2 * kv * d + 3 * d * f + 2 * d
+        per_layer = 2 * d * d + 2 * kv * d + 3 * d * f + 2 * d + (2 * self.head_dim if self.qk_norm else 0)
         return self.n_layers * per_layer + v * d * (1 if self.tie_embeddings else 2) + d
 
     def flops_per_token(self, seq_len: int) -> float:
@@ -118,9 +122,25 @@ class Attention(nn.Module):
         self.wv = _Weight(self.n_kv * self.hd, args.dim)
         self.wo = _Weight(args.dim, args.n_heads * self.hd)
         self.packed = None  # (weight view, main_grad view) of [wq; wk; wv] set by the flat store
+        self.q_norm = RMSNorm(self.hd, args.norm_eps) if args.qk_norm else None
+        self.k_norm = RMSNorm(self.hd, args.norm_eps) if args.qk_norm else None
 
-    def forward(self, x, cos, sin):
+    def attend(self, qkv, cos, sin, docs=None):
+        """Attention of a packed projection that is not rotated yet; ``docs``: (starts, positions) of documents."""
+        if self.q_norm is not None:
+            qkv = OD.qk_norm_rope(qkv, self.q_norm.weight, self.k_norm.weight, cos, sin, self.n_heads, self.n_kv, self.hd, self.q_norm.eps,
+                                  positions=None if docs is None else docs[1])
+        else:      # the angle between two rows is that of their distance: places in the sequence serve documents too
+            qkv = OF.rope(qkv, cos, sin, self.n_heads + self.n_kv, self.hd)
+        if docs is not None:
+            return OD.attention_documents(qkv, docs[0], self.n_heads, self.n_kv, self.hd)
+        return OF.attention_packed(qkv, self.n_heads, self.n_kv, self.hd)
+
+    def forward(self, x, cos, sin, docs=None):
         B, S, _ = x.shape
+        if self.q_norm is not None or docs is not None:
+            w, mg = self.packed or (torch.cat((self.wq.weight, self.wk.weight, self.wv.weight), dim=0), None)
+            return self.wo(self.attend(OF.linear(x, w, mg), cos, sin, docs))
         if self.packed is not None:          # projections, rotary embedding and attention as one node on the own kernels
             return OF.attention_block(x, self.packed[0], self.wo.weight, cos, sin, self.n_heads, self.n_kv, self.hd,
                                       self.packed[1], getattr(self.wo.weight, "main_grad", None))
@@ -155,11 +175,11 @@ class TransformerBlock(nn.Module):
         self.weight_init_std = (0.02 / (2 * (layer_id + 1)) ** 0.5 if args.depth_init
                                 else 0.02 / (2 * args.n_layers) ** 0.5)
 
-    def forward(self, x, cos, sin):
-        h = x + self.attention(self.attention_norm(x), cos, sin)
+    def forward(self, x, cos, sin, docs=None):
+        h = x + self.attention(self.attention_norm(x), cos, sin, docs)
         return h + self.feed_forward(self.ffn_norm(h))
 
-    def forward_fused(self, res, delta, cos, sin):
+    def forward_fused(self, res, delta, cos, sin, docs=None):
         """Same block on a split residual stream: the hidden state is ``res + delta`` and the sum is
         formed inside the norm kernels (``delta`` None: ``res`` alone).  Returns the next ``(res, delta)``.
 
@@ -173,7 +193,10 @@ class TransformerBlock(nn.Module):
             wqkv, mg_qkv = att.packed or (torch.cat((att.wq.weight, att.wk.weight, att.wv.weight)), None)
             w13, mg13 = ff.packed or (torch.cat((ff.w1.weight, ff.w3.weight)), None)
             res, y, rows = OQ.add_rmsnorm_saved8(res, delta, n1.weight, n1.eps)
-            a = OQ.attention_block_saved8(y, wqkv, att.wo.weight, cos, sin, att.n_heads, att.n_kv, att.hd, rows, n1.weight, mg_qkv)
+            if att.q_norm is not None or docs is not None:
+                a = att.wo(att.attend(OQ.linear_saved8(y, wqkv, rows, n1.weight, mg_qkv), cos, sin, docs))
+            else:
+                a = OQ.attention_block_saved8(y, wqkv, att.wo.weight, cos, sin, att.n_heads, att.n_kv, att.hd, rows, n1.weight, mg_qkv)
             res, y, rows = OQ.add_rmsnorm_saved8(res, a, n2.weight, n2.eps)
             return res, OQ.feed_forward_saved8(y, w13, ff.w2.weight, rows, n2.weight, mg13)
         if getattr(self, "recompute_ops", False) and att.packed is not None and ff.packed is not None:
@@ -182,21 +205,21 @@ class TransformerBlock(nn.Module):
                 qkv = OF.norm_linear(res, None, nw.weight, eps, att.packed[0], att.packed[1])
             else:
                 res, qkv = OF.norm_linear(res, delta, nw.weight, eps, att.packed[0], att.packed[1])
-            qkv = OF.rope(qkv, cos, sin, att.n_heads + att.n_kv, att.hd)
-            a = att.wo(OF.attention_packed(qkv, att.n_heads, att.n_kv, att.hd))
+            a = att.wo(att.attend(qkv, cos, sin, docs))
             res, h13 = OF.norm_linear(res, a, self.ffn_norm.weight, self.ffn_norm.eps, ff.packed[0], ff.packed[1])
             return res, OF.swiglu_linear(h13, ff.w2.weight)
         if delta is None:
             y = self.attention_norm(res)
         else:
             res, y = OF.add_rmsnorm(res, delta, self.attention_norm.weight, self.attention_norm.eps)
-        a = self.attention(y, cos, sin)
+        a = self.attention(y, cos, sin, docs)
         res, y = OF.add_rmsnorm(res, a, self.ffn_norm.weight, self.ffn_norm.eps)
         return res, self.feed_forward(y)
 
     def init_weights(self, generator=None):
-        for norm in (self.attention_norm, self.ffn_norm):
-            nn.init.ones_(norm.weight)
+        for norm in (self.attention_norm, self.ffn_norm, self.attention.q_norm, self.attention.k_norm):
+            if norm is not None:
+                nn.init.ones_(norm.weight)
         for lin in (self.attention.wq, self.attention.wk, self.attention.wv, self.feed_forward.w1):
             nn.init.trunc_normal_(lin.weight, mean=0.0, std=0.02, generator=generator)
         for lin in (self.attention.wo, self.feed_forward.w2, self.feed_forward.w3):
@@ -236,6 +259,13 @@ class LlamaModel(nn.Module):
             cos, sin = OF.rope_tables(self.args.max_seq_len, self.args.head_dim, self.args.rope_theta, device)
             self._rope_cache[key] = (cos.contiguous(), sin.contiguous())
         return self._rope_cache[key]
+
+    def _documents(self, tokens: torch.Tensor):
+        """(first row of its document, place in it) of every token, where the sequences hold documents."""
+        if self.args.document_eos < 0:
+            return None
+        starts = OD.document_starts(tokens, self.args.document_eos)
+        return starts, torch.arange(tokens.shape[1], dtype=torch.int32, device=tokens.device) - starts
 
     # -- init ------------------------------------------------------------------------------
     @torch.no_grad()
@@ -279,6 +309,7 @@ class LlamaModel(nn.Module):
     # -- forward ---------------------------------------------------------------------------
     def hidden_states(self, tokens: torch.Tensor) -> torch.Tensor:
         cos, sin = self._rope(tokens.device)
+        docs = self._documents(tokens)
         # With sharded parameters (parallel/fsdp.py) the weights of a block are only present while the block runs:
         # `pg` brings them in ahead of the block in both directions of the pass.
         pg = getattr(self, "_param_gather", None)
@@ -298,9 +329,9 @@ class LlamaModel(nn.Module):
                 fn = self._gated_block(pg, f"layers.{key}", layer)
             if every and count % every == 0 and torch.is_grad_enabled():
                 from torch.utils.checkpoint import checkpoint
-                h, delta = checkpoint(fn, h, delta, cos, sin, use_reentrant=False)
+                h, delta = checkpoint(fn, h, delta, cos, sin, docs, use_reentrant=False)
             else:
-                h, delta = fn(h, delta, cos, sin)
+                h, delta = fn(h, delta, cos, sin, docs)
             if pg is not None:
                 h, delta = pg.leave(f"layers.{key}", h, delta)
         if pg is not None:
@@ -311,12 +342,12 @@ class LlamaModel(nn.Module):
 
     @staticmethod
     def _gated_block(pg, group: str, layer):
-        def run(h, delta, cos, sin):
+        def run(h, delta, cos, sin, docs=None):
             if delta is None:
                 h = pg.enter(group, h)
             else:
                 h, delta = pg.enter(group, h, delta)
-            return layer.forward_fused(h, delta, cos, sin)
+            return layer.forward_fused(h, delta, cos, sin, docs)
         return run
 
     def forward(self, tokens: torch.Tensor, labels: torch.Tensor | None = None) -> torch.Tensor:
@@ -326,6 +357,13 @@ class LlamaModel(nn.Module):
              ignore_index: int = -100) -> torch.Tensor:
         """Mean cross entropy over ``labels != ignore_index``.  The gradient that flows back is
         ``grad_scale`` times the gradient of this mean (see ``ops.functional.cross_entropy``)."""
+        if self.args.fused_loss:
+            w = self.output.weight
+            mg = getattr(w, "main_grad", None)
+            if mg is not None and not torch.is_tensor(mg):
+                raise ValueError("LlamaModel: fused_loss adds the output projection's gradient to a buffer of its own rank; with sharded "
+                                 "parameters (shard_params) leave it off")
+            return OD.linear_cross_entropy(self.hidden_states(tokens), w, labels, grad_scale, ignore_index, mg)
         logits = self.forward(tokens)
         return OF.cross_entropy(logits, labels, grad_scale, ignore_index)
 

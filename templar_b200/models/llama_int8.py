@@ -34,18 +34,17 @@ class Int8Llama:
         pack = lambda own, *ws: own[0] if own is not None else torch.cat([w.weight for w in ws])  # noqa: E731
         return {"wqkv": ops.quantize_weight(pack(att.packed, att.wq, att.wk, att.wv)), "wo": ops.quantize_weight(att.wo.weight),
                 "w13": ops.quantize_weight(pack(ff.packed, ff.w1, ff.w3)), "w2": ops.quantize_weight(ff.w2.weight),
-                "n1": layer.attention_norm, "n2": layer.ffn_norm, "heads": (att.n_heads, att.n_kv, att.hd)}
+                "n1": layer.attention_norm, "n2": layer.ffn_norm, "attention": att}
 
     @torch.no_grad()
     def hidden_states(self, tokens: torch.Tensor) -> torch.Tensor:
         m = self._model
         cos, sin = m._rope(tokens.device)
+        docs = m._documents(tokens)
         h, delta = OF.embedding(tokens, m.tok_embeddings.weight), None
         for b in self.blocks:
-            H, KV, hd = b["heads"]
             h, rows = ops.add_rmsnorm_q8(h, delta, b["n1"].weight, b["n1"].eps)
-            qkv = OF.rope(ops.linear_q8(rows, b["wqkv"], h.dtype), cos, sin, H + KV, hd)
-            delta = ops.linear_q8(OF.attention_packed(qkv, H, KV, hd), b["wo"])
+            delta = ops.linear_q8(b["attention"].attend(ops.linear_q8(rows, b["wqkv"], h.dtype), cos, sin, docs), b["wo"])
             h, rows = ops.add_rmsnorm_q8(h, delta, b["n2"].weight, b["n2"].eps)
             delta = ops.linear_q8(ops.swiglu_q8(ops.linear_q8(rows, b["w13"], h.dtype)), b["w2"], h.dtype)
         if delta is None:
@@ -61,4 +60,6 @@ class Int8Llama:
     @torch.no_grad()
     def loss(self, tokens: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
         """Mean cross entropy over ``labels != ignore_index``."""
+        if self.args.fused_loss:
+            return ops.linear_cross_entropy(self.hidden_states(tokens), self._model.output.weight, labels, ignore_index=ignore_index)
         return OF.cross_entropy(self.forward(tokens), labels, 1.0, ignore_index)

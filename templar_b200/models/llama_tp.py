@@ -164,6 +164,8 @@ class TPLlamaModel(LlamaModel):
     """Holds rank ``tp.rank``'s shard of a LLaMA; ``loss()`` is the training entry point."""
 
     def __init__(self, args: ModelArgs, tp_rank: int, tp_world: int):
+        if args.qk_norm or args.document_eos >= 0 or args.fused_loss:
+            raise ValueError("TPLlamaModel: qk_norm, document_eos and fused_loss are options of LlamaModel (heads and vocabulary whole on a rank)")
         nn.Module.__init__(self)
         self.args = self.model_args = args
         self.tp_rank, self.tp_world = tp_rank, tp_world

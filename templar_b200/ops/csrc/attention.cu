@@ -40,10 +40,6 @@ struct AttnFwdParams {
   int B, S, H, KV;
   float scale_log2;       // softmax scale * log2(e)
   unsigned int* status;
-  // documents: row s of sequence b sees the keys max(starts[b * S + s], 0) .. s only; blocks[b * nQ + i] takes the least start in
-  // query block i of a row that sees anything (INT_MAX: none does), which the backward kernel walks by
-  const int* starts;
-  int* blocks;
 };
 
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
@@ -205,27 +201,6 @@ __device__ __forceinline__ float attn_row_max(uint32_t ts_lane, int r) {
   }
   return mx;
 }
-// The same with the columns from lo to hi alone (documents).
-__device__ __forceinline__ float attn_row_max_range(uint32_t (&v)[128], int lo, int hi) {
-  float mx = -INFINITY;
-#pragma unroll
-  for (int e = 0; e < 128; ++e) {
-    if (e < lo || e > hi) v[e] = 0xff800000u;
-    mx = fmaxf(mx, __uint_as_float(v[e]));
-  }
-  return mx;
-}
-__device__ __forceinline__ float attn_row_max_range(uint32_t ts_lane, int lo, int hi) {
-  float mx = -INFINITY;
-#pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    uint32_t v[32];
-    tmem_ld32(ts_lane + c * 32, v);
-#pragma unroll
-    for (int e = 0; e < 32; ++e) mx = fmaxf(mx, (c * 32 + e < lo || c * 32 + e > hi) ? -INFINITY : __uint_as_float(v[e]));
-  }
-  return mx;
-}
 // P = exp2(S * scale - m) written as packed bf16 to 64 columns; returns the row sum of P.
 __device__ __forceinline__ float attn_row_exp(const uint32_t (&v)[128], uint32_t tp_lane, float sl2, float m_used) {
   const unsigned long long sl2x2 = pack_f32x2(__float_as_uint(sl2), __float_as_uint(sl2));
@@ -250,9 +225,9 @@ __device__ __forceinline__ float attn_row_exp(const uint32_t (&v)[128], uint32_t
   return s0 + s1;
 }
 
-// the same over the first 64 columns of S; MASK 1: the columns up to hi, 2: from lo to hi, are kept
-template <int MASK>
-__device__ __forceinline__ float attn_row_exp(uint32_t ts_lane, int lo, int hi, float sl2, float m_used) {
+// the same over the first 64 columns of S
+template <bool DIAG>
+__device__ __forceinline__ float attn_row_exp(uint32_t ts_lane, int r, float sl2, float m_used) {
   const unsigned long long sl2x2 = pack_f32x2(__float_as_uint(sl2), __float_as_uint(sl2));
   const unsigned long long negm = pack_f32x2(__float_as_uint(-m_used), __float_as_uint(-m_used));
   unsigned long long sum = 0ull;                         // (0.f, 0.f)
@@ -265,9 +240,9 @@ __device__ __forceinline__ float attn_row_exp(uint32_t ts_lane, int lo, int hi, 
       float a0, a1;
       unpack_f32x2(fma_f32x2(pack_f32x2(v[2 * e], v[2 * e + 1]), sl2x2, negm), a0, a1);
       float p0 = exp2f(a0), p1 = exp2f(a1);
-      if (MASK) {
-        if (c * 32 + 2 * e > hi || (MASK == 2 && c * 32 + 2 * e < lo)) p0 = 0.f;
-        if (c * 32 + 2 * e + 1 > hi || (MASK == 2 && c * 32 + 2 * e + 1 < lo)) p1 = 0.f;
+      if (DIAG) {
+        if (c * 32 + 2 * e > r) p0 = 0.f;
+        if (c * 32 + 2 * e + 1 > r) p1 = 0.f;
       }
       sum = add_f32x2(sum, pack_f32x2(__float_as_uint(p0), __float_as_uint(p1)));
       __nv_bfloat162 hh = __floats2bfloat162_rn(p0, p1);
@@ -280,7 +255,7 @@ __device__ __forceinline__ float attn_row_exp(uint32_t ts_lane, int lo, int hi, 
   return s0 + s1;
 }
 
-template <int DH, bool DOCS>
+template <int DH>
 __global__ void __launch_bounds__(FWD_THREADS, 2)
 attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
   constexpr int TILE_BYTES = tile_bytes<DH>();
@@ -289,7 +264,6 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
   __shared__ __align__(8) uint64_t bar_q, bar_k_full, bar_k_empty, bar_v_full, bar_v_empty, bar_s_full, bar_s_read, bar_p_full, bar_o_full;
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
-  __shared__ int s_least[4];                               // documents: the least start of each softmax warp's rows
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int nQ = (p.S + BQ - 1) / BQ;
@@ -298,7 +272,7 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
   const int qi = nQ - 1 - (int)(blockIdx.x / hb);
   const int h = (int)(blockIdx.x % hb) % p.H, b = (int)(blockIdx.x % hb) / p.H;
   const int g = h / (p.H / p.KV);
-  int j0 = 0, nb = qi + 1;                                 // kv blocks j0 .. j0 + nb - 1; causal: 0 .. qi
+  const int nb = qi + 1;                                   // causal: kv blocks 0..qi
   const int row0 = qi * BQ;                                // position of the first query row; rows past S read as zeros
   const int qcol = h * DH, kcol = (p.H + g) * DH, vcol = (p.H + p.KV + g) * DH;
   volatile int* abort_flag = &s_abort;
@@ -322,22 +296,6 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
   tcgen05_fence_after();
   grid_wait();
   grid_release();
-  int start = 0;                                           // first key of this softmax thread's row
-  if constexpr (DOCS) {
-    // documents: from the block of the least start of a row that sees anything; a row past the end or without a key asks for none
-    if (warp >= 2) {
-      const int r = (warp & 3) * 32 + lane, s = row0 + r;
-      start = s < p.S ? max(p.starts[(long long)b * p.S + s], 0) : INT_MAX;
-      if (start > s) start = INT_MAX;
-      const int least = __reduce_min_sync(0xffffffffu, start);
-      if (lane == 0) s_least[warp - 2] = least;
-    }
-    __syncthreads();
-    const int least = min(min(s_least[0], s_least[1]), min(s_least[2], s_least[3]));
-    j0 = least == INT_MAX ? 0 : least / BKV;
-    nb = least == INT_MAX ? 0 : qi - j0 + 1;
-    if (p.blocks && h == 0 && threadIdx.x == 0) p.blocks[(long long)b * nQ + qi] = least;
-  }
   const uint32_t tmem_base = s_tmem_base;
   // S columns 0..127, O from column 128.  P lies over S at DH = 128; at 64 it has the 64 columns that O leaves, so that the
   // next block's S is computed as soon as the softmax warps hold this one's in registers (AHEAD).
@@ -348,8 +306,7 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
   if (warp == 0) {
     {
       const bool leader = elect_one();
-      const bool any = !DOCS || nb > 0;
-      if (leader && any) {
+      if (leader) {
         mbar_expect_tx(smem_u32(&bar_q), TILE_BYTES);
         load_tile<DH>(sQ, &p.tmQKV, smem_u32(&bar_q), qcol, row0, b);
       }
@@ -357,7 +314,7 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
       int n_k = 0, n_v = 0;                                // tiles asked for
       for (int j = 0; j < nb && ok; ++j) {
         const uint32_t ph = j & 1;
-        const int krow = (j0 + j) * BKV;
+        const int krow = j * BKV;
         if (!(ok = mbar_wait_warp(smem_u32(&bar_k_empty), ph ^ 1, abort_flag))) break;
         if (leader) {
           mbar_expect_tx(smem_u32(&bar_k_full), TILE_BYTES);
@@ -373,7 +330,7 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
       }
       if (leader) {
         Drain drain;                                         // no load may land after the CTA has retired: a role may have given up
-        if (any) drain.wait(smem_u32(&bar_q), 0);
+        drain.wait(smem_u32(&bar_q), 0);
         if (n_k) drain.wait(smem_u32(&bar_k_full), (uint32_t)((n_k - 1) & 1));
         if (n_v) drain.wait(smem_u32(&bar_v_full), (uint32_t)((n_v - 1) & 1));
       }
@@ -397,7 +354,7 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
         }
         return true;
       };
-      bool ok = (!DOCS || nb > 0) && mbar_wait_warp(smem_u32(&bar_q), 0, abort_flag);
+      bool ok = mbar_wait_warp(smem_u32(&bar_q), 0, abort_flag);
       if (AHEAD && ok) ok = issue_s(0);
       for (int j = 0; j < nb && ok; ++j) {
         const uint32_t ph = j & 1;
@@ -430,15 +387,7 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tcgen05_fence_after();
-      const bool diag = j0 + j == qi;
-      // documents: the columns of this block that the row sees; without a mask where all rows of the warp see all of them
-      int lo = 0, hi = r;
-      bool masked = diag;
-      if constexpr (DOCS) {
-        lo = start == INT_MAX ? BKV : start - (j0 + j) * BKV;        // nothing: behind the last column
-        hi = diag ? r : BKV - 1;
-        masked = diag || __any_sync(0xffffffffu, lo > 0);
-      }
+      const bool diag = j == qi;
       uint32_t sv[AHEAD ? 128 : 1];                        // AHEAD: the row, loaded once
       float mx;
       if constexpr (AHEAD) {
@@ -446,11 +395,9 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_s_read));
-        if constexpr (DOCS) mx = masked ? attn_row_max_range(sv, lo, hi) : attn_row_max<false>(sv, r);
-        else mx = diag ? attn_row_max<true>(sv, r) : attn_row_max<false>(sv, r);
+        mx = diag ? attn_row_max<true>(sv, r) : attn_row_max<false>(sv, r);
       } else {
-        if constexpr (DOCS) mx = masked ? attn_row_max_range(tS + lane_off, lo, hi) : attn_row_max<false>(tS + lane_off, r);
-        else mx = diag ? attn_row_max<true>(tS + lane_off, r) : attn_row_max<false>(tS + lane_off, r);
+        mx = diag ? attn_row_max<true>(tS + lane_off, r) : attn_row_max<false>(tS + lane_off, r);
       }
       if (AHEAD && j > 0) {                // O and the P columns: the product of block j-1 has finished with them
         ok = mbar_wait(smem_u32(&bar_v_empty), (uint32_t)((j - 1) & 1), abort_flag);
@@ -475,21 +422,18 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
           }
         }
       }
-      // documents: a row that has seen no key yet has no maximum, and all its scores here are masked
-      const float m_ref = DOCS && m_used == -INFINITY ? 0.f : m_used;
-      if constexpr (AHEAD) l += attn_row_exp(sv, tP + lane_off, p.scale_log2, m_ref);
-      else l += masked ? attn_row_exp<DOCS ? 2 : 1>(tS + lane_off, lo, hi, p.scale_log2, m_ref) : attn_row_exp<0>(tS + lane_off, lo, hi, p.scale_log2, m_ref);
+      if constexpr (AHEAD) l += attn_row_exp(sv, tP + lane_off, p.scale_log2, m_used);
+      else l += diag ? attn_row_exp<true>(tS + lane_off, r, p.scale_log2, m_used) : attn_row_exp<false>(tS + lane_off, r, p.scale_log2, m_used);
       tmem_wait_st();
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bar_p_full));
     }
     // epilogue: O / l -> bf16 -> swizzled staging (the Q tile is no longer read) -> TMA store
-    if (ok && (!DOCS || nb > 0)) ok = mbar_wait(smem_u32(&bar_o_full), 0, abort_flag);
+    if (ok) ok = mbar_wait(smem_u32(&bar_o_full), 0, abort_flag);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tcgen05_fence_after();
-      const bool empty = DOCS && start == INT_MAX;           // a row that sees nothing is zero
       const float inv_l = 1.f / l;
       const uint32_t stage = sQ + (uint32_t)quad * (32u * DH * 2u);
       const int orow = row0 + quad * 32;
@@ -498,19 +442,14 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
       for (int c = 0; c < DH / 32; ++c) {
         uint32_t v[32];
         tmem_ld32(tO + c * 32 + lane_off, v);
-        if (DOCS && empty) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = 0u;
-        }
-        const float by = empty ? 1.f : inv_l;
         const uint32_t rowaddr = stage + (uint32_t)(c >> 1) * 4096u + (uint32_t)lane * 128u;
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
           uint32_t pw[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            __nv_bfloat162 hh = __floats2bfloat162_rn(__uint_as_float(v[8 * q4 + 2 * e]) * by,
-                                                      __uint_as_float(v[8 * q4 + 2 * e + 1]) * by);
+            __nv_bfloat162 hh = __floats2bfloat162_rn(__uint_as_float(v[8 * q4 + 2 * e]) * inv_l,
+                                                      __uint_as_float(v[8 * q4 + 2 * e + 1]) * inv_l);
             pw[e] = *reinterpret_cast<uint32_t*>(&hh);
           }
           const uint32_t jj = (uint32_t)((c & 1) * 4 + q4);
@@ -526,8 +465,7 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       }
-      // an infinite sum makes the backward pass's weights of the row zero
-      if (p.lse && row0 + r < p.S) p.lse[((long long)b * p.H + h) * p.S + row0 + r] = empty ? INFINITY : (m_used + log2f(l)) * 0.6931471805599453f;
+      if (p.lse && row0 + r < p.S) p.lse[((long long)b * p.H + h) * p.S + row0 + r] = (m_used + log2f(l)) * 0.6931471805599453f;
     }
   }
   __syncwarp();
@@ -543,20 +481,19 @@ attn_fwd_kernel(const __grid_constant__ AttnFwdParams p) {
 }  // namespace
 
 namespace {
-template <int DH, bool DOCS>
+template <int DH>
 int launch_fwd(const void* qkv, void* out, float* lse, int B, int S, int H, int KV, long long ld_qkv, long long ld_o,
-               float scale, unsigned int* status, cudaStream_t st, const int* starts = nullptr, int* blocks = nullptr) {
+               float scale, unsigned int* status, cudaStream_t st) {
   AttnFwdParams p = {};
   if (!make_map3(&p.tmQKV, qkv, (long long)(H + 2 * KV) * DH, S, B, ld_qkv, 64, 128)) return -202;
   if (!make_map3(&p.tmO, out, (long long)H * DH, S, B, ld_o, 64, 32)) return -203;
   p.lse = lse; p.B = B; p.S = S; p.H = H; p.KV = KV;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = status;
-  p.starts = starts; p.blocks = blocks;
-  cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<DH, DOCS>, cudaFuncAttributeMaxDynamicSharedMemorySize, fwd_smem<DH>());
+  cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, fwd_smem<DH>());
   if (e != cudaSuccess) return (int)e;
   const unsigned grid = (unsigned)(((S + BQ - 1) / BQ) * H * B);
-  return (int)launch_pdl(attn_fwd_kernel<DH, DOCS>, grid, FWD_THREADS, fwd_smem<DH>(), st, p);
+  return (int)launch_pdl(attn_fwd_kernel<DH>, grid, FWD_THREADS, fwd_smem<DH>(), st, p);
 }
 }  // namespace
 
@@ -567,10 +504,336 @@ TPLR_API int tplr_attention_fwd(const void* qkv, void* out, float* lse, int B, i
   TPLR_ENTER();
   if (B <= 0 || S <= 0) return 0;
   if (H % KV || (ld_qkv % 8) || (ld_o % 8) || ((uintptr_t)qkv & 15) || ((uintptr_t)out & 15)) return -201;
-  if (head_dim == 128) return launch_fwd<128, false>(qkv, out, lse, B, S, H, KV, ld_qkv, ld_o, scale, status, (cudaStream_t)stream);
-  if (head_dim == 64) return launch_fwd<64, false>(qkv, out, lse, B, S, H, KV, ld_qkv, ld_o, scale, status, (cudaStream_t)stream);
+  if (head_dim == 128) return launch_fwd<128>(qkv, out, lse, B, S, H, KV, ld_qkv, ld_o, scale, status, (cudaStream_t)stream);
+  if (head_dim == 64) return launch_fwd<64>(qkv, out, lse, B, S, H, KV, ld_qkv, ld_o, scale, status, (cudaStream_t)stream);
   return -201;
 }
+
+// ------------------------------------------------------------------------------------------ //
+// Forward within documents: row s of a sequence sees the keys max(starts[s], 0) .. s.  A CTA has a query block of one head as above and
+// walks the key blocks from that of its rows' least start to the diagonal; a block that all rows of a warp see whole runs without
+// a mask.  Eight softmax warps, two a quadrant of tensor memory with half of a row's columns each: what bounds a block is the
+// chain from S over the exponentials to the product with V, and a row of 128 in one thread is the longest part of it.  The two
+// exchange their maxima through shared memory, join their waits in the same barrier (a warp that gave up takes the other one
+// along), and keep sums of their own to the end.  P lies in the S columns of the warp that makes it, at DH = 64 in columns of its own.
+// ------------------------------------------------------------------------------------------ //
+namespace {
+
+constexpr int DOCS_THREADS = 320;
+
+struct AttnDocsParams {
+  CUtensorMap tmQKV;      // as in the forward kernel above
+  CUtensorMap tmO;
+  float* lse;
+  int B, S, H, KV;
+  float scale_log2;
+  unsigned int* status;
+  const int* starts;      // [B, S]
+  int* blocks;            // [B, nQ], or null: takes the least start of a row in the query block that sees anything (INT_MAX: none does)
+};
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
+// Both warps of a quadrant come here with an answer and leave with the joint one.
+__device__ __forceinline__ bool pair_agrees(bool ok, int quad) {
+  uint32_t both;
+  asm volatile("{\n\t.reg .pred mine, all;\n\tsetp.ne.u32 mine, %2, 0;\n\tbar.red.and.pred all, %1, 64, mine;\n\tselp.u32 %0, 1, 0, all;\n\t}"
+               : "=r"(both) : "r"(quad + 1), "r"((uint32_t)ok) : "memory");
+  return both != 0;
+}
+
+template <int DH>
+__global__ void __launch_bounds__(DOCS_THREADS, 2)
+attn_docs_fwd_kernel(const __grid_constant__ AttnDocsParams p) {
+  constexpr int TILE_BYTES = tile_bytes<DH>();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(8) uint64_t bar_q, bar_k_full, bar_k_empty, bar_v_full, bar_v_empty, bar_s_full, bar_s_read, bar_p_full, bar_o_full;
+  __shared__ uint32_t s_tmem_base;
+  __shared__ int s_abort;
+  __shared__ int s_least[4];
+  __shared__ float s_part[2][2][128];                      // [block parity][column half][row]: maxima, at the end sums
+
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int nQ = (p.S + BQ - 1) / BQ;
+  const int hb = p.H * p.B;
+  const int qi = nQ - 1 - (int)(blockIdx.x / hb);          // late query blocks first: they may see the most
+  const int h = (int)(blockIdx.x % hb) % p.H, b = (int)(blockIdx.x % hb) / p.H;
+  const int g = h / (p.H / p.KV);
+  const int row0 = qi * BQ;
+  const int qcol = h * DH, kcol = (p.H + g) * DH, vcol = (p.H + p.KV + g) * DH;
+  volatile int* abort_flag = &s_abort;
+
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    mbar_init(smem_u32(&bar_q), 1);
+    mbar_init(smem_u32(&bar_k_full), 1); mbar_init(smem_u32(&bar_k_empty), 1);
+    mbar_init(smem_u32(&bar_v_full), 1); mbar_init(smem_u32(&bar_v_empty), 1);
+    mbar_init(smem_u32(&bar_s_full), 1); mbar_init(smem_u32(&bar_s_read), 8); mbar_init(smem_u32(&bar_p_full), 8);
+    mbar_init(smem_u32(&bar_o_full), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&s_tmem_base)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  grid_wait();
+  grid_release();
+  const int quad = warp & 3, r = quad * 32 + lane;         // softmax warps: query row inside the block = TMEM lane
+  int start = INT_MAX;                                     // first key of this thread's row; INT_MAX: it sees none, or is past the end
+  if (warp >= 2) {
+    const int s = row0 + r;
+    if (s < p.S) start = max(p.starts[(long long)b * p.S + s], 0);
+    if (start > s) start = INT_MAX;
+    const int least = __reduce_min_sync(0xffffffffu, start);
+    if (lane == 0 && warp < 6) s_least[quad] = least;
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const int least = min(min(s_least[0], s_least[1]), min(s_least[2], s_least[3]));
+  const int j0 = least == INT_MAX ? 0 : least / BKV;
+  const int nb = least == INT_MAX ? 0 : qi - j0 + 1;       // key blocks j0 .. qi
+  if (p.blocks && h == 0 && threadIdx.x == 0) p.blocks[(long long)b * nQ + qi] = least;
+  const uint32_t tmem_base = s_tmem_base;
+  // S columns 0..127, O from column 128; P over S at DH = 128, at 64 in the 64 columns that O leaves, so that the next block's S is
+  // computed as soon as the softmax warps hold this one's (AHEAD)
+  constexpr bool AHEAD = DH == 64;
+  constexpr int P_HALF = AHEAD ? 32 : 64;                  // columns from one warp's P to the other's
+  const uint32_t tS = tmem_base, tO = tmem_base + 128, tP = AHEAD ? tmem_base + 192 : tmem_base;
+  const uint32_t sQ = smem_u32(smem), sK = sQ + TILE_BYTES, sV = sK + TILE_BYTES;
+
+  if (warp == 0) {
+    const bool leader = elect_one();
+    if (leader && nb > 0) {
+      mbar_expect_tx(smem_u32(&bar_q), TILE_BYTES);
+      load_tile<DH>(sQ, &p.tmQKV, smem_u32(&bar_q), qcol, row0, b);
+    }
+    bool ok = true;
+    int n_k = 0, n_v = 0;                                  // tiles asked for
+    for (int j = 0; j < nb && ok; ++j) {
+      const uint32_t ph = j & 1;
+      const int krow = (j0 + j) * BKV;
+      if (!(ok = mbar_wait_warp(smem_u32(&bar_k_empty), ph ^ 1, abort_flag))) break;
+      if (leader) {
+        mbar_expect_tx(smem_u32(&bar_k_full), TILE_BYTES);
+        load_tile<DH>(sK, &p.tmQKV, smem_u32(&bar_k_full), kcol, krow, b);
+      }
+      ++n_k;
+      if (!(ok = mbar_wait_warp(smem_u32(&bar_v_empty), ph ^ 1, abort_flag))) break;
+      if (leader) {
+        mbar_expect_tx(smem_u32(&bar_v_full), TILE_BYTES);
+        load_tile<DH>(sV, &p.tmQKV, smem_u32(&bar_v_full), vcol, krow, b);
+      }
+      ++n_v;
+    }
+    if (leader) {
+      Drain drain;                                         // no load may land after the CTA has retired: a role may have given up
+      if (nb > 0) drain.wait(smem_u32(&bar_q), 0);
+      if (n_k) drain.wait(smem_u32(&bar_k_full), (uint32_t)((n_k - 1) & 1));
+      if (n_v) drain.wait(smem_u32(&bar_v_full), (uint32_t)((n_v - 1) & 1));
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    const uint32_t id_qk = idesc_mn(128, false, false), id_pv = idesc_mn(DH, false, true);
+    const DescBase bQ = desc_base(sQ, 16, 1024), bK = desc_base(sK, 16, 1024), bV = desc_base(sV, 128 * 128, 1024);
+    auto issue_s = [&](int j) -> bool {                    // S(j) = Q K(j)^T
+      if (!mbar_wait_warp(smem_u32(&bar_k_full), (uint32_t)(j & 1), abort_flag)) return false;
+      tcgen05_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int kk = 0; kk < DH / 16; ++kk) {
+          const uint32_t off = (uint32_t)(kk >> 2) * (128u * 128u / 16u) + (uint32_t)(kk & 3) * 2u;    // 16-byte units
+          umma_bf16_b(tS, bQ, off, bK, off, id_qk, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(smem_u32(&bar_s_full));
+        umma_commit(smem_u32(&bar_k_empty));
+      }
+      return true;
+    };
+    bool ok = nb > 0 && mbar_wait_warp(smem_u32(&bar_q), 0, abort_flag);
+    if (AHEAD && ok) ok = issue_s(0);
+    for (int j = 0; j < nb && ok; ++j) {
+      const uint32_t ph = j & 1;
+      if (!AHEAD) {
+        if (!(ok = issue_s(j))) break;
+      } else if (j + 1 < nb) {
+        if (!(ok = mbar_wait_warp(smem_u32(&bar_s_read), ph, abort_flag))) break;
+        if (!(ok = issue_s(j + 1))) break;
+      }
+      if (!(ok = mbar_wait_warp(smem_u32(&bar_p_full), ph, abort_flag))) break;
+      if (!(ok = mbar_wait_warp(smem_u32(&bar_v_full), ph, abort_flag))) break;
+      tcgen05_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int kk = 0; kk < BKV / 16; ++kk)
+          umma_ts_bf16_b(tO, tP + (kk >> 2) * P_HALF + 8 * (kk & 3), bV, (uint32_t)kk * 128u, id_pv, (j > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(smem_u32(&bar_v_empty));
+        if (j == nb - 1) umma_commit(smem_u32(&bar_o_full));
+      }
+    }
+  } else {
+    const int ch = (warp - 2) >> 2;                        // columns [64 ch, 64 ch + 64) of S, half of O's
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    float m_used = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < nb; ++j) {
+      ok = mbar_wait_warp(smem_u32(&bar_s_full), j & 1, abort_flag);
+      tcgen05_fence_after();
+      const bool diag = j0 + j == qi;
+      const int lo = (start == INT_MAX ? BKV : start - (j0 + j) * BKV) - ch * 64;      // the columns that the row sees; nothing: behind the last
+      const int hi = (diag ? r : BKV - 1) - ch * 64;
+      uint32_t v[64];
+      tmem_ld32_nowait(tS + ch * 64 + lane_off, v);
+      tmem_ld32_nowait(tS + ch * 64 + 32 + lane_off, v + 32);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      behind_wait32(v);
+      behind_wait32(v + 32);
+      if (AHEAD) {
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_s_read));
+      }
+      if (__any_sync(0xffffffffu, lo > 0 || hi < 63)) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e) if (e < lo || e > hi) v[e] = 0xff800000u;         // -inf: exp2 makes it zero
+      }
+      float mx = -INFINITY, mx2 = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 64; e += 4) {
+        mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+        mx2 = max3(mx2, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+      }
+      mx = fmaxf(mx, mx2);
+      if (AHEAD && j > 0 && ok) {            // O and the P columns: the product of block j - 1 has finished with them
+        ok = mbar_wait_warp(smem_u32(&bar_v_empty), (uint32_t)((j - 1) & 1), abort_flag);
+        tcgen05_fence_after();
+      }
+      s_part[j & 1][ch][r] = mx;
+      if (!(ok = pair_agrees(ok, quad))) break;
+      mx = fmaxf(mx, s_part[j & 1][ch ^ 1][r]);
+      const float m_new = fmaxf(m_used, mx * p.scale_log2);
+      const bool need = m_new > m_used + RESCALE_THRESHOLD;       // true for the first block with a key (m_used = -inf)
+      if (__any_sync(0xffffffffu, need)) {
+        const float alpha = need ? exp2f(m_used - m_new) : 1.f;   // 0 for the first block
+        if (need) { m_used = m_new; l *= alpha; }
+        if (j > 0) {
+          // PV of block j - 1 has finished with O: waited for above, or (not AHEAD) S of block j was issued behind it
+#pragma unroll 1
+          for (int c = 0; c < DH / 32; ++c) {
+            uint32_t o[16];
+            const uint32_t at = tO + ch * (DH / 2) + c * 16 + lane_off;
+            tmem_ld16(at, o);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st16(at, o);
+          }
+        }
+      }
+      // a row that has seen no key yet has no maximum, and all its scores here are masked
+      const float m_ref = m_used == -INFINITY ? 0.f : m_used;
+      const unsigned long long sl2x2 = pack_f32x2(__float_as_uint(p.scale_log2), __float_as_uint(p.scale_log2));
+      const unsigned long long negm = pack_f32x2(__float_as_uint(-m_ref), __float_as_uint(-m_ref));
+      unsigned long long sum = 0ull;                       // (0.f, 0.f)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float a0, a1;
+          unpack_f32x2(fma_f32x2(pack_f32x2(v[c * 32 + 2 * e], v[c * 32 + 2 * e + 1]), sl2x2, negm), a0, a1);
+          const float p0 = exp2f(a0), p1 = exp2f(a1);
+          sum = add_f32x2(sum, pack_f32x2(__float_as_uint(p0), __float_as_uint(p1)));
+          const __nv_bfloat162 hh = __floats2bfloat162_rn(p0, p1);
+          pk[e] = *reinterpret_cast<const uint32_t*>(&hh);
+        }
+        tmem_st16(tP + ch * P_HALF + c * 16 + lane_off, pk);
+      }
+      float s0, s1;
+      unpack_f32x2(sum, s0, s1);
+      l += s0 + s1;
+      tmem_wait_st();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_p_full));
+    }
+    // epilogue: O / l -> bf16 -> swizzled staging (the Q tile is no longer read) -> TMA store.  Every wait behind the loop is joined,
+    // and both warps leave it together, so a warp that comes here finds the other.
+    if (ok) {
+      if (nb > 0) ok = mbar_wait_warp(smem_u32(&bar_o_full), 0, abort_flag);
+      s_part[nb & 1][ch][r] = l;
+      ok = pair_agrees(ok, quad);
+    }
+    if (ok) {
+      tcgen05_fence_after();
+      l = s_part[nb & 1][0][r] + s_part[nb & 1][1][r];
+      const bool empty = start == INT_MAX;                 // a row that sees nothing is zero
+      const float inv_l = 1.f / l;
+      const uint32_t stage = sQ + (uint32_t)quad * (32u * DH * 2u) + (DH == 128 ? (uint32_t)ch * 4096u : 0u);
+      const int orow = row0 + quad * 32;
+      const uint32_t sw = (uint32_t)(lane & 7), rowaddr = stage + (uint32_t)lane * 128u;
+#pragma unroll
+      for (int c = 0; c < DH / 64; ++c) {
+        uint32_t o[32];
+        tmem_ld32(tO + ch * (DH / 2) + c * 32 + lane_off, o);
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          uint32_t pw[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const __nv_bfloat162 hh = __floats2bfloat162_rn(__uint_as_float(o[8 * q4 + 2 * e]) * inv_l, __uint_as_float(o[8 * q4 + 2 * e + 1]) * inv_l);
+            pw[e] = empty ? 0u : *reinterpret_cast<const uint32_t*>(&hh);
+          }
+          const uint32_t jj = (uint32_t)((DH == 128 ? c : ch) * 4 + q4);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + ((jj ^ sw) << 4)), "r"(pw[0]), "r"(pw[1]),
+                       "r"(pw[2]), "r"(pw[3]) : "memory");
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (DH == 64) (void)pair_agrees(true, quad);         // one box of 64 columns for both
+      if (lane == 0 && orow < p.S && (DH == 128 || ch == 0)) {
+        tma_store_3d(&p.tmO, stage, qcol + (DH == 128 ? ch * 64 : 0), orow, b);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      }
+      // an infinite sum makes the backward pass's weights of the row zero
+      if (p.lse && ch == 0 && row0 + r < p.S)
+        p.lse[((long long)b * p.H + h) * p.S + row0 + r] = empty ? INFINITY : (m_used + log2f(l)) * 0.6931471805599453f;
+    }
+  }
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem_base) : "memory");
+  }
+  if (threadIdx.x == 0 && s_abort && p.status) atomicOr(p.status, TPLR_ST_WAIT_TIMEOUT);
+}
+
+template <int DH>
+int launch_docs_fwd(const void* qkv, const int* starts, void* out, float* lse, int* blocks, int B, int S, int H, int KV, long long ld_qkv,
+                    long long ld_o, float scale, unsigned int* status, cudaStream_t st) {
+  AttnDocsParams p = {};
+  if (!make_map3(&p.tmQKV, qkv, (long long)(H + 2 * KV) * DH, S, B, ld_qkv, 64, 128)) return -202;
+  if (!make_map3(&p.tmO, out, (long long)H * DH, S, B, ld_o, 64, 32)) return -203;
+  p.lse = lse; p.B = B; p.S = S; p.H = H; p.KV = KV;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.status = status; p.starts = starts; p.blocks = blocks;
+  cudaError_t e = cudaFuncSetAttribute(attn_docs_fwd_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, fwd_smem<DH>());
+  if (e != cudaSuccess) return (int)e;
+  const unsigned grid = (unsigned)(((S + BQ - 1) / BQ) * H * B);
+  return (int)launch_pdl(attn_docs_fwd_kernel<DH>, grid, DOCS_THREADS, fwd_smem<DH>(), st, p);
+}
+}  // namespace
 
 // tplr_attention_fwd within documents: row s of sequence b sees the keys max(starts[b * S + s], 0) .. s; one whose start lies behind it
 // sees nothing, and its output is zero.  starts: [B, S] int32, any values.  blocks: [B, ceil(S / 128)] int32 for the backward
@@ -580,9 +843,9 @@ TPLR_API int tplr_attention_docs_fwd(const void* qkv, const int* starts, void* o
   TPLR_ENTER();
   if (B <= 0 || S <= 0) return 0;
   if (KV <= 0 || H % KV || (ld_qkv % 8) || (ld_o % 8) || ((uintptr_t)qkv & 15) || ((uintptr_t)out & 15) || !starts) return -201;
-  auto run = head_dim == 128 ? launch_fwd<128, true> : launch_fwd<64, true>;
   if (head_dim != 128 && head_dim != 64) return -201;
-  return run(qkv, out, lse, B, S, H, KV, ld_qkv, ld_o, scale, status, (cudaStream_t)stream, starts, blocks);
+  auto run = head_dim == 128 ? launch_docs_fwd<128> : launch_docs_fwd<64>;
+  return run(qkv, starts, out, lse, blocks, B, S, H, KV, ld_qkv, ld_o, scale, status, (cudaStream_t)stream);
 }
 
 // ------------------------------------------------------------------------------------------ //
@@ -1121,6 +1384,43 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const __nv_bfloat16* __
   if (lane == 0 && live) delta[((tok / S) * H + h) * S + tok % S] = s;
 }
 
+// The same for the backward pass within documents, which also zeroes dq32 [tokens, H * DH] on the way: 16 bytes of a row a lane, four
+// rows a thread in flight.
+template <int DH>
+__global__ void __launch_bounds__(256) attn_docs_prepare_kernel(const __nv_bfloat16* o, const __nv_bfloat16* dout, float* delta, float* dq32,
+                                                                long long rows, int S, int H) {
+  constexpr int LANES = DH / 8, GROUPS = 256 / LANES, ROWS = 4;
+  grid_wait();
+  grid_release();
+  const int lane = threadIdx.x % LANES;
+  const long long first = (long long)blockIdx.x * (GROUPS * ROWS) + threadIdx.x / LANES;
+  uint4 a[ROWS], d[ROWS];
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    const long long at = min(first + k * GROUPS, rows - 1) * DH + lane * 8;
+    a[k] = *reinterpret_cast<const uint4*>(o + at);
+    d[k] = *reinterpret_cast<const uint4*>(dout + at);
+  }
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    const long long row = first + k * GROUPS;
+    const uint32_t x[4] = {a[k].x, a[k].y, a[k].z, a[k].w}, y[4] = {d[k].x, d[k].y, d[k].z, d[k].w};
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s = fmaf(__uint_as_float(x[e] << 16), __uint_as_float(y[e] << 16), s);
+      s = fmaf(__uint_as_float(x[e] & 0xffff0000u), __uint_as_float(y[e] & 0xffff0000u), s);
+    }
+#pragma unroll
+    for (int m = LANES / 2; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+    if (row >= rows) break;                          // the same for the lanes of a row; rows grow with k
+    float4* q = reinterpret_cast<float4*>(dq32 + row * DH + lane * 8);
+    q[0] = q[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const long long tok = row / H;
+    if (lane == 0) delta[((tok / S) * H + row % H) * S + tok % S] = s;
+  }
+}
+
 // dq32 [tokens, q_cols] fp32 -> first q_cols columns (heads of HD) of the packed bf16 gradient, eight values a thread; PARTS: the
 // next kv_cols columns (dK | dV of a split walk) are the sums, in order, of `split` parts in part [tokens, split, kv_cols].
 // cosb / sinb not null: the pairs are rotated back, in the first rot_cols columns, by the angles of (token % S, pair index in the
@@ -1556,7 +1856,12 @@ int launch_bwd(const void* qkv, const void* out, const void* dout, const float* 
                unsigned int* status, cudaStream_t st, bool delta_ready, const int* starts = nullptr, const int* blocks = nullptr) {
   const long long tokens = (long long)B * S;
   const int C = (H + 2 * KV) * HD;
-  if (!delta_ready) {
+  if (DOCS) {
+    const long long rows = tokens * H, per_cta = 4 * 256 / (HD / 8);
+    const cudaError_t e = launch_pdl(attn_docs_prepare_kernel<HD>, (unsigned)((rows + per_cta - 1) / per_cta), 256, 0, st,
+                                     (const __nv_bfloat16*)out, (const __nv_bfloat16*)dout, delta, dq32, rows, S, H);
+    if (e != cudaSuccess) return (int)e;
+  } else if (!delta_ready) {
     constexpr int per_cta = 256 / (HD / 4);
     attn_delta_kernel<HD><<<(unsigned)((tokens * H + per_cta - 1) / per_cta), 256, 0, st>>>(
         (const __nv_bfloat16*)out, (const __nv_bfloat16*)dout, delta, tokens, S, H, ld_o);
@@ -1672,22 +1977,22 @@ TPLR_API int tplr_attention_bwd_unrope_delta(const void* qkv, const void* out, c
                             true);
 }
 
-// Fp32 elements per token of the scratch that tplr_attention_docs_bwd needs, laid out as tplr_attention_bwd's.
+// Fp32 elements per token of the scratch that tplr_attention_docs_bwd needs, contents irrelevant.
 TPLR_API int tplr_attention_docs_bwd_scratch_cols(int B, int S, int H, int KV, int head_dim) {
   const int split = bwd_split_walk(B, S, H, KV);
   return (H + (split > 1 ? 2 * KV * split : 0)) * head_dim;
 }
 
-// Gradient of tplr_attention_docs_fwd, whose starts and blocks it takes; otherwise as tplr_attention_bwd.
+// Gradient of tplr_attention_docs_fwd, whose starts and blocks it takes; out and dout dense, otherwise as tplr_attention_bwd.
 TPLR_API int tplr_attention_docs_bwd(const void* qkv, const int* starts, const int* blocks, const void* out, const void* dout,
                                      const float* lse, float* delta, float* dq32, void* dqkv, int B, int S, int H, int KV, int head_dim,
-                                     long long ld_qkv, long long ld_o, float scale, unsigned int* status, void* stream) {
+                                     long long ld_qkv, float scale, unsigned int* status, void* stream) {
   TPLR_ENTER();
   if (B <= 0 || S <= 0) return 0;
-  if ((head_dim != 128 && head_dim != 64) || KV <= 0 || H % KV || (ld_qkv % 8) || (ld_o % 8) || ((uintptr_t)qkv & 15) || !starts || !blocks ||
-      ((uintptr_t)dqkv & 15) || ((uintptr_t)dout & 15) || ((uintptr_t)out & 7) || ((uintptr_t)dq32 & 15))
+  if ((head_dim != 128 && head_dim != 64) || KV <= 0 || H % KV || (ld_qkv % 8) || ((uintptr_t)qkv & 15) || !starts || !blocks ||
+      ((uintptr_t)dqkv & 15) || ((uintptr_t)dout & 15) || ((uintptr_t)out & 15) || ((uintptr_t)dq32 & 15))
     return -201;
   auto run = head_dim == 128 ? launch_bwd<128, true> : launch_bwd<64, true>;
-  return run(qkv, out, dout, lse, delta, dq32, dqkv, B, S, H, KV, ld_qkv, ld_o, scale, nullptr, nullptr, status, (cudaStream_t)stream,
-             false, starts, blocks);
+  return run(qkv, out, dout, lse, delta, dq32, dqkv, B, S, H, KV, ld_qkv, (long long)H * head_dim, scale, nullptr, nullptr, status,
+             (cudaStream_t)stream, false, starts, blocks);
 }

@@ -88,11 +88,10 @@ class _AttentionDocuments(torch.autograd.Function):
             dqkv = torch.empty(B, S, ld, dtype=qkv.dtype, device=qkv.device)[..., :C]
             cols = native.lib().tplr_attention_docs_bwd_scratch_cols(B, S, n_heads, n_kv, hd)
             dq32 = torch.empty(B * S * cols, dtype=torch.float32, device=qkv.device)
-            dq32[:B * S * n_heads * hd].zero_()
             delta = torch.empty(B, n_heads, S, dtype=torch.float32, device=qkv.device)
             native.check(native.lib().tplr_attention_docs_bwd(
                 qkv.data_ptr(), starts.data_ptr(), blocks.data_ptr(), out.data_ptr(), do.data_ptr(), lse.data_ptr(), delta.data_ptr(),
-                dq32.data_ptr(), dqkv.data_ptr(), B, S, n_heads, n_kv, hd, ld, out.stride(1), hd ** -0.5,
+                dq32.data_ptr(), dqkv.data_ptr(), B, S, n_heads, n_kv, hd, ld, hd ** -0.5,
                 OF.status_word(qkv.device).data_ptr(), native.stream_ptr()), "attention_docs_bwd")
         return dqkv, None, None, None, None
 

@@ -117,10 +117,13 @@ def test_whole_sequences_match_the_causal_kernels(hd):
     dout = normal(g, 2, 515, 4 * hd)
     a = OF._AttentionPacked.apply(qkv, 4, 1, hd)
     b = ops.attention_documents(qkv, torch.zeros(2, 515, dtype=torch.int64, device=DEV), 4, 1, hd)
-    assert torch.equal(a, b)
     (da,), (db,) = torch.autograd.grad(a, qkv, dout), torch.autograd.grad(b, qkv, dout)
-    assert torch.equal(da[..., 4 * hd:], db[..., 4 * hd:])
-    torch.testing.assert_close(da.float(), db.float(), rtol=2 * U, atol=1e-6)      # dq is added up in any order: one step of bf16
+    # the two add a row's weights, and dout * out, in another order: sums 2^-22 apart, which turn few of the roundings to bf16 over, each by a
+    # step of 2 U of its value
+    for x, y in ((a, b), (da, db)):
+        x, y = x.detach().float(), y.detach().float()
+        assert (x - y).norm() <= U / 4 * x.norm()
+        assert ((x - y).abs() > 2 * U * x.abs() + 2 * U * x.abs().mean()).sum() == 0
 
 
 @pytest.mark.parametrize("hd", [64, 128])
