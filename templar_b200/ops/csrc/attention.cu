@@ -510,345 +510,6 @@ TPLR_API int tplr_attention_fwd(const void* qkv, void* out, float* lse, int B, i
 }
 
 // ------------------------------------------------------------------------------------------ //
-// Forward within documents: row s of a sequence sees the keys max(starts[s], 0) .. s.  A CTA has a query block of one head as above and
-// walks the key blocks from that of its rows' least start to the diagonal; a block that all rows of a warp see whole runs without
-// a mask.  Eight softmax warps, two a quadrant of tensor memory with half of a row's columns each: what bounds a block is the
-// chain from S over the exponentials to the product with V, and a row of 128 in one thread is the longest part of it.  The two
-// exchange their maxima through shared memory, join their waits in the same barrier (a warp that gave up takes the other one
-// along), and keep sums of their own to the end.  P lies in the S columns of the warp that makes it, at DH = 64 in columns of its own.
-// ------------------------------------------------------------------------------------------ //
-namespace {
-
-constexpr int DOCS_THREADS = 320;
-
-struct AttnDocsParams {
-  CUtensorMap tmQKV;      // as in the forward kernel above
-  CUtensorMap tmO;
-  float* lse;
-  int B, S, H, KV;
-  float scale_log2;
-  unsigned int* status;
-  const int* starts;      // [B, S]
-  int* blocks;            // [B, nQ], or null: takes the least start of a row in the query block that sees anything (INT_MAX: none does)
-};
-
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr) : "memory");
-}
-// Both warps of a quadrant come here with an answer and leave with the joint one.
-__device__ __forceinline__ bool pair_agrees(bool ok, int quad) {
-  uint32_t both;
-  asm volatile("{\n\t.reg .pred mine, all;\n\tsetp.ne.u32 mine, %2, 0;\n\tbar.red.and.pred all, %1, 64, mine;\n\tselp.u32 %0, 1, 0, all;\n\t}"
-               : "=r"(both) : "r"(quad + 1), "r"((uint32_t)ok) : "memory");
-  return both != 0;
-}
-
-template <int DH>
-__global__ void __launch_bounds__(DOCS_THREADS, 2)
-attn_docs_fwd_kernel(const __grid_constant__ AttnDocsParams p) {
-  constexpr int TILE_BYTES = tile_bytes<DH>();
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t bar_q, bar_k_full, bar_k_empty, bar_v_full, bar_v_empty, bar_s_full, bar_s_read, bar_p_full, bar_o_full;
-  __shared__ uint32_t s_tmem_base;
-  __shared__ int s_abort;
-  __shared__ int s_least[4];
-  __shared__ float s_part[2][2][128];                      // [block parity][column half][row]: maxima, at the end sums
-
-  const int warp = warp_index(), lane = threadIdx.x & 31;
-  const int nQ = (p.S + BQ - 1) / BQ;
-  const int hb = p.H * p.B;
-  const int qi = nQ - 1 - (int)(blockIdx.x / hb);          // late query blocks first: they may see the most
-  const int h = (int)(blockIdx.x % hb) % p.H, b = (int)(blockIdx.x % hb) / p.H;
-  const int g = h / (p.H / p.KV);
-  const int row0 = qi * BQ;
-  const int qcol = h * DH, kcol = (p.H + g) * DH, vcol = (p.H + p.KV + g) * DH;
-  volatile int* abort_flag = &s_abort;
-
-  if (threadIdx.x == 0) {
-    s_abort = 0;
-    mbar_init(smem_u32(&bar_q), 1);
-    mbar_init(smem_u32(&bar_k_full), 1); mbar_init(smem_u32(&bar_k_empty), 1);
-    mbar_init(smem_u32(&bar_v_full), 1); mbar_init(smem_u32(&bar_v_empty), 1);
-    mbar_init(smem_u32(&bar_s_full), 1); mbar_init(smem_u32(&bar_s_read), 8); mbar_init(smem_u32(&bar_p_full), 8);
-    mbar_init(smem_u32(&bar_o_full), 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&s_tmem_base)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  grid_wait();
-  grid_release();
-  const int quad = warp & 3, r = quad * 32 + lane;         // softmax warps: query row inside the block = TMEM lane
-  int start = INT_MAX;                                     // first key of this thread's row; INT_MAX: it sees none, or is past the end
-  if (warp >= 2) {
-    const int s = row0 + r;
-    if (s < p.S) start = max(p.starts[(long long)b * p.S + s], 0);
-    if (start > s) start = INT_MAX;
-    const int least = __reduce_min_sync(0xffffffffu, start);
-    if (lane == 0 && warp < 6) s_least[quad] = least;
-  }
-  tcgen05_fence_before();
-  __syncthreads();
-  tcgen05_fence_after();
-  const int least = min(min(s_least[0], s_least[1]), min(s_least[2], s_least[3]));
-  const int j0 = least == INT_MAX ? 0 : least / BKV;
-  const int nb = least == INT_MAX ? 0 : qi - j0 + 1;       // key blocks j0 .. qi
-  if (p.blocks && h == 0 && threadIdx.x == 0) p.blocks[(long long)b * nQ + qi] = least;
-  const uint32_t tmem_base = s_tmem_base;
-  // S columns 0..127, O from column 128; P over S at DH = 128, at 64 in the 64 columns that O leaves, so that the next block's S is
-  // computed as soon as the softmax warps hold this one's (AHEAD)
-  constexpr bool AHEAD = DH == 64;
-  constexpr int P_HALF = AHEAD ? 32 : 64;                  // columns from one warp's P to the other's
-  const uint32_t tS = tmem_base, tO = tmem_base + 128, tP = AHEAD ? tmem_base + 192 : tmem_base;
-  const uint32_t sQ = smem_u32(smem), sK = sQ + TILE_BYTES, sV = sK + TILE_BYTES;
-
-  if (warp == 0) {
-    const bool leader = elect_one();
-    if (leader && nb > 0) {
-      mbar_expect_tx(smem_u32(&bar_q), TILE_BYTES);
-      load_tile<DH>(sQ, &p.tmQKV, smem_u32(&bar_q), qcol, row0, b);
-    }
-    bool ok = true;
-    int n_k = 0, n_v = 0;                                  // tiles asked for
-    for (int j = 0; j < nb && ok; ++j) {
-      const uint32_t ph = j & 1;
-      const int krow = (j0 + j) * BKV;
-      if (!(ok = mbar_wait_warp(smem_u32(&bar_k_empty), ph ^ 1, abort_flag))) break;
-      if (leader) {
-        mbar_expect_tx(smem_u32(&bar_k_full), TILE_BYTES);
-        load_tile<DH>(sK, &p.tmQKV, smem_u32(&bar_k_full), kcol, krow, b);
-      }
-      ++n_k;
-      if (!(ok = mbar_wait_warp(smem_u32(&bar_v_empty), ph ^ 1, abort_flag))) break;
-      if (leader) {
-        mbar_expect_tx(smem_u32(&bar_v_full), TILE_BYTES);
-        load_tile<DH>(sV, &p.tmQKV, smem_u32(&bar_v_full), vcol, krow, b);
-      }
-      ++n_v;
-    }
-    if (leader) {
-      Drain drain;                                         // no load may land after the CTA has retired: a role may have given up
-      if (nb > 0) drain.wait(smem_u32(&bar_q), 0);
-      if (n_k) drain.wait(smem_u32(&bar_k_full), (uint32_t)((n_k - 1) & 1));
-      if (n_v) drain.wait(smem_u32(&bar_v_full), (uint32_t)((n_v - 1) & 1));
-    }
-  } else if (warp == 1) {
-    const bool leader = elect_one();
-    const uint32_t id_qk = idesc_mn(128, false, false), id_pv = idesc_mn(DH, false, true);
-    const DescBase bQ = desc_base(sQ, 16, 1024), bK = desc_base(sK, 16, 1024), bV = desc_base(sV, 128 * 128, 1024);
-    auto issue_s = [&](int j) -> bool {                    // S(j) = Q K(j)^T
-      if (!mbar_wait_warp(smem_u32(&bar_k_full), (uint32_t)(j & 1), abort_flag)) return false;
-      tcgen05_fence_after();
-      if (leader) {
-#pragma unroll
-        for (int kk = 0; kk < DH / 16; ++kk) {
-          const uint32_t off = (uint32_t)(kk >> 2) * (128u * 128u / 16u) + (uint32_t)(kk & 3) * 2u;    // 16-byte units
-          umma_bf16_b(tS, bQ, off, bK, off, id_qk, kk > 0 ? 1u : 0u);
-        }
-        umma_commit(smem_u32(&bar_s_full));
-        umma_commit(smem_u32(&bar_k_empty));
-      }
-      return true;
-    };
-    bool ok = nb > 0 && mbar_wait_warp(smem_u32(&bar_q), 0, abort_flag);
-    if (AHEAD && ok) ok = issue_s(0);
-    for (int j = 0; j < nb && ok; ++j) {
-      const uint32_t ph = j & 1;
-      if (!AHEAD) {
-        if (!(ok = issue_s(j))) break;
-      } else if (j + 1 < nb) {
-        if (!(ok = mbar_wait_warp(smem_u32(&bar_s_read), ph, abort_flag))) break;
-        if (!(ok = issue_s(j + 1))) break;
-      }
-      if (!(ok = mbar_wait_warp(smem_u32(&bar_p_full), ph, abort_flag))) break;
-      if (!(ok = mbar_wait_warp(smem_u32(&bar_v_full), ph, abort_flag))) break;
-      tcgen05_fence_after();
-      if (leader) {
-#pragma unroll
-        for (int kk = 0; kk < BKV / 16; ++kk)
-          umma_ts_bf16_b(tO, tP + (kk >> 2) * P_HALF + 8 * (kk & 3), bV, (uint32_t)kk * 128u, id_pv, (j > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(smem_u32(&bar_v_empty));
-        if (j == nb - 1) umma_commit(smem_u32(&bar_o_full));
-      }
-    }
-  } else {
-    const int ch = (warp - 2) >> 2;                        // columns [64 ch, 64 ch + 64) of S, half of O's
-    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-    float m_used = -INFINITY, l = 0.f;
-    bool ok = true;
-    for (int j = 0; j < nb; ++j) {
-      ok = mbar_wait_warp(smem_u32(&bar_s_full), j & 1, abort_flag);
-      tcgen05_fence_after();
-      const bool diag = j0 + j == qi;
-      const int lo = (start == INT_MAX ? BKV : start - (j0 + j) * BKV) - ch * 64;      // the columns that the row sees; nothing: behind the last
-      const int hi = (diag ? r : BKV - 1) - ch * 64;
-      uint32_t v[64];
-      tmem_ld32_nowait(tS + ch * 64 + lane_off, v);
-      tmem_ld32_nowait(tS + ch * 64 + 32 + lane_off, v + 32);
-      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      behind_wait32(v);
-      behind_wait32(v + 32);
-      if (AHEAD) {
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_s_read));
-      }
-      if (__any_sync(0xffffffffu, lo > 0 || hi < 63)) {
-#pragma unroll
-        for (int e = 0; e < 64; ++e) if (e < lo || e > hi) v[e] = 0xff800000u;         // -inf: exp2 makes it zero
-      }
-      float mx = -INFINITY, mx2 = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 64; e += 4) {
-        mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-        mx2 = max3(mx2, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
-      }
-      mx = fmaxf(mx, mx2);
-      if (AHEAD && j > 0 && ok) {            // O and the P columns: the product of block j - 1 has finished with them
-        ok = mbar_wait_warp(smem_u32(&bar_v_empty), (uint32_t)((j - 1) & 1), abort_flag);
-        tcgen05_fence_after();
-      }
-      s_part[j & 1][ch][r] = mx;
-      if (!(ok = pair_agrees(ok, quad))) break;
-      mx = fmaxf(mx, s_part[j & 1][ch ^ 1][r]);
-      const float m_new = fmaxf(m_used, mx * p.scale_log2);
-      const bool need = m_new > m_used + RESCALE_THRESHOLD;       // true for the first block with a key (m_used = -inf)
-      if (__any_sync(0xffffffffu, need)) {
-        const float alpha = need ? exp2f(m_used - m_new) : 1.f;   // 0 for the first block
-        if (need) { m_used = m_new; l *= alpha; }
-        if (j > 0) {
-          // PV of block j - 1 has finished with O: waited for above, or (not AHEAD) S of block j was issued behind it
-#pragma unroll 1
-          for (int c = 0; c < DH / 32; ++c) {
-            uint32_t o[16];
-            const uint32_t at = tO + ch * (DH / 2) + c * 16 + lane_off;
-            tmem_ld16(at, o);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st16(at, o);
-          }
-        }
-      }
-      // a row that has seen no key yet has no maximum, and all its scores here are masked
-      const float m_ref = m_used == -INFINITY ? 0.f : m_used;
-      const unsigned long long sl2x2 = pack_f32x2(__float_as_uint(p.scale_log2), __float_as_uint(p.scale_log2));
-      const unsigned long long negm = pack_f32x2(__float_as_uint(-m_ref), __float_as_uint(-m_ref));
-      unsigned long long sum = 0ull;                       // (0.f, 0.f)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float a0, a1;
-          unpack_f32x2(fma_f32x2(pack_f32x2(v[c * 32 + 2 * e], v[c * 32 + 2 * e + 1]), sl2x2, negm), a0, a1);
-          const float p0 = exp2f(a0), p1 = exp2f(a1);
-          sum = add_f32x2(sum, pack_f32x2(__float_as_uint(p0), __float_as_uint(p1)));
-          const __nv_bfloat162 hh = __floats2bfloat162_rn(p0, p1);
-          pk[e] = *reinterpret_cast<const uint32_t*>(&hh);
-        }
-        tmem_st16(tP + ch * P_HALF + c * 16 + lane_off, pk);
-      }
-      float s0, s1;
-      unpack_f32x2(sum, s0, s1);
-      l += s0 + s1;
-      tmem_wait_st();
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_p_full));
-    }
-    // epilogue: O / l -> bf16 -> swizzled staging (the Q tile is no longer read) -> TMA store.  Every wait behind the loop is joined,
-    // and both warps leave it together, so a warp that comes here finds the other.
-    if (ok) {
-      if (nb > 0) ok = mbar_wait_warp(smem_u32(&bar_o_full), 0, abort_flag);
-      s_part[nb & 1][ch][r] = l;
-      ok = pair_agrees(ok, quad);
-    }
-    if (ok) {
-      tcgen05_fence_after();
-      l = s_part[nb & 1][0][r] + s_part[nb & 1][1][r];
-      const bool empty = start == INT_MAX;                 // a row that sees nothing is zero
-      const float inv_l = 1.f / l;
-      const uint32_t stage = sQ + (uint32_t)quad * (32u * DH * 2u) + (DH == 128 ? (uint32_t)ch * 4096u : 0u);
-      const int orow = row0 + quad * 32;
-      const uint32_t sw = (uint32_t)(lane & 7), rowaddr = stage + (uint32_t)lane * 128u;
-#pragma unroll
-      for (int c = 0; c < DH / 64; ++c) {
-        uint32_t o[32];
-        tmem_ld32(tO + ch * (DH / 2) + c * 32 + lane_off, o);
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          uint32_t pw[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const __nv_bfloat162 hh = __floats2bfloat162_rn(__uint_as_float(o[8 * q4 + 2 * e]) * inv_l, __uint_as_float(o[8 * q4 + 2 * e + 1]) * inv_l);
-            pw[e] = empty ? 0u : *reinterpret_cast<const uint32_t*>(&hh);
-          }
-          const uint32_t jj = (uint32_t)((DH == 128 ? c : ch) * 4 + q4);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + ((jj ^ sw) << 4)), "r"(pw[0]), "r"(pw[1]),
-                       "r"(pw[2]), "r"(pw[3]) : "memory");
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (DH == 64) (void)pair_agrees(true, quad);         // one box of 64 columns for both
-      if (lane == 0 && orow < p.S && (DH == 128 || ch == 0)) {
-        tma_store_3d(&p.tmO, stage, qcol + (DH == 128 ? ch * 64 : 0), orow, b);
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-      }
-      // an infinite sum makes the backward pass's weights of the row zero
-      if (p.lse && ch == 0 && row0 + r < p.S)
-        p.lse[((long long)b * p.H + h) * p.S + row0 + r] = empty ? INFINITY : (m_used + log2f(l)) * 0.6931471805599453f;
-    }
-  }
-  __syncwarp();
-  tcgen05_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tcgen05_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem_base) : "memory");
-  }
-  if (threadIdx.x == 0 && s_abort && p.status) atomicOr(p.status, TPLR_ST_WAIT_TIMEOUT);
-}
-
-template <int DH>
-int launch_docs_fwd(const void* qkv, const int* starts, void* out, float* lse, int* blocks, int B, int S, int H, int KV, long long ld_qkv,
-                    long long ld_o, float scale, unsigned int* status, cudaStream_t st) {
-  AttnDocsParams p = {};
-  if (!make_map3(&p.tmQKV, qkv, (long long)(H + 2 * KV) * DH, S, B, ld_qkv, 64, 128)) return -202;
-  if (!make_map3(&p.tmO, out, (long long)H * DH, S, B, ld_o, 64, 32)) return -203;
-  p.lse = lse; p.B = B; p.S = S; p.H = H; p.KV = KV;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  p.status = status; p.starts = starts; p.blocks = blocks;
-  cudaError_t e = cudaFuncSetAttribute(attn_docs_fwd_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, fwd_smem<DH>());
-  if (e != cudaSuccess) return (int)e;
-  const unsigned grid = (unsigned)(((S + BQ - 1) / BQ) * H * B);
-  return (int)launch_pdl(attn_docs_fwd_kernel<DH>, grid, DOCS_THREADS, fwd_smem<DH>(), st, p);
-}
-}  // namespace
-
-// tplr_attention_fwd within documents: row s of sequence b sees the keys max(starts[b * S + s], 0) .. s; one whose start lies behind it
-// sees nothing, and its output is zero.  starts: [B, S] int32, any values.  blocks: [B, ceil(S / 128)] int32 for the backward
-// pass, or null.
-TPLR_API int tplr_attention_docs_fwd(const void* qkv, const int* starts, void* out, float* lse, int* blocks, int B, int S, int H, int KV,
-                                     int head_dim, long long ld_qkv, long long ld_o, float scale, unsigned int* status, void* stream) {
-  TPLR_ENTER();
-  if (B <= 0 || S <= 0) return 0;
-  if (KV <= 0 || H % KV || (ld_qkv % 8) || (ld_o % 8) || ((uintptr_t)qkv & 15) || ((uintptr_t)out & 15) || !starts) return -201;
-  if (head_dim != 128 && head_dim != 64) return -201;
-  auto run = head_dim == 128 ? launch_docs_fwd<128> : launch_docs_fwd<64>;
-  return run(qkv, starts, out, lse, blocks, B, S, H, KV, ld_qkv, ld_o, scale, status, (cudaStream_t)stream);
-}
-
-// ------------------------------------------------------------------------------------------ //
 // Backward.  CTA = one 128-row key/value block of one kv head and the query heads of its group, or a part of them; it
 // walks those heads and the query blocks at or below the diagonal.  Per step:
 //   S = Q K^T, dP = dO V^T            (tensor cores -> TMEM)
@@ -893,8 +554,6 @@ struct AttnBwdParams {
   // the gradient is wanted with respect to the un-rotated projection: dK is rotated back in the epilogue
   const float* rope_cos;
   const float* rope_sin;
-  const int* starts;    // documents: as in the forward kernel, which left `blocks`
-  const int* blocks;
 };
 
 __device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
@@ -906,7 +565,7 @@ __device__ __forceinline__ void tma_reduce_add_3d(const CUtensorMap* map, uint32
                ::"l"(map), "r"(src), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
-template <int DH, bool DOCS>
+template <int DH>
 __global__ void __launch_bounds__(bwd_threads<DH>(), 1)
 attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
   constexpr int TILE_BYTES = tile_bytes<DH>();
@@ -916,7 +575,6 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
       bar_p_ready, bar_ds_ready, bar_dq_full, bar_dq_free;
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
-  __shared__ int s_last;                                   // documents: the last query block that sees any key of this block
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int nQ = (p.S + BQ - 1) / BQ;
@@ -926,14 +584,14 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
   const int g = (int)(blockIdx.x % gb) / p.split % p.KV, b = (int)(blockIdx.x % gb) / p.split / p.KV;
   const int heads = p.H / p.KV / p.split;                  // query heads of this CTA
   const int h0 = (g * p.split + sub) * heads;
-  int n_i = nQ - j, n_it = heads * n_i;                    // query blocks j .. j + n_i - 1; causal: to the last
+  const int n_i = nQ - j;                                  // query blocks j..nQ-1
+  const int n_it = heads * n_i;
   const int kvrow0 = j * BKV;                              // position of the first key row; rows past S read as zeros
   const int kcol = (p.H + g) * DH, vcol = (p.H + p.KV + g) * DH;
   volatile int* abort_flag = &s_abort;
 
   if (threadIdx.x == 0) {
     s_abort = 0;
-    s_last = -1;
     mbar_init(smem_u32(&bar_kv), 1);
     for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&bar_q_full[s]), 1); mbar_init(smem_u32(&bar_q_empty[s]), 1); }
     mbar_init(smem_u32(&bar_do_full), 1); mbar_init(smem_u32(&bar_do_empty), 1);
@@ -952,17 +610,6 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
   tcgen05_fence_after();
   grid_wait();
   grid_release();
-  if constexpr (DOCS) {
-    // a block in between whose rows begin behind this one is walked with all its weights masked: starts that grow with the
-    // row, as documents' do, have none
-    int last = -1;
-    for (int i = j + (int)threadIdx.x; i < nQ; i += bwd_threads<DH>())
-      if (p.blocks[(long long)b * nQ + i] < kvrow0 + BKV) last = i;
-    if (last >= 0) atomicMax(&s_last, last);
-    __syncthreads();
-    n_i = max(s_last - j + 1, 0);
-    n_it = heads * n_i;
-  }
   const uint32_t tmem_base = s_tmem_base;
   // dQ of a step lies over its dP at DH = 128; at 64 it has columns of its own
   const uint32_t tS = tmem_base, tdP = tmem_base + 128, tdV = tmem_base + 256, tdK = tmem_base + 256 + DH, tdQ = DH == 64 ? tmem_base + 384 : tdP;
@@ -1031,7 +678,7 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
         for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(tdP, kdO, TPLR_KOFF(kk), kV, TPLR_KOFF(kk), id_kk, kk > 0 ? 1u : 0u);
         umma_commit(smem_u32(&bar_dp_full));
       };
-      bool ok = (!DOCS || n_it > 0) && mbar_wait_warp(smem_u32(&bar_kv), 0, abort_flag);
+      bool ok = mbar_wait_warp(smem_u32(&bar_kv), 0, abort_flag);
       if (ok) ok = mbar_wait_warp(smem_u32(&bar_q_full[0]), 0, abort_flag);
       if (ok) { tcgen05_fence_after(); issue_s(0); }
       if (ok) ok = mbar_wait_warp(smem_u32(&bar_do_full), 0, abort_flag);
@@ -1127,13 +774,12 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
     const uint32_t prow = sP + (uint32_t)ch * (PT_BYTES / 2) + (uint32_t)r * 128u;
     const uint32_t drow = sdS + (uint32_t)ch * (PT_BYTES / 2) + (uint32_t)r * 128u;
     // the row statistics of step t; a query row past the end of the sequence has no weight: lse = +inf makes its P zero
-    auto stats = [&](int t, float& lse2, float& dl, int& st) {
+    auto stats = [&](int t, float& lse2, float& dl) {
       const int h = h0 + t / n_i, row = (j + t % n_i) * BQ + r;
       const long long at = ((long long)b * p.H + h) * p.S + row;
       const bool live = row < p.S;
       lse2 = live ? p.lse[at] : INFINITY;
       dl = live ? p.delta[at] : 0.f;
-      if (DOCS) st = live ? max(p.starts[(long long)b * p.S + row], 0) : 0;
     };
     // DH = 128: dQ of step tt (fp32 in tensor memory) into the global fp32 dQ with TMA reduce-add: one group of copies for each box
     auto drain = [&](int tt) -> bool {
@@ -1164,23 +810,21 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
       }
       return true;
     };
-    float lse_n = 0.f, dl_n = 0.f;
-    int st_n = 0;
-    if (!DOCS || n_it > 0) stats(0, lse_n, dl_n, st_n);
+    float lse_n, dl_n;
+    stats(0, lse_n, dl_n);
     bool ok = true;
     for (int t = 0; t < n_it && ok; ++t) {
       const int i = j + t % n_i;
       const float lse2 = lse_n * 1.4426950408889634f, dls = dl_n * p.scale;
-      const int lo = DOCS ? st_n - kvrow0 : 0;               // documents: first column of this block that the row sees
-      if (t + 1 < n_it) stats(t + 1, lse_n, dl_n, st_n);     // in flight during this step
+      if (t + 1 < n_it) stats(t + 1, lse_n, dl_n);           // in flight during this step
       ok = mbar_wait(smem_u32(&bar_s_full), t & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tcgen05_fence_after();
       // P of this warp's 64 columns, kept in fp32 for dS; the diagonal block runs the variant with the causal mask
       float pv[64];
-      auto exp_part = [&](auto DIAG, auto LOW) {
-        constexpr bool kDiag = decltype(DIAG)::value, kLow = decltype(LOW)::value;
+      auto exp_part = [&](auto DIAG) {
+        constexpr bool kDiag = decltype(DIAG)::value;
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
           uint32_t sv[32];
@@ -1189,16 +833,11 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
           for (int e = 0; e < 32; ++e) {
             float x = exp2f(fmaf(__uint_as_float(sv[e]), p.scale_log2, -lse2));
             if (kDiag && ch * 64 + cc * 32 + e > r) x = 0.f;
-            if (kLow && ch * 64 + cc * 32 + e < lo) x = 0.f;
             pv[cc * 32 + e] = x;
           }
         }
       };
-      using yes = cuda::std::true_type;
-      using no = cuda::std::false_type;
-      if (DOCS && __any_sync(0xffffffffu, lo > 0)) { if (i == j) exp_part(yes{}, yes{}); else exp_part(no{}, yes{}); }
-      else if (i == j) exp_part(yes{}, no{});
-      else exp_part(no{}, no{});
+      if (i == j) exp_part(cuda::std::true_type{}); else exp_part(cuda::std::false_type{});
       if (t > 0) {
         if constexpr (DH == 128) {
           // dQ of the step before: its products ran while this step's exponentials were taken.  Its last commit covers every
@@ -1278,10 +917,6 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
           __syncwarp();
           uint32_t v[32];
           tmem_ld32((acc ? tdK : tdV) + col + lane_off, v);
-          if (DOCS && n_it == 0) {                       // keys that no row sees
-#pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = 0u;
-          }
           const uint32_t rowaddr = buf + (uint32_t)lane * 128u;
 #pragma unroll
           for (int q8 = 0; q8 < 8; ++q8)
@@ -1308,10 +943,6 @@ attn_bwd_kernel(const __grid_constant__ AttnBwdParams p) {
           for (int hf = 0; hf < 2; ++hf) {
             uint32_t v[32];
             tmem_ld32(tacc + col + hf * 32 + lane_off, v);
-            if (DOCS && n_it == 0) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = 0u;
-            }
             if (acc == 1 && p.rope_cos) {          // dK back through the rotation of this key row: the opposite angle
               const long long tb = (long long)min(orow0 + lane, p.S - 1) * (DH / 2) + (col + hf * 32) / 2;
               const float4* cp = reinterpret_cast<const float4*>(p.rope_cos + tb);
@@ -1382,43 +1013,6 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const __nv_bfloat16* __
 #pragma unroll
   for (int k = LANES / 2; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
   if (lane == 0 && live) delta[((tok / S) * H + h) * S + tok % S] = s;
-}
-
-// The same for the backward pass within documents, which also zeroes dq32 [tokens, H * DH] on the way: 16 bytes of a row a lane, four
-// rows a thread in flight.
-template <int DH>
-__global__ void __launch_bounds__(256) attn_docs_prepare_kernel(const __nv_bfloat16* o, const __nv_bfloat16* dout, float* delta, float* dq32,
-                                                                long long rows, int S, int H) {
-  constexpr int LANES = DH / 8, GROUPS = 256 / LANES, ROWS = 4;
-  grid_wait();
-  grid_release();
-  const int lane = threadIdx.x % LANES;
-  const long long first = (long long)blockIdx.x * (GROUPS * ROWS) + threadIdx.x / LANES;
-  uint4 a[ROWS], d[ROWS];
-#pragma unroll
-  for (int k = 0; k < ROWS; ++k) {
-    const long long at = min(first + k * GROUPS, rows - 1) * DH + lane * 8;
-    a[k] = *reinterpret_cast<const uint4*>(o + at);
-    d[k] = *reinterpret_cast<const uint4*>(dout + at);
-  }
-#pragma unroll
-  for (int k = 0; k < ROWS; ++k) {
-    const long long row = first + k * GROUPS;
-    const uint32_t x[4] = {a[k].x, a[k].y, a[k].z, a[k].w}, y[4] = {d[k].x, d[k].y, d[k].z, d[k].w};
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      s = fmaf(__uint_as_float(x[e] << 16), __uint_as_float(y[e] << 16), s);
-      s = fmaf(__uint_as_float(x[e] & 0xffff0000u), __uint_as_float(y[e] & 0xffff0000u), s);
-    }
-#pragma unroll
-    for (int m = LANES / 2; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-    if (row >= rows) break;                          // the same for the lanes of a row; rows grow with k
-    float4* q = reinterpret_cast<float4*>(dq32 + row * DH + lane * 8);
-    q[0] = q[1] = make_float4(0.f, 0.f, 0.f, 0.f);
-    const long long tok = row / H;
-    if (lane == 0) delta[((tok / S) * H + row % H) * S + tok % S] = s;
-  }
 }
 
 // dq32 [tokens, q_cols] fp32 -> first q_cols columns (heads of HD) of the packed bf16 gradient, eight values a thread; PARTS: the
@@ -1847,26 +1441,20 @@ extern "C" int tplr_rope(void* buf, const float* cosb, const float* sinb, long l
                          long long row_stride, int inverse, void* stream);
 
 static int bwd_split(int B, int S, int H, int KV, int head_dim);
-static int bwd_split_walk(int B, int S, int H, int KV);
 
 namespace {
-template <int HD, bool DOCS>
+template <int HD>
 int launch_bwd(const void* qkv, const void* out, const void* dout, const float* lse, float* delta, float* dq32, void* dqkv, int B,
                int S, int H, int KV, long long ld_qkv, long long ld_o, float scale, const float* cosb, const float* sinb,
-               unsigned int* status, cudaStream_t st, bool delta_ready, const int* starts = nullptr, const int* blocks = nullptr) {
+               unsigned int* status, cudaStream_t st, bool delta_ready) {
   const long long tokens = (long long)B * S;
   const int C = (H + 2 * KV) * HD;
-  if (DOCS) {
-    const long long rows = tokens * H, per_cta = 4 * 256 / (HD / 8);
-    const cudaError_t e = launch_pdl(attn_docs_prepare_kernel<HD>, (unsigned)((rows + per_cta - 1) / per_cta), 256, 0, st,
-                                     (const __nv_bfloat16*)out, (const __nv_bfloat16*)dout, delta, dq32, rows, S, H);
-    if (e != cudaSuccess) return (int)e;
-  } else if (!delta_ready) {
+  if (!delta_ready) {
     constexpr int per_cta = 256 / (HD / 4);
     attn_delta_kernel<HD><<<(unsigned)((tokens * H + per_cta - 1) / per_cta), 256, 0, st>>>(
         (const __nv_bfloat16*)out, (const __nv_bfloat16*)dout, delta, tokens, S, H, ld_o);
   }
-  if (!DOCS && HD == 128 && S % 128 == 0 && g_bwd_variant == 2) {
+  if (HD == 128 && S % 128 == 0 && g_bwd_variant == 2) {
     // pipelined kernel: dq32 is used as the transposed scratch [B*H*128, S]
     AttnBwd2Params p = {};
     if (!make_map(&p.tmKV, qkv, C, tokens, ld_qkv, 64, 128)) return -202;
@@ -1887,7 +1475,7 @@ int launch_bwd(const void* qkv, const void* out, const void* dout, const float* 
   AttnBwdParams p = {};
   if (!make_map3(&p.tmQKV, qkv, C, S, B, ld_qkv, 64, 128)) return -202;
   if (!make_map3(&p.tmDO, dout, (long long)H * HD, S, B, (long long)H * HD, 64, 128)) return -203;
-  p.split = DOCS ? bwd_split_walk(B, S, H, KV) : bwd_split(B, S, H, KV, HD);
+  p.split = bwd_split(B, S, H, KV, HD);
   float* part = dq32 + tokens * H * HD;                        // the parts of dK and dV lie behind dQ
   const int kv_cols = p.split > 1 ? 2 * KV * HD : 0;
   if (!make_map3(&p.tmDQ, dq32, (long long)H * HD, S, B, (long long)H * HD, 32, 32, true)) return -204;
@@ -1896,10 +1484,9 @@ int launch_bwd(const void* qkv, const void* out, const void* dout, const float* 
   p.lse = lse; p.delta = delta; p.B = B; p.S = S; p.H = H; p.KV = KV;
   p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   p.rope_cos = cosb; p.rope_sin = sinb;
-  p.starts = starts; p.blocks = blocks;
-  cudaError_t e = cudaFuncSetAttribute(attn_bwd_kernel<HD, DOCS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bwd_smem<HD>());
+  cudaError_t e = cudaFuncSetAttribute(attn_bwd_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, bwd_smem<HD>());
   if (e != cudaSuccess) return (int)e;
-  e = launch_pdl(attn_bwd_kernel<HD, DOCS>, (unsigned)(((S + BKV - 1) / BKV) * KV * B * p.split), bwd_threads<HD>(), bwd_smem<HD>(), st, p);
+  e = launch_pdl(attn_bwd_kernel<HD>, (unsigned)(((S + BKV - 1) / BKV) * KV * B * p.split), bwd_threads<HD>(), bwd_smem<HD>(), st, p);
   if (e != cudaSuccess) return (int)e;
   auto cast = kv_cols ? attn_dq_cast_kernel<HD, true> : attn_dq_cast_kernel<HD, false>;
   return (int)launch_pdl(cast, tplr_sm_count() * 8, 256, 0, st, dq32, part, p.split, (__nv_bfloat16*)dqkv, tokens, H * HD, kv_cols, (H + KV) * HD, ld_qkv, cosb, sinb, S);
@@ -1913,10 +1500,7 @@ int launch_bwd(const void* qkv, const void* out, const void* dout, const float* 
 // (64 CTAs), 46 us in four parts (256 CTAs; the pass that adds them 2 us more); B 6, S 640 (240 CTAs) 103 us whole, 113 us in
 // two parts; B 4, S 1024 (256 CTAs) 151 us whole, 163 us in two.
 static int bwd_split(int B, int S, int H, int KV, int head_dim) {
-  return head_dim == 128 && S % 128 == 0 && g_bwd_variant == 2 ? 1 : bwd_split_walk(B, S, H, KV);
-}
-static int bwd_split_walk(int B, int S, int H, int KV) {
-  if (KV <= 0 || H % KV) return 1;
+  if (KV <= 0 || H % KV || (head_dim == 128 && S % 128 == 0 && g_bwd_variant == 2)) return 1;
   const int group = H / KV;
   const long long n = (S + BKV - 1) / BKV, ctas = n * KV * B;
   int split = 1;
@@ -1940,9 +1524,9 @@ static int attention_bwd_impl(const void* qkv, const void* out, const void* dout
   if ((head_dim != 128 && head_dim != 64) || H % KV || (ld_qkv % 8) || (ld_o % 8) || ((uintptr_t)qkv & 15) ||
       ((uintptr_t)dqkv & 15) || ((uintptr_t)dout & 15) || ((uintptr_t)out & 7) || ((uintptr_t)dq32 & 15))
     return -201;
-  auto run = head_dim == 128 ? launch_bwd<128, false> : launch_bwd<64, false>;
+  auto run = head_dim == 128 ? launch_bwd<128> : launch_bwd<64>;
   return run(qkv, out, dout, lse, delta, dq32, dqkv, B, S, H, KV, ld_qkv, ld_o, scale, cosb, sinb, status, (cudaStream_t)stream,
-             delta_ready, nullptr, nullptr);
+             delta_ready);
 }
 
 TPLR_API int tplr_attention_bwd(const void* qkv, const void* out, const void* dout, const float* lse, float* delta,
@@ -1977,22 +1561,1037 @@ TPLR_API int tplr_attention_bwd_unrope_delta(const void* qkv, const void* out, c
                             true);
 }
 
-// Fp32 elements per token of the scratch that tplr_attention_docs_bwd needs, contents irrelevant.
-TPLR_API int tplr_attention_docs_bwd_scratch_cols(int B, int S, int H, int KV, int head_dim) {
-  const int split = bwd_split_walk(B, S, H, KV);
-  return (H + (split > 1 ? 2 * KV * split : 0)) * head_dim;
+// ------------------------------------------------------------------------------------------ //
+// Forward within documents: row s of a sequence sees the keys max(starts[s], 0) .. s.  A CTA has a query block of one head as above and
+// walks the key blocks from the diagonal down to that of its rows' least start (so the first tiles are on their way before the
+// starts are known); a block that all rows of a warp see whole runs without a mask.  Eight softmax warps, two a quadrant of tensor memory with half of a row's columns each: what bounds a block is the
+// chain from S over the exponentials to the product with V, and a row of 128 in one thread is the longest part of it.  The two
+// exchange their maxima through shared memory, join their waits in the same barrier (a warp that gave up takes the other one
+// along), and keep sums of their own to the end.  P lies in the S columns of the warp that makes it, at DH = 64 in columns of its own.
+// ------------------------------------------------------------------------------------------ //
+namespace {
+
+constexpr int DOCS_THREADS = 320;
+
+struct AttnDocsParams {
+  CUtensorMap tmQKV;      // as in the forward kernel above
+  CUtensorMap tmO;
+  float* lse;
+  int B, S, H, KV;
+  float scale_log2;
+  unsigned int* status;
+  const int* starts;      // [B, S]
+  int* blocks;            // [B, nQ], or null: takes the least start of a row in the query block that sees anything (INT_MAX: none does)
+};
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
+// Both warps of a quadrant come here with an answer and leave with the joint one.
+__device__ __forceinline__ bool pair_agrees(bool ok, int quad) {
+  uint32_t both;
+  asm volatile("{\n\t.reg .pred mine, all;\n\tsetp.ne.u32 mine, %2, 0;\n\tbar.red.and.pred all, %1, 64, mine;\n\tselp.u32 %0, 1, 0, all;\n\t}"
+               : "=r"(both) : "r"(quad + 1), "r"((uint32_t)ok) : "memory");
+  return both != 0;
 }
 
-// Gradient of tplr_attention_docs_fwd, whose starts and blocks it takes; out and dout dense, otherwise as tplr_attention_bwd.
+template <int DH>
+__global__ void __launch_bounds__(DOCS_THREADS, 2)
+attn_docs_fwd_kernel(const __grid_constant__ AttnDocsParams p) {
+  constexpr int TILE_BYTES = tile_bytes<DH>();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(8) uint64_t bar_q, bar_k_full, bar_k_empty, bar_v_full, bar_v_empty, bar_s_full, bar_s_read, bar_p_full, bar_o_full;
+  __shared__ uint32_t s_tmem_base;
+  __shared__ int s_abort;
+  __shared__ int s_least[4];
+  __shared__ float s_part[2][2][128];                      // [block parity][column half][row]: maxima, at the end sums
+
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int nQ = (p.S + BQ - 1) / BQ;
+  const int hb = p.H * p.B;
+  const int qi = nQ - 1 - (int)(blockIdx.x / hb);          // late query blocks first: they may see the most
+  const int h = (int)(blockIdx.x % hb) % p.H, b = (int)(blockIdx.x % hb) / p.H;
+  const int g = h / (p.H / p.KV);
+  const int row0 = qi * BQ;
+  const int qcol = h * DH, kcol = (p.H + g) * DH, vcol = (p.H + p.KV + g) * DH;
+  volatile int* abort_flag = &s_abort;
+
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    mbar_init(smem_u32(&bar_q), 1);
+    mbar_init(smem_u32(&bar_k_full), 1); mbar_init(smem_u32(&bar_k_empty), 1);
+    mbar_init(smem_u32(&bar_v_full), 1); mbar_init(smem_u32(&bar_v_empty), 1);
+    mbar_init(smem_u32(&bar_s_full), 1); mbar_init(smem_u32(&bar_s_read), 8); mbar_init(smem_u32(&bar_p_full), 8);
+    mbar_init(smem_u32(&bar_o_full), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&s_tmem_base)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  const uint32_t sQ = smem_u32(smem), sK = sQ + TILE_BYTES, sV = sK + TILE_BYTES;
+  if (threadIdx.x == 0) { prefetch_map(&p.tmQKV); prefetch_map(&p.tmO); }
+  grid_wait();
+  grid_release();
+  if (threadIdx.x == 0) {                                  // Q and the diagonal's K and V; the barriers are this thread's own so far
+    mbar_expect_tx(smem_u32(&bar_q), TILE_BYTES);
+    load_tile<DH>(sQ, &p.tmQKV, smem_u32(&bar_q), qcol, row0, b);
+    mbar_expect_tx(smem_u32(&bar_k_full), TILE_BYTES);
+    load_tile<DH>(sK, &p.tmQKV, smem_u32(&bar_k_full), kcol, row0, b);
+    mbar_expect_tx(smem_u32(&bar_v_full), TILE_BYTES);
+    load_tile<DH>(sV, &p.tmQKV, smem_u32(&bar_v_full), vcol, row0, b);
+  }
+  __syncwarp();
+  const int quad = warp & 3, r = quad * 32 + lane;         // softmax warps: query row inside the block = TMEM lane
+  int start = INT_MAX;                                     // first key of this thread's row; INT_MAX: it sees none, or is past the end
+  if (warp >= 2) {
+    const int s = row0 + r;
+    if (s < p.S) start = max(p.starts[(long long)b * p.S + s], 0);
+    if (start > s) start = INT_MAX;
+    const int least = __reduce_min_sync(0xffffffffu, start);
+    if (lane == 0 && warp < 6) s_least[quad] = least;
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const int least = min(min(s_least[0], s_least[1]), min(s_least[2], s_least[3]));
+  const int nb = least == INT_MAX ? 0 : qi - least / BKV + 1;      // key blocks qi, qi - 1, ..
+  if (p.blocks && h == 0 && threadIdx.x == 0) p.blocks[(long long)b * nQ + qi] = least;
+  const uint32_t tmem_base = s_tmem_base;
+  // S columns 0..127, O from column 128; P over S at DH = 128, at 64 in the 64 columns that O leaves, so that the next block's S is
+  // computed as soon as the softmax warps hold this one's (AHEAD)
+  constexpr bool AHEAD = DH == 64;
+  constexpr int P_HALF = AHEAD ? 32 : 64;                  // columns from one warp's P to the other's
+  const uint32_t tS = tmem_base, tO = tmem_base + 128, tP = AHEAD ? tmem_base + 192 : tmem_base;
+
+  if (warp == 0) {
+    const bool leader = elect_one();
+    bool ok = true;
+    int n_k = 1, n_v = 1;                                  // tiles asked for
+    for (int j = 1; j < nb && ok; ++j) {
+      const uint32_t ph = j & 1;
+      const int krow = (qi - j) * BKV;
+      if (!(ok = mbar_wait_warp(smem_u32(&bar_k_empty), ph ^ 1, abort_flag))) break;
+      if (leader) {
+        mbar_expect_tx(smem_u32(&bar_k_full), TILE_BYTES);
+        load_tile<DH>(sK, &p.tmQKV, smem_u32(&bar_k_full), kcol, krow, b);
+      }
+      ++n_k;
+      if (!(ok = mbar_wait_warp(smem_u32(&bar_v_empty), ph ^ 1, abort_flag))) break;
+      if (leader) {
+        mbar_expect_tx(smem_u32(&bar_v_full), TILE_BYTES);
+        load_tile<DH>(sV, &p.tmQKV, smem_u32(&bar_v_full), vcol, krow, b);
+      }
+      ++n_v;
+    }
+    if (leader) {
+      Drain drain;                                         // no load may land after the CTA has retired: a role may have given up
+      drain.wait(smem_u32(&bar_q), 0);
+      drain.wait(smem_u32(&bar_k_full), (uint32_t)((n_k - 1) & 1));
+      drain.wait(smem_u32(&bar_v_full), (uint32_t)((n_v - 1) & 1));
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    const uint32_t id_qk = idesc_mn(128, false, false), id_pv = idesc_mn(DH, false, true);
+    const DescBase bQ = desc_base(sQ, 16, 1024), bK = desc_base(sK, 16, 1024), bV = desc_base(sV, 128 * 128, 1024);
+    auto issue_s = [&](int j) -> bool {                    // S(j) = Q K(j)^T
+      if (!mbar_wait_warp(smem_u32(&bar_k_full), (uint32_t)(j & 1), abort_flag)) return false;
+      tcgen05_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int kk = 0; kk < DH / 16; ++kk) {
+          const uint32_t off = (uint32_t)(kk >> 2) * (128u * 128u / 16u) + (uint32_t)(kk & 3) * 2u;    // 16-byte units
+          umma_bf16_b(tS, bQ, off, bK, off, id_qk, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(smem_u32(&bar_s_full));
+        umma_commit(smem_u32(&bar_k_empty));
+      }
+      return true;
+    };
+    bool ok = nb > 0 && mbar_wait_warp(smem_u32(&bar_q), 0, abort_flag);
+    if (AHEAD && ok) ok = issue_s(0);
+    for (int j = 0; j < nb && ok; ++j) {
+      const uint32_t ph = j & 1;
+      if (!AHEAD) {
+        if (!(ok = issue_s(j))) break;
+      } else if (j + 1 < nb) {
+        if (!(ok = mbar_wait_warp(smem_u32(&bar_s_read), ph, abort_flag))) break;
+        if (!(ok = issue_s(j + 1))) break;
+      }
+      if (!(ok = mbar_wait_warp(smem_u32(&bar_p_full), ph, abort_flag))) break;
+      if (!(ok = mbar_wait_warp(smem_u32(&bar_v_full), ph, abort_flag))) break;
+      tcgen05_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int kk = 0; kk < BKV / 16; ++kk)
+          umma_ts_bf16_b(tO, tP + (kk >> 2) * P_HALF + 8 * (kk & 3), bV, (uint32_t)kk * 128u, id_pv, (j > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(smem_u32(&bar_v_empty));
+        if (j == nb - 1) umma_commit(smem_u32(&bar_o_full));
+      }
+    }
+  } else {
+    const int ch = (warp - 2) >> 2;                        // columns [64 ch, 64 ch + 64) of S, half of O's
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    float m_used = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < nb; ++j) {
+      ok = mbar_wait_warp(smem_u32(&bar_s_full), j & 1, abort_flag);
+      tcgen05_fence_after();
+      const bool diag = j == 0;
+      const int lo = (start == INT_MAX ? BKV : start - (qi - j) * BKV) - ch * 64;      // the columns that the row sees; nothing: behind the last
+      const int hi = (diag ? r : BKV - 1) - ch * 64;
+      uint32_t v[64];
+      tmem_ld32_nowait(tS + ch * 64 + lane_off, v);
+      tmem_ld32_nowait(tS + ch * 64 + 32 + lane_off, v + 32);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      behind_wait32(v);
+      behind_wait32(v + 32);
+      if (AHEAD) {
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_s_read));
+      }
+      if (__any_sync(0xffffffffu, lo > 0 || hi < 63)) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e) if (e < lo || e > hi) v[e] = 0xff800000u;         // -inf: exp2 makes it zero
+      }
+      float mx = -INFINITY, mx2 = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 64; e += 4) {
+        mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+        mx2 = max3(mx2, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+      }
+      mx = fmaxf(mx, mx2);
+      if (AHEAD && j > 0 && ok) {            // O and the P columns: the product of block j - 1 has finished with them
+        ok = mbar_wait_warp(smem_u32(&bar_v_empty), (uint32_t)((j - 1) & 1), abort_flag);
+        tcgen05_fence_after();
+      }
+      s_part[j & 1][ch][r] = mx;
+      if (!(ok = pair_agrees(ok, quad))) break;
+      mx = fmaxf(mx, s_part[j & 1][ch ^ 1][r]);
+      const float m_new = fmaxf(m_used, mx * p.scale_log2);
+      const bool need = m_new > m_used + RESCALE_THRESHOLD;       // true for the first block with a key (m_used = -inf)
+      if (__any_sync(0xffffffffu, need)) {
+        const float alpha = need ? exp2f(m_used - m_new) : 1.f;   // 0 for the first block
+        if (need) { m_used = m_new; l *= alpha; }
+        if (j > 0) {
+          // PV of block j - 1 has finished with O: waited for above, or (not AHEAD) S of block j was issued behind it
+#pragma unroll 1
+          for (int c = 0; c < DH / 32; ++c) {
+            uint32_t o[16];
+            const uint32_t at = tO + ch * (DH / 2) + c * 16 + lane_off;
+            tmem_ld16(at, o);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st16(at, o);
+          }
+        }
+      }
+      // a row that sees nothing has no maximum, and all its scores are masked
+      const float m_ref = m_used == -INFINITY ? 0.f : m_used;
+      const unsigned long long sl2x2 = pack_f32x2(__float_as_uint(p.scale_log2), __float_as_uint(p.scale_log2));
+      const unsigned long long negm = pack_f32x2(__float_as_uint(-m_ref), __float_as_uint(-m_ref));
+      unsigned long long sum = 0ull;                       // (0.f, 0.f)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float a0, a1;
+          unpack_f32x2(fma_f32x2(pack_f32x2(v[c * 32 + 2 * e], v[c * 32 + 2 * e + 1]), sl2x2, negm), a0, a1);
+          const float p0 = exp2f(a0), p1 = exp2f(a1);
+          sum = add_f32x2(sum, pack_f32x2(__float_as_uint(p0), __float_as_uint(p1)));
+          const __nv_bfloat162 hh = __floats2bfloat162_rn(p0, p1);
+          pk[e] = *reinterpret_cast<const uint32_t*>(&hh);
+        }
+        tmem_st16(tP + ch * P_HALF + c * 16 + lane_off, pk);
+      }
+      float s0, s1;
+      unpack_f32x2(sum, s0, s1);
+      l += s0 + s1;
+      tmem_wait_st();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_p_full));
+    }
+    // epilogue: O / l -> bf16 -> swizzled staging (the Q tile is no longer read) -> TMA store.  Every wait behind the loop is joined,
+    // and both warps leave it together, so a warp that comes here finds the other.
+    if (ok) {
+      // without a block: the Q tile has landed before its bytes are written over
+      ok = nb > 0 ? mbar_wait_warp(smem_u32(&bar_o_full), 0, abort_flag) : mbar_wait_warp(smem_u32(&bar_q), 0, abort_flag);
+      s_part[nb & 1][ch][r] = l;
+      ok = pair_agrees(ok, quad);
+    }
+    if (ok) {
+      tcgen05_fence_after();
+      l = s_part[nb & 1][0][r] + s_part[nb & 1][1][r];
+      const bool empty = start == INT_MAX;                 // a row that sees nothing is zero
+      const float inv_l = 1.f / l;
+      const uint32_t stage = sQ + (uint32_t)quad * (32u * DH * 2u) + (DH == 128 ? (uint32_t)ch * 4096u : 0u);
+      const int orow = row0 + quad * 32;
+      const uint32_t sw = (uint32_t)(lane & 7), rowaddr = stage + (uint32_t)lane * 128u;
+#pragma unroll
+      for (int c = 0; c < DH / 64; ++c) {
+        uint32_t o[32];
+        tmem_ld32(tO + ch * (DH / 2) + c * 32 + lane_off, o);
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          uint32_t pw[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const __nv_bfloat162 hh = __floats2bfloat162_rn(__uint_as_float(o[8 * q4 + 2 * e]) * inv_l, __uint_as_float(o[8 * q4 + 2 * e + 1]) * inv_l);
+            pw[e] = empty ? 0u : *reinterpret_cast<const uint32_t*>(&hh);
+          }
+          const uint32_t jj = (uint32_t)((DH == 128 ? c : ch) * 4 + q4);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + ((jj ^ sw) << 4)), "r"(pw[0]), "r"(pw[1]),
+                       "r"(pw[2]), "r"(pw[3]) : "memory");
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (DH == 64) (void)pair_agrees(true, quad);         // one box of 64 columns for both
+      if (lane == 0 && orow < p.S && (DH == 128 || ch == 0)) {
+        tma_store_3d(&p.tmO, stage, qcol + (DH == 128 ? ch * 64 : 0), orow, b);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      }
+      // an infinite sum makes the backward pass's weights of the row zero
+      if (p.lse && ch == 0 && row0 + r < p.S)
+        p.lse[((long long)b * p.H + h) * p.S + row0 + r] = empty ? INFINITY : (m_used + log2f(l)) * 0.6931471805599453f;
+    }
+  }
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem_base) : "memory");
+  }
+  if (threadIdx.x == 0 && s_abort && p.status) atomicOr(p.status, TPLR_ST_WAIT_TIMEOUT);
+}
+
+template <int DH>
+int launch_docs_fwd(const void* qkv, const int* starts, void* out, float* lse, int* blocks, int B, int S, int H, int KV, long long ld_qkv,
+                    long long ld_o, float scale, unsigned int* status, cudaStream_t st) {
+  AttnDocsParams p = {};
+  if (!make_map3(&p.tmQKV, qkv, (long long)(H + 2 * KV) * DH, S, B, ld_qkv, 64, 128)) return -202;
+  if (!make_map3(&p.tmO, out, (long long)H * DH, S, B, ld_o, 64, 32)) return -203;
+  p.lse = lse; p.B = B; p.S = S; p.H = H; p.KV = KV;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.status = status; p.starts = starts; p.blocks = blocks;
+  cudaError_t e = cudaFuncSetAttribute(attn_docs_fwd_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, fwd_smem<DH>());
+  if (e != cudaSuccess) return (int)e;
+  const unsigned grid = (unsigned)(((S + BQ - 1) / BQ) * H * B);
+  return (int)launch_pdl(attn_docs_fwd_kernel<DH>, grid, DOCS_THREADS, fwd_smem<DH>(), st, p);
+}
+}  // namespace
+
+// tplr_attention_fwd within documents: row s of sequence b sees the keys max(starts[b * S + s], 0) .. s; one whose start lies behind it
+// sees nothing, and its output is zero.  starts: [B, S] int32, any values.  blocks: [B, ceil(S / 128)] int32 for the backward
+// pass, or null.
+TPLR_API int tplr_attention_docs_fwd(const void* qkv, const int* starts, void* out, float* lse, int* blocks, int B, int S, int H, int KV,
+                                     int head_dim, long long ld_qkv, long long ld_o, float scale, unsigned int* status, void* stream) {
+  TPLR_ENTER();
+  if (B <= 0 || S <= 0) return 0;
+  if (KV <= 0 || H % KV || (ld_qkv % 8) || (ld_o % 8) || ((uintptr_t)qkv & 15) || ((uintptr_t)out & 15) || !starts) return -201;
+  if (head_dim != 128 && head_dim != 64) return -201;
+  auto run = head_dim == 128 ? launch_docs_fwd<128> : launch_docs_fwd<64>;
+  return run(qkv, starts, out, lse, blocks, B, S, H, KV, ld_qkv, ld_o, scale, status, (cudaStream_t)stream);
+}
+
+// ------------------------------------------------------------------------------------------ //
+// Backward within documents: two kernels, neither of which adds into memory, so the gradient has the same bits on every run.
+//
+// dQ: a CTA has a query block of one head, as the forward kernel, and walks the same key blocks in the same order.  Per step S = Q K^T, dP = dO V^T
+// (tensor cores -> TMEM), P = exp2(S * scale - lse), dS = P * (dP - delta) * scale (softmax warps, a query row a thread pair), dS as bf16 over
+// the dP columns, dQ += dS K with dS from tensor memory.  Two S buffers, so that the next exponentials run under this step's products.
+// delta, the row sum of dO * O, is formed on the way and left for the other kernel.
+//
+// dK, dV: a CTA has a key/value block of one kv head and the query heads of its group, or a part of them, and walks the query blocks
+// from the diagonal to the last that sees any of its keys.  Everything is transposed, with the key row as the TMEM lane:
+//   S^T = K Q^T, dP^T = V dO^T;  P^T and dS^T as packed bf16 over them;  dV += P^T dO, dK += dS^T Q
+// with P^T and dS^T from tensor memory: neither goes through shared memory, whose traffic bounds the kernel above (4600 of its 5250
+// cycles a step at DH = 128).  lse, delta and the starts belong to columns here: a warp of its own brings them to shared memory.
+//
+// Seven products instead of five, but each step is shorter, and there is no fp32 dQ to be zeroed, added into, read and rounded.
+// ------------------------------------------------------------------------------------------ //
+namespace {
+
+constexpr int DQ_THREADS = 320, DKV_THREADS = 352;
+constexpr int RING3 = 3;                                   // K (dQ) or Q (dK, dV): held from the first product of a step to its last
+// Q, dO; three K, two V   |   K, V; three Q, two dO; and the small things behind them.  The tiles start at the window's 1024-byte boundary.
+template <int DH> constexpr int docs_bwd_tiles() { return 7 * tile_bytes<DH>(); }
+template <int DH> constexpr int docs_bwd_smem() { return docs_bwd_tiles<DH>() + 3072; }
+
+struct DocsBwdShared {
+  uint64_t bar_res;                                        // the resident tiles
+  uint64_t ring_full[RING3], ring_empty[RING3], pair_full[2], pair_empty[2];
+  uint64_t s_full[2], dp_full, p_ready, ds_ready, acc_full, stat_full[2], stat_empty[2];
+  uint32_t tmem_base;
+  int abort, last;
+  float part[2][128];                                      // dQ: halves of delta
+};
+struct DocsStats { float nlse[128], ndelta[128]; uint8_t lo[128]; };       // dK, dV: of a query block; negated, in the units of the products
+static_assert(sizeof(DocsBwdShared) <= 1536 && 512 + 2 * sizeof(DocsStats) <= 3072, "the small things fit behind the tiles");
+
+struct AttnDocsBwdParams {
+  CUtensorMap tmQKV;      // [B, S, C] bf16, box 64 x 128 x 1, 128-byte swizzle
+  CUtensorMap tmDO;       // [B, S, H * DH] bf16, the same box
+  CUtensorMap tmDQKV;     // [B, S, C] bf16, box 64 x 32 x 1
+  CUtensorMap tmPart;     // split: [B, S, split * 2 * KV * DH] fp32, box 32 x 32 x 1 (dK | dV of every part)
+  const __nv_bfloat16* out;
+  const float* lse;
+  float* delta;           // [B, H, S]
+  const int* starts;
+  const int* blocks;
+  int B, S, H, KV;
+  int split;              // CTAs that share a group's query heads; > 1: each stores its part of dK and dV in fp32
+  float scale, scale_log2;
+  unsigned int* status;
+};
+
+__device__ __forceinline__ unsigned long long mul_f32x2(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ unsigned long long two(float x) { return pack_f32x2(__float_as_uint(x), __float_as_uint(x)); }
+__device__ __forceinline__ uint32_t bf16x2_of(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// 32 fp32 values of a lane's row -> bf16 in half `hh` of its row of a swizzled 32 x 64 box
+__device__ __forceinline__ void box_row(uint32_t rowaddr, uint32_t sw, int hh, const uint32_t* v, bool zero) {
+#pragma unroll
+  for (int q4 = 0; q4 < 4; ++q4) {
+    uint32_t pw[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pw[e] = zero ? 0u : bf16x2_of(__uint_as_float(v[8 * q4 + 2 * e]), __uint_as_float(v[8 * q4 + 2 * e + 1]));
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + ((((uint32_t)(hh * 4 + q4)) ^ sw) << 4)), "r"(pw[0]), "r"(pw[1]),
+                 "r"(pw[2]), "r"(pw[3]) : "memory");
+  }
+}
+__device__ __forceinline__ void docs_bwd_init(DocsBwdShared& sh, int warp) {
+  if (threadIdx.x == 0) {
+    sh.abort = 0;
+    sh.last = -1;
+    mbar_init(smem_u32(&sh.bar_res), 1);
+    for (int s = 0; s < RING3; ++s) { mbar_init(smem_u32(&sh.ring_full[s]), 1); mbar_init(smem_u32(&sh.ring_empty[s]), 1); }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(smem_u32(&sh.pair_full[s]), 1); mbar_init(smem_u32(&sh.pair_empty[s]), 1); mbar_init(smem_u32(&sh.s_full[s]), 1);
+      mbar_init(smem_u32(&sh.stat_full[s]), 1); mbar_init(smem_u32(&sh.stat_empty[s]), 8);
+    }
+    mbar_init(smem_u32(&sh.dp_full), 1); mbar_init(smem_u32(&sh.p_ready), 8); mbar_init(smem_u32(&sh.ds_ready), 8);
+    mbar_init(smem_u32(&sh.acc_full), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem_base)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+}
+__device__ __forceinline__ void docs_bwd_end(const AttnDocsBwdParams& p, DocsBwdShared& sh, int warp) {
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh.tmem_base) : "memory");
+  }
+  if (threadIdx.x == 0 && sh.abort && p.status) atomicOr(p.status, TPLR_ST_WAIT_TIMEOUT);
+}
+// offsets of a 16-wide k step in a tile of 128 rows, in 16-byte units: along the 128-byte rows, and along the rows of the tile
+__device__ __forceinline__ constexpr uint32_t koff(int kk) { return (uint32_t)(kk >> 2) * (128u * 128u / 16u) + (uint32_t)(kk & 3) * 2u; }
+__device__ __forceinline__ constexpr uint32_t moff(int kk) { return (uint32_t)kk * 128u; }
+
+template <int DH>
+__global__ void __launch_bounds__(DQ_THREADS, 1)
+attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
+  constexpr int TILE_BYTES = tile_bytes<DH>();
+  extern __shared__ __align__(1024) uint8_t smem[];
+  DocsBwdShared& sh = *reinterpret_cast<DocsBwdShared*>(smem + docs_bwd_tiles<DH>());
+
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int nQ = (p.S + BQ - 1) / BQ;
+  const int hb = p.H * p.B;
+  const int qi = nQ - 1 - (int)(blockIdx.x / hb);
+  const int h = (int)(blockIdx.x % hb) % p.H, b = (int)(blockIdx.x % hb) / p.H;
+  const int g = h / (p.H / p.KV);
+  const int row0 = qi * BQ;
+  const int qcol = h * DH, kcol = (p.H + g) * DH, vcol = (p.H + p.KV + g) * DH;
+  volatile int* abort_flag = &sh.abort;
+
+  const uint32_t sQ = smem_u32(smem), sdO = sQ + TILE_BYTES, sK = sdO + TILE_BYTES, sV = sK + RING3 * TILE_BYTES;
+  docs_bwd_init(sh, warp);
+  if (threadIdx.x == 0) { prefetch_map(&p.tmQKV); prefetch_map(&p.tmDO); prefetch_map(&p.tmDQKV); }
+  grid_wait();
+  grid_release();
+  if (threadIdx.x == 0) {                                  // Q, dO and the diagonal's K and V; the barriers are this thread's own so far
+    mbar_expect_tx(smem_u32(&sh.bar_res), 2 * TILE_BYTES);
+    load_tile<DH>(sQ, &p.tmQKV, smem_u32(&sh.bar_res), qcol, row0, b);
+    load_tile<DH>(sdO, &p.tmDO, smem_u32(&sh.bar_res), qcol, row0, b);
+    mbar_expect_tx(smem_u32(&sh.ring_full[0]), TILE_BYTES);
+    load_tile<DH>(sK, &p.tmQKV, smem_u32(&sh.ring_full[0]), kcol, row0, b);
+    mbar_expect_tx(smem_u32(&sh.pair_full[0]), TILE_BYTES);
+    load_tile<DH>(sV, &p.tmQKV, smem_u32(&sh.pair_full[0]), vcol, row0, b);
+  }
+  __syncwarp();
+  const int least = p.blocks[(long long)b * nQ + qi];
+  const int nb = least == INT_MAX ? 0 : qi - least / BKV + 1;      // key blocks qi, qi - 1, ..
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = sh.tmem_base;
+  const uint32_t tdP = tmem_base + 128, tdQ = tmem_base + 256;       // S of even steps in columns 0..127, of odd ones in 384..511
+
+  if (warp == 0) {
+    const bool leader = elect_one();
+    bool ok = true;
+    int n_k = 1, n_v = 1, s3 = 1;
+    uint32_t ph3 = 0;
+    for (int t = 1; t < nb && ok; ++t) {
+      const int krow = (qi - t) * BKV, s2 = t & 1;
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.ring_empty[s3]), ph3 ^ 1u, abort_flag))) break;
+      if (leader) {
+        mbar_expect_tx(smem_u32(&sh.ring_full[s3]), TILE_BYTES);
+        load_tile<DH>(sK + s3 * TILE_BYTES, &p.tmQKV, smem_u32(&sh.ring_full[s3]), kcol, krow, b);
+      }
+      ++n_k;
+      if (++s3 == RING3) { s3 = 0; ph3 ^= 1u; }
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.pair_empty[s2]), (uint32_t)(((t >> 1) & 1) ^ 1), abort_flag))) break;
+      if (leader) {
+        mbar_expect_tx(smem_u32(&sh.pair_full[s2]), TILE_BYTES);
+        load_tile<DH>(sV + s2 * TILE_BYTES, &p.tmQKV, smem_u32(&sh.pair_full[s2]), vcol, krow, b);
+      }
+      ++n_v;
+    }
+    if (leader) {
+      Drain drain;                                         // no load may land after the CTA has retired: a role may have given up
+      drain.wait(smem_u32(&sh.bar_res), 0);
+      for (int t = max(n_k - RING3, 0); t < n_k; ++t) drain.wait(smem_u32(&sh.ring_full[t % RING3]), (uint32_t)((t / RING3) & 1));
+      for (int t = max(n_v - 2, 0); t < n_v; ++t) drain.wait(smem_u32(&sh.pair_full[t & 1]), (uint32_t)((t >> 1) & 1));
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    const uint32_t id_kk = idesc_mn(128, false, false), id_km = idesc_mn(DH, false, true);
+    const DescBase kQ = desc_base(sQ, 16, 1024), kdO = desc_base(sdO, 16, 1024), kK = desc_base(sK, 16, 1024), kV = desc_base(sV, 16, 1024),
+                   mK = desc_base(sK, 128 * 128, 1024);
+    int s3 = 0;                                            // ring place of the next S's K
+    uint32_t ph3 = 0;
+    auto issue_s = [&](int t) -> bool {
+      if (!mbar_wait_warp(smem_u32(&sh.ring_full[s3]), ph3, abort_flag)) return false;
+      tcgen05_fence_after();
+      if (leader) {
+        const uint32_t d = tmem_base + (t & 1) * 384, k = (uint32_t)s3 * (TILE_BYTES / 16);
+#pragma unroll
+        for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(d, kQ, koff(kk), kK, k + koff(kk), id_kk, kk > 0 ? 1u : 0u);
+        umma_commit(smem_u32(&sh.s_full[t & 1]));
+      }
+      if (++s3 == RING3) { s3 = 0; ph3 ^= 1u; }
+      return true;
+    };
+    auto issue_dp = [&](int t) -> bool {
+      if (!mbar_wait_warp(smem_u32(&sh.pair_full[t & 1]), (uint32_t)((t >> 1) & 1), abort_flag)) return false;
+      tcgen05_fence_after();
+      if (leader) {
+        const uint32_t v = (uint32_t)(t & 1) * (TILE_BYTES / 16);
+#pragma unroll
+        for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(tdP, kdO, koff(kk), kV, v + koff(kk), id_kk, kk > 0 ? 1u : 0u);
+        umma_commit(smem_u32(&sh.dp_full));
+        umma_commit(smem_u32(&sh.pair_empty[t & 1]));
+      }
+      return true;
+    };
+    bool ok = nb > 0 && mbar_wait_warp(smem_u32(&sh.bar_res), 0, abort_flag);
+    if (ok) ok = issue_s(0);
+    if (ok) ok = issue_dp(0);
+    int r3 = 0;                                            // ring place of this step's K
+    for (int t = 0; t < nb && ok; ++t) {
+      // the S buffer of step t + 1 was read by every warp in front of dS(t - 1)
+      if (t + 1 < nb && !(ok = issue_s(t + 1))) break;
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.ds_ready), t & 1, abort_flag))) break;
+      tcgen05_fence_after();
+      if (leader) {
+        const uint32_t k = (uint32_t)r3 * (TILE_BYTES / 16);
+#pragma unroll
+        for (int kk = 0; kk < BKV / 16; ++kk)              // dQ[q, d] += dS[q, kv] K[kv, d]; dS packed in the first half of each warp's dP columns
+          umma_ts_bf16_b(tdQ, tdP + (kk >> 2) * 64 + 8 * (kk & 3), mK, k + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(smem_u32(&sh.ring_empty[r3]));
+        if (t == nb - 1) umma_commit(smem_u32(&sh.acc_full));
+      }
+      if (++r3 == RING3) r3 = 0;
+      if (t + 1 < nb && !(ok = issue_dp(t + 1))) break;    // behind dQ(t), which reads dS(t) from its columns
+    }
+  } else {
+    const int quad = warp & 3, ch = (warp - 2) >> 2;       // TMEM lanes, column half
+    const int r = quad * 32 + lane, row = row0 + r;
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const uint32_t sw = (uint32_t)(lane & 7);
+    const long long at = ((long long)b * p.H + h) * p.S + row;
+    int start = INT_MAX;                                   // INT_MAX: the row sees nothing, or is past the end
+    float lse2 = INFINITY;
+    uint4 o[DH / 16];                                      // this half of the row's output
+#pragma unroll
+    for (int q = 0; q < DH / 16; ++q) o[q] = make_uint4(0u, 0u, 0u, 0u);
+    if (row < p.S) {
+      start = max(p.starts[(long long)b * p.S + row], 0);
+      if (start > row) start = INT_MAX;
+      if (start != INT_MAX) {
+        lse2 = p.lse[at] * 1.4426950408889634f;
+        const uint4* orow = reinterpret_cast<const uint4*>(p.out + ((long long)b * p.S + row) * ((long long)p.H * DH) + h * DH + ch * (DH / 2));
+#pragma unroll
+        for (int q = 0; q < DH / 16; ++q) o[q] = orow[q];
+      }
+    }
+    bool ok = mbar_wait_warp(smem_u32(&sh.bar_res), 0, abort_flag);
+    float delta = 0.f;
+    if (ok) {
+      // this lane's row of dO: 64 columns a box of 128-byte rows
+      const uint32_t drow = sdO + (DH == 128 ? (uint32_t)ch * (128u * 128u) : 0u) + (uint32_t)r * 128u;
+#pragma unroll
+      for (int q = 0; q < DH / 16; ++q) {
+        uint32_t d[4];
+        const uint32_t jj = (uint32_t)(DH == 128 ? q : ch * 4 + q);
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(drow + ((jj ^ sw) << 4)) : "memory");
+        const uint32_t ow[4] = {o[q].x, o[q].y, o[q].z, o[q].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          delta = fmaf(__uint_as_float(ow[e] << 16), __uint_as_float(d[e] << 16), delta);
+          delta = fmaf(__uint_as_float(ow[e] & 0xffff0000u), __uint_as_float(d[e] & 0xffff0000u), delta);
+        }
+      }
+      sh.part[ch][r] = delta;
+    }
+    ok = pair_agrees(ok, quad);
+    if (ok) {
+      delta = start == INT_MAX ? 0.f : sh.part[0][r] + sh.part[1][r];
+      if (ch == 0 && row < p.S) p.delta[at] = delta;
+    }
+    const unsigned long long sl2 = two(p.scale_log2), nl = two(-lse2), sc = two(p.scale), nd = two(-delta * p.scale);
+    for (int t = 0; t < nb && ok; ++t) {
+      const bool diag = t == 0;
+      const int lo = (start == INT_MAX ? BKV : start - (qi - t) * BKV) - ch * 64, hi = (diag ? r : BKV - 1) - ch * 64;
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.s_full[t & 1]), (uint32_t)((t >> 1) & 1), abort_flag))) break;
+      tcgen05_fence_after();
+      uint32_t v[64];
+      const uint32_t tS = tmem_base + (t & 1) * 384 + ch * 64 + lane_off;
+      tmem_ld32_nowait(tS, v);
+      tmem_ld32_nowait(tS + 32, v + 32);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      behind_wait32(v);
+      behind_wait32(v + 32);
+#pragma unroll
+      for (int e = 0; e < 64; e += 2) {
+        float a0, a1;
+        unpack_f32x2(fma_f32x2(pack_f32x2(v[e], v[e + 1]), sl2, nl), a0, a1);
+        v[e] = __float_as_uint(exp2f(a0));
+        v[e + 1] = __float_as_uint(exp2f(a1));
+      }
+      if (__any_sync(0xffffffffu, lo > 0 || hi < 63)) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e) if (e < lo || e > hi) v[e] = 0u;
+      }
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.dp_full), t & 1, abort_flag))) break;
+      tcgen05_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t dp[32], pk[16];
+        tmem_ld32(tdP + ch * 64 + c * 32 + lane_off, dp);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float d0, d1;
+          unpack_f32x2(mul_f32x2(pack_f32x2(v[c * 32 + 2 * e], v[c * 32 + 2 * e + 1]), fma_f32x2(pack_f32x2(dp[2 * e], dp[2 * e + 1]), sc, nd)), d0, d1);
+          pk[e] = bf16x2_of(d0, d1);
+        }
+        tmem_st16(tdP + ch * 64 + c * 16 + lane_off, pk);
+      }
+      tmem_wait_st();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.ds_ready));
+    }
+    // dQ -> bf16 -> the bytes of the Q tile -> the query columns of the gradient
+    if (ok && nb > 0) ok = mbar_wait_warp(smem_u32(&sh.acc_full), 0, abort_flag);
+    ok = pair_agrees(ok, quad);
+    if (ok) {
+      tcgen05_fence_after();
+      const uint32_t stage = sQ + (uint32_t)quad * (32u * DH * 2u) + (DH == 128 ? (uint32_t)ch * 4096u : 0u), rowaddr = stage + (uint32_t)lane * 128u;
+#pragma unroll
+      for (int c = 0; c < DH / 64; ++c) {
+        uint32_t q[32];
+        tmem_ld32(tdQ + ch * (DH / 2) + c * 32 + lane_off, q);
+        box_row(rowaddr, sw, DH == 128 ? c : ch, q, nb == 0);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (DH == 64) (void)pair_agrees(true, quad);         // one box of 64 columns for both
+      if (lane == 0 && row0 + quad * 32 < p.S && (DH == 128 || ch == 0)) {
+        tma_store_3d(&p.tmDQKV, stage, qcol + (DH == 128 ? ch * 64 : 0), row0 + quad * 32, b);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      }
+    }
+  }
+  docs_bwd_end(p, sh, warp);
+}
+
+template <int DH>
+__global__ void __launch_bounds__(DKV_THREADS, 1)
+attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
+  constexpr int TILE_BYTES = tile_bytes<DH>();
+  extern __shared__ __align__(1024) uint8_t smem[];
+  DocsBwdShared& sh = *reinterpret_cast<DocsBwdShared*>(smem + docs_bwd_tiles<DH>());
+  DocsStats* stats = reinterpret_cast<DocsStats*>(smem + docs_bwd_tiles<DH>() + 512);      // over `part`, which this kernel has no use for
+
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int nQ = (p.S + BQ - 1) / BQ;
+  const int gb = p.KV * p.B * p.split;
+  const int j = (int)(blockIdx.x / gb);                    // key block; small j (which may be seen by the most rows) first
+  const int sub = (int)(blockIdx.x % gb) % p.split;
+  const int g = (int)(blockIdx.x % gb) / p.split % p.KV, b = (int)(blockIdx.x % gb) / p.split / p.KV;
+  const int heads = p.H / p.KV / p.split, h0 = (g * p.split + sub) * heads;      // query heads of this CTA
+  const int kvrow0 = j * BKV;
+  const int kcol = (p.H + g) * DH, vcol = (p.H + p.KV + g) * DH;
+  volatile int* abort_flag = &sh.abort;
+
+  const uint32_t sK = smem_u32(smem), sV = sK + TILE_BYTES, sQ = sV + TILE_BYTES, sdO = sQ + RING3 * TILE_BYTES;
+  docs_bwd_init(sh, warp);
+  if (threadIdx.x == 0) { prefetch_map(&p.tmQKV); prefetch_map(&p.tmDO); prefetch_map(&p.tmDQKV); }
+  __syncthreads();                                         // `last` is set
+  grid_wait();
+  grid_release();
+  if (threadIdx.x == 0) {                                  // K, V and the diagonal's Q and dO, on their way while the walk's end is looked up
+    mbar_expect_tx(smem_u32(&sh.bar_res), 2 * TILE_BYTES);
+    load_tile<DH>(sK, &p.tmQKV, smem_u32(&sh.bar_res), kcol, kvrow0, b);
+    load_tile<DH>(sV, &p.tmQKV, smem_u32(&sh.bar_res), vcol, kvrow0, b);
+    mbar_expect_tx(smem_u32(&sh.ring_full[0]), TILE_BYTES);
+    load_tile<DH>(sQ, &p.tmQKV, smem_u32(&sh.ring_full[0]), h0 * DH, kvrow0, b);
+    mbar_expect_tx(smem_u32(&sh.pair_full[0]), TILE_BYTES);
+    load_tile<DH>(sdO, &p.tmDO, smem_u32(&sh.pair_full[0]), h0 * DH, kvrow0, b);
+  }
+  __syncwarp();
+  // the last query block that sees any key of this one.  A block in between whose rows begin behind it is walked with all its weights
+  // masked: starts that grow with the row, as documents' do, have none.
+  int last = -1;
+  for (int i = j + (int)threadIdx.x; i < nQ; i += DKV_THREADS)
+    if (p.blocks[(long long)b * nQ + i] < kvrow0 + BKV) last = i;
+  if (last >= 0) atomicMax(&sh.last, last);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const int n_i = max(sh.last - j + 1, 0), n_it = heads * n_i;
+  const uint32_t tmem_base = sh.tmem_base;
+  const uint32_t tS = tmem_base, tdP = tmem_base + 128, tdV = tmem_base + 256, tdK = tmem_base + 384;
+
+  if (warp == 0) {
+    const bool leader = elect_one();
+    bool ok = true;
+    int n_q = 1, n_do = 1, s3 = 1, h = h0, i = 1;
+    uint32_t ph3 = 0;
+    if (i == n_i) { i = 0; ++h; }
+    for (int t = 1; t < n_it && ok; ++t) {
+      const int qrow0 = (j + i) * BQ, s2 = t & 1;
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.ring_empty[s3]), ph3 ^ 1u, abort_flag))) break;
+      if (leader) {
+        mbar_expect_tx(smem_u32(&sh.ring_full[s3]), TILE_BYTES);
+        load_tile<DH>(sQ + s3 * TILE_BYTES, &p.tmQKV, smem_u32(&sh.ring_full[s3]), h * DH, qrow0, b);
+      }
+      ++n_q;
+      if (++s3 == RING3) { s3 = 0; ph3 ^= 1u; }
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.pair_empty[s2]), (uint32_t)(((t >> 1) & 1) ^ 1), abort_flag))) break;
+      if (leader) {
+        mbar_expect_tx(smem_u32(&sh.pair_full[s2]), TILE_BYTES);
+        load_tile<DH>(sdO + s2 * TILE_BYTES, &p.tmDO, smem_u32(&sh.pair_full[s2]), h * DH, qrow0, b);
+      }
+      ++n_do;
+      if (++i == n_i) { i = 0; ++h; }
+    }
+    if (leader) {
+      Drain drain;                                         // no load may land after the CTA has retired: a role may have given up
+      drain.wait(smem_u32(&sh.bar_res), 0);
+      for (int t = max(n_q - RING3, 0); t < n_q; ++t) drain.wait(smem_u32(&sh.ring_full[t % RING3]), (uint32_t)((t / RING3) & 1));
+      for (int t = max(n_do - 2, 0); t < n_do; ++t) drain.wait(smem_u32(&sh.pair_full[t & 1]), (uint32_t)((t >> 1) & 1));
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    const uint32_t id_kk = idesc_mn(128, false, false), id_km = idesc_mn(DH, false, true);
+    const DescBase kK = desc_base(sK, 16, 1024), kV = desc_base(sV, 16, 1024), kQ = desc_base(sQ, 16, 1024), kdO = desc_base(sdO, 16, 1024),
+                   mQ = desc_base(sQ, 128 * 128, 1024), mdO = desc_base(sdO, 128 * 128, 1024);
+    int s3 = 0;                                            // ring place of the next S's Q
+    uint32_t ph3 = 0;
+    auto issue_s = [&]() -> bool {                         // S^T = K Q^T
+      if (!mbar_wait_warp(smem_u32(&sh.ring_full[s3]), ph3, abort_flag)) return false;
+      tcgen05_fence_after();
+      if (leader) {
+        const uint32_t q = (uint32_t)s3 * (TILE_BYTES / 16);
+#pragma unroll
+        for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(tS, kK, koff(kk), kQ, q + koff(kk), id_kk, kk > 0 ? 1u : 0u);
+        umma_commit(smem_u32(&sh.s_full[0]));
+      }
+      if (++s3 == RING3) { s3 = 0; ph3 ^= 1u; }
+      return true;
+    };
+    auto issue_dp = [&](int t) -> bool {                   // dP^T = V dO^T
+      if (!mbar_wait_warp(smem_u32(&sh.pair_full[t & 1]), (uint32_t)((t >> 1) & 1), abort_flag)) return false;
+      tcgen05_fence_after();
+      if (leader) {
+        const uint32_t d = (uint32_t)(t & 1) * (TILE_BYTES / 16);
+#pragma unroll
+        for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(tdP, kV, koff(kk), kdO, d + koff(kk), id_kk, kk > 0 ? 1u : 0u);
+        umma_commit(smem_u32(&sh.dp_full));
+      }
+      return true;
+    };
+    bool ok = n_it > 0 && mbar_wait_warp(smem_u32(&sh.bar_res), 0, abort_flag);
+    if (ok) ok = issue_s();
+    if (ok) ok = issue_dp(0);
+    int r3 = 0;                                            // ring place of this step's Q
+    for (int t = 0; t < n_it && ok; ++t) {
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.p_ready), t & 1, abort_flag))) break;       // P^T over S^T, read by every warp
+      tcgen05_fence_after();
+      if (leader) {
+        const uint32_t d = (uint32_t)(t & 1) * (TILE_BYTES / 16);
+#pragma unroll
+        for (int kk = 0; kk < BQ / 16; ++kk)               // dV[kv, d] += P^T[kv, q] dO[q, d]
+          umma_ts_bf16_b(tdV, tS + (kk >> 2) * 64 + 8 * (kk & 3), mdO, d + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(smem_u32(&sh.pair_empty[t & 1]));      // dP(t) read dO(t) before
+      }
+      if (t + 1 < n_it && !(ok = issue_s())) break;        // behind dV(t), which reads P^T(t) from its columns
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.ds_ready), t & 1, abort_flag))) break;      // dS^T over dP^T
+      tcgen05_fence_after();
+      if (leader) {
+        const uint32_t q = (uint32_t)r3 * (TILE_BYTES / 16);
+#pragma unroll
+        for (int kk = 0; kk < BQ / 16; ++kk)               // dK[kv, d] += dS^T[kv, q] Q[q, d]
+          umma_ts_bf16_b(tdK, tdP + (kk >> 2) * 64 + 8 * (kk & 3), mQ, q + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(smem_u32(&sh.ring_empty[r3]));
+        if (t == n_it - 1) umma_commit(smem_u32(&sh.acc_full));
+      }
+      if (++r3 == RING3) r3 = 0;
+      if (t + 1 < n_it && !(ok = issue_dp(t + 1))) break;
+    }
+  } else if (warp == 10) {
+    // lse, delta and starts of a step's query block, four rows a lane, asked for while the step before is used
+    bool ok = true;
+    int h = h0, i = 0;
+    float nl[4], nd[4];
+    int lo[4];
+    auto fetch = [&] {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = (j + i) * BQ + lane * 4 + e;
+        const long long at = ((long long)b * p.H + h) * p.S + row;
+        const bool live = row < p.S;
+        nl[e] = live ? -p.lse[at] * 1.4426950408889634f : -INFINITY;       // a row that sees nothing has an infinite lse: its weights are zero
+        nd[e] = live ? -p.delta[at] * p.scale : 0.f;
+        lo[e] = live ? min(max(p.starts[(long long)b * p.S + row], kvrow0) - kvrow0, BKV) : 0;
+      }
+      if (++i == n_i) { i = 0; ++h; }
+    };
+    if (n_it > 0) fetch();
+    for (int t = 0; t < n_it && ok; ++t) {
+      const int s = t & 1;
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.stat_empty[s]), (uint32_t)(((t >> 1) & 1) ^ 1), abort_flag))) break;
+      *reinterpret_cast<float4*>(stats[s].nlse + lane * 4) = make_float4(nl[0], nl[1], nl[2], nl[3]);
+      *reinterpret_cast<float4*>(stats[s].ndelta + lane * 4) = make_float4(nd[0], nd[1], nd[2], nd[3]);
+      *reinterpret_cast<uchar4*>(stats[s].lo + lane * 4) = make_uchar4((uint8_t)lo[0], (uint8_t)lo[1], (uint8_t)lo[2], (uint8_t)lo[3]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.stat_full[s]));
+      if (t + 1 < n_it) fetch();
+    }
+  } else {
+    const int quad = warp & 3, ch = (warp - 2) >> 2;       // TMEM lanes, half of the step's query rows
+    const int r = quad * 32 + lane;                        // key row of the block = TMEM lane
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const uint32_t sw = (uint32_t)(lane & 7);
+    const unsigned long long sl2 = two(p.scale_log2), sc = two(p.scale);
+    bool ok = true;
+    int i = 0;
+    for (int t = 0; t < n_it && ok; ++t) {
+      const DocsStats& st = stats[t & 1];
+      const bool diag = i == 0;
+      if (++i == n_i) i = 0;
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.stat_full[t & 1]), (uint32_t)((t >> 1) & 1), abort_flag))) break;
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.s_full[0]), t & 1, abort_flag))) break;
+      tcgen05_fence_after();
+      uint32_t v[64];                                      // P, in fp32 for dS
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        tmem_ld32(tS + ch * 64 + c * 32 + lane_off, v + c * 32);
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 nl = *reinterpret_cast<const float4*>(st.nlse + ch * 64 + c * 32 + e);
+          uint32_t* w = v + c * 32 + e;
+          float a0, a1, a2, a3;
+          unpack_f32x2(fma_f32x2(pack_f32x2(w[0], w[1]), sl2, pack_f32x2(__float_as_uint(nl.x), __float_as_uint(nl.y))), a0, a1);
+          unpack_f32x2(fma_f32x2(pack_f32x2(w[2], w[3]), sl2, pack_f32x2(__float_as_uint(nl.z), __float_as_uint(nl.w))), a2, a3);
+          w[0] = __float_as_uint(exp2f(a0)); w[1] = __float_as_uint(exp2f(a1));
+          w[2] = __float_as_uint(exp2f(a2)); w[3] = __float_as_uint(exp2f(a3));
+        }
+      }
+      // a query row before the key, or whose document begins behind it, does not see it
+      const uint32_t* lo4 = reinterpret_cast<const uint32_t*>(st.lo + ch * 64);
+      if (__any_sync(0xffffffffu, lo4[lane & 15] != 0u)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t w = lo4[e];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) if ((int)((w >> (8 * k)) & 255u) > r) v[4 * e + k] = 0u;
+        }
+      }
+      if (diag) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e) if (ch * 64 + e < r) v[e] = 0u;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) pk[e] = bf16x2_of(__uint_as_float(v[c * 32 + 2 * e]), __uint_as_float(v[c * 32 + 2 * e + 1]));
+        tmem_st16(tS + ch * 64 + c * 16 + lane_off, pk);
+      }
+      tmem_wait_st();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.p_ready));
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.dp_full), t & 1, abort_flag))) break;
+      tcgen05_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t dp[32], pk[16];
+        tmem_ld32(tdP + ch * 64 + c * 32 + lane_off, dp);
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 nd = *reinterpret_cast<const float4*>(st.ndelta + ch * 64 + c * 32 + e);
+          const uint32_t* w = v + c * 32 + e;
+          float d0, d1, d2, d3;
+          unpack_f32x2(mul_f32x2(pack_f32x2(w[0], w[1]), fma_f32x2(pack_f32x2(dp[e], dp[e + 1]), sc, pack_f32x2(__float_as_uint(nd.x), __float_as_uint(nd.y)))), d0, d1);
+          unpack_f32x2(mul_f32x2(pack_f32x2(w[2], w[3]), fma_f32x2(pack_f32x2(dp[e + 2], dp[e + 3]), sc, pack_f32x2(__float_as_uint(nd.z), __float_as_uint(nd.w)))), d2, d3);
+          pk[e / 2] = bf16x2_of(d0, d1);
+          pk[e / 2 + 1] = bf16x2_of(d2, d3);
+        }
+        tmem_st16(tdP + ch * 64 + c * 16 + lane_off, pk);
+      }
+      tmem_wait_st();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) { mbar_arrive(smem_u32(&sh.ds_ready)); mbar_arrive(smem_u32(&sh.stat_empty[t & 1])); }
+    }
+    // dV and dK of this block.  Whole group in this CTA: TMEM -> bf16 -> staging in the Q tiles, which nothing reads any more -> the packed
+    // gradient; a part of it: in fp32 in columns of its own, which a last pass adds in order.  Without a step the first Q tile has to land.
+    if (ok) ok = n_it > 0 ? mbar_wait_warp(smem_u32(&sh.acc_full), 0, abort_flag) : mbar_wait_warp(smem_u32(&sh.ring_full[0]), 0, abort_flag);
+    if (ok) {
+      tcgen05_fence_after();
+      const int orow0 = kvrow0 + quad * 32;
+      const uint32_t stage = sQ + (uint32_t)(warp - 2) * (DH == 128 ? 8192u : 4096u), rowaddr = stage + (uint32_t)lane * 128u;
+      if (p.split > 1) {
+#pragma unroll 1
+        for (int x = 0; x < DH / 32; ++x) {                // 32-column boxes of dV, then of dK; this warp takes one column half of each
+          const int acc = x / (DH / 64), col = (DH / 64 * ch + x % (DH / 64)) * 32;
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
+          uint32_t w[32];
+          tmem_ld32((acc ? tdK : tdV) + col + lane_off, w);
+#pragma unroll
+          for (int q8 = 0; q8 < 8; ++q8) {
+            uint32_t f[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = n_it == 0 ? 0u : w[4 * q8 + e];
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + (((uint32_t)q8 ^ sw) << 4)), "r"(f[0]), "r"(f[1]), "r"(f[2]),
+                         "r"(f[3]) : "memory");
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            if (orow0 < p.S) tma_store_3d(&p.tmPart, stage, (sub * 2 * p.KV + (acc ? g : p.KV + g)) * DH + col, orow0, b);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < DH / 64; ++x) {                // at 128 columns a half of dV, then of dK; at 64 one of them
+          const int acc = DH == 128 ? x : ch, col = DH == 128 ? ch * 64 : 0;
+          const uint32_t tacc = acc ? tdK : tdV;
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t w[32];
+            tmem_ld32(tacc + col + hf * 32 + lane_off, w);
+            box_row(rowaddr + (uint32_t)x * 4096u, sw, hf, w, n_it == 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && orow0 < p.S) {
+            tma_store_3d(&p.tmDQKV, stage + (uint32_t)x * 4096u, (acc ? kcol : vcol) + col, orow0, b);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        }
+      }
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  }
+  docs_bwd_end(p, sh, warp);
+}
+
+// CTAs that share a group's query heads: the rule of the kernels above, for the longest walk that the starts may ask for.
+int docs_split(int B, int S, int H, int KV) {
+  const int group = H / KV;
+  const long long n = (S + BKV - 1) / BKV, ctas = n * KV * B;
+  int split = 1;
+  for (int s = 1; s <= group && 10 * ctas * split * (n + 1) < 18 * n * tplr_sm_count(); ++s)
+    if (group % s == 0) split = s;
+  return split;
+}
+
+template <int DH>
+int launch_docs_bwd(const void* qkv, const int* starts, const int* blocks, const void* out, const void* dout, const float* lse, float* delta,
+                    float* part, void* dqkv, int B, int S, int H, int KV, long long ld_qkv, float scale, unsigned int* status, cudaStream_t st) {
+  AttnDocsBwdParams p = {};
+  const int C = (H + 2 * KV) * DH, split = docs_split(B, S, H, KV), kv_cols = 2 * KV * DH;
+  if (split > 1 && !part) return -201;
+  if (!make_map3(&p.tmQKV, qkv, C, S, B, ld_qkv, 64, 128)) return -202;
+  if (!make_map3(&p.tmDO, dout, (long long)H * DH, S, B, (long long)H * DH, 64, 128)) return -203;
+  if (!make_map3(&p.tmDQKV, dqkv, C, S, B, C, 64, 32)) return -205;
+  if (split > 1 && !make_map3(&p.tmPart, part, (long long)split * kv_cols, S, B, (long long)split * kv_cols, 32, 32, true)) return -204;
+  p.out = (const __nv_bfloat16*)out; p.lse = lse; p.delta = delta; p.starts = starts; p.blocks = blocks;
+  p.B = B; p.S = S; p.H = H; p.KV = KV; p.split = split; p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
+  constexpr int SMEM = docs_bwd_smem<DH>();
+  const unsigned n = (unsigned)((S + BKV - 1) / BKV);
+  cudaError_t e = cudaFuncSetAttribute(attn_docs_dq_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_docs_dkv_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  if (e == cudaSuccess) e = launch_pdl(attn_docs_dq_kernel<DH>, n * H * B, DQ_THREADS, SMEM, st, p);
+  if (e == cudaSuccess) e = launch_pdl(attn_docs_dkv_kernel<DH>, n * KV * B * split, DKV_THREADS, SMEM, st, p);
+  if (e != cudaSuccess || split == 1) return (int)e;
+  // the parts' sums into the key and value columns; no query columns here
+  return (int)launch_pdl(attn_dq_cast_kernel<DH, true>, tplr_sm_count() * 8, 256, 0, st, part, part, split, (__nv_bfloat16*)dqkv + H * DH,
+                         (long long)B * S, 0, kv_cols, 0, (long long)C, nullptr, nullptr, S);
+}
+}  // namespace
+
+// Fp32 elements per token of tplr_attention_docs_bwd's workspace `part` (0: none).
+TPLR_API int tplr_attention_docs_bwd_scratch_cols(int B, int S, int H, int KV, int head_dim) {
+  if (B <= 0 || S <= 0 || KV <= 0 || H % KV) return 0;
+  const int split = docs_split(B, S, H, KV);
+  return split > 1 ? 2 * KV * split * head_dim : 0;
+}
+
+// Gradient of tplr_attention_docs_fwd, whose starts, blocks and lse it takes: dqkv [B, S, (H + 2 KV) * head_dim] dense.  out and dout dense;
+// delta: [B, H, S] fp32 scratch; part: B * S * tplr_attention_docs_bwd_scratch_cols fp32 elements, contents irrelevant.
 TPLR_API int tplr_attention_docs_bwd(const void* qkv, const int* starts, const int* blocks, const void* out, const void* dout,
-                                     const float* lse, float* delta, float* dq32, void* dqkv, int B, int S, int H, int KV, int head_dim,
+                                     const float* lse, float* delta, float* part, void* dqkv, int B, int S, int H, int KV, int head_dim,
                                      long long ld_qkv, float scale, unsigned int* status, void* stream) {
   TPLR_ENTER();
   if (B <= 0 || S <= 0) return 0;
-  if ((head_dim != 128 && head_dim != 64) || KV <= 0 || H % KV || (ld_qkv % 8) || ((uintptr_t)qkv & 15) || !starts || !blocks ||
-      ((uintptr_t)dqkv & 15) || ((uintptr_t)dout & 15) || ((uintptr_t)out & 15) || ((uintptr_t)dq32 & 15))
+  if ((head_dim != 128 && head_dim != 64) || KV <= 0 || H % KV || (ld_qkv % 8) || !starts || !blocks ||
+      (((uintptr_t)qkv | (uintptr_t)dqkv | (uintptr_t)dout | (uintptr_t)out | (uintptr_t)part) & 15))
     return -201;
-  auto run = head_dim == 128 ? launch_bwd<128, true> : launch_bwd<64, true>;
-  return run(qkv, out, dout, lse, delta, dq32, dqkv, B, S, H, KV, ld_qkv, (long long)H * head_dim, scale, nullptr, nullptr, status,
-             (cudaStream_t)stream, false, starts, blocks);
+  auto run = head_dim == 128 ? launch_docs_bwd<128> : launch_docs_bwd<64>;
+  return run(qkv, starts, blocks, out, dout, lse, delta, part, dqkv, B, S, H, KV, ld_qkv, scale, status, (cudaStream_t)stream);
 }

@@ -84,15 +84,14 @@ class _AttentionDocuments(torch.autograd.Function):
         B, S, C = qkv.shape
         with _on(qkv):
             do = OF._dense(dout)
-            # the kernel stores dk and dv with the rows of qkv
-            dqkv = torch.empty(B, S, ld, dtype=qkv.dtype, device=qkv.device)[..., :C]
+            dqkv = torch.empty(B, S, C, dtype=qkv.dtype, device=qkv.device)
             cols = native.lib().tplr_attention_docs_bwd_scratch_cols(B, S, n_heads, n_kv, hd)
-            dq32 = torch.empty(B * S * cols, dtype=torch.float32, device=qkv.device)
+            part = torch.empty(B * S * cols, dtype=torch.float32, device=qkv.device) if cols else None
             delta = torch.empty(B, n_heads, S, dtype=torch.float32, device=qkv.device)
             native.check(native.lib().tplr_attention_docs_bwd(
                 qkv.data_ptr(), starts.data_ptr(), blocks.data_ptr(), out.data_ptr(), do.data_ptr(), lse.data_ptr(), delta.data_ptr(),
-                dq32.data_ptr(), dqkv.data_ptr(), B, S, n_heads, n_kv, hd, ld, hd ** -0.5,
-                OF.status_word(qkv.device).data_ptr(), native.stream_ptr()), "attention_docs_bwd")
+                native.ptr(part), dqkv.data_ptr(), B, S, n_heads, n_kv, hd, ld, hd ** -0.5, OF.status_word(qkv.device).data_ptr(),
+                native.stream_ptr()), "attention_docs_bwd")
         return dqkv, None, None, None, None
 
 
@@ -126,8 +125,8 @@ def attention_documents(qkv: torch.Tensor, starts: torch.Tensor, n_heads: int, n
     ``max(starts[b, s], 0) .. s``; returns [B, S, H * hd], zero in rows whose start lies behind them.  ``starts``: whole numbers [B, S].
 
     Every row has to hold finite numbers, one that nothing sees too, and so has the gradient: the rows of a block of 128 meet in the
-    same products, where a weight of zero times an infinity is not zero.  On the own kernels (bf16, heads of 64 or 128) the
-    gradient of the queries is added up in fp32 in an order that may change from run to run, as :func:`attention_packed`'s is."""
+    same products, where a weight of zero times an infinity is not zero.  The kernels (bf16, heads of 64 or 128) add nothing
+    into memory: results and gradients have the same bits on every run."""
     _heads("attention_documents", qkv, n_heads, n_kv, hd)
     B, S, C = qkv.shape
     if starts.shape != (B, S) or starts.is_floating_point() or starts.is_complex() or starts.dtype == torch.bool:
