@@ -21,6 +21,7 @@
 #include "tcgen05.cuh"
 #include <cuda/std/type_traits>
 #include <limits.h>
+#include <stddef.h>
 #include <stdlib.h>
 
 namespace {
@@ -1581,7 +1582,8 @@ struct AttnDocsParams {
   float scale_log2;
   unsigned int* status;
   const int* starts;      // [B, S]
-  int* blocks;            // [B, nQ], or null: takes the least start of a row in the query block that sees anything (INT_MAX: none does)
+  int* blocks;            // [B, nQ], or null: takes the least start of a row in the query block that sees anything (INT_MAX: none does);
+                          // behind it two counters for the backward kernels, zeroed here
 };
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
@@ -1664,6 +1666,7 @@ attn_docs_fwd_kernel(const __grid_constant__ AttnDocsParams p) {
   const int least = min(min(s_least[0], s_least[1]), min(s_least[2], s_least[3]));
   const int nb = least == INT_MAX ? 0 : qi - least / BKV + 1;      // key blocks qi, qi - 1, ..
   if (p.blocks && h == 0 && threadIdx.x == 0) p.blocks[(long long)b * nQ + qi] = least;
+  if (p.blocks && blockIdx.x == 0 && threadIdx.x < 2) p.blocks[(long long)p.B * nQ + threadIdx.x] = 0;
   const uint32_t tmem_base = s_tmem_base;
   // S columns 0..127, O from column 128; P over S at DH = 128, at 64 in the 64 columns that O leaves, so that the next block's S is
   // computed as soon as the softmax warps hold this one's (AHEAD)
@@ -1894,8 +1897,8 @@ int launch_docs_fwd(const void* qkv, const int* starts, void* out, float* lse, i
 }  // namespace
 
 // tplr_attention_fwd within documents: row s of sequence b sees the keys max(starts[b * S + s], 0) .. s; one whose start lies behind it
-// sees nothing, and its output is zero.  starts: [B, S] int32, any values.  blocks: [B, ceil(S / 128)] int32 for the backward
-// pass, or null.
+// sees nothing, and its output is zero.  starts: [B, S] int32, any values.  blocks: B * ceil(S / 128) + 2 int32 for the
+// backward pass, or null.
 TPLR_API int tplr_attention_docs_fwd(const void* qkv, const int* starts, void* out, float* lse, int* blocks, int B, int S, int H, int KV,
                                      int head_dim, long long ld_qkv, long long ld_o, float scale, unsigned int* status, void* stream) {
   TPLR_ENTER();
@@ -1909,18 +1912,22 @@ TPLR_API int tplr_attention_docs_fwd(const void* qkv, const int* starts, void* o
 // ------------------------------------------------------------------------------------------ //
 // Backward within documents: two kernels, neither of which adds into memory, so the gradient has the same bits on every run.
 //
-// dQ: a CTA has a query block of one head, as the forward kernel, and walks the same key blocks in the same order.  Per step S = Q K^T, dP = dO V^T
-// (tensor cores -> TMEM), P = exp2(S * scale - lse), dS = P * (dP - delta) * scale (softmax warps, a query row a thread pair), dS as bf16 over
-// the dP columns, dQ += dS K with dS from tensor memory.  Two S buffers, so that the next exponentials run under this step's products.
-// delta, the row sum of dO * O, is formed on the way and left for the other kernel.
+// dQ: a tile is a query block of one head, as in the forward kernel, and walks the same key blocks in the same order.  Per step
+// S = Q K^T, dP = dO V^T (tensor cores -> TMEM), P = exp2(S * scale - lse), dS = P * (dP - delta) * scale (softmax warps, a query row a thread
+// pair), dS as bf16 over the dP columns, dQ += dS K with dS from tensor memory.  Two S buffers, so that the next exponentials run
+// under this step's products.  delta, the row sum of dO * O, is formed on the way and left for the other kernel.
 //
-// dK, dV: a CTA has a key/value block of one kv head and the query heads of its group, or a part of them, and walks the query blocks
+// dK, dV: a tile is a key/value block of one kv head and the query heads of its group, or a part of them, and walks the query blocks
 // from the diagonal to the last that sees any of its keys.  Everything is transposed, with the key row as the TMEM lane:
 //   S^T = K Q^T, dP^T = V dO^T;  P^T and dS^T as packed bf16 over them;  dV += P^T dO, dK += dS^T Q
-// with P^T and dS^T from tensor memory: neither goes through shared memory, whose traffic bounds the kernel above (4600 of its 5250
+// with P^T and dS^T from tensor memory: neither goes through shared memory, whose traffic bounds the causal kernel above (4600 of its 5250
 // cycles a step at DH = 128).  lse, delta and the starts belong to columns here: a warp of its own brings them to shared memory.
 //
 // Seven products instead of five, but each step is shorter, and there is no fp32 dQ to be zeroed, added into, read and rounded.
+// Walks within documents are short (four steps on average for texts of 512), and one CTA fills an SM, so its start, first loads and
+// stores would stand alone: CTAs stay and take tile after tile from a counter (static shares leave some SMs idle at the end: walks
+// differ), the loads run ahead into the next tile, and the results go from registers to memory in whole sectors, since every byte of shared
+// memory is a tile's.
 // ------------------------------------------------------------------------------------------ //
 namespace {
 
@@ -1931,28 +1938,31 @@ template <int DH> constexpr int docs_bwd_tiles() { return 7 * tile_bytes<DH>(); 
 template <int DH> constexpr int docs_bwd_smem() { return docs_bwd_tiles<DH>() + 3072; }
 
 struct DocsBwdShared {
-  uint64_t bar_res;                                        // the resident tiles
+  uint64_t res_full, res_empty;                            // the tile's resident operands
   uint64_t ring_full[RING3], ring_empty[RING3], pair_full[2], pair_empty[2];
-  uint64_t s_full[2], dp_full, p_ready, ds_ready, acc_full, stat_full[2], stat_empty[2];
+  uint64_t s_full[2], dp_full, p_ready, ds_ready, acc_full, stat_full[2], stat_empty[2], tile_full[2], tile_empty[2];
   uint32_t tmem_base;
-  int abort, last;
+  int abort;
+  int2 tile[2];                                            // (tile or -1, blocks of its walk)
   float part[2][128];                                      // dQ: halves of delta
 };
 struct DocsStats { float nlse[128], ndelta[128]; uint8_t lo[128]; };       // dK, dV: of a query block; negated, in the units of the products
-static_assert(sizeof(DocsBwdShared) <= 1536 && 512 + 2 * sizeof(DocsStats) <= 3072, "the small things fit behind the tiles");
+static_assert(sizeof(DocsBwdShared) <= 1536 && offsetof(DocsBwdShared, part) <= 512 && 512 + 2 * sizeof(DocsStats) <= 3072,
+              "the small things fit behind the tiles");
 
 struct AttnDocsBwdParams {
   CUtensorMap tmQKV;      // [B, S, C] bf16, box 64 x 128 x 1, 128-byte swizzle
   CUtensorMap tmDO;       // [B, S, H * DH] bf16, the same box
-  CUtensorMap tmDQKV;     // [B, S, C] bf16, box 64 x 32 x 1
-  CUtensorMap tmPart;     // split: [B, S, split * 2 * KV * DH] fp32, box 32 x 32 x 1 (dK | dV of every part)
   const __nv_bfloat16* out;
+  __nv_bfloat16* dqkv;    // [B, S, C] dense
+  float* part;            // split: [B, S, split, 2 * KV * DH] (dK | dV of every part)
   const float* lse;
   float* delta;           // [B, H, S]
   const int* starts;
   const int* blocks;
-  int B, S, H, KV;
-  int split;              // CTAs that share a group's query heads; > 1: each stores its part of dK and dV in fp32
+  int* next;              // tiles taken beyond the first of every CTA; zero, and zero again at the end
+  int B, S, H, KV, tiles;
+  int split;              // tiles that share a group's query heads; > 1: each stores its part of dK and dV in fp32
   float scale, scale_log2;
   unsigned int* status;
 };
@@ -1967,26 +1977,33 @@ __device__ __forceinline__ uint32_t bf16x2_of(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// 32 fp32 values of a lane's row -> bf16 in half `hh` of its row of a swizzled 32 x 64 box
-__device__ __forceinline__ void box_row(uint32_t rowaddr, uint32_t sw, int hh, const uint32_t* v, bool zero) {
+// a whole 32-byte sector
+__device__ __forceinline__ void store_sector(void* to, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+               "r"(w[6]), "r"(w[7]) : "memory");
+}
+// 32 accumulator columns of this lane's row -> 64 bytes of bf16
+__device__ __forceinline__ void store_row32(__nv_bfloat16* to, uint32_t tmem, bool zero, bool live) {
+  uint32_t v[32];
+  tmem_ld32(tmem, v);
 #pragma unroll
-  for (int q4 = 0; q4 < 4; ++q4) {
-    uint32_t pw[4];
+  for (int q = 0; q < 2; ++q) {
+    uint32_t w[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) pw[e] = zero ? 0u : bf16x2_of(__uint_as_float(v[8 * q4 + 2 * e]), __uint_as_float(v[8 * q4 + 2 * e + 1]));
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + ((((uint32_t)(hh * 4 + q4)) ^ sw) << 4)), "r"(pw[0]), "r"(pw[1]),
-                 "r"(pw[2]), "r"(pw[3]) : "memory");
+    for (int e = 0; e < 8; ++e) w[e] = zero ? 0u : bf16x2_of(__uint_as_float(v[16 * q + 2 * e]), __uint_as_float(v[16 * q + 2 * e + 1]));
+    if (live) store_sector(to + 16 * q, w);
   }
 }
-__device__ __forceinline__ void docs_bwd_init(DocsBwdShared& sh, int warp) {
+__device__ __forceinline__ void docs_bwd_init(DocsBwdShared& sh, int warp, int consumers) {
   if (threadIdx.x == 0) {
     sh.abort = 0;
-    sh.last = -1;
-    mbar_init(smem_u32(&sh.bar_res), 1);
+    mbar_init(smem_u32(&sh.res_full), 1);
+    mbar_init(smem_u32(&sh.res_empty), consumers == 9 ? 9 : 1);        // dQ: the softmax warps read dO too
     for (int s = 0; s < RING3; ++s) { mbar_init(smem_u32(&sh.ring_full[s]), 1); mbar_init(smem_u32(&sh.ring_empty[s]), 1); }
     for (int s = 0; s < 2; ++s) {
       mbar_init(smem_u32(&sh.pair_full[s]), 1); mbar_init(smem_u32(&sh.pair_empty[s]), 1); mbar_init(smem_u32(&sh.s_full[s]), 1);
       mbar_init(smem_u32(&sh.stat_full[s]), 1); mbar_init(smem_u32(&sh.stat_empty[s]), 8);
+      mbar_init(smem_u32(&sh.tile_full[s]), 1); mbar_init(smem_u32(&sh.tile_empty[s]), consumers);
     }
     mbar_init(smem_u32(&sh.dp_full), 1); mbar_init(smem_u32(&sh.p_ready), 8); mbar_init(smem_u32(&sh.ds_ready), 8);
     mbar_init(smem_u32(&sh.acc_full), 1);
@@ -1997,6 +2014,9 @@ __device__ __forceinline__ void docs_bwd_init(DocsBwdShared& sh, int warp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem_base)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
 }
 __device__ __forceinline__ void docs_bwd_end(const AttnDocsBwdParams& p, DocsBwdShared& sh, int warp) {
   __syncwarp();
@@ -2007,6 +2027,35 @@ __device__ __forceinline__ void docs_bwd_end(const AttnDocsBwdParams& p, DocsBwd
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh.tmem_base) : "memory");
   }
   if (threadIdx.x == 0 && sh.abort && p.status) atomicOr(p.status, TPLR_ST_WAIT_TIMEOUT);
+}
+// The k-th tile of a CTA for the roles that use it; false: there is none, or a wait ran out.
+__device__ __forceinline__ bool take_tile(DocsBwdShared& sh, int k, int lane, volatile int* abort_flag, int& tile, int& blocks) {
+  if (!mbar_wait_warp(smem_u32(&sh.tile_full[k & 1]), (uint32_t)((k >> 1) & 1), abort_flag)) return false;
+  tile = *reinterpret_cast<volatile int*>(&sh.tile[k & 1].x);
+  blocks = *reinterpret_cast<volatile int*>(&sh.tile[k & 1].y);
+  __syncwarp();
+  if (lane == 0) mbar_arrive(smem_u32(&sh.tile_empty[k & 1]));
+  return tile >= 0;
+}
+// The loading warp's side: publishes the k-th tile; false: a wait ran out.
+__device__ __forceinline__ bool give_tile(DocsBwdShared& sh, int k, int lane, volatile int* abort_flag, int tile, int blocks) {
+  if (!mbar_wait_warp(smem_u32(&sh.tile_empty[k & 1]), (uint32_t)(((k >> 1) & 1) ^ 1), abort_flag)) return false;
+  if (lane == 0) {
+    sh.tile[k & 1] = make_int2(tile, blocks);
+    mbar_arrive(smem_u32(&sh.tile_full[k & 1]));
+  }
+  return true;
+}
+// The tile behind this one.  Every CTA asks until it is told of none, so there are as many questions as tiles; the last one leaves the
+// counter as it was.
+__device__ __forceinline__ int next_tile(const AttnDocsBwdParams& p, int lane) {
+  int n = 0;
+  if (lane == 0) {
+    n = atomicAdd(p.next, 1);
+    if (n == p.tiles - 1) *p.next = 0;
+    n += (int)gridDim.x;
+  }
+  return __shfl_sync(0xffffffffu, n, 0);
 }
 // offsets of a 16-wide k step in a tile of 128 rows, in 16-byte units: along the 128-byte rows, and along the rows of the tile
 __device__ __forceinline__ constexpr uint32_t koff(int kk) { return (uint32_t)(kk >> 2) * (128u * 128u / 16u) + (uint32_t)(kk & 3) * 2u; }
@@ -2020,62 +2069,67 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
   DocsBwdShared& sh = *reinterpret_cast<DocsBwdShared*>(smem + docs_bwd_tiles<DH>());
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
-  const int nQ = (p.S + BQ - 1) / BQ;
-  const int hb = p.H * p.B;
-  const int qi = nQ - 1 - (int)(blockIdx.x / hb);
-  const int h = (int)(blockIdx.x % hb) % p.H, b = (int)(blockIdx.x % hb) / p.H;
-  const int g = h / (p.H / p.KV);
-  const int row0 = qi * BQ;
-  const int qcol = h * DH, kcol = (p.H + g) * DH, vcol = (p.H + p.KV + g) * DH;
+  const int nQ = (p.S + BQ - 1) / BQ, hb = p.H * p.B, group = p.H / p.KV;
+  const int C = (p.H + 2 * p.KV) * DH;
   volatile int* abort_flag = &sh.abort;
-
   const uint32_t sQ = smem_u32(smem), sdO = sQ + TILE_BYTES, sK = sdO + TILE_BYTES, sV = sK + RING3 * TILE_BYTES;
-  docs_bwd_init(sh, warp);
-  if (threadIdx.x == 0) { prefetch_map(&p.tmQKV); prefetch_map(&p.tmDO); prefetch_map(&p.tmDQKV); }
+  // tiles: late query blocks first, all heads and sequences of one behind each other
+  auto place = [&](int tile, int& qi, int& h, int& b) {
+    qi = nQ - 1 - tile / hb;
+    h = tile % hb % p.H;
+    b = tile % hb / p.H;
+  };
+  if (threadIdx.x == 0) { prefetch_map(&p.tmQKV); prefetch_map(&p.tmDO); }
+  docs_bwd_init(sh, warp, 9);
   grid_wait();
   grid_release();
-  if (threadIdx.x == 0) {                                  // Q, dO and the diagonal's K and V; the barriers are this thread's own so far
-    mbar_expect_tx(smem_u32(&sh.bar_res), 2 * TILE_BYTES);
-    load_tile<DH>(sQ, &p.tmQKV, smem_u32(&sh.bar_res), qcol, row0, b);
-    load_tile<DH>(sdO, &p.tmDO, smem_u32(&sh.bar_res), qcol, row0, b);
-    mbar_expect_tx(smem_u32(&sh.ring_full[0]), TILE_BYTES);
-    load_tile<DH>(sK, &p.tmQKV, smem_u32(&sh.ring_full[0]), kcol, row0, b);
-    mbar_expect_tx(smem_u32(&sh.pair_full[0]), TILE_BYTES);
-    load_tile<DH>(sV, &p.tmQKV, smem_u32(&sh.pair_full[0]), vcol, row0, b);
-  }
-  __syncwarp();
-  const int least = p.blocks[(long long)b * nQ + qi];
-  const int nb = least == INT_MAX ? 0 : qi - least / BKV + 1;      // key blocks qi, qi - 1, ..
-  tcgen05_fence_before();
-  __syncthreads();
-  tcgen05_fence_after();
   const uint32_t tmem_base = sh.tmem_base;
   const uint32_t tdP = tmem_base + 128, tdQ = tmem_base + 256;       // S of even steps in columns 0..127, of odd ones in 384..511
 
   if (warp == 0) {
-    const bool leader = elect_one();
     bool ok = true;
-    int n_k = 1, n_v = 1, s3 = 1;
+    int k = 0, n_k = 0, n_v = 0, s3 = 0;                   // tiles begun, K and V tiles asked for
     uint32_t ph3 = 0;
-    for (int t = 1; t < nb && ok; ++t) {
-      const int krow = (qi - t) * BKV, s2 = t & 1;
-      if (!(ok = mbar_wait_warp(smem_u32(&sh.ring_empty[s3]), ph3 ^ 1u, abort_flag))) break;
-      if (leader) {
-        mbar_expect_tx(smem_u32(&sh.ring_full[s3]), TILE_BYTES);
-        load_tile<DH>(sK + s3 * TILE_BYTES, &p.tmQKV, smem_u32(&sh.ring_full[s3]), kcol, krow, b);
+    for (int tile = (int)blockIdx.x;; ++k) {
+      int qi = 0, h = 0, b = 0, nb = 0;
+      if (tile < p.tiles) {
+        place(tile, qi, h, b);
+        const int least = p.blocks[(long long)b * nQ + qi];
+        nb = least == INT_MAX ? 0 : qi - least / BKV + 1;  // key blocks qi, qi - 1, ..
       }
-      ++n_k;
-      if (++s3 == RING3) { s3 = 0; ph3 ^= 1u; }
-      if (!(ok = mbar_wait_warp(smem_u32(&sh.pair_empty[s2]), (uint32_t)(((t >> 1) & 1) ^ 1), abort_flag))) break;
-      if (leader) {
-        mbar_expect_tx(smem_u32(&sh.pair_full[s2]), TILE_BYTES);
-        load_tile<DH>(sV + s2 * TILE_BYTES, &p.tmQKV, smem_u32(&sh.pair_full[s2]), vcol, krow, b);
+      if (!(ok = give_tile(sh, k, lane, abort_flag, tile < p.tiles ? tile : -1, nb)) || tile >= p.tiles) break;
+      const int row0 = qi * BQ, qcol = h * DH, kcol = (p.H + h / group) * DH, vcol = (p.H + p.KV + h / group) * DH;
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.res_empty), (uint32_t)((k & 1) ^ 1), abort_flag))) break;
+      if (lane == 0) {
+        mbar_expect_tx(smem_u32(&sh.res_full), 2 * TILE_BYTES);
+        load_tile<DH>(sQ, &p.tmQKV, smem_u32(&sh.res_full), qcol, row0, b);
+        load_tile<DH>(sdO, &p.tmDO, smem_u32(&sh.res_full), qcol, row0, b);
       }
-      ++n_v;
+      __syncwarp();
+      for (int t = 0; t < nb && ok; ++t) {
+        const int krow = (qi - t) * BKV, s2 = n_v & 1;
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.ring_empty[s3]), ph3 ^ 1u, abort_flag))) break;
+        if (lane == 0) {
+          mbar_expect_tx(smem_u32(&sh.ring_full[s3]), TILE_BYTES);
+          load_tile<DH>(sK + s3 * TILE_BYTES, &p.tmQKV, smem_u32(&sh.ring_full[s3]), kcol, krow, b);
+        }
+        __syncwarp();
+        ++n_k;
+        if (++s3 == RING3) { s3 = 0; ph3 ^= 1u; }
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.pair_empty[s2]), (uint32_t)(((n_v >> 1) & 1) ^ 1), abort_flag))) break;
+        if (lane == 0) {
+          mbar_expect_tx(smem_u32(&sh.pair_full[s2]), TILE_BYTES);
+          load_tile<DH>(sV + s2 * TILE_BYTES, &p.tmQKV, smem_u32(&sh.pair_full[s2]), vcol, krow, b);
+        }
+        __syncwarp();
+        ++n_v;
+      }
+      if (!ok) { ++k; break; }
+      tile = next_tile(p, lane);                           // not before its loads can begin: walks differ, and a tile taken early waits
     }
-    if (leader) {
+    if (lane == 0) {
       Drain drain;                                         // no load may land after the CTA has retired: a role may have given up
-      drain.wait(smem_u32(&sh.bar_res), 0);
+      if (k) drain.wait(smem_u32(&sh.res_full), (uint32_t)((k - 1) & 1));
       for (int t = max(n_k - RING3, 0); t < n_k; ++t) drain.wait(smem_u32(&sh.ring_full[t % RING3]), (uint32_t)((t / RING3) & 1));
       for (int t = max(n_v - 2, 0); t < n_v; ++t) drain.wait(smem_u32(&sh.pair_full[t & 1]), (uint32_t)((t >> 1) & 1));
     }
@@ -2084,160 +2138,168 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
     const uint32_t id_kk = idesc_mn(128, false, false), id_km = idesc_mn(DH, false, true);
     const DescBase kQ = desc_base(sQ, 16, 1024), kdO = desc_base(sdO, 16, 1024), kK = desc_base(sK, 16, 1024), kV = desc_base(sV, 16, 1024),
                    mK = desc_base(sK, 128 * 128, 1024);
-    int s3 = 0;                                            // ring place of the next S's K
+    int s3 = 0, r3 = 0;                                    // ring places of the next S's and of the next dQ's K
     uint32_t ph3 = 0;
-    auto issue_s = [&](int t) -> bool {
+    int n = 0;                                             // steps so far
+    auto issue_s = [&](int step) -> bool {
       if (!mbar_wait_warp(smem_u32(&sh.ring_full[s3]), ph3, abort_flag)) return false;
       tcgen05_fence_after();
       if (leader) {
-        const uint32_t d = tmem_base + (t & 1) * 384, k = (uint32_t)s3 * (TILE_BYTES / 16);
+        const uint32_t d = tmem_base + (step & 1) * 384, q = (uint32_t)s3 * (TILE_BYTES / 16);
 #pragma unroll
-        for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(d, kQ, koff(kk), kK, k + koff(kk), id_kk, kk > 0 ? 1u : 0u);
-        umma_commit(smem_u32(&sh.s_full[t & 1]));
+        for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(d, kQ, koff(kk), kK, q + koff(kk), id_kk, kk > 0 ? 1u : 0u);
+        umma_commit(smem_u32(&sh.s_full[step & 1]));
       }
       if (++s3 == RING3) { s3 = 0; ph3 ^= 1u; }
       return true;
     };
-    auto issue_dp = [&](int t) -> bool {
-      if (!mbar_wait_warp(smem_u32(&sh.pair_full[t & 1]), (uint32_t)((t >> 1) & 1), abort_flag)) return false;
+    auto issue_dp = [&](int step, bool last) -> bool {
+      if (!mbar_wait_warp(smem_u32(&sh.pair_full[step & 1]), (uint32_t)((step >> 1) & 1), abort_flag)) return false;
       tcgen05_fence_after();
       if (leader) {
-        const uint32_t v = (uint32_t)(t & 1) * (TILE_BYTES / 16);
+        const uint32_t v = (uint32_t)(step & 1) * (TILE_BYTES / 16);
 #pragma unroll
         for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(tdP, kdO, koff(kk), kV, v + koff(kk), id_kk, kk > 0 ? 1u : 0u);
         umma_commit(smem_u32(&sh.dp_full));
-        umma_commit(smem_u32(&sh.pair_empty[t & 1]));
+        umma_commit(smem_u32(&sh.pair_empty[step & 1]));
+        if (last) umma_commit(smem_u32(&sh.res_empty));    // no product reads Q or dO any more
       }
       return true;
     };
-    bool ok = nb > 0 && mbar_wait_warp(smem_u32(&sh.bar_res), 0, abort_flag);
-    if (ok) ok = issue_s(0);
-    if (ok) ok = issue_dp(0);
-    int r3 = 0;                                            // ring place of this step's K
-    for (int t = 0; t < nb && ok; ++t) {
-      // the S buffer of step t + 1 was read by every warp in front of dS(t - 1)
-      if (t + 1 < nb && !(ok = issue_s(t + 1))) break;
-      if (!(ok = mbar_wait_warp(smem_u32(&sh.ds_ready), t & 1, abort_flag))) break;
-      tcgen05_fence_after();
-      if (leader) {
-        const uint32_t k = (uint32_t)r3 * (TILE_BYTES / 16);
-#pragma unroll
-        for (int kk = 0; kk < BKV / 16; ++kk)              // dQ[q, d] += dS[q, kv] K[kv, d]; dS packed in the first half of each warp's dP columns
-          umma_ts_bf16_b(tdQ, tdP + (kk >> 2) * 64 + 8 * (kk & 3), mK, k + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(smem_u32(&sh.ring_empty[r3]));
-        if (t == nb - 1) umma_commit(smem_u32(&sh.acc_full));
+    bool ok = true;
+    int tile, nb;
+    for (int k = 0; ok && take_tile(sh, k, lane, abort_flag, tile, nb); ++k) {
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.res_full), (uint32_t)(k & 1), abort_flag))) break;
+      if (nb == 0) {
+        if (leader) mbar_arrive(smem_u32(&sh.res_empty));
+        continue;
       }
-      if (++r3 == RING3) r3 = 0;
-      if (t + 1 < nb && !(ok = issue_dp(t + 1))) break;    // behind dQ(t), which reads dS(t) from its columns
+      // the S buffer of the first step was read by every warp in front of the last dS but one, its dP columns by the last dQ
+      if (!(ok = issue_s(n))) break;
+      if (!(ok = issue_dp(n, nb == 1))) break;
+      for (int t = 0; t < nb; ++t, ++n) {
+        if (t + 1 < nb && !(ok = issue_s(n + 1))) break;
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.ds_ready), n & 1, abort_flag))) break;
+        tcgen05_fence_after();
+        if (leader) {
+          const uint32_t q = (uint32_t)r3 * (TILE_BYTES / 16);
+#pragma unroll
+          for (int kk = 0; kk < BKV / 16; ++kk)            // dQ[q, d] += dS[q, kv] K[kv, d]; dS packed in the first half of each warp's dP columns
+            umma_ts_bf16_b(tdQ, tdP + (kk >> 2) * 64 + 8 * (kk & 3), mK, q + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(smem_u32(&sh.ring_empty[r3]));
+          if (t == nb - 1) umma_commit(smem_u32(&sh.acc_full));
+        }
+        if (++r3 == RING3) r3 = 0;
+        if (t + 1 < nb && !(ok = issue_dp(n + 1, t + 2 == nb))) break;       // behind dQ(t), which reads dS(t) from its columns
+      }
     }
   } else {
     const int quad = warp & 3, ch = (warp - 2) >> 2;       // TMEM lanes, column half
-    const int r = quad * 32 + lane, row = row0 + r;
+    const int r = quad * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const uint32_t sw = (uint32_t)(lane & 7);
-    const long long at = ((long long)b * p.H + h) * p.S + row;
-    int start = INT_MAX;                                   // INT_MAX: the row sees nothing, or is past the end
-    float lse2 = INFINITY;
-    uint4 o[DH / 16];                                      // this half of the row's output
+    const unsigned long long sl2 = two(p.scale_log2), sc = two(p.scale);
+    int n = 0, n_acc = 0;                                  // steps and tiles with a step so far
+    int tile, nb;
+    bool ok = true;
+    for (int k = 0;; ++k) {
+      // both warps of a pair leave the loop together: they join their answers wherever one could leave alone
+      ok = take_tile(sh, k, lane, abort_flag, tile, nb);
+      if (!pair_agrees(ok, quad)) break;
+      int qi, h, b;
+      place(tile, qi, h, b);
+      const int row = qi * BQ + r;
+      const long long at = ((long long)b * p.H + h) * p.S + row;
+      int start = INT_MAX;                                 // INT_MAX: the row sees nothing, or is past the end
+      float lse2 = INFINITY;
+      uint4 o[DH / 16];                                    // this half of the row's output
 #pragma unroll
-    for (int q = 0; q < DH / 16; ++q) o[q] = make_uint4(0u, 0u, 0u, 0u);
-    if (row < p.S) {
-      start = max(p.starts[(long long)b * p.S + row], 0);
-      if (start > row) start = INT_MAX;
-      if (start != INT_MAX) {
-        lse2 = p.lse[at] * 1.4426950408889634f;
-        const uint4* orow = reinterpret_cast<const uint4*>(p.out + ((long long)b * p.S + row) * ((long long)p.H * DH) + h * DH + ch * (DH / 2));
+      for (int q = 0; q < DH / 16; ++q) o[q] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < p.S) {
+        start = max(p.starts[(long long)b * p.S + row], 0);
+        if (start > row) start = INT_MAX;
+        if (start != INT_MAX) {
+          lse2 = p.lse[at] * 1.4426950408889634f;
+          const uint4* orow = reinterpret_cast<const uint4*>(p.out + ((long long)b * p.S + row) * ((long long)p.H * DH) + h * DH + ch * (DH / 2));
 #pragma unroll
-        for (int q = 0; q < DH / 16; ++q) o[q] = orow[q];
-      }
-    }
-    bool ok = mbar_wait_warp(smem_u32(&sh.bar_res), 0, abort_flag);
-    float delta = 0.f;
-    if (ok) {
-      // this lane's row of dO: 64 columns a box of 128-byte rows
-      const uint32_t drow = sdO + (DH == 128 ? (uint32_t)ch * (128u * 128u) : 0u) + (uint32_t)r * 128u;
-#pragma unroll
-      for (int q = 0; q < DH / 16; ++q) {
-        uint32_t d[4];
-        const uint32_t jj = (uint32_t)(DH == 128 ? q : ch * 4 + q);
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(drow + ((jj ^ sw) << 4)) : "memory");
-        const uint32_t ow[4] = {o[q].x, o[q].y, o[q].z, o[q].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          delta = fmaf(__uint_as_float(ow[e] << 16), __uint_as_float(d[e] << 16), delta);
-          delta = fmaf(__uint_as_float(ow[e] & 0xffff0000u), __uint_as_float(d[e] & 0xffff0000u), delta);
+          for (int q = 0; q < DH / 16; ++q) o[q] = orow[q];
         }
       }
-      sh.part[ch][r] = delta;
-    }
-    ok = pair_agrees(ok, quad);
-    if (ok) {
+      ok = mbar_wait_warp(smem_u32(&sh.res_full), (uint32_t)(k & 1), abort_flag);
+      float delta = 0.f;
+      if (ok) {
+        // this lane's row of dO: 64 columns a box of 128-byte rows
+        const uint32_t drow = sdO + (DH == 128 ? (uint32_t)ch * (128u * 128u) : 0u) + (uint32_t)r * 128u;
+#pragma unroll
+        for (int q = 0; q < DH / 16; ++q) {
+          uint32_t d[4];
+          const uint32_t jj = (uint32_t)(DH == 128 ? q : ch * 4 + q);
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(drow + ((jj ^ sw) << 4)) : "memory");
+          const uint32_t ow[4] = {o[q].x, o[q].y, o[q].z, o[q].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            delta = fmaf(__uint_as_float(ow[e] << 16), __uint_as_float(d[e] << 16), delta);
+            delta = fmaf(__uint_as_float(ow[e] & 0xffff0000u), __uint_as_float(d[e] & 0xffff0000u), delta);
+          }
+        }
+        sh.part[ch][r] = delta;                            // read by the partner in front of the joint barrier at the tile's end
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.res_empty));
+      }
+      if (!(ok = pair_agrees(ok, quad))) break;
       delta = start == INT_MAX ? 0.f : sh.part[0][r] + sh.part[1][r];
       if (ch == 0 && row < p.S) p.delta[at] = delta;
-    }
-    const unsigned long long sl2 = two(p.scale_log2), nl = two(-lse2), sc = two(p.scale), nd = two(-delta * p.scale);
-    for (int t = 0; t < nb && ok; ++t) {
-      const bool diag = t == 0;
-      const int lo = (start == INT_MAX ? BKV : start - (qi - t) * BKV) - ch * 64, hi = (diag ? r : BKV - 1) - ch * 64;
-      if (!(ok = mbar_wait_warp(smem_u32(&sh.s_full[t & 1]), (uint32_t)((t >> 1) & 1), abort_flag))) break;
-      tcgen05_fence_after();
-      uint32_t v[64];
-      const uint32_t tS = tmem_base + (t & 1) * 384 + ch * 64 + lane_off;
-      tmem_ld32_nowait(tS, v);
-      tmem_ld32_nowait(tS + 32, v + 32);
-      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      behind_wait32(v);
-      behind_wait32(v + 32);
+      const unsigned long long nl = two(-lse2), nd = two(-delta * p.scale);
+      for (int t = 0; t < nb; ++t, ++n) {
+        const bool diag = t == 0;
+        const int lo = (start == INT_MAX ? BKV : start - (qi - t) * BKV) - ch * 64, hi = (diag ? r : BKV - 1) - ch * 64;
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.s_full[n & 1]), (uint32_t)((n >> 1) & 1), abort_flag))) break;
+        tcgen05_fence_after();
+        uint32_t v[64];
+        const uint32_t tS = tmem_base + (n & 1) * 384 + ch * 64 + lane_off;
+        tmem_ld32_nowait(tS, v);
+        tmem_ld32_nowait(tS + 32, v + 32);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        behind_wait32(v);
+        behind_wait32(v + 32);
 #pragma unroll
-      for (int e = 0; e < 64; e += 2) {
-        float a0, a1;
-        unpack_f32x2(fma_f32x2(pack_f32x2(v[e], v[e + 1]), sl2, nl), a0, a1);
-        v[e] = __float_as_uint(exp2f(a0));
-        v[e + 1] = __float_as_uint(exp2f(a1));
-      }
-      if (__any_sync(0xffffffffu, lo > 0 || hi < 63)) {
-#pragma unroll
-        for (int e = 0; e < 64; ++e) if (e < lo || e > hi) v[e] = 0u;
-      }
-      if (!(ok = mbar_wait_warp(smem_u32(&sh.dp_full), t & 1, abort_flag))) break;
-      tcgen05_fence_after();
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t dp[32], pk[16];
-        tmem_ld32(tdP + ch * 64 + c * 32 + lane_off, dp);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float d0, d1;
-          unpack_f32x2(mul_f32x2(pack_f32x2(v[c * 32 + 2 * e], v[c * 32 + 2 * e + 1]), fma_f32x2(pack_f32x2(dp[2 * e], dp[2 * e + 1]), sc, nd)), d0, d1);
-          pk[e] = bf16x2_of(d0, d1);
+        for (int e = 0; e < 64; e += 2) {
+          float a0, a1;
+          unpack_f32x2(fma_f32x2(pack_f32x2(v[e], v[e + 1]), sl2, nl), a0, a1);
+          v[e] = __float_as_uint(exp2f(a0));
+          v[e + 1] = __float_as_uint(exp2f(a1));
         }
-        tmem_st16(tdP + ch * 64 + c * 16 + lane_off, pk);
-      }
-      tmem_wait_st();
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.ds_ready));
-    }
-    // dQ -> bf16 -> the bytes of the Q tile -> the query columns of the gradient
-    if (ok && nb > 0) ok = mbar_wait_warp(smem_u32(&sh.acc_full), 0, abort_flag);
-    ok = pair_agrees(ok, quad);
-    if (ok) {
-      tcgen05_fence_after();
-      const uint32_t stage = sQ + (uint32_t)quad * (32u * DH * 2u) + (DH == 128 ? (uint32_t)ch * 4096u : 0u), rowaddr = stage + (uint32_t)lane * 128u;
+        if (__any_sync(0xffffffffu, lo > 0 || hi < 63)) {
 #pragma unroll
-      for (int c = 0; c < DH / 64; ++c) {
-        uint32_t q[32];
-        tmem_ld32(tdQ + ch * (DH / 2) + c * 32 + lane_off, q);
-        box_row(rowaddr, sw, DH == 128 ? c : ch, q, nb == 0);
+          for (int e = 0; e < 64; ++e) if (e < lo || e > hi) v[e] = 0u;
+        }
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.dp_full), n & 1, abort_flag))) break;
+        tcgen05_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t dp[32], pk[16];
+          tmem_ld32(tdP + ch * 64 + c * 32 + lane_off, dp);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float d0, d1;
+            unpack_f32x2(mul_f32x2(pack_f32x2(v[c * 32 + 2 * e], v[c * 32 + 2 * e + 1]), fma_f32x2(pack_f32x2(dp[2 * e], dp[2 * e + 1]), sc, nd)), d0, d1);
+            pk[e] = bf16x2_of(d0, d1);
+          }
+          tmem_st16(tdP + ch * 64 + c * 16 + lane_off, pk);
+        }
+        tmem_wait_st();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.ds_ready));
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (DH == 64) (void)pair_agrees(true, quad);         // one box of 64 columns for both
-      if (lane == 0 && row0 + quad * 32 < p.S && (DH == 128 || ch == 0)) {
-        tma_store_3d(&p.tmDQKV, stage, qcol + (DH == 128 ? ch * 64 : 0), row0 + quad * 32, b);
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-      }
+      // dQ -> bf16 -> the query columns of the gradient
+      if (ok && nb > 0) ok = mbar_wait_warp(smem_u32(&sh.acc_full), (uint32_t)(n_acc++ & 1), abort_flag);
+      if (!(ok = pair_agrees(ok, quad))) break;
+      tcgen05_fence_after();
+      __nv_bfloat16* to = p.dqkv + ((long long)b * p.S + row) * C + h * DH + ch * (DH / 2);
+#pragma unroll
+      for (int c = 0; c < DH / 64; ++c) store_row32(to + c * 32, tdQ + ch * (DH / 2) + c * 32 + lane_off, nb == 0, row < p.S);
+      tcgen05_fence_before();                              // the next tile's first dQ is behind this warp's next dS
     }
   }
   docs_bwd_end(p, sh, warp);
@@ -2252,71 +2314,80 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
   DocsStats* stats = reinterpret_cast<DocsStats*>(smem + docs_bwd_tiles<DH>() + 512);      // over `part`, which this kernel has no use for
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
-  const int nQ = (p.S + BQ - 1) / BQ;
-  const int gb = p.KV * p.B * p.split;
-  const int j = (int)(blockIdx.x / gb);                    // key block; small j (which may be seen by the most rows) first
-  const int sub = (int)(blockIdx.x % gb) % p.split;
-  const int g = (int)(blockIdx.x % gb) / p.split % p.KV, b = (int)(blockIdx.x % gb) / p.split / p.KV;
-  const int heads = p.H / p.KV / p.split, h0 = (g * p.split + sub) * heads;      // query heads of this CTA
-  const int kvrow0 = j * BKV;
-  const int kcol = (p.H + g) * DH, vcol = (p.H + p.KV + g) * DH;
+  const int nQ = (p.S + BQ - 1) / BQ, gb = p.KV * p.B * p.split;
+  const int heads = p.H / p.KV / p.split;                  // query heads of a tile
+  const int C = (p.H + 2 * p.KV) * DH;
   volatile int* abort_flag = &sh.abort;
-
   const uint32_t sK = smem_u32(smem), sV = sK + TILE_BYTES, sQ = sV + TILE_BYTES, sdO = sQ + RING3 * TILE_BYTES;
-  docs_bwd_init(sh, warp);
-  if (threadIdx.x == 0) { prefetch_map(&p.tmQKV); prefetch_map(&p.tmDO); prefetch_map(&p.tmDQKV); }
-  __syncthreads();                                         // `last` is set
+  // tiles: early key blocks, which may be seen by the most rows, first
+  struct Place { int j, sub, g, b, h0; };
+  auto place = [&](int tile) {
+    Place a;
+    a.j = tile / gb;
+    a.sub = tile % gb % p.split;
+    a.g = tile % gb / p.split % p.KV;
+    a.b = tile % gb / p.split / p.KV;
+    a.h0 = (a.g * p.split + a.sub) * heads;
+    return a;
+  };
+  if (threadIdx.x == 0) { prefetch_map(&p.tmQKV); prefetch_map(&p.tmDO); }
+  docs_bwd_init(sh, warp, 10);
   grid_wait();
   grid_release();
-  if (threadIdx.x == 0) {                                  // K, V and the diagonal's Q and dO, on their way while the walk's end is looked up
-    mbar_expect_tx(smem_u32(&sh.bar_res), 2 * TILE_BYTES);
-    load_tile<DH>(sK, &p.tmQKV, smem_u32(&sh.bar_res), kcol, kvrow0, b);
-    load_tile<DH>(sV, &p.tmQKV, smem_u32(&sh.bar_res), vcol, kvrow0, b);
-    mbar_expect_tx(smem_u32(&sh.ring_full[0]), TILE_BYTES);
-    load_tile<DH>(sQ, &p.tmQKV, smem_u32(&sh.ring_full[0]), h0 * DH, kvrow0, b);
-    mbar_expect_tx(smem_u32(&sh.pair_full[0]), TILE_BYTES);
-    load_tile<DH>(sdO, &p.tmDO, smem_u32(&sh.pair_full[0]), h0 * DH, kvrow0, b);
-  }
-  __syncwarp();
-  // the last query block that sees any key of this one.  A block in between whose rows begin behind it is walked with all its weights
-  // masked: starts that grow with the row, as documents' do, have none.
-  int last = -1;
-  for (int i = j + (int)threadIdx.x; i < nQ; i += DKV_THREADS)
-    if (p.blocks[(long long)b * nQ + i] < kvrow0 + BKV) last = i;
-  if (last >= 0) atomicMax(&sh.last, last);
-  tcgen05_fence_before();
-  __syncthreads();
-  tcgen05_fence_after();
-  const int n_i = max(sh.last - j + 1, 0), n_it = heads * n_i;
   const uint32_t tmem_base = sh.tmem_base;
   const uint32_t tS = tmem_base, tdP = tmem_base + 128, tdV = tmem_base + 256, tdK = tmem_base + 384;
 
   if (warp == 0) {
-    const bool leader = elect_one();
     bool ok = true;
-    int n_q = 1, n_do = 1, s3 = 1, h = h0, i = 1;
+    int k = 0, n_q = 0, n_do = 0, s3 = 0;                  // tiles begun, Q and dO tiles asked for
     uint32_t ph3 = 0;
-    if (i == n_i) { i = 0; ++h; }
-    for (int t = 1; t < n_it && ok; ++t) {
-      const int qrow0 = (j + i) * BQ, s2 = t & 1;
-      if (!(ok = mbar_wait_warp(smem_u32(&sh.ring_empty[s3]), ph3 ^ 1u, abort_flag))) break;
-      if (leader) {
-        mbar_expect_tx(smem_u32(&sh.ring_full[s3]), TILE_BYTES);
-        load_tile<DH>(sQ + s3 * TILE_BYTES, &p.tmQKV, smem_u32(&sh.ring_full[s3]), h * DH, qrow0, b);
+    for (int tile = (int)blockIdx.x;; ++k) {
+      Place a = {};
+      int n_i = 0;
+      if (tile < p.tiles) {
+        // the last query block that sees any key of this one.  A block in between whose rows begin behind it is walked with all its
+        // weights masked: starts that grow with the row, as documents' do, have none.
+        a = place(tile);
+        int last = -1;
+        for (int i = a.j + lane; i < nQ; i += 32)
+          if (p.blocks[(long long)a.b * nQ + i] < (a.j + 1) * BKV) last = i;
+        n_i = max(__reduce_max_sync(0xffffffffu, last) - a.j + 1, 0);
       }
-      ++n_q;
-      if (++s3 == RING3) { s3 = 0; ph3 ^= 1u; }
-      if (!(ok = mbar_wait_warp(smem_u32(&sh.pair_empty[s2]), (uint32_t)(((t >> 1) & 1) ^ 1), abort_flag))) break;
-      if (leader) {
-        mbar_expect_tx(smem_u32(&sh.pair_full[s2]), TILE_BYTES);
-        load_tile<DH>(sdO + s2 * TILE_BYTES, &p.tmDO, smem_u32(&sh.pair_full[s2]), h * DH, qrow0, b);
+      if (!(ok = give_tile(sh, k, lane, abort_flag, tile < p.tiles ? tile : -1, n_i)) || tile >= p.tiles) break;
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.res_empty), (uint32_t)((k & 1) ^ 1), abort_flag))) break;
+      if (lane == 0) {
+        mbar_expect_tx(smem_u32(&sh.res_full), 2 * TILE_BYTES);
+        load_tile<DH>(sK, &p.tmQKV, smem_u32(&sh.res_full), (p.H + a.g) * DH, a.j * BKV, a.b);
+        load_tile<DH>(sV, &p.tmQKV, smem_u32(&sh.res_full), (p.H + p.KV + a.g) * DH, a.j * BKV, a.b);
       }
-      ++n_do;
-      if (++i == n_i) { i = 0; ++h; }
+      __syncwarp();
+      const int n_it = heads * n_i;
+      int h = a.h0, i = 0;
+      for (int t = 0; t < n_it && ok; ++t) {
+        const int qrow0 = (a.j + i) * BQ, s2 = n_do & 1;
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.ring_empty[s3]), ph3 ^ 1u, abort_flag))) break;
+        if (lane == 0) {
+          mbar_expect_tx(smem_u32(&sh.ring_full[s3]), TILE_BYTES);
+          load_tile<DH>(sQ + s3 * TILE_BYTES, &p.tmQKV, smem_u32(&sh.ring_full[s3]), h * DH, qrow0, a.b);
+        }
+        __syncwarp();
+        ++n_q;
+        if (++s3 == RING3) { s3 = 0; ph3 ^= 1u; }
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.pair_empty[s2]), (uint32_t)(((n_do >> 1) & 1) ^ 1), abort_flag))) break;
+        if (lane == 0) {
+          mbar_expect_tx(smem_u32(&sh.pair_full[s2]), TILE_BYTES);
+          load_tile<DH>(sdO + s2 * TILE_BYTES, &p.tmDO, smem_u32(&sh.pair_full[s2]), h * DH, qrow0, a.b);
+        }
+        __syncwarp();
+        ++n_do;
+        if (++i == n_i) { i = 0; ++h; }
+      }
+      if (!ok) { ++k; break; }
+      tile = next_tile(p, lane);                           // not before its loads can begin: walks differ, and a tile taken early waits
     }
-    if (leader) {
+    if (lane == 0) {
       Drain drain;                                         // no load may land after the CTA has retired: a role may have given up
-      drain.wait(smem_u32(&sh.bar_res), 0);
+      if (k) drain.wait(smem_u32(&sh.res_full), (uint32_t)((k - 1) & 1));
       for (int t = max(n_q - RING3, 0); t < n_q; ++t) drain.wait(smem_u32(&sh.ring_full[t % RING3]), (uint32_t)((t / RING3) & 1));
       for (int t = max(n_do - 2, 0); t < n_do; ++t) drain.wait(smem_u32(&sh.pair_full[t & 1]), (uint32_t)((t >> 1) & 1));
     }
@@ -2325,8 +2396,9 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
     const uint32_t id_kk = idesc_mn(128, false, false), id_km = idesc_mn(DH, false, true);
     const DescBase kK = desc_base(sK, 16, 1024), kV = desc_base(sV, 16, 1024), kQ = desc_base(sQ, 16, 1024), kdO = desc_base(sdO, 16, 1024),
                    mQ = desc_base(sQ, 128 * 128, 1024), mdO = desc_base(sdO, 128 * 128, 1024);
-    int s3 = 0;                                            // ring place of the next S's Q
+    int s3 = 0, r3 = 0;                                    // ring places of the next S's and of the next dK's Q
     uint32_t ph3 = 0;
+    int n = 0;                                             // steps so far
     auto issue_s = [&]() -> bool {                         // S^T = K Q^T
       if (!mbar_wait_warp(smem_u32(&sh.ring_full[s3]), ph3, abort_flag)) return false;
       tcgen05_fence_after();
@@ -2339,203 +2411,204 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       if (++s3 == RING3) { s3 = 0; ph3 ^= 1u; }
       return true;
     };
-    auto issue_dp = [&](int t) -> bool {                   // dP^T = V dO^T
-      if (!mbar_wait_warp(smem_u32(&sh.pair_full[t & 1]), (uint32_t)((t >> 1) & 1), abort_flag)) return false;
+    auto issue_dp = [&](int step, bool last) -> bool {     // dP^T = V dO^T
+      if (!mbar_wait_warp(smem_u32(&sh.pair_full[step & 1]), (uint32_t)((step >> 1) & 1), abort_flag)) return false;
       tcgen05_fence_after();
       if (leader) {
-        const uint32_t d = (uint32_t)(t & 1) * (TILE_BYTES / 16);
+        const uint32_t d = (uint32_t)(step & 1) * (TILE_BYTES / 16);
 #pragma unroll
         for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(tdP, kV, koff(kk), kdO, d + koff(kk), id_kk, kk > 0 ? 1u : 0u);
         umma_commit(smem_u32(&sh.dp_full));
+        if (last) umma_commit(smem_u32(&sh.res_empty));    // no product reads K or V any more
       }
       return true;
     };
-    bool ok = n_it > 0 && mbar_wait_warp(smem_u32(&sh.bar_res), 0, abort_flag);
-    if (ok) ok = issue_s();
-    if (ok) ok = issue_dp(0);
-    int r3 = 0;                                            // ring place of this step's Q
-    for (int t = 0; t < n_it && ok; ++t) {
-      if (!(ok = mbar_wait_warp(smem_u32(&sh.p_ready), t & 1, abort_flag))) break;       // P^T over S^T, read by every warp
-      tcgen05_fence_after();
-      if (leader) {
-        const uint32_t d = (uint32_t)(t & 1) * (TILE_BYTES / 16);
-#pragma unroll
-        for (int kk = 0; kk < BQ / 16; ++kk)               // dV[kv, d] += P^T[kv, q] dO[q, d]
-          umma_ts_bf16_b(tdV, tS + (kk >> 2) * 64 + 8 * (kk & 3), mdO, d + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(smem_u32(&sh.pair_empty[t & 1]));      // dP(t) read dO(t) before
+    bool ok = true;
+    int tile, n_i;
+    for (int k = 0; ok && take_tile(sh, k, lane, abort_flag, tile, n_i); ++k) {
+      const int n_it = heads * n_i;
+      if (!(ok = mbar_wait_warp(smem_u32(&sh.res_full), (uint32_t)(k & 1), abort_flag))) break;
+      if (n_it == 0) {
+        if (leader) mbar_arrive(smem_u32(&sh.res_empty));
+        continue;
       }
-      if (t + 1 < n_it && !(ok = issue_s())) break;        // behind dV(t), which reads P^T(t) from its columns
-      if (!(ok = mbar_wait_warp(smem_u32(&sh.ds_ready), t & 1, abort_flag))) break;      // dS^T over dP^T
-      tcgen05_fence_after();
-      if (leader) {
-        const uint32_t q = (uint32_t)r3 * (TILE_BYTES / 16);
+      if (!(ok = issue_s())) break;                        // behind the last dV, which reads P^T from these columns, as dP behind the last dK
+      if (!(ok = issue_dp(n, n_it == 1))) break;
+      for (int t = 0; t < n_it; ++t, ++n) {
+        // P^T over S^T, read by every warp; in a tile's first step every warp has read the last tile's accumulators before
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.p_ready), n & 1, abort_flag))) break;
+        tcgen05_fence_after();
+        if (leader) {
+          const uint32_t d = (uint32_t)(n & 1) * (TILE_BYTES / 16);
 #pragma unroll
-        for (int kk = 0; kk < BQ / 16; ++kk)               // dK[kv, d] += dS^T[kv, q] Q[q, d]
-          umma_ts_bf16_b(tdK, tdP + (kk >> 2) * 64 + 8 * (kk & 3), mQ, q + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(smem_u32(&sh.ring_empty[r3]));
-        if (t == n_it - 1) umma_commit(smem_u32(&sh.acc_full));
+          for (int kk = 0; kk < BQ / 16; ++kk)             // dV[kv, d] += P^T[kv, q] dO[q, d]
+            umma_ts_bf16_b(tdV, tS + (kk >> 2) * 64 + 8 * (kk & 3), mdO, d + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(smem_u32(&sh.pair_empty[n & 1]));    // dP(t) read dO(t) before
+        }
+        if (t + 1 < n_it && !(ok = issue_s())) break;      // behind dV(t), which reads P^T(t) from its columns
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.ds_ready), n & 1, abort_flag))) break;      // dS^T over dP^T
+        tcgen05_fence_after();
+        if (leader) {
+          const uint32_t q = (uint32_t)r3 * (TILE_BYTES / 16);
+#pragma unroll
+          for (int kk = 0; kk < BQ / 16; ++kk)             // dK[kv, d] += dS^T[kv, q] Q[q, d]
+            umma_ts_bf16_b(tdK, tdP + (kk >> 2) * 64 + 8 * (kk & 3), mQ, q + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(smem_u32(&sh.ring_empty[r3]));
+          if (t == n_it - 1) umma_commit(smem_u32(&sh.acc_full));
+        }
+        if (++r3 == RING3) r3 = 0;
+        if (t + 1 < n_it && !(ok = issue_dp(n + 1, t + 2 == n_it))) break;
       }
-      if (++r3 == RING3) r3 = 0;
-      if (t + 1 < n_it && !(ok = issue_dp(t + 1))) break;
     }
   } else if (warp == 10) {
     // lse, delta and starts of a step's query block, four rows a lane, asked for while the step before is used
     bool ok = true;
-    int h = h0, i = 0;
-    float nl[4], nd[4];
-    int lo[4];
-    auto fetch = [&] {
+    int n = 0, tile, n_i;
+    for (int k = 0; ok && take_tile(sh, k, lane, abort_flag, tile, n_i); ++k) {
+      const Place a = place(tile);
+      const int n_it = heads * n_i, kvrow0 = a.j * BKV;
+      int h = a.h0, i = 0;
+      float nl[4], nd[4];
+      int lo[4];
+      auto fetch = [&] {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = (j + i) * BQ + lane * 4 + e;
-        const long long at = ((long long)b * p.H + h) * p.S + row;
-        const bool live = row < p.S;
-        nl[e] = live ? -p.lse[at] * 1.4426950408889634f : -INFINITY;       // a row that sees nothing has an infinite lse: its weights are zero
-        nd[e] = live ? -p.delta[at] * p.scale : 0.f;
-        lo[e] = live ? min(max(p.starts[(long long)b * p.S + row], kvrow0) - kvrow0, BKV) : 0;
+        for (int e = 0; e < 4; ++e) {
+          const int row = (a.j + i) * BQ + lane * 4 + e;
+          const long long at = ((long long)a.b * p.H + h) * p.S + row;
+          const bool live = row < p.S;
+          nl[e] = live ? -p.lse[at] * 1.4426950408889634f : -INFINITY;       // a row that sees nothing has an infinite lse: its weights are zero
+          nd[e] = live ? -p.delta[at] * p.scale : 0.f;
+          lo[e] = live ? min(max(p.starts[(long long)a.b * p.S + row], kvrow0) - kvrow0, BKV) : 0;
+        }
+        if (++i == n_i) { i = 0; ++h; }
+      };
+      if (n_it > 0) fetch();
+      for (int t = 0; t < n_it; ++t, ++n) {
+        const int s = n & 1;
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.stat_empty[s]), (uint32_t)(((n >> 1) & 1) ^ 1), abort_flag))) break;
+        *reinterpret_cast<float4*>(stats[s].nlse + lane * 4) = make_float4(nl[0], nl[1], nl[2], nl[3]);
+        *reinterpret_cast<float4*>(stats[s].ndelta + lane * 4) = make_float4(nd[0], nd[1], nd[2], nd[3]);
+        *reinterpret_cast<uchar4*>(stats[s].lo + lane * 4) = make_uchar4((uint8_t)lo[0], (uint8_t)lo[1], (uint8_t)lo[2], (uint8_t)lo[3]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.stat_full[s]));
+        if (t + 1 < n_it) fetch();
       }
-      if (++i == n_i) { i = 0; ++h; }
-    };
-    if (n_it > 0) fetch();
-    for (int t = 0; t < n_it && ok; ++t) {
-      const int s = t & 1;
-      if (!(ok = mbar_wait_warp(smem_u32(&sh.stat_empty[s]), (uint32_t)(((t >> 1) & 1) ^ 1), abort_flag))) break;
-      *reinterpret_cast<float4*>(stats[s].nlse + lane * 4) = make_float4(nl[0], nl[1], nl[2], nl[3]);
-      *reinterpret_cast<float4*>(stats[s].ndelta + lane * 4) = make_float4(nd[0], nd[1], nd[2], nd[3]);
-      *reinterpret_cast<uchar4*>(stats[s].lo + lane * 4) = make_uchar4((uint8_t)lo[0], (uint8_t)lo[1], (uint8_t)lo[2], (uint8_t)lo[3]);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.stat_full[s]));
-      if (t + 1 < n_it) fetch();
     }
   } else {
     const int quad = warp & 3, ch = (warp - 2) >> 2;       // TMEM lanes, half of the step's query rows
     const int r = quad * 32 + lane;                        // key row of the block = TMEM lane
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-    const uint32_t sw = (uint32_t)(lane & 7);
     const unsigned long long sl2 = two(p.scale_log2), sc = two(p.scale);
     bool ok = true;
-    int i = 0;
-    for (int t = 0; t < n_it && ok; ++t) {
-      const DocsStats& st = stats[t & 1];
-      const bool diag = i == 0;
-      if (++i == n_i) i = 0;
-      if (!(ok = mbar_wait_warp(smem_u32(&sh.stat_full[t & 1]), (uint32_t)((t >> 1) & 1), abort_flag))) break;
-      if (!(ok = mbar_wait_warp(smem_u32(&sh.s_full[0]), t & 1, abort_flag))) break;
-      tcgen05_fence_after();
-      uint32_t v[64];                                      // P, in fp32 for dS
+    int n = 0, n_acc = 0, tile, n_i;                       // steps and tiles with a step so far
+    for (int k = 0; ok && take_tile(sh, k, lane, abort_flag, tile, n_i); ++k) {
+      const Place a = place(tile);
+      const int n_it = heads * n_i;
+      int i = 0;
+      for (int t = 0; t < n_it; ++t, ++n) {
+        const DocsStats& st = stats[n & 1];
+        const bool diag = i == 0;
+        if (++i == n_i) i = 0;
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.stat_full[n & 1]), (uint32_t)((n >> 1) & 1), abort_flag))) break;
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.s_full[0]), n & 1, abort_flag))) break;
+        tcgen05_fence_after();
+        uint32_t v[64];                                    // P, in fp32 for dS
+        tmem_ld32_nowait(tS + ch * 64 + lane_off, v);
+        tmem_ld32_nowait(tS + ch * 64 + 32 + lane_off, v + 32);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        behind_wait32(v);
+        behind_wait32(v + 32);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        tmem_ld32(tS + ch * 64 + c * 32 + lane_off, v + c * 32);
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float4 nl = *reinterpret_cast<const float4*>(st.nlse + ch * 64 + c * 32 + e);
-          uint32_t* w = v + c * 32 + e;
+        for (int e = 0; e < 64; e += 4) {
+          const float4 nl = *reinterpret_cast<const float4*>(st.nlse + ch * 64 + e);
+          uint32_t* w = v + e;
           float a0, a1, a2, a3;
           unpack_f32x2(fma_f32x2(pack_f32x2(w[0], w[1]), sl2, pack_f32x2(__float_as_uint(nl.x), __float_as_uint(nl.y))), a0, a1);
           unpack_f32x2(fma_f32x2(pack_f32x2(w[2], w[3]), sl2, pack_f32x2(__float_as_uint(nl.z), __float_as_uint(nl.w))), a2, a3);
           w[0] = __float_as_uint(exp2f(a0)); w[1] = __float_as_uint(exp2f(a1));
           w[2] = __float_as_uint(exp2f(a2)); w[3] = __float_as_uint(exp2f(a3));
         }
-      }
-      // a query row before the key, or whose document begins behind it, does not see it
-      const uint32_t* lo4 = reinterpret_cast<const uint32_t*>(st.lo + ch * 64);
-      if (__any_sync(0xffffffffu, lo4[lane & 15] != 0u)) {
+        // a query row before the key, or whose document begins behind it, does not see it
+        const uint32_t* lo4 = reinterpret_cast<const uint32_t*>(st.lo + ch * 64);
+        if (__any_sync(0xffffffffu, lo4[lane & 15] != 0u)) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const uint32_t w = lo4[e];
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t w = lo4[e];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) if ((int)((w >> (8 * k)) & 255u) > r) v[4 * e + k] = 0u;
+            for (int q = 0; q < 4; ++q) if ((int)((w >> (8 * q)) & 255u) > r) v[4 * e + q] = 0u;
+          }
         }
-      }
-      if (diag) {
+        if (diag) {
 #pragma unroll
-        for (int e = 0; e < 64; ++e) if (ch * 64 + e < r) v[e] = 0u;
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) pk[e] = bf16x2_of(__uint_as_float(v[c * 32 + 2 * e]), __uint_as_float(v[c * 32 + 2 * e + 1]));
-        tmem_st16(tS + ch * 64 + c * 16 + lane_off, pk);
-      }
-      tmem_wait_st();
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.p_ready));
-      if (!(ok = mbar_wait_warp(smem_u32(&sh.dp_full), t & 1, abort_flag))) break;
-      tcgen05_fence_after();
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t dp[32], pk[16];
-        tmem_ld32(tdP + ch * 64 + c * 32 + lane_off, dp);
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float4 nd = *reinterpret_cast<const float4*>(st.ndelta + ch * 64 + c * 32 + e);
-          const uint32_t* w = v + c * 32 + e;
-          float d0, d1, d2, d3;
-          unpack_f32x2(mul_f32x2(pack_f32x2(w[0], w[1]), fma_f32x2(pack_f32x2(dp[e], dp[e + 1]), sc, pack_f32x2(__float_as_uint(nd.x), __float_as_uint(nd.y)))), d0, d1);
-          unpack_f32x2(mul_f32x2(pack_f32x2(w[2], w[3]), fma_f32x2(pack_f32x2(dp[e + 2], dp[e + 3]), sc, pack_f32x2(__float_as_uint(nd.z), __float_as_uint(nd.w)))), d2, d3);
-          pk[e / 2] = bf16x2_of(d0, d1);
-          pk[e / 2 + 1] = bf16x2_of(d2, d3);
+          for (int e = 0; e < 64; ++e) if (ch * 64 + e < r) v[e] = 0u;
         }
-        tmem_st16(tdP + ch * 64 + c * 16 + lane_off, pk);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) pk[e] = bf16x2_of(__uint_as_float(v[c * 32 + 2 * e]), __uint_as_float(v[c * 32 + 2 * e + 1]));
+          tmem_st16(tS + ch * 64 + c * 16 + lane_off, pk);
+        }
+        tmem_wait_st();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.p_ready));
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.dp_full), n & 1, abort_flag))) break;
+        tcgen05_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t dp[32], pk[16];
+          tmem_ld32(tdP + ch * 64 + c * 32 + lane_off, dp);
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 nd = *reinterpret_cast<const float4*>(st.ndelta + ch * 64 + c * 32 + e);
+            const uint32_t* w = v + c * 32 + e;
+            float d0, d1, d2, d3;
+            unpack_f32x2(mul_f32x2(pack_f32x2(w[0], w[1]), fma_f32x2(pack_f32x2(dp[e], dp[e + 1]), sc, pack_f32x2(__float_as_uint(nd.x), __float_as_uint(nd.y)))), d0, d1);
+            unpack_f32x2(mul_f32x2(pack_f32x2(w[2], w[3]), fma_f32x2(pack_f32x2(dp[e + 2], dp[e + 3]), sc, pack_f32x2(__float_as_uint(nd.z), __float_as_uint(nd.w)))), d2, d3);
+            pk[e / 2] = bf16x2_of(d0, d1);
+            pk[e / 2 + 1] = bf16x2_of(d2, d3);
+          }
+          tmem_st16(tdP + ch * 64 + c * 16 + lane_off, pk);
+        }
+        tmem_wait_st();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) { mbar_arrive(smem_u32(&sh.ds_ready)); mbar_arrive(smem_u32(&sh.stat_empty[n & 1])); }
       }
-      tmem_wait_st();
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) { mbar_arrive(smem_u32(&sh.ds_ready)); mbar_arrive(smem_u32(&sh.stat_empty[t & 1])); }
-    }
-    // dV and dK of this block.  Whole group in this CTA: TMEM -> bf16 -> staging in the Q tiles, which nothing reads any more -> the packed
-    // gradient; a part of it: in fp32 in columns of its own, which a last pass adds in order.  Without a step the first Q tile has to land.
-    if (ok) ok = n_it > 0 ? mbar_wait_warp(smem_u32(&sh.acc_full), 0, abort_flag) : mbar_wait_warp(smem_u32(&sh.ring_full[0]), 0, abort_flag);
-    if (ok) {
+      // dV and dK of this block.  Whole group in this tile: rounded into the packed gradient; a part of it: in fp32 in columns of its own, which
+      // a last pass adds in order.
+      if (ok && n_it > 0) ok = mbar_wait_warp(smem_u32(&sh.acc_full), (uint32_t)(n_acc++ & 1), abort_flag);
+      if (!ok) break;
       tcgen05_fence_after();
-      const int orow0 = kvrow0 + quad * 32;
-      const uint32_t stage = sQ + (uint32_t)(warp - 2) * (DH == 128 ? 8192u : 4096u), rowaddr = stage + (uint32_t)lane * 128u;
-      if (p.split > 1) {
+      const int row = a.j * BKV + r;
+      const long long tok = (long long)a.b * p.S + row;
 #pragma unroll 1
-        for (int x = 0; x < DH / 32; ++x) {                // 32-column boxes of dV, then of dK; this warp takes one column half of each
-          const int acc = x / (DH / 64), col = (DH / 64 * ch + x % (DH / 64)) * 32;
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          __syncwarp();
-          uint32_t w[32];
-          tmem_ld32((acc ? tdK : tdV) + col + lane_off, w);
+      for (int acc = 0; acc < 2; ++acc) {                  // dV, dK; this warp has one column half of each
+        const int head = acc ? a.g : p.KV + a.g;
+        const uint32_t from = (acc ? tdK : tdV) + ch * (DH / 2) + lane_off;
+        if (p.split > 1) {
+          float* to = p.part + (tok * p.split + a.sub) * (2LL * p.KV * DH) + head * DH + ch * (DH / 2);
 #pragma unroll
-          for (int q8 = 0; q8 < 8; ++q8) {
-            uint32_t f[4];
+          for (int c = 0; c < DH / 64; ++c) {
+            uint32_t v[32];
+            tmem_ld32(from + c * 32, v);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] = n_it == 0 ? 0u : w[4 * q8 + e];
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rowaddr + (((uint32_t)q8 ^ sw) << 4)), "r"(f[0]), "r"(f[1]), "r"(f[2]),
-                         "r"(f[3]) : "memory");
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) {
-            if (orow0 < p.S) tma_store_3d(&p.tmPart, stage, (sub * 2 * p.KV + (acc ? g : p.KV + g)) * DH + col, orow0, b);
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          }
-        }
-      } else {
+            for (int q = 0; q < 4; ++q) {
+              uint32_t w[8];
 #pragma unroll
-        for (int x = 0; x < DH / 64; ++x) {                // at 128 columns a half of dV, then of dK; at 64 one of them
-          const int acc = DH == 128 ? x : ch, col = DH == 128 ? ch * 64 : 0;
-          const uint32_t tacc = acc ? tdK : tdV;
+              for (int e = 0; e < 8; ++e) w[e] = n_it == 0 ? 0u : v[8 * q + e];
+              if (row < p.S) store_sector(to + c * 32 + q * 8, w);
+            }
+          }
+        } else {
+          __nv_bfloat16* to = p.dqkv + tok * C + (p.H + head) * DH + ch * (DH / 2);
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            uint32_t w[32];
-            tmem_ld32(tacc + col + hf * 32 + lane_off, w);
-            box_row(rowaddr + (uint32_t)x * 4096u, sw, hf, w, n_it == 0);
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0 && orow0 < p.S) {
-            tma_store_3d(&p.tmDQKV, stage + (uint32_t)x * 4096u, (acc ? kcol : vcol) + col, orow0, b);
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          }
+          for (int c = 0; c < DH / 64; ++c) store_row32(to + c * 32, from + c * 32, n_it == 0, row < p.S);
         }
       }
+      tcgen05_fence_before();                              // the next tile's first dV is behind this warp's next P
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   }
   docs_bwd_end(p, sh, warp);
 }
@@ -2551,26 +2624,30 @@ int docs_split(int B, int S, int H, int KV) {
 }
 
 template <int DH>
-int launch_docs_bwd(const void* qkv, const int* starts, const int* blocks, const void* out, const void* dout, const float* lse, float* delta,
+int launch_docs_bwd(const void* qkv, const int* starts, int* blocks, const void* out, const void* dout, const float* lse, float* delta,
                     float* part, void* dqkv, int B, int S, int H, int KV, long long ld_qkv, float scale, unsigned int* status, cudaStream_t st) {
   AttnDocsBwdParams p = {};
   const int C = (H + 2 * KV) * DH, split = docs_split(B, S, H, KV), kv_cols = 2 * KV * DH;
+  if ((long long)((S + BKV - 1) / BKV) * H * B > 0x7fffffff / 2) return -201;
   if (split > 1 && !part) return -201;
   if (!make_map3(&p.tmQKV, qkv, C, S, B, ld_qkv, 64, 128)) return -202;
   if (!make_map3(&p.tmDO, dout, (long long)H * DH, S, B, (long long)H * DH, 64, 128)) return -203;
-  if (!make_map3(&p.tmDQKV, dqkv, C, S, B, C, 64, 32)) return -205;
-  if (split > 1 && !make_map3(&p.tmPart, part, (long long)split * kv_cols, S, B, (long long)split * kv_cols, 32, 32, true)) return -204;
-  p.out = (const __nv_bfloat16*)out; p.lse = lse; p.delta = delta; p.starts = starts; p.blocks = blocks;
-  p.B = B; p.S = S; p.H = H; p.KV = KV; p.split = split; p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
+  const int n = (S + BKV - 1) / BKV, sms = tplr_sm_count();
+  p.out = (const __nv_bfloat16*)out; p.dqkv = (__nv_bfloat16*)dqkv; p.part = part; p.lse = lse; p.delta = delta; p.starts = starts;
+  p.blocks = blocks; p.B = B; p.S = S; p.H = H; p.KV = KV; p.split = split; p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
+  p.status = status;
   constexpr int SMEM = docs_bwd_smem<DH>();
-  const unsigned n = (unsigned)((S + BKV - 1) / BKV);
   cudaError_t e = cudaFuncSetAttribute(attn_docs_dq_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_docs_dkv_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-  if (e == cudaSuccess) e = launch_pdl(attn_docs_dq_kernel<DH>, n * H * B, DQ_THREADS, SMEM, st, p);
-  if (e == cudaSuccess) e = launch_pdl(attn_docs_dkv_kernel<DH>, n * KV * B * split, DKV_THREADS, SMEM, st, p);
+  p.tiles = n * H * B;
+  p.next = blocks + (long long)B * n;
+  if (e == cudaSuccess) e = launch_pdl(attn_docs_dq_kernel<DH>, (unsigned)(p.tiles < sms ? p.tiles : sms), DQ_THREADS, SMEM, st, p);
+  p.tiles = n * KV * B * split;
+  ++p.next;
+  if (e == cudaSuccess) e = launch_pdl(attn_docs_dkv_kernel<DH>, (unsigned)(p.tiles < sms ? p.tiles : sms), DKV_THREADS, SMEM, st, p);
   if (e != cudaSuccess || split == 1) return (int)e;
   // the parts' sums into the key and value columns; no query columns here
-  return (int)launch_pdl(attn_dq_cast_kernel<DH, true>, tplr_sm_count() * 8, 256, 0, st, part, part, split, (__nv_bfloat16*)dqkv + H * DH,
+  return (int)launch_pdl(attn_dq_cast_kernel<DH, true>, tplr_sm_count() * 8, 256, 0, st, part, part, split, p.dqkv + H * DH,
                          (long long)B * S, 0, kv_cols, 0, (long long)C, nullptr, nullptr, S);
 }
 }  // namespace
@@ -2582,15 +2659,16 @@ TPLR_API int tplr_attention_docs_bwd_scratch_cols(int B, int S, int H, int KV, i
   return split > 1 ? 2 * KV * split * head_dim : 0;
 }
 
-// Gradient of tplr_attention_docs_fwd, whose starts, blocks and lse it takes: dqkv [B, S, (H + 2 KV) * head_dim] dense.  out and dout dense;
-// delta: [B, H, S] fp32 scratch; part: B * S * tplr_attention_docs_bwd_scratch_cols fp32 elements, contents irrelevant.
-TPLR_API int tplr_attention_docs_bwd(const void* qkv, const int* starts, const int* blocks, const void* out, const void* dout,
+// Gradient of tplr_attention_docs_fwd, whose starts, blocks (left as they are) and lse it takes: dqkv [B, S, (H + 2 KV) * head_dim] dense.
+// out and dout dense; dqkv and part on 32-byte boundaries; delta: [B, H, S] fp32 scratch; part: B * S *
+// tplr_attention_docs_bwd_scratch_cols fp32 elements, contents irrelevant.
+TPLR_API int tplr_attention_docs_bwd(const void* qkv, const int* starts, int* blocks, const void* out, const void* dout,
                                      const float* lse, float* delta, float* part, void* dqkv, int B, int S, int H, int KV, int head_dim,
                                      long long ld_qkv, float scale, unsigned int* status, void* stream) {
   TPLR_ENTER();
   if (B <= 0 || S <= 0) return 0;
   if ((head_dim != 128 && head_dim != 64) || KV <= 0 || H % KV || (ld_qkv % 8) || !starts || !blocks ||
-      (((uintptr_t)qkv | (uintptr_t)dqkv | (uintptr_t)dout | (uintptr_t)out | (uintptr_t)part) & 15))
+      (((uintptr_t)qkv | (uintptr_t)dout | (uintptr_t)out) & 15) || (((uintptr_t)dqkv | (uintptr_t)part) & 31))
     return -201;
   auto run = head_dim == 128 ? launch_docs_bwd<128> : launch_docs_bwd<64>;
   return run(qkv, starts, blocks, out, dout, lse, delta, part, dqkv, B, S, H, KV, ld_qkv, scale, status, (cudaStream_t)stream);

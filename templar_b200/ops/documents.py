@@ -100,7 +100,7 @@ def _attention_documents(qkv, ld, starts, n_heads, n_kv, hd, keep):
     with _on(qkv):
         out = torch.empty(B, S, n_heads * hd, dtype=qkv.dtype, device=qkv.device)
         lse = torch.empty(B, n_heads, S, dtype=torch.float32, device=qkv.device) if keep else None
-        blocks = torch.empty(B, -(-S // 128), dtype=torch.int32, device=qkv.device) if keep else None
+        blocks = torch.empty(B * -(-S // 128) + 2, dtype=torch.int32, device=qkv.device) if keep else None
         native.check(native.lib().tplr_attention_docs_fwd(
             qkv.data_ptr(), starts.data_ptr(), out.data_ptr(), native.ptr(lse), native.ptr(blocks), B, S, n_heads, n_kv, hd, ld, n_heads * hd,
             hd ** -0.5, OF.status_word(qkv.device).data_ptr(), native.stream_ptr()), "attention_docs_fwd")
