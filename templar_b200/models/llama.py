@@ -360,7 +360,7 @@ class LlamaModel(nn.Module):
         if self.args.fused_loss:
             w = self.output.weight
             mg = getattr(w, "main_grad", None)
-            if mg is not None and not torch.is_tensor(mg):
+            if mg is not None and not torch.is_tensor(mg) and torch.is_grad_enabled():
                 raise ValueError("LlamaModel: fused_loss adds the output projection's gradient to a buffer of its own rank; with sharded "
                                  "parameters (shard_params) leave it off")
             return OD.linear_cross_entropy(self.hidden_states(tokens), w, labels, grad_scale, ignore_index, mg)

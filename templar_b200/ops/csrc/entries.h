@@ -55,4 +55,31 @@ int tplr_gemm2_swiglu_saved8(const void* X, const void* W, void* Q, float* scale
 int tplr_gemm2_swiglu_bwd_saved8(const void* dY, const void* W2, const void* Q, const float* scale, void* dGU, void* H, int M, int F, int K,
                                  long long lddy, long long ldw2, long long ldq, long long ld_scale, long long lddgu, long long ldh,
                                  unsigned int* status, void* stream);
+// sequences of several documents
+int tplr_attention_docs_fwd(const void* qkv, const int* starts, void* out, float* lse, int* blocks, int B, int S, int H, int KV, int head_dim,
+                            long long ld_qkv, long long ld_o, float scale, unsigned int* status, void* stream);
+int tplr_attention_docs_bwd_scratch_cols(int B, int S, int H, int KV, int head_dim);
+int tplr_attention_docs_bwd(const void* qkv, const int* starts, int* blocks, const void* out, const void* dout, const float* lse, float* delta,
+                            float* part, void* dqkv, int B, int S, int H, int KV, int head_dim, long long ld_qkv, float scale,
+                            unsigned int* status, void* stream);
+int tplr_qk_norm_rope(const void* x, long long ldx, void* y, const void* wq, const void* wk, const float* cosb, const float* sinb,
+                      const int* pos, long long tokens, int S, int table_rows, int n_q, int n_k, int hd, float eps, unsigned int* status,
+                      void* stream);
+int tplr_qk_norm_rope_parts(long long tokens, int n_q, int n_k, int hd);
+int tplr_qk_norm_rope_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* wq, const void* wk, const float* cosb,
+                          const float* sinb, const int* pos, void* dx, float* part, void* dwq, void* dwk, float* add_q, float* add_k,
+                          long long tokens, int S, int table_rows, int n_q, int n_k, int hd, float eps, unsigned int* status, void* stream);
+int tplr_gemm2_softmax_columns(int M, int N, int K);
+int tplr_gemm2_softmax(const void* X, const void* W, void* P, const long long* labels, float* stats, float* target, int M, int N, int K,
+                       long long ldx, long long ldw, long long ldp, unsigned int* status, void* stream);
+int tplr_gemm2_rows(const void* A, const void* B, void* C, float* ws, const float* row_scale, int M, int N, int K, long long lda,
+                    long long ldb, long long ldc, unsigned int* status, void* stream);
+int tplr_vocab_count(const long long* labels, long long T, long long ignore, int V, int* n_valid, unsigned int* status, void* stream);
+int tplr_vocab_losses(const float* stats, const float* target, const long long* labels, float* losses, float* lse, long long T, int parts, int V,
+                      long long ignore, void* stream);
+int tplr_vocab_rows(void* E, long long ld, const float* stats, const float* target, const long long* labels, const float* row_grad,
+                    const int* n_valid, float grad_scale, const void* x, long long ldx, void* xs, float* row_scale, float* losses, long long T,
+                    int parts, int columns, int V, int D, long long ignore, void* stream);
+int tplr_vocab_mean(const float* losses, long long T, const int* n_valid, float* loss, void* stream);
+int tplr_vocab_scale(const void* x, int x_fp32, const float* by, void* y, int add_fp32, long long n, void* stream);
 }

@@ -8,11 +8,13 @@
 // functional.py decides which calls come here (operand types, strides and alignment) and keeps its nodes for all others.
 // Tensors are saved as saved variables only; the gradient buffers of the flat store are held by reference as there.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "../csrc/entries.h"
@@ -54,6 +56,20 @@ struct Entries {
   decltype(&tplr_linear_q8_few) linear_q8_few;
   decltype(&tplr_gemm2_swiglu_saved8) swiglu_saved8;
   decltype(&tplr_gemm2_swiglu_bwd_saved8) swiglu_bwd_saved8;
+  decltype(&tplr_attention_docs_fwd) docs_fwd;
+  decltype(&tplr_attention_docs_bwd_scratch_cols) docs_bwd_scratch_cols;
+  decltype(&tplr_attention_docs_bwd) docs_bwd;
+  decltype(&tplr_qk_norm_rope) qk_norm;
+  decltype(&tplr_qk_norm_rope_parts) qk_norm_parts;
+  decltype(&tplr_qk_norm_rope_bwd) qk_norm_bwd;
+  decltype(&tplr_gemm2_softmax_columns) softmax_columns;
+  decltype(&tplr_gemm2_softmax) softmax;
+  decltype(&tplr_gemm2_rows) gemm_rows;
+  decltype(&tplr_vocab_count) vocab_count;
+  decltype(&tplr_vocab_losses) vocab_losses;
+  decltype(&tplr_vocab_rows) vocab_rows;
+  decltype(&tplr_vocab_mean) vocab_mean;
+  decltype(&tplr_vocab_scale) vocab_scale;
 } E;
 
 void bind(const std::string& path) {
@@ -92,6 +108,20 @@ void bind(const std::string& path) {
   get(E.linear_q8_few, "tplr_linear_q8_few");
   get(E.swiglu_saved8, "tplr_gemm2_swiglu_saved8");
   get(E.swiglu_bwd_saved8, "tplr_gemm2_swiglu_bwd_saved8");
+  get(E.docs_fwd, "tplr_attention_docs_fwd");
+  get(E.docs_bwd_scratch_cols, "tplr_attention_docs_bwd_scratch_cols");
+  get(E.docs_bwd, "tplr_attention_docs_bwd");
+  get(E.qk_norm, "tplr_qk_norm_rope");
+  get(E.qk_norm_parts, "tplr_qk_norm_rope_parts");
+  get(E.qk_norm_bwd, "tplr_qk_norm_rope_bwd");
+  get(E.softmax_columns, "tplr_gemm2_softmax_columns");
+  get(E.softmax, "tplr_gemm2_softmax");
+  get(E.gemm_rows, "tplr_gemm2_rows");
+  get(E.vocab_count, "tplr_vocab_count");
+  get(E.vocab_losses, "tplr_vocab_losses");
+  get(E.vocab_rows, "tplr_vocab_rows");
+  get(E.vocab_mean, "tplr_vocab_mean");
+  get(E.vocab_scale, "tplr_vocab_scale");
 }
 
 void check(int err, const char* what) {
@@ -551,6 +581,276 @@ struct FeedForwardSaved8 : Function<FeedForwardSaved8> {
   }
 };
 
+// ------------------------------------------------------------------------------------------ sequences of several documents
+// A call whose operands the kernels take as they are comes straight here: None sends it to the checks of documents.py, which say what is
+// wrong or bring it into shape.
+typedef std::optional<Tensor> Maybe;
+bool here(const Tensor& t, c10::DeviceIndex d) { return t.is_cuda() && t.get_device() == d; }
+bool heads_fit(const Tensor& qkv, int64_t heads, int64_t kv, int64_t hd) {
+  return qkv.dim() == 3 && qkv.scalar_type() == at::kBFloat16 && qkv.numel() > 0 && heads > 0 && kv > 0 && hd > 0 && heads % kv == 0 &&
+         qkv.size(2) == (heads + 2 * kv) * hd;
+}
+bool buffer_fits(const Maybe& b, const Tensor& w) {
+  return !b || (b->scalar_type() == at::kFloat && b->sizes() == w.sizes() && b->is_contiguous() && b->device() == w.device() &&
+                reinterpret_cast<uintptr_t>(b->data_ptr()) % 16 == 0);
+}
+bool on_boundary(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+Tensor copy(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
+float* ptr32(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// [B, S, C] as rows evenly apart in whole 16-byte pieces, ld elements from one to the next (documents.py, _packed_rows)
+Tensor packed(const Tensor& t, ll& ld) {
+  const ll B = t.size(0), S = t.size(1), C = t.size(2);
+  ld = S > 1 ? t.stride(1) : B > 1 ? t.stride(0) : C;
+  if (t.stride(2) == 1 && ld >= C && ld % 8 == 0 && (B == 1 || t.stride(0) == S * ld) && on_boundary(t)) return t;
+  ld = C;
+  return copy(t);
+}
+// a matrix as the products take it (documents.py, _operand)
+Tensor operand(const Tensor& t) {
+  return t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && on_boundary(t) ? t : copy(t);
+}
+
+// (out, lse, blocks); the last two for a backward pass alone
+std::tuple<Tensor, Tensor, Tensor> docs_forward(const Tensor& qkv, ll ld, const Tensor& starts, int64_t heads, int64_t kv, int64_t hd,
+                                                const Tensor& status, bool keep) {
+  const ll B = qkv.size(0), S = qkv.size(1);
+  Tensor out = bf16({B, S, heads * hd}, qkv), lse, blocks;
+  if (keep) {
+    lse = f32({B, heads, S}, qkv);
+    blocks = at::empty({B * ((S + 127) / 128) + 2}, starts.options());
+  }
+  check(E.docs_fwd(qkv.data_ptr(), starts.data_ptr<int>(), out.data_ptr(), ptr32(lse), keep ? blocks.data_ptr<int>() : nullptr, (int)B, (int)S,
+                   (int)heads, (int)kv, (int)hd, ld, heads * hd, (float)std::pow((double)hd, -0.5), word(status), stream()),
+        "attention_docs_fwd");
+  return {out, lse, blocks};
+}
+
+struct AttentionDocuments : Function<AttentionDocuments> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& qkv_in, Aside starts, int64_t heads, int64_t kv, int64_t hd, Aside status) {
+    ll ld;
+    const Tensor qkv = packed(qkv_in, ld);
+    auto [out, lse, blocks] = docs_forward(qkv, ld, starts.t, heads, kv, hd, status.t, true);
+    ctx->save_for_backward({qkv, starts.t, out, lse, blocks});
+    keep(ctx, "status", status);
+    ctx->saved_data["dims"] = std::vector<int64_t>{heads, kv, hd, ld};
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    auto s = ctx->get_saved_variables();
+    const Tensor &qkv = s[0], &starts = s[1], &out = s[2], &lse = s[3], &blocks = s[4];
+    const auto d = ctx->saved_data["dims"].toIntVector();
+    const ll B = qkv.size(0), S = qkv.size(1), heads = d[0], kv = d[1], hd = d[2];
+    const Tensor dout = dense(g[0]);
+    Tensor dqkv = bf16({B, S, qkv.size(2)}, qkv), delta = f32({B, heads, S}, qkv), part;
+    if (const ll cols = E.docs_bwd_scratch_cols((int)B, (int)S, (int)heads, (int)kv, (int)hd)) part = f32({B * S * cols}, qkv);
+    check(E.docs_bwd(qkv.data_ptr(), starts.data_ptr<int>(), blocks.data_ptr<int>(), out.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(),
+                     delta.data_ptr<float>(), ptr32(part), dqkv.data_ptr(), (int)B, (int)S, (int)heads, (int)kv, (int)hd, d[3],
+                     (float)std::pow((double)hd, -0.5), word(aside(ctx, "status")), stream()),
+          "attention_docs_bwd");
+    return {dqkv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+Maybe attention_documents(const Tensor& qkv, const Tensor& starts, int64_t heads, int64_t kv, int64_t hd, const Tensor& status) {
+  const auto dev = c10::cuda::current_device();
+  if (!here(qkv, dev) || !heads_fit(qkv, heads, kv, hd) || (hd != 64 && hd != 128) || !here(starts, dev) || starts.scalar_type() != at::kInt ||
+      starts.dim() != 2 || starts.size(0) != qkv.size(0) || starts.size(1) != qkv.size(1) || !starts.is_contiguous())
+    return std::nullopt;
+  if (at::GradMode::is_enabled() && qkv.requires_grad()) return AttentionDocuments::apply(qkv, Aside{starts}, heads, kv, hd, Aside{status});
+  ll ld;
+  const Tensor rows = packed(qkv, ld);
+  return std::get<0>(docs_forward(rows, ld, starts, heads, kv, hd, status, false));
+}
+
+Tensor qk_norm_forward(const Tensor& x, ll ld, const Tensor& wq, const Tensor& wk, const Tensor& cos, const Tensor& sin, const Tensor& pos,
+                       int64_t heads, int64_t kv, int64_t hd, double eps, const Tensor& status) {
+  Tensor y = bf16(x.sizes(), x);
+  check(E.qk_norm(x.data_ptr(), ld, y.data_ptr(), wq.data_ptr(), wk.data_ptr(), cos.data_ptr<float>(), sin.data_ptr<float>(),
+                  pos.defined() ? pos.data_ptr<int>() : nullptr, x.size(0) * x.size(1), (int)x.size(1), (int)cos.size(0), (int)heads, (int)kv,
+                  (int)hd, (float)eps, word(status), stream()),
+        "qk_norm_rope");
+  return y;
+}
+struct QKNormRope : Function<QKNormRope> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& qkv, const Tensor& wq_in, const Tensor& wk_in, Aside cos, Aside sin, Aside pos,
+                        int64_t heads, int64_t kv, int64_t hd, double eps, Aside buffer_q, Aside buffer_k, Aside status) {
+    ll ld;
+    const Tensor x = packed(qkv, ld), wq = dense(wq_in), wk = dense(wk_in);
+    Tensor y = qk_norm_forward(x, ld, wq, wk, cos.t, sin.t, pos.t, heads, kv, hd, eps, status.t);
+    ctx->save_for_backward({x, wq, wk, cos.t, sin.t, pos.t});
+    keep(ctx, "buffer_q", buffer_q);
+    keep(ctx, "buffer_k", buffer_k);
+    keep(ctx, "status", status);
+    ctx->saved_data["dims"] = std::vector<int64_t>{heads, kv, hd, ld};
+    ctx->saved_data["eps"] = eps;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    auto s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &wq = s[1], &wk = s[2], &cos = s[3], &sin = s[4], &pos = s[5];
+    const auto d = ctx->saved_data["dims"].toIntVector();
+    const ll B = x.size(0), S = x.size(1), hd = d[2];
+    const Tensor bq = aside(ctx, "buffer_q"), bk = aside(ctx, "buffer_k");
+    ll ldd;
+    const Tensor dy = packed(g[0], ldd);
+    Tensor dx = bf16(x.sizes(), x), part = f32({E.qk_norm_parts(B * S, (int)d[0], (int)d[1], (int)hd), 2 * hd}, x), dwq, dwk;
+    if (!bq.defined() && ctx->needs_input_grad(1)) dwq = bf16({hd}, wq);
+    if (!bk.defined() && ctx->needs_input_grad(2)) dwk = bf16({hd}, wk);
+    check(E.qk_norm_bwd(dy.data_ptr(), ldd, x.data_ptr(), d[3], wq.data_ptr(), wk.data_ptr(), cos.data_ptr<float>(), sin.data_ptr<float>(),
+                        pos.defined() ? pos.data_ptr<int>() : nullptr, dx.data_ptr(), part.data_ptr<float>(), ptr(dwq), ptr(dwk), ptr32(bq),
+                        ptr32(bk), B * S, (int)S, (int)cos.size(0), (int)d[0], (int)d[1], (int)hd, (float)ctx->saved_data["eps"].toDouble(),
+                        word(aside(ctx, "status")), stream()),
+          "qk_norm_rope_bwd");
+    return {dx, dwq.defined() ? dwq.view(wq.sizes()) : dwq, dwk.defined() ? dwk.view(wk.sizes()) : dwk, Tensor(), Tensor(), Tensor(), Tensor(),
+            Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+Maybe qk_norm_rope(const Tensor& qkv, const Tensor& wq, const Tensor& wk, const Tensor& cos, const Tensor& sin, const Maybe& at, int64_t heads,
+                   int64_t kv, int64_t hd, double eps, const Maybe& bq, const Maybe& bk, const Tensor& status) {
+  const auto dev = c10::cuda::current_device();
+  if (!here(qkv, dev) || !heads_fit(qkv, heads, kv, hd) || hd % 8 || hd > 256 || !buffer_fits(bq, wq) || !buffer_fits(bk, wk)) return std::nullopt;
+  for (const Tensor* w : {&wq, &wk})
+    if (!here(*w, dev) || w->scalar_type() != at::kBFloat16 || w->numel() != hd) return std::nullopt;
+  for (const Tensor* t : {&cos, &sin})
+    if (!here(*t, dev) || t->scalar_type() != at::kFloat || t->dim() != 2 || t->size(1) != hd / 2 || t->size(0) != cos.size(0) ||
+        !t->is_contiguous() || !on_boundary(*t))
+      return std::nullopt;
+  if (cos.size(0) < (at ? 1 : qkv.size(1))) return std::nullopt;
+  if (at && (!here(*at, dev) || at->scalar_type() != at::kInt || at->dim() != 2 || at->size(0) != qkv.size(0) || at->size(1) != qkv.size(1) ||
+             !at->is_contiguous()))
+    return std::nullopt;
+  const Aside pos{at ? *at : Tensor()}, buffer_q{bq ? *bq : Tensor()}, buffer_k{bk ? *bk : Tensor()};
+  if (at::GradMode::is_enabled() && (qkv.requires_grad() || wq.requires_grad() || wk.requires_grad()))
+    return QKNormRope::apply(qkv, wq, wk, Aside{cos}, Aside{sin}, pos, heads, kv, hd, eps, buffer_q, buffer_k, Aside{status});
+  ll ld;
+  const Tensor x = packed(qkv, ld);
+  return qk_norm_forward(x, ld, dense(wq), dense(wk), cos, sin, pos.t, heads, kv, hd, eps, status);
+}
+
+// tokens of a run whose weights fit `bytes`: of even size, whole tiles of 256 (documents.py, _chunks)
+ll run_length(ll T, ll V, ll bytes) {
+  const ll most = std::max<ll>(256, bytes / (2 * V) / 256 * 256), n = (T + most - 1) / most;
+  return ((T + n - 1) / n + 255) / 256 * 256;
+}
+// Workspaces of the product with the softmax in pieces (documents.py, _Pieces): one buffer of fp32, the weights, the scaled rows.
+struct Pieces {
+  Tensor numbers, e, xs;
+  float *stats, *target, *scale;
+  ll V, D, ld;
+  Pieces(const Tensor& x, const Tensor& w, ll rows, bool store, bool scaled) : V(w.size(0)), D(w.size(1)), ld((w.size(0) + 7) / 8 * 8) {
+    const ll per = (V + 63) / 64 * 2;                  // pieces of 64 columns or more
+    numbers = f32({rows * (per + 2)}, x);
+    stats = numbers.data_ptr<float>();
+    target = stats + rows * per;
+    scale = target + rows;
+    if (store) e = bf16({rows, ld}, x);
+    if (scaled) xs = bf16({rows, D}, x);
+  }
+  // columns of a piece
+  ll run(const Tensor& x, ll T, const Tensor& w, const void* from, const ll* labels, const Tensor& status) {
+    check(E.softmax(from, w.data_ptr(), ptr(e), labels, stats, target, (int)T, (int)V, (int)D, x.stride(0), w.stride(0), ld, word(status), stream()),
+          "gemm2_softmax");
+    return E.softmax_columns((int)T, (int)V, (int)D);
+  }
+};
+const char* row_of(const Tensor& x, ll at) { return static_cast<const char*>(x.data_ptr()) + 2 * at * x.stride(0); }
+
+Tensor token_losses(const Tensor& x, const Tensor& w, const Tensor& labels, int64_t ignore, int64_t bytes, const Tensor& status) {
+  const ll T = x.size(0), V = w.size(0), run = std::min(T, run_length(T, 16 * ((V + 127) / 128), bytes));
+  Tensor losses = f32({T}, x);
+  Pieces ws(x, w, run, false, false);
+  const ll* lab = reinterpret_cast<const ll*>(labels.data_ptr<int64_t>());
+  for (ll a = 0; a < T; a += run) {
+    const ll n = std::min(run, T - a), columns = ws.run(x, n, w, row_of(x, a), lab + a, status);
+    check(E.vocab_losses(ws.stats, ws.target, lab + a, losses.data_ptr<float>() + a, nullptr, n, (int)((V + columns - 1) / columns), (int)V, ignore,
+                         stream()),
+          "vocab_losses");
+  }
+  return losses;
+}
+Tensor count_labels(const Tensor& labels, const Tensor& like, int64_t ignore, ll V, const Tensor& status) {
+  Tensor n = at::empty({1}, like.options().dtype(at::kInt));
+  check(E.vocab_count(reinterpret_cast<const ll*>(labels.data_ptr<int64_t>()), labels.numel(), ignore, (int)V, n.data_ptr<int>(), word(status), stream()),
+        "vocab_count");
+  return n;
+}
+Tensor mean_loss(const Tensor& losses, const Tensor& n_valid) {
+  Tensor loss = f32({}, losses);
+  check(E.vocab_mean(losses.data_ptr<float>(), losses.numel(), n_valid.data_ptr<int>(), loss.data_ptr<float>(), stream()), "vocab_mean");
+  return loss;
+}
+// t * by in bf16, or added onto the buffer
+Tensor scaled_by(const Tensor& t, const Tensor& by, const Tensor& buffer, at::IntArrayRef shape) {
+  Tensor out = buffer.defined() ? buffer : at::empty(shape, t.options().dtype(at::kBFloat16));
+  check(E.vocab_scale(t.data_ptr(), t.scalar_type() == at::kFloat, by.data_ptr<float>(), out.data_ptr(), buffer.defined(), t.numel(), stream()),
+        "vocab_scale");
+  return buffer.defined() ? Tensor() : out;
+}
+
+struct LinearCrossEntropy : Function<LinearCrossEntropy> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& w_in, Aside labels, double grad_scale, int64_t ignore,
+                        Aside buffer, int64_t bytes, Aside status) {
+    const Tensor x = operand(rows(x_in)), w = operand(w_in);
+    const ll T = x.size(0), V = w.size(0), D = w.size(1), run = std::min(T, run_length(T, V, bytes));
+    const bool want_x = x_in.requires_grad(), want_w = w_in.requires_grad();
+    Tensor n_valid = count_labels(labels.t, x, ignore, V, status.t), losses = f32({T}, x), dx, dw;
+    Pieces ws(x, w, run, true, want_w);
+    if (want_x) dx = bf16({T, D}, x);
+    const bool single = run >= T && !buffer.t.defined();
+    if (want_w) dw = single ? bf16({V, D}, x) : f32({V, D}, x);
+    const ll* lab = reinterpret_cast<const ll*>(labels.t.data_ptr<int64_t>());
+    for (ll a = 0; a < T; a += run) {
+      const ll n = std::min(run, T - a), columns = ws.run(x, n, w, row_of(x, a), lab + a, status.t);
+      check(E.vocab_rows(ws.e.data_ptr(), ws.ld, ws.stats, ws.target, lab + a, nullptr, n_valid.data_ptr<int>(), (float)grad_scale, row_of(x, a),
+                         x.stride(0), ptr(ws.xs), ws.scale, losses.data_ptr<float>() + a, n, (int)((V + columns - 1) / columns), (int)columns,
+                         (int)V, (int)D, ignore, stream()),
+            "vocab_rows");
+      if (want_x) {
+        Tensor planes;
+        if (const ll parts = E.out_splits((int)n, (int)D, (int)V); parts > 1) planes = f32({parts * ((n + 31) / 32 * 32) * D}, x);
+        check(E.gemm_rows(ws.e.data_ptr(), w.data_ptr(), const_cast<char*>(row_of(dx, a)), ptr32(planes), ws.scale, (int)n, (int)D, (int)V, ws.ld,
+                          w.stride(0), D, word(status.t), stream()),
+              "gemm2_rows");
+      }
+      if (want_w) {
+        const Tensor e = ws.e.narrow(0, 0, n).narrow(1, 0, V), xs = ws.xs.narrow(0, 0, n);
+        if (a > 0 || single) {
+          gemm(e, xs, dw, true, true, a > 0 ? 1 : 0, status.t);
+        } else {                                         // the first of several stores fp32
+          check(E.gemm(e.data_ptr(), xs.data_ptr(), dw.data_ptr(), (int)V, (int)D, (int)n, ws.ld, D, D, 1, 1, 2, word(status.t), 0, stream()),
+                "tplr_gemm_bf16");
+        }
+      }
+    }
+    ctx->save_for_backward({dx, dw});
+    keep(ctx, "buffer", buffer);
+    ctx->saved_data["shape"] = x_in.sizes().vec();
+    return mean_loss(losses, n_valid);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    auto s = ctx->get_saved_variables();
+    const Tensor by = g[0].to(at::kFloat);
+    Tensor dx, dw;
+    if (s[0].defined()) dx = scaled_by(s[0], by, Tensor(), ctx->saved_data["shape"].toIntVector());
+    if (s[1].defined()) dw = scaled_by(s[1], by, aside(ctx, "buffer"), s[1].sizes());
+    return {dx, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+// The mean, or every token's loss where nothing asks for a gradient; None also for a gradient of single tokens.
+Maybe linear_cross_entropy(const Tensor& x, const Tensor& w, const Tensor& labels, double grad_scale, int64_t ignore, const Maybe& buffer, bool mean,
+                           int64_t bytes, const Tensor& status) {
+  const auto dev = c10::cuda::current_device();
+  const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad());
+  if (!here(x, dev) || !here(w, dev) || !here(labels, dev) || x.scalar_type() != at::kBFloat16 || w.scalar_type() != at::kBFloat16 ||
+      labels.scalar_type() != at::kLong || !labels.is_contiguous() || x.dim() < 1 || w.dim() != 2 || w.numel() == 0 || x.numel() == 0 ||
+      w.size(1) % 8 || x.size(-1) != w.size(1) || labels.sizes() != x.sizes().slice(0, x.dim() - 1) || (grad && !mean) || !buffer_fits(buffer, w))
+    return std::nullopt;
+  if (grad) return LinearCrossEntropy::apply(x, w, Aside{labels}, grad_scale, ignore, Aside{buffer ? *buffer : Tensor()}, bytes, Aside{status});
+  const Tensor losses = token_losses(operand(rows(x)), operand(w), labels, ignore, bytes, status);
+  return mean ? mean_loss(losses, count_labels(labels, losses, ignore, w.size(0), status)) : losses.view(labels.sizes());
+}
+
 Aside opt(const std::optional<Tensor>& t) { return Aside{t ? *t : Tensor()}; }
 
 }  // namespace
@@ -602,4 +902,7 @@ PYBIND11_MODULE(tplr_host, m) {
                                   const std::optional<Tensor>& xscale, const std::optional<Tensor>& xweight) {
     return FeedForwardSaved8::apply(x, w13, w2, opt(b13), opt(b2), Aside{status}, opt(xq), opt(xscale), opt(xweight));
   }, nogil());
+  m.def("attention_documents", &attention_documents, nogil());
+  m.def("qk_norm_rope", &qk_norm_rope, nogil());
+  m.def("linear_cross_entropy", &linear_cross_entropy, nogil());
 }

@@ -27,6 +27,10 @@ def _on(t: torch.Tensor):
     return torch.cuda.device(t.device)
 
 
+def _word(t: torch.Tensor) -> torch.Tensor:
+    return OF._status_words.get(t.get_device()) if t.get_device() in OF._status_words else OF.status_word(t.device)
+
+
 def _same_device(what: str, t: torch.Tensor, **others) -> None:
     for name, o in others.items():
         if o is not None and o.device != t.device:
@@ -127,6 +131,9 @@ def attention_documents(qkv: torch.Tensor, starts: torch.Tensor, n_heads: int, n
     Every row has to hold finite numbers, one that nothing sees too, and so has the gradient: the rows of a block of 128 meet in the
     same products, where a weight of zero times an infinity is not zero.  The kernels (bf16, heads of 64 or 128) add nothing
     into memory: results and gradients have the same bits on every run."""
+    # operands that the kernels take as they are need no further look
+    if qkv.is_cuda and (host := native.host()) and (out := host.attention_documents(qkv, starts, n_heads, n_kv, hd, _word(qkv))) is not None:
+        return out
     _heads("attention_documents", qkv, n_heads, n_kv, hd)
     B, S, C = qkv.shape
     if starts.shape != (B, S) or starts.is_floating_point() or starts.is_complex() or starts.dtype == torch.bool:
@@ -137,6 +144,9 @@ def attention_documents(qkv: torch.Tensor, starts: torch.Tensor, n_heads: int, n
     if starts.dtype != torch.int32:
         starts = starts.clamp(0, 2 ** 31 - 1).to(torch.int32) if starts.dtype == torch.int64 else starts.to(torch.int32)
     starts = starts.contiguous()
+    if host := native.host():
+        with _on(qkv):
+            return host.attention_documents(qkv, starts, n_heads, n_kv, hd, _word(qkv))
     if torch.is_grad_enabled() and qkv.requires_grad:
         return _AttentionDocuments.apply(qkv, starts, n_heads, n_kv, hd)
     rows, ld = _packed_rows(qkv)
@@ -225,6 +235,13 @@ def qk_norm_rope(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, cos: tor
     turned by the rotary embedding (interleaved pairs, tables of :func:`rope_tables`), in one pass; value heads as they are.
     ``positions``: int32 [B, S], the row of the tables that a token takes (its place in its document); without them its place
     in the sequence.  A position outside the tables takes their first or last row, and the kernels report it in the status word."""
+    if main_grad_q is None:
+        main_grad_q = getattr(wq, "main_grad", None)
+    if main_grad_k is None:
+        main_grad_k = getattr(wk, "main_grad", None)
+    if qkv.is_cuda and (host := native.host()) and (y := host.qk_norm_rope(qkv, wq, wk, cos, sin, positions, n_heads, n_kv, hd, eps, main_grad_q,
+                                                                           main_grad_k, _word(qkv))) is not None:
+        return y
     _heads("qk_norm_rope", qkv, n_heads, n_kv, hd)
     B, S, C = qkv.shape
     if wq.numel() != hd or wk.numel() != hd:
@@ -235,10 +252,6 @@ def qk_norm_rope(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, cos: tor
     if positions is not None and (positions.shape != (B, S) or positions.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"qk_norm_rope: int32 positions [{B}, {S}] expected, got {positions.dtype} {tuple(positions.shape)}")
     _same_device("qk_norm_rope", qkv, wq=wq, wk=wk, cos=cos, sin=sin, positions=positions)
-    if main_grad_q is None:
-        main_grad_q = getattr(wq, "main_grad", None)
-    if main_grad_k is None:
-        main_grad_k = getattr(wk, "main_grad", None)
     if not (OF._native_ok(qkv, wq, wk) and hd % 8 == 0 and hd <= 256 and cos.dtype == sin.dtype == torch.float32) or B * S == 0:
         if main_grad_q is not None and wq.requires_grad:
             wq = _AddMainGrad.apply(wq, main_grad_q)
@@ -248,6 +261,11 @@ def qk_norm_rope(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, cos: tor
     cos, sin = OF._dense(cos), OF._dense(sin)
     if positions is not None:
         positions = positions.clamp(-1, 2 ** 31 - 1).to(torch.int32).contiguous() if positions.dtype == torch.int64 else positions.contiguous()
+    if host := native.host():
+        with _on(qkv):
+            y = host.qk_norm_rope(qkv, wq, wk, cos, sin, positions, n_heads, n_kv, hd, eps, main_grad_q, main_grad_k, _word(qkv))
+        if y is not None:
+            return y
     if torch.is_grad_enabled() and (qkv.requires_grad or wq.requires_grad or wk.requires_grad):
         return _QKNormRope.apply(qkv, wq, wk, cos, sin, positions, n_heads, n_kv, hd, eps, main_grad_q, main_grad_k)
     rows, ld = _packed_rows(qkv)
@@ -427,9 +445,19 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
     token's own, in the shape of ``labels``, zero where it is ignored.  A label that is neither ``ignore_index`` nor a column counts as ignored, and
     the kernels report it in the status word.  The gradient is ``grad_scale`` times the loss's, and the incoming one counts.
 
-    The kernels hold ``exp(logit)`` (relative to a piece's largest where that is far from zero) for a run of tokens at a time (``CHUNK_BYTES``), from which the gradients of
-    ``x`` and ``w`` are made at once; where nothing asks for a gradient, two numbers for every 64 or 128 columns.  A mean makes its gradients in the forward
-    pass; one gradient of ``"none"`` costs the product a second time."""
+    The kernels hold ``exp(logit)`` (relative to a piece's largest where that is far from zero) for a run of tokens at a time
+    (``CHUNK_BYTES``), from which the gradients of ``x`` and ``w`` are made at once; where nothing asks for a gradient, two numbers for
+    every 64 or 128 columns.  A mean makes its gradients in the forward pass; the gradient of ``"none"`` costs the product a second time."""
+    if main_grad is None:
+        main_grad = getattr(w, "main_grad", None)
+    if main_grad is not None and not torch.is_tensor(main_grad):
+        if torch.is_grad_enabled() and w.requires_grad:
+            raise ValueError("linear_cross_entropy: the weight's gradient is a buffer here, not shards of other ranks")
+        main_grad = None
+    mean, ignore_index = reduction == "mean", int(ignore_index)
+    host = native.host() if x.is_cuda and (mean or reduction == "none") and OF.gemm_backend() == "tcgen05_2sm" else None
+    if host and (out := host.linear_cross_entropy(x, w, labels, grad_scale, ignore_index, main_grad, mean, CHUNK_BYTES, _word(x))) is not None:
+        return out
     if reduction not in ("mean", "none"):
         raise ValueError(f"linear_cross_entropy: reduction is 'mean' or 'none', got {reduction!r}")
     if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1] or w.shape[0] < 1 or w.shape[1] < 1:
@@ -437,10 +465,6 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
     if labels.shape != x.shape[:-1] or labels.is_floating_point() or labels.dtype == torch.bool:
         raise ValueError(f"linear_cross_entropy: labels {tuple(x.shape[:-1])} expected, got {labels.dtype} {tuple(labels.shape)}")
     _same_device("linear_cross_entropy", x, w=w, labels=labels)
-    if main_grad is None:
-        main_grad = getattr(w, "main_grad", None)
-    if main_grad is not None and not torch.is_tensor(main_grad):
-        raise ValueError("linear_cross_entropy: the weight's gradient is a buffer here, not shards of other ranks")
     flat = labels.reshape(-1).contiguous().to(torch.int64)
     grad = torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
     T = flat.numel()
@@ -448,19 +472,24 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
         if main_grad is not None and grad and w.requires_grad:
             w = _AddMainGrad.apply(w, main_grad)
         out = _linear_cross_entropy_torch(x, w, flat, float(grad_scale), ignore_index, reduction)
-        return out if reduction == "mean" else out.view(labels.shape)
+        return out if mean else out.view(labels.shape)
+    if host:
+        with _on(x):
+            out = host.linear_cross_entropy(x, w, flat.view(labels.shape), grad_scale, ignore_index, main_grad, mean, CHUNK_BYTES, _word(x))
+        if out is not None:
+            return out
     if grad:
-        node = _LinearCrossEntropy if reduction == "mean" else _LinearTokenLosses
-        out = node.apply(x, w, flat, float(grad_scale), int(ignore_index), main_grad)
-        return out if reduction == "mean" else out.view(labels.shape)
+        node = _LinearCrossEntropy if mean else _LinearTokenLosses
+        out = node.apply(x, w, flat, float(grad_scale), ignore_index, main_grad)
+        return out if mean else out.view(labels.shape)
     x2, wd = _operand(x.detach().reshape(-1, x.shape[-1])), _operand(w.detach())
     with _on(x2):
-        losses, _ = _token_losses(x2, wd, flat, int(ignore_index))
+        losses, _ = _token_losses(x2, wd, flat, ignore_index)
         if reduction == "none":
             return losses.view(labels.shape)
         n_valid = torch.empty(1, dtype=torch.int32, device=x2.device)
         loss = torch.empty((), dtype=torch.float32, device=x2.device)
-        native.check(native.lib().tplr_vocab_count(flat.data_ptr(), T, int(ignore_index), w.shape[0], n_valid.data_ptr(),
+        native.check(native.lib().tplr_vocab_count(flat.data_ptr(), T, ignore_index, w.shape[0], n_valid.data_ptr(),
                                                    OF.status_word(x2.device).data_ptr(), native.stream_ptr()), "vocab_count")
         native.check(native.lib().tplr_vocab_mean(losses.data_ptr(), T, n_valid.data_ptr(), loss.data_ptr(), native.stream_ptr()), "vocab_mean")
     return loss
