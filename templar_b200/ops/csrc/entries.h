@@ -78,7 +78,7 @@ int tplr_vocab_count(const long long* labels, long long T, long long ignore, int
 int tplr_vocab_losses(const float* stats, const float* target, const long long* labels, float* losses, float* lse, long long T, int parts, int V,
                       long long ignore, void* stream);
 int tplr_vocab_rows(void* E, long long ld, const float* stats, const float* target, const long long* labels, const float* row_grad,
-                    const int* n_valid, float grad_scale, const void* x, long long ldx, void* xs, float* row_scale, float* losses, long long T,
+                    const int* n_valid, float grad_scale, const void* x, long long ldx, void* xs, long long ldxs, float* row_scale, float* losses, long long T,
                     int parts, int columns, int V, int D, long long ignore, void* stream);
 int tplr_vocab_mean(const float* losses, long long T, const int* n_valid, float* loss, void* stream);
 int tplr_vocab_scale(const void* x, int x_fp32, const float* by, void* y, int add_fp32, long long n, void* stream);

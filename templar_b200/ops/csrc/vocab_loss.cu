@@ -63,11 +63,11 @@ __global__ void __launch_bounds__(256) vocab_losses_kernel(const float2* stats, 
   }
 }
 
-// What both products need of a row (see above), a warp a row: f in row_scale, E in place of e, f x in xs (dense rows of D); and the
+// What both products need of a row (see above), a warp a row: f in row_scale, E in place of e, f x in xs; and the
 // row's loss.  g = row_grad[row], or grad_scale / *n_valid.
 __global__ void __launch_bounds__(256) vocab_rows_kernel(bf16* e, long long ld, const float2* stats, const float* target, const long long* labels,
                                                          const float* row_grad, const int* n_valid, float grad_scale, const bf16* x, long long ldx,
-                                                         bf16* xs, float* row_scale, float* losses, long long T, int parts, int columns, int V,
+                                                         bf16* xs, long long ldxs, float* row_scale, float* losses, long long T, int parts, int columns, int V,
                                                          int D, long long ignore) {
   grid_wait();
   grid_release();
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(256) vocab_rows_kernel(bf16* e, long long ld, 
   if (lane == 0) row_scale[row] = f;
   if (!xs) return;
   const uint4* xr = reinterpret_cast<const uint4*>(x + row * ldx);
-  uint4* out = reinterpret_cast<uint4*>(xs + row * D);
+  uint4* out = reinterpret_cast<uint4*>(xs + row * ldxs);
 #pragma unroll 4
   for (int i = lane; i < D / 8; i += 32) {
     uint4 q = make_uint4(0u, 0u, 0u, 0u);
@@ -205,17 +205,17 @@ TPLR_API int tplr_vocab_losses(const float* stats, const float* target, const lo
 }
 
 // What tplr_gemm2_softmax left of T rows, E [T, V] (rows of ld elements), made ready for the products of the gradients: dx = row_scale * (E w),
-// dw = E^T xs.  x [T, D] (rows of ldx elements), xs [T, D] dense or null; losses [T] may be null.  row_grad [T] the gradients of the rows'
+// dw = E^T xs.  x and xs [T, D] (rows of ldx and ldxs elements), xs or null; losses [T] may be null.  row_grad [T] the gradients of the rows'
 // losses, or null: grad_scale / n_valid[0] for every row.  columns: of a piece.
 TPLR_API int tplr_vocab_rows(void* E, long long ld, const float* stats, const float* target, const long long* labels, const float* row_grad,
-                             const int* n_valid, float grad_scale, const void* x, long long ldx, void* xs, float* row_scale, float* losses,
+                             const int* n_valid, float grad_scale, const void* x, long long ldx, void* xs, long long ldxs, float* row_scale, float* losses,
                              long long T, int parts, int columns, int V, int D, long long ignore, void* stream) {
   TPLR_ENTER();
   if (T <= 0) return 0;
-  if ((ld % 8) || ld < V || (columns % 8) || columns <= 0 || (ldx % 8) || (D % 8) || (((uintptr_t)E | (uintptr_t)x | (uintptr_t)xs) & 15)) return -401;
+  if ((ld % 8) || ld < V || (columns % 8) || columns <= 0 || (ldx % 8) || (ldxs % 8) || (xs && ldxs < D) || (D % 8) || (((uintptr_t)E | (uintptr_t)x | (uintptr_t)xs) & 15)) return -401;
   return (int)launch_pdl(vocab_rows_kernel, (unsigned)((T + 7) / 8), 256, 0, (cudaStream_t)stream, (bf16*)E, ld,
                          reinterpret_cast<const float2*>(stats), target, labels, row_grad, n_valid, grad_scale, (const bf16*)x, ldx, (bf16*)xs,
-                         row_scale, losses, T, parts, columns, V, D, ignore);
+                         ldxs, row_scale, losses, T, parts, columns, V, D, ignore);
 }
 
 // loss[0] = sum of losses [T] / max(n_valid[0], 1)

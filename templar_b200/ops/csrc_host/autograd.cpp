@@ -737,15 +737,16 @@ ll run_length(ll T, ll V, ll bytes) {
 struct Pieces {
   Tensor numbers, e, xs;
   float *stats, *target, *scale;
-  ll V, D, ld;
-  Pieces(const Tensor& x, const Tensor& w, ll rows, bool store, bool scaled) : V(w.size(0)), D(w.size(1)), ld((w.size(0) + 7) / 8 * 8) {
+  ll V, D, ld, ldxs;                                   // rows on 128-byte boundaries, as the products' copies take them best
+  Pieces(const Tensor& x, const Tensor& w, ll rows, bool store, bool scaled)
+      : V(w.size(0)), D(w.size(1)), ld((w.size(0) + 63) / 64 * 64), ldxs((w.size(1) + 63) / 64 * 64) {
     const ll per = (V + 63) / 64 * 2;                  // pieces of 64 columns or more
     numbers = f32({rows * (per + 2)}, x);
     stats = numbers.data_ptr<float>();
     target = stats + rows * per;
     scale = target + rows;
     if (store) e = bf16({rows, ld}, x);
-    if (scaled) xs = bf16({rows, D}, x);
+    if (scaled) xs = bf16({rows, ldxs}, x);
   }
   // columns of a piece
   ll run(const Tensor& x, ll T, const Tensor& w, const void* from, const ll* labels, const Tensor& status) {
@@ -803,7 +804,7 @@ struct LinearCrossEntropy : Function<LinearCrossEntropy> {
     for (ll a = 0; a < T; a += run) {
       const ll n = std::min(run, T - a), columns = ws.run(x, n, w, row_of(x, a), lab + a, status.t);
       check(E.vocab_rows(ws.e.data_ptr(), ws.ld, ws.stats, ws.target, lab + a, nullptr, n_valid.data_ptr<int>(), (float)grad_scale, row_of(x, a),
-                         x.stride(0), ptr(ws.xs), ws.scale, losses.data_ptr<float>() + a, n, (int)((V + columns - 1) / columns), (int)columns,
+                         x.stride(0), ptr(ws.xs), ws.ldxs, ws.scale, losses.data_ptr<float>() + a, n, (int)((V + columns - 1) / columns), (int)columns,
                          (int)V, (int)D, ignore, stream()),
             "vocab_rows");
       if (want_x) {
@@ -814,11 +815,11 @@ struct LinearCrossEntropy : Function<LinearCrossEntropy> {
               "gemm2_rows");
       }
       if (want_w) {
-        const Tensor e = ws.e.narrow(0, 0, n).narrow(1, 0, V), xs = ws.xs.narrow(0, 0, n);
+        const Tensor e = ws.e.narrow(0, 0, n).narrow(1, 0, V), xs = ws.xs.narrow(0, 0, n).narrow(1, 0, D);
         if (a > 0 || single) {
           gemm(e, xs, dw, true, true, a > 0 ? 1 : 0, status.t);
         } else {                                         // the first of several stores fp32
-          check(E.gemm(e.data_ptr(), xs.data_ptr(), dw.data_ptr(), (int)V, (int)D, (int)n, ws.ld, D, D, 1, 1, 2, word(status.t), 0, stream()),
+          check(E.gemm(e.data_ptr(), xs.data_ptr(), dw.data_ptr(), (int)V, (int)D, (int)n, ws.ld, ws.ldxs, D, 1, 1, 2, word(status.t), 0, stream()),
                 "tplr_gemm_bf16");
         }
       }

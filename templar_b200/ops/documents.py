@@ -289,12 +289,14 @@ class _Pieces:
     def __init__(self, x2, w, rows: int, store: bool, scaled_rows: bool = False):
         self.V, self.D = w.shape
         dev = x2.device
-        self.ld = -(-self.V // 8) * 8
+        # rows on 128-byte boundaries, as the products' copies take them best: 1111 tokens, 1000 x 50257, dx 132 us with rows of 50264
+        # elements, 105 with 50304, dw 107 and 92
+        self.ld, self.ldxs = (-(-n // 64) * 64 for n in w.shape)
         self.e = torch.empty(rows, self.ld, dtype=torch.bfloat16, device=dev) if store else None
         self.stats = torch.empty(rows * -(-self.V // 64) * 2, dtype=torch.float32, device=dev)      # pieces of 64 columns or more
         self.target = torch.empty(rows, dtype=torch.float32, device=dev)
         self.scale = torch.empty(rows, dtype=torch.float32, device=dev) if store else None
-        self.xs = torch.empty(rows, self.D, dtype=torch.bfloat16, device=dev) if scaled_rows else None
+        self.xs = torch.empty(rows, self.ldxs, dtype=torch.bfloat16, device=dev) if scaled_rows else None
 
     def run(self, x, w, labels) -> tuple[int, int]:
         """(pieces of a row, columns of a piece)"""
@@ -333,7 +335,7 @@ def _gradients(x2, w, labels, ignore_index, row_grad, n_valid, grad_scale, losse
         parts, columns = ws.run(x, w, labels[a:b])
         native.check(L.tplr_vocab_rows(
             ws.e.data_ptr(), ws.ld, ws.stats.data_ptr(), ws.target.data_ptr(), labels[a:].data_ptr(),
-            None if row_grad is None else row_grad[a:].data_ptr(), native.ptr(n_valid), grad_scale, x.data_ptr(), x.stride(0), native.ptr(ws.xs),
+            None if row_grad is None else row_grad[a:].data_ptr(), native.ptr(n_valid), grad_scale, x.data_ptr(), x.stride(0), native.ptr(ws.xs), ws.ldxs,
             ws.scale.data_ptr(), None if losses is None else losses[a:].data_ptr(), b - a, parts, columns, V, D, ignore_index,
             native.stream_ptr()), "vocab_rows")
         if want_x:
@@ -345,9 +347,9 @@ def _gradients(x2, w, labels, ignore_index, row_grad, n_valid, grad_scale, losse
             single = len(runs) == 1 and not keep32
             if dw is None:
                 dw = torch.empty(V, D, dtype=torch.bfloat16 if single else torch.float32, device=x2.device)
-                OF.gemm(e, ws.xs[:b - a], a_mn=True, b_mn=True, out=dw)
+                OF.gemm(e, ws.xs[:b - a, :D], a_mn=True, b_mn=True, out=dw)
             else:
-                OF.gemm(e, ws.xs[:b - a], a_mn=True, b_mn=True, out=dw, accumulate=True)
+                OF.gemm(e, ws.xs[:b - a, :D], a_mn=True, b_mn=True, out=dw, accumulate=True)
     return dx, dw
 
 
