@@ -2099,14 +2099,20 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       }
       if (!(ok = give_tile(sh, k, lane, abort_flag, tile < p.tiles ? tile : -1, nb)) || tile >= p.tiles) break;
       const int row0 = qi * BQ, qcol = h * DH, kcol = (p.H + h / group) * DH, vcol = (p.H + p.KV + h / group) * DH;
-      if (!(ok = mbar_wait_warp(smem_u32(&sh.res_empty), (uint32_t)((k & 1) ^ 1), abort_flag))) break;
-      if (lane == 0) {
-        mbar_expect_tx(smem_u32(&sh.res_full), 2 * TILE_BYTES);
-        load_tile<DH>(sQ, &p.tmQKV, smem_u32(&sh.res_full), qcol, row0, b);
-        load_tile<DH>(sdO, &p.tmDO, smem_u32(&sh.res_full), qcol, row0, b);
-      }
-      __syncwarp();
+      bool resident = false;
+      auto load_resident = [&]() -> bool {
+        if (!mbar_wait_warp(smem_u32(&sh.res_empty), (uint32_t)((k & 1) ^ 1), abort_flag)) return false;
+        if (lane == 0) {
+          mbar_expect_tx(smem_u32(&sh.res_full), 2 * TILE_BYTES);
+          load_tile<DH>(sQ, &p.tmQKV, smem_u32(&sh.res_full), qcol, row0, b);
+          load_tile<DH>(sdO, &p.tmDO, smem_u32(&sh.res_full), qcol, row0, b);
+        }
+        __syncwarp();
+        return resident = true;
+      };
+      // the first K and V go ahead: their places are free while the last tile's Q and dO are still in use
       for (int t = 0; t < nb && ok; ++t) {
+        if (t == 1 && !(ok = load_resident())) break;
         const int krow = (qi - t) * BKV, s2 = n_v & 1;
         if (!(ok = mbar_wait_warp(smem_u32(&sh.ring_empty[s3]), ph3 ^ 1u, abort_flag))) break;
         if (lane == 0) {
@@ -2124,7 +2130,8 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         __syncwarp();
         ++n_v;
       }
-      if (!ok) { ++k; break; }
+      if (ok && !resident) ok = load_resident();
+      if (!ok) { k += resident; break; }
       tile = next_tile(p, lane);                           // not before its loads can begin: walks differ, and a tile taken early waits
     }
     if (lane == 0) {
@@ -2200,31 +2207,38 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
     const uint32_t sw = (uint32_t)(lane & 7);
     const unsigned long long sl2 = two(p.scale_log2), sc = two(p.scale);
     int n = 0, n_acc = 0;                                  // steps and tiles with a step so far
-    int tile, nb;
     bool ok = true;
-    for (int k = 0;; ++k) {
-      // both warps of a pair leave the loop together: they join their answers wherever one could leave alone
-      ok = take_tile(sh, k, lane, abort_flag, tile, nb);
-      if (!pair_agrees(ok, quad)) break;
-      int qi, h, b;
+    // the k-th tile and this thread's row of it: asked for before the tile in front of it is finished, so that they are there in time
+    int tile, nb, qi, h, b, row, start;                    // start INT_MAX: the row sees nothing, or is past the end
+    long long at;
+    float lse2;
+    uint4 o[DH / 16];                                      // this half of the row's output
+    auto take = [&](int k) -> bool {
+      if (!take_tile(sh, k, lane, abort_flag, tile, nb)) return false;
       place(tile, qi, h, b);
-      const int row = qi * BQ + r;
-      const long long at = ((long long)b * p.H + h) * p.S + row;
-      int start = INT_MAX;                                 // INT_MAX: the row sees nothing, or is past the end
-      float lse2 = INFINITY;
-      uint4 o[DH / 16];                                    // this half of the row's output
+      row = qi * BQ + r;
+      at = ((long long)b * p.H + h) * p.S + row;
+      start = INT_MAX;
+      lse2 = INFINITY;
 #pragma unroll
       for (int q = 0; q < DH / 16; ++q) o[q] = make_uint4(0u, 0u, 0u, 0u);
       if (row < p.S) {
         start = max(p.starts[(long long)b * p.S + row], 0);
-        if (start > row) start = INT_MAX;
-        if (start != INT_MAX) {
-          lse2 = p.lse[at] * 1.4426950408889634f;
-          const uint4* orow = reinterpret_cast<const uint4*>(p.out + ((long long)b * p.S + row) * ((long long)p.H * DH) + h * DH + ch * (DH / 2));
+        lse2 = p.lse[at];                                  // infinite where the row sees nothing, whose output is zero
+        const uint4* orow = reinterpret_cast<const uint4*>(p.out + ((long long)b * p.S + row) * ((long long)p.H * DH) + h * DH + ch * (DH / 2));
 #pragma unroll
-          for (int q = 0; q < DH / 16; ++q) o[q] = orow[q];
-        }
+        for (int q = 0; q < DH / 16; ++q) o[q] = orow[q];
       }
+      return true;
+    };
+    bool more = take(0);
+    for (int k = 0;; ++k) {
+      // both warps of a pair leave the loop together: they join their answers wherever one could leave alone
+      if (!pair_agrees(more, quad)) break;
+      if (start > row) start = INT_MAX;
+      lse2 *= 1.4426950408889634f;
+      __nv_bfloat16* const to = p.dqkv + ((long long)b * p.S + row) * C + h * DH + ch * (DH / 2);
+      const bool live = row < p.S;
       ok = mbar_wait_warp(smem_u32(&sh.res_full), (uint32_t)(k & 1), abort_flag);
       float delta = 0.f;
       if (ok) {
@@ -2248,9 +2262,10 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       }
       if (!(ok = pair_agrees(ok, quad))) break;
       delta = start == INT_MAX ? 0.f : sh.part[0][r] + sh.part[1][r];
-      if (ch == 0 && row < p.S) p.delta[at] = delta;
+      if (ch == 0 && live) p.delta[at] = delta;
       const unsigned long long nl = two(-lse2), nd = two(-delta * p.scale);
-      for (int t = 0; t < nb; ++t, ++n) {
+      const int steps = nb;
+      for (int t = 0; t < steps; ++t, ++n) {
         const bool diag = t == 0;
         const int lo = (start == INT_MAX ? BKV : start - (qi - t) * BKV) - ch * 64, hi = (diag ? r : BKV - 1) - ch * 64;
         if (!(ok = mbar_wait_warp(smem_u32(&sh.s_full[n & 1]), (uint32_t)((n >> 1) & 1), abort_flag))) break;
@@ -2293,12 +2308,12 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         if (lane == 0) mbar_arrive(smem_u32(&sh.ds_ready));
       }
       // dQ -> bf16 -> the query columns of the gradient
-      if (ok && nb > 0) ok = mbar_wait_warp(smem_u32(&sh.acc_full), (uint32_t)(n_acc++ & 1), abort_flag);
+      more = ok && take(k + 1);
+      if (ok && steps > 0) ok = mbar_wait_warp(smem_u32(&sh.acc_full), (uint32_t)(n_acc++ & 1), abort_flag);
       if (!(ok = pair_agrees(ok, quad))) break;
       tcgen05_fence_after();
-      __nv_bfloat16* to = p.dqkv + ((long long)b * p.S + row) * C + h * DH + ch * (DH / 2);
 #pragma unroll
-      for (int c = 0; c < DH / 64; ++c) store_row32(to + c * 32, tdQ + ch * (DH / 2) + c * 32 + lane_off, nb == 0, row < p.S);
+      for (int c = 0; c < DH / 64; ++c) store_row32(to + c * 32, tdQ + ch * (DH / 2) + c * 32 + lane_off, steps == 0, live);
       tcgen05_fence_before();                              // the next tile's first dQ is behind this warp's next dS
     }
   }
@@ -2354,16 +2369,22 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         n_i = max(__reduce_max_sync(0xffffffffu, last) - a.j + 1, 0);
       }
       if (!(ok = give_tile(sh, k, lane, abort_flag, tile < p.tiles ? tile : -1, n_i)) || tile >= p.tiles) break;
-      if (!(ok = mbar_wait_warp(smem_u32(&sh.res_empty), (uint32_t)((k & 1) ^ 1), abort_flag))) break;
-      if (lane == 0) {
-        mbar_expect_tx(smem_u32(&sh.res_full), 2 * TILE_BYTES);
-        load_tile<DH>(sK, &p.tmQKV, smem_u32(&sh.res_full), (p.H + a.g) * DH, a.j * BKV, a.b);
-        load_tile<DH>(sV, &p.tmQKV, smem_u32(&sh.res_full), (p.H + p.KV + a.g) * DH, a.j * BKV, a.b);
-      }
-      __syncwarp();
       const int n_it = heads * n_i;
+      bool resident = false;
+      auto load_resident = [&]() -> bool {
+        if (!mbar_wait_warp(smem_u32(&sh.res_empty), (uint32_t)((k & 1) ^ 1), abort_flag)) return false;
+        if (lane == 0) {
+          mbar_expect_tx(smem_u32(&sh.res_full), 2 * TILE_BYTES);
+          load_tile<DH>(sK, &p.tmQKV, smem_u32(&sh.res_full), (p.H + a.g) * DH, a.j * BKV, a.b);
+          load_tile<DH>(sV, &p.tmQKV, smem_u32(&sh.res_full), (p.H + p.KV + a.g) * DH, a.j * BKV, a.b);
+        }
+        __syncwarp();
+        return resident = true;
+      };
       int h = a.h0, i = 0;
+      // the first Q and dO go ahead: their places are free while the last tile's K and V are still in use
       for (int t = 0; t < n_it && ok; ++t) {
+        if (t == 1 && !(ok = load_resident())) break;
         const int qrow0 = (a.j + i) * BQ, s2 = n_do & 1;
         if (!(ok = mbar_wait_warp(smem_u32(&sh.ring_empty[s3]), ph3 ^ 1u, abort_flag))) break;
         if (lane == 0) {
@@ -2382,7 +2403,8 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         ++n_do;
         if (++i == n_i) { i = 0; ++h; }
       }
-      if (!ok) { ++k; break; }
+      if (ok && !resident) ok = load_resident();
+      if (!ok) { k += resident; break; }
       tile = next_tile(p, lane);                           // not before its loads can begin: walks differ, and a tile taken early waits
     }
     if (lane == 0) {
