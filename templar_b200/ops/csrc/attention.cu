@@ -1914,12 +1914,14 @@ TPLR_API int tplr_attention_docs_fwd(const void* qkv, const int* starts, void* o
 //
 // dQ: a tile is a query block of one head, as in the forward kernel, and walks the same key blocks in the same order.  Per step
 // S = Q K^T, dP = dO V^T (tensor cores -> TMEM), P = exp2(S * scale - lse), dS = P * (dP - delta) * scale (softmax warps, a query row a thread
-// pair), dS as bf16 over the dP columns, dQ += dS K with dS from tensor memory.  Two S buffers, so that the next exponentials run
-// under this step's products.  delta, the row sum of dO * O, is formed on the way and left for the other kernel.
+// pair), dS as bf16 over the dP columns, dQ += dS K with dS from tensor memory.  S is free again as soon as the warps hold it, and dP has
+// two buffers, so the next step's S and dP are computed while this one's exponentials are taken.  delta, the row sum of dO * O, is
+// formed on the way and left for the other kernel.
 //
 // dK, dV: a tile is a key/value block of one kv head and the query heads of its group, or a part of them, and walks the query blocks
 // from the diagonal to the last that sees any of its keys.  Everything is transposed, with the key row as the TMEM lane:
 //   S^T = K Q^T, dP^T = V dO^T;  P^T and dS^T as packed bf16 over them;  dV += P^T dO, dK += dS^T Q
+// (at DH = 64 with two buffers for S^T; at 128 the accumulators leave no room)
 // with P^T and dS^T from tensor memory: neither goes through shared memory, whose traffic bounds the causal kernel above (4600 of its 5250
 // cycles a step at DH = 128).  lse, delta and the starts belong to columns here: a warp of its own brings them to shared memory.
 //
@@ -1940,7 +1942,7 @@ template <int DH> constexpr int docs_bwd_smem() { return docs_bwd_tiles<DH>() + 
 struct DocsBwdShared {
   uint64_t res_full, res_empty;                            // the tile's resident operands
   uint64_t ring_full[RING3], ring_empty[RING3], pair_full[2], pair_empty[2];
-  uint64_t s_full[2], dp_full, p_ready, ds_ready, acc_full, stat_full[2], stat_empty[2], tile_full[2], tile_empty[2];
+  uint64_t s_full[2], dp_full, p_ready[2], ds_ready[2], acc_full, stat_full[2], stat_empty[2], tile_full[2], tile_empty[2];
   uint32_t tmem_base;
   int abort;
   int2 tile[2];                                            // (tile or -1, blocks of its walk)
@@ -2004,8 +2006,10 @@ __device__ __forceinline__ void docs_bwd_init(DocsBwdShared& sh, int warp, int c
       mbar_init(smem_u32(&sh.pair_full[s]), 1); mbar_init(smem_u32(&sh.pair_empty[s]), 1); mbar_init(smem_u32(&sh.s_full[s]), 1);
       mbar_init(smem_u32(&sh.stat_full[s]), 1); mbar_init(smem_u32(&sh.stat_empty[s]), 8);
       mbar_init(smem_u32(&sh.tile_full[s]), 1); mbar_init(smem_u32(&sh.tile_empty[s]), consumers);
+      // a barrier for even and one for odd steps: a warp may be a step ahead of another
+      mbar_init(smem_u32(&sh.p_ready[s]), 8); mbar_init(smem_u32(&sh.ds_ready[s]), 8);
     }
-    mbar_init(smem_u32(&sh.dp_full), 1); mbar_init(smem_u32(&sh.p_ready), 8); mbar_init(smem_u32(&sh.ds_ready), 8);
+    mbar_init(smem_u32(&sh.dp_full), 1);
     mbar_init(smem_u32(&sh.acc_full), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -2084,7 +2088,9 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
   grid_wait();
   grid_release();
   const uint32_t tmem_base = sh.tmem_base;
-  const uint32_t tdP = tmem_base + 128, tdQ = tmem_base + 256;       // S of even steps in columns 0..127, of odd ones in 384..511
+  const uint32_t tdP0 = tmem_base + 128, tdQ = tmem_base + 256;      // S in columns 0..127; dP of even steps in 128..255, of odd ones in 384..511
+  auto dp_of = [&](int step) { return tdP0 + (step & 1) * 256; };
+  auto dp_bar = [&](int step) { return smem_u32(step & 1 ? &sh.s_full[1] : &sh.dp_full); };
 
   if (warp == 0) {
     bool ok = true;
@@ -2150,24 +2156,25 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
     int n = 0;                                             // steps so far
     auto issue_s = [&](int step) -> bool {
       if (!mbar_wait_warp(smem_u32(&sh.ring_full[s3]), ph3, abort_flag)) return false;
+      if (step > 0 && !mbar_wait_warp(smem_u32(&sh.p_ready[(step - 1) & 1]), (uint32_t)(((step - 1) >> 1) & 1), abort_flag)) return false;      // every warp holds the last S
       tcgen05_fence_after();
       if (leader) {
-        const uint32_t d = tmem_base + (step & 1) * 384, q = (uint32_t)s3 * (TILE_BYTES / 16);
+        const uint32_t q = (uint32_t)s3 * (TILE_BYTES / 16);
 #pragma unroll
-        for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(d, kQ, koff(kk), kK, q + koff(kk), id_kk, kk > 0 ? 1u : 0u);
-        umma_commit(smem_u32(&sh.s_full[step & 1]));
+        for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(tmem_base, kQ, koff(kk), kK, q + koff(kk), id_kk, kk > 0 ? 1u : 0u);
+        umma_commit(smem_u32(&sh.s_full[0]));
       }
       if (++s3 == RING3) { s3 = 0; ph3 ^= 1u; }
       return true;
     };
-    auto issue_dp = [&](int step, bool last) -> bool {
+    auto issue_dp = [&](int step, bool last) -> bool {     // behind dQ(step - 2), which reads dS from the same columns
       if (!mbar_wait_warp(smem_u32(&sh.pair_full[step & 1]), (uint32_t)((step >> 1) & 1), abort_flag)) return false;
       tcgen05_fence_after();
       if (leader) {
-        const uint32_t v = (uint32_t)(step & 1) * (TILE_BYTES / 16);
+        const uint32_t v = (uint32_t)(step & 1) * (TILE_BYTES / 16), d = dp_of(step);
 #pragma unroll
-        for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(tdP, kdO, koff(kk), kV, v + koff(kk), id_kk, kk > 0 ? 1u : 0u);
-        umma_commit(smem_u32(&sh.dp_full));
+        for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(d, kdO, koff(kk), kV, v + koff(kk), id_kk, kk > 0 ? 1u : 0u);
+        umma_commit(dp_bar(step));
         umma_commit(smem_u32(&sh.pair_empty[step & 1]));
         if (last) umma_commit(smem_u32(&sh.res_empty));    // no product reads Q or dO any more
       }
@@ -2181,23 +2188,21 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         if (leader) mbar_arrive(smem_u32(&sh.res_empty));
         continue;
       }
-      // the S buffer of the first step was read by every warp in front of the last dS but one, its dP columns by the last dQ
       if (!(ok = issue_s(n))) break;
       if (!(ok = issue_dp(n, nb == 1))) break;
       for (int t = 0; t < nb; ++t, ++n) {
-        if (t + 1 < nb && !(ok = issue_s(n + 1))) break;
-        if (!(ok = mbar_wait_warp(smem_u32(&sh.ds_ready), n & 1, abort_flag))) break;
+        if (t + 1 < nb && !(ok = issue_s(n + 1) && issue_dp(n + 1, t + 2 == nb))) break;
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.ds_ready[n & 1]), (uint32_t)((n >> 1) & 1), abort_flag))) break;
         tcgen05_fence_after();
         if (leader) {
-          const uint32_t q = (uint32_t)r3 * (TILE_BYTES / 16);
+          const uint32_t q = (uint32_t)r3 * (TILE_BYTES / 16), d = dp_of(n);
 #pragma unroll
           for (int kk = 0; kk < BKV / 16; ++kk)            // dQ[q, d] += dS[q, kv] K[kv, d]; dS packed in the first half of each warp's dP columns
-            umma_ts_bf16_b(tdQ, tdP + (kk >> 2) * 64 + 8 * (kk & 3), mK, q + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
+            umma_ts_bf16_b(tdQ, d + (kk >> 2) * 64 + 8 * (kk & 3), mK, q + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
           umma_commit(smem_u32(&sh.ring_empty[r3]));
           if (t == nb - 1) umma_commit(smem_u32(&sh.acc_full));
         }
         if (++r3 == RING3) r3 = 0;
-        if (t + 1 < nb && !(ok = issue_dp(n + 1, t + 2 == nb))) break;       // behind dQ(t), which reads dS(t) from its columns
       }
     }
   } else {
@@ -2268,15 +2273,18 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       for (int t = 0; t < steps; ++t, ++n) {
         const bool diag = t == 0;
         const int lo = (start == INT_MAX ? BKV : start - (qi - t) * BKV) - ch * 64, hi = (diag ? r : BKV - 1) - ch * 64;
-        if (!(ok = mbar_wait_warp(smem_u32(&sh.s_full[n & 1]), (uint32_t)((n >> 1) & 1), abort_flag))) break;
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.s_full[0]), n & 1, abort_flag))) break;
         tcgen05_fence_after();
         uint32_t v[64];
-        const uint32_t tS = tmem_base + (n & 1) * 384 + ch * 64 + lane_off;
+        const uint32_t tS = tmem_base + ch * 64 + lane_off, tdP = dp_of(n);
         tmem_ld32_nowait(tS, v);
         tmem_ld32_nowait(tS + 32, v + 32);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         behind_wait32(v);
         behind_wait32(v + 32);
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.p_ready[n & 1]));
 #pragma unroll
         for (int e = 0; e < 64; e += 2) {
           float a0, a1;
@@ -2288,7 +2296,7 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
 #pragma unroll
           for (int e = 0; e < 64; ++e) if (e < lo || e > hi) v[e] = 0u;
         }
-        if (!(ok = mbar_wait_warp(smem_u32(&sh.dp_full), n & 1, abort_flag))) break;
+        if (!(ok = mbar_wait_warp(dp_bar(n), (uint32_t)((n >> 1) & 1), abort_flag))) break;
         tcgen05_fence_after();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -2305,7 +2313,7 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         tmem_wait_st();
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.ds_ready));
+        if (lane == 0) mbar_arrive(smem_u32(&sh.ds_ready[n & 1]));
       }
       // dQ -> bf16 -> the query columns of the gradient
       more = ok && take(k + 1);
@@ -2350,7 +2358,10 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
   grid_wait();
   grid_release();
   const uint32_t tmem_base = sh.tmem_base;
-  const uint32_t tS = tmem_base, tdP = tmem_base + 128, tdV = tmem_base + 256, tdK = tmem_base + 384;
+  // S^T of even steps in columns 0..127; at DH = 64 of odd ones in 384..511, so that the next step's is computed ahead
+  constexpr bool AHEAD = DH == 64;
+  const uint32_t tdP = tmem_base + 128, tdV = tmem_base + 256, tdK = tmem_base + 256 + DH;
+  auto s_of = [&](int step) { return AHEAD ? tmem_base + (step & 1) * 384 : tmem_base; };
 
   if (warp == 0) {
     bool ok = true;
@@ -2421,14 +2432,14 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
     int s3 = 0, r3 = 0;                                    // ring places of the next S's and of the next dK's Q
     uint32_t ph3 = 0;
     int n = 0;                                             // steps so far
-    auto issue_s = [&]() -> bool {                         // S^T = K Q^T
+    auto issue_s = [&](int step) -> bool {                 // S^T = K Q^T, behind the dV that reads P^T from its columns
       if (!mbar_wait_warp(smem_u32(&sh.ring_full[s3]), ph3, abort_flag)) return false;
       tcgen05_fence_after();
       if (leader) {
-        const uint32_t q = (uint32_t)s3 * (TILE_BYTES / 16);
+        const uint32_t q = (uint32_t)s3 * (TILE_BYTES / 16), d = s_of(step);
 #pragma unroll
-        for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(tS, kK, koff(kk), kQ, q + koff(kk), id_kk, kk > 0 ? 1u : 0u);
-        umma_commit(smem_u32(&sh.s_full[0]));
+        for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(d, kK, koff(kk), kQ, q + koff(kk), id_kk, kk > 0 ? 1u : 0u);
+        umma_commit(smem_u32(&sh.s_full[AHEAD ? step & 1 : 0]));
       }
       if (++s3 == RING3) { s3 = 0; ph3 ^= 1u; }
       return true;
@@ -2454,21 +2465,22 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         if (leader) mbar_arrive(smem_u32(&sh.res_empty));
         continue;
       }
-      if (!(ok = issue_s())) break;                        // behind the last dV, which reads P^T from these columns, as dP behind the last dK
-      if (!(ok = issue_dp(n, n_it == 1))) break;
+      if (!(ok = issue_s(n))) break;
+      if (!(ok = issue_dp(n, n_it == 1))) break;           // behind the last dK, which reads dS^T from these columns
       for (int t = 0; t < n_it; ++t, ++n) {
+        if (AHEAD && t + 1 < n_it && !(ok = issue_s(n + 1))) break;
         // P^T over S^T, read by every warp; in a tile's first step every warp has read the last tile's accumulators before
-        if (!(ok = mbar_wait_warp(smem_u32(&sh.p_ready), n & 1, abort_flag))) break;
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.p_ready[n & 1]), (uint32_t)((n >> 1) & 1), abort_flag))) break;
         tcgen05_fence_after();
         if (leader) {
-          const uint32_t d = (uint32_t)(n & 1) * (TILE_BYTES / 16);
+          const uint32_t d = (uint32_t)(n & 1) * (TILE_BYTES / 16), tP = s_of(n);
 #pragma unroll
           for (int kk = 0; kk < BQ / 16; ++kk)             // dV[kv, d] += P^T[kv, q] dO[q, d]
-            umma_ts_bf16_b(tdV, tS + (kk >> 2) * 64 + 8 * (kk & 3), mdO, d + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
+            umma_ts_bf16_b(tdV, tP + (kk >> 2) * 64 + 8 * (kk & 3), mdO, d + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
           umma_commit(smem_u32(&sh.pair_empty[n & 1]));    // dP(t) read dO(t) before
         }
-        if (t + 1 < n_it && !(ok = issue_s())) break;      // behind dV(t), which reads P^T(t) from its columns
-        if (!(ok = mbar_wait_warp(smem_u32(&sh.ds_ready), n & 1, abort_flag))) break;      // dS^T over dP^T
+        if (!AHEAD && t + 1 < n_it && !(ok = issue_s(n + 1))) break;
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.ds_ready[n & 1]), (uint32_t)((n >> 1) & 1), abort_flag))) break;      // dS^T over dP^T
         tcgen05_fence_after();
         if (leader) {
           const uint32_t q = (uint32_t)r3 * (TILE_BYTES / 16);
@@ -2532,8 +2544,9 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         const bool diag = i == 0;
         if (++i == n_i) i = 0;
         if (!(ok = mbar_wait_warp(smem_u32(&sh.stat_full[n & 1]), (uint32_t)((n >> 1) & 1), abort_flag))) break;
-        if (!(ok = mbar_wait_warp(smem_u32(&sh.s_full[0]), n & 1, abort_flag))) break;
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.s_full[AHEAD ? n & 1 : 0]), (uint32_t)(AHEAD ? (n >> 1) & 1 : n & 1), abort_flag))) break;
         tcgen05_fence_after();
+        const uint32_t tS = s_of(n);
         uint32_t v[64];                                    // P, in fp32 for dS
         tmem_ld32_nowait(tS + ch * 64 + lane_off, v);
         tmem_ld32_nowait(tS + ch * 64 + 32 + lane_off, v + 32);
@@ -2574,7 +2587,7 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         tmem_wait_st();
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.p_ready));
+        if (lane == 0) mbar_arrive(smem_u32(&sh.p_ready[n & 1]));
         if (!(ok = mbar_wait_warp(smem_u32(&sh.dp_full), n & 1, abort_flag))) break;
         tcgen05_fence_after();
 #pragma unroll
@@ -2596,7 +2609,7 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         tmem_wait_st();
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) { mbar_arrive(smem_u32(&sh.ds_ready)); mbar_arrive(smem_u32(&sh.stat_empty[n & 1])); }
+        if (lane == 0) { mbar_arrive(smem_u32(&sh.ds_ready[n & 1])); mbar_arrive(smem_u32(&sh.stat_empty[n & 1])); }
       }
       // dV and dK of this block.  Whole group in this tile: rounded into the packed gradient; a part of it: in fp32 in columns of its own, which
       // a last pass adds in order.

@@ -131,7 +131,7 @@ def test_attention_documents_gives_the_same_bits_every_time(hd):
     dout = normal(g, 3, 1100, 8 * hd)
     starts = starts_of("long", 3, 1100, g)
     runs = []
-    for _ in range(4):
+    for _ in range(12):                                        # more tiles than CTAs, each CTA's warps a step apart at times
         out = ops.attention_documents(qkv, starts, 8, 4, hd)
         runs.append((out.detach(), *torch.autograd.grad(out, qkv, dout)))
     assert all(torch.equal(x, y) for r in runs[1:] for x, y in zip(r, runs[0]))
@@ -441,3 +441,101 @@ def test_loss_takes_views():
     wide[:, 5:77] = x
     for xv, wv in ((wide[:, 5:77], w), (x.t().contiguous().t(), w.t().contiguous().t()), (x[:, None].expand(90, 1, 72)[:, 0], w)):
         assert torch.equal(ops.linear_cross_entropy(xv, wv, labels.to(torch.int32), reduction="none"), want)
+
+
+# ------------------------------------------------------------------------------------------ together, captured, on other streams
+def training_step(qkv, starts, positions, wq, wk, cos, sin, w, labels, H, KV, hd):
+    """The operators one behind the other, as a block and the model's end call them; gradients of everything."""
+    q = ops.qk_norm_rope(qkv, wq, wk, cos, sin, H, KV, hd, positions=positions)
+    x = ops.attention_documents(q, starts, H, KV, hd)
+    loss = ops.linear_cross_entropy(x, w, labels)
+    return (loss, *torch.autograd.grad(loss, (qkv, wq, wk, w)))
+
+
+def step_inputs(seed, B=2, S=300, H=4, KV=2, hd=64, V=1003):
+    g = gen(seed)
+    cos, sin = ops.rope_tables(S, hd, device=DEV)
+    starts = starts_of("docs", B, S, g)
+    labels = torch.randint(0, V, (B, S), generator=g, device=DEV)
+    labels[:, ::9] = -100
+    t = dict(qkv=normal(g, B, S, (H + 2 * KV) * hd), wq=normal(g, hd), wk=normal(g, hd), w=normal(g, V, H * hd, std=0.1))
+    return dict({k: v.requires_grad_() for k, v in t.items()}, starts=starts, positions=torch.arange(S, device=DEV, dtype=torch.int32) - starts,
+                cos=cos, sin=sin, labels=labels), (H, KV, hd)
+
+
+@pytest.mark.parametrize("H,KV,hd", [(4, 2, 64), (2, 1, 128)])
+def test_the_operators_together(H, KV, hd):
+    a, _ = step_inputs(31, H=H, KV=KV, hd=hd)
+    got = training_step(**a, H=H, KV=KV, hd=hd)
+    # the same in fp64 by the formulas that run where no kernel does
+    b = {k: v.detach().double().requires_grad_(v.requires_grad) if v.is_floating_point() else v for k, v in a.items()}
+    q = OD._qk_norm_rope_torch(b["qkv"], b["wq"], b["wk"], b["cos"], b["sin"], b["positions"], H, KV, hd, 1e-5)
+    x = OD._attention_documents_torch(q, b["starts"], H, KV, hd)
+    loss = OD._linear_cross_entropy_torch(x, b["w"], b["labels"].reshape(-1), 1.0, -100, "mean")
+    want = (loss, *torch.autograd.grad(loss, (b["qkv"], b["wq"], b["wk"], b["w"])))
+    torch.testing.assert_close(got[0].double(), want[0].double(), rtol=1e-3, atol=0)
+    # roundings on the way to a gradient: the rotated rows, the outputs, the weights and products of three operators, ten of U / 2 at most on
+    # average, added in squares
+    for x, y in zip(got[1:], want[1:]):
+        assert (x.double() - y.double()).norm() <= 10 ** 0.5 * U * y.double().norm()
+
+
+def test_captured_and_replayed():
+    a, (H, KV, hd) = step_inputs(41)
+    other, _ = step_inputs(42)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            training_step(**a, H=H, KV=KV, hd=hd)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for _ in range(2):                                         # two graphs with workspaces of their own
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(training_step(**a, H=H, KV=KV, hd=hd))
+    for data in (other, a, other):
+        with torch.no_grad():
+            for k, v in data.items():
+                a[k].copy_(v) if data is not a else None
+        want = training_step(**a, H=H, KV=KV, hd=hd)
+        for g in graphs + graphs:
+            g.replay()
+        for out in outs:
+            assert all(torch.equal(x, y) for x, y in zip(out, want))
+
+
+def test_two_streams_at_once():
+    a, (H, KV, hd) = step_inputs(51)
+    b, _ = step_inputs(52, S=411)
+    want = [training_step(**t, H=H, KV=KV, hd=hd) for t in (a, b)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [None, None]
+    for _ in range(5):
+        for i, (s, t) in enumerate(zip(streams, (a, b))):
+            with torch.cuda.stream(s):
+                got[i] = training_step(**t, H=H, KV=KV, hd=hd)
+        torch.cuda.synchronize()
+        for x, y in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(x, y))
+
+
+def test_offsets_beyond_32_bits():
+    """33 sequences of 8192 rows of 8192 columns: the last sequence as if it were alone."""
+    B, S, H, KV, hd = 33, 8192, 32, 16, 128
+    g = gen(61)
+    qkv = torch.empty(B, S, (H + 2 * KV) * hd, dtype=torch.bfloat16, device=DEV).normal_(generator=g).requires_grad_()
+    assert qkv.numel() > 2 ** 31
+    starts = starts_of("long", B, S, g)
+    wq, wk = (normal(g, hd).requires_grad_() for _ in range(2))
+    cos, sin = ops.rope_tables(S, hd, device=DEV)
+    dout = torch.empty(B, S, H * hd, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    rows = ops.qk_norm_rope(qkv, wq, wk, cos, sin, H, KV, hd)
+    out = ops.attention_documents(rows, starts, H, KV, hd)
+    (grad,) = torch.autograd.grad(out, qkv, dout)
+    last = qkv.detach()[-1:].clone().requires_grad_()
+    one = ops.attention_documents(ops.qk_norm_rope(last, wq, wk, cos, sin, H, KV, hd), starts[-1:], H, KV, hd)
+    (gone,) = torch.autograd.grad(one, last, dout[-1:])
+    assert torch.equal(out[-1:], one) and torch.equal(grad[-1:, :, :H * hd], gone[..., :H * hd])
+    # alone its groups' heads may be split over tiles, whose parts are added in fp32: another order
+    torch.testing.assert_close(grad[-1:].float(), gone.float(), rtol=2 * U, atol=2 * U * gone.float().abs().mean().item())
