@@ -1920,9 +1920,9 @@ TPLR_API int tplr_attention_docs_fwd(const void* qkv, const int* starts, void* o
 //
 // dK, dV: a tile is a key/value block of one kv head and the query heads of its group, or a part of them, and walks the query blocks
 // from the diagonal to the last that sees any of its keys.  Everything is transposed, with the key row as the TMEM lane:
-//   S^T = K Q^T, dP^T = V dO^T;  P^T and dS^T as packed bf16 over them;  dV += P^T dO, dK += dS^T Q
-// (at DH = 64 with two buffers for S^T; at 128 the accumulators leave no room)
-// with P^T and dS^T from tensor memory: neither goes through shared memory, whose traffic bounds the causal kernel above (4600 of its 5250
+//   S^T = K Q^T, dP^T = V dO^T;  P^T and dS^T as packed bf16, side by side over dP^T;  dV += P^T dO, dK += dS^T Q
+// S is free again as soon as the warps hold it, so the next step's is computed while this one's exponentials are taken.
+// P^T and dS^T are read from tensor memory: neither goes through shared memory, whose traffic bounds the causal kernel above (4600 of its 5250
 // cycles a step at DH = 128).  lse, delta and the starts belong to columns here: a warp of its own brings them to shared memory.
 //
 // Seven products instead of five, but each step is shorter, and there is no fp32 dQ to be zeroed, added into, read and rounded.
@@ -1942,7 +1942,7 @@ template <int DH> constexpr int docs_bwd_smem() { return docs_bwd_tiles<DH>() + 
 struct DocsBwdShared {
   uint64_t res_full, res_empty;                            // the tile's resident operands
   uint64_t ring_full[RING3], ring_empty[RING3], pair_full[2], pair_empty[2];
-  uint64_t s_full[2], dp_full, p_ready[2], ds_ready[2], acc_full, stat_full[2], stat_empty[2], tile_full[2], tile_empty[2];
+  uint64_t s_full[2], s_read, dp_full, p_ready[2], ds_ready[2], acc_full, stat_full[2], stat_empty[2], tile_full[2], tile_empty[2];
   uint32_t tmem_base;
   int abort;
   int2 tile[2];                                            // (tile or -1, blocks of its walk)
@@ -2009,7 +2009,7 @@ __device__ __forceinline__ void docs_bwd_init(DocsBwdShared& sh, int warp, int c
       // a barrier for even and one for odd steps: a warp may be a step ahead of another
       mbar_init(smem_u32(&sh.p_ready[s]), 8); mbar_init(smem_u32(&sh.ds_ready[s]), 8);
     }
-    mbar_init(smem_u32(&sh.dp_full), 1);
+    mbar_init(smem_u32(&sh.dp_full), 1); mbar_init(smem_u32(&sh.s_read), 8);
     mbar_init(smem_u32(&sh.acc_full), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -2156,7 +2156,7 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
     int n = 0;                                             // steps so far
     auto issue_s = [&](int step) -> bool {
       if (!mbar_wait_warp(smem_u32(&sh.ring_full[s3]), ph3, abort_flag)) return false;
-      if (step > 0 && !mbar_wait_warp(smem_u32(&sh.p_ready[(step - 1) & 1]), (uint32_t)(((step - 1) >> 1) & 1), abort_flag)) return false;      // every warp holds the last S
+      if (step > 0 && !mbar_wait_warp(smem_u32(&sh.s_read), (step - 1) & 1, abort_flag)) return false;      // every warp holds the last S
       tcgen05_fence_after();
       if (leader) {
         const uint32_t q = (uint32_t)s3 * (TILE_BYTES / 16);
@@ -2284,7 +2284,7 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         behind_wait32(v + 32);
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.p_ready[n & 1]));
+        if (lane == 0) mbar_arrive(smem_u32(&sh.s_read));
 #pragma unroll
         for (int e = 0; e < 64; e += 2) {
           float a0, a1;
@@ -2358,10 +2358,8 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
   grid_wait();
   grid_release();
   const uint32_t tmem_base = sh.tmem_base;
-  // S^T of even steps in columns 0..127; at DH = 64 of odd ones in 384..511, so that the next step's is computed ahead
-  constexpr bool AHEAD = DH == 64;
-  const uint32_t tdP = tmem_base + 128, tdV = tmem_base + 256, tdK = tmem_base + 256 + DH;
-  auto s_of = [&](int step) { return AHEAD ? tmem_base + (step & 1) * 384 : tmem_base; };
+  // S^T in columns 0..127; dP^T in 128..255, over which each warp writes its half of P^T and of dS^T, 32 columns each
+  const uint32_t tS = tmem_base, tdP = tmem_base + 128, tdV = tmem_base + 256, tdK = tmem_base + 384;
 
   if (warp == 0) {
     bool ok = true;
@@ -2432,14 +2430,15 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
     int s3 = 0, r3 = 0;                                    // ring places of the next S's and of the next dK's Q
     uint32_t ph3 = 0;
     int n = 0;                                             // steps so far
-    auto issue_s = [&](int step) -> bool {                 // S^T = K Q^T, behind the dV that reads P^T from its columns
+    auto issue_s = [&](int step) -> bool {                 // S^T = K Q^T
       if (!mbar_wait_warp(smem_u32(&sh.ring_full[s3]), ph3, abort_flag)) return false;
+      if (step > 0 && !mbar_wait_warp(smem_u32(&sh.s_read), (step - 1) & 1, abort_flag)) return false;       // every warp holds the last S
       tcgen05_fence_after();
       if (leader) {
-        const uint32_t q = (uint32_t)s3 * (TILE_BYTES / 16), d = s_of(step);
+        const uint32_t q = (uint32_t)s3 * (TILE_BYTES / 16);
 #pragma unroll
-        for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(d, kK, koff(kk), kQ, q + koff(kk), id_kk, kk > 0 ? 1u : 0u);
-        umma_commit(smem_u32(&sh.s_full[AHEAD ? step & 1 : 0]));
+        for (int kk = 0; kk < DH / 16; ++kk) umma_bf16_b(tS, kK, koff(kk), kQ, q + koff(kk), id_kk, kk > 0 ? 1u : 0u);
+        umma_commit(smem_u32(&sh.s_full[0]));
       }
       if (++s3 == RING3) { s3 = 0; ph3 ^= 1u; }
       return true;
@@ -2466,27 +2465,26 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         continue;
       }
       if (!(ok = issue_s(n))) break;
-      if (!(ok = issue_dp(n, n_it == 1))) break;           // behind the last dK, which reads dS^T from these columns
+      if (!(ok = issue_dp(n, n_it == 1))) break;           // behind the last dV and dK, which read P^T and dS^T from these columns
       for (int t = 0; t < n_it; ++t, ++n) {
-        if (AHEAD && t + 1 < n_it && !(ok = issue_s(n + 1))) break;
-        // P^T over S^T, read by every warp; in a tile's first step every warp has read the last tile's accumulators before
+        if (t + 1 < n_it && !(ok = issue_s(n + 1))) break;
+        // P^T over dP^T; in a tile's first step every warp has read the last tile's accumulators before
         if (!(ok = mbar_wait_warp(smem_u32(&sh.p_ready[n & 1]), (uint32_t)((n >> 1) & 1), abort_flag))) break;
         tcgen05_fence_after();
         if (leader) {
-          const uint32_t d = (uint32_t)(n & 1) * (TILE_BYTES / 16), tP = s_of(n);
+          const uint32_t d = (uint32_t)(n & 1) * (TILE_BYTES / 16);
 #pragma unroll
           for (int kk = 0; kk < BQ / 16; ++kk)             // dV[kv, d] += P^T[kv, q] dO[q, d]
-            umma_ts_bf16_b(tdV, tP + (kk >> 2) * 64 + 8 * (kk & 3), mdO, d + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
+            umma_ts_bf16_b(tdV, tdP + (kk >> 2) * 64 + 8 * (kk & 3), mdO, d + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
           umma_commit(smem_u32(&sh.pair_empty[n & 1]));    // dP(t) read dO(t) before
         }
-        if (!AHEAD && t + 1 < n_it && !(ok = issue_s(n + 1))) break;
-        if (!(ok = mbar_wait_warp(smem_u32(&sh.ds_ready[n & 1]), (uint32_t)((n >> 1) & 1), abort_flag))) break;      // dS^T over dP^T
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.ds_ready[n & 1]), (uint32_t)((n >> 1) & 1), abort_flag))) break;      // dS^T beside it
         tcgen05_fence_after();
         if (leader) {
           const uint32_t q = (uint32_t)r3 * (TILE_BYTES / 16);
 #pragma unroll
           for (int kk = 0; kk < BQ / 16; ++kk)             // dK[kv, d] += dS^T[kv, q] Q[q, d]
-            umma_ts_bf16_b(tdK, tdP + (kk >> 2) * 64 + 8 * (kk & 3), mQ, q + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
+            umma_ts_bf16_b(tdK, tdP + 32 + (kk >> 2) * 64 + 8 * (kk & 3), mQ, q + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
           umma_commit(smem_u32(&sh.ring_empty[r3]));
           if (t == n_it - 1) umma_commit(smem_u32(&sh.acc_full));
         }
@@ -2544,15 +2542,17 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         const bool diag = i == 0;
         if (++i == n_i) i = 0;
         if (!(ok = mbar_wait_warp(smem_u32(&sh.stat_full[n & 1]), (uint32_t)((n >> 1) & 1), abort_flag))) break;
-        if (!(ok = mbar_wait_warp(smem_u32(&sh.s_full[AHEAD ? n & 1 : 0]), (uint32_t)(AHEAD ? (n >> 1) & 1 : n & 1), abort_flag))) break;
+        if (!(ok = mbar_wait_warp(smem_u32(&sh.s_full[0]), n & 1, abort_flag))) break;
         tcgen05_fence_after();
-        const uint32_t tS = s_of(n);
         uint32_t v[64];                                    // P, in fp32 for dS
         tmem_ld32_nowait(tS + ch * 64 + lane_off, v);
         tmem_ld32_nowait(tS + ch * 64 + 32 + lane_off, v + 32);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         behind_wait32(v);
         behind_wait32(v + 32);
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.s_read));
 #pragma unroll
         for (int e = 0; e < 64; e += 4) {
           const float4 nl = *reinterpret_cast<const float4*>(st.nlse + ch * 64 + e);
@@ -2577,23 +2577,24 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
 #pragma unroll
           for (int e = 0; e < 64; ++e) if (ch * 64 + e < r) v[e] = 0u;
         }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) pk[e] = bf16x2_of(__uint_as_float(v[c * 32 + 2 * e]), __uint_as_float(v[c * 32 + 2 * e + 1]));
-          tmem_st16(tS + ch * 64 + c * 16 + lane_off, pk);
-        }
-        tmem_wait_st();
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.p_ready[n & 1]));
         if (!(ok = mbar_wait_warp(smem_u32(&sh.dp_full), n & 1, abort_flag))) break;
         tcgen05_fence_after();
+        // this warp's 64 columns of dP: P goes over the first 32, once they are held, dS over the others
+        uint32_t ds[32];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          uint32_t dp[32], pk[16];
+          uint32_t dp[32];
           tmem_ld32(tdP + ch * 64 + c * 32 + lane_off, dp);
+          if (c == 0) {
+            uint32_t pk[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) pk[e] = bf16x2_of(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+            tmem_st32(tdP + ch * 64 + lane_off, pk);
+            tmem_wait_st();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh.p_ready[n & 1]));
+          }
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
             const float4 nd = *reinterpret_cast<const float4*>(st.ndelta + ch * 64 + c * 32 + e);
@@ -2601,11 +2602,11 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
             float d0, d1, d2, d3;
             unpack_f32x2(mul_f32x2(pack_f32x2(w[0], w[1]), fma_f32x2(pack_f32x2(dp[e], dp[e + 1]), sc, pack_f32x2(__float_as_uint(nd.x), __float_as_uint(nd.y)))), d0, d1);
             unpack_f32x2(mul_f32x2(pack_f32x2(w[2], w[3]), fma_f32x2(pack_f32x2(dp[e + 2], dp[e + 3]), sc, pack_f32x2(__float_as_uint(nd.z), __float_as_uint(nd.w)))), d2, d3);
-            pk[e / 2] = bf16x2_of(d0, d1);
-            pk[e / 2 + 1] = bf16x2_of(d2, d3);
+            ds[c * 16 + e / 2] = bf16x2_of(d0, d1);
+            ds[c * 16 + e / 2 + 1] = bf16x2_of(d2, d3);
           }
-          tmem_st16(tdP + ch * 64 + c * 16 + lane_off, pk);
         }
+        tmem_st32(tdP + ch * 64 + 32 + lane_off, ds);
         tmem_wait_st();
         tcgen05_fence_before();
         __syncwarp();
