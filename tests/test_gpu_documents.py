@@ -137,6 +137,18 @@ def test_attention_documents_gives_the_same_bits_every_time(hd):
     assert all(torch.equal(x, y) for r in runs[1:] for x, y in zip(r, runs[0]))
 
 
+def test_attention_gradient_twice_and_of_a_sum():
+    """The same graph differentiated again, and with a gradient that has no memory of its own (an expanded number)."""
+    g = gen(14)
+    qkv = normal(g, 40, 260, 4 * 64).requires_grad_()          # 240 tiles: every CTA takes several
+    out = ops.attention_documents(qkv, starts_of("docs", 40, 260, g), 2, 1, 64)
+    one = torch.ones((), dtype=torch.bfloat16, device=DEV).expand_as(out)
+    first = torch.autograd.grad(out, qkv, one, retain_graph=True)[0]
+    second = torch.autograd.grad(out.sum(dtype=torch.float32), qkv, retain_graph=True)[0]
+    third = torch.autograd.grad(out, qkv, one.contiguous() * 2)[0]
+    assert torch.equal(first, second) and torch.equal(first * 2, third)
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 def test_packed_documents_are_the_documents_alone(hd):
     """Documents that begin at whole blocks meet the same tiles as in a sequence of their own, so their outputs have the same bits."""
@@ -433,6 +445,23 @@ def test_rows_that_count_for_nothing_may_hold_anything():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_loss_of_one_row_and_of_a_class_that_is_ignored():
+    g = gen(13)
+    x, w, labels = rows_and_labels(g, 50, 64, 129, ignored=0)
+    labels[::2] = 3
+    one = ops.linear_cross_entropy(x[1], w, labels[1])         # a row without a batch, a label without a dimension
+    assert one.shape == () and torch.equal(one, ops.linear_cross_entropy(x[1:2], w, labels[1:2]))
+    assert torch.equal(ops.linear_cross_entropy(x[1], w, labels[1], reduction="none"), one)
+    x.requires_grad_()
+    w.requires_grad_()
+    other = torch.where(labels == 3, -100, labels)
+    for reduction in ("mean", "none"):
+        a, b = ops.linear_cross_entropy(x, w, labels, ignore_index=3, reduction=reduction), ops.linear_cross_entropy(x, w, other, reduction=reduction)
+        assert torch.equal(a, b)
+        assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(a.sum(), (x, w)), torch.autograd.grad(b.sum(), (x, w))))
+    assert int(OF.status_word(DEV).item()) == 0
+
+
 def test_loss_takes_views():
     g = gen(12)
     x, w, labels = rows_and_labels(g, 90, 72, 333)
@@ -449,7 +478,8 @@ def training_step(qkv, starts, positions, wq, wk, cos, sin, w, labels, H, KV, hd
     q = ops.qk_norm_rope(qkv, wq, wk, cos, sin, H, KV, hd, positions=positions)
     x = ops.attention_documents(q, starts, H, KV, hd)
     loss = ops.linear_cross_entropy(x, w, labels)
-    return (loss, *torch.autograd.grad(loss, (qkv, wq, wk, w)))
+    grads = torch.autograd.grad(loss, (qkv, wq, wk, w))
+    return (loss.detach(), *grads)       # no graph of these leaves is left alive when another one is captured
 
 
 def step_inputs(seed, B=2, S=300, H=4, KV=2, hd=64, V=1003):
