@@ -69,14 +69,14 @@ int tplr_qk_norm_rope_parts(long long tokens, int n_q, int n_k, int hd);
 int tplr_qk_norm_rope_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* wq, const void* wk, const float* cosb,
                           const float* sinb, const int* pos, void* dx, float* part, void* dwq, void* dwk, float* add_q, float* add_k,
                           long long tokens, int S, int table_rows, int n_q, int n_k, int hd, float eps, unsigned int* status, void* stream);
-int tplr_gemm2_softmax_columns(int M, int N, int K);
+int tplr_gemm2_softmax_columns(int M, int N, int K, int store);
 int tplr_gemm2_softmax(const void* X, const void* W, void* P, const long long* labels, float* stats, float* target, int M, int N, int K,
                        long long ldx, long long ldw, long long ldp, unsigned int* status, void* stream);
 int tplr_gemm2_rows(const void* A, const void* B, void* C, float* ws, const float* row_scale, int M, int N, int K, long long lda,
                     long long ldb, long long ldc, unsigned int* status, void* stream);
 int tplr_vocab_count(const long long* labels, long long T, long long ignore, int V, int* n_valid, unsigned int* status, void* stream);
-int tplr_vocab_losses(const float* stats, const float* target, const long long* labels, float* losses, float* lse, long long T, int parts, int V,
-                      long long ignore, void* stream);
+int tplr_vocab_losses(const float* stats, const float* target, const long long* labels, float* losses, long long T, int parts, int V, long long ignore,
+                      void* stream);
 int tplr_vocab_rows(void* E, long long ld, const float* stats, const float* target, const long long* labels, const float* row_grad,
                     const int* n_valid, float grad_scale, const void* x, long long ldx, void* xs, long long ldxs, float* row_scale, float* losses, long long T,
                     int parts, int columns, int V, int D, long long ignore, void* stream);

@@ -43,10 +43,11 @@ constexpr int MAX_STAGES = 8;                      // narrower tiles have smalle
 static_assert(4 * 8192 <= STAGE_BYTES, "the freed stage holds four warps' second pair");
 // Warps that drain the accumulator: one a quadrant of tensor memory, or two where the epilogue is as long as the main loop of a short K,
 // so that one has instructions while the other waits.  What they stage beyond 32 KB takes a stage of the ring.
-constexpr int epi_warps(int epi) { return epi == 7 || epi == 8 || epi == 10 || epi == 12 || epi == 13 ? 8 : 4; }
+constexpr int epi_warps(int epi) { return epi == 7 || epi == 8 || epi == 10 || epi == 12 || epi == 13 || epi == 15 ? 8 : 4; }
 constexpr int num_threads(int epi) { return 64 + 32 * epi_warps(epi); }
 constexpr int ring_stages(int epi) { return epi == 5 || epi == 10 ? EPI5_STAGES : STAGES; }
 constexpr int MAX_RANKS = 8;
+constexpr int SOFTMAX_FEW = 128;                   // rows whose softmax without stored weights takes the transposed product
 constexpr int CHUNK_ROWS = 128;                    // gather / scatter flag granularity (rows)
 
 struct Gemm2Params {
@@ -96,7 +97,8 @@ struct Gemm2Params {
   float* q8_scale;
   long long q8_ld;
   // softmax over the columns in pieces (EPI 12, 13): a piece is half a tile's columns, sm_parts pieces a row; (reference, sum of
-  // exp(logit - it)) goes to sm_stats[row * sm_parts + piece], the logit of the row's label to sm_target[row]
+  // exp(logit - it)) goes to sm_stats[row * sm_parts + piece], the logit of the row's label to sm_target[row].  EPI 15 has the
+  // product transposed: rows are the softmax's columns here, a piece 32 of them
   const long long* sm_labels;
   float2* sm_stats;
   float* sm_target;
@@ -1023,12 +1025,62 @@ __device__ __forceinline__ void epilogue_softmax(const Gemm2Params& p, uint32_t 
   }
 }
 
+// The same for a few tokens (EPI 15), whose product is made the other way round, rows of the weight along the tile's 256: a lane has a column
+// of the softmax, a piece is the 32 of a warp.  The largest of a token's 32 logits is one reduction of the warp over their bits in
+// the order of their values, the sums of 16 tokens meet in 16 shuffles, each lane keeping half of what it held.  A tile takes the tokens
+// there are in place of 256, so the weight's bytes bound it: 30 x 768 x 32000, cold, 17.0 us against 22.6 with tokens along the
+// tile, 128 x 2048 x 32000 36.2 and 38.5, 30 x 4096 x 128256 174 and 190 (6.0 TB/s); 128 x 768 x 32000 is even, at 21.9 and 19.8, and
+// above 128 tokens there is nothing to gain.
+__device__ __forceinline__ void epilogue_softmax_few(const Gemm2Params& p, uint32_t tmem_acc, int quad, int turn, int lane, int m0) {
+  const int half = p.tile_n / 2;                     // tokens of a warp
+  const int row0 = m0 + quad * 32;
+  if (row0 >= p.M) return;                           // warp-uniform
+  const uint32_t acc = tmem_acc + ((uint32_t)(quad * 32) << 16);
+  const bool live = row0 + lane < p.M;
+  constexpr float LOG2E = 1.4426950408889634f;
+#pragma unroll 1
+  for (int c = turn * half; c < (turn + 1) * half && c < p.N; c += 16) {
+    uint32_t r[16];
+    float v[16], my_ref = 0.f;
+    tmem_ld16(acc + c, r);
+    const int token = c + (lane & 15);               // whose numbers this lane stores
+    const long long label = token < p.N ? p.sm_labels[token] - row0 : -1;
+    const int mine = label >= 0 && label < min(32, p.M - row0) ? (int)label : -1;
+    for (unsigned hits = __ballot_sync(0xffffffffu, mine >= 0) & 0xffffu; hits; hits &= hits - 1) {
+      const int t = __ffs(hits) - 1;
+      if (__shfl_sync(0xffffffffu, mine, t) != lane) continue;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) if (e == t) p.sm_target[c + e] = __uint_as_float(r[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      if (!live) r[e] = 0xff800000u;
+      const int bits = (int)r[e];
+      const int key = __reduce_max_sync(0xffffffffu, bits >= 0 ? bits : bits ^ 0x7fffffff);
+      const float top = __int_as_float(key >= 0 ? key : key ^ 0x7fffffff);
+      const float ref = fabsf(top) <= SM_NEAR || top == -INFINITY ? 0.f : top;
+      if ((lane & 15) == e) my_ref = ref;
+      v[e] = live ? ex2(fmaf(__uint_as_float(r[e]), LOG2E, -ref * LOG2E)) : 0.f;
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+#pragma unroll
+      for (int e = 0; e < o; ++e) {
+        const float give = lane & o ? v[e] : v[e + o], keep = lane & o ? v[e + o] : v[e];
+        v[e] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+      }
+    }
+    v[0] += __shfl_xor_sync(0xffffffffu, v[0], 16);
+    if (lane < 16 && token < p.N) p.sm_stats[(long long)token * p.sm_parts + (row0 >> 5)] = make_float2(my_ref, v[0]);
+  }
+}
+
 // EPI: 0 store bf16, 1 fp32 accumulate (C += acc), 2 store fp32, 3 fused SwiGLU of a packed [w1; w3] projection,
 // 4 store bf16 with the rotary embedding applied to the leading columns, 5 backward of the SwiGLU on the data gradient
 // of the down projection, 6 data gradient of the attention output projection with the attention backward's delta term,
 // 7 / 8 product of 8-bit rows stored as bf16 / fp32, 9 as 3 with the projection kept in 8 bits, 10 as 5 from it,
 // 11 product of 8-bit rows, int32 sums of a part of K to a plane of its own, 12 softmax over the columns in pieces, 13 their numbers alone,
-// 14 as 0 with a factor for each row
+// 14 as 0 with a factor for each row, 15 the numbers of 13 from the transposed product of a few rows
 template <bool A_MN, bool B_MN, int EPI>
 __global__ void __launch_bounds__(num_threads(EPI), 1)
 gemm2_kernel(const __grid_constant__ Gemm2Params p) {
@@ -1233,6 +1285,7 @@ gemm2_kernel(const __grid_constant__ Gemm2Params p) {
           epilogue_rope<64>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes);
         else if (EPI == 11) epilogue_tma<2>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes, w.t % p.k_splits);
         else if (EPI == 12 || EPI == 13) epilogue_softmax<EPI == 12>(p, tmem_acc, quad, turn, lane, m0, n0, sEpi + (uint32_t)(warp - 2) * 4096u, n_boxes);
+        else if (EPI == 15) epilogue_softmax_few(p, tmem_acc, quad, turn, lane, m0);
         else if (I8)       epilogue_q8<EPI == 8>(p, tmem_acc, quad, turn, lane, m0, n0, sEpi + (uint32_t)(warp - 2) * 4096u, n_boxes);
         else if (p.c_tma)  epilogue_tma<EPI>(p, tmem_acc, quad, lane, m0, n0, sEpi + (uint32_t)quad * 8192u, n_boxes, w.t % p.k_splits);
         else               epilogue_direct<EPI>(p, tmem_acc, quad, lane, m0, n0);
@@ -1336,7 +1389,7 @@ int launch2(Gemm2Params& p, int n_comm_pairs, int max_pairs, cudaStream_t st) {
   attr[1] = pdl_attr(p.world == 1);
   cfg.attrs = attr; cfg.numAttrs = 2;
   // all CTAs must be resident at once: compute CTAs wait for comm CTAs of the same launch
-  static int max_clusters[2][2][15] = {};
+  static int max_clusters[2][2][16] = {};
   int& mc = max_clusters[A_MN][B_MN][EPI];
   if (mc == 0) {
     cfg.gridDim = dim3(2 * (tplr_sm_count() / 2));
@@ -1367,7 +1420,7 @@ int dispatch2(Gemm2Params& p, int a_mn, int b_mn, int epi, int n_comm_pairs, int
   TPLR_GEMM2_CASE(1, 0, 0) TPLR_GEMM2_CASE(1, 0, 1) TPLR_GEMM2_CASE(1, 0, 2)
   TPLR_GEMM2_CASE(0, 0, 3) TPLR_GEMM2_CASE(0, 0, 4) TPLR_GEMM2_CASE(0, 1, 5) TPLR_GEMM2_CASE(0, 1, 6)
   TPLR_GEMM2_CASE(0, 0, 7) TPLR_GEMM2_CASE(0, 0, 8) TPLR_GEMM2_CASE(0, 0, 9) TPLR_GEMM2_CASE(0, 1, 10) TPLR_GEMM2_CASE(0, 0, 11)
-  TPLR_GEMM2_CASE(0, 0, 12) TPLR_GEMM2_CASE(0, 0, 13) TPLR_GEMM2_CASE(0, 1, 14)
+  TPLR_GEMM2_CASE(0, 0, 12) TPLR_GEMM2_CASE(0, 0, 13) TPLR_GEMM2_CASE(0, 1, 14) TPLR_GEMM2_CASE(0, 0, 15)
 #undef TPLR_GEMM2_CASE
   return -104;
 }
@@ -1818,9 +1871,13 @@ TPLR_API int tplr_gemm2_rope(const void* X, const void* W, void* QKV, int M, int
   return dispatch2(p, 0, 0, 4, 0, 0, (cudaStream_t)stream);
 }
 
-// Columns of a piece of tplr_gemm2_softmax for these sizes: a row has ceil(N / columns) pieces.
+// Columns of a piece of tplr_gemm2_softmax for these sizes, P given or not: a row has ceil(N / columns) pieces, 64 columns or more in all but
+// the products of up to SOFTMAX_FEW rows without P.
 static int softmax_tile(int M, int N, int K) { return pick_tile(M, N, K, false, false, 0, 1, 128); }
-TPLR_API int tplr_gemm2_softmax_columns(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? softmax_tile(M, N, K) / 2 : 128; }
+TPLR_API int tplr_gemm2_softmax_columns(int M, int N, int K, int store) {
+  if (M <= 0 || N <= 0 || K <= 0) return 128;
+  return !store && M <= SOFTMAX_FEW ? 32 : softmax_tile(M, N, K) / 2;
+}
 
 // The product Z = X W^T (X [M, K], W [N, K] bf16, K-major) with the softmax over its columns in pieces of tplr_gemm2_softmax_columns
 // columns (see epilogue_softmax); Z itself is not stored.  stats [M, pieces] pairs (reference, sum of exp(Z - it)), target [M] the logit of
@@ -1832,11 +1889,14 @@ TPLR_API int tplr_gemm2_softmax(const void* X, const void* W, void* P, const lon
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   if (((uintptr_t)P & 15) || (ldp % 8) || ((uintptr_t)stats & 7) || (P && ldp < N)) return -101;
   Gemm2Params p = {};
-  const int tile_n = softmax_tile(M, N, K);
-  if (int r = fill_common(p, X, W, P, M, N, K, ldx, ldw, P ? ldp : 8, 0, 0, 0, status, tile_n)) return r;
+  const bool few = !P && M <= SOFTMAX_FEW;
+  const int tile_n = few ? (M + 31) / 32 * 32 : softmax_tile(M, N, K), columns = few ? 32 : tile_n / 2;
+  if (int r = few ? fill_common(p, W, X, nullptr, N, M, K, ldw, ldx, 8, 0, 0, 0, status, tile_n)
+                  : fill_common(p, X, W, P, M, N, K, ldx, ldw, P ? ldp : 8, 0, 0, 0, status, tile_n))
+    return r;
   p.sm_labels = labels; p.sm_stats = reinterpret_cast<float2*>(stats); p.sm_target = target;
-  p.sm_parts = (N + tile_n / 2 - 1) / (tile_n / 2);
-  return dispatch2(p, 0, 0, P ? 12 : 13, 0, 0, (cudaStream_t)stream);
+  p.sm_parts = (N + columns - 1) / columns;
+  return dispatch2(p, 0, 0, few ? 15 : P ? 12 : 13, 0, 0, (cudaStream_t)stream);
 }
 
 // int32 elements of the workspace that tplr_gemm2_q8 takes for this size (0: none).

@@ -36,31 +36,47 @@ __global__ void __launch_bounds__(1024) vocab_count_kernel(const long long* labe
   if (threadIdx.x == 0) out[0] = total;
 }
 
-// Loss of each row, a warp a row.
+// Loss of each row: a warp a row, or (WIDE) its block of eight, where there are no more rows than SMs: 30 rows of 1000 pieces, product
+// and this, 20.6 us with a warp a row, 16.1 with a block.
+template <bool WIDE>
 __global__ void __launch_bounds__(256) vocab_losses_kernel(const float2* stats, const float* target, const long long* labels, float* losses,
-                                                           float* lse_out, long long T, int parts, int V, long long ignore) {
+                                                           long long T, int parts, int V, long long ignore) {
+  __shared__ float red[2][8];
   grid_wait();
   grid_release();
-  const long long row = blockIdx.x * 8LL + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row = WIDE ? (long long)blockIdx.x : blockIdx.x * 8LL + warp;
   if (row >= T) return;
+  const int first = WIDE ? (int)threadIdx.x : lane, step = WIDE ? 256 : 32;
   const long long label = labels[row];
   const bool counts = label != ignore && label >= 0 && label < V;
-  float loss = 0.f, lse = 0.f;
-  if (counts) {                                      // the same in all lanes
+  float loss = 0.f;
+  if (counts) {                                      // the same in all lanes, and all of a block's threads where it has one row
     const float2* st = stats + row * parts;
     float m = -INFINITY;
-    for (int i = lane; i < parts; i += 32) m = fmaxf(m, st[i].x);
+#pragma unroll 4
+    for (int i = first; i < parts; i += step) m = fmaxf(m, st[i].x);
     m = warp_max(m);
+    if (WIDE) {
+      if (lane == 0) red[0][warp] = m;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = fmaxf(m, red[0][i]);
+    }
     float s = 0.f;
-    for (int i = lane; i < parts; i += 32) { const float2 v = st[i]; s += v.y * __expf(v.x - m); }
-    lse = m + logf(warp_sum(s));
-    loss = lse - target[row];
+#pragma unroll 4
+    for (int i = first; i < parts; i += step) { const float2 v = st[i]; s += v.y * __expf(v.x - m); }
+    s = warp_sum(s);
+    if (WIDE) {
+      if (lane == 0) red[1][warp] = s;
+      __syncthreads();
+      s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += red[1][i];
+    }
+    loss = m + logf(s) - target[row];
   }
-  if (lane == 0) {
-    losses[row] = loss;
-    if (lse_out) lse_out[row] = lse;
-  }
+  if (WIDE ? threadIdx.x == 0 : lane == 0) losses[row] = loss;
 }
 
 // What both products need of a row (see above), a warp a row: f in row_scale, E in place of e, f x in xs; and the
@@ -195,13 +211,14 @@ TPLR_API int tplr_vocab_count(const long long* labels, long long T, long long ig
   return (int)launch_pdl(vocab_count_kernel, 1, 1024, 0, (cudaStream_t)stream, labels, T, ignore, V, n_valid, status);
 }
 
-// losses [T] (and, if given, lse [T]) from tplr_gemm2_softmax's stats [T, parts] and target [T]
-TPLR_API int tplr_vocab_losses(const float* stats, const float* target, const long long* labels, float* losses, float* lse, long long T,
-                               int parts, int V, long long ignore, void* stream) {
+// losses [T] from tplr_gemm2_softmax's stats [T, parts] and target [T]
+TPLR_API int tplr_vocab_losses(const float* stats, const float* target, const long long* labels, float* losses, long long T, int parts, int V,
+                               long long ignore, void* stream) {
   TPLR_ENTER();
   if (T <= 0) return 0;
-  return (int)launch_pdl(vocab_losses_kernel, (unsigned)((T + 7) / 8), 256, 0, (cudaStream_t)stream, reinterpret_cast<const float2*>(stats), target,
-                         labels, losses, lse, T, parts, V, ignore);
+  const bool wide = T <= tplr_sm_count();
+  return (int)launch_pdl(wide ? vocab_losses_kernel<true> : vocab_losses_kernel<false>, (unsigned)(wide ? T : (T + 7) / 8), 256, 0, (cudaStream_t)stream,
+                         reinterpret_cast<const float2*>(stats), target, labels, losses, T, parts, V, ignore);
 }
 
 // What tplr_gemm2_softmax left of T rows, E [T, V] (rows of ld elements), made ready for the products of the gradients: dx = row_scale * (E w),
@@ -224,16 +241,15 @@ TPLR_API int tplr_vocab_mean(const float* losses, long long T, const int* n_vali
   return (int)launch_pdl(vocab_mean_kernel, 1, 1024, 0, (cudaStream_t)stream, losses, T, n_valid, loss);
 }
 
-// y = x * by[0] for n (a multiple of 8) values, dense, on 16-byte boundaries: x bf16 or fp32, y bf16, or fp32 that is added onto
+// y = x * by[0] for n (a multiple of 8) values, dense, on 16-byte boundaries: x bf16 or fp32, y bf16; or, of fp32 alone, y fp32 that is added onto
 TPLR_API int tplr_vocab_scale(const void* x, int x_fp32, const float* by, void* y, int add_fp32, long long n, void* stream) {
   TPLR_ENTER();
   if (n <= 0) return 0;
-  if ((n % 8) || (((uintptr_t)x | (uintptr_t)y) & 15)) return -401;
+  if ((n % 8) || (((uintptr_t)x | (uintptr_t)y) & 15) || (add_fp32 && !x_fp32)) return -401;
   const long long blocks = (n / 8 + 255) / 256, most = 8LL * tplr_sm_count();
   const unsigned grid = (unsigned)(blocks < most ? blocks : most);
   cudaStream_t st = (cudaStream_t)stream;
-  if (x_fp32 && add_fp32) return (int)launch_pdl(vocab_scale_kernel<float, true>, grid, 256, 0, st, (const float*)x, by, y, n / 8);
+  if (add_fp32) return (int)launch_pdl(vocab_scale_kernel<float, true>, grid, 256, 0, st, (const float*)x, by, y, n / 8);
   if (x_fp32) return (int)launch_pdl(vocab_scale_kernel<float, false>, grid, 256, 0, st, (const float*)x, by, y, n / 8);
-  if (add_fp32) return (int)launch_pdl(vocab_scale_kernel<bf16, true>, grid, 256, 0, st, (const bf16*)x, by, y, n / 8);
   return (int)launch_pdl(vocab_scale_kernel<bf16, false>, grid, 256, 0, st, (const bf16*)x, by, y, n / 8);
 }

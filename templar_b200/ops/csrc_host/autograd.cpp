@@ -740,7 +740,8 @@ struct Pieces {
   ll V, D, ld, ldxs;                                   // rows on 128-byte boundaries, as the products' copies take them best
   Pieces(const Tensor& x, const Tensor& w, ll rows, bool store, bool scaled)
       : V(w.size(0)), D(w.size(1)), ld((w.size(0) + 63) / 64 * 64), ldxs((w.size(1) + 63) / 64 * 64) {
-    const ll per = (V + 63) / 64 * 2;                  // pieces of 64 columns or more
+    // pieces of 64 columns or more, or fewer tokens with smaller ones, the last run's too
+    const ll least = std::min(64, E.softmax_columns((int)rows, (int)V, (int)D, store)), per = (V + least - 1) / least * 2;
     numbers = f32({rows * (per + 2)}, x);
     stats = numbers.data_ptr<float>();
     target = stats + rows * per;
@@ -752,7 +753,7 @@ struct Pieces {
   ll run(const Tensor& x, ll T, const Tensor& w, const void* from, const ll* labels, const Tensor& status) {
     check(E.softmax(from, w.data_ptr(), ptr(e), labels, stats, target, (int)T, (int)V, (int)D, x.stride(0), w.stride(0), ld, word(status), stream()),
           "gemm2_softmax");
-    return E.softmax_columns((int)T, (int)V, (int)D);
+    return E.softmax_columns((int)T, (int)V, (int)D, e.defined());
   }
 };
 const char* row_of(const Tensor& x, ll at) { return static_cast<const char*>(x.data_ptr()) + 2 * at * x.stride(0); }
@@ -764,8 +765,7 @@ Tensor token_losses(const Tensor& x, const Tensor& w, const Tensor& labels, int6
   const ll* lab = reinterpret_cast<const ll*>(labels.data_ptr<int64_t>());
   for (ll a = 0; a < T; a += run) {
     const ll n = std::min(run, T - a), columns = ws.run(x, n, w, row_of(x, a), lab + a, status);
-    check(E.vocab_losses(ws.stats, ws.target, lab + a, losses.data_ptr<float>() + a, nullptr, n, (int)((V + columns - 1) / columns), (int)V, ignore,
-                         stream()),
+    check(E.vocab_losses(ws.stats, ws.target, lab + a, losses.data_ptr<float>() + a, n, (int)((V + columns - 1) / columns), (int)V, ignore, stream()),
           "vocab_losses");
   }
   return losses;

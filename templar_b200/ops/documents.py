@@ -293,14 +293,16 @@ class _Pieces:
         # elements, 105 with 50304, dw 107 and 92
         self.ld, self.ldxs = (-(-n // 64) * 64 for n in w.shape)
         self.e = torch.empty(rows, self.ld, dtype=torch.bfloat16, device=dev) if store else None
-        self.stats = torch.empty(rows * -(-self.V // 64) * 2, dtype=torch.float32, device=dev)      # pieces of 64 columns or more
+        # pieces of 64 columns or more, or fewer tokens with smaller ones, the last run's too
+        least = min(64, native.lib().tplr_gemm2_softmax_columns(rows, self.V, self.D, int(store)))
+        self.stats = torch.empty(rows * -(-self.V // least) * 2, dtype=torch.float32, device=dev)
         self.target = torch.empty(rows, dtype=torch.float32, device=dev)
         self.scale = torch.empty(rows, dtype=torch.float32, device=dev) if store else None
         self.xs = torch.empty(rows, self.ldxs, dtype=torch.bfloat16, device=dev) if scaled_rows else None
 
     def run(self, x, w, labels) -> tuple[int, int]:
         """(pieces of a row, columns of a piece)"""
-        columns = native.lib().tplr_gemm2_softmax_columns(x.shape[0], self.V, self.D)
+        columns = native.lib().tplr_gemm2_softmax_columns(x.shape[0], self.V, self.D, int(self.e is not None))
         native.check(native.lib().tplr_gemm2_softmax(
             x.data_ptr(), w.data_ptr(), native.ptr(self.e), labels.data_ptr(), self.stats.data_ptr(), self.target.data_ptr(), x.shape[0], self.V,
             self.D, x.stride(0), w.stride(0), self.ld, OF.status_word(x.device).data_ptr(), native.stream_ptr()), "gemm2_softmax")
@@ -308,16 +310,16 @@ class _Pieces:
 
 
 def _token_losses(x2, w, labels, ignore_index):
-    """(losses, log of the sums) of every token, fp32."""
+    """Every token's loss, fp32."""
     T, V = x2.shape[0], w.shape[0]
-    losses, lse = (torch.empty(T, dtype=torch.float32, device=x2.device) for _ in range(2))
-    runs = _chunks(T, 16 * -(-V // 128))             # 8 bytes a piece of 64 columns or more
+    losses = torch.empty(T, dtype=torch.float32, device=x2.device)
+    runs = _chunks(T, 16 * -(-V // 128))             # 8 bytes a piece
     ws = _Pieces(x2, w, runs[0][1], False)
     for a, b in runs:
         parts, _ = ws.run(x2[a:b], w, labels[a:b])
         native.check(native.lib().tplr_vocab_losses(ws.stats.data_ptr(), ws.target.data_ptr(), labels[a:].data_ptr(), losses[a:].data_ptr(),
-                                                    lse[a:].data_ptr(), b - a, parts, V, ignore_index, native.stream_ptr()), "vocab_losses")
-    return losses, lse
+                                                    b - a, parts, V, ignore_index, native.stream_ptr()), "vocab_losses")
+    return losses
 
 
 def _gradients(x2, w, labels, ignore_index, row_grad, n_valid, grad_scale, losses, want_x, want_w, keep32):
@@ -405,7 +407,7 @@ class _LinearTokenLosses(torch.autograd.Function):
     def forward(ctx, x, w, labels, grad_scale, ignore_index, main_grad):
         x2, wd = _operand(x.reshape(-1, x.shape[-1])), _operand(w)
         with _on(x2):
-            losses, _ = _token_losses(x2, wd, labels, ignore_index)
+            losses = _token_losses(x2, wd, labels, ignore_index)
         ctx.save_for_backward(x2, wd, labels)
         ctx.cfg = (x.shape, grad_scale, ignore_index, main_grad)
         return losses
@@ -486,7 +488,7 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
         return out if mean else out.view(labels.shape)
     x2, wd = _operand(x.detach().reshape(-1, x.shape[-1])), _operand(w.detach())
     with _on(x2):
-        losses, _ = _token_losses(x2, wd, flat, ignore_index)
+        losses = _token_losses(x2, wd, flat, ignore_index)
         if reduction == "none":
             return losses.view(labels.shape)
         n_valid = torch.empty(1, dtype=torch.int32, device=x2.device)

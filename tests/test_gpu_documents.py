@@ -430,6 +430,40 @@ def test_loss_of_logits_far_from_zero(shift, some):
     check_loss(x, w, labels)
 
 
+@pytest.mark.parametrize("shift", [0.0, 95.0, -95.0])
+@pytest.mark.parametrize("T,D,V", [(1, 8, 1), (1, 2048, 257), (2, 72, 31), (15, 64, 33), (17, 200, 32000), (33, 768, 255), (64, 128, 512), (97, 1000, 50257),
+                                   (127, 64, 4097), (128, 264, 20000)])
+def test_losses_of_few_tokens(T, D, V, shift):
+    """Scoring without a gradient: up to 128 tokens take the product with the weight's rows along the tile."""
+    g = gen(3 * T + V)
+    x, w, labels = rows_and_labels(g, T, D, V)
+    if T > 2:
+        labels[0], labels[1], labels[2] = V - 1, 0, -100
+    x[:, 0] = 10
+    w[:, 0] = torch.where(torch.arange(V, device=DEV) // 40 % 3 == 1, shift / 10, 0.0)        # pieces of several references in a row
+    (want, el), *_ = loss64(x, w, labels)
+    each = ops.linear_cross_entropy(x, w, labels, reduction="none")
+    close(each, want, el, "losses")
+    assert torch.equal(each, ops.linear_cross_entropy(x.clone(), w, labels, reduction="none"))
+    if T > 2:
+        x[2] = float("nan")                                    # a token that does not count, and whose neighbours do
+        assert torch.equal(each, ops.linear_cross_entropy(x, w, labels, reduction="none"))
+        x[1] = float("nan")
+        got = ops.linear_cross_entropy(x, w, labels, reduction="none")
+        assert got[1].isnan() and torch.equal(got[2:], each[2:]) and torch.equal(got[:1], each[:1])
+    assert int(OF.status_word(DEV).item()) == 0
+
+
+def test_losses_in_runs_of_which_the_last_is_short(monkeypatch):
+    g = gen(31)
+    x, w, labels = rows_and_labels(g, 600, 64, 700)
+    want = ops.linear_cross_entropy(x, w, labels, reduction="none")
+    monkeypatch.setattr(OD, "CHUNK_BYTES", 1)                  # runs of 256, 256 and 88
+    got = ops.linear_cross_entropy(x, w, labels, reduction="none")
+    (_, el), *_ = loss64(x, w, labels)
+    close(got, want.double(), 2 * el, "losses")
+
+
 def test_rows_that_count_for_nothing_may_hold_anything():
     g = gen(22)
     x, w, labels = rows_and_labels(g, 140, 64, 900)
