@@ -1934,7 +1934,7 @@ template <int DH> constexpr int docs_bwd_smem() { return docs_bwd_tiles<DH>() + 
 struct DocsBwdShared {
   uint64_t res_full, res_empty;                            // the tile's resident operands
   uint64_t ring_full[RING3], ring_empty[RING3], pair_full[2], pair_empty[2];
-  uint64_t s_full[2], s_read, dp_full, p_ready[2], ds_ready[2], acc_full, stat_full[2], stat_empty[2], tile_full[2], tile_empty[2];
+  uint64_t s_full[2], s_read, dp_full, p_ready[2], ds_ready[2], acc_full, dv_full, stat_full[2], stat_empty[2], tile_full[2], tile_empty[2];
   uint32_t tmem_base;
   int abort;
   int2 tile[2];                                            // (tile or -1, blocks of its walk)
@@ -1976,17 +1976,35 @@ __device__ __forceinline__ void store_sector(void* to, const uint32_t* w) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
                "r"(w[6]), "r"(w[7]) : "memory");
 }
-// 32 accumulator columns of this lane's row -> 64 bytes of bf16
-__device__ __forceinline__ void store_row32(__nv_bfloat16* to, uint32_t tmem, bool zero, bool live) {
-  uint32_t v[32];
-  tmem_ld32(tmem, v);
+// NS sectors of this lane's row -> memory, the lanes of a group of NS a row at a time: a store touches 32 / NS rows and whole runs of them.
+// They swap sectors first, so that lane i holds the i-th of every row.  `first`: the group's first row, `live` its rows that are there.
+template <int NS>
+__device__ __forceinline__ void store_rows(void* first, long long pitch, uint32_t (&w)[8 * NS], int lane, int live) {
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    uint32_t w[8];
+  for (int o = NS / 2; o > 0; o >>= 1) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = zero ? 0u : bf16x2_of(__uint_as_float(v[16 * q + 2 * e]), __uint_as_float(v[16 * q + 2 * e + 1]));
-    if (live) store_sector(to + 16 * q, w);
+    for (int q = 0; q < 8 * NS; ++q) {
+      if (q / 8 & o) continue;
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, lane & o ? w[q] : w[q + 8 * o], o);
+      if (lane & o) w[q] = got; else w[q + 8 * o] = got;
+    }
   }
+  char* to = static_cast<char*>(first) + (lane & (NS - 1)) * 32;
+#pragma unroll
+  for (int q = 0; q < NS; ++q) if (q < live) store_sector(to + q * pitch, w + 8 * q);
+}
+// half a row of an accumulator, DH / 2 columns, as bf16
+template <int DH>
+__device__ __forceinline__ void store_half(void* first, long long pitch, uint32_t tmem, bool zero, int lane, int live) {
+  uint32_t w[DH / 4];
+#pragma unroll
+  for (int c = 0; c < DH / 64; ++c) {
+    uint32_t v[32];
+    tmem_ld32(tmem + c * 32, v);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) w[16 * c + e] = zero ? 0u : bf16x2_of(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+  }
+  store_rows<DH / 32>(first, pitch, w, lane, live);
 }
 __device__ __forceinline__ void docs_bwd_init(DocsBwdShared& sh, int warp, int consumers) {
   if (threadIdx.x == 0) {
@@ -2002,7 +2020,7 @@ __device__ __forceinline__ void docs_bwd_init(DocsBwdShared& sh, int warp, int c
       mbar_init(smem_u32(&sh.p_ready[s]), 8); mbar_init(smem_u32(&sh.ds_ready[s]), 8);
     }
     mbar_init(smem_u32(&sh.dp_full), 1); mbar_init(smem_u32(&sh.s_read), 8);
-    mbar_init(smem_u32(&sh.acc_full), 1);
+    mbar_init(smem_u32(&sh.acc_full), 1); mbar_init(smem_u32(&sh.dv_full), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -2172,6 +2190,8 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       }
       return true;
     };
+    // one loop over all tiles' steps, so that each product is issued from one place: a step's S and dP go ahead of the dQ of the step in
+    // front, the next tile's ahead of the last one's
     bool ok = true;
     int tile, nb;
     for (int k = 0; ok && take_tile(sh, k, lane, abort_flag, tile, nb); ++k) {
@@ -2205,7 +2225,7 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
     const unsigned long long sl2 = two(p.scale_log2), sc = two(p.scale);
     int n = 0, n_acc = 0;                                  // steps and tiles with a step so far
     bool ok = true;
-    // the k-th tile and this thread's row of it: asked for before the tile in front of it is finished, so that they are there in time
+    // the k-th tile and this thread's row of it: asked for before the tile in front of it is finished
     int tile, nb, qi, h, b, row, start;                    // start INT_MAX: the row sees nothing, or is past the end
     long long at;
     float lse2;
@@ -2220,7 +2240,7 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
 #pragma unroll
       for (int q = 0; q < DH / 16; ++q) o[q] = make_uint4(0u, 0u, 0u, 0u);
       if (row < p.S) {
-        start = max(p.starts[(long long)b * p.S + row], 0);
+        start = p.starts[(long long)b * p.S + row];
         lse2 = p.lse[at];                                  // infinite where the row sees nothing, whose output is zero
         const uint4* orow = reinterpret_cast<const uint4*>(p.out + ((long long)b * p.S + row) * ((long long)p.H * DH) + h * DH + ch * (DH / 2));
 #pragma unroll
@@ -2228,14 +2248,27 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       }
       return true;
     };
+    // dQ of the tile begun last -> bf16 -> the query columns of the gradient
+    __nv_bfloat16* to = nullptr;                           // the first row of this lane's group of DH / 32, and how many of its rows are there
+    int live = 0;
+    bool none = false;
+    auto finish = [&]() -> bool {
+      bool done = none || mbar_wait_warp(smem_u32(&sh.acc_full), (uint32_t)(n_acc & 1), abort_flag);
+      n_acc += !none;
+      if (!(done = pair_agrees(done, quad))) return false;
+      tcgen05_fence_after();
+      store_half<DH>(to, 2LL * C, tdQ + ch * (DH / 2) + lane_off, none, lane, live);
+      tcgen05_fence_before();                              // the next tile's first dQ is behind this warp's next dS
+      return true;
+    };
+    int last = -1;                                         // the tile whose dQ is not stored yet
     bool more = take(0);
     for (int k = 0;; ++k) {
       // both warps of a pair leave the loop together: they join their answers wherever one could leave alone
       if (!pair_agrees(more, quad)) break;
+      start = max(start, 0);
       if (start > row) start = INT_MAX;
       lse2 *= 1.4426950408889634f;
-      __nv_bfloat16* const to = p.dqkv + ((long long)b * p.S + row) * C + h * DH + ch * (DH / 2);
-      const bool live = row < p.S;
       ok = mbar_wait_warp(smem_u32(&sh.res_full), (uint32_t)(k & 1), abort_flag);
       float delta = 0.f;
       if (ok) {
@@ -2253,13 +2286,18 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
             delta = fmaf(__uint_as_float(ow[e] & 0xffff0000u), __uint_as_float(d[e] & 0xffff0000u), delta);
           }
         }
-        sh.part[ch][r] = delta;                            // read by the partner in front of the joint barrier at the tile's end
+        sh.part[ch][r] = delta;                            // read by the partner in front of the joint barrier before the next tile
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.res_empty));
       }
       if (!(ok = pair_agrees(ok, quad))) break;
       delta = start == INT_MAX ? 0.f : sh.part[0][r] + sh.part[1][r];
-      if (ch == 0 && live) p.delta[at] = delta;
+      if (ch == 0 && row < p.S) p.delta[at] = delta;
+      // the tile in front: its last product was on its way meanwhile
+      if (k > 0 && !(ok = finish())) break;
+      live = p.S - (row & ~(DH / 32 - 1));
+      to = p.dqkv + ((long long)b * p.S + (row & ~(DH / 32 - 1))) * C + h * DH + ch * (DH / 2);
+      none = nb == 0;
       const unsigned long long nl = two(-lse2), nd = two(-delta * p.scale);
       const int steps = nb;
       for (int t = 0; t < steps; ++t, ++n) {
@@ -2307,15 +2345,10 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.ds_ready[n & 1]));
       }
-      // dQ -> bf16 -> the query columns of the gradient
       more = ok && take(k + 1);
-      if (ok && steps > 0) ok = mbar_wait_warp(smem_u32(&sh.acc_full), (uint32_t)(n_acc++ & 1), abort_flag);
-      if (!(ok = pair_agrees(ok, quad))) break;
-      tcgen05_fence_after();
-#pragma unroll
-      for (int c = 0; c < DH / 64; ++c) store_row32(to + c * 32, tdQ + ch * (DH / 2) + c * 32 + lane_off, steps == 0, live);
-      tcgen05_fence_before();                              // the next tile's first dQ is behind this warp's next dS
+      last = k;
     }
+    if (pair_agrees(ok && last >= 0, quad)) (void)finish();
   }
   docs_bwd_end(p, sh, warp);
 }
@@ -2469,6 +2502,7 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
           for (int kk = 0; kk < BQ / 16; ++kk)             // dV[kv, d] += P^T[kv, q] dO[q, d]
             umma_ts_bf16_b(tdV, tdP + (kk >> 2) * 64 + 8 * (kk & 3), mdO, d + moff(kk), id_km, (t > 0 || kk > 0) ? 1u : 0u);
           umma_commit(smem_u32(&sh.pair_empty[n & 1]));    // dP(t) read dO(t) before
+          if (t == n_it - 1) umma_commit(smem_u32(&sh.dv_full));
         }
         if (!(ok = mbar_wait_warp(smem_u32(&sh.ds_ready[n & 1]), (uint32_t)((n >> 1) & 1), abort_flag))) break;      // dS^T beside it
         tcgen05_fence_after();
@@ -2606,13 +2640,13 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       }
       // dV and dK of this block.  Whole group in this tile: rounded into the packed gradient; a part of it: in fp32 in columns of its own, which
       // a last pass adds in order.
-      if (ok && n_it > 0) ok = mbar_wait_warp(smem_u32(&sh.acc_full), (uint32_t)(n_acc++ & 1), abort_flag);
-      if (!ok) break;
-      tcgen05_fence_after();
-      const int row = a.j * BKV + r;
+      // rows go out in groups of lanes (store_rows): of 4 in fp32, of DH / 32 in bf16
+      const int row = a.j * BKV + (r & ~((p.split > 1 ? 4 : DH / 32) - 1)), live = p.S - row;
       const long long tok = (long long)a.b * p.S + row;
 #pragma unroll 1
-      for (int acc = 0; acc < 2; ++acc) {                  // dV, dK; this warp has one column half of each
+      for (int acc = 0; acc < 2 && ok; ++acc) {            // dV, and dK, whose last product comes later; this warp has one column half of each
+        if (n_it > 0 && !(ok = mbar_wait_warp(smem_u32(acc ? &sh.acc_full : &sh.dv_full), (uint32_t)(n_acc & 1), abort_flag))) break;
+        tcgen05_fence_after();
         const int head = acc ? a.g : p.KV + a.g;
         const uint32_t from = (acc ? tdK : tdV) + ch * (DH / 2) + lane_off;
         if (p.split > 1) {
@@ -2622,19 +2656,15 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
             uint32_t v[32];
             tmem_ld32(from + c * 32, v);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint32_t w[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) w[e] = n_it == 0 ? 0u : v[8 * q + e];
-              if (row < p.S) store_sector(to + c * 32 + q * 8, w);
-            }
+            for (int e = 0; e < 32; ++e) v[e] = n_it == 0 ? 0u : v[e];
+            store_rows<4>(to + c * 32, 8LL * p.split * p.KV * DH, v, lane, live);
           }
         } else {
-          __nv_bfloat16* to = p.dqkv + tok * C + (p.H + head) * DH + ch * (DH / 2);
-#pragma unroll
-          for (int c = 0; c < DH / 64; ++c) store_row32(to + c * 32, from + c * 32, n_it == 0, row < p.S);
+          store_half<DH>(p.dqkv + tok * C + (p.H + head) * DH + ch * (DH / 2), 2LL * C, from, n_it == 0, lane, live);
         }
       }
+      if (!ok) break;
+      n_acc += n_it > 0;
       tcgen05_fence_before();                              // the next tile's first dV is behind this warp's next P
     }
   }
