@@ -2190,8 +2190,6 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       }
       return true;
     };
-    // one loop over all tiles' steps, so that each product is issued from one place: a step's S and dP go ahead of the dQ of the step in
-    // front, the next tile's ahead of the last one's
     bool ok = true;
     int tile, nb;
     for (int k = 0; ok && take_tile(sh, k, lane, abort_flag, tile, nb); ++k) {

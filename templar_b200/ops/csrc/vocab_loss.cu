@@ -169,12 +169,14 @@ __global__ void __launch_bounds__(1024) vocab_mean_kernel(const float* x, long l
   if (threadIdx.x == 0) out[0] = (float)(s / (double)max(n_valid[0], 1));
 }
 
-// y = x * (*by), from bf16 or fp32 to bf16, or onto fp32; eight values a thread
+// y = x * (*by), from bf16 or fp32 to bf16, or onto fp32; eight values a thread.  In its own place x is left alone where the factor is 1, as
+// that of a loss that is walked back from itself is: 50257 x 1000, 29 us otherwise.
 template <class In, bool ADD>
 __global__ void __launch_bounds__(256) vocab_scale_kernel(const In* x, const float* by, void* y, long long n8) {
   grid_wait();
   grid_release();
   const float f = *by;
+  if (sizeof(In) == 2 && static_cast<const void*>(x) == y && f == 1.f) return;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n8; i += gridDim.x * 256LL) {
     float v[8];
     if (sizeof(In) == 2) {

@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -781,9 +782,10 @@ Tensor mean_loss(const Tensor& losses, const Tensor& n_valid) {
   check(E.vocab_mean(losses.data_ptr<float>(), losses.numel(), n_valid.data_ptr<int>(), loss.data_ptr<float>(), stream()), "vocab_mean");
   return loss;
 }
-// t * by in bf16, or added onto the buffer
-Tensor scaled_by(const Tensor& t, const Tensor& by, const Tensor& buffer, at::IntArrayRef shape) {
-  Tensor out = buffer.defined() ? buffer : at::empty(shape, t.options().dtype(at::kBFloat16));
+// t * by in bf16, or added onto the buffer; `ours`: in t's own place, where nobody sees t again
+Tensor scaled_by(const Tensor& t, const Tensor& by, const Tensor& buffer, at::IntArrayRef shape, bool ours) {
+  ours = ours && t.scalar_type() == at::kBFloat16;
+  Tensor out = buffer.defined() ? buffer : ours ? t.view(shape) : at::empty(shape, t.options().dtype(at::kBFloat16));
   check(E.vocab_scale(t.data_ptr(), t.scalar_type() == at::kFloat, by.data_ptr<float>(), out.data_ptr(), buffer.defined(), t.numel(), stream()),
         "vocab_scale");
   return buffer.defined() ? Tensor() : out;
@@ -832,9 +834,11 @@ struct LinearCrossEntropy : Function<LinearCrossEntropy> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     auto s = ctx->get_saved_variables();
     const Tensor by = g[0].to(at::kFloat);
+    // a graph that is not kept lets go of what it saved behind this call, and cannot be walked again
+    const bool ours = !torch::autograd::get_current_graph_task_keep_graph();
     Tensor dx, dw;
-    if (s[0].defined()) dx = scaled_by(s[0], by, Tensor(), ctx->saved_data["shape"].toIntVector());
-    if (s[1].defined()) dw = scaled_by(s[1], by, aside(ctx, "buffer"), s[1].sizes());
+    if (s[0].defined()) dx = scaled_by(s[0], by, Tensor(), ctx->saved_data["shape"].toIntVector(), ours);
+    if (s[1].defined()) dw = scaled_by(s[1], by, aside(ctx, "buffer"), s[1].sizes(), ours);
     return {dx, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };

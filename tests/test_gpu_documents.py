@@ -392,6 +392,32 @@ def test_loss_scales_main_grad_and_graph_use():
     assert torch.equal(only, dw)
 
 
+@pytest.mark.parametrize("chunk", [OD.CHUNK_BYTES, 2 * 777 * 300])          # dw in bf16, of several runs in fp32
+def test_gradients_that_the_loss_made_belong_to_one_call(chunk, monkeypatch):
+    monkeypatch.setattr(OD, "CHUNK_BYTES", chunk)
+    g = gen(61)
+    x, w, labels = rows_and_labels(g, 600, 64, 777)
+    x.requires_grad_()
+    w.requires_grad_()
+    one = torch.autograd.grad(ops.linear_cross_entropy(x, w, labels), (x, w))
+    kept = [t.clone() for t in one]
+    loss = ops.linear_cross_entropy(x, w, labels)
+    first = torch.autograd.grad(loss, (x, w), grad_outputs=loss.new_tensor(0.25), retain_graph=True)
+    second = torch.autograd.grad(loss, (x, w), grad_outputs=loss.new_tensor(0.5), retain_graph=True)
+    third = torch.autograd.grad(loss, (x, w))
+    for k, o, a, b, c in zip(kept, one, first, second, third):
+        assert torch.equal(k, o) and torch.equal(a * 4, k) and torch.equal(b * 2, k) and torch.equal(c, k)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, (x, w))                      # the graph is gone
+    for times in (1, 2, 3):
+        (2 * ops.linear_cross_entropy(x, w, labels)).backward()          # .grad gathers, and is nobody else's
+        if times == 1:
+            assert torch.equal(x.grad, 2 * kept[0]) and torch.equal(w.grad, 2 * kept[1])
+    for t, k in ((x, kept[0]), (w, kept[1])):
+        # two sums, rounded to bf16 each: 1 + U of 4 and of 6 times the gradient
+        close(t.grad, 6 * k.double(), 2.01 * U * 6 * k.abs().double(), "grad")
+
+
 def test_loss_without_labels_far_logits_and_bad_labels():
     g = gen(7)
     x, w, labels = rows_and_labels(g, 150, 64, 500)
