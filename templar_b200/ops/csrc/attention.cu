@@ -1937,7 +1937,7 @@ struct DocsBwdShared {
   uint64_t s_full[2], s_read, dp_full, p_ready[2], ds_ready[2], acc_full, dv_full, stat_full[2], stat_empty[2], tile_full[2], tile_empty[2];
   uint32_t tmem_base;
   int abort;
-  int2 tile[2];                                            // (tile or -1, blocks of its walk)
+  int4 tile[2];                                            // blocks of its walk, or -1: there is none; its place
   float part[2][128];                                      // dQ: halves of delta
 };
 struct DocsStats { float nlse[128], ndelta[128]; uint8_t lo[128]; };       // dK, dV: of a query block; negated, in the units of the products
@@ -2043,19 +2043,19 @@ __device__ __forceinline__ void docs_bwd_end(const AttnDocsBwdParams& p, DocsBwd
   if (threadIdx.x == 0 && sh.abort && p.status) atomicOr(p.status, TPLR_ST_WAIT_TIMEOUT);
 }
 // The k-th tile of a CTA for the roles that use it; false: there is none, or a wait ran out.
-__device__ __forceinline__ bool take_tile(DocsBwdShared& sh, int k, int lane, volatile int* abort_flag, int& tile, int& blocks) {
+__device__ __forceinline__ bool take_tile(DocsBwdShared& sh, int k, int lane, volatile int* abort_flag, int4& tile) {
   if (!mbar_wait_warp(smem_u32(&sh.tile_full[k & 1]), (uint32_t)((k >> 1) & 1), abort_flag)) return false;
-  tile = *reinterpret_cast<volatile int*>(&sh.tile[k & 1].x);
-  blocks = *reinterpret_cast<volatile int*>(&sh.tile[k & 1].y);
+  const volatile int* at = &sh.tile[k & 1].x;
+  tile = make_int4(at[0], at[1], at[2], at[3]);
   __syncwarp();
   if (lane == 0) mbar_arrive(smem_u32(&sh.tile_empty[k & 1]));
-  return tile >= 0;
+  return tile.x >= 0;
 }
 // The loading warp's side: publishes the k-th tile; false: a wait ran out.
-__device__ __forceinline__ bool give_tile(DocsBwdShared& sh, int k, int lane, volatile int* abort_flag, int tile, int blocks) {
+__device__ __forceinline__ bool give_tile(DocsBwdShared& sh, int k, int lane, volatile int* abort_flag, int4 tile) {
   if (!mbar_wait_warp(smem_u32(&sh.tile_empty[k & 1]), (uint32_t)(((k >> 1) & 1) ^ 1), abort_flag)) return false;
   if (lane == 0) {
-    sh.tile[k & 1] = make_int2(tile, blocks);
+    sh.tile[k & 1] = tile;
     mbar_arrive(smem_u32(&sh.tile_full[k & 1]));
   }
   return true;
@@ -2106,34 +2106,46 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
     bool ok = true;
     int k = 0, n_k = 0, n_v = 0, s3 = 0;                   // tiles begun, K and V tiles asked for
     uint32_t ph3 = 0;
-    for (int tile = (int)blockIdx.x;; ++k) {
-      int qi = 0, h = 0, b = 0, nb = 0;
+    int qi, h, b, nb;
+    // publishes the k-th tile
+    auto give = [&](int k, int tile) -> bool {
+      qi = h = b = nb = 0;
       if (tile < p.tiles) {
         place(tile, qi, h, b);
         const int least = p.blocks[(long long)b * nQ + qi];
         nb = least == INT_MAX ? 0 : qi - least / BKV + 1;  // key blocks qi, qi - 1, ..
+        // the softmax warps read the block's output row by row when its turn comes, and would wait for memory
+        for (int r = lane; r < BQ && qi * BQ + r < p.S; r += 32) {
+          const char* row = reinterpret_cast<const char*>(p.out + ((long long)b * p.S + qi * BQ + r) * ((long long)p.H * DH) + h * DH);
+#pragma unroll
+          for (int line = 0; line < DH / 64; ++line) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + line * 128));
+        }
       }
-      if (!(ok = give_tile(sh, k, lane, abort_flag, tile < p.tiles ? tile : -1, nb)) || tile >= p.tiles) break;
-      const int row0 = qi * BQ, qcol = h * DH, kcol = (p.H + h / group) * DH, vcol = (p.H + p.KV + h / group) * DH;
+      return give_tile(sh, k, lane, abort_flag, make_int4(tile < p.tiles ? nb : -1, qi, h, b));
+    };
+    int tile = (int)blockIdx.x;
+    ok = give(0, tile);
+    for (; ok && tile < p.tiles; ++k) {
+      const int row0 = qi * BQ, qcol = h * DH, kcol = (p.H + h / group) * DH, vcol = (p.H + p.KV + h / group) * DH, seq = b, steps = nb, q0 = qi;
       bool resident = false;
       auto load_resident = [&]() -> bool {
         if (!mbar_wait_warp(smem_u32(&sh.res_empty), (uint32_t)((k & 1) ^ 1), abort_flag)) return false;
         if (lane == 0) {
           mbar_expect_tx(smem_u32(&sh.res_full), 2 * TILE_BYTES);
-          load_tile<DH>(sQ, &p.tmQKV, smem_u32(&sh.res_full), qcol, row0, b);
-          load_tile<DH>(sdO, &p.tmDO, smem_u32(&sh.res_full), qcol, row0, b);
+          load_tile<DH>(sQ, &p.tmQKV, smem_u32(&sh.res_full), qcol, row0, seq);
+          load_tile<DH>(sdO, &p.tmDO, smem_u32(&sh.res_full), qcol, row0, seq);
         }
         __syncwarp();
         return resident = true;
       };
       // the first K and V go ahead: their places are free while the last tile's Q and dO are still in use
-      for (int t = 0; t < nb && ok; ++t) {
-        if (t == 1 && !(ok = load_resident())) break;
-        const int krow = (qi - t) * BKV, s2 = n_v & 1;
+      for (int t = 0; t < steps && ok; ++t) {
+        if (t == 1 && !resident && !(ok = load_resident())) break;
+        const int krow = (q0 - t) * BKV, s2 = n_v & 1;
         if (!(ok = mbar_wait_warp(smem_u32(&sh.ring_empty[s3]), ph3 ^ 1u, abort_flag))) break;
         if (lane == 0) {
           mbar_expect_tx(smem_u32(&sh.ring_full[s3]), TILE_BYTES);
-          load_tile<DH>(sK + s3 * TILE_BYTES, &p.tmQKV, smem_u32(&sh.ring_full[s3]), kcol, krow, b);
+          load_tile<DH>(sK + s3 * TILE_BYTES, &p.tmQKV, smem_u32(&sh.ring_full[s3]), kcol, krow, seq);
         }
         __syncwarp();
         ++n_k;
@@ -2141,14 +2153,23 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         if (!(ok = mbar_wait_warp(smem_u32(&sh.pair_empty[s2]), (uint32_t)(((n_v >> 1) & 1) ^ 1), abort_flag))) break;
         if (lane == 0) {
           mbar_expect_tx(smem_u32(&sh.pair_full[s2]), TILE_BYTES);
-          load_tile<DH>(sV + s2 * TILE_BYTES, &p.tmQKV, smem_u32(&sh.pair_full[s2]), vcol, krow, b);
+          load_tile<DH>(sV + s2 * TILE_BYTES, &p.tmQKV, smem_u32(&sh.pair_full[s2]), vcol, krow, seq);
         }
         __syncwarp();
         ++n_v;
+        // the next tile is taken a step ahead of its first loads: in time for those who wait for its number, and not earlier, as walks differ
+        if (t == max(steps - 2, 0)) {
+          if (!resident && !(ok = load_resident())) break;
+          tile = next_tile(p, lane);
+          if (!(ok = give(k + 1, tile))) break;
+        }
       }
       if (ok && !resident) ok = load_resident();
       if (!ok) { k += resident; break; }
-      tile = next_tile(p, lane);                           // not before its loads can begin: walks differ, and a tile taken early waits
+      if (steps == 0) {
+        tile = next_tile(p, lane);
+        ok = give(k + 1, tile);
+      }
     }
     if (lane == 0) {
       Drain drain;                                         // no load may land after the CTA has retired: a role may have given up
@@ -2191,8 +2212,9 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       return true;
     };
     bool ok = true;
-    int tile, nb;
-    for (int k = 0; ok && take_tile(sh, k, lane, abort_flag, tile, nb); ++k) {
+    int4 tile;
+    for (int k = 0; ok && take_tile(sh, k, lane, abort_flag, tile); ++k) {
+      const int nb = tile.x;
       if (!(ok = mbar_wait_warp(smem_u32(&sh.res_full), (uint32_t)(k & 1), abort_flag))) break;
       if (nb == 0) {
         if (leader) mbar_arrive(smem_u32(&sh.res_empty));
@@ -2223,24 +2245,27 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
     const unsigned long long sl2 = two(p.scale_log2), sc = two(p.scale);
     int n = 0, n_acc = 0;                                  // steps and tiles with a step so far
     bool ok = true;
-    // the k-th tile and this thread's row of it: asked for before the tile in front of it is finished
-    int tile, nb, qi, h, b, row, start;                    // start INT_MAX: the row sees nothing, or is past the end
-    long long at;
-    float lse2;
+    // a tile, and this thread's row of it
+    struct Row {
+      int4 tile;                                           // steps, query block, head, sequence
+      int row, start;                                      // start INT_MAX: the row sees nothing, or is past the end
+      float lse2;
+    } next;
     uint4 o[DH / 16];                                      // this half of the row's output
-    auto take = [&](int k) -> bool {
-      if (!take_tile(sh, k, lane, abort_flag, tile, nb)) return false;
-      place(tile, qi, h, b);
-      row = qi * BQ + r;
-      at = ((long long)b * p.H + h) * p.S + row;
-      start = INT_MAX;
-      lse2 = INFINITY;
+    // the k-th tile; what is asked for here is not touched before the tile in front has been stored
+    auto ask = [&](int k) -> bool {
+      if (!take_tile(sh, k, lane, abort_flag, next.tile)) return false;
+      const int h = next.tile.z, b = next.tile.w;
+      next.row = next.tile.y * BQ + r;
+      next.start = INT_MAX;
+      next.lse2 = INFINITY;
 #pragma unroll
       for (int q = 0; q < DH / 16; ++q) o[q] = make_uint4(0u, 0u, 0u, 0u);
-      if (row < p.S) {
-        start = p.starts[(long long)b * p.S + row];
-        lse2 = p.lse[at];                                  // infinite where the row sees nothing, whose output is zero
-        const uint4* orow = reinterpret_cast<const uint4*>(p.out + ((long long)b * p.S + row) * ((long long)p.H * DH) + h * DH + ch * (DH / 2));
+      if (next.row < p.S) {
+        const long long tok = (long long)b * p.S + next.row;
+        next.start = p.starts[tok];
+        next.lse2 = p.lse[((long long)b * p.H + h) * p.S + next.row];      // infinite where the row sees nothing, whose output is zero
+        const uint4* orow = reinterpret_cast<const uint4*>(p.out + tok * ((long long)p.H * DH) + h * DH + ch * (DH / 2));
 #pragma unroll
         for (int q = 0; q < DH / 16; ++q) o[q] = orow[q];
       }
@@ -2260,13 +2285,19 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       return true;
     };
     int last = -1;                                         // the tile whose dQ is not stored yet
-    bool more = take(0);
+    bool more = ask(0);
     for (int k = 0;; ++k) {
       // both warps of a pair leave the loop together: they join their answers wherever one could leave alone
       if (!pair_agrees(more, quad)) break;
-      start = max(start, 0);
+      if (k > 0 && !(ok = finish())) break;                // the tile in front
+      const int row = next.row, steps = next.tile.x, qi = next.tile.y, h = next.tile.z, b = next.tile.w;
+      live = p.S - (row & ~(DH / 32 - 1));
+      to = p.dqkv + ((long long)b * p.S + (row & ~(DH / 32 - 1))) * C + h * DH + ch * (DH / 2);
+      none = steps == 0;
+      last = k;
+      int start = max(next.start, 0);
       if (start > row) start = INT_MAX;
-      lse2 *= 1.4426950408889634f;
+      const float lse2 = next.lse2 * 1.4426950408889634f;
       ok = mbar_wait_warp(smem_u32(&sh.res_full), (uint32_t)(k & 1), abort_flag);
       float delta = 0.f;
       if (ok) {
@@ -2290,15 +2321,11 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       }
       if (!(ok = pair_agrees(ok, quad))) break;
       delta = start == INT_MAX ? 0.f : sh.part[0][r] + sh.part[1][r];
-      if (ch == 0 && row < p.S) p.delta[at] = delta;
-      // the tile in front: its last product was on its way meanwhile
-      if (k > 0 && !(ok = finish())) break;
-      live = p.S - (row & ~(DH / 32 - 1));
-      to = p.dqkv + ((long long)b * p.S + (row & ~(DH / 32 - 1))) * C + h * DH + ch * (DH / 2);
-      none = nb == 0;
+      if (ch == 0 && row < p.S) p.delta[((long long)b * p.H + h) * p.S + row] = delta;
       const unsigned long long nl = two(-lse2), nd = two(-delta * p.scale);
-      const int steps = nb;
+      if (steps == 0) more = ask(k + 1);
       for (int t = 0; t < steps; ++t, ++n) {
+        if (t + 1 == steps) more = ask(k + 1);
         const bool diag = t == 0;
         const int lo = (start == INT_MAX ? BKV : start - (qi - t) * BKV) - ch * 64, hi = (diag ? r : BKV - 1) - ch * 64;
         if (!(ok = mbar_wait_warp(smem_u32(&sh.s_full[0]), n & 1, abort_flag))) break;
@@ -2343,8 +2370,7 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.ds_ready[n & 1]));
       }
-      more = ok && take(k + 1);
-      last = k;
+      more = more && ok;
     }
     if (pair_agrees(ok && last >= 0, quad)) (void)finish();
   }
@@ -2367,13 +2393,14 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
   const uint32_t sK = smem_u32(smem), sV = sK + TILE_BYTES, sQ = sV + TILE_BYTES, sdO = sQ + RING3 * TILE_BYTES;
   // tiles: early key blocks, which may be seen by the most rows, first
   struct Place { int j, sub, g, b, h0; };
-  auto place = [&](int tile) {
+  // the key block, the group and its part, the sequence
+  auto place = [&](int4 tile) {
     Place a;
-    a.j = tile / gb;
-    a.sub = tile % gb % p.split;
-    a.g = tile % gb / p.split % p.KV;
-    a.b = tile % gb / p.split / p.KV;
-    a.h0 = (a.g * p.split + a.sub) * heads;
+    a.j = tile.y;
+    a.g = p.split > 1 ? tile.z / p.split : tile.z;
+    a.sub = tile.z - a.g * p.split;
+    a.b = tile.w;
+    a.h0 = tile.z * heads;
     return a;
   };
   if (threadIdx.x == 0) { prefetch_map(&p.tmQKV); prefetch_map(&p.tmDO); }
@@ -2388,20 +2415,28 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
     bool ok = true;
     int k = 0, n_q = 0, n_do = 0, s3 = 0;                  // tiles begun, Q and dO tiles asked for
     uint32_t ph3 = 0;
-    for (int tile = (int)blockIdx.x;; ++k) {
-      Place a = {};
-      int n_i = 0;
+    int4 now = make_int4(0, 0, 0, 0);
+    // publishes the k-th tile
+    auto give = [&](int k, int tile) -> bool {
+      now.x = -1;
       if (tile < p.tiles) {
         // the last query block that sees any key of this one.  A block in between whose rows begin behind it is walked with all its
         // weights masked: starts that grow with the row, as documents' do, have none.
-        a = place(tile);
+        now.y = tile / gb;
+        now.z = tile % gb % (p.KV * p.split);
+        now.w = tile % gb / (p.KV * p.split);
         int last = -1;
-        for (int i = a.j + lane; i < nQ; i += 32)
-          if (p.blocks[(long long)a.b * nQ + i] < (a.j + 1) * BKV) last = i;
-        n_i = max(__reduce_max_sync(0xffffffffu, last) - a.j + 1, 0);
+        for (int i = now.y + lane; i < nQ; i += 32)
+          if (p.blocks[(long long)now.w * nQ + i] < (now.y + 1) * BKV) last = i;
+        now.x = max(__reduce_max_sync(0xffffffffu, last) - now.y + 1, 0);
       }
-      if (!(ok = give_tile(sh, k, lane, abort_flag, tile < p.tiles ? tile : -1, n_i)) || tile >= p.tiles) break;
-      const int n_it = heads * n_i;
+      return give_tile(sh, k, lane, abort_flag, now);
+    };
+    int tile = (int)blockIdx.x;
+    ok = give(0, tile);
+    for (; ok && tile < p.tiles; ++k) {
+      const Place a = place(now);
+      const int n_i = now.x, n_it = heads * n_i;
       bool resident = false;
       auto load_resident = [&]() -> bool {
         if (!mbar_wait_warp(smem_u32(&sh.res_empty), (uint32_t)((k & 1) ^ 1), abort_flag)) return false;
@@ -2416,7 +2451,7 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       int h = a.h0, i = 0;
       // the first Q and dO go ahead: their places are free while the last tile's K and V are still in use
       for (int t = 0; t < n_it && ok; ++t) {
-        if (t == 1 && !(ok = load_resident())) break;
+        if (t == 1 && !resident && !(ok = load_resident())) break;
         const int qrow0 = (a.j + i) * BQ, s2 = n_do & 1;
         if (!(ok = mbar_wait_warp(smem_u32(&sh.ring_empty[s3]), ph3 ^ 1u, abort_flag))) break;
         if (lane == 0) {
@@ -2434,10 +2469,18 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
         __syncwarp();
         ++n_do;
         if (++i == n_i) { i = 0; ++h; }
+        if (t == max(n_it - 2, 0)) {                       // the next tile, as in dQ's kernel
+          if (!resident && !(ok = load_resident())) break;
+          tile = next_tile(p, lane);
+          if (!(ok = give(k + 1, tile))) break;
+        }
       }
       if (ok && !resident) ok = load_resident();
       if (!ok) { k += resident; break; }
-      tile = next_tile(p, lane);                           // not before its loads can begin: walks differ, and a tile taken early waits
+      if (n_it == 0) {
+        tile = next_tile(p, lane);
+        ok = give(k + 1, tile);
+      }
     }
     if (lane == 0) {
       Drain drain;                                         // no load may land after the CTA has retired: a role may have given up
@@ -2479,9 +2522,9 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       return true;
     };
     bool ok = true;
-    int tile, n_i;
-    for (int k = 0; ok && take_tile(sh, k, lane, abort_flag, tile, n_i); ++k) {
-      const int n_it = heads * n_i;
+    int4 tile;
+    for (int k = 0; ok && take_tile(sh, k, lane, abort_flag, tile); ++k) {
+      const int n_it = heads * tile.x;
       if (!(ok = mbar_wait_warp(smem_u32(&sh.res_full), (uint32_t)(k & 1), abort_flag))) break;
       if (n_it == 0) {
         if (leader) mbar_arrive(smem_u32(&sh.res_empty));
@@ -2519,10 +2562,11 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
   } else if (warp == 10) {
     // lse, delta and starts of a step's query block, four rows a lane, asked for while the step before is used
     bool ok = true;
-    int n = 0, tile, n_i;
-    for (int k = 0; ok && take_tile(sh, k, lane, abort_flag, tile, n_i); ++k) {
+    int n = 0;
+    int4 tile;
+    for (int k = 0; ok && take_tile(sh, k, lane, abort_flag, tile); ++k) {
       const Place a = place(tile);
-      const int n_it = heads * n_i, kvrow0 = a.j * BKV;
+      const int n_i = tile.x, n_it = heads * n_i, kvrow0 = a.j * BKV;
       int h = a.h0, i = 0;
       float nl[4], nd[4];
       int lo[4];
@@ -2556,10 +2600,11 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const unsigned long long sl2 = two(p.scale_log2), sc = two(p.scale);
     bool ok = true;
-    int n = 0, n_acc = 0, tile, n_i;                       // steps and tiles with a step so far
-    for (int k = 0; ok && take_tile(sh, k, lane, abort_flag, tile, n_i); ++k) {
+    int n = 0, n_acc = 0;                                  // steps and tiles with a step so far
+    int4 tile;
+    for (int k = 0; ok && take_tile(sh, k, lane, abort_flag, tile); ++k) {
       const Place a = place(tile);
-      const int n_it = heads * n_i;
+      const int n_i = tile.x, n_it = heads * n_i;
       int i = 0;
       for (int t = 0; t < n_it; ++t, ++n) {
         const DocsStats& st = stats[n & 1];
