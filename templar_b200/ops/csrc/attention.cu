@@ -1586,6 +1586,18 @@ struct AttnDocsParams {
                           // behind it two counters for the backward kernels, zeroed here
 };
 
+// A mask of 64 columns as bits, tested one by one: 1.2 instructions a column, where two comparisons and a choice are 3.
+__device__ __forceinline__ uint64_t columns(int lo, int hi) {              // lo .. hi, either of which may lie outside
+  if (hi < max(lo, 0) || lo > 63) return 0;
+  return (~0ull << max(lo, 0)) & (~0ull >> (63 - min(hi, 63)));
+}
+__device__ __forceinline__ void keep_columns(uint32_t* v, uint64_t mask, uint32_t other) {
+  const uint32_t m0 = (uint32_t)mask, m1 = (uint32_t)(mask >> 32);
+#pragma unroll
+  for (int e = 0; e < 32; ++e) if (!(m0 >> e & 1u)) v[e] = other;
+#pragma unroll
+  for (int e = 0; e < 32; ++e) if (!(m1 >> e & 1u)) v[32 + e] = other;
+}
 // Both warps of a quadrant come here with an answer and leave with the joint one.
 __device__ __forceinline__ bool pair_agrees(bool ok, int quad) {
   uint32_t both;
@@ -1754,8 +1766,7 @@ attn_docs_fwd_kernel(const __grid_constant__ AttnDocsParams p) {
         if (lane == 0) mbar_arrive(smem_u32(&bar_s_read));
       }
       if (__any_sync(0xffffffffu, lo > 0 || hi < 63)) {
-#pragma unroll
-        for (int e = 0; e < 64; ++e) if (e < lo || e > hi) v[e] = 0xff800000u;         // -inf: exp2 makes it zero
+        keep_columns(v, columns(lo, hi), 0xff800000u);      // -inf: exp2 makes it zero
       }
       float mx = -INFINITY, mx2 = -INFINITY;
 #pragma unroll
@@ -1996,15 +2007,14 @@ __device__ __forceinline__ void store_rows(void* first, long long pitch, uint32_
 // half a row of an accumulator, DH / 2 columns, as bf16
 template <int DH>
 __device__ __forceinline__ void store_half(void* first, long long pitch, uint32_t tmem, bool zero, int lane, int live) {
-  uint32_t w[DH / 4];
 #pragma unroll
   for (int c = 0; c < DH / 64; ++c) {
-    uint32_t v[32];
+    uint32_t v[32], w[16];
     tmem_ld32(tmem + c * 32, v);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) w[16 * c + e] = zero ? 0u : bf16x2_of(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+    for (int e = 0; e < 16; ++e) w[e] = zero ? 0u : bf16x2_of(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+    store_rows<2>(static_cast<char*>(first) + 64 * c, pitch, w, lane, live);
   }
-  store_rows<DH / 32>(first, pitch, w, lane, live);
 }
 __device__ __forceinline__ void docs_bwd_init(DocsBwdShared& sh, int warp, int consumers) {
   if (threadIdx.x == 0) {
@@ -2272,7 +2282,7 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       return true;
     };
     // dQ of the tile begun last -> bf16 -> the query columns of the gradient
-    __nv_bfloat16* to = nullptr;                           // the first row of this lane's group of DH / 32, and how many of its rows are there
+    __nv_bfloat16* to = nullptr;                           // the first row of this lane's group of two, and how many rows there are from it
     int live = 0;
     bool none = false;
     auto finish = [&]() -> bool {
@@ -2291,8 +2301,8 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       if (!pair_agrees(more, quad)) break;
       if (k > 0 && !(ok = finish())) break;                // the tile in front
       const int row = next.row, steps = next.tile.x, qi = next.tile.y, h = next.tile.z, b = next.tile.w;
-      live = p.S - (row & ~(DH / 32 - 1));
-      to = p.dqkv + ((long long)b * p.S + (row & ~(DH / 32 - 1))) * C + h * DH + ch * (DH / 2);
+      live = p.S - (row & ~1);
+      to = p.dqkv + ((long long)b * p.S + (row & ~1)) * C + h * DH + ch * (DH / 2);
       none = steps == 0;
       last = k;
       int start = max(next.start, 0);
@@ -2348,8 +2358,7 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
           v[e + 1] = __float_as_uint(exp2f(a1));
         }
         if (__any_sync(0xffffffffu, lo > 0 || hi < 63)) {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) if (e < lo || e > hi) v[e] = 0u;
+          keep_columns(v, columns(lo, hi), 0u);
         }
         if (!(ok = mbar_wait_warp(dp_bar(n), (uint32_t)((n >> 1) & 1), abort_flag))) break;
         tcgen05_fence_after();
@@ -2375,6 +2384,19 @@ attn_docs_dq_kernel(const __grid_constant__ AttnDocsBwdParams p) {
     if (pair_agrees(ok && last >= 0, quad)) (void)finish();
   }
   docs_bwd_end(p, sh, warp);
+}
+
+// Lane e comes with the first of the warp's 32 keys that query row e sees; lane r leaves with the query rows that see key r: a matrix of
+// 32 x 32 bits, transposed.
+__device__ __forceinline__ uint32_t seen_by(int first, int lane) {
+  uint32_t x = first <= 0 ? ~0u : first > 31 ? 0u : ~0u << first, low = 0x0000ffffu;
+#pragma unroll
+  for (int j = 16; j > 0; j >>= 1) {
+    const uint32_t y = __shfl_xor_sync(0xffffffffu, x, j);
+    x = lane & j ? (x & ~low) | (y & ~low) >> j : (x & low) | (y & low) << j;
+    low ^= low << (j >> 1);
+  }
+  return x;
 }
 
 template <int DH>
@@ -2633,18 +2655,12 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
           w[2] = __float_as_uint(exp2f(a2)); w[3] = __float_as_uint(exp2f(a3));
         }
         // a query row before the key, or whose document begins behind it, does not see it
-        const uint32_t* lo4 = reinterpret_cast<const uint32_t*>(st.lo + ch * 64);
-        if (__any_sync(0xffffffffu, lo4[lane & 15] != 0u)) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint32_t w = lo4[e];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) if ((int)((w >> (8 * q)) & 255u) > r) v[4 * e + q] = 0u;
-          }
-        }
-        if (diag) {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) if (ch * 64 + e < r) v[e] = 0u;
+        const int first0 = st.lo[ch * 64 + lane] - quad * 32, first1 = st.lo[ch * 64 + 32 + lane] - quad * 32;
+        const bool begins = __any_sync(0xffffffffu, max(first0, first1) > 0);
+        if (begins || diag) {
+          uint64_t mask = diag ? columns(r - ch * 64, 63) : ~0ull;
+          if (begins) mask &= (uint64_t)seen_by(first1, lane) << 32 | seen_by(first0, lane);
+          keep_columns(v, mask, 0u);
         }
         if (!(ok = mbar_wait_warp(smem_u32(&sh.dp_full), n & 1, abort_flag))) break;
         tcgen05_fence_after();
@@ -2683,8 +2699,8 @@ attn_docs_dkv_kernel(const __grid_constant__ AttnDocsBwdParams p) {
       }
       // dV and dK of this block.  Whole group in this tile: rounded into the packed gradient; a part of it: in fp32 in columns of its own, which
       // a last pass adds in order.
-      // rows go out in groups of lanes (store_rows): of 4 in fp32, of DH / 32 in bf16
-      const int row = a.j * BKV + (r & ~((p.split > 1 ? 4 : DH / 32) - 1)), live = p.S - row;
+      // rows go out in groups of lanes (store_rows): of 4 in fp32, of 2 in bf16
+      const int row = a.j * BKV + (r & ~((p.split > 1 ? 4 : 2) - 1)), live = p.S - row;
       const long long tok = (long long)a.b * p.S + row;
 #pragma unroll 1
       for (int acc = 0; acc < 2 && ok; ++acc) {            // dV, and dK, whose last product comes later; this warp has one column half of each
