@@ -957,6 +957,9 @@ __device__ __forceinline__ bool epilogue_swiglu_bwd_q8(const Gemm2Params& p, uin
 // which the two products behind take along.  A pass over the [M, N] weights that brings every piece to the row's largest logit
 // instead took 197 us where this product takes 693 (8192 x 2048 x 32000).  Within SM_NEAR the sums stay far inside fp32:
 // exp(40) = 2e17, and a weight is only lost where it is below 1e-20 of the row's sum.
+//
+// One B200: 4096 x 4096 x 128256 without the weights 2626 us, 1640 TFLOP/s, the tensor pipe 98 % busy (the plain product's own time); 1111 x 1000 x
+// 50257 with them 126 us, 112 MB stored, the pipe 48 %: 13 % of its rows are the last tile's, and 16 k blocks do not cover an epilogue.
 constexpr float SM_NEAR = 40.f;
 __device__ __forceinline__ float ex2(float x) {
   float r;

@@ -9,6 +9,9 @@
 // and E is not read or written here but for the label's column and pieces of another reference.  f x is rounded to bf16, as d would be.
 //
 // A row whose label is ignored, or is no column, has loss and gradient zero.  Sums over rows and pieces are taken in one order.
+//
+// One B200, 1111 rows of 1000, 50257 columns: the product with the softmax 126 us, this file's pass over rows 11, dx 94 + 6, dw 79, count and mean 5
+// each; logits stored, read and turned into their gradient would be 670 MB more, 100 us.
 #include "common.cuh"
 
 namespace {
