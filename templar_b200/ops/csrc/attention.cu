@@ -1953,7 +1953,7 @@ constexpr int DQ_THREADS = 320, DKV_THREADS = 352;
 constexpr int RING3 = 3;                                   // K (dQ) or Q (dK, dV): held from the first product of a step to its last
 // Q, dO; three K, two V   |   K, V; three Q, two dO; and the small things behind them.  The tiles start at the window's 1024-byte boundary.
 template <int DH> constexpr int docs_bwd_tiles() { return 7 * tile_bytes<DH>(); }
-template <int DH> constexpr int docs_bwd_smem() { return docs_bwd_tiles<DH>() + 3072; }
+template <int DH> constexpr int docs_bwd_smem() { return docs_bwd_tiles<DH>() + 3 * 1024; }
 
 struct DocsBwdShared {
   uint64_t res_full, res_empty;                            // the tile's resident operands
@@ -1965,7 +1965,7 @@ struct DocsBwdShared {
   float part[2][128];                                      // dQ: halves of delta
 };
 struct DocsStats { float nlse[128], ndelta[128]; uint8_t lo[128]; };       // dK, dV: of a query block; negated, in the units of the products
-static_assert(sizeof(DocsBwdShared) <= 1536 && offsetof(DocsBwdShared, part) <= 512 && 512 + 2 * sizeof(DocsStats) <= 3072,
+static_assert(sizeof(DocsBwdShared) <= 1536 && offsetof(DocsBwdShared, part) <= 512 && 512 + 2 * sizeof(DocsStats) <= 3 * 1024,
               "the small things fit behind the tiles");
 
 struct AttnDocsBwdParams {

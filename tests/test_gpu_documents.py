@@ -404,6 +404,8 @@ def test_gradients_that_the_loss_made_belong_to_one_call(chunk, monkeypatch):
     loss = ops.linear_cross_entropy(x, w, labels)
     first = torch.autograd.grad(loss, (x, w), grad_outputs=loss.new_tensor(0.25), retain_graph=True)
     second = torch.autograd.grad(loss, (x, w), grad_outputs=loss.new_tensor(0.5), retain_graph=True)
+    node = loss.grad_fn(loss.new_tensor(0.5))                  # called by hand: nothing says that the graph goes
+    assert all(torch.equal(a, b) for a, b in zip(node[:2], second))
     third = torch.autograd.grad(loss, (x, w))
     for k, o, a, b, c in zip(kept, one, first, second, third):
         assert torch.equal(k, o) and torch.equal(a * 4, k) and torch.equal(b * 2, k) and torch.equal(c, k)
@@ -457,7 +459,7 @@ def test_loss_of_logits_far_from_zero(shift, some):
 
 
 @pytest.mark.parametrize("shift", [0.0, 95.0, -95.0])
-@pytest.mark.parametrize("T,D,V", [(1, 8, 1), (1, 2048, 257), (2, 72, 31), (15, 64, 33), (17, 200, 32000), (33, 768, 255), (64, 128, 512), (97, 1000, 50257),
+@pytest.mark.parametrize("T,D,V", [(1, 8, 1), (1, 2048, 257), (2, 72, 31), (15, 64, 33), (17, 200, 32000), (33, 768, 255), (64, 128, 512), (80, 136, 3001), (97, 1000, 50257),
                                    (127, 64, 4097), (128, 264, 20000)])
 def test_losses_of_few_tokens(T, D, V, shift):
     """Scoring without a gradient: up to 128 tokens take the product with the weight's rows along the tile."""
