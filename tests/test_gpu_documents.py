@@ -7,6 +7,7 @@ import torch
 from templar_b200 import ops
 from templar_b200.ops import documents as OD
 from templar_b200.ops import functional as OF
+from templar_b200.ops import native
 
 pytestmark = pytest.mark.gpu
 U = torch.finfo(torch.bfloat16).eps / 2
@@ -631,3 +632,37 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(out[-1:], one) and torch.equal(grad[-1:, :, :H * hd], gone[..., :H * hd])
     # alone its groups' heads may be split over tiles, whose parts are added in fp32: another order
     torch.testing.assert_close(grad[-1:].float(), gone.float(), rtol=2 * U, atol=2 * U * gone.float().abs().mean().item())
+
+
+def test_nodes_in_python_and_in_cpp_make_the_same_bits(monkeypatch):
+    """Without the host library the same operators run as nodes in Python."""
+    g = gen(71)
+    H, KV, hd, B, S = 4, 2, 64, 2, 300
+    qkv = torch.randn(B, S, (H + 2 * KV) * hd, generator=g, device=DEV).to(torch.bfloat16).requires_grad_()
+    wq, wk = (torch.rand(hd, generator=g, device=DEV).to(torch.bfloat16).requires_grad_() for _ in range(2))
+    cos, sin = OF.rope_tables(512, hd, device=DEV)
+    ends = torch.rand(B, S, generator=g, device=DEV) < 0.02
+    starts = torch.where(ends, torch.arange(S, device=DEV, dtype=torch.int32), 0).cummax(1).values.to(torch.int32)
+    do = torch.randn(B, S, H * hd, generator=g, device=DEV).to(torch.bfloat16)
+    x, w, labels = rows_and_labels(g, 600, 64, 777)
+    x.requires_grad_()
+    w.requires_grad_()
+
+    def everything():
+        z = ops.qk_norm_rope(qkv, wq, wk, cos, sin, H, KV, hd)
+        out = ops.attention_documents(z, starts, H, KV, hd)
+        made = [out, *torch.autograd.grad(out, (qkv, wq, wk), do)]
+        with torch.no_grad():
+            made += [ops.attention_documents(z, starts, H, KV, hd)]
+            made += [ops.linear_cross_entropy(x[:n], w, labels[:n], reduction=r) for n in (20, 600) for r in ("mean", "none")]
+        for n in (20, 600):
+            loss = ops.linear_cross_entropy(x[:n], w, labels[:n])
+            made += [loss, *torch.autograd.grad(3 * loss, (x, w))]
+            each = ops.linear_cross_entropy(x[:n], w, labels[:n], reduction="none")
+            made += [each, *torch.autograd.grad(each.sum(), (x, w))]
+        return made
+
+    cpp = everything()
+    monkeypatch.setattr(native, "host", lambda: None)
+    assert all(torch.equal(a, b) for a, b in zip(everything(), cpp))
+    assert int(OF.status_word(DEV).item()) == 0
