@@ -37,6 +37,12 @@ def _same_device(what: str, t: torch.Tensor, **others) -> None:
             raise ValueError(f"{what}: {name} is on {o.device}, the rows are on {t.device}")
 
 
+def _fitting_buffer(what: str, name: str, w: torch.Tensor, main_grad: torch.Tensor) -> None:
+    """The kernels add ``w``'s gradient into the buffer by its address."""
+    if main_grad.device != w.device or main_grad.numel() != w.numel():
+        raise ValueError(f"{what}: {name} of {w.numel()} numbers on {w.device} expected, got {main_grad.numel()} on {main_grad.device}")
+
+
 def _heads(what: str, qkv: torch.Tensor, n_heads: int, n_kv: int, hd: int) -> None:
     if qkv.dim() != 3 or n_heads < 1 or n_kv < 1 or n_heads % n_kv or hd < 1 or qkv.shape[2] != (n_heads + 2 * n_kv) * hd:
         raise ValueError(f"{what}: a packed projection [B, S, (H + 2 KV) * hd] expected, got {tuple(qkv.shape)} for {n_heads} query heads on "
@@ -239,6 +245,10 @@ def qk_norm_rope(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, cos: tor
         main_grad_q = getattr(wq, "main_grad", None)
     if main_grad_k is None:
         main_grad_k = getattr(wk, "main_grad", None)
+    if any(b is not None and not torch.is_tensor(b) for b in (main_grad_q, main_grad_k)):
+        if torch.is_grad_enabled() and (qkv.requires_grad or wq.requires_grad or wk.requires_grad):
+            raise ValueError("qk_norm_rope: the weights' gradients are buffers here, not shards of other ranks")
+        main_grad_q = main_grad_k = None
     if qkv.is_cuda and (host := native.host()) and (y := host.qk_norm_rope(qkv, wq, wk, cos, sin, positions, n_heads, n_kv, hd, eps, main_grad_q,
                                                                            main_grad_k, _word(qkv))) is not None:
         return y
@@ -252,6 +262,10 @@ def qk_norm_rope(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, cos: tor
     if positions is not None and (positions.shape != (B, S) or positions.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"qk_norm_rope: int32 positions [{B}, {S}] expected, got {positions.dtype} {tuple(positions.shape)}")
     _same_device("qk_norm_rope", qkv, wq=wq, wk=wk, cos=cos, sin=sin, positions=positions)
+    grad = torch.is_grad_enabled() and (qkv.requires_grad or wq.requires_grad or wk.requires_grad)
+    for name, w, main_grad in (("main_grad_q", wq, main_grad_q), ("main_grad_k", wk, main_grad_k)):
+        if grad and main_grad is not None:
+            _fitting_buffer("qk_norm_rope", name, w, main_grad)
     if not (OF._native_ok(qkv, wq, wk) and hd % 8 == 0 and hd <= 256 and cos.dtype == sin.dtype == torch.float32) or B * S == 0:
         if main_grad_q is not None and wq.requires_grad:
             wq = _AddMainGrad.apply(wq, main_grad_q)
@@ -266,7 +280,7 @@ def qk_norm_rope(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, cos: tor
             y = host.qk_norm_rope(qkv, wq, wk, cos, sin, positions, n_heads, n_kv, hd, eps, main_grad_q, main_grad_k, _word(qkv))
         if y is not None:
             return y
-    if torch.is_grad_enabled() and (qkv.requires_grad or wq.requires_grad or wk.requires_grad):
+    if grad:
         return _QKNormRope.apply(qkv, wq, wk, cos, sin, positions, n_heads, n_kv, hd, eps, main_grad_q, main_grad_k)
     rows, ld = _packed_rows(qkv)
     return _qk_norm_rope(rows, ld, OF._dense(wq), OF._dense(wk), cos, sin, positions, n_heads, n_kv, hd, eps)
@@ -471,6 +485,8 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
     _same_device("linear_cross_entropy", x, w=w, labels=labels)
     flat = labels.reshape(-1).contiguous().to(torch.int64)
     grad = torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
+    if main_grad is not None and grad and w.requires_grad:
+        _fitting_buffer("linear_cross_entropy", "main_grad", w, main_grad)
     T = flat.numel()
     if not OF._native_ok(x, w) or w.shape[1] % 8 or T == 0:
         if main_grad is not None and grad and w.requires_grad:
