@@ -205,19 +205,25 @@ __global__ void __launch_bounds__(WARPS * 32, 4) qk_norm_bwd_kernel(const QkNorm
   }
 }
 
-// The blocks' sums added in one order, 32 columns a block: into out (bf16) or onto add (fp32), for wq and for wk.
+// The blocks' sums added in one order, 32 columns a block: into out (bf16) or onto add (fp32), for wq and for wk.  Where both have the same
+// buffer (one weight for queries and keys) a thread has both sums of an element: two threads that add onto it could lose one.
 __global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const float* part, int blocks, int hd, bf16* dwq, bf16* dwk, float* add_q,
                                                           float* add_k) {
   __shared__ float red[32][33];
   grid_wait();
   grid_release();
   const int col = blockIdx.x * 32 + (threadIdx.x & 31), row = threadIdx.x >> 5;
+  const bool both = add_q && add_q == add_k;
+  const int cols = both ? hd : 2 * hd;
   float t = 0.f;
-  if (col < 2 * hd)
+  if (col < cols) {
     for (int k = row; k < blocks; k += 32) t += part[(long long)k * 2 * hd + col];
+    if (both)
+      for (int k = row; k < blocks; k += 32) t += part[(long long)k * 2 * hd + hd + col];
+  }
   red[row][threadIdx.x & 31] = t;
   __syncthreads();
-  if (row != 0 || col >= 2 * hd) return;
+  if (row != 0 || col >= cols) return;
   t = 0.f;
 #pragma unroll
   for (int k = 0; k < 32; ++k) t += red[k][threadIdx.x & 31];
@@ -272,7 +278,8 @@ TPLR_API int tplr_qk_norm_rope_parts(long long tokens, int n_q, int n_k, int hd)
 }
 
 // dx (dense) from dy (rows of lddy elements) and the forward's x; part: tplr_qk_norm_rope_parts rows of 2 * hd fp32, contents
-// irrelevant.  Each weight's gradient is added onto add_* (fp32) where that is given, else stored to dw* (bf16) where that is.
+// irrelevant.  Each weight's gradient is added onto add_* (fp32) where that is given, else stored to dw* (bf16) where that is.  add_q and
+// add_k may be the same buffer, but not overlap in part.
 TPLR_API int tplr_qk_norm_rope_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* wq, const void* wk,
                                    const float* cosb, const float* sinb, const int* pos, void* dx, float* part, void* dwq, void* dwk,
                                    float* add_q, float* add_k, long long tokens, int S, int table_rows, int n_q, int n_k, int hd, float eps,
@@ -283,7 +290,7 @@ TPLR_API int tplr_qk_norm_rope_bwd(const void* dy, long long lddy, const void* x
   p.x = (const bf16*)x; p.ldx = ldx; p.dy = (const bf16*)dy; p.lddy = lddy; p.y = (bf16*)dx; p.wq = (const bf16*)wq; p.wk = (const bf16*)wk;
   p.cosb = cosb; p.sinb = sinb; p.pos = pos; p.tokens = tokens; p.S = S; p.table_rows = table_rows; p.n_q = n_q; p.n_k = n_k; p.hd = hd;
   p.eps = eps; p.inv_hd = 1.f / (float)hd; p.part = part; p.status = status;
-  if (!fits(p)) return -301;
+  if (!fits(p) || (add_q && add_k && add_q != add_k && add_q < add_k + hd && add_k < add_q + hd)) return -301;
   p.chunks = chunks_of(n_q, n_k, hd, BWD_STEPS);
   auto kern = lanes_of(hd) == 8 ? qk_norm_bwd_kernel<8, BWD_STEPS> : lanes_of(hd) == 16 ? qk_norm_bwd_kernel<16, BWD_STEPS>
                                                                                         : qk_norm_bwd_kernel<32, BWD_STEPS>;

@@ -718,6 +718,10 @@ Maybe qk_norm_rope(const Tensor& qkv, const Tensor& wq, const Tensor& wk, const 
         !t->is_contiguous() || !on_boundary(*t))
       return std::nullopt;
   if (cos.size(0) < (at ? 1 : qkv.size(1))) return std::nullopt;
+  // two weights may add into one buffer, but not into parts of each other's
+  if (bq && bk && bq->data_ptr() != bk->data_ptr() && bq->data_ptr<float>() < bk->data_ptr<float>() + hd &&
+      bk->data_ptr<float>() < bq->data_ptr<float>() + hd)
+    return std::nullopt;
   if (at && (!here(*at, dev) || at->scalar_type() != at::kInt || at->dim() != 2 || at->size(0) != qkv.size(0) || at->size(1) != qkv.size(1) ||
              !at->is_contiguous()))
     return std::nullopt;

@@ -240,7 +240,8 @@ def qk_norm_rope(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, cos: tor
     """``qkv`` [B, S, (H + 2 KV) * hd] with every query head normed and weighted by ``wq`` [hd], every key head by ``wk`` [hd], and both
     turned by the rotary embedding (interleaved pairs, tables of :func:`rope_tables`), in one pass; value heads as they are.
     ``positions``: int32 [B, S], the row of the tables that a token takes (its place in its document); without them its place
-    in the sequence.  A position outside the tables takes their first or last row, and the kernels report it in the status word."""
+    in the sequence.  A position outside the tables takes their first or last row, and the kernels report it in the status word.
+    One weight may serve both, and one buffer may take both gradients."""
     if main_grad_q is None:
         main_grad_q = getattr(wq, "main_grad", None)
     if main_grad_k is None:
@@ -266,6 +267,10 @@ def qk_norm_rope(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, cos: tor
     for name, w, main_grad in (("main_grad_q", wq, main_grad_q), ("main_grad_k", wk, main_grad_k)):
         if grad and main_grad is not None:
             _fitting_buffer("qk_norm_rope", name, w, main_grad)
+    if grad and main_grad_q is not None and main_grad_k is not None:
+        q, k = ((t.data_ptr(), t.data_ptr() + t.nbytes) for t in (main_grad_q, main_grad_k))
+        if q[0] != k[0] and q[0] < k[1] and k[0] < q[1]:
+            raise ValueError("qk_norm_rope: main_grad_q and main_grad_k are one buffer or two, they do not overlap in part")
     if not (OF._native_ok(qkv, wq, wk) and hd % 8 == 0 and hd <= 256 and cos.dtype == sin.dtype == torch.float32) or B * S == 0:
         if main_grad_q is not None and wq.requires_grad:
             wq = _AddMainGrad.apply(wq, main_grad_q)

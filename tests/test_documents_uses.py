@@ -50,3 +50,50 @@ def test_buffers_that_are_not_the_weights_are_refused(device):
     for b in (other, low):
         ops.linear_cross_entropy(x.detach(), w, labels, main_grad=b).backward()
         torch.testing.assert_close(b.flatten().float(), dw.flatten().float(), rtol=2 * U, atol=1e-7)
+
+
+def test_buffers_that_overlap_in_part_are_refused():
+    H, KV, hd, S = 2, 1, 8, 5
+    qkv, wq, wk = (normal(i, *s).requires_grad_() for i, s in ((1, (1, S, (H + 2 * KV) * hd)), (2, (hd,)), (3, (hd,))))
+    cos, sin = ops.rope_tables(S, hd)
+    long = torch.zeros(2 * hd)
+    run = lambda a, b: ops.qk_norm_rope(qkv, wq, wk, cos, sin, H, KV, hd, main_grad_q=a, main_grad_k=b)  # noqa: E731
+    for i, j in ((0, 4), (1, 0), (7, 0)):
+        with pytest.raises(ValueError, match="overlap"):
+            run(long[i:i + hd], long[j:j + hd])
+    run(long[:hd], long[hd:]).sum().backward()
+    apart = long.clone()
+    run(long[:hd], long[:hd]).sum().backward()
+    torch.testing.assert_close(long[:hd], 2 * apart[:hd] + apart[hd:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("host", [True, False])
+@pytest.mark.parametrize("B,S,H,KV,hd", [(1, 1, 1, 1, 8), (2, 700, 4, 2, 64), (1, 3000, 16, 4, 128), (1, 90, 5, 5, 256)])
+def test_one_buffer_for_the_gradients_of_both_weights(B, S, H, KV, hd, host, monkeypatch):
+    if not host:
+        monkeypatch.setattr(native, "host", lambda: None)
+    x = normal(1, B, S, (H + 2 * KV) * hd, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    w = normal(2, hd, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    cos, sin = ops.rope_tables(1, hd, device=DEV)
+    at = torch.zeros(B, S, dtype=torch.int32, device=DEV)      # no angle, and gradients of the rows' own sign: every term of the sums is positive
+    dy = torch.sign(x.detach())
+    run = lambda wq, wk, mq, mk: ops.qk_norm_rope(x, wq, wk, cos, sin, H, KV, hd, positions=at, main_grad_q=mq, main_grad_k=mk).backward(dy)  # noqa: E731
+    q, k = (torch.zeros(hd, device=DEV) for _ in range(2))
+    other = w.detach().clone().requires_grad_()
+    run(w, other, q, k)
+    assert (q > 0).all() and (k > 0).all()
+    first = None
+    for _ in range(4):
+        one, two = (torch.ones(hd, device=DEV) for _ in range(2))
+        run(w, other, one, one)
+        w.main_grad = two
+        run(w, w, None, None)                                  # the buffer of one weight that serves both
+        del w.main_grad
+        assert torch.equal(one, two) and (first is None or torch.equal(one, first))
+        first = one
+    # both are sums of the same positive numbers, of less than 64 steps in fp32 for each thread and 32 behind them
+    torch.testing.assert_close(first, 1 + q + k, rtol=96 * 2.0 ** -24, atol=0)
+    (dw,) = torch.autograd.grad(ops.qk_norm_rope(x, w, w, cos, sin, H, KV, hd, positions=at), w, dy)
+    torch.testing.assert_close(dw.float(), q + k, rtol=3 * U, atol=0)          # each of two gradients rounded, and their sum
+    assert int(OF.status_word(DEV).item()) == 0
