@@ -1587,8 +1587,7 @@ struct AttnDocsParams {
   float scale_log2;
   unsigned int* status;
   const int* starts;      // [B, S]
-  int* blocks;            // [B, nQ], or null: takes the least start of a row in the query block that sees anything (INT_MAX: none does);
-                          // behind it two counters for the backward kernels, zeroed here
+  int* blocks;            // [B, nQ], or null: takes the least start of a row in the query block that sees anything (INT_MAX: none does)
 };
 
 // A mask of 64 columns as bits, tested one by one: 1.2 instructions a column, where two comparisons and a choice are 3.
@@ -1675,7 +1674,6 @@ attn_docs_fwd_kernel(const __grid_constant__ AttnDocsParams p) {
   const int least = min(min(s_least[0], s_least[1]), min(s_least[2], s_least[3]));
   const int nb = least == INT_MAX ? 0 : qi - least / BKV + 1;      // key blocks qi, qi - 1, ..
   if (p.blocks && h == 0 && threadIdx.x == 0) p.blocks[(long long)b * nQ + qi] = least;
-  if (p.blocks && blockIdx.x == 0 && threadIdx.x < 2) p.blocks[(long long)p.B * nQ + threadIdx.x] = 0;
   const uint32_t tmem_base = s_tmem_base;
   // S columns 0..127, O from column 128; P over S at DH = 128, at 64 in the 64 columns that O leaves, so that the next block's S is
   // computed as soon as the softmax warps hold this one's (AHEAD)
@@ -1905,7 +1903,7 @@ int launch_docs_fwd(const void* qkv, const int* starts, void* out, float* lse, i
 }  // namespace
 
 // tplr_attention_fwd within documents: row s of sequence b sees the keys max(starts[b * S + s], 0) .. s; one whose start lies behind it
-// sees nothing, and its output is zero.  starts: [B, S] int32, any values.  blocks: B * ceil(S / 128) + 2 int32 for the
+// sees nothing, and its output is zero.  starts: [B, S] int32, any values.  blocks: B * ceil(S / 128) int32 for the
 // backward pass, or null.
 TPLR_API int tplr_attention_docs_fwd(const void* qkv, const int* starts, void* out, float* lse, int* blocks, int B, int S, int H, int KV,
                                      int head_dim, long long ld_qkv, long long ld_o, float scale, unsigned int* status, void* stream) {
@@ -1978,7 +1976,7 @@ struct AttnDocsBwdParams {
   float* delta;           // [B, H, S]
   const int* starts;
   const int* blocks;
-  int* next;              // tiles taken beyond the first of every CTA; zero, and zero again at the end
+  int* next;              // tiles taken beyond the first of every CTA, from zero; null where every CTA has one
   int B, S, H, KV, tiles;
   int split;              // tiles that share a group's query heads; > 1: each stores its part of dK and dV in fp32
   float scale, scale_log2;
@@ -2083,16 +2081,17 @@ __device__ __forceinline__ bool give_tile(DocsBwdShared& sh, int k, int lane, vo
   }
   return true;
 }
-// The tile behind this one.  Every CTA asks until it is told of none, so there are as many questions as tiles; the last one leaves the
-// counter as it was.
+// The tile behind this one.
 __device__ __forceinline__ int next_tile(const AttnDocsBwdParams& p, int lane) {
-  int n = 0;
-  if (lane == 0) {
-    n = atomicAdd(p.next, 1);
-    if (n == p.tiles - 1) *p.next = 0;
-    n += (int)gridDim.x;
-  }
+  int n = p.tiles;
+  if (p.next && lane == 0) n = (int)gridDim.x + atomicAdd(p.next, 1);
   return __shfl_sync(0xffffffffu, n, 0);
+}
+// The two counters belong to one call: walks of one graph may overlap, and one whose wait ran out leaves them anywhere.
+__global__ void attn_docs_counters_kernel(int* next) {
+  grid_wait();
+  grid_release();
+  if (threadIdx.x < 2) next[threadIdx.x] = 0;
 }
 // offsets of a 16-wide k step in a tile of 128 rows, in 16-byte units: along the 128-byte rows, and along the rows of the tile
 __device__ __forceinline__ constexpr uint32_t koff(int kk) { return (uint32_t)(kk >> 2) * (128u * 128u / 16u) + (uint32_t)(kk & 3) * 2u; }
@@ -2754,8 +2753,8 @@ int docs_split(int B, int S, int H, int KV) {
 }
 
 template <int DH>
-int launch_docs_bwd(const void* qkv, const int* starts, int* blocks, const void* out, const void* dout, const float* lse, float* delta,
-                    float* part, void* dqkv, int B, int S, int H, int KV, long long ld_qkv, float scale, unsigned int* status, cudaStream_t st) {
+int launch_docs_bwd(const void* qkv, const int* starts, const int* blocks, const void* out, const void* dout, const float* lse, float* delta,
+                    int* next, float* part, void* dqkv, int B, int S, int H, int KV, long long ld_qkv, float scale, unsigned int* status, cudaStream_t st) {
   AttnDocsBwdParams p = {};
   const int C = (H + 2 * KV) * DH, split = docs_split(B, S, H, KV), kv_cols = 2 * KV * DH;
   if ((long long)((S + BKV - 1) / BKV) * H * B > 0x7fffffff / 2) return -201;
@@ -2769,11 +2768,12 @@ int launch_docs_bwd(const void* qkv, const int* starts, int* blocks, const void*
   constexpr int SMEM = docs_bwd_smem<DH>();
   cudaError_t e = cudaFuncSetAttribute(attn_docs_dq_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_docs_dkv_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-  p.tiles = n * H * B;
-  p.next = blocks + (long long)B * n;
+  p.tiles = n * H * B;                                     // as many as dK and dV have, or more
+  p.next = p.tiles > sms ? next : nullptr;
+  if (e == cudaSuccess && p.next) e = launch_pdl(attn_docs_counters_kernel, 1, 32, 0, st, p.next);
   if (e == cudaSuccess) e = launch_pdl(attn_docs_dq_kernel<DH>, (unsigned)(p.tiles < sms ? p.tiles : sms), DQ_THREADS, SMEM, st, p);
   p.tiles = n * KV * B * split;
-  ++p.next;
+  if (p.next) ++p.next;
   if (e == cudaSuccess) e = launch_pdl(attn_docs_dkv_kernel<DH>, (unsigned)(p.tiles < sms ? p.tiles : sms), DKV_THREADS, SMEM, st, p);
   if (e != cudaSuccess || split == 1) return (int)e;
   // the parts' sums into the key and value columns; no query columns here
@@ -2789,17 +2789,17 @@ TPLR_API int tplr_attention_docs_bwd_scratch_cols(int B, int S, int H, int KV, i
   return split > 1 ? 2 * KV * split * head_dim : 0;
 }
 
-// Gradient of tplr_attention_docs_fwd, whose starts, blocks (left as they are) and lse it takes: dqkv [B, S, (H + 2 KV) * head_dim] dense.
-// out and dout dense; dqkv and part on 32-byte boundaries; delta: [B, H, S] fp32 scratch; part: B * S *
-// tplr_attention_docs_bwd_scratch_cols fp32 elements, contents irrelevant.
-TPLR_API int tplr_attention_docs_bwd(const void* qkv, const int* starts, int* blocks, const void* out, const void* dout,
-                                     const float* lse, float* delta, float* part, void* dqkv, int B, int S, int H, int KV, int head_dim,
+// Gradient of tplr_attention_docs_fwd, whose starts, blocks and lse it takes: dqkv [B, S, (H + 2 KV) * head_dim] dense.
+// out and dout dense; dqkv and part on 32-byte boundaries; scratch, contents irrelevant: delta [B, H, S] fp32, next two int32, part B * S *
+// tplr_attention_docs_bwd_scratch_cols fp32.
+TPLR_API int tplr_attention_docs_bwd(const void* qkv, const int* starts, const int* blocks, const void* out, const void* dout,
+                                     const float* lse, float* delta, int* next, float* part, void* dqkv, int B, int S, int H, int KV, int head_dim,
                                      long long ld_qkv, float scale, unsigned int* status, void* stream) {
   TPLR_ENTER();
   if (B <= 0 || S <= 0) return 0;
-  if ((head_dim != 128 && head_dim != 64) || KV <= 0 || H % KV || (ld_qkv % 8) || !starts || !blocks ||
+  if ((head_dim != 128 && head_dim != 64) || KV <= 0 || H % KV || (ld_qkv % 8) || !starts || !blocks || !next ||
       (((uintptr_t)qkv | (uintptr_t)dout | (uintptr_t)out) & 15) || (((uintptr_t)dqkv | (uintptr_t)part) & 31))
     return -201;
   auto run = head_dim == 128 ? launch_docs_bwd<128> : launch_docs_bwd<64>;
-  return run(qkv, starts, blocks, out, dout, lse, delta, part, dqkv, B, S, H, KV, ld_qkv, scale, status, (cudaStream_t)stream);
+  return run(qkv, starts, blocks, out, dout, lse, delta, next, part, dqkv, B, S, H, KV, ld_qkv, scale, status, (cudaStream_t)stream);
 }

@@ -59,8 +59,8 @@ int tplr_gemm2_swiglu_bwd_saved8(const void* dY, const void* W2, const void* Q, 
 int tplr_attention_docs_fwd(const void* qkv, const int* starts, void* out, float* lse, int* blocks, int B, int S, int H, int KV, int head_dim,
                             long long ld_qkv, long long ld_o, float scale, unsigned int* status, void* stream);
 int tplr_attention_docs_bwd_scratch_cols(int B, int S, int H, int KV, int head_dim);
-int tplr_attention_docs_bwd(const void* qkv, const int* starts, int* blocks, const void* out, const void* dout, const float* lse, float* delta,
-                            float* part, void* dqkv, int B, int S, int H, int KV, int head_dim, long long ld_qkv, float scale,
+int tplr_attention_docs_bwd(const void* qkv, const int* starts, const int* blocks, const void* out, const void* dout, const float* lse, float* delta,
+                            int* next, float* part, void* dqkv, int B, int S, int H, int KV, int head_dim, long long ld_qkv, float scale,
                             unsigned int* status, void* stream);
 int tplr_qk_norm_rope(const void* x, long long ldx, void* y, const void* wq, const void* wk, const float* cosb, const float* sinb,
                       const int* pos, long long tokens, int S, int table_rows, int n_q, int n_k, int hd, float eps, unsigned int* status,

@@ -620,7 +620,7 @@ std::tuple<Tensor, Tensor, Tensor> docs_forward(const Tensor& qkv, ll ld, const 
   Tensor out = bf16({B, S, heads * hd}, qkv), lse, blocks;
   if (keep) {
     lse = f32({B, heads, S}, qkv);
-    blocks = at::empty({B * ((S + 127) / 128) + 2}, starts.options());
+    blocks = at::empty({B * ((S + 127) / 128)}, starts.options());
   }
   check(E.docs_fwd(qkv.data_ptr(), starts.data_ptr<int>(), out.data_ptr(), ptr32(lse), keep ? blocks.data_ptr<int>() : nullptr, (int)B, (int)S,
                    (int)heads, (int)kv, (int)hd, ld, heads * hd, (float)std::pow((double)hd, -0.5), word(status), stream()),
@@ -644,10 +644,10 @@ struct AttentionDocuments : Function<AttentionDocuments> {
     const auto d = ctx->saved_data["dims"].toIntVector();
     const ll B = qkv.size(0), S = qkv.size(1), heads = d[0], kv = d[1], hd = d[2];
     const Tensor dout = dense(g[0]);
-    Tensor dqkv = bf16({B, S, qkv.size(2)}, qkv), delta = f32({B, heads, S}, qkv), part;
+    Tensor dqkv = bf16({B, S, qkv.size(2)}, qkv), delta = f32({B, heads, S}, qkv), next = at::empty({2}, starts.options()), part;
     if (const ll cols = E.docs_bwd_scratch_cols((int)B, (int)S, (int)heads, (int)kv, (int)hd)) part = f32({B * S * cols}, qkv);
     check(E.docs_bwd(qkv.data_ptr(), starts.data_ptr<int>(), blocks.data_ptr<int>(), out.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(),
-                     delta.data_ptr<float>(), ptr32(part), dqkv.data_ptr(), (int)B, (int)S, (int)heads, (int)kv, (int)hd, d[3],
+                     delta.data_ptr<float>(), next.data_ptr<int>(), ptr32(part), dqkv.data_ptr(), (int)B, (int)S, (int)heads, (int)kv, (int)hd, d[3],
                      (float)std::pow((double)hd, -0.5), word(aside(ctx, "status")), stream()),
           "attention_docs_bwd");
     return {dqkv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};

@@ -98,9 +98,10 @@ class _AttentionDocuments(torch.autograd.Function):
             cols = native.lib().tplr_attention_docs_bwd_scratch_cols(B, S, n_heads, n_kv, hd)
             part = torch.empty(B * S * cols, dtype=torch.float32, device=qkv.device) if cols else None
             delta = torch.empty(B, n_heads, S, dtype=torch.float32, device=qkv.device)
+            following = torch.empty(2, dtype=torch.int32, device=qkv.device)
             native.check(native.lib().tplr_attention_docs_bwd(
                 qkv.data_ptr(), starts.data_ptr(), blocks.data_ptr(), out.data_ptr(), do.data_ptr(), lse.data_ptr(), delta.data_ptr(),
-                native.ptr(part), dqkv.data_ptr(), B, S, n_heads, n_kv, hd, ld, hd ** -0.5, OF.status_word(qkv.device).data_ptr(),
+                following.data_ptr(), native.ptr(part), dqkv.data_ptr(), B, S, n_heads, n_kv, hd, ld, hd ** -0.5, OF.status_word(qkv.device).data_ptr(),
                 native.stream_ptr()), "attention_docs_bwd")
         return dqkv, None, None, None, None
 
@@ -110,7 +111,7 @@ def _attention_documents(qkv, ld, starts, n_heads, n_kv, hd, keep):
     with _on(qkv):
         out = torch.empty(B, S, n_heads * hd, dtype=qkv.dtype, device=qkv.device)
         lse = torch.empty(B, n_heads, S, dtype=torch.float32, device=qkv.device) if keep else None
-        blocks = torch.empty(B * -(-S // 128) + 2, dtype=torch.int32, device=qkv.device) if keep else None
+        blocks = torch.empty(B * -(-S // 128), dtype=torch.int32, device=qkv.device) if keep else None
         native.check(native.lib().tplr_attention_docs_fwd(
             qkv.data_ptr(), starts.data_ptr(), out.data_ptr(), native.ptr(lse), native.ptr(blocks), B, S, n_heads, n_kv, hd, ld, n_heads * hd,
             hd ** -0.5, OF.status_word(qkv.device).data_ptr(), native.stream_ptr()), "attention_docs_fwd")

@@ -146,7 +146,7 @@ def _declare(L: ctypes.CDLL) -> None:
         "tplr_attention_fwd": [vp, vp, vp, i, i, i, i, i, ll, ll, f, vp, vp],
         "tplr_attention_bwd": [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, ll, ll, f, vp, vp],
         "tplr_attention_docs_fwd": [vp, vp, vp, vp, vp, i, i, i, i, i, ll, ll, f, vp, vp],
-        "tplr_attention_docs_bwd": [vp, vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, ll, f, vp, vp],
+        "tplr_attention_docs_bwd": [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, ll, f, vp, vp],
         "tplr_attention_docs_bwd_scratch_cols": [i, i, i, i, i],
         "tplr_qk_norm_rope": [vp, ll, vp, vp, vp, vp, vp, vp, ll, i, i, i, i, i, f, vp, vp],
         "tplr_qk_norm_rope_parts": [ll, i, i, i],

@@ -97,3 +97,46 @@ def test_one_buffer_for_the_gradients_of_both_weights(B, S, H, KV, hd, host, mon
     (dw,) = torch.autograd.grad(ops.qk_norm_rope(x, w, w, cos, sin, H, KV, hd, positions=at), w, dy)
     torch.testing.assert_close(dw.float(), q + k, rtol=3 * U, atol=0)          # each of two gradients rounded, and their sum
     assert int(OF.status_word(DEV).item()) == 0
+
+
+# ------------------------------------------------------------------------------------------ walks of one graph at the same time
+@pytest.mark.gpu
+@pytest.mark.parametrize("host", [True, False])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_walks_of_one_graph_that_overlap(hd, host, monkeypatch):
+    """One kept graph of the attention walked on two streams at once, and by two captured backward passes replayed side by side: more tiles
+    than CTAs, which each walk hands out by itself."""
+    if not host:
+        monkeypatch.setattr(native, "host", lambda: None)
+    B, S, H, KV = 6, 900, 12, 4
+    qkv = normal(1, B, S, (H + 2 * KV) * hd, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    starts = ops.document_starts(torch.randint(0, 200, (B, S), generator=torch.Generator().manual_seed(2)), 0).to(DEV)
+    douts = [normal(3 + i, B, S, H * hd, device=DEV, dtype=torch.bfloat16) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(streams[0]):
+        out = ops.attention_documents(qkv, starts, H, KV, hd)
+        walk = lambda d: out.grad_fn(d) if callable(out.grad_fn) else out.grad_fn.apply(d)[0]  # noqa: E731
+        want = [walk(d) for d in douts]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for s, d in zip(streams, douts):
+            with torch.cuda.stream(s):
+                got.append(walk(d))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert torch.equal(g, w)
+    graphs, held = [], []
+    for s, d in zip(streams, douts):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=s):
+            held.append(walk(d))
+    for _ in range(20):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for g, w in zip(held, want):
+            assert torch.equal(g, w)
+    assert int(OF.status_word(DEV).item()) == 0
