@@ -13,6 +13,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from . import functional as OF
 from . import native
@@ -35,6 +36,16 @@ def _same_device(what: str, t: torch.Tensor, **others) -> None:
     for name, o in others.items():
         if o is not None and o.device != t.device:
             raise ValueError(f"{what}: {name} is on {o.device}, the rows are on {t.device}")
+
+
+def _has_tangent(*ts: torch.Tensor) -> bool:
+    """A forward-mode derivative is asked for.  The formulas carry it; from the kernels an output would come without one, and read as
+    a derivative of zero."""
+    return fwAD._current_level >= 0 and any(t.is_floating_point() and fwAD.unpack_dual(t).tangent is not None for t in ts)
+
+
+def _no_forward_mode(what: str) -> NotImplementedError:
+    return NotImplementedError(f"{what}: the kernels have no forward-mode derivative")
 
 
 def _fitting_buffer(what: str, name: str, w: torch.Tensor, main_grad: torch.Tensor) -> None:
@@ -138,8 +149,9 @@ def attention_documents(qkv: torch.Tensor, starts: torch.Tensor, n_heads: int, n
     Every row has to hold finite numbers, one that nothing sees too, and so has the gradient: the rows of a block of 128 meet in the
     same products, where a weight of zero times an infinity is not zero.  The kernels (bf16, heads of 64 or 128) add nothing
     into memory: results and gradients have the same bits on every run."""
+    tangent = _has_tangent(qkv)
     # operands that the kernels take as they are need no further look
-    if qkv.is_cuda and (host := native.host()) and (out := host.attention_documents(qkv, starts, n_heads, n_kv, hd, _word(qkv))) is not None:
+    if qkv.is_cuda and not tangent and (host := native.host()) and (out := host.attention_documents(qkv, starts, n_heads, n_kv, hd, _word(qkv))) is not None:
         return out
     _heads("attention_documents", qkv, n_heads, n_kv, hd)
     B, S, C = qkv.shape
@@ -148,6 +160,8 @@ def attention_documents(qkv: torch.Tensor, starts: torch.Tensor, n_heads: int, n
     _same_device("attention_documents", qkv, starts=starts)
     if not (qkv.is_cuda and qkv.dtype == torch.bfloat16 and hd in OF.OWN_HEAD_DIMS) or B * S == 0:
         return _attention_documents_torch(qkv, starts, n_heads, n_kv, hd)
+    if tangent:
+        raise _no_forward_mode("attention_documents")
     if starts.dtype != torch.int32:
         starts = starts.clamp(0, 2 ** 31 - 1).to(torch.int32) if starts.dtype == torch.int64 else starts.to(torch.int32)
     starts = starts.contiguous()
@@ -251,7 +265,8 @@ def qk_norm_rope(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, cos: tor
         if torch.is_grad_enabled() and (qkv.requires_grad or wq.requires_grad or wk.requires_grad):
             raise ValueError("qk_norm_rope: the weights' gradients are buffers here, not shards of other ranks")
         main_grad_q = main_grad_k = None
-    if qkv.is_cuda and (host := native.host()) and (y := host.qk_norm_rope(qkv, wq, wk, cos, sin, positions, n_heads, n_kv, hd, eps, main_grad_q,
+    tangent = _has_tangent(qkv, wq, wk, cos, sin)
+    if qkv.is_cuda and not tangent and (host := native.host()) and (y := host.qk_norm_rope(qkv, wq, wk, cos, sin, positions, n_heads, n_kv, hd, eps, main_grad_q,
                                                                            main_grad_k, _word(qkv))) is not None:
         return y
     _heads("qk_norm_rope", qkv, n_heads, n_kv, hd)
@@ -278,6 +293,8 @@ def qk_norm_rope(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, cos: tor
         if main_grad_k is not None and wk.requires_grad:
             wk = _AddMainGrad.apply(wk, main_grad_k)
         return _qk_norm_rope_torch(qkv, wq, wk, cos, sin, positions, n_heads, n_kv, hd, eps)
+    if tangent:
+        raise _no_forward_mode("qk_norm_rope")
     cos, sin = OF._dense(cos), OF._dense(sin)
     if positions is not None:
         positions = positions.clamp(-1, 2 ** 31 - 1).to(torch.int32).contiguous() if positions.dtype == torch.int64 else positions.contiguous()
@@ -478,8 +495,8 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
         if torch.is_grad_enabled() and w.requires_grad:
             raise ValueError("linear_cross_entropy: the weight's gradient is a buffer here, not shards of other ranks")
         main_grad = None
-    mean, ignore_index = reduction == "mean", int(ignore_index)
-    host = native.host() if x.is_cuda and (mean or reduction == "none") and OF.gemm_backend() == "tcgen05_2sm" else None
+    mean, ignore_index, tangent = reduction == "mean", int(ignore_index), _has_tangent(x, w)
+    host = native.host() if x.is_cuda and not tangent and (mean or reduction == "none") and OF.gemm_backend() == "tcgen05_2sm" else None
     if host and (out := host.linear_cross_entropy(x, w, labels, grad_scale, ignore_index, main_grad, mean, CHUNK_BYTES, _word(x))) is not None:
         return out
     if reduction not in ("mean", "none"):
@@ -499,6 +516,8 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
             w = _AddMainGrad.apply(w, main_grad)
         out = _linear_cross_entropy_torch(x, w, flat, float(grad_scale), ignore_index, reduction)
         return out if mean else out.view(labels.shape)
+    if tangent:
+        raise _no_forward_mode("linear_cross_entropy")
     if host:
         with _on(x):
             out = host.linear_cross_entropy(x, w, flat.view(labels.shape), grad_scale, ignore_index, main_grad, mean, CHUNK_BYTES, _word(x))

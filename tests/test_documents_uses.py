@@ -140,3 +140,59 @@ def test_walks_of_one_graph_that_overlap(hd, host, monkeypatch):
         for g, w in zip(held, want):
             assert torch.equal(g, w)
     assert int(OF.status_word(DEV).item()) == 0
+
+
+# ------------------------------------------------------------------------------------------ forward mode
+def calls(device, dtype):
+    """(operator of one operand, the operand) for every operand that has a derivative."""
+    H, KV, hd, B, S, V = 4, 2, 64, 2, 70, 300
+    t = lambda seed, *shape: normal(seed, *shape, std=0.5, device=device, dtype=dtype)  # noqa: E731
+    qkv, wq, wk, x, w = t(1, B, S, (H + 2 * KV) * hd), t(2, hd), t(3, hd), t(4, B, S, 128), t(5, V, 128)
+    starts = ops.document_starts(torch.randint(0, 9, (B, S), generator=torch.Generator().manual_seed(6)), 0).to(device)
+    labels = torch.randint(0, V, (B, S), generator=torch.Generator().manual_seed(7)).to(device)
+    cos, sin = ops.rope_tables(S, hd, device=device)
+    norm = lambda **k: ops.qk_norm_rope(**{**dict(qkv=qkv, wq=wq, wk=wk, cos=cos, sin=sin, n_heads=H, n_kv=KV, hd=hd), **k})  # noqa: E731
+    return {"attention": (lambda a: ops.attention_documents(a, starts, H, KV, hd), qkv),
+            "norm of qkv": (lambda a: norm(qkv=a), qkv), "norm, wq": (lambda a: norm(wq=a), wq), "norm, wk": (lambda a: norm(wk=a), wk),
+            "norm, tables": (lambda a: norm(cos=a), cos),
+            "loss of x": (lambda a: ops.linear_cross_entropy(a, w, labels), x), "loss, w": (lambda a: ops.linear_cross_entropy(x, a, labels), w),
+            "losses of x": (lambda a: ops.linear_cross_entropy(a, w, labels, reduction="none"), x),
+            "losses, w": (lambda a: ops.linear_cross_entropy(x, a, labels, reduction="none"), w)}
+
+
+NAMES = ["attention", "norm of qkv", "norm, wq", "norm, wk", "norm, tables", "loss of x", "loss, w", "losses of x", "losses, w"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_the_formulas_carry_a_tangent(name):
+    op, a = calls("cpu", torch.float32)[name]
+    v = normal(8, *a.shape)
+    with fwAD.dual_level():
+        tangent = fwAD.unpack_dual(op(fwAD.make_dual(a, v))).tangent
+    a = a.clone().requires_grad_()
+    out = op(a)
+    d = normal(9, *out.shape)
+    (g,) = torch.autograd.grad(out, a, d)
+    # <d, J v> = <J^T d, v>: two sums in fp32, each off relative to the sizes of its terms
+    torch.testing.assert_close((tangent * d).sum(), (g * v).sum(), rtol=1e-3, atol=1e-5 * float((tangent * d).abs().sum() + (g * v).abs().sum()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("host", [True, False])
+@pytest.mark.parametrize("name", NAMES)
+def test_the_kernels_refuse_a_tangent(name, host, monkeypatch):
+    """A result without a tangent would read as a derivative of zero."""
+    if not host:
+        monkeypatch.setattr(native, "host", lambda: None)
+    op, a = calls(DEV, torch.bfloat16)[name]
+    plain = op(a)
+    with fwAD.dual_level():
+        dual = fwAD.make_dual(a, torch.ones_like(a))
+        with pytest.raises(NotImplementedError, match="forward"):
+            op(dual)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward"):
+            op(dual)
+        assert torch.equal(op(a), plain)                       # inside a level, of plain tensors
+    other, b = calls(DEV, torch.float32)[name]                 # no kernel's type: the formulas
+    with fwAD.dual_level():
+        assert fwAD.unpack_dual(other(fwAD.make_dual(b, torch.ones_like(b)))).tangent is not None
