@@ -9,6 +9,7 @@
 // Tensors are saved as saved variables only; the gradient buffers of the flat store are held by reference as there.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -838,8 +839,9 @@ struct LinearCrossEntropy : Function<LinearCrossEntropy> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     auto s = ctx->get_saved_variables();
     const Tensor by = g[0].to(at::kFloat);
-    // a graph that is not kept lets go of what it saved behind this call, and cannot be walked again
-    const bool ours = !torch::autograd::get_current_graph_task_keep_graph();
+    // A graph that is not kept lets go of what it saved behind this call, and cannot be walked again; a captured call can, by every replay.
+    const bool ours = !torch::autograd::get_current_graph_task_keep_graph() &&
+                      c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None;
     Tensor dx, dw;
     if (s[0].defined()) dx = scaled_by(s[0], by, Tensor(), ctx->saved_data["shape"].toIntVector(), ours);
     if (s[1].defined()) dw = scaled_by(s[1], by, aside(ctx, "buffer"), s[1].sizes(), ours);

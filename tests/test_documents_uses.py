@@ -196,3 +196,32 @@ def test_the_kernels_refuse_a_tangent(name, host, monkeypatch):
     other, b = calls(DEV, torch.float32)[name]                 # no kernel's type: the formulas
     with fwAD.dual_level():
         assert fwAD.unpack_dual(other(fwAD.make_dual(b, torch.ones_like(b)))).tangent is not None
+
+
+# ------------------------------------------------------------------------------------------ graphs walked more than once
+@pytest.mark.gpu
+@pytest.mark.parametrize("chunk", [OD.CHUNK_BYTES, 2 * 500 * 300])          # dw in bf16, of several runs in fp32
+def test_a_captured_backward_pass_replayed_twice(chunk, monkeypatch):
+    """The forward pass in one CUDA graph, the backward pass in another, as graphed callables have them: every replay of the second gives the
+    gradient of the first's last replay."""
+    monkeypatch.setattr(OD, "CHUNK_BYTES", chunk)
+    x, w = (normal(i, n, 64, device=DEV, dtype=torch.bfloat16).requires_grad_() for i, n in ((1, 600), (2, 500)))
+    labels = torch.randint(0, 500, (600,), generator=torch.Generator().manual_seed(3)).to(DEV)
+    by = torch.full((), 0.5, device=DEV)
+    want = [t.clone() for t in torch.autograd.grad(ops.linear_cross_entropy(x, w, labels), (x, w), by)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(ops.linear_cross_entropy(x, w, labels), (x, w), by)
+    side.synchronize()
+    forward, backward = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(forward, stream=side):
+        loss = ops.linear_cross_entropy(x, w, labels)
+    with torch.cuda.graph(backward, stream=side, pool=forward.pool()):
+        got = torch.autograd.grad(loss, (x, w), by)
+    del loss
+    for _ in range(2):
+        forward.replay()
+        for _ in range(3):
+            backward.replay()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
