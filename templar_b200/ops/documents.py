@@ -200,7 +200,7 @@ class _QKNormRope(torch.autograd.Function):
             for w, mg, needed in ((wq, mg_q, ctx.needs_input_grad[1]), (wk, mg_k, ctx.needs_input_grad[2])):
                 direct = mg is not None and mg.dtype == torch.float32 and mg.is_contiguous() and mg.numel() == hd
                 add.append(mg if direct else None)
-                out.append(None if direct or not (needed or mg is not None) else torch.empty(hd, dtype=w.dtype, device=w.device))
+                out.append(None if direct or not (needed or mg is not None) else torch.empty(w.shape, dtype=w.dtype, device=w.device))
                 later.append(mg if mg is not None and not direct else None)
             native.check(L.tplr_qk_norm_rope_bwd(
                 d.data_ptr(), ldd, rows.data_ptr(), ld, wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), native.ptr(positions),

@@ -225,3 +225,20 @@ def test_a_captured_backward_pass_replayed_twice(chunk, monkeypatch):
         for _ in range(3):
             backward.replay()
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------------------------ weights of one row
+@pytest.mark.gpu
+@pytest.mark.parametrize("host", [True, False])
+def test_norm_weights_may_have_any_shape_of_their_numbers(host, monkeypatch):
+    if not host:
+        monkeypatch.setattr(native, "host", lambda: None)
+    H, KV, hd, B, S = 4, 2, 64, 2, 70
+    qkv, wq, wk = (normal(i, *s, device=DEV, dtype=torch.bfloat16).requires_grad_() for i, s in ((1, (B, S, (H + 2 * KV) * hd)), (2, (hd,)), (3, (hd,))))
+    cos, sin = ops.rope_tables(S, hd, device=DEV)
+    run = lambda a, b: torch.autograd.grad(ops.qk_norm_rope(qkv, a, b, cos, sin, H, KV, hd).float().square().sum(), (qkv, a, b))  # noqa: E731
+    want = run(wq, wk)
+    row, grid = wq.detach().view(1, hd).requires_grad_(), wk.detach().view(8, 8).requires_grad_()
+    got = run(row, grid)
+    assert got[1].shape == (1, hd) and got[2].shape == (8, 8)
+    assert all(torch.equal(a.flatten(), b.flatten()) for a, b in zip(got, want))
