@@ -75,8 +75,8 @@ int tplr_gemm2_softmax(const void* X, const void* W, void* P, const long long* l
 int tplr_gemm2_rows(const void* A, const void* B, void* C, float* ws, const float* row_scale, int M, int N, int K, long long lda,
                     long long ldb, long long ldc, unsigned int* status, void* stream);
 int tplr_vocab_count(const long long* labels, long long T, long long ignore, int V, int* n_valid, unsigned int* status, void* stream);
-int tplr_vocab_losses(const float* stats, const float* target, const long long* labels, float* losses, long long T, int parts, int V, long long ignore,
-                      void* stream);
+int tplr_vocab_losses(const float* stats, const float* target, const long long* labels, float* losses, long long T, int parts, int columns, int V,
+                      long long ignore, void* stream);
 int tplr_vocab_rows(void* E, long long ld, const float* stats, const float* target, const long long* labels, const float* row_grad,
                     const int* n_valid, float grad_scale, const void* x, long long ldx, void* xs, long long ldxs, float* row_scale, float* losses, long long T,
                     int parts, int columns, int V, int D, long long ignore, void* stream);

@@ -97,8 +97,8 @@ struct Gemm2Params {
   float* q8_scale;
   long long q8_ld;
   // softmax over the columns in pieces (EPI 12, 13): a piece is half a tile's columns, sm_parts pieces a row; (reference, sum of
-  // exp(logit - it)) goes to sm_stats[row * sm_parts + piece], the logit of the row's label to sm_target[row].  EPI 15 has the
-  // product transposed: rows are the softmax's columns here, a piece 32 of them
+  // 2^(logit log2 e - it) without the row's label) goes to sm_stats[row * sm_parts + piece], that exponent of the label to
+  // sm_target[row].  EPI 15 has the product transposed: rows are the softmax's columns here, a piece 32 of them
   const long long* sm_labels;
   float2* sm_stats;
   float* sm_target;
@@ -958,9 +958,17 @@ __device__ __forceinline__ bool epilogue_swiglu_bwd_q8(const Gemm2Params& p, uin
 // instead took 197 us where this product takes 693 (8192 x 2048 x 32000).  Within SM_NEAR the sums stay far inside fp32:
 // exp(40) = 2e17, and a weight is only lost where it is below 1e-20 of the row's sum.
 //
+// Exponents are of 2, and references whole, so that one fused multiply-add rounds a weight's exponent once, and pieces of other references
+// are brought together by powers of 2.  The label's column is in no sum: 1 - p of the label, which its gradient is and a loss near zero, is
+// the others' sum over that of all, where the difference of a rounded p and 1 would have no digits left once the model is sure.
+//
 // One B200: 4096 x 4096 x 128256 without the weights 2626 us, 1640 TFLOP/s, the tensor pipe 98 % busy (the plain product's own time); 1111 x 1000 x
 // 50257 with them 126 us, 112 MB stored, the pipe 48 %: 13 % of its rows are the last tile's, and 16 k blocks do not cover an epilogue.
-constexpr float SM_NEAR = 40.f;
+constexpr float SM_NEAR = 40.f, LOG2E = 1.4426950408889634f;
+// A piece's reference by its largest logit
+__device__ __forceinline__ float sm_reference(float top) {
+  return fabsf(top) <= SM_NEAR || top == -INFINITY ? 0.f : rintf(top * LOG2E);
+}
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -977,7 +985,7 @@ __device__ __forceinline__ void epilogue_softmax(const Gemm2Params& p, uint32_t 
   const bool live = row0 + lane < p.M;
   const long long label = live ? p.sm_labels[row0 + lane] - c0 : -1;
   const int mine = label >= 0 && label < width ? (int)label : -1;
-  float top = -INFINITY, target = 0.f;
+  float top = -INFINITY;
 #pragma unroll 1
   for (int c = 0; c < width; c += 32) {
     uint32_t r[32];
@@ -986,19 +994,13 @@ __device__ __forceinline__ void epilogue_softmax(const Gemm2Params& p, uint32_t 
 #pragma unroll
       for (int e = 0; e < 32; ++e) if (c + e >= width) r[e] = 0xff800000u;
     }
-    if (__any_sync(0xffffffffu, (mine >> 5) == (c >> 5))) {
-#pragma unroll
-      for (int e = 0; e < 32; ++e) if (c + e == mine) target = __uint_as_float(r[e]);
-    }
     float top2 = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 32; e += 2) { top = fmaxf(top, __uint_as_float(r[e])); top2 = fmaxf(top2, __uint_as_float(r[e + 1])); }
     top = fmaxf(top, top2);
   }
-  constexpr float LOG2E = 1.4426950408889634f;
-  const float ref = fabsf(top) <= SM_NEAR || top == -INFINITY ? 0.f : top;
-  const float neg = -ref * LOG2E;
-  float sum = 0.f, sum2 = 0.f;
+  const float ref = sm_reference(top);
+  float sum = 0.f, sum2 = 0.f, target = 0.f;
 #pragma unroll 1
   for (int c = 0; c < width; c += 64) {
     if (STORE) {
@@ -1011,11 +1013,17 @@ __device__ __forceinline__ void epilogue_softmax(const Gemm2Params& p, uint32_t 
       float v[32];
       tmem_ld32(acc + c + hh * 32, r);
 #pragma unroll
-      for (int e = 0; e < 32; ++e) v[e] = ex2(fmaf(__uint_as_float(r[e]), LOG2E, neg));
+      for (int e = 0; e < 32; ++e) v[e] = fmaf(__uint_as_float(r[e]), LOG2E, -ref);
+      if (__any_sync(0xffffffffu, (mine >> 5) == ((c + hh * 32) >> 5))) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) if (c + hh * 32 + e == mine) { target = v[e]; v[e] = -INFINITY; }
+      }
       if (c + hh * 32 + 32 > width) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) if (c + hh * 32 + e >= width) v[e] = 0.f;
+        for (int e = 0; e < 32; ++e) if (c + hh * 32 + e >= width) v[e] = -INFINITY;
       }
+#pragma unroll
+      for (int e = 0; e < 32; ++e) v[e] = ex2(v[e]);
 #pragma unroll
       for (int e = 0; e < 32; e += 2) { sum += v[e]; sum2 += v[e + 1]; }
       if (STORE) box_half(buf, lane, hh, v);
@@ -1040,7 +1048,6 @@ __device__ __forceinline__ void epilogue_softmax_few(const Gemm2Params& p, uint3
   if (row0 >= p.M) return;                           // warp-uniform
   const uint32_t acc = tmem_acc + ((uint32_t)(quad * 32) << 16);
   const bool live = row0 + lane < p.M;
-  constexpr float LOG2E = 1.4426950408889634f;
 #pragma unroll 1
   for (int c = turn * half; c < (turn + 1) * half && c < p.N; c += 16) {
     uint32_t r[16];
@@ -1049,22 +1056,24 @@ __device__ __forceinline__ void epilogue_softmax_few(const Gemm2Params& p, uint3
     const int token = c + (lane & 15);               // whose numbers this lane stores
     const long long label = token < p.N ? p.sm_labels[token] - row0 : -1;
     const int mine = label >= 0 && label < min(32, p.M - row0) ? (int)label : -1;
-    for (unsigned hits = __ballot_sync(0xffffffffu, mine >= 0) & 0xffffu; hits; hits &= hits - 1) {
-      const int t = __ffs(hits) - 1;
-      if (__shfl_sync(0xffffffffu, mine, t) != lane) continue;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) if (e == t) p.sm_target[c + e] = __uint_as_float(r[e]);
-    }
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       if (!live) r[e] = 0xff800000u;
       const int bits = (int)r[e];
       const int key = __reduce_max_sync(0xffffffffu, bits >= 0 ? bits : bits ^ 0x7fffffff);
       const float top = __int_as_float(key >= 0 ? key : key ^ 0x7fffffff);
-      const float ref = fabsf(top) <= SM_NEAR || top == -INFINITY ? 0.f : top;
+      const float ref = sm_reference(top);
       if ((lane & 15) == e) my_ref = ref;
-      v[e] = live ? ex2(fmaf(__uint_as_float(r[e]), LOG2E, -ref * LOG2E)) : 0.f;
+      v[e] = live ? fmaf(__uint_as_float(r[e]), LOG2E, -ref) : -INFINITY;
     }
+    for (unsigned hits = __ballot_sync(0xffffffffu, mine >= 0) & 0xffffu; hits; hits &= hits - 1) {
+      const int t = __ffs(hits) - 1;
+      if (__shfl_sync(0xffffffffu, mine, t) != lane) continue;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) if (e == t) { p.sm_target[c + e] = v[e]; v[e] = -INFINITY; }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = ex2(v[e]);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) {
 #pragma unroll
@@ -1883,9 +1892,9 @@ TPLR_API int tplr_gemm2_softmax_columns(int M, int N, int K, int store) {
 }
 
 // The product Z = X W^T (X [M, K], W [N, K] bf16, K-major) with the softmax over its columns in pieces of tplr_gemm2_softmax_columns
-// columns (see epilogue_softmax); Z itself is not stored.  stats [M, pieces] pairs (reference, sum of exp(Z - it)), target [M] the logit of
-// the row's label (not written where the label is not a column).  P, if given: [M, N] bf16, rows of ldp (a multiple of 8) elements,
-// exp(Z - the piece's reference).
+// columns (see epilogue_softmax); Z itself is not stored.  stats [M, pieces] pairs (reference, sum of 2^(Z log2 e - it) over the columns but
+// the row's label), target [M] that exponent of the label, with its piece's reference (not written where the label is not a column).  P, if
+// given: [M, N] bf16, rows of ldp (a multiple of 8) elements, the numbers of the sums, zero for the label.
 TPLR_API int tplr_gemm2_softmax(const void* X, const void* W, void* P, const long long* labels, float* stats, float* target, int M, int N, int K,
                                 long long ldx, long long ldw, long long ldp, unsigned int* status, void* stream) {
   TPLR_ENTER();

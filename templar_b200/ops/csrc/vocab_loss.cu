@@ -1,10 +1,10 @@
-// Cross entropy from the pieces that tplr_gemm2_softmax leaves of a row of logits: (r_i, s_i) of every piece i, its reference and the sum of
-// its e_ij = exp(z_ij - r_i); the target's logit z; and the e_ij in bf16.  With c the largest reference of the row and
-// s = sum_i s_i exp(r_i - c):
-//   lse = c + log(s),   loss = lse - z,   d_ij = g * (exp(z_ij - lse) - [ij is the label])
+// Cross entropy from the pieces that tplr_gemm2_softmax leaves of a row of logits z: (r_i, s_i) of every piece i, its whole reference and the
+// sum of its e_ij = 2^(z_ij log2 e - r_i) but for the label's; the label's exponent a, relative to its own piece's reference r; and the e_ij in
+// bf16.  With c the largest reference of the row, all weights but the label's t = sum_i s_i 2^(r_i - c), and the label's e = 2^(a + r - c):
+//   s = t + e,   loss = log(s / e) = log1p(t / e),   d_ij = g * (e_ij 2^(r_i - c) / s - [ij is the label])
 // with g the gradient of the row's loss.  d is the row's factor f = g / s times E, which is e_ij where the piece's reference is c, as
-// it nearly always is, e_ij exp(r_i - c) where it is not, and s (exp(z - lse) - 1) in the label's column, made from the
-// fp32 logit: where the model is sure of it, the difference of a rounded weight and 1 would be little more than the rounding.  So
+// it nearly always is, e_ij 2^(r_i - c) where it is not, and e - s = -t in the label's column.  Where the model is sure of the label, t has all its
+// digits, and the difference of p and 1 would be little more than p's rounding.  So
 //   dx = f * (E w),   dw = E^T (f x)
 // and E is not read or written here but for the label's column and pieces of another reference.  f x is rounded to bf16, as d would be.
 //
@@ -39,11 +39,16 @@ __global__ void __launch_bounds__(1024) vocab_count_kernel(const long long* labe
   if (threadIdx.x == 0) out[0] = total;
 }
 
+// log(s / e) of a row with t beside the label's e = 2^a: by t / e where the label is the more likely, else by the logarithm of s, as e may be zero.
+__device__ __forceinline__ float row_loss(float t, float e, float a) {
+  return t < e ? log1pf(t / e) : (log2f(t + e) - a) * 0.6931471805599453f;
+}
+
 // Loss of each row: a warp a row, or (WIDE) its block of eight, where there are no more rows than SMs: 30 rows of 1000 pieces, product
 // and this, 20.6 us with a warp a row, 16.1 with a block.
 template <bool WIDE>
 __global__ void __launch_bounds__(256) vocab_losses_kernel(const float2* stats, const float* target, const long long* labels, float* losses,
-                                                           long long T, int parts, int V, long long ignore) {
+                                                           long long T, int parts, int columns, int V, long long ignore) {
   __shared__ float red[2][8];
   grid_wait();
   grid_release();
@@ -68,7 +73,7 @@ __global__ void __launch_bounds__(256) vocab_losses_kernel(const float2* stats, 
     }
     float s = 0.f;
 #pragma unroll 4
-    for (int i = first; i < parts; i += step) { const float2 v = st[i]; s += v.y * __expf(v.x - m); }
+    for (int i = first; i < parts; i += step) { const float2 v = st[i]; s += v.y * exp2f(v.x - m); }
     s = warp_sum(s);
     if (WIDE) {
       if (lane == 0) red[1][warp] = s;
@@ -77,7 +82,8 @@ __global__ void __launch_bounds__(256) vocab_losses_kernel(const float2* stats, 
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += red[1][i];
     }
-    loss = m + logf(s) - target[row];
+    const float a = target[row] + (st[label / columns].x - m);
+    loss = row_loss(s, exp2f(a), a);
   }
   if (WIDE ? threadIdx.x == 0 : lane == 0) losses[row] = loss;
 }
@@ -97,19 +103,21 @@ __global__ void __launch_bounds__(256) vocab_rows_kernel(bf16* e, long long ld, 
   bf16* er = e + row * ld;
   const long long label = labels[row];
   const bool counts = label != ignore && label >= 0 && label < V;
-  float c = -INFINITY, low = INFINITY, s = 0.f;
+  float c = -INFINITY, low = INFINITY, t = 0.f, a = 0.f;
   for (int i = lane; i < parts; i += 32) { c = fmaxf(c, st[i].x); low = fminf(low, st[i].x); }
   c = warp_max(c);
   low = -warp_max(-low);
-  for (int i = lane; i < parts; i += 32) { const float2 v = st[i]; s += v.y * __expf(v.x - c); }
-  s = warp_sum(s);
+  for (int i = lane; i < parts; i += 32) { const float2 v = st[i]; t += v.y * exp2f(v.x - c); }
+  t = warp_sum(t);
+  if (counts) a = target[row] + (st[label / columns].x - c);
+  const float e1 = counts ? exp2f(a) : 0.f, s = t + e1;
   const float g = !counts ? 0.f : row_grad ? row_grad[row] : grad_scale / (float)max(n_valid[0], 1);
   const float f = counts ? g / s : 0.f;
   if (counts) {
     if (low < c) {                                   // the same in all lanes
       for (int i = 0; i < parts; ++i) {
         if (st[i].x == c) continue;
-        const float by = __expf(st[i].x - c);
+        const float by = exp2f(st[i].x - c);
         for (int k = i * columns + lane * 8; k < min(i * columns + columns, V); k += 256) {      // the columns behind V are nobody's
           uint4 q = *reinterpret_cast<uint4*>(er + k);
           uint32_t w[4] = {q.x, q.y, q.z, q.w};
@@ -124,9 +132,8 @@ __global__ void __launch_bounds__(256) vocab_rows_kernel(bf16* e, long long ld, 
       __syncwarp();
     }
     if (lane == 0) {
-      const float lse = c + logf(s), z = target[row];
-      er[label] = __float2bfloat16(s * (__expf(z - lse) - 1.f));
-      if (losses) losses[row] = lse - z;
+      er[label] = __float2bfloat16(-t);
+      if (losses) losses[row] = row_loss(t, e1, a);
     }
   } else {
     // what the row holds is multiplied by zero, which takes numbers
@@ -216,14 +223,15 @@ TPLR_API int tplr_vocab_count(const long long* labels, long long T, long long ig
   return (int)launch_pdl(vocab_count_kernel, 1, 1024, 0, (cudaStream_t)stream, labels, T, ignore, V, n_valid, status);
 }
 
-// losses [T] from tplr_gemm2_softmax's stats [T, parts] and target [T]
-TPLR_API int tplr_vocab_losses(const float* stats, const float* target, const long long* labels, float* losses, long long T, int parts, int V,
-                               long long ignore, void* stream) {
+// losses [T] from tplr_gemm2_softmax's stats [T, parts], of columns each, and target [T]
+TPLR_API int tplr_vocab_losses(const float* stats, const float* target, const long long* labels, float* losses, long long T, int parts, int columns,
+                               int V, long long ignore, void* stream) {
   TPLR_ENTER();
   if (T <= 0) return 0;
+  if (columns <= 0 || (long long)parts * columns < V) return -401;
   const bool wide = T <= tplr_sm_count();
   return (int)launch_pdl(wide ? vocab_losses_kernel<true> : vocab_losses_kernel<false>, (unsigned)(wide ? T : (T + 7) / 8), 256, 0, (cudaStream_t)stream,
-                         reinterpret_cast<const float2*>(stats), target, labels, losses, T, parts, V, ignore);
+                         reinterpret_cast<const float2*>(stats), target, labels, losses, T, parts, columns, V, ignore);
 }
 
 // What tplr_gemm2_softmax left of T rows, E [T, V] (rows of ld elements), made ready for the products of the gradients: dx = row_scale * (E w),
@@ -234,7 +242,7 @@ TPLR_API int tplr_vocab_rows(void* E, long long ld, const float* stats, const fl
                              long long T, int parts, int columns, int V, int D, long long ignore, void* stream) {
   TPLR_ENTER();
   if (T <= 0) return 0;
-  if ((ld % 8) || ld < V || (columns % 8) || columns <= 0 || (ldx % 8) || (ldxs % 8) || (xs && ldxs < D) || (D % 8) || (((uintptr_t)E | (uintptr_t)x | (uintptr_t)xs) & 15)) return -401;
+  if ((ld % 8) || ld < V || (columns % 8) || columns <= 0 || (long long)parts * columns < V || (ldx % 8) || (ldxs % 8) || (xs && ldxs < D) || (D % 8) || (((uintptr_t)E | (uintptr_t)x | (uintptr_t)xs) & 15)) return -401;
   return (int)launch_pdl(vocab_rows_kernel, (unsigned)((T + 7) / 8), 256, 0, (cudaStream_t)stream, (bf16*)E, ld,
                          reinterpret_cast<const float2*>(stats), target, labels, row_grad, n_valid, grad_scale, (const bf16*)x, ldx, (bf16*)xs,
                          ldxs, row_scale, losses, T, parts, columns, V, D, ignore);

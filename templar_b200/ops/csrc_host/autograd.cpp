@@ -771,7 +771,8 @@ Tensor token_losses(const Tensor& x, const Tensor& w, const Tensor& labels, int6
   const ll* lab = reinterpret_cast<const ll*>(labels.data_ptr<int64_t>());
   for (ll a = 0; a < T; a += run) {
     const ll n = std::min(run, T - a), columns = ws.run(x, n, w, row_of(x, a), lab + a, status);
-    check(E.vocab_losses(ws.stats, ws.target, lab + a, losses.data_ptr<float>() + a, n, (int)((V + columns - 1) / columns), (int)V, ignore, stream()),
+    check(E.vocab_losses(ws.stats, ws.target, lab + a, losses.data_ptr<float>() + a, n, (int)((V + columns - 1) / columns), (int)columns,
+                         (int)V, ignore, stream()),
           "vocab_losses");
   }
   return losses;

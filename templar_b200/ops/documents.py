@@ -353,9 +353,9 @@ def _token_losses(x2, w, labels, ignore_index):
     runs = _chunks(T, 16 * -(-V // 128))             # 8 bytes a piece
     ws = _Pieces(x2, w, runs[0][1], False)
     for a, b in runs:
-        parts, _ = ws.run(x2[a:b], w, labels[a:b])
+        parts, columns = ws.run(x2[a:b], w, labels[a:b])
         native.check(native.lib().tplr_vocab_losses(ws.stats.data_ptr(), ws.target.data_ptr(), labels[a:].data_ptr(), losses[a:].data_ptr(),
-                                                    b - a, parts, V, ignore_index, native.stream_ptr()), "vocab_losses")
+                                                    b - a, parts, columns, V, ignore_index, native.stream_ptr()), "vocab_losses")
     return losses
 
 

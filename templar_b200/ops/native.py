@@ -154,7 +154,7 @@ def _declare(L: ctypes.CDLL) -> None:
         "tplr_gemm2_softmax_columns": [i, i, i, i],
         "tplr_gemm2_softmax": [vp, vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, vp, vp],
         "tplr_vocab_count": [vp, ll, ll, i, vp, vp, vp],
-        "tplr_vocab_losses": [vp, vp, vp, vp, ll, i, i, ll, vp],
+        "tplr_vocab_losses": [vp, vp, vp, vp, ll, i, i, i, ll, vp],
         "tplr_vocab_rows": [vp, ll, vp, vp, vp, vp, vp, f, vp, ll, vp, ll, vp, vp, ll, i, i, i, i, ll, vp],
         "tplr_gemm2_rows": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, vp, vp],
         "tplr_vocab_mean": [vp, ll, vp, vp, vp],

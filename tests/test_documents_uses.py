@@ -242,3 +242,61 @@ def test_norm_weights_may_have_any_shape_of_their_numbers(host, monkeypatch):
     got = run(row, grid)
     assert got[1].shape == (1, hd) and got[2].shape == (8, 8)
     assert all(torch.equal(a.flatten(), b.flatten()) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------------------------ labels that the model is sure of
+def sure(T, D, V, far, seed=0):
+    """x, w, labels: rows whose label has probabilities of one half to 1 - 1e-9; far: all logits moved by as much."""
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn(V, D, generator=g)
+    labels = torch.randint(0, V, (T,), generator=g)
+    w = w / w.norm(dim=1, keepdim=True)
+    x = w[labels] * torch.linspace(9, 36, T)[:, None]
+    x[:, 0], w[:, 0] = 10, far / 10
+    return x.to(DEV, torch.bfloat16), w.to(DEV, torch.bfloat16), labels.to(DEV)
+
+
+def sure64(x, w, labels):
+    """(losses, bound), d logits of their sum, its bound.  What is off is relative to 1 - p in the label's column, as to p in the others, so
+    that the gradient of a label that is nearly certain has digits: 1 - p is formed in 64 bits from the other columns."""
+    xd, wd = x.detach().double(), w.detach().double()
+    z, at, D = xd @ wd.t(), labels[:, None], x.shape[1]
+    # fp32 sums of products of 16 in the tensor cores, one step for each; exponents below 128 rounded to fp32, 128 ln 2 2^-24, and the exponential's own
+    ez = (D / 16 + 2) * 2.0 ** -23 * (xd.abs() @ wd.abs().t()).amax(1, keepdim=True)
+    e = 2 * ez + 1e-5
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    p = torch.exp(z - lse)
+    others = z.scatter(1, at, float("-inf"))
+    rest = torch.exp(torch.logsumexp(others, 1, keepdim=True) - lse)       # 1 - p of the label
+    losses = torch.log1p(rest / p.gather(1, at))
+    d = p.scatter(1, at, -rest)
+    ed = (2.02 * U + e) * d.abs()                              # a weight rounded, a row times its factor rounded
+    return (losses[:, 0], (e * rest + 2.0 ** -21 * losses)[:, 0]), d, ed, rest
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("far", [0.0, 30.0, -30.0, 300.0, -1000.0])
+@pytest.mark.parametrize("T,D,V", [(100, 64, 1000), (300, 128, 5003)])
+def test_gradients_of_labels_that_are_nearly_certain(T, D, V, far):
+    x, w, labels = sure(T, D, V, far)
+    (want, el), d, ed, rest = sure64(x, w, labels)
+    if far == 0:
+        assert rest.min() < 1e-7 and rest.max() > 0.1
+    x.requires_grad_()
+    w.requires_grad_()
+    xd, wd = x.detach().double(), w.detach().double()
+    with torch.no_grad():
+        each = ops.linear_cross_entropy(x, w, labels, reduction="none").double()
+    assert ((each - want).abs() <= el).all(), ((each - want).abs() / el).max().item()
+    # a row at a time: its label's column of dw is -(1 - p) x, whatever the others are
+    for t in range(0, T, 7):
+        loss = ops.linear_cross_entropy(x[t:t + 1], w, labels[t:t + 1])
+        (dw,) = torch.autograd.grad(loss, w)
+        assert (loss.double() - want[t]).abs() <= el[t] + 2.0 ** -23 * want[t]
+        ref = d[t, :, None] * xd[t]
+        off = (dw.double() - ref).abs() - (1.02 * ed[t, :, None] * xd[t].abs() + U * ref.abs() + 1e-30)
+        assert off.max() <= 0, (t, rest[t].item(), off.max().item())
+    dx, dw = torch.autograd.grad(ops.linear_cross_entropy(x, w, labels), (x, w))
+    for got, ref, b, size in ((dx, d @ wd, ed @ wd.abs(), d.abs() @ wd.abs()), (dw, d.t() @ xd, ed.t() @ xd.abs(), d.abs().t() @ xd.abs())):
+        off = (got.double() * T - ref).abs() - (1.02 * b + U * ref.abs() + 2.0 ** -18 * size + 1e-30)
+        assert off.max() <= 0
