@@ -965,9 +965,14 @@ __device__ __forceinline__ bool epilogue_swiglu_bwd_q8(const Gemm2Params& p, uin
 // One B200: 4096 x 4096 x 128256 without the weights 2626 us, 1640 TFLOP/s, the tensor pipe 98 % busy (the plain product's own time); 1111 x 1000 x
 // 50257 with them 126 us, 112 MB stored, the pipe 48 %: 13 % of its rows are the last tile's, and 16 k blocks do not cover an epilogue.
 constexpr float SM_NEAR = 40.f, LOG2E = 1.4426950408889634f;
-// A piece's reference by its largest logit
-__device__ __forceinline__ float sm_reference(float top) {
-  return fabsf(top) <= SM_NEAR || top == -INFINITY ? 0.f : rintf(top * LOG2E);
+// A piece's reference by its largest logit, and what else is to be taken from its exponents: nothing, but where the reference's own
+// rounding is large (logits of 1e7 and more), whose exponents would not end near zero.
+__device__ __forceinline__ float sm_reference(float top, float& more) {
+  more = 0.f;
+  if (fabsf(top) <= SM_NEAR || top == -INFINITY) return 0.f;
+  const float ref = rintf(top * LOG2E), left = fmaf(top, LOG2E, -ref);
+  if (fabsf(left) > 1.f) more = left;
+  return ref;
 }
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -999,7 +1004,9 @@ __device__ __forceinline__ void epilogue_softmax(const Gemm2Params& p, uint32_t 
     for (int e = 0; e < 32; e += 2) { top = fmaxf(top, __uint_as_float(r[e])); top2 = fmaxf(top2, __uint_as_float(r[e + 1])); }
     top = fmaxf(top, top2);
   }
-  const float ref = sm_reference(top);
+  float more;
+  const float ref = sm_reference(top, more);
+  const bool some_more = __any_sync(0xffffffffu, more != 0.f);
   float sum = 0.f, sum2 = 0.f, target = 0.f;
 #pragma unroll 1
   for (int c = 0; c < width; c += 64) {
@@ -1014,6 +1021,10 @@ __device__ __forceinline__ void epilogue_softmax(const Gemm2Params& p, uint32_t 
       tmem_ld32(acc + c + hh * 32, r);
 #pragma unroll
       for (int e = 0; e < 32; ++e) v[e] = fmaf(__uint_as_float(r[e]), LOG2E, -ref);
+      if (some_more) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] -= more;
+      }
       if (__any_sync(0xffffffffu, (mine >> 5) == ((c + hh * 32) >> 5))) {
 #pragma unroll
         for (int e = 0; e < 32; ++e) if (c + hh * 32 + e == mine) { target = v[e]; v[e] = -INFINITY; }
@@ -1062,9 +1073,10 @@ __device__ __forceinline__ void epilogue_softmax_few(const Gemm2Params& p, uint3
       const int bits = (int)r[e];
       const int key = __reduce_max_sync(0xffffffffu, bits >= 0 ? bits : bits ^ 0x7fffffff);
       const float top = __int_as_float(key >= 0 ? key : key ^ 0x7fffffff);
-      const float ref = sm_reference(top);
+      float more;
+      const float ref = sm_reference(top, more);
       if ((lane & 15) == e) my_ref = ref;
-      v[e] = live ? fmaf(__uint_as_float(r[e]), LOG2E, -ref) : -INFINITY;
+      v[e] = live ? fmaf(__uint_as_float(r[e]), LOG2E, -ref) - more : -INFINITY;
     }
     for (unsigned hits = __ballot_sync(0xffffffffu, mine >= 0) & 0xffffu; hits; hits &= hits - 1) {
       const int t = __ffs(hits) - 1;

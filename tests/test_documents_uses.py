@@ -300,3 +300,31 @@ def test_gradients_of_labels_that_are_nearly_certain(T, D, V, far):
     for got, ref, b, size in ((dx, d @ wd, ed @ wd.abs(), d.abs() @ wd.abs()), (dw, d.t() @ xd, ed.t() @ xd.abs(), d.abs().t() @ xd.abs())):
         off = (got.double() * T - ref).abs() - (1.02 * b + U * ref.abs() + 2.0 ** -18 * size + 1e-30)
         assert off.max() <= 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e10, 1e20, 1e30])
+@pytest.mark.parametrize("T", [40, 200])
+def test_logits_of_any_size(T, size):
+    """The largest logit's exponent ends at zero, however coarse fp32 is at its size: the loss is the distance of two logits."""
+    x, w = normal(1, T, 64, std=size ** 0.5, device=DEV, dtype=torch.bfloat16), normal(2, 300, 64, std=size ** 0.5, device=DEV, dtype=torch.bfloat16)
+    xd, wd = x.double(), w.double()
+    z = xd @ wd.t()
+    ez = (64 / 16 + 2) * 2.0 ** -23 * (xd.abs() @ wd.abs().t()).amax(1)
+    labels = z.argmax(1)
+    labels[::2] = (labels[::2] + 1) % 300
+    want = torch.logsumexp(z, 1) - z.gather(1, labels[:, None])[:, 0]
+    got = ops.linear_cross_entropy(x, w, labels, reduction="none").double()
+    bound = 2 * ez + 2.0 ** -21 * want + 2e-5                  # and whole references of logits: as the logits themselves
+    assert ((got - want).abs() <= bound + 2.0 ** -22 * z.abs().amax(1)).all()
+    x.requires_grad_()
+    w.requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, labels)
+    assert (loss.double() - want.mean()).abs() <= (bound + 2.0 ** -22 * z.abs().amax(1)).mean()
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    assert dx.isfinite().all() and dw.isfinite().all()
+    top2 = z.topk(2, 1).values
+    if size > 1e3 and ((top2[:, 0] - top2[:, 1]) > 4 * ez + 200).all():        # one column has all the weight
+        d = torch.nn.functional.one_hot(z.argmax(1), 300).double() - torch.nn.functional.one_hot(labels, 300)
+        ref = d @ wd / T
+        assert ((dx.double() - ref).abs() <= 4 * U * (d.abs() @ wd.abs()) / T).all()
