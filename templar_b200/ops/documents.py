@@ -470,8 +470,9 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
 
 
 def _linear_cross_entropy_torch(x, w, labels, grad_scale, ignore_index, reduction):
-    z = x.reshape(-1, x.shape[-1]).float() @ w.float().t()
     counts = (labels != ignore_index) & (labels >= 0) & (labels < w.shape[0])
+    # a row that does not count may hold anything: no infinity meets its gradient of zero
+    z = torch.where(counts[:, None], x.reshape(-1, x.shape[-1]).float(), 0.0) @ w.float().t()
     losses = torch.logsumexp(z, dim=1) - z.gather(1, labels.clamp(0, w.shape[0] - 1)[:, None])[:, 0]
     losses = torch.where(counts, losses, 0.0)
     if reduction == "mean":

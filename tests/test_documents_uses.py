@@ -328,3 +328,18 @@ def test_logits_of_any_size(T, size):
         d = torch.nn.functional.one_hot(z.argmax(1), 300).double() - torch.nn.functional.one_hot(labels, 300)
         ref = d @ wd / T
         assert ((dx.double() - ref).abs() <= 4 * U * (d.abs() @ wd.abs()) / T).all()
+
+
+# ------------------------------------------------------------------------------------------ the formulas
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+def test_rows_without_a_label_may_hold_anything_in_the_formulas_too(what, reduction):
+    x, w, labels = normal(1, 6, 8), normal(2, 11, 8), torch.tensor([3, -100, 10, 99, 0, -100])
+    results = []
+    for fill in (0.5, what):
+        a, b = x.clone(), w.clone().requires_grad_()
+        a[1], a[3] = fill, fill                                # ignored, and no column
+        a.requires_grad_()
+        loss = ops.linear_cross_entropy(a, b, labels, reduction=reduction)
+        results.append((loss, *torch.autograd.grad(loss.sum(), (a, b))))
+    assert all(torch.equal(p, q) for p, q in zip(*results))
