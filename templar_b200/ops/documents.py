@@ -83,7 +83,7 @@ def document_starts(tokens: torch.Tensor, eos_id: int, window: int = 0) -> torch
     if tokens.shape[1] > 1:
         first[:, 1:] = torch.where(tokens[:, :-1] == eos_id, rows[1:], 0)
         first = first.cummax(1).values.to(torch.int32)
-    return torch.maximum(first, rows - (int(window) - 1)) if window > 0 else first
+    return torch.maximum(first, rows - (min(int(window), tokens.shape[1]) - 1)) if window > 0 else first
 
 
 # --------------------------------------------------------------------------- #

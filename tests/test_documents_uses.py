@@ -343,3 +343,10 @@ def test_rows_without_a_label_may_hold_anything_in_the_formulas_too(what, reduct
         loss = ops.linear_cross_entropy(a, b, labels, reduction=reduction)
         results.append((loss, *torch.autograd.grad(loss.sum(), (a, b))))
     assert all(torch.equal(p, q) for p, q in zip(*results))
+
+
+@pytest.mark.parametrize("window", [8, 9, 2 ** 31 - 1, 2 ** 31, 2 ** 31 + 5, 2 ** 40, 2 ** 70])
+def test_windows_longer_than_the_sequence_leave_the_documents_whole(window):
+    tokens = torch.tensor([[5, 6, 2, 7, 2, 2, 8, 9]])
+    assert torch.equal(ops.document_starts(tokens, 2, window=window), ops.document_starts(tokens, 2))
+    assert ops.document_starts(tokens[:, :0], 2, window=window).shape == (1, 0)
