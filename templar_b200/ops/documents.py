@@ -155,8 +155,10 @@ def attention_documents(qkv: torch.Tensor, starts: torch.Tensor, n_heads: int, n
         return out
     _heads("attention_documents", qkv, n_heads, n_kv, hd)
     B, S, C = qkv.shape
-    if starts.shape != (B, S) or starts.is_floating_point() or starts.is_complex() or starts.dtype == torch.bool:
-        raise ValueError(f"attention_documents: whole numbers [{B}, {S}] expected as starts, got {starts.dtype} {tuple(starts.shape)}")
+    if starts.shape != (B, S) or starts.is_floating_point() or starts.is_complex() or starts.dtype in (torch.bool, torch.uint64):
+        raise ValueError(f"attention_documents: whole numbers [{B}, {S}] (not uint64) expected as starts, got {starts.dtype} {tuple(starts.shape)}")
+    if starts.dtype in (torch.uint16, torch.uint32):
+        starts = starts.to(torch.int64)
     _same_device("attention_documents", qkv, starts=starts)
     if not (qkv.is_cuda and qkv.dtype == torch.bfloat16 and hd in OF.OWN_HEAD_DIMS) or B * S == 0:
         return _attention_documents_torch(qkv, starts, n_heads, n_kv, hd)

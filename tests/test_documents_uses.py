@@ -350,3 +350,17 @@ def test_windows_longer_than_the_sequence_leave_the_documents_whole(window):
     tokens = torch.tensor([[5, 6, 2, 7, 2, 2, 8, 9]])
     assert torch.equal(ops.document_starts(tokens, 2, window=window), ops.document_starts(tokens, 2))
     assert ops.document_starts(tokens[:, :0], 2, window=window).shape == (1, 0)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param(DEV, marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.uint16, torch.uint32, torch.int64])
+def test_starts_of_every_whole_type(dtype, device):
+    H, KV, hd, S = 2, 1, 64, 140
+    qkv = normal(1, 1, S, (H + 2 * KV) * hd, device=device, dtype=torch.bfloat16)
+    starts = torch.arange(S, dtype=torch.int64)[None] // 10 * 10
+    starts[:, 125:] = torch.iinfo(dtype).max                   # as behind the row as the type can say
+    want = ops.attention_documents(qkv, starts.clamp(max=2 ** 31 - 1).to(torch.int32).to(device), H, KV, hd)
+    got = ops.attention_documents(qkv, starts.to(dtype).to(device), H, KV, hd)
+    assert torch.equal(got, want)
+    with pytest.raises(ValueError):
+        ops.attention_documents(qkv, starts.to(torch.uint64).to(device), H, KV, hd)
