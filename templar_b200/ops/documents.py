@@ -11,6 +11,7 @@ to the same formulas in PyTorch, as in :mod:`templar_b200.ops.functional`.
 from __future__ import annotations
 
 import contextlib
+import warnings
 
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -129,6 +130,9 @@ def _attention_documents(qkv, ld, starts, n_heads, n_kv, hd, keep):
     return out, lse, blocks
 
 
+_fallback_seen: set = set()
+
+
 def _attention_documents_torch(qkv, starts, n_heads, n_kv, hd):
     B, S, _ = qkv.shape
     q, k, v = (t.float().transpose(1, 2) for t in OF._split_qkv(qkv, n_heads, n_kv, hd))
@@ -148,7 +152,8 @@ def attention_documents(qkv: torch.Tensor, starts: torch.Tensor, n_heads: int, n
 
     Every row has to hold finite numbers, one that nothing sees too, and so has the gradient: the rows of a block of 128 meet in the
     same products, where a weight of zero times an infinity is not zero.  The kernels (bf16, heads of 64 or 128) add nothing
-    into memory: results and gradients have the same bits on every run."""
+    into memory: results and gradients have the same bits on every run.  Other heads and types take formulas in PyTorch, with the scores of
+    every head in memory, which is said once."""
     tangent = _has_tangent(qkv)
     # operands that the kernels take as they are need no further look
     if qkv.is_cuda and not tangent and (host := native.host()) and (out := host.attention_documents(qkv, starts, n_heads, n_kv, hd, _word(qkv))) is not None:
@@ -161,6 +166,11 @@ def attention_documents(qkv: torch.Tensor, starts: torch.Tensor, n_heads: int, n
         starts = starts.to(torch.int64)
     _same_device("attention_documents", qkv, starts=starts)
     if not (qkv.is_cuda and qkv.dtype == torch.bfloat16 and hd in OF.OWN_HEAD_DIMS) or B * S == 0:
+        if qkv.is_cuda and B * S > 0 and (hd, qkv.dtype) not in _fallback_seen:
+            # said once per kind: the scores of every head are in memory there, and a run that is slow or out of memory for it should say why
+            _fallback_seen.add((hd, qkv.dtype))
+            warnings.warn(f"attention_documents: heads of {hd}, {qkv.dtype} are outside the own kernels (bf16, heads of 64 or 128); using formulas in "
+                          f"PyTorch for them, with [B, H, S, S] scores in memory", stacklevel=2)
         return _attention_documents_torch(qkv, starts, n_heads, n_kv, hd)
     if tangent:
         raise _no_forward_mode("attention_documents")

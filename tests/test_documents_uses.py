@@ -1,6 +1,8 @@
 """Operators on packed documents in uses that are easily got wrong: forward mode, one buffer for two weights, graphs walked more than once,
 labels that the model is sure of.  On the CPU the formulas, on the GPU the kernels."""
 
+import warnings
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -364,3 +366,19 @@ def test_starts_of_every_whole_type(dtype, device):
     assert torch.equal(got, want)
     with pytest.raises(ValueError):
         ops.attention_documents(qkv, starts.to(torch.uint64).to(device), H, KV, hd)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,dtype", [(80, torch.bfloat16), (64, torch.float32)])
+def test_attention_outside_the_kernels_is_said_once(hd, dtype, monkeypatch):
+    monkeypatch.setattr(OD, "_fallback_seen", set())
+    qkv, starts = normal(1, 2, 30, 4 * hd, device=DEV, dtype=dtype), torch.zeros(2, 30, dtype=torch.int32, device=DEV)
+    with pytest.warns(UserWarning, match=f"attention_documents: heads of {hd}"):
+        ops.attention_documents(qkv, starts, 2, 1, hd)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        ops.attention_documents(qkv, starts, 2, 1, hd)
+        ops.attention_documents(qkv[:, :0], starts[:, :0], 2, 1, hd)
+        own = normal(2, 2, 30, 4 * 64, device=DEV, dtype=torch.bfloat16)
+        ops.attention_documents(own, starts, 2, 1, 64)
+        ops.attention_documents(own.cpu(), starts.cpu(), 2, 1, 64)
