@@ -382,3 +382,30 @@ def test_attention_outside_the_kernels_is_said_once(hd, dtype, monkeypatch):
         own = normal(2, 2, 30, 4 * 64, device=DEV, dtype=torch.bfloat16)
         ops.attention_documents(own, starts, 2, 1, 64)
         ops.attention_documents(own.cpu(), starts.cpu(), 2, 1, 64)
+
+
+# ------------------------------------------------------------------------------------------ a buffer and several runs of tokens
+@pytest.mark.gpu
+@pytest.mark.parametrize("host", [True, False])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_buffer_takes_the_sum_of_several_runs(reduction, host, monkeypatch):
+    if not host:
+        monkeypatch.setattr(native, "host", lambda: None)
+    T, D, V = 900, 72, 777
+    monkeypatch.setattr(OD, "CHUNK_BYTES", 2 * V * 300)
+    assert len(OD._chunks(T, V)) == 4
+    x, w = (normal(i, n, D, std=0.4, device=DEV, dtype=torch.bfloat16).requires_grad_() for i, n in ((1, T), (2, V)))
+    labels = torch.randint(0, V, (T,), generator=torch.Generator().manual_seed(3)).to(DEV)
+    labels[::11] = -100
+    run = lambda b: ops.linear_cross_entropy(x, w, labels, main_grad=b, reduction=reduction).sum()  # noqa: E731
+    dx, dw = torch.autograd.grad(run(None), (x, w))
+    main = torch.zeros(V, D, device=DEV)
+    (gx,) = torch.autograd.grad(run(main), (x,))
+    assert torch.equal(main.to(torch.bfloat16), dw) and torch.equal(gx, dx)        # the same sum in fp32, rounded by the caller
+    once = main.clone()
+    loss = run(main)
+    (0.5 * loss).backward(retain_graph=True)
+    loss.backward()
+    # two additions in fp32, and a product with a half, which is exact
+    torch.testing.assert_close(main, 2.5 * once, rtol=3 * 2.0 ** -24, atol=0)
+    assert w.grad is None and torch.equal(x.grad, (0.5 * dx.float()).to(torch.bfloat16) + dx)
