@@ -61,6 +61,7 @@ __global__ void __launch_bounds__(256) vocab_losses_kernel(const float2* stats, 
   float loss = 0.f;
   if (counts) {                                      // the same in all lanes, and all of a block's threads where it has one row
     const float2* st = stats + row * parts;
+    const float own = target[row], ref = st[(int)label / columns].x;
     float m = -INFINITY;
 #pragma unroll 4
     for (int i = first; i < parts; i += step) m = fmaxf(m, st[i].x);
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__(256) vocab_losses_kernel(const float2* stats, 
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += red[1][i];
     }
-    const float a = target[row] + (st[label / columns].x - m);
+    const float a = own + (ref - m);
     loss = row_loss(s, exp2f(a), a);
   }
   if (WIDE ? threadIdx.x == 0 : lane == 0) losses[row] = loss;
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(256) vocab_rows_kernel(bf16* e, long long ld, 
   low = -warp_max(-low);
   for (int i = lane; i < parts; i += 32) { const float2 v = st[i]; t += v.y * exp2f(v.x - c); }
   t = warp_sum(t);
-  if (counts) a = target[row] + (st[label / columns].x - c);
+  if (counts) a = target[row] + (st[(int)label / columns].x - c);
   const float e1 = counts ? exp2f(a) : 0.f, s = t + e1;
   const float g = !counts ? 0.f : row_grad ? row_grad[row] : grad_scale / (float)max(n_valid[0], 1);
   const float f = counts ? g / s : 0.f;
