@@ -47,7 +47,8 @@ constexpr int epi_warps(int epi) { return epi == 7 || epi == 8 || epi == 10 || e
 constexpr int num_threads(int epi) { return 64 + 32 * epi_warps(epi); }
 constexpr int ring_stages(int epi) { return epi == 5 || epi == 10 ? EPI5_STAGES : STAGES; }
 constexpr int MAX_RANKS = 8;
-constexpr int SOFTMAX_FEW = 128;                   // rows whose softmax without stored weights takes the transposed product
+// Rows whose softmax without stored weights takes the transposed product (times at epilogue_softmax_few)
+bool softmax_few(int M, int K) { return M <= 32 || (M <= 128 && K >= 12 * M); }
 constexpr int CHUNK_ROWS = 128;                    // gather / scatter flag granularity (rows)
 
 struct Gemm2Params {
@@ -1050,9 +1051,11 @@ __device__ __forceinline__ void epilogue_softmax(const Gemm2Params& p, uint32_t 
 // The same for a few tokens (EPI 15), whose product is made the other way round, rows of the weight along the tile's 256: a lane has a column
 // of the softmax, a piece is the 32 of a warp.  The largest of a token's 32 logits is one reduction of the warp over their bits in
 // the order of their values, the sums of 16 tokens meet in 16 shuffles, each lane keeping half of what it held.  A tile takes the tokens
-// there are in place of 256, so the weight's bytes bound it: 30 x 768 x 32000, cold, 17.0 us against 22.6 with tokens along the
-// tile, 128 x 2048 x 32000 36.2 and 38.5, 30 x 4096 x 128256 174 and 190 (6.0 TB/s); 128 x 768 x 32000 is even, at 21.9 and 19.8, and
-// above 128 tokens there is nothing to gain.
+// there are in place of 256, so the weight's bytes bound it; its epilogue is longer for each token, which a short K does not cover.  Microseconds
+// of a call, cold, this way and with tokens along the tile, 32000 columns: 30 x 768 22.6 and 26.7, 64 x 768 24.6 and 26.6, 96 x 768 28.2 and 24.6,
+// 128 x 768 30.7 and 24.6, 96 x 1024 30.7 and 28.7, 96 x 1280 even, 128 x 1280 34.8 and 32.8, 128 x 1536 even, 128 x 2048 even, 32 x 2048 41.0 and
+// 43.0; 128256 columns: 30 x 4096 182 and 193, 128 x 4096 188 and 195, 128 x 1536 92 and 88.  Hence softmax_few: above 128 tokens there is nothing
+// to gain.
 __device__ __forceinline__ void epilogue_softmax_few(const Gemm2Params& p, uint32_t tmem_acc, int quad, int turn, int lane, int m0) {
   const int half = p.tile_n / 2;                     // tokens of a warp
   const int row0 = m0 + quad * 32;
@@ -1896,11 +1899,11 @@ TPLR_API int tplr_gemm2_rope(const void* X, const void* W, void* QKV, int M, int
 }
 
 // Columns of a piece of tplr_gemm2_softmax for these sizes, P given or not: a row has ceil(N / columns) pieces, 64 columns or more in all but
-// the products of up to SOFTMAX_FEW rows without P.
+// the products of a few rows without P (softmax_few).
 static int softmax_tile(int M, int N, int K) { return pick_tile(M, N, K, false, false, 0, 1, 128); }
 TPLR_API int tplr_gemm2_softmax_columns(int M, int N, int K, int store) {
   if (M <= 0 || N <= 0 || K <= 0) return 128;
-  return !store && M <= SOFTMAX_FEW ? 32 : softmax_tile(M, N, K) / 2;
+  return !store && softmax_few(M, K) ? 32 : softmax_tile(M, N, K) / 2;
 }
 
 // The product Z = X W^T (X [M, K], W [N, K] bf16, K-major) with the softmax over its columns in pieces of tplr_gemm2_softmax_columns
@@ -1913,7 +1916,7 @@ TPLR_API int tplr_gemm2_softmax(const void* X, const void* W, void* P, const lon
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   if (((uintptr_t)P & 15) || (ldp % 8) || ((uintptr_t)stats & 7) || (P && ldp < N)) return -101;
   Gemm2Params p = {};
-  const bool few = !P && M <= SOFTMAX_FEW;
+  const bool few = !P && softmax_few(M, K);
   const int tile_n = few ? (M + 31) / 32 * 32 : softmax_tile(M, N, K), columns = few ? 32 : tile_n / 2;
   if (int r = few ? fill_common(p, W, X, nullptr, N, M, K, ldw, ldx, 8, 0, 0, 0, status, tile_n)
                   : fill_common(p, X, W, P, M, N, K, ldx, ldw, P ? ldp : 8, 0, 0, 0, status, tile_n))

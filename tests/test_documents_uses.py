@@ -409,3 +409,20 @@ def test_a_buffer_takes_the_sum_of_several_runs(reduction, host, monkeypatch):
     # two additions in fp32, and a product with a half, which is exact
     torch.testing.assert_close(main, 2.5 * once, rtol=3 * 2.0 ** -24, atol=0)
     assert w.grad is None and torch.equal(x.grad, (0.5 * dx.float()).to(torch.bfloat16) + dx)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,D,V", [(32, 8, 33), (33, 400, 1003), (33, 392, 1003), (64, 768, 4097), (64, 760, 4097), (96, 1152, 5003), (96, 1144, 5003),
+                                   (128, 1536, 20000), (128, 1528, 20000), (128, 4096, 1000)])
+def test_losses_of_few_tokens_on_both_sides_of_the_rule(T, D, V):
+    """The product with the weight's rows along the tile, and the next width that takes the tokens along it."""
+    x, w, labels = sure(T, D, V, 0.0, seed=T + D)
+    labels[1::3] = torch.randint(0, V, (len(labels[1::3]),), generator=torch.Generator().manual_seed(1)).to(DEV)
+    labels[0] = V - 1
+    (want, el), *_ = sure64(x, w, labels)
+    each = ops.linear_cross_entropy(x, w, labels, reduction="none")
+    off = (each.double() - want).abs() - el
+    assert off.max() <= 0
+    part = ops.linear_cross_entropy(x[:31], w, labels[:31], reduction="none").double()
+    assert ((part - want[:31]).abs() <= el[:31]).all()
+    assert int(OF.status_word(DEV).item()) == 0
