@@ -295,7 +295,8 @@ def qk_norm_rope(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, cos: tor
     for name, w, main_grad in (("main_grad_q", wq, main_grad_q), ("main_grad_k", wk, main_grad_k)):
         if grad and main_grad is not None:
             _fitting_buffer("qk_norm_rope", name, w, main_grad)
-    if grad and main_grad_q is not None and main_grad_k is not None:
+    # other buffers than dense ones in fp32 are added onto one behind the other
+    if grad and all(t is not None and t.dtype == torch.float32 and t.is_contiguous() for t in (main_grad_q, main_grad_k)):
         q, k = ((t.data_ptr(), t.data_ptr() + t.nbytes) for t in (main_grad_q, main_grad_k))
         if q[0] != k[0] and q[0] < k[1] and k[0] < q[1]:
             raise ValueError("qk_norm_rope: main_grad_q and main_grad_k are one buffer or two, they do not overlap in part")

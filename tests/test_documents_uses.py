@@ -69,6 +69,18 @@ def test_buffers_that_overlap_in_part_are_refused():
     torch.testing.assert_close(long[:hd], 2 * apart[:hd] + apart[hd:])
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param(DEV, marks=pytest.mark.gpu)])
+def test_buffers_in_each_others_gaps(device):
+    H, KV, hd, S = 2, 1, 64, 90
+    qkv, wq, wk = (normal(i, *s, device=device, dtype=torch.bfloat16).requires_grad_() for i, s in ((1, (1, S, (H + 2 * KV) * hd)), (2, (hd,)), (3, (hd,))))
+    cos, sin = ops.rope_tables(S, hd, device=device)
+    run = lambda **k: ops.qk_norm_rope(qkv, wq, wk, cos, sin, H, KV, hd, **k).float().square().sum()  # noqa: E731
+    gq, gk = torch.autograd.grad(run(), (wq, wk))
+    both = torch.zeros(hd, 2, device=device)
+    run(main_grad_q=both[:, 0], main_grad_k=both[:, 1]).backward()
+    assert torch.equal(both[:, 0].to(torch.bfloat16), gq) and torch.equal(both[:, 1].to(torch.bfloat16), gk)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("host", [True, False])
 @pytest.mark.parametrize("B,S,H,KV,hd", [(1, 1, 1, 1, 8), (2, 700, 4, 2, 64), (1, 3000, 16, 4, 128), (1, 90, 5, 5, 256)])
