@@ -2087,7 +2087,8 @@ __device__ __forceinline__ int next_tile(const AttnDocsBwdParams& p, int lane) {
   if (p.next && lane == 0) n = (int)gridDim.x + atomicAdd(p.next, 1);
   return __shfl_sync(0xffffffffu, n, 0);
 }
-// The two counters belong to one call: walks of one graph may overlap, and one whose wait ran out leaves them anywhere.
+// The two counters belong to one call: walks of one graph may overlap, and one whose wait ran out leaves them anywhere.  A launch of its own,
+// 1.2 us, where there are more tiles than SMs: 3 x 1999, 12 heads of 64, forward and backward, 70.5 -> 72 us.
 __global__ void attn_docs_counters_kernel(int* next) {
   grid_wait();
   grid_release();
